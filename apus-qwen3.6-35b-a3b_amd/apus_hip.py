@@ -53,6 +53,9 @@ EXPORTS = [
     "apus_hip_gdn_prefill_noalloc", "apus_hip_set_spin_limit", "apus_hip_attn_split_check",
     "apus_hip_gdn_layer_decode", "apus_hip_gdn_layer_decode_slots",
     "apus_hip_attn_layer_decode", "apus_hip_attn_layer_decode_paged",
+    "apus_hip_mxfp4_quantize", "apus_hip_mxfp4_dequantize", "apus_hip_mxfp4_gemm_dev",
+    "apus_hip_mxfp4_gemm_mx_dev", "apus_hip_moe_work_create", "apus_hip_moe_work_destroy",
+    "apus_hip_moe_layer_decode",
 ]
 
 
@@ -91,6 +94,16 @@ class AttnProj(C.Structure):
     """ApusHipAttnProj (include/apus_hip.h): a full-attention layer's
     projections."""
     _fields_ = [("hidden", _sz), ("wq", _vp), ("wk", _vp), ("wv", _vp), ("wo", _vp)]
+
+
+class MoeLayer(C.Structure):
+    """ApusHipMoeLayer (include/apus_hip.h)."""
+    _fields_ = [("hidden", _sz), ("inter", _sz), ("experts", _sz), ("topk", _sz),
+                ("shared_inter", _sz), ("norm_topk", C.c_int), ("mxfp4", C.c_int),
+                ("w_router", _vp), ("w_gate_up", _vp), ("w_down", _vp),
+                ("w_shared_gate_up", _vp), ("w_shared_down", _vp), ("w_shared_gate", _vp),
+                ("s_gate_up", _vp), ("s_down", _vp), ("s_shared_gate_up", _vp),
+                ("s_shared_down", _vp)]
 
 
 _lib = None
@@ -712,6 +725,139 @@ def free_gdn_layer(L):
 
 def free_attn_layer(L):
     _chk(load().apus_hip_attn_layer_free(C.byref(L)))
+
+
+# ---- MXFP4
+def _rows(t, what, ncols=None):
+    """(pointer, rows, columns, pitch) of a 2-D device tensor of 2-byte
+    elements whose rows are contiguous (any pitch)."""
+    if not t.is_cuda or t.dim() != 2 or t.element_size() != 2:
+        raise ValueError(f"{what}: a 2-D GPU tensor of bf16 values or codes, not {tuple(t.shape)} "
+                         f"{t.dtype} on {t.device}")
+    m, n = t.shape
+    if ncols is not None and n != ncols:
+        raise ValueError(f"{what}: rows of {n} elements, expected {ncols}")
+    if n > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: elements of a row must be contiguous")
+    return _vp(t.data_ptr()), m, n, t.stride(0) if m > 1 else n
+
+
+def _bytes(t, shape, what):
+    """Pointer of a dense device tensor of bytes of this shape."""
+    if not t.is_cuda or t.element_size() != 1 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous GPU tensor of bytes of shape {tuple(shape)}, not "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return _vp(t.data_ptr())
+
+
+def _same_device(*ts):
+    if len({t.device for t in ts if t is not None}) > 1:
+        raise ValueError(f"tensors on several devices: {[str(t.device) for t in ts if t is not None]}")
+
+
+def mxfp4_quantize(x, codes, scales):
+    """x [M, K] bf16 (rows of any pitch) -> codes [M, K/2], scales [M, K/32]
+    (uint8): MXFP4, apus_hip_mxfp4_quantize."""
+    _same_device(x, codes, scales)
+    xp, M, K, ldx = _rows(x, "x")
+    _chk(load().apus_hip_mxfp4_quantize(xp, _sz(ldx), _bytes(codes, (M, K // 2), "codes"),
+                                        _bytes(scales, (M, K // 32), "scales"), _sz(M), _sz(K)))
+
+
+def mxfp4_dequantize(codes, scales, x):
+    """The bf16 values of codes, scales into x [M, K] (rows of any pitch)."""
+    _same_device(x, codes, scales)
+    xp, M, K, ldx = _rows(x, "x")
+    _chk(load().apus_hip_mxfp4_dequantize(_bytes(codes, (M, K // 2), "codes"),
+                                          _bytes(scales, (M, K // 32), "scales"), xp, _sz(ldx),
+                                          _sz(M), _sz(K)))
+
+
+def mxfp4_gemm(w, ws, x, y):
+    """y [M, O] = x [M, K] w^T, w [O, K/2], ws [O, K/32] MXFP4, x and y bf16
+    with rows of any pitch."""
+    _same_device(w, ws, x, y)
+    xp, M, K, ldx = _rows(x, "x")
+    O = w.shape[0]
+    yp, ym, _, ldy = _rows(y, "y", O)
+    if ym != M:
+        raise ValueError(f"y: {ym} rows, expected {M}")
+    _chk(load().apus_hip_mxfp4_gemm_dev(_bytes(w, (O, K // 2), "w"), _bytes(ws, (O, K // 32), "ws"),
+                                        xp, _sz(ldx), yp, _sz(ldy), _sz(M), _sz(O), _sz(K)))
+
+
+def mxfp4_gemm_mx(w, ws, x, xs, y):
+    """As mxfp4_gemm with the activations in MXFP4: x [M, K/2], xs [M, K/32]."""
+    _same_device(w, ws, x, xs, y)
+    M, K, O = x.shape[0], x.shape[1] * 2, w.shape[0]
+    yp, ym, _, ldy = _rows(y, "y", O)
+    if ym != M:
+        raise ValueError(f"y: {ym} rows, expected {M}")
+    _chk(load().apus_hip_mxfp4_gemm_mx_dev(_bytes(w, (O, K // 2), "w"),
+                                           _bytes(ws, (O, K // 32), "ws"), _bytes(x, (M, K // 2), "x"),
+                                           _bytes(xs, (M, K // 32), "xs"), yp, _sz(ldy), _sz(M),
+                                           _sz(O), _sz(K)))
+
+
+# ---- mixture of experts
+def moe_layer(dims, w, norm_topk=True):
+    """ApusHipMoeLayer from dims (hidden, inter, experts, topk, shared_inter;
+    shared_inter 0: no shared expert) and device tensors w_router, w_gate_up,
+    w_down and, with a shared expert, w_shared_gate_up, w_shared_down and
+    (optional) w_shared_gate. With s_gate_up, s_down (s_shared_gate_up,
+    s_shared_down) the experts' weights are MXFP4 codes and these their
+    scales. The layer keeps the tensors alive."""
+    hidden, inter, experts, topk, shared = dims
+    mx = "s_gate_up" in w
+    _same_device(*w.values())
+    shapes = {"w_gate_up": (experts, 2 * inter, hidden), "w_down": (experts, hidden, inter)}
+    if shared:
+        shapes.update(w_shared_gate_up=(2 * shared, hidden), w_shared_down=(hidden, shared))
+    ptr = {}
+
+    def take(name, shape, size):
+        t = w[name]
+        if not t.is_cuda or not t.is_contiguous() or t.element_size() != size or tuple(t.shape) != shape:
+            raise ValueError(f"{name}: a contiguous GPU tensor of {size}-byte elements of shape {shape}, "
+                             f"not {tuple(t.shape)} {t.dtype} on {t.device}")
+        ptr[name] = t.data_ptr()
+
+    take("w_router", (experts, hidden), 2)
+    if shared and w.get("w_shared_gate") is not None:
+        take("w_shared_gate", (hidden,), 2)
+    for n, shape in shapes.items():
+        take(n, shape[:-1] + (shape[-1] // 2,) if mx else shape, 1 if mx else 2)
+        if mx:
+            take("s" + n[1:], shape[:-1] + (shape[-1] // 32,), 1)
+    L = MoeLayer(hidden=hidden, inter=inter, experts=experts, topk=topk, shared_inter=shared,
+                 norm_topk=int(bool(norm_topk)), mxfp4=int(mx), **ptr)
+    L._tensors = dict(w)
+    return L
+
+
+class MoeWork:
+    """apus_hip_moe_work_*: the device buffers of moe_layer_decode calls of up
+    to max_tokens tokens on layers of one shape. Calls that may overlap (other
+    streams, graphs replayed at once) need one each."""
+
+    def __init__(self, layer, max_tokens):
+        self.h = C.c_void_p()
+        _chk(load().apus_hip_moe_work_create(C.byref(layer), _sz(max_tokens), C.byref(self.h)))
+
+    def destroy(self):
+        if self.h:
+            _chk(load().apus_hip_moe_work_destroy(self.h))
+            self.h = C.c_void_p()
+
+
+def moe_layer_decode(layer, work, x, y):
+    """A mixture-of-experts layer on a decode step's tokens: x [T, hidden]
+    -> y [T, hidden], contiguous bf16 device tensors; y may be x."""
+    _same_device(x, y, layer._tensors["w_router"])
+    for t, n in ((x, "x"), (y, "y")):
+        if t.dim() != 2 or t.shape != x.shape or t.shape[1] != layer.hidden or t.element_size() != 2:
+            raise ValueError(f"{n}: [T, {layer.hidden}] bf16, not {tuple(t.shape)} {t.dtype}")
+    _chk(load().apus_hip_moe_layer_decode(C.byref(layer), work.h, _sz(x.shape[0]), _dp(x), _dp(y)))
 
 
 # ---- named-intermediate capture

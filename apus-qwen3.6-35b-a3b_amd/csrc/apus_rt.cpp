@@ -94,9 +94,14 @@ int hip_fail(hipError_t e, const char *what, const char *file, int line) {
                      hipGetErrorString(e), file, line);
 }
 
-int ensure_ready() {
+int check_enabled() {
     if (disabled_by_env())
         return set_error(kErrDisabled, "disabled by APUS_HIP_DISABLE");
+    return kOk;
+}
+
+int ensure_ready() {
+    if (int r = check_enabled()) return r;
     if (g_ready) return kOk;
     int n = 0;
     hipError_t e = hipGetDeviceCount(&n);

@@ -29,6 +29,7 @@ int hip_fail(hipError_t e, const char *what, const char *file, int line);
 // Lazily initialises the device on first use (device 0 unless
 // apus_hip_init chose another). Returns kOk or an error code.
 int ensure_ready();
+int check_enabled();   // kErrDisabled under APUS_HIP_DISABLE, else kOk
 hipStream_t stream();
 int cu_count();     // compute units of the current device
 int current_device();

@@ -1,0 +1,18 @@
+// mx.h -- host checks shared by the MXFP4 and mixture-of-experts entry points.
+// These check their arguments before they look for a device, so that a bad
+// call is refused the same way with and without one.
+#pragma once
+#include "apus_rt.h"
+
+namespace apus {
+
+int mx_check_dims(size_t M, size_t O, size_t K);   // sizes under 2^31, K in whole blocks
+int mx_ready();                                    // ensure_ready, on the calling thread's device
+
+}  // namespace apus
+
+#define APUS_ENABLED()                                                       \
+    do {                                                                     \
+        int r_ = ::apus::check_enabled();                                    \
+        if (r_ != ::apus::kOk) return r_;                                    \
+    } while (0)

@@ -569,6 +569,79 @@ int apus_hip_attn_layer_decode_paged(const ApusHipAttnLayer *L, const ApusHipAtt
                                      const int32_t *pos0, const uint16_t *ln1,
                                      const ApusHipKvCache *kv, uint16_t *ao);
 
+/* ---- MXFP4: 4-bit weights and activations -------------------------------
+ * The OCP microscaling format, for a row of K elements (K a multiple of
+ * 32): every 32 consecutive elements share a scale 2^(s - 127), s one byte
+ * (255: the block is NaN); an element is e2m1 (sign; 0 .5 1 1.5 2 3 4 6),
+ * two to a byte, the even element in the low half. codes [rows][K/2],
+ * scales [rows][K/32], dense. Device pointers; codes and bf16 rows 16-byte
+ * aligned. ldx / ldy: elements from one bf16 row to the next (ldx a
+ * multiple of 8), so that a column slice of a wider buffer can be given. An
+ * output may not overlap an input. No host data, no scratch: a call may be
+ * captured into a graph, and calls on different data may run at once. Bad
+ * arguments are refused with or without a device. */
+
+/* x [M][K] bf16 -> codes, scales. The scale is 2^(floor(log2 of the
+ * block's largest magnitude) - 2), at least 2^-127; elements round to
+ * nearest, ties to even, and saturate at 6 scales; zero keeps its sign. A
+ * block that holds an infinity or NaN becomes NaN as a whole. */
+int apus_hip_mxfp4_quantize(const uint16_t *x, size_t ldx, uint8_t *codes, uint8_t *scales,
+                            size_t M, size_t K);
+/* The values of codes, scales as bf16 (exact, but for the largest scales,
+ * whose values past bf16's range become infinite). */
+int apus_hip_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, uint16_t *x,
+                              size_t ldx, size_t M, size_t K);
+/* y[m][o] = rnd(sum_k w[o][k] x[m][k]): w MXFP4 (O rows of K), x bf16, y
+ * bf16, fp32 accumulation in the kernel's order (the tolerance class of
+ * apus_hip_bf16_gemm_mfma_dev: |c - r| <= 2e-3 (|r| + sum_k |w x|)). K = 0
+ * gives zeros. */
+int apus_hip_mxfp4_gemm_dev(const uint8_t *w, const uint8_t *ws, const uint16_t *x, size_t ldx,
+                            uint16_t *y, size_t ldy, size_t M, size_t O, size_t K);
+/* The same with x in MXFP4 too (codes x [M][K/2], scales xs [M][K/32]), on
+ * the matrix cores' 4-bit form. */
+int apus_hip_mxfp4_gemm_mx_dev(const uint8_t *w, const uint8_t *ws, const uint8_t *x,
+                               const uint8_t *xs, uint16_t *y, size_t ldy, size_t M, size_t O,
+                               size_t K);
+
+/* ---- a mixture-of-experts layer for a decode step ------------------------
+ * Per token x (a layer's normed input):
+ *   l = w_router x; the topk experts of largest l (ties: the lowest index);
+ *   p = softmax of l over the chosen ones (norm_topk) or over all experts;
+ *   y = sum_e p_e w_down[e] (silu(gate) * up), (gate | up) = w_gate_up[e] x,
+ *       + sigmoid(w_shared_gate . x) times the same of the shared expert.
+ * Logits, softmax and sums are fp32; y is rounded once. Logits that are NaN
+ * count as the largest (that token's y is NaN). The experts' weights are
+ * bf16, or MXFP4 with their scales; the router's are bf16. */
+typedef struct {
+    size_t hidden, inter;           /* multiples of 32 */
+    size_t experts, topk;           /* up to 1024, up to 32 */
+    size_t shared_inter;            /* 0: no shared expert */
+    int norm_topk;                  /* p sums to 1 over the chosen experts */
+    int mxfp4;                      /* expert weights: 0 bf16, 1 MXFP4 codes */
+    const uint16_t *w_router;       /* [experts][hidden] */
+    const void *w_gate_up;          /* [experts][2 inter][hidden], gate rows first */
+    const void *w_down;             /* [experts][hidden][inter] */
+    const void *w_shared_gate_up;   /* [2 shared_inter][hidden] */
+    const void *w_shared_down;      /* [hidden][shared_inter] */
+    const uint16_t *w_shared_gate;  /* [hidden], or NULL: weight 1 */
+    const uint8_t *s_gate_up, *s_down, *s_shared_gate_up, *s_shared_down;
+} ApusHipMoeLayer;
+
+/* The device buffers of calls of up to max_tokens (<= 1024) tokens on layers
+ * of this one's sizes (its weights are not looked at). Calls that share one
+ * run one after the other: on one stream, or ordered by the caller; calls or
+ * graph replays that may overlap need one each. It must outlive the graphs
+ * that captured its calls. destroy waits for the library's stream. */
+typedef struct ApusHipMoeWork ApusHipMoeWork;
+int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHipMoeWork **out);
+int apus_hip_moe_work_destroy(ApusHipMoeWork *w);
+
+/* x [T][hidden] -> y [T][hidden], bf16, 16-byte aligned; y may be x. T up to
+ * the workspace's (0: nothing is done). Neither allocates nor waits, and may
+ * be captured into a graph. */
+int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_t T,
+                              const uint16_t *x, uint16_t *y);
+
 #ifdef __cplusplus
 }
 #endif
