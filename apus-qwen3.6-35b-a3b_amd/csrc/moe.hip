@@ -6,10 +6,13 @@
 //       + sigmoid(w_shared_gate . x) shared(x),
 // everything in fp32, rounded once, at y. The weights are bf16 or MXFP4.
 //
-// For few tokens the layer is the reading of the chosen experts' weights.
-// Launches: router logits; the choice; gate, up and silu of every (expert,
-// 16 outputs) with that expert's tokens as the columns of an MFMA; down of
-// every (expert, 64 outputs) into fp32 partial rows; the weighted sum.
+// For few tokens the layer is the reading of the chosen experts' weights, so
+// every kernel streams weights through the MFMA with tokens as its 16 columns.
+// Launches: k_moe_router, logits and, by the last workgroup of each 16 tokens
+// to finish, the choice; k_moe_up, gate, up and silu of every (expert, 16
+// outputs); then either k_moe_down, down of every (expert, 64 outputs) into
+// fp32 partial rows, and k_moe_combine, their weighted sum, or for up to
+// kFewTokens tokens k_moe_down_few, both in one.
 // The intermediate h = silu(g) u goes to the down product as two bf16 numbers
 // (its leading 8 bits and the rest rounded to 8), which keeps 16 bits of it: the
 // product reads weights, not h, so the second MFMA costs no time, and a single
@@ -35,11 +38,17 @@ struct ApusHipMoeWork {
     float *wts;          // [T][topk + 1]: p, then the shared expert's weight
     uint16_t *h;         // [T topk][2][inter], then [T][2][shared]
     float *part;         // [T topk + T][hidden]
+    uint32_t *done;      // workgroups of k_moe_router done, per 16 tokens, then of
+                         // those the ones that have chosen (0 between calls)
+    int4 *slots;         // expert, first of its choices in list, how many (up to kGroup)
+    uint16_t *list;      // [T topk]: choices by expert
 };
 
 namespace {
 
 constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
+constexpr int kFewTokens = 4;          // up to here a choice is a slot of its own
+constexpr int kGroup = 32;             // most rows of a slot
 
 struct MoeArgs {
     const uint16_t *x, *w_router, *w_sgate;
@@ -47,264 +56,697 @@ struct MoeArgs {
     const uint8_t *s_gu, *s_dn, *s_sgu, *s_sdn;
     float *logits, *wts, *part;
     int32_t *ids;
+    uint32_t *done;
+    int4 *slots;
+    uint16_t *list;
     uint16_t *h;
     uint16_t *y;
-    int T, H, I, E, k, Is, norm;
+    int T, H, I, E, k, Is, norm, nslots;
 };
 
 // ---- router ---------------------------------------------------------------
-// 16 experts (the shared gate as one more) x 16 tokens a workgroup, K over
-// its 4 wavefronts.
-__global__ __launch_bounds__(256) void k_moe_router(MoeArgs a) {
-    __shared__ mx_f32x4 red[4][64];
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int E1 = a.E + 1, e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
-    const int er = min(e0 + r, a.w_sgate ? a.E : a.E - 1);
-    const auto wr = er < a.E ? WBf16::row(a.w_router, nullptr, er, a.H, g)
-                             : WBf16::row(a.w_sgate, nullptr, 0, a.H, g);
-    const auto xr = XBf16<WBf16>::row(a.x, a.H, min(t0 + r, a.T - 1), g);
-    mx_f32x4 acc{};
-    for (int k = wave * 128; k < a.H; k += 512) {
-        WBf16::Frag wf;
-        XBf16<WBf16>::Frag xf;
-        WBf16::load(wf, wr, k, a.H);
-        XBf16<WBf16>::load(xf, xr, k, a.H);
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            acc = mfma16(WBf16::operand(wf, j), __builtin_bit_cast(mx_bf16x8, xf.v[j]), acc);
-    }
-    red[wave][lane] = acc;
-    __syncthreads();
-    if (wave) return;
-    acc = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    if (t0 + r >= a.T) return;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (e0 + 4 * g + i < E1) a.logits[(size_t)(t0 + r) * E1 + e0 + 4 * g + i] = acc[i];
-}
+// slots that T tokens can fill
+size_t moe_slots(size_t T, size_t k, size_t E) { return std::min(T * k, E) + T * k / kGroup; }
 
-// Order of logits as unsigned numbers: NaN above all, -0 and +0 alike.
+// Order of logits as unsigned numbers: NaN above all, -0 and +0 alike. No
+// number's key is 0.
 __device__ __forceinline__ uint32_t order_key(float f) {
     uint32_t u = __float_as_uint(f + 0.0f);
     if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
     if (u == 0x80000000u) u = 0;
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return k == 0xffffffffu ? NAN : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// A wavefront's choice for token t: lane l holds logits l, l + 64, ...
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+// over the wavefront: within rows of 16 by lane permutations, the four rows
+// from scalars
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, dpp<0xb1>(v));                            // lane ^ 1
+    v = max(v, dpp<0x4e>(v));                            // lane ^ 2
+    v = max(v, dpp<0x141>(v));                           // mirrored halves of a row
+    v = max(v, dpp<0x140>(v));                           // mirrored row
+    auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    return max(max(at(0), at(16)), max(at(32), at(48)));
+}
+__device__ __forceinline__ float wave_sum(float f) {
+    auto add = [](float a, uint32_t b) { return a + __uint_as_float(b); };
+    f = add(f, dpp<0xb1>(__float_as_uint(f)));
+    f = add(f, dpp<0x4e>(__float_as_uint(f)));
+    f = add(f, dpp<0x141>(__float_as_uint(f)));
+    f = add(f, dpp<0x140>(__float_as_uint(f)));
+    return (lane_bcast(f, 0) + lane_bcast(f, 16)) + (lane_bcast(f, 32) + lane_bcast(f, 48));
+}
+
+// A wavefront's choice for token t, in index order: lane l holds logits l,
+// l + 64, ... The k-th largest key is found a bit at a time from the top,
+// counting by ballots (k rounds of a maximum over the wavefront took 8 us, this
+// takes under one); of the keys equal to it the lowest indices are taken.
 template <int NJ>
 __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
     const float *lg = a.logits + (size_t)t * (a.E + 1);
+    // (written by other workgroups of this launch: read where they met)
+    auto logit = [&](int e) { return __hip_atomic_load(lg + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     float l[NJ];
-    uint32_t key[NJ];                      // 0: past E, or taken (no number's key is 0)
+    uint32_t key[NJ], best = 0;            // key 0: past E
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int e = lane + 64 * j;
-        l[j] = e < a.E ? lg[e] : 0.0f;
+        l[j] = logit(min(e, a.E - 1));
         key[j] = e < a.E ? order_key(l[j]) : 0;
     }
-    float top = 0.0f, mine = 0.0f, sum = 0.0f;
-    int my_e = 0;
-    for (int n = 0; n < a.k; n++) {
-        uint32_t bk = 0;
-        int be = 0;
-        float bl = 0.0f;
+    const float sgate = logit(a.w_sgate ? a.E : 0);
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
-            if (key[j] > bk) {             // (ties: the lane's lowest index first)
-                bk = key[j];
-                be = lane + 64 * j;
-                bl = l[j];
-            }
+    for (int j = 0; j < NJ; j++) best = max(best, key[j]);
+    const float top = key_value(wave_max(best));
+    auto count = [&](uint32_t v) {         // keys >= v
+        int n = 0;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t ok = __shfl_xor(bk, d);
-            const int oe = __shfl_xor(be, d);
-            const float ol = __shfl_xor(bl, d);
-            if (ok > bk || (ok == bk && oe < be)) {
-                bk = ok;
-                be = oe;
-                bl = ol;
-            }
+        for (int j = 0; j < NJ; j++) n += __popcll(__ballot(key[j] >= v));
+        return n;
+    };
+    uint32_t v = 0;
+    int above = 0;                         // keys > v
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t c = v | 1u << b;
+        const int n = count(c);
+        if (n >= a.k) v = c;
+        if (n == a.k) break;
+    }
+    above = v == 0xffffffffu ? 0 : count(v + 1);
+    int ties = a.k - above, at = 0;        // of the keys equal to v, the first `ties`
+    const uint64_t below = (1ull << lane) - 1;
+    float p[NJ], sum = 0.0f;
+    int pos[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const uint64_t eq = __ballot(key[j] == v);
+        const bool in = key[j] > v || (key[j] == v && __popcll(eq & below) < ties);
+        const uint64_t m = __ballot(in);
+        pos[j] = in ? at + __popcll(m & below) : -1;
+        at += __popcll(m);
+        ties -= min(ties, (int)__popcll(eq));
+        p[j] = expf(l[j] - top);
+        if (lane + 64 * j < a.E && (in || !a.norm)) sum += p[j];
+    }
+    sum = wave_sum(sum);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+        if (pos[j] >= 0) {
+            __hip_atomic_store(a.ids + t * a.k + pos[j], lane + 64 * j, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+            a.wts[t * (a.k + 1) + pos[j]] = p[j] / sum;
         }
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-            if (be == lane + 64 * j) key[j] = 0;
-        if (n == 0) top = bl;
-        const float p = expf(bl - top);
-        sum += p;
-        if (lane == n) {
-            mine = p;
-            my_e = be;
-        }
-    }
-    if (!a.norm) {
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-            if (lane + 64 * j < a.E) s += expf(l[j] - top);
-        sum = wave_sum(s);
-    }
-    if (lane < a.k) {
-        a.ids[t * a.k + lane] = my_e;
-        a.wts[t * (a.k + 1) + lane] = mine / sum;
-    }
     if (lane == 0)
-        a.wts[t * (a.k + 1) + a.k] = a.w_sgate ? 1.0f / (1.0f + expf(-lg[a.E])) : 1.0f;
+        a.wts[t * (a.k + 1) + a.k] = a.w_sgate ? 1.0f / (1.0f + expf(-sgate)) : 1.0f;
 }
 
-__global__ __launch_bounds__(256) void k_moe_topk(MoeArgs a) {
-    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (t >= a.T) return;
-    if (a.E <= 256) choose<4>(a, t, lane);
-    else choose<16>(a, t, lane);
+constexpr int kRouterWaves = 16;
+
+// The choices of all tokens by expert, by one workgroup: count, sum, place. (In
+// which order an expert's choices come does not matter: a choice's values do
+// not depend on its place.)
+__device__ __forceinline__ void make_slots(const MoeArgs &a, int lane, int wave) {
+    __shared__ int cursor[kMoeMaxExperts], wsum[2][kRouterWaves];
+    const int tid = threadIdx.x, n = a.T * a.k;
+    auto id = [&](int q) {                 // (chosen by other workgroups of this launch)
+        const int e = __hip_atomic_load(a.ids + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return min(max(e, 0), a.E - 1);    // (in range whatever ids holds)
+    };
+    cursor[tid] = 0;
+    __syncthreads();
+    for (int q = tid; q < n; q += 64 * kRouterWaves) atomicAdd(&cursor[id(q)], 1);
+    __syncthreads();
+    // thread e: running sums over the experts, of the choices and of the slots
+    const int c = cursor[tid], k = (c + kGroup - 1) / kGroup;
+    int at = c, slot = k;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(at, d), u = __shfl_up(slot, d);
+        if (lane >= d) {
+            at += o;
+            slot += u;
+        }
+    }
+    if (lane == 63) {
+        wsum[0][wave] = at;
+        wsum[1][wave] = slot;
+    }
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < kRouterWaves; w++) {
+        if (w < wave) {
+            at += wsum[0][w];
+            slot += wsum[1][w];
+        }
+        total += wsum[1][w];
+    }
+    for (int i = 0; i < k; i++)
+        a.slots[slot - k + i] = make_int4(tid, at - c + i * kGroup, min(kGroup, c - i * kGroup), 0);
+    for (int i = total + tid; i < a.nslots; i += 64 * kRouterWaves) a.slots[i] = make_int4(0, 0, 0, 0);
+    cursor[tid] = at - c;
+    __syncthreads();
+    for (int q = tid; q < n; q += 64 * kRouterWaves) a.list[atomicAdd(&cursor[id(q)], 1)] = (uint16_t)q;
+}
+
+// 16 experts (the shared gate as one more) x 16 tokens a workgroup, K over its
+// 16 wavefronts. The last workgroup of the 16 tokens to finish chooses for
+// them, a wavefront each, and the last of those sorts the choices: what a
+// workgroup hands on it stores where all XCDs see it, waits for the stores, and
+// counts itself; nobody waits for anybody.
+static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
+template <int NJ>
+__global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
+    __shared__ mx_f32x4 red[kRouterWaves][64];
+    __shared__ int last;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int E1 = a.E + 1, t0 = blockIdx.y * 16;
+    // the last workgroup of a shared gate takes its one row, as expert E
+    const bool gate = a.w_sgate && blockIdx.x == gridDim.x - 1;
+    const int e0 = gate ? a.E : blockIdx.x * 16, ne = gate ? 1 : min(16, a.E - e0);
+    const auto wt = gate ? WBf16::tile(a.w_sgate, nullptr, 0, 1, a.H) : WBf16::tile(a.w_router, nullptr, e0, ne, a.H);
+    const auto wl = WBf16::lane(lane, a.H);
+    using X = XBf16<WBf16>;
+    const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
+    const uint32_t xl = X::lane((uint32_t)(t0 + r) * (uint32_t)a.H * 2, g);
+    mx_f32x4 acc{};
+    for (int st = wave; st * 128 < a.H; st += kRouterWaves) {
+        WBf16::Frag wf;
+        X::Frag xf;
+        WBf16::load(wf, wt, wl, st, a.H);
+        X::load(xf, xb, xl, st, a.H);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            acc = mfma16(WBf16::operand(wf, j), __builtin_bit_cast(mx_bf16x8, xf.v[j]), acc);
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    auto count = [&](uint32_t *done, uint32_t of) {      // thread 0: the last of `of`?
+        const uint32_t n = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = n == of - 1;
+        if (last) *done = 0;                             // for the next call
+    };
+    if (wave == 0) {
+        mx_f32x4 s[4] = {};
+#pragma unroll
+        for (int i = 0; i < kRouterWaves; i++) s[i & 3] += red[i][lane];
+        acc = (s[0] + s[1]) + (s[2] + s[3]);
+        if (t0 + r < a.T) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (4 * g + i < ne)
+                    __hip_atomic_store(a.logits + (size_t)(t0 + r) * E1 + e0 + 4 * g + i, acc[i],
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (lane == 0) count(a.done + blockIdx.y, gridDim.x);
+    }
+    __syncthreads();
+    if (!last) return;
+    if (t0 + wave < a.T) choose<NJ>(a, t0 + wave, lane);
+    if (a.T <= kFewTokens) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) count(a.done + gridDim.y, gridDim.y);
+    __syncthreads();
+    if (last) make_slots(a, lane, wave);
 }
 
 // ---- experts ----------------------------------------------------------------
-// Blocks of a launch: first nsh for the shared expert, then per slot nper. A
-// slot is an expert, or, where the tokens make fewer choices than there are
-// experts, a choice; of the choices of one expert the first does the work.
-// Returns the expert (E: shared), or -1: nothing to do. list: the choices
-// t * k + n that fell on it (shared: T k + t), cnt of them, in any order (a
-// choice's values do not depend on its place).
-__device__ __forceinline__ int gather(const MoeArgs &a, int b, int nsh, int nper, int &part,
-                                      uint16_t *list, int *cnt) {
-    const int n = a.T * a.k;
-    if (b < nsh) {
-        part = b;
-        for (int t = threadIdx.x; t < a.T; t += blockDim.x) list[t] = (uint16_t)(n + t);
-        if (threadIdx.x == 0) *cnt = a.T;
-        __syncthreads();
-        return a.E;
+// What a workgroup works on: n rows of the activations, for the expert's row
+// blocks. Blocks of a launch: first the shared expert's, nsh row blocks for
+// every kGroup tokens; then nper row blocks per slot. A slot is up to kGroup of
+// an expert's choices (a popular expert has several, side by side on the chip
+// instead of one after the other), or with few tokens a choice.
+struct Task {
+    int e, part, first, n;                 // e == E: shared; n = 0: nothing
+    const uint16_t *list;                  // or null: choices first, first + 1, ..
+};
+__device__ __forceinline__ Task task_of(const MoeArgs &a, int b, int nsh, int nper) {
+    const int groups = nsh ? (a.T + kGroup - 1) / kGroup : 0;
+    if (b < nsh * groups) {
+        const int t = b / nsh * kGroup;
+        return {a.E, b % nsh, a.T * a.k + t, min(kGroup, a.T - t), nullptr};
     }
-    const int slot = (b - nsh) / nper;
-    part = (b - nsh) % nper;
-    const bool by_choice = n < a.E;
-    const int e = by_choice ? a.ids[slot] : slot;
-    if (threadIdx.x == 0) *cnt = 0;
-    __syncthreads();
-    int dup = 0;
-    for (int q = threadIdx.x; q < n; q += blockDim.x)
-        if (a.ids[q] == e) {
-            dup |= by_choice && q < slot;
-            // (a token chooses an expert once: at most T; the test holds for
-            // any contents of ids)
-            const int p = atomicAdd(cnt, 1);
-            if (p < (int)kMoeMaxTokens) list[p] = (uint16_t)q;
-        }
-    dup = __syncthreads_or(dup);
-    if (threadIdx.x == 0 && *cnt > a.T) *cnt = a.T;
-    __syncthreads();
-    return dup || *cnt == 0 ? -1 : e;
+    b -= nsh * groups;
+    const int slot = b / nper, part = b % nper;
+    if (a.T <= kFewTokens)
+        return {__builtin_amdgcn_readfirstlane(a.ids[slot]), part, slot, 1, nullptr};
+    const int4 s = a.slots[slot];
+    return {__builtin_amdgcn_readfirstlane(s.x), part, 0, __builtin_amdgcn_readfirstlane(s.z),
+            a.list + __builtin_amdgcn_readfirstlane(s.y)};
+}
+__device__ __forceinline__ int choice(const Task &k, int i) {
+    i = min(i, k.n - 1);
+    return k.list ? k.list[i] : k.first + i;
 }
 
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
-// h = silu(gate x) * (up x): 16 outputs of one expert for its tokens, 16 at a
-// time, K over the 4 wavefronts.
+// h of choice q: its two planes, a row of I each; the elements before it, and all
+__device__ __forceinline__ uint32_t h_at(const MoeArgs &a, int q, bool sh) {
+    const uint32_t n = a.T * a.k;
+    return sh ? n * 2 * a.I + (q - n) * 2 * a.Is : q * 2 * a.I;
+}
+__device__ __forceinline__ uint32_t h_all(const MoeArgs &a) { return 2 * a.T * (a.k * a.I + a.Is); }
+
+// h as its leading bits, cut, and the rest, rounded (none of an infinity or NaN)
+__device__ __forceinline__ void split_h(float v, uint16_t &hi, uint16_t &lo) {
+    const uint32_t bits = __float_as_uint(v);
+    const bool fin = (bits & 0x7f800000u) != 0x7f800000u;
+    hi = fin ? (uint16_t)(bits >> 16) : f2bf(v);
+    lo = fin ? f2bf(v - bf2f(hi)) : 0;
+}
+
+// Two forms of each expert kernel. k_moe_up and k_moe_down share a row block's K
+// out over the 8 wavefronts of a workgroup, whose partial sums meet in LDS: most
+// bytes on their way at once for a task, for calls with few of them. Where the
+// row blocks are enough wavefronts to fill the chip, in k_moe_up_stream and
+// k_moe_down_stream each walks all of K for its rows by itself.
+constexpr int kMoeWaves = 8;
+
+// h = silu(gate x) * (up x): 16 outputs a workgroup, 16 rows at a time
 template <class W>
-__global__ __launch_bounds__(256) void k_moe_up(MoeArgs a, int nsh, int nper) {
-    __shared__ uint16_t list[kMoeMaxTokens];
-    __shared__ int cnt;
-    __shared__ mx_f32x4 red[4][2][64];
-    int part;
-    const int e = gather(a, blockIdx.x, nsh, nper, part, list, &cnt);
-    if (e < 0) return;
+__global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, int nper) {
+    __shared__ mx_f32x4 red[kMoeWaves * 2][64];
+    __shared__ int rows[16];
+    constexpr int S = 2;                   // steps in flight at once
+    using X = XBf16<W>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool sh = e == a.E;
-    const int I = sh ? a.Is : a.I, n = cnt, o0 = part * 16;
-    const size_t row0 = sh ? 0 : (size_t)e * 2 * I;
-    const void *w = sh ? a.w_sgu : a.w_gu;
-    const uint8_t *ws = sh ? a.s_sgu : a.s_gu;
-    const auto wg = W::row(w, ws, row0 + o0 + r, a.H, g);
-    const auto wu = W::row(w, ws, row0 + I + o0 + r, a.H, g);
-    for (int c0 = 0; c0 < n; c0 += 16) {
-        const int q = list[min(c0 + r, n - 1)];
-        const int t = sh ? q - a.T * a.k : q / a.k;
-        const auto xr = XBf16<W>::row(a.x, a.H, t, g);
-        mx_f32x4 ag{}, au{};
-        for (int k = wave * 128; k < a.H; k += 512) {
-            typename W::Frag fg, fu;
-            typename XBf16<W>::Frag fx;
-            W::load(fg, wg, k, a.H);
-            W::load(fu, wu, k, a.H);
-            XBf16<W>::load(fx, xr, k, a.H);
+    const Task task = task_of(a, blockIdx.x, nsh, nper);
+    if (task.n == 0) return;
+    const bool sh = task.e == a.E;
+    const int I = sh ? a.Is : a.I, o0 = task.part * 16;
+    typename W::Tile wt[2];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const mx_bf16x8 xv = __builtin_bit_cast(mx_bf16x8, fx.v[j]);
-                ag = mfma16(W::operand(fg, j), xv, ag);
-                au = mfma16(W::operand(fu, j), xv, au);
-            }
-        }
-        red[wave][0][lane] = ag;
-        red[wave][1][lane] = au;
-        __syncthreads();
-        if (wave == 0 && c0 + r < n) {
-            ag = (red[0][0][lane] + red[1][0][lane]) + (red[2][0][lane] + red[3][0][lane]);
-            au = (red[0][1][lane] + red[1][1][lane]) + (red[2][1][lane] + red[3][1][lane]);
-            uint16_t *h = a.h + (sh ? (size_t)a.T * a.k * 2 * a.I + (size_t)t * 2 * I : (size_t)q * 2 * I);
+    for (int i = 0; i < 2; i++)
+        wt[i] = W::tile(sh ? a.w_sgu : a.w_gu, sh ? a.s_sgu : a.s_gu,
+                        (sh ? 0 : (size_t)task.e * 2 * I) + i * I + o0, 16, a.H);
+    const auto wl = W::lane(lane, a.H);
+    const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
+    for (int c = 0; c < task.n; c += 16) {
+        const int q = choice(task, c + r);
+        const uint32_t xl = X::lane((uint32_t)(sh ? q - a.T * a.k : q / a.k) * (uint32_t)a.H * 2, g);
+        mx_f32x4 acc[2] = {};
+        for (int st = wave * S; st * 128 < a.H; st += kMoeWaves * S) {
+            typename W::Frag fw[S][2];
+            typename X::Frag fx[S];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float v = silu(ag[i]) * au[i];
-                // the leading bits, cut, and the rest, rounded (none of an
-                // infinity or NaN)
-                const uint32_t u = __float_as_uint(v);
-                const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-                const uint16_t hi = fin ? (uint16_t)(u >> 16) : f2bf(v);
-                const int o = o0 + 4 * g + i;
-                h[o] = hi;
-                h[I + o] = fin ? f2bf(v - bf2f(hi)) : 0;
-            }
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) W::load(fw[s][i], wt[i], wl, st + s, a.H);
+#pragma unroll
+            for (int s = 0; s < S; s++) X::load(fx[s], xb, xl, st + s, a.H);
+            // (all loads issued before the first use)
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        acc[i] = mfma16(W::operand(fw[s][i], j), __builtin_bit_cast(mx_bf16x8, fx[s].v[j]), acc[i]);
         }
+        if (c) __syncthreads();                          // red's readers are done
+        red[wave * 2][lane] = acc[0];
+        red[wave * 2 + 1][lane] = acc[1];
+        if (wave == 0 && g == 0) rows[r] = q;
         __syncthreads();
+        // a thread finishes one output of a row, 16 outputs of a row side by side
+        const int o = threadIdx.x & 15, row = threadIdx.x >> 4;
+        if (row < 16 && c + row < task.n) {
+            float s[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kMoeWaves; w++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    s[i] += reinterpret_cast<const float *>(&red[w * 2 + i][(o >> 2) * 16 + row])[o & 3];
+            uint16_t *h = a.h + h_at(a, rows[row], sh) + o0 + o;
+            split_h(silu(s[0]) * s[1], h[0], h[I]);
+        }
     }
 }
 
-// part[choice] = down h: 64 outputs of one expert, 16 a wavefront
+// wavefronts that share a row block's K in k_moe_down, a step each (longer rows:
+// more rounds), for I inner elements, and the rows of a workgroup
+__host__ __device__ constexpr int down_split(int I) { return I > 512 ? 8 : I > 256 ? 4 : I > 128 ? 2 : 1; }
+__host__ __device__ constexpr int down_rows(int I) { return kMoeWaves / down_split(I) * 32; }
+
+// part[choice] = down h: 32 outputs a group of wavefronts, 16 rows at a time
 template <class W>
-__global__ __launch_bounds__(256) void k_moe_down(MoeArgs a, int nsh, int nper) {
-    __shared__ uint16_t list[kMoeMaxTokens];
-    __shared__ int cnt;
-    int part;
-    const int e = gather(a, blockIdx.x, nsh, nper, part, list, &cnt);
-    if (e < 0) return;
+__global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh, int nper) {
+    constexpr int RT = 2;
+    __shared__ mx_f32x4 red[kMoeWaves * RT][64];
+    __shared__ int rows[16];
+    using X = XBf16<W>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool sh = e == a.E;
-    const int I = sh ? a.Is : a.I, n = cnt, o0 = part * 64 + wave * 16;
-    if (o0 >= a.H) return;                 // (H is a multiple of 32; no barrier follows)
-    const size_t row0 = sh ? 0 : (size_t)e * a.H;
-    const auto wr = W::row(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn, row0 + o0 + r, I, g);
-    for (int c0 = 0; c0 < n; c0 += 16) {
-        const int q = list[min(c0 + r, n - 1)];
-        const uint16_t *h = a.h + (sh ? (size_t)a.T * a.k * 2 * a.I + (size_t)(q - a.T * a.k) * 2 * I
-                                      : (size_t)q * 2 * I);
-        const auto xh = XBf16<W>::row(h, 0, 0, g), xl = XBf16<W>::row(h + I, 0, 0, g);
-        mx_f32x4 acc{};
-        for (int k = 0; k < I; k += 128) {
-            typename W::Frag fw;
-            typename XBf16<W>::Frag fh, fl;
-            W::load(fw, wr, k, I);
-            XBf16<W>::load(fh, xh, k, I);
-            XBf16<W>::load(fl, xl, k, I);
+    const Task task = task_of(a, blockIdx.x, nsh, nper);
+    if (task.n == 0) return;
+    const bool sh = task.e == a.E;
+    const int I = sh ? a.Is : a.I, ks = down_split(I), kw = wave % ks, rg = wave / ks;
+    const int o0 = task.part * down_rows(I);
+    typename W::Tile wt[RT];               // (a tile past H, not stored, repeats the last)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const mx_bf16x8 wv = W::operand(fw, j);
-                acc = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fh.v[j]), acc);
-                acc = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fl.v[j]), acc);
+    for (int t = 0; t < RT; t++)
+        wt[t] = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn,
+                        (sh ? 0 : (size_t)task.e * a.H) + min(o0 + (rg * RT + t) * 16, a.H - 16), 16, I);
+    const auto wl = W::lane(lane, I);
+    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
+    for (int c = 0; c < task.n; c += 16) {
+        const int q = choice(task, c + r);
+        const uint32_t xl = X::lane(h_at(a, q, sh) * 2, g);
+        mx_f32x4 acc[RT] = {};
+        for (int st = kw; st * 128 < I; st += ks) {
+            typename W::Frag fw[RT];
+            typename X::Frag fh, fl;
+#pragma unroll
+            for (int t = 0; t < RT; t++) W::load(fw[t], wt[t], wl, st, I);
+            X::load(fh, hb, xl, st, I);
+            X::load(fl, hb, xl + I * 2, st, I);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    const mx_bf16x8 wv = W::operand(fw[t], j);
+                    acc[t] = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fh.v[j]), acc[t]);
+                    acc[t] = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fl.v[j]), acc[t]);
+                }
+        }
+        if (c) __syncthreads();                          // red's readers are done
+#pragma unroll
+        for (int t = 0; t < RT; t++) red[wave * RT + t][lane] = acc[t];
+        if (wave == 0 && g == 0) rows[r] = q;
+        __syncthreads();
+        // a thread finishes 4 outputs of a row
+        for (int e = threadIdx.x; e < kMoeWaves / ks * RT * 64; e += 64 * kMoeWaves) {
+            const int l = e & 63, t = (e >> 6) % RT, x = (e >> 6) / RT;
+            const int o = o0 + (x * RT + t) * 16;
+            if (c + (l & 15) >= task.n || o >= a.H) continue;
+            mx_f32x4 s = red[x * ks * RT + t][l];
+            for (int y = 1; y < ks; y++) s += red[(x * ks + y) * RT + t][l];
+            *reinterpret_cast<mx_f32x4 *>(a.part + (size_t)rows[l & 15] * a.H + o + 4 * (l >> 4)) = s;
+        }
+    }
+}
+
+// ---- the same, a wavefront alone: no partial sums, no barrier, and D steps of
+// weights and activations on their way all along its walk. Rows come along their
+// length and become operands in LDS of the wavefront's own.
+constexpr int kStreamWaves = 4;
+
+constexpr int kDownH = 32 * 1024;      // LDS bytes that k_moe_down_stream has for h of 16 rows
+
+// (what comes before stays before)
+__device__ __forceinline__ void fence() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// steps [0, n) of a walk: load(slot, step), and mul(slot, step), which takes the
+// slot's operands before it requests the step D after. The last round may go up
+// to D - 1 steps past n: zeros.
+template <int D, class Mul>
+__device__ __forceinline__ void walk_on(int n, Mul mul) {
+    for (int b = 0; b < n; b += D) {
+#pragma unroll
+        for (int d = 0; d < D; d++) mul(d, b + d);
+    }
+}
+template <int D, class Load, class Mul>
+__device__ __forceinline__ void walk(int n, Load load, Mul mul) {
+#pragma unroll
+    for (int d = 0; d < D; d++) load(d, d);
+    fence();
+    walk_on<D>(n, mul);
+}
+
+template <class W, int RT, int NT, int D>
+__device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, int o0, char *m, int lane) {
+    using X = XBf16<W>;
+    const int r = lane & 15, g = lane >> 4;
+    const bool sh = task.e == a.E;
+    const int I = sh ? a.Is : a.I;
+    typename W::Tile wt[RT][2];            // (a tile past I, not stored, repeats the last)
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            wt[t][i] = W::tile(sh ? a.w_sgu : a.w_gu, sh ? a.s_sgu : a.s_gu,
+                               (sh ? 0 : (size_t)task.e * 2 * I) + i * I + min(o0 + 16 * t, I - 16), 16, a.H);
+    const auto wl = W::raw_lane(lane, a.H);
+    const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
+    int q[NT];
+    uint32_t xl[NT][4];
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+        q[u] = choice(task, 16 * u + r);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int x = choice(task, 16 * u + 4 * i + g);
+            xl[u][i] = (uint32_t)(sh ? x - a.T * a.k : x / a.k) * (uint32_t)a.H * 2;
+        }
+    }
+    typename W::Raw fw[D][RT][2];
+    RowsBf16::Raw fx[D][NT];
+    char *const mx = m + RT * 2 * W::kTile;
+    auto load = [&](int d, int st) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) W::load_raw(fw[d][t][i], wt[t][i], wl, st, a.H);
+#pragma unroll
+        for (int u = 0; u < NT; u++) X::load_raw(fx[d][u], xb, xl[u], st, a.H);
+    };
+    mx_f32x4 acc[RT][2][NT] = {};
+    walk<D>((a.H + 127) / 128, load, [&](int d, int st) {
+#pragma unroll
+        for (int t = 0; t < RT * 2; t++) W::put(m + t * W::kTile, fw[d][t / 2][t % 2], lane);
+#pragma unroll
+        for (int u = 0; u < NT; u++) RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u], lane);
+        typename W::Frag f[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT * 2; t++) W::get(f[t / 2][t % 2], m + t * W::kTile, fw[d][t / 2][t % 2], lane);
+        fence();
+        load(d, st + D);
+        fence();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            mx_bf16x8 x[NT];
+#pragma unroll
+            for (int u = 0; u < NT; u++) x[u] = X::piece(mx + u * RowsBf16::kTile, j, lane);
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const mx_bf16x8 w = W::operand(f[t][i], j);
+#pragma unroll
+                    for (int u = 0; u < NT; u++) acc[t][i][u] = mfma16(w, x[u], acc[t][i][u]);
+                }
+        }
+        fence();
+    });
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+        if (16 * u + r >= task.n) continue;
+        uint16_t *h = a.h + h_at(a, q[u], sh);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int o = o0 + 16 * t + 4 * g;
+            if (o >= I) continue;
+            uint16_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split_h(silu(acc[t][0][u][i]) * acc[t][1][u][i], hi[i], lo[i]);
+            *reinterpret_cast<ushort4 *>(h + o) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<ushort4 *>(h + I + o) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+}
+
+template <class W, int RT, int NT>
+__global__ __launch_bounds__(64 * kStreamWaves, W::mx ? 3 : 2) void k_moe_up_stream(MoeArgs a, int nsh, int nper) {
+    constexpr int LDS = RT * 2 * W::kTile + NT * RowsBf16::kTile;
+    __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Task task = task_of(a, blockIdx.x, nsh, nper);
+    const int o0 = (task.part * kStreamWaves + wave) * 16 * RT;
+    if (task.n == 0 || o0 >= (task.e == a.E ? a.Is : a.I)) return;       // (no barrier in this kernel)
+    if (NT > 1 && task.n > 16) up_stream<W, RT, NT, 2>(a, task, o0, sm + wave * LDS, lane);
+    else up_stream<W, RT, 1, 2>(a, task, o0, sm + wave * LDS, lane);
+}
+
+// part[choice] = down h: 16 RT outputs a block, P blocks a wavefront in one walk.
+// h of the task's rows is brought to LDS once for all the workgroup's blocks.
+__host__ __device__ constexpr int down_pitch(int I) { return (I + 127) / 128 * 256; }     // bytes of a plane's row
+template <class W, int RT, int NT, int D>
+__device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, int b0, int nb, const char *h, char *m,
+                                            int lane) {
+    using X = XBf16<W>;
+    const int r = lane & 15, g = lane >> 4;
+    const bool sh = task.e == a.E;
+    const int I = sh ? a.Is : a.I, steps = (I + 127) / 128, pitch = down_pitch(I);
+    const auto wl = W::raw_lane(lane, I);
+    typename W::Raw fw[D][RT];
+    int lb = b0, ls = 0, mb = b0, ms = 0;  // row block and step to load, to multiply
+    auto load = [&](int d, int) {
+        const bool in = lb < b0 + nb;                    // (past the last: zeros)
+#pragma unroll
+        for (int t = 0; t < RT; t++)       // (a tile past H, not stored, repeats the last)
+            W::load_raw(fw[d][t],
+                        W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn,
+                                (sh ? 0 : (size_t)task.e * a.H) + min((in ? lb * RT + t : 0) * 16, a.H - 16), 16, I),
+                        wl, in ? ls : steps, I);
+        if (++ls == steps) {
+            ls = 0;
+            lb++;
+        }
+    };
+    mx_f32x4 acc[RT][NT] = {};
+#pragma unroll
+    for (int d = 0; d < D; d++) load(d, d);
+    fence();
+    __syncthreads();                       // h is in place
+    walk_on<D>(nb * steps, [&](int d, int st) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) W::put(m + t * W::kTile, fw[d][t], lane);
+        typename W::Frag f[RT];
+#pragma unroll
+        for (int t = 0; t < RT; t++) W::get(f[t], m + t * W::kTile, fw[d][t], lane);
+        fence();
+        load(d, st + D);
+        fence();
+        // (a step past the last, of zero weights, reads the last step's h)
+        const char *hs = h + r * 2 * pitch + min(ms, steps - 1) * 256;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            mx_bf16x8 hi[NT], lo[NT];
+#pragma unroll
+            for (int u = 0; u < NT; u++) {
+                const char *p = hs + u * 32 * pitch + ((X::piece_of(j, g) ^ r) << 4);
+                hi[u] = *reinterpret_cast<const mx_bf16x8 *>(p);
+                lo[u] = *reinterpret_cast<const mx_bf16x8 *>(p + pitch);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const mx_bf16x8 w = W::operand(f[t], j);
+#pragma unroll
+                for (int u = 0; u < NT; u++) {
+                    acc[t][u] = mfma16(w, hi[u], acc[t][u]);
+                    acc[t][u] = mfma16(w, lo[u], acc[t][u]);
+                }
             }
         }
-        if (c0 + r < n)
-            *reinterpret_cast<mx_f32x4 *>(a.part + (size_t)q * a.H + o0 + 4 * g) = acc;
+        fence();
+        if (++ms < steps) return;
+        ms = 0;
+#pragma unroll
+        for (int u = 0; u < NT; u++)
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const int o = (mb * RT + t) * 16;
+                if (16 * u + r < task.n && o < a.H && mb < b0 + nb)
+                    *reinterpret_cast<mx_f32x4 *>(a.part + (size_t)choice(task, 16 * u + r) * a.H + o + 4 * g) = acc[t][u];
+                acc[t][u] = mx_f32x4{};
+            }
+        mb++;
+    });
+}
+
+template <class W, int RT, int NT>
+__global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a, int nsh, int nper, int P) {
+    constexpr int LDS = RT * W::kTile;
+    __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS + NT * kDownH];
+    char *const h = sm + kStreamWaves * LDS;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Task task = task_of(a, blockIdx.x, nsh, nper);
+    if (task.n == 0) return;
+    const bool sh = task.e == a.E;
+    const int I = sh ? a.Is : a.I, pitch = down_pitch(I), pc = pitch / 16;
+    // 16-byte piece c of row i's plane p, at c ^ i within its 256 bytes; zeros past I
+    for (int e = threadIdx.x; e < task.n * 2 * pc; e += 64 * kStreamWaves) {
+        const int c = e % pc, i = e / pc / 2, p = e / pc % 2;
+        u32x4 v{};
+        if (c * 8 < I) v = *reinterpret_cast<const u32x4 *>(a.h + h_at(a, choice(task, i), sh) + p * I + c * 8);
+        *reinterpret_cast<u32x4 *>(h + (i * 2 + p) * pitch + ((c ^ (i & 15)) << 4)) = v;
     }
+    const int blocks = (a.H + 16 * RT - 1) / (16 * RT), b0 = (task.part * kStreamWaves + wave) * P;
+    const int nb = min(P, blocks - b0);
+    // (every wavefront comes to the one barrier)
+    if (NT > 1 && task.n > 16) down_stream<W, RT, NT, 2>(a, task, b0, nb, h, sm + wave * LDS, lane);
+    else down_stream<W, RT, 1, 2>(a, task, b0, nb, h, sm + wave * LDS, lane);
+}
+
+// y of up to kFewTokens tokens: 16 outputs a workgroup, the steps of 128 k of
+// every (token, expert) dealt to its 8 wavefronts. A step's product lands in
+// the token's column with the expert's weight; the columns of other tokens
+// (all multiplied with this token's h) are left out.
+template <class W>
+__global__ __launch_bounds__(512) void k_moe_down_few(MoeArgs a) {
+    __shared__ mx_f32x4 red[8][64];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int o0 = blockIdx.x * 16, n = a.T * a.k;
+    const int si = (a.I + 127) / 128, ss = (a.Is + 127) / 128;
+    const int units = n * si + (a.Is ? a.T * ss : 0);
+    constexpr int U = W::mx ? 4 : 2;
+    using X = XBf16<W>;
+    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
+    mx_f32x4 acc{};
+    for (int b = wave; b < units; b += 8 * U) {
+        typename W::Frag fw[U];
+        typename X::Frag fh[U], fl[U];
+        float p[U];
+        bool on[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const bool live = b + 8 * i < units;
+            const int u = live ? b + 8 * i : b;
+            const bool sh = u >= n * si;
+            const int q = sh ? n + (u - n * si) / ss : u / si;
+            const int st = sh ? (u - n * si) % ss : u % si, I = sh ? a.Is : a.I;
+            const int t = sh ? q - n : q / a.k;
+            const int e = __builtin_amdgcn_readfirstlane(sh ? 0 : a.ids[q]);
+            p[i] = a.wts[sh ? t * (a.k + 1) + a.k : t * (a.k + 1) + q % a.k];
+            on[i] = live && t == r;
+            const auto wt = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn, (size_t)e * a.H + o0, 16, I);
+            const uint32_t xl = X::lane(h_at(a, q, sh) * 2, g);
+            W::load(fw[i], wt, W::lane(lane, I), st, I);
+            X::load(fh[i], hb, xl, st, I);
+            X::load(fl[i], hb, xl + I * 2, st, I);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            mx_f32x4 d{};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const mx_bf16x8 wv = W::operand(fw[i], j);
+                d = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fh[i].v[j]), d);
+                d = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fl[i].v[j]), d);
+            }
+            if (on[i]) acc += d * p[i];
+        }
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave || r >= a.T) return;
+    acc = ((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane])) +
+          ((red[4][lane] + red[5][lane]) + (red[6][lane] + red[7][lane]));
+    *reinterpret_cast<ushort4 *>(a.y + (size_t)r * a.H + o0 + 4 * g) =
+        make_ushort4(f2bf(acc[0]), f2bf(acc[1]), f2bf(acc[2]), f2bf(acc[3]));
 }
 
 // y = rnd(sum over the choices, in order, then the shared expert)
@@ -324,17 +766,72 @@ __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a) {
     *reinterpret_cast<ushort4 *>(a.y + (size_t)t * a.H + c) = o;
 }
 
+// the launch of an expert kernel: nsh row parts of the shared expert per kGroup
+// tokens, nper of every slot
+struct Grid {
+    int nsh, nper;
+    unsigned n;
+};
+Grid grid_of(const MoeArgs &a, size_t slots, size_t nper, size_t nsh) {
+    if (!a.Is) nsh = 0;
+    return {(int)nsh, (int)nper, (unsigned)(nsh * cdiv(a.T, kGroup) + slots * nper)};
+}
+
+template <class W>
+int up_run(const MoeArgs &a, size_t slots) {
+    const Grid g = grid_of(a, slots, a.I / 16, a.Is / 16);
+    APUS_TIMED("k_moe_up", k_moe_up<W><<<g.n, 64 * kMoeWaves, 0, stream()>>>(a, g.nsh, g.nper));
+    return launch_check("k_moe_up");
+}
+template <class W>
+int down_run(const MoeArgs &a, size_t slots) {
+    const Grid g = grid_of(a, slots, cdiv(a.H, down_rows(a.I)), cdiv(a.H, down_rows(a.Is)));
+    APUS_TIMED("k_moe_down", k_moe_down<W><<<g.n, 64 * kMoeWaves, 0, stream()>>>(a, g.nsh, g.nper));
+    return launch_check("k_moe_down");
+}
+template <class W, int NT>
+int up_stream_run(const MoeArgs &a, size_t slots) {
+    const int rows = 16 * kStreamWaves;
+    const Grid g = grid_of(a, slots, cdiv(a.I, rows), cdiv(a.Is, rows));
+    APUS_TIMED("k_moe_up_stream",
+               k_moe_up_stream<W, 1, NT><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper));
+    return launch_check("k_moe_up_stream");
+}
+template <class W, int NT>
+int down_stream_run(const MoeArgs &a, size_t slots) {
+    // blocks of 32 outputs a wavefront, so that the launch keeps about 1024
+    // workgroups: more share a workgroup's copy of h
+    const size_t blocks = cdiv(a.H, 32 * kStreamWaves);
+    const int P = (int)std::max<size_t>(1, std::min<size_t>(4, slots * blocks / 1024));
+    const size_t nper = cdiv(blocks, P);
+    const Grid g = grid_of(a, slots, nper, nper);
+    APUS_TIMED("k_moe_down_stream",
+               k_moe_down_stream<W, 2, NT><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper, P));
+    return launch_check("k_moe_down_stream");
+}
+
+// The streaming forms from 1024 wavefronts on (4 a CU; hidden 2048, inter 512,
+// MXFP4, us for the layer split | streamed: 5 tokens 41 | 38, 16 tokens 76 | 57, 64
+// tokens 130 | 97). bf16 weights' up product is 4 times the bytes a step, which
+// the split form keeps on their way as well with few rows a slot (64 tokens 129 |
+// 136 us, 325 tokens 245 | 190).
 template <class W>
 int experts_run(const MoeArgs &a) {
-    const size_t slots = (size_t)std::min(a.T * a.k, a.E);
-    {
-        const int nsh = a.Is / 16, nper = a.I / 16;
-        APUS_TIMED("k_moe_up", k_moe_up<W><<<(unsigned)(nsh + slots * nper), 256, 0, stream()>>>(a, nsh, nper));
-        APUS_LAUNCHED("k_moe_up");
+    const size_t slots = a.nslots;
+    const bool one = a.T <= 16;            // no slot has more than 16 rows
+    const bool ups = slots * a.I / 16 >= 1024 && (W::mx || a.T * a.k >= 4 * a.E);
+    if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, 2>(a, slots))
+        return r;
+    if (a.T <= kFewTokens) {
+        APUS_TIMED("k_moe_down_few", k_moe_down_few<W><<<(unsigned)a.H / 16, 512, 0, stream()>>>(a));
+        return launch_check("k_moe_down_few");
     }
-    const int nper = (int)cdiv(a.H, 64), nsh = a.Is ? nper : 0;
-    APUS_TIMED("k_moe_down", k_moe_down<W><<<(unsigned)(nsh + slots * nper), 256, 0, stream()>>>(a, nsh, nper));
-    return launch_check("k_moe_down");
+    const bool downs = slots * a.H / 32 >= 1024 && 32 * down_pitch(std::max(a.I, a.Is)) <= kDownH;
+    if (int r = !downs ? down_run<W>(a, slots) : one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, 2>(a, slots))
+        return r;
+    APUS_TIMED("k_moe_combine",
+               k_moe_combine<<<cdiv((size_t)a.T * (a.H / 4), 256), 256, 0, stream()>>>(a));
+    return launch_check("k_moe_combine");
 }
 
 int check_layer(const ApusHipMoeLayer *L) {
@@ -378,6 +875,9 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
     if (!max_tokens || max_tokens > kMoeMaxTokens)
         return set_error(kErrUnsupported, "a mixture-of-experts call takes 1 .. %zu tokens (%zu)",
                          kMoeMaxTokens, max_tokens);
+    const size_t hs = max_tokens * (L->topk * L->inter + L->shared_inter) * 4;
+    if (hs > 0x7fff0000u || max_tokens * L->hidden * 2 > 0x7fff0000u)
+        return set_error(kErrUnsupported, "mixture-of-experts intermediates of up to 2 GiB");
     if (int r = mx_ready()) return r;
     auto *w = new ApusHipMoeWork{max_tokens, L->hidden, L->inter, L->experts, L->topk, L->shared_inter};
     const size_t T = max_tokens, k = L->topk;
@@ -388,12 +888,22 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
         return at;
     };
     const size_t logits = take(T * (L->experts + 1) * 4), ids = take(T * k * 4),
-                 wts = take(T * (k + 1) * 4), h = take(T * (k * L->inter + L->shared_inter) * 4),
-                 part = take(T * (k + 1) * L->hidden * 4);
+                 wts = take(T * (k + 1) * 4), 
+                 h = take(hs),
+                 part = take(T * (k + 1) * L->hidden * 4), done = take(((T + 15) / 16 + 1) * 4),
+                 slots = take(moe_slots(T, k, L->experts) * 16), list = take(T * k * 2);
     if (hipMalloc((void **)&w->base, n) != hipSuccess) {
         delete w;
         return set_error(kErrHip, "hipMalloc of %zu bytes failed", n);
     }
+    if (hipMemset(w->base + done, 0, ((T + 15) / 16 + 1) * 4) != hipSuccess) {
+        (void)hipFree(w->base);
+        delete w;
+        return set_error(kErrHip, "clearing the workspace failed");
+    }
+    w->done = (uint32_t *)(w->base + done);
+    w->slots = (int4 *)(w->base + slots);
+    w->list = (uint16_t *)(w->base + list);
     w->logits = (float *)(w->base + logits);
     w->ids = (int32_t *)(w->base + ids);
     w->wts = (float *)(w->base + wts);
@@ -448,6 +958,9 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.wts = w->wts;
     a.part = w->part;
     a.ids = w->ids;
+    a.done = w->done;
+    a.slots = w->slots;
+    a.list = w->list;
     a.h = w->h;
     a.T = (int)T;
     a.H = (int)L->hidden;
@@ -456,14 +969,12 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.k = (int)L->topk;
     a.Is = (int)L->shared_inter;
     a.norm = L->norm_topk;
-    const dim3 rg(cdiv(L->experts + (a.w_sgate ? 1 : 0), 16), cdiv(T, 16));
-    APUS_TIMED("k_moe_router", k_moe_router<<<rg, 256, 0, stream()>>>(a));
+    a.nslots = (int)(T <= kFewTokens ? T * L->topk : moe_slots(T, L->topk, L->experts));
+    const dim3 rg(cdiv(L->experts, 16) + (a.w_sgate ? 1 : 0), cdiv(T, 16));
+    APUS_TIMED("k_moe_router", if (a.E <= 256) k_moe_router<4><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
+               else k_moe_router<16><<<rg, 64 * kRouterWaves, 0, stream()>>>(a));
     APUS_LAUNCHED("k_moe_router");
-    APUS_TIMED("k_moe_topk", k_moe_topk<<<cdiv(T, 4), 256, 0, stream()>>>(a));
-    APUS_LAUNCHED("k_moe_topk");
-    if (int r = L->mxfp4 ? experts_run<WMx>(a) : experts_run<WBf16>(a)) return r;
-    APUS_TIMED("k_moe_combine", k_moe_combine<<<cdiv(T * (L->hidden / 4), 256), 256, 0, stream()>>>(a));
-    return launch_check("k_moe_combine");
+    return L->mxfp4 ? experts_run<WMx>(a) : experts_run<WBf16>(a);
 }
 
 }  // extern "C"

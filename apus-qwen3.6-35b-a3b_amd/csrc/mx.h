@@ -9,6 +9,13 @@ namespace apus {
 int mx_check_dims(size_t M, size_t O, size_t K);   // sizes under 2^31, K in whole blocks
 int mx_ready();                                    // ensure_ready, on the calling thread's device
 
+// products for many rows (mx_wide.hip): tiles of 128 x 128 (shape 2) or 256 x 256
+// (shape 4)
+int mx_gemm_wide(const uint8_t *w, const uint8_t *ws, const uint8_t *x, const uint8_t *xs,
+                 uint16_t *y, size_t ldy, int M, int O, int K, int shape);
+int mx_gemm_wide16(const uint8_t *w, const uint8_t *ws, const uint16_t *x, size_t ldx, uint16_t *y,
+                   size_t ldy, int M, int O, int K, int shape);
+
 }  // namespace apus
 
 #define APUS_ENABLED()                                                       \

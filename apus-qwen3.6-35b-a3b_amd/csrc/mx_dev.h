@@ -34,85 +34,181 @@ __device__ __forceinline__ mx_bf16x8 mx_widen(uint32_t c, uint32_t s) {
     return mx_bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
-// A wavefront's operands of one step of 128 k. Lane l serves row l % 16 (of
-// the weights, or of the activations), k group g = l / 16. Both operands of a
-// product assign k to (lane group, MFMA) in the same way, and any way will do:
-// MXFP4 weights give lane group g the whole 32-element block g (16 bytes and
-// its scale), MFMA j its codes 8 j ..; bf16 weights give MFMA j the 32 k from
-// 32 j, group g 8 of them, so that the 4 lanes of a row read 64 bytes in one
-// piece. live: this lane's k of the step lie inside K (K is a multiple of 32);
-// outside, both operands are zero.
+// Loads through a buffer resource: the address is a base and size in scalar
+// registers, a lane's offset and a uniform one, so that a tile's 16 rows take
+// one address register (as 64-bit pointers the loops' addresses did not fit the
+// registers), and an offset past the size reads zero (the uniform offset stays
+// under the size: the check subtracts it).
+__device__ f32x4_t llvm_raw_buffer_load_v4f32(i32x4 r, int voff, int soff, int aux)
+    __asm("llvm.amdgcn.raw.buffer.load.v4f32");
+__device__ uint8_t llvm_raw_buffer_load_u8(i32x4 r, int voff, int soff, int aux)
+    __asm("llvm.amdgcn.raw.buffer.load.i8");
+constexpr uint32_t kPast = 0x7fffffff;       // an offset past every tile
+__device__ __forceinline__ u32x4 ld16(i32x4 r, uint32_t off, int at) {
+    return __builtin_bit_cast(u32x4, llvm_raw_buffer_load_v4f32(r, (int)off, at, 0));
+}
+
+// A wavefront's operands of one step of 128 k for the 16-wide MFMAs. Lane l
+// serves row l % 16 (of the weights, or of the activations), k group g = l / 16.
+// Both operands of a product assign k to (lane group, MFMA) in the same way, and
+// any way will do: MXFP4 weights give lane group g the whole 32-element block g
+// (16 bytes and its scale), MFMA j its codes 8 j ..; bf16 weights give MFMA j the
+// 32 k from 32 j, group g 8 of them. What lies past K (a multiple of 32) reads as
+// zero, in both operands.
+//
+// Two ways from memory to these operands. load: each lane loads its own (Frag).
+// Neighbouring lanes then read different rows, and the address unit takes such a
+// load a lane at a time, about 60 clocks instead of 16: for calls that wait for
+// latency, not for it. load_raw, put, get: lanes load along the rows (Raw), write
+// what they got to LDS of the wavefront's own and read the operands from there.
+// The LDS places are permuted so that neither side's lanes share banks.
+
+// 16 rows of a step of 128 bf16 values: load i has rows 4 i .., 16 lanes a row
+struct RowsBf16 {
+    static constexpr int kTile = 4096;       // LDS bytes
+    struct Raw {
+        u32x4 v[4];
+    };
+    static __device__ __forceinline__ void put(char *m, const Raw &f, int l) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 4 * i + (l >> 4);
+            *reinterpret_cast<u32x4 *>(m + row * 256 + (((l & 15) ^ row) << 4)) = f.v[i];
+        }
+    }
+    // 16-byte piece c of this lane's row
+    static __device__ __forceinline__ u32x4 piece(const char *m, int c, int l) {
+        return *reinterpret_cast<const u32x4 *>(m + (l & 15) * 256 + ((c ^ (l & 15)) << 4));
+    }
+};
+
 struct WBf16 {
     static constexpr bool mx = false;
-    struct Row {
-        const char *p;
+    static constexpr int kTile = RowsBf16::kTile;
+    struct Tile {
+        i32x4 w;
+    };
+    struct Lane {
+        uint32_t off;
     };
     struct Frag {
         u32x4 v[4];
     };
-    static __device__ __forceinline__ Row row(const void *w, const uint8_t *, size_t r, int K, int g) {
-        return {(const char *)w + r * (size_t)K * 2 + g * 16};
+    typedef RowsBf16::Raw Raw;
+    // up to 16 rows from r0 (uniform) of w [][K]; rows past them read as zero
+    static __device__ __forceinline__ Tile tile(const void *w, const uint8_t *, size_t r0, int rows, int K) {
+        return {dma_rsrc((const char *)w + r0 * (size_t)K * 2, (uint32_t)rows * (uint32_t)K * 2)};
     }
-    static __device__ __forceinline__ void load(Frag &f, const Row &r, int k, int K) {
+    static __device__ __forceinline__ Lane lane(int l, int K) {
+        return {(uint32_t)(l & 15) * (uint32_t)K * 2 + (l >> 4) * 16};
+    }
+    static __device__ __forceinline__ void load(Frag &f, const Tile &t, const Lane &l, int step, int K) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const bool live = k + 32 * j < K;
-            f.v[j] = *reinterpret_cast<const u32x4 *>(r.p + (size_t)(live ? k + 32 * j : 0) * 2);
-            if (!live) f.v[j] = u32x4{};
+            const int k = step * 128 + 32 * j;
+            f.v[j] = ld16(t.w, k < K ? l.off : kPast, k < K ? k * 2 : 0);
         }
     }
     static __device__ __forceinline__ mx_bf16x8 operand(const Frag &f, int j) {
         return __builtin_bit_cast(mx_bf16x8, f.v[j]);
     }
+    static __device__ __forceinline__ Lane raw_lane(int l, int K) {
+        return {(uint32_t)(l >> 4) * (uint32_t)K * 2 + (l & 15) * 16};
+    }
+    static __device__ __forceinline__ void load_raw(Raw &f, const Tile &t, const Lane &l, int step, int K) {
+        const int k = step * 128;
+        const bool live = k + 8 * (int)(threadIdx.x & 15) < K;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            f.v[i] = ld16(t.w, live ? l.off + 8 * i * (uint32_t)K : kPast, k < K ? k * 2 : 0);
+    }
+    static __device__ __forceinline__ void put(char *m, const Raw &f, int l) { RowsBf16::put(m, f, l); }
+    static __device__ __forceinline__ void get(Frag &f, const char *m, const Raw &, int l) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) f.v[j] = RowsBf16::piece(m, 4 * j + (l >> 4), l);
+    }
 };
 struct WMx {
     static constexpr bool mx = true;
-    struct Row {
-        const uint8_t *p, *s;
+    static constexpr int kTile = 1024;
+    struct Tile {
+        i32x4 w, s;
+    };
+    struct Lane {
+        uint32_t off, soff;
     };
     struct Frag {
         u32x4 v;
         uint32_t s;
     };
-    static __device__ __forceinline__ Row row(const void *w, const uint8_t *ws, size_t r, int K, int g) {
-        return {(const uint8_t *)w + r * (size_t)(K / 2) + g * 16, ws + r * (size_t)(K / kMxBlock)};
+    typedef Frag Raw;
+    static __device__ __forceinline__ Tile tile(const void *w, const uint8_t *ws, size_t r0, int rows, int K) {
+        return {dma_rsrc((const uint8_t *)w + r0 * (size_t)(K / 2), (uint32_t)rows * (uint32_t)(K / 2)),
+                dma_rsrc(ws + r0 * (size_t)(K / kMxBlock), (uint32_t)rows * (uint32_t)(K / kMxBlock))};
     }
-    static __device__ __forceinline__ void load(Frag &f, const Row &r, int k, int K) {
-        const int g = (threadIdx.x >> 4) & 3;
-        const bool live = k + 32 * g < K;
-        f.v = *reinterpret_cast<const u32x4 *>(r.p + (live ? k / 2 : -16 * g));
-        f.s = r.s[live ? k / kMxBlock + g : 0];
-        if (!live) {
-            f.v = u32x4{};
-            f.s = 127;
-        }
+    static __device__ __forceinline__ Lane at(int row, int block, int K) {
+        return {(uint32_t)row * (uint32_t)(K / 2) + block * 16, (uint32_t)row * (uint32_t)(K / kMxBlock) + block};
+    }
+    static __device__ __forceinline__ Lane lane(int l, int K) { return at(l & 15, l >> 4, K); }
+    // block: this lane's of the step (past K: zero codes, at the scale 2^-127)
+    static __device__ __forceinline__ void load_block(Frag &f, const Tile &t, const Lane &l, int step, int block, int K) {
+        const int k = step * 128;
+        const bool live = k + 32 * block < K;
+        f.v = ld16(t.w, live ? l.off : kPast, k < K ? k / 2 : 0);
+        f.s = llvm_raw_buffer_load_u8(t.s, (int)(live ? l.soff : kPast), k < K ? k / kMxBlock : 0, 0);
+    }
+    static __device__ __forceinline__ void load(Frag &f, const Tile &t, const Lane &l, int step, int K) {
+        load_block(f, t, l, step, (threadIdx.x >> 4) & 3, K);
     }
     static __device__ __forceinline__ mx_bf16x8 operand(const Frag &f, int j) {
         return mx_widen(f.v[j], f.s);
     }
+    // 4 lanes a row; the scales go between lanes without LDS memory
+    static __device__ __forceinline__ Lane raw_lane(int l, int K) { return at(l >> 2, l & 3, K); }
+    static __device__ __forceinline__ void load_raw(Raw &f, const Tile &t, const Lane &l, int step, int K) {
+        load_block(f, t, l, step, threadIdx.x & 3, K);
+    }
+    static __device__ __forceinline__ void put(char *m, const Raw &f, int l) {
+        const int row = l >> 2;
+        *reinterpret_cast<u32x4 *>(m + row * 64 + (((l & 3) ^ (row >> 2)) << 4)) = f.v;
+    }
+    static __device__ __forceinline__ void get(Frag &f, const char *m, const Raw &raw, int l) {
+        const int r = l & 15, g = l >> 4;
+        f.v = *reinterpret_cast<const u32x4 *>(m + r * 64 + ((g ^ (r >> 2)) << 4));
+        f.s = (uint32_t)__builtin_amdgcn_ds_bpermute((r * 4 + g) * 4, (int)raw.s);
+    }
 };
 
-// bf16 activations for weights of kind W
+// bf16 activations for weights of kind W: the row at byte `off` of a buffer
 template <class W>
 struct XBf16 {
-    struct Row {
-        const char *p;
-    };
     struct Frag {
         u32x4 v[4];
     };
-    static __device__ __forceinline__ Row row(const uint16_t *x, size_t ld, size_t r, int g) {
-        return {(const char *)(x + r * ld + (W::mx ? 32 * g : 8 * g))};
-    }
-    static __device__ __forceinline__ void load(Frag &f, const Row &r, int k, int K) {
-        const int g = (threadIdx.x >> 4) & 3;
+    static __device__ __forceinline__ uint32_t lane(uint32_t off, int g) { return off + (W::mx ? 64 * g : 16 * g); }
+    static __device__ __forceinline__ void load(Frag &f, i32x4 x, uint32_t l, int step, int K) {
+        const int g = (threadIdx.x >> 4) & 3, k = step * 128;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const bool live = W::mx ? k + 32 * g < K : k + 32 * j < K;
-            const int off = W::mx ? (live ? k : -32 * g) + 8 * j : (live ? k + 32 * j : 0);
-            f.v[j] = *reinterpret_cast<const u32x4 *>(r.p + (ptrdiff_t)off * 2);
-            if (!live) f.v[j] = u32x4{};
+            const bool in = W::mx ? k < K : k + 32 * j < K;                  // (uniform)
+            const bool live = W::mx ? k + 32 * g < K : in;
+            f.v[j] = ld16(x, live ? l : kPast, in ? 2 * k + (W::mx ? 16 : 64) * j : 0);
         }
+    }
+    // rows[i]: byte offsets of the rows 4 i + lane / 16; loads past the first XR are
+    // of rows that are not there
+    template <int XR = 4>
+    static __device__ __forceinline__ void load_raw(RowsBf16::Raw &f, i32x4 x, const uint32_t (&rows)[4], int step, int K) {
+        const int c = threadIdx.x & 15, k = step * 128;
+        const bool live = k + 8 * c < K;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            f.v[i] = i < XR ? ld16(x, live ? rows[i] + 16 * c : kPast, k < K ? 2 * k : 0) : u32x4{};
+    }
+    // the 16-byte piece of a step that lane group g takes to MFMA j
+    static __device__ __forceinline__ int piece_of(int j, int g) { return W::mx ? 4 * g + j : 4 * j + g; }
+    static __device__ __forceinline__ mx_bf16x8 piece(const char *m, int j, int l) {
+        return __builtin_bit_cast(mx_bf16x8, RowsBf16::piece(m, piece_of(j, l >> 4), l));
     }
 };
 

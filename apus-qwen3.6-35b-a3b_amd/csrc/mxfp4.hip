@@ -74,49 +74,119 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict
 }
 
 // ---- products of few rows --------------------------------------------------
-// A workgroup forms 16 outputs x 16 rows; its 4 wavefronts take every fourth
-// step of 128 k, and their partial sums meet in LDS.
-template <bool XMX>
-__global__ __launch_bounds__(256) void k_mx_gemm_few(const uint8_t *__restrict__ w,
-                                                     const uint8_t *__restrict__ ws,
-                                                     const void *__restrict__ x,
-                                                     const uint8_t *__restrict__ xs, size_t ldx,
-                                                     uint16_t *__restrict__ y, size_t ldy, int M,
-                                                     int O, int K, int nbo) {
-    __shared__ mx_f32x4 red[4][64];
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+// A workgroup forms 16 RT outputs x 16 NT rows; its 8 wavefronts take every
+// eighth pair of steps of 128 k, all their loads on the way before the first is
+// used, and their partial sums meet in LDS. Rows come along their length and
+// become operands in LDS of the wavefront's own (mx_dev.h). XR: the loads of four
+// rows that a tile of bf16 activations has (1 for up to 4 rows).
+constexpr int kFewWaves = 8;
+
+template <bool XMX, int RT, int NT, int XR>
+__global__ __launch_bounds__(64 * kFewWaves) void k_mx_gemm_few(const uint8_t *__restrict__ w,
+                                                                const uint8_t *__restrict__ ws,
+                                                                const void *__restrict__ x,
+                                                                const uint8_t *__restrict__ xs, size_t ldx,
+                                                                uint16_t *__restrict__ y, size_t ldy, int M,
+                                                                int O, int K, int nbo) {
+    constexpr int S = !XMX && NT > 2 ? 1 : 2;            // steps in flight (registers)
+    constexpr int XT = XMX ? WMx::kTile : RowsBf16::kTile;
+    constexpr int PART = RT * 1024 + XT > RT * NT * 1024 ? RT * 1024 + XT : RT * NT * 1024;
+    __shared__ __attribute__((aligned(16))) char sm[kFewWaves * PART];
+    using X = XBf16<WMx>;
+    const int lane = threadIdx.x & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int o0 = (blockIdx.x % nbo) * 16, m0 = (blockIdx.x / nbo) * 16;
-    // (outputs past O and rows past M repeat the last one; they are not stored)
-    const auto wr = WMx::row(w, ws, (size_t)min(o0 + r, O - 1), K, g);
-    const size_t m = (size_t)min(m0 + r, M - 1);
-    mx_f32x4 acc{};
-    for (int k = wave * 128; k < K; k += 512) {
-        WMx::Frag wf;
-        WMx::load(wf, wr, k, K);
-        if constexpr (XMX) {
-            const auto xr = WMx::row(x, xs, m, K, g);
-            WMx::Frag xf;
-            WMx::load(xf, xr, k, K);
-            acc = mfma16_mx(wf, xf, acc);
-        } else {
-            const auto xr = XBf16<WMx>::row((const uint16_t *)x, ldx, m, g);
-            XBf16<WMx>::Frag xf;
-            XBf16<WMx>::load(xf, xr, k, K);
+    const int o0 = (blockIdx.x % nbo) * 16 * RT, m0 = (blockIdx.x / nbo) * 16 * NT;
+    char *const mine = sm + wave * PART, *const mx = mine + RT * 1024;
+    // (outputs past O and rows past M read as zero, and are not stored)
+    WMx::Tile wt[RT], xt[NT];
+    i32x4 xb[NT];
+    uint32_t xl[NT][4];
+    const uint32_t pitch = (uint32_t)ldx * 2;
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                acc = mfma16(WMx::operand(wf, j), __builtin_bit_cast(mx_bf16x8, xf.v[j]), acc);
+    for (int t = 0; t < RT; t++)
+        wt[t] = WMx::tile(w, ws, min(o0 + 16 * t, O - 1), max(0, min(16, O - o0 - 16 * t)), K);
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+        const int m = min(m0 + 16 * u, M - 1), rows = max(0, min(16, M - m0 - 16 * u));
+        if constexpr (XMX) {
+            xt[u] = WMx::tile(x, xs, m, rows, K);
+        } else {
+            xb[u] = dma_rsrc((const uint16_t *)x + (size_t)m * ldx, rows ? (rows - 1) * pitch + K * 2 : 0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) xl[u][i] = 4 * i + g < rows ? (4 * i + g) * pitch : kPast - 256;
         }
     }
-    red[wave][lane] = acc;
-    __syncthreads();
-    if (wave) return;
-    acc = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    if (m0 + r >= M) return;
+    const auto wl = WMx::raw_lane(lane, K);
+    const int steps = (K + 127) / 128;
+    mx_f32x4 acc[RT][NT] = {};
+    for (int st = wave * 2; st < steps; st += st & 1 || S == 2 ? kFewWaves * 2 - (S == 1) : 1) {
+        WMx::Raw fw[S][RT], fq[S][NT];
+        RowsBf16::Raw fx[S][NT];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int o = o0 + 4 * g + i;
-        if (o < O) y[(size_t)(m0 + r) * ldy + o] = f2bf(acc[i]);
+        for (int s = 0; s < S; s++) {
+#pragma unroll
+            for (int t = 0; t < RT; t++) WMx::load_raw(fw[s][t], wt[t], wl, st + s, K);
+#pragma unroll
+            for (int u = 0; u < NT; u++) {
+                if constexpr (XMX) WMx::load_raw(fq[s][u], xt[u], wl, st + s, K);
+                else X::load_raw<XR>(fx[s][u], xb[u], xl[u], st + s, K);
+            }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            WMx::Frag f[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                WMx::put(mine + t * 1024, fw[s][t], lane);
+                WMx::get(f[t], mine + t * 1024, fw[s][t], lane);
+            }
+#pragma unroll
+            for (int u = 0; u < NT; u++) {
+                if constexpr (XMX) {
+                    WMx::Frag q;
+                    WMx::put(mx, fq[s][u], lane);
+                    WMx::get(q, mx, fq[s][u], lane);
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[t][u] = mfma16_mx(f[t], q, acc[t][u]);
+                } else {
+                    RowsBf16::put(mx, fx[s][u], lane);
+                    mx_bf16x8 v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] = X::piece(mx, j, lane);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int t = 0; t < RT; t++)
+                            acc[t][u] = mfma16(WMx::operand(f[t], j), v[j], acc[t][u]);
+                }
+            }
+        }
+    }
+    // [wave][row tile][tile]
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int u = 0; u < NT; u++) *reinterpret_cast<mx_f32x4 *>(mine + (t * NT + u) * 1024 + lane * 16) = acc[t][u];
+    __syncthreads();
+    // a thread finishes 4 outputs of a row, a row's outputs side by side
+    const bool vec = ((ldy | (size_t)O) & 3) == 0 && ((uintptr_t)y & 7) == 0;
+    for (int e = threadIdx.x; e < RT * NT * 64; e += 64 * kFewWaves) {
+        const int q = e % (4 * RT), r = e / (4 * RT), o = o0 + 4 * q, m = m0 + r;
+        if (m >= M || o >= O) continue;
+        const char *p = sm + (q / 4 * NT + r / 16) * 1024 + (q % 4 * 16 + r % 16) * 16;
+        mx_f32x4 s = *reinterpret_cast<const mx_f32x4 *>(p);
+#pragma unroll
+        for (int v = 1; v < kFewWaves; v++) s += *reinterpret_cast<const mx_f32x4 *>(p + v * PART);
+        uint16_t *yo = y + (size_t)m * ldy + o;
+        if (vec) {
+            *reinterpret_cast<ushort4 *>(yo) = make_ushort4(f2bf(s[0]), f2bf(s[1]), f2bf(s[2]), f2bf(s[3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (o + i < O) yo[i] = f2bf(s[i]);
+        }
     }
 }
 
@@ -130,6 +200,9 @@ __global__ __launch_bounds__(256) void k_mx_zero_rows(uint16_t *__restrict__ y, 
 unsigned stream_grid(size_t threads) {
     return (unsigned)std::min<size_t>((threads + 255) / 256, (size_t)cu_count() * 32);
 }
+
+// 32-bit offsets reach 256 rows of activations or codes
+constexpr size_t kMxMaxPitch = (size_t)1 << 21;
 
 // Two sets of M rows (first row, bytes between rows, bytes of a row) share
 // bytes. Rows of one pitch may interleave (column slices of one buffer);
@@ -164,10 +237,63 @@ int gemm_check(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t
         if ((uintptr_t)x % 16 || ldx % 8)
             return set_error(kErrUnsupported, "activation rows need 16-byte alignment (pitch %zu)", ldx);
         if (ldx < K) return set_error(kErrArgument, "rows of %zu elements with pitch %zu", K, ldx);
+        if (ldx > kMxMaxPitch) return set_error(kErrUnsupported, "rows of pitch %zu", ldx);
         if (rows_overlap(x, ldx * 2, K * 2, y, ldy * 2, O * 2, M))
             return set_error(kErrArgument, "the output overlaps the activations");
     }
     return kOk;
+}
+
+template <bool XMX, int RT, int NT, int XR>
+int few_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *xs, size_t ldx,
+            uint16_t *y, size_t ldy, size_t M, size_t O, size_t K) {
+    const size_t nbo = cdiv(O, 16 * RT), n = nbo * cdiv(M, 16 * NT);
+    if (n > 0x7fffffffu) return set_error(kErrUnsupported, "MXFP4 gemm too large");
+    APUS_TIMED("k_mx_gemm_few", k_mx_gemm_few<XMX, RT, NT, XR><<<(unsigned)n, 64 * kFewWaves, 0, stream()>>>(
+                                    w, ws, x, xs, ldx, y, ldy, (int)M, (int)O, (int)K, (int)nbo));
+    return launch_check("k_mx_gemm_few");
+}
+
+// Estimated times in us of the product's forms, from what they take over 512 ..
+// 12352 outputs x 48 .. 1024 rows and K = 2048, 4096 (within 15 % nearly all over
+// that range). What a form takes goes by the workgroups of the busiest CU and, but
+// for a fixed part, by K.
+struct FewCost {
+    float fixed, one, two;                  // one, two: tiles of 16 and 32 outputs x 64 rows
+};
+constexpr FewCost kFewCost[] = {{2.5f, 3.6f, 5.6f}, {2.6f, 1.3f, 2.0f}};         // bf16, MXFP4 activations
+struct WideCost {
+    float f1, k1, f2, k2;                   // 128 x 128 tiles: one on the busiest CU, two
+    float f4, k4, fill;                     // 256 x 256: per round; with every CU busy
+};
+constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 7.0f, 43.0f, 16.0f},
+                                  {3.2f, 4.8f, 4.0f, 10.0f, 6.5f, 10.5f, 12.0f}};
+
+size_t rounds(size_t n) { return (n + cu_count() - 1) / cu_count(); }
+
+// 32 outputs a workgroup instead of 16? (few rows: from two workgroups a CU on.)
+template <bool XMX>
+bool few_pays_two(size_t n2, size_t n1, size_t M) {
+    if (M <= 32) return n1 >= 2 * (size_t)cu_count();
+    const FewCost &c = kFewCost[XMX];
+    return c.two * rounds(n2) < c.one * rounds(n1);
+}
+
+// The tile shape of the many-row kernel to take, or 0: the few-row one.
+template <bool XMX>
+int wide_shape(size_t M, size_t O, size_t K) {
+    const float kk = (float)K / 2048.0f;
+    const FewCost &c = kFewCost[XMX];
+    const WideCost &v = kWideCost[XMX];
+    const size_t nbm = cdiv(M, 64);
+    const float few = c.fixed + kk * std::min(c.one * rounds(cdiv(O, 16) * nbm), c.two * rounds(cdiv(O, 32) * nbm));
+    const size_t r2 = rounds((size_t)cdiv(O, 128) * cdiv(M, 128));
+    const float w2 = (r2 / 2) * (v.f2 + v.k2 * kk) + (r2 % 2) * (v.f1 + v.k1 * kk);
+    const size_t n4 = (size_t)cdiv(O, 256) * cdiv(M, 256), r4 = rounds(n4);
+    const float w4 = r4 * (v.f4 + v.k4 * kk) +
+                     v.fill * std::min((float)r4, (float)n4 / cu_count());
+    if (few <= w2 && few <= w4) return 0;
+    return w2 <= w4 ? 2 : 4;
 }
 
 template <bool XMX>
@@ -178,11 +304,26 @@ int gemm_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *
         k_mx_zero_rows<<<stream_grid(M * O), 256, 0, stream()>>>(y, ldy, O, M * O);
         return launch_check("k_mx_zero_rows");
     }
-    const unsigned nbo = cdiv(O, 16), nbm = cdiv(M, 16);
-    if ((size_t)nbo * nbm > 0x7fffffffu) return set_error(kErrUnsupported, "MXFP4 gemm too large");
-    APUS_TIMED("k_mx_gemm_few", k_mx_gemm_few<XMX><<<nbo * nbm, 256, 0, stream()>>>(
-                                    w, ws, x, xs, ldx, y, ldy, (int)M, (int)O, (int)K, (int)nbo));
-    return launch_check("k_mx_gemm_few");
+    if (M > 32) {
+        const int shape = wide_shape<XMX>(M, O, K);
+        if constexpr (XMX) {
+            if (shape) return mx_gemm_wide(w, ws, (const uint8_t *)x, xs, y, ldy, (int)M, (int)O, (int)K, shape);
+        } else {
+            if (shape) return mx_gemm_wide16(w, ws, (const uint16_t *)x, ldx, y, ldy, (int)M, (int)O, (int)K, shape);
+        }
+    }
+    const size_t tiles = cdiv(M, 16), nt = cdiv(tiles, cdiv(tiles, 4)), nbm = cdiv(tiles, nt);
+    const bool two = few_pays_two<XMX>(cdiv(O, 32) * nbm, cdiv(O, 16) * nbm, M);
+#define FEW(NT, XR)                                                                          \
+    two ? few_run<XMX, 2, NT, XR>(w, ws, x, xs, ldx, y, ldy, M, O, K)                        \
+        : few_run<XMX, 1, NT, XR>(w, ws, x, xs, ldx, y, ldy, M, O, K)
+    switch (nt) {
+        case 1: return M <= 4 ? FEW(1, 1) : FEW(1, 4);
+        case 2: return FEW(2, 4);
+        case 3: return FEW(3, 4);
+        default: return FEW(4, 4);
+    }
+#undef FEW
 }
 
 }  // namespace
@@ -190,8 +331,8 @@ int gemm_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *
 namespace apus {
 
 int mx_check_dims(size_t M, size_t O, size_t K) {
-    if (M > 0x7fffffffu || O > 0x7fffffffu || K > 0x7fffffffu)
-        return set_error(kErrUnsupported, "MXFP4 dims past 2^31");
+    if (M > 0x7fffffffu || O > 0x7fffffffu || K > kMxMaxPitch)
+        return set_error(kErrUnsupported, "MXFP4 dims past 2^31, or rows past 2^21 elements");
     if (K % kMxBlock)
         return set_error(kErrUnsupported, "MXFP4 rows come in blocks of %d (K=%zu)", kMxBlock, K);
     return kOk;

@@ -126,11 +126,15 @@ def moe(x, w, topk, norm, mx):
 
 
 def check(got, ref, bound, what=""):
-    """Every element of a bf16 tensor within its bound; prints the worst."""
+    """Every element of a bf16 tensor within its bound, and the tensor within
+    what the one rounding allows: 2^-8 of its norm, and 2^-12 for the sums,
+    whose errors do not all point one way as the elements' bounds have it."""
     d = (got.double() - ref).abs()
     r = float((d / bound).max()) if d.numel() else 0.0
-    print(f"[mx] {what}: worst error {r:.3f} of its bound", flush=True)
+    n = float(d.norm() / ref.norm().clamp_min(1e-300)) if d.numel() else 0.0
+    print(f"[mx] {what}: worst error {r:.3f} of its bound, normwise {n:.2e}", flush=True)
     assert bool((d <= bound).all()), f"{what}: {r} of the bound"
+    assert n <= UBF + 2.0 ** -12, f"{what}: normwise {n}"
 
 
 def normal(gen, *shape, scale=1.0, device="cuda"):

@@ -213,3 +213,23 @@ def test_moe_refusals(hip):
     with pytest.raises(hip.ApusHipError) as e:             # no workspace any more
         hip.moe_layer_decode(L, work, x[:1], torch.empty_like(x[:1]))
     assert e.value.code == 3
+
+
+# the forms that rules on sizes choose between: slots and row blocks on either
+# side of the streaming kernels' thresholds, inner sizes past what they hold,
+# several rounds of K, slots of more than 16 and several slots of one expert
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("T,H,I,E,topk,Is", [(5, 2048, 512, 40, 8, 512), (8, 1056, 544, 64, 8, 96),
+                                             (20, 4128, 96, 32, 6, 64), (100, 544, 512, 24, 8, 544),
+                                             (200, 2080, 160, 12, 4, 32), (300, 256, 1056, 10, 5, 0),
+                                             (70, 2048, 480, 100, 8, 1056), (1000, 96, 64, 130, 2, 64),
+                                             (3, 4128, 1184, 9, 5, 2080)])
+def test_moe_forms(hip, T, H, I, E, topk, Is, mx):
+    import torch
+    print(f"[moe] forms T={T} H={H} I={I} E={E} topk={topk} Is={Is} mx={mx}", flush=True)
+    g = _gen(torch, T + H + I)
+    w = mx_ref.moe_weights(g, H, I, E, Is, True, mx)
+    x = mx_ref.safe_tokens(g, w, T, topk, H)
+    r, b, gap = mx_ref.moe(x, w, topk, True, mx)
+    assert float(gap.min()) > 0
+    mx_ref.check(_run(hip, torch, w, x, topk, True), r, b, "forms")

@@ -237,3 +237,29 @@ def test_python_refusals(hip):
         hip.mxfp4_gemm(u8(65, 32), u8(65, 2), b[:, :64], b[:, 63:])
     assert e.value.code == 3
     hip.mxfp4_gemm(u8(64, 32), u8(64, 2), b[:, :64], b[:, 64:])        # beside x in one buffer
+
+
+# the forms of the product: shapes that the estimates give to each (few rows in
+# tiles of 1 to 4 x 16 with 16 and 32 outputs, 128- and 256-wide tiles), with row,
+# output and K edges in each; K past one pair of steps a wavefront, K of 4096 and
+# more, odd numbers of blocks
+@pytest.mark.parametrize("M,O,K", [(4, 12345, 2080), (5, 8200, 4128), (31, 9000, 96), (33, 520, 8192),
+                                   (47, 20000, 224), (50, 12352, 160), (64, 4100, 2144), (100, 12360, 1056),
+                                   (250, 6001, 2208), (513, 4104, 288), (2050, 2049, 4192), (4100, 4090, 8224),
+                                   (2048, 8192, 4096)])
+@pytest.mark.parametrize("mx", [False, True])
+def test_gemm_forms(hip, M, O, K, mx):
+    import torch
+    print(f"[mx] forms M={M} O={O} K={K} mx={mx}", flush=True)
+    x, w, ws = _operands(torch, M, O, K, 0, M + O + K)
+    x = x.contiguous()
+    y = torch.empty(M, O, dtype=torch.bfloat16, device="cuda")
+    if mx:
+        c, s = _quantize(hip, torch, x)
+        hip.mxfp4_gemm_mx(w, ws, c, s, y)
+        xv = mx_ref.values(c, s)
+    else:
+        hip.mxfp4_gemm(w, ws, x, y)
+        xv = x.double()
+    r, b = mx_ref.gemm(mx_ref.values(w, ws), xv)
+    mx_ref.check(y, r, b, f"forms mx={mx}")
