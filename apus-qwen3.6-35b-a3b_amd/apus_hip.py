@@ -113,6 +113,8 @@ def load(path=None):
     """Load the library (once). Raises if it was not built. APUS_HIP_LIB
     overrides the path (A/B runs of alternative builds)."""
     global _lib
+    if _lib is not None:                   # (looking the path up costs a microsecond)
+        return _lib
     path = path or os.environ.get("APUS_HIP_LIB") or LIB_PATH
     if _lib is None:
         # torch ships its own libamdhip64.so.7. Importing it first makes the
@@ -134,6 +136,11 @@ def load(path=None):
         _lib.apus_hip_last_error.restype = _sz
         _lib.apus_hip_kv_pool_free_blocks.restype = _sz
         _lib.apus_hip_st_ntensors.restype = _sz
+        # (argument types declared: plain integers go in as they are)
+        for name, types in (("mxfp4_quantize", "pzppzz"), ("mxfp4_dequantize", "pppzzz"),
+                            ("mxfp4_gemm_dev", "pppzpzzzz"), ("mxfp4_gemm_mx_dev", "pppppzzzz"),
+                            ("moe_layer_decode", "ppzpp")):
+            getattr(_lib, "apus_hip_" + name).argtypes = [_vp if t == "p" else _sz for t in types]
     return _lib
 
 
@@ -728,75 +735,77 @@ def free_attn_layer(L):
 
 
 # ---- MXFP4
-def _rows(t, what, ncols=None):
-    """(pointer, rows, columns, pitch) of a 2-D device tensor of 2-byte
-    elements whose rows are contiguous (any pitch)."""
-    if not t.is_cuda or t.dim() != 2 or t.element_size() != 2:
-        raise ValueError(f"{what}: a 2-D GPU tensor of bf16 values or codes, not {tuple(t.shape)} "
-                         f"{t.dtype} on {t.device}")
+def _rows(t, what, dev, ncols=None):
+    """(pointer, rows, columns, pitch) of a 2-D tensor of 2-byte elements on
+    device dev whose rows are contiguous (any pitch)."""
+    if t.get_device() != dev or t.dim() != 2 or t.element_size() != 2:
+        raise ValueError(f"{what}: a 2-D tensor of bf16 values or codes on GPU {dev}, not "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
     m, n = t.shape
     if ncols is not None and n != ncols:
         raise ValueError(f"{what}: rows of {n} elements, expected {ncols}")
-    if n > 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    if one != 1 and n > 1:
         raise ValueError(f"{what}: elements of a row must be contiguous")
-    return _vp(t.data_ptr()), m, n, t.stride(0) if m > 1 else n
+    return t.data_ptr(), m, n, ld if m > 1 else n
 
 
-def _bytes(t, shape, what):
-    """Pointer of a dense device tensor of bytes of this shape."""
-    if not t.is_cuda or t.element_size() != 1 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{what}: a contiguous GPU tensor of bytes of shape {tuple(shape)}, not "
+def _bytes(t, rows, cols, what, dev):
+    """Pointer of a dense [rows, cols] tensor of bytes on device dev."""
+    if t.get_device() != dev or t.element_size() != 1 or t.shape != (rows, cols) or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous tensor of bytes of shape {(rows, cols)} on GPU {dev}, not "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return _vp(t.data_ptr())
+    return t.data_ptr()
 
 
-def _same_device(*ts):
-    if len({t.device for t in ts if t is not None}) > 1:
-        raise ValueError(f"tensors on several devices: {[str(t.device) for t in ts if t is not None]}")
+def _gpu(t, what):
+    """The index of t's GPU."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{what}: a GPU tensor, not one on {t.device}")
+    return dev
 
 
 def mxfp4_quantize(x, codes, scales):
     """x [M, K] bf16 (rows of any pitch) -> codes [M, K/2], scales [M, K/32]
     (uint8): MXFP4, apus_hip_mxfp4_quantize."""
-    _same_device(x, codes, scales)
-    xp, M, K, ldx = _rows(x, "x")
-    _chk(load().apus_hip_mxfp4_quantize(xp, _sz(ldx), _bytes(codes, (M, K // 2), "codes"),
-                                        _bytes(scales, (M, K // 32), "scales"), _sz(M), _sz(K)))
+    dev = _gpu(x, "x")
+    xp, M, K, ldx = _rows(x, "x", dev)
+    _chk(load().apus_hip_mxfp4_quantize(xp, ldx, _bytes(codes, M, K // 2, "codes", dev),
+                                        _bytes(scales, M, K // 32, "scales", dev), M, K))
 
 
 def mxfp4_dequantize(codes, scales, x):
     """The bf16 values of codes, scales into x [M, K] (rows of any pitch)."""
-    _same_device(x, codes, scales)
-    xp, M, K, ldx = _rows(x, "x")
-    _chk(load().apus_hip_mxfp4_dequantize(_bytes(codes, (M, K // 2), "codes"),
-                                          _bytes(scales, (M, K // 32), "scales"), xp, _sz(ldx),
-                                          _sz(M), _sz(K)))
+    dev = _gpu(x, "x")
+    xp, M, K, ldx = _rows(x, "x", dev)
+    _chk(load().apus_hip_mxfp4_dequantize(_bytes(codes, M, K // 2, "codes", dev),
+                                          _bytes(scales, M, K // 32, "scales", dev), xp, ldx, M, K))
 
 
 def mxfp4_gemm(w, ws, x, y):
     """y [M, O] = x [M, K] w^T, w [O, K/2], ws [O, K/32] MXFP4, x and y bf16
     with rows of any pitch."""
-    _same_device(w, ws, x, y)
-    xp, M, K, ldx = _rows(x, "x")
+    dev = _gpu(x, "x")
+    xp, M, K, ldx = _rows(x, "x", dev)
     O = w.shape[0]
-    yp, ym, _, ldy = _rows(y, "y", O)
+    yp, ym, _, ldy = _rows(y, "y", dev, O)
     if ym != M:
         raise ValueError(f"y: {ym} rows, expected {M}")
-    _chk(load().apus_hip_mxfp4_gemm_dev(_bytes(w, (O, K // 2), "w"), _bytes(ws, (O, K // 32), "ws"),
-                                        xp, _sz(ldx), yp, _sz(ldy), _sz(M), _sz(O), _sz(K)))
+    _chk(load().apus_hip_mxfp4_gemm_dev(_bytes(w, O, K // 2, "w", dev), _bytes(ws, O, K // 32, "ws", dev),
+                                        xp, ldx, yp, ldy, M, O, K))
 
 
 def mxfp4_gemm_mx(w, ws, x, xs, y):
     """As mxfp4_gemm with the activations in MXFP4: x [M, K/2], xs [M, K/32]."""
-    _same_device(w, ws, x, xs, y)
+    dev = _gpu(x, "x")
     M, K, O = x.shape[0], x.shape[1] * 2, w.shape[0]
-    yp, ym, _, ldy = _rows(y, "y", O)
+    yp, ym, _, ldy = _rows(y, "y", dev, O)
     if ym != M:
         raise ValueError(f"y: {ym} rows, expected {M}")
-    _chk(load().apus_hip_mxfp4_gemm_mx_dev(_bytes(w, (O, K // 2), "w"),
-                                           _bytes(ws, (O, K // 32), "ws"), _bytes(x, (M, K // 2), "x"),
-                                           _bytes(xs, (M, K // 32), "xs"), yp, _sz(ldy), _sz(M),
-                                           _sz(O), _sz(K)))
+    _chk(load().apus_hip_mxfp4_gemm_mx_dev(_bytes(w, O, K // 2, "w", dev),
+                                           _bytes(ws, O, K // 32, "ws", dev), _bytes(x, M, K // 2, "x", dev),
+                                           _bytes(xs, M, K // 32, "xs", dev), yp, ldy, M, O, K))
 
 
 # ---- mixture of experts
@@ -809,7 +818,9 @@ def moe_layer(dims, w, norm_topk=True):
     scales. The layer keeps the tensors alive."""
     hidden, inter, experts, topk, shared = dims
     mx = "s_gate_up" in w
-    _same_device(*w.values())
+    devs = {t.device for t in w.values() if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"weights on several devices: {sorted(map(str, devs))}")
     shapes = {"w_gate_up": (experts, 2 * inter, hidden), "w_down": (experts, hidden, inter)}
     if shared:
         shapes.update(w_shared_gate_up=(2 * shared, hidden), w_shared_down=(hidden, shared))
@@ -853,11 +864,13 @@ class MoeWork:
 def moe_layer_decode(layer, work, x, y):
     """A mixture-of-experts layer on a decode step's tokens: x [T, hidden]
     -> y [T, hidden], contiguous bf16 device tensors; y may be x."""
-    _same_device(x, y, layer._tensors["w_router"])
+    dev, H = _gpu(layer._tensors["w_router"], "w_router"), layer.hidden
     for t, n in ((x, "x"), (y, "y")):
-        if t.dim() != 2 or t.shape != x.shape or t.shape[1] != layer.hidden or t.element_size() != 2:
-            raise ValueError(f"{n}: [T, {layer.hidden}] bf16, not {tuple(t.shape)} {t.dtype}")
-    _chk(load().apus_hip_moe_layer_decode(C.byref(layer), work.h, _sz(x.shape[0]), _dp(x), _dp(y)))
+        if (t.get_device() != dev or t.shape != x.shape or t.dim() != 2 or t.shape[1] != H
+                or t.element_size() != 2 or not t.is_contiguous()):
+            raise ValueError(f"{n}: contiguous [T, {H}] bf16 on GPU {dev}, not {tuple(t.shape)} {t.dtype} "
+                             f"on {t.device}")
+    _chk(load().apus_hip_moe_layer_decode(C.byref(layer), work.h, x.shape[0], x.data_ptr(), y.data_ptr()))
 
 
 # ---- named-intermediate capture

@@ -47,7 +47,7 @@ struct ApusHipMoeWork {
 namespace {
 
 constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
-constexpr int kFewTokens = 4;          // up to here a choice is a slot of its own
+constexpr int kFewTokens = 2;          // up to here a choice is a slot of its own
 constexpr int kGroup = 32;             // most rows of a slot
 
 struct MoeArgs {
@@ -104,13 +104,14 @@ __device__ __forceinline__ float wave_sum(float f) {
 }
 
 // A wavefront's choice for token t, in index order: lane l holds logits l,
-// l + 64, ... The k-th largest key is found a bit at a time from the top,
+// l + 64, ... The k-th largest key is found two bits at a time from the top,
 // counting by ballots (k rounds of a maximum over the wavefront took 8 us, this
-// takes under one); of the keys equal to it the lowest indices are taken.
+// takes about one); of the keys equal to it the lowest indices are taken.
+// The logits were written by other workgroups of this launch, and are read where
+// those meet.
 template <int NJ>
 __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
     const float *lg = a.logits + (size_t)t * (a.E + 1);
-    // (written by other workgroups of this launch: read where they met)
     auto logit = [&](int e) { return __hip_atomic_load(lg + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     float l[NJ];
     uint32_t key[NJ], best = 0;            // key 0: past E
@@ -131,17 +132,16 @@ __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
         return n;
     };
     uint32_t v = 0;
-    int above = 0;                         // keys > v
-    for (int b = 31; b >= 0; b--) {
-        const uint32_t c = v | 1u << b;
-        const int n = count(c);
-        if (n >= a.k) v = c;
-        if (n == a.k) break;
+    for (int b = 30; b >= 0; b -= 2) {
+        const uint32_t c1 = v | 1u << b, c2 = v | 2u << b, c3 = v | 3u << b;
+        const int n1 = count(c1), n2 = count(c2), n3 = count(c3);
+        if (n1 < a.k) continue;
+        v = n3 >= a.k ? c3 : n2 >= a.k ? c2 : c1;
+        if ((n3 >= a.k ? n3 : n2 >= a.k ? n2 : n1) == a.k) break;
     }
-    above = v == 0xffffffffu ? 0 : count(v + 1);
+    const int above = v == 0xffffffffu ? 0 : count(v + 1);           // keys > v
     int ties = a.k - above, at = 0;        // of the keys equal to v, the first `ties`
     const uint64_t below = (1ull << lane) - 1;
-    float p[NJ], sum = 0.0f;
     int pos[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
@@ -151,8 +151,12 @@ __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
         pos[j] = in ? at + __popcll(m & below) : -1;
         at += __popcll(m);
         ties -= min(ties, (int)__popcll(eq));
+    }
+    float p[NJ], sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
         p[j] = expf(l[j] - top);
-        if (lane + 64 * j < a.E && (in || !a.norm)) sum += p[j];
+        if (lane + 64 * j < a.E && (pos[j] >= 0 || !a.norm)) sum += p[j];
     }
     sum = wave_sum(sum);
 #pragma unroll
@@ -169,18 +173,25 @@ __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
 constexpr int kRouterWaves = 16;
 
 // The choices of all tokens by expert, by one workgroup: count, sum, place. (In
-// which order an expert's choices come does not matter: a choice's values do
-// not depend on its place.)
+// which order an expert's choices come does not matter: a choice's values do not
+// depend on its place.)
 __device__ __forceinline__ void make_slots(const MoeArgs &a, int lane, int wave) {
     __shared__ int cursor[kMoeMaxExperts], wsum[2][kRouterWaves];
+    constexpr int THREADS = 64 * kRouterWaves, KEEP = 4;
     const int tid = threadIdx.x, n = a.T * a.k;
     auto id = [&](int q) {                 // (chosen by other workgroups of this launch)
         const int e = __hip_atomic_load(a.ids + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return min(max(e, 0), a.E - 1);    // (in range whatever ids holds)
     };
+    int mine[KEEP];                        // the first ids, read once
+#pragma unroll
+    for (int i = 0; i < KEEP; i++) mine[i] = tid + i * THREADS < n ? id(tid + i * THREADS) : 0;
     cursor[tid] = 0;
     __syncthreads();
-    for (int q = tid; q < n; q += 64 * kRouterWaves) atomicAdd(&cursor[id(q)], 1);
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (tid + i * THREADS < n) atomicAdd(&cursor[mine[i]], 1);
+    for (int q = tid + KEEP * THREADS; q < n; q += THREADS) atomicAdd(&cursor[id(q)], 1);
     __syncthreads();
     // thread e: running sums over the experts, of the choices and of the slots
     const int c = cursor[tid], k = (c + kGroup - 1) / kGroup;
@@ -208,17 +219,22 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, int lane, int wave)
     }
     for (int i = 0; i < k; i++)
         a.slots[slot - k + i] = make_int4(tid, at - c + i * kGroup, min(kGroup, c - i * kGroup), 0);
-    for (int i = total + tid; i < a.nslots; i += 64 * kRouterWaves) a.slots[i] = make_int4(0, 0, 0, 0);
+    for (int i = total + tid; i < a.nslots; i += THREADS) a.slots[i] = make_int4(0, 0, 0, 0);
     cursor[tid] = at - c;
     __syncthreads();
-    for (int q = tid; q < n; q += 64 * kRouterWaves) a.list[atomicAdd(&cursor[id(q)], 1)] = (uint16_t)q;
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (tid + i * THREADS < n) a.list[atomicAdd(&cursor[mine[i]], 1)] = (uint16_t)(tid + i * THREADS);
+    for (int q = tid + KEEP * THREADS; q < n; q += THREADS) a.list[atomicAdd(&cursor[id(q)], 1)] = (uint16_t)q;
 }
 
 // 16 experts (the shared gate as one more) x 16 tokens a workgroup, K over its
-// 16 wavefronts. The last workgroup of the 16 tokens to finish chooses for
-// them, a wavefront each, and the last of those sorts the choices: what a
-// workgroup hands on it stores where all XCDs see it, waits for the stores, and
-// counts itself; nobody waits for anybody.
+// 16 wavefronts. The last workgroup of the 16 tokens to finish chooses for them, a
+// wavefront each, and with more than a few tokens the last of those sorts the
+// choices: what a workgroup hands on it stores where all XCDs see it, waits for the
+// stores, and counts itself; nobody waits for anybody. (One token: 8.2 us, 4.2 of
+// them to the logits. Choosing in every workgroup of the next launch instead costs
+// that launch as much as is saved here, 4 us, most of it fetching the code.)
 static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
 template <int NJ>
 __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
@@ -296,8 +312,7 @@ __device__ __forceinline__ Task task_of(const MoeArgs &a, int b, int nsh, int np
     }
     b -= nsh * groups;
     const int slot = b / nper, part = b % nper;
-    if (a.T <= kFewTokens)
-        return {__builtin_amdgcn_readfirstlane(a.ids[slot]), part, slot, 1, nullptr};
+    if (a.T <= kFewTokens) return {__builtin_amdgcn_readfirstlane(a.ids[slot]), part, slot, 1, nullptr};
     const int4 s = a.slots[slot];
     return {__builtin_amdgcn_readfirstlane(s.x), part, 0, __builtin_amdgcn_readfirstlane(s.z),
             a.list + __builtin_amdgcn_readfirstlane(s.y)};
@@ -689,42 +704,55 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a
 }
 
 // y of up to kFewTokens tokens: 16 outputs a workgroup, the steps of 128 k of
-// every (token, expert) dealt to its 8 wavefronts. A step's product lands in
-// the token's column with the expert's weight; the columns of other tokens
-// (all multiplied with this token's h) are left out.
+// every (token, expert) dealt to its 12 wavefronts (9 experts of 4 steps, one
+// token: 3 each, all on their way at once). A step's product lands in the token's
+// column with the expert's weight; the columns of other tokens (all multiplied
+// with this token's h) are left out.
+constexpr int kFewWaves = 12;
 template <class W>
-__global__ __launch_bounds__(512) void k_moe_down_few(MoeArgs a) {
-    __shared__ mx_f32x4 red[8][64];
+__global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
+    __shared__ mx_f32x4 red[kFewWaves][64];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = blockIdx.x * 16, n = a.T * a.k;
     const int si = (a.I + 127) / 128, ss = (a.Is + 127) / 128;
     const int units = n * si + (a.Is ? a.T * ss : 0);
-    constexpr int U = W::mx ? 4 : 2;
+    constexpr int U = 3;
     using X = XBf16<W>;
     const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
     mx_f32x4 acc{};
-    for (int b = wave; b < units; b += 8 * U) {
-        typename W::Frag fw[U];
-        typename X::Frag fh[U], fl[U];
+    for (int b = wave; b < units; b += kFewWaves * U) {
+        // choice, its expert, step and weight of each
+        int q[U], e[U], st[U];
         float p[U];
-        bool on[U];
+        bool on[U], sh[U];
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const bool live = b + 8 * i < units;
-            const int u = live ? b + 8 * i : b;
-            const bool sh = u >= n * si;
-            const int q = sh ? n + (u - n * si) / ss : u / si;
-            const int st = sh ? (u - n * si) % ss : u % si, I = sh ? a.Is : a.I;
-            const int t = sh ? q - n : q / a.k;
-            const int e = __builtin_amdgcn_readfirstlane(sh ? 0 : a.ids[q]);
-            p[i] = a.wts[sh ? t * (a.k + 1) + a.k : t * (a.k + 1) + q % a.k];
+            const bool live = b + kFewWaves * i < units;
+            const int u = live ? b + kFewWaves * i : b;
+            sh[i] = u >= n * si;
+            q[i] = sh[i] ? n + (u - n * si) / ss : u / si;
+            st[i] = sh[i] ? (u - n * si) % ss : u % si;
+            const int t = sh[i] ? q[i] - n : q[i] / a.k;
+            e[i] = a.ids[sh[i] ? 0 : q[i]];
+            p[i] = a.wts[t * (a.k + 1) + (sh[i] ? a.k : q[i] % a.k)];
             on[i] = live && t == r;
-            const auto wt = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn, (size_t)e * a.H + o0, 16, I);
-            const uint32_t xl = X::lane(h_at(a, q, sh) * 2, g);
-            W::load(fw[i], wt, W::lane(lane, I), st, I);
-            X::load(fh[i], hb, xl, st, I);
-            X::load(fl[i], hb, xl + I * 2, st, I);
+        }
+        typename W::Frag fw[U];
+        typename X::Frag fh[U], fl[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int I = sh[i] ? a.Is : a.I;
+            const uint32_t xl = X::lane(h_at(a, q[i], sh[i]) * 2, g);
+            X::load(fh[i], hb, xl, st[i], I);
+            X::load(fl[i], hb, xl + I * 2, st[i], I);
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int I = sh[i] ? a.Is : a.I, x = __builtin_amdgcn_readfirstlane(e[i]);
+            const auto wt = W::tile(sh[i] ? a.w_sdn : a.w_dn, sh[i] ? a.s_sdn : a.s_dn,
+                                    (sh[i] ? 0 : (size_t)x * a.H) + o0, 16, I);
+            W::load(fw[i], wt, W::lane(lane, I), st[i], I);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
@@ -743,8 +771,10 @@ __global__ __launch_bounds__(512) void k_moe_down_few(MoeArgs a) {
     red[wave][lane] = acc;
     __syncthreads();
     if (wave || r >= a.T) return;
-    acc = ((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane])) +
-          ((red[4][lane] + red[5][lane]) + (red[6][lane] + red[7][lane]));
+    mx_f32x4 s[4] = {};
+#pragma unroll
+    for (int i = 0; i < kFewWaves; i++) s[i & 3] += red[i][lane];
+    acc = (s[0] + s[1]) + (s[2] + s[3]);
     *reinterpret_cast<ushort4 *>(a.y + (size_t)r * a.H + o0 + 4 * g) =
         make_ushort4(f2bf(acc[0]), f2bf(acc[1]), f2bf(acc[2]), f2bf(acc[3]));
 }
@@ -823,7 +853,7 @@ int experts_run(const MoeArgs &a) {
     if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, 2>(a, slots))
         return r;
     if (a.T <= kFewTokens) {
-        APUS_TIMED("k_moe_down_few", k_moe_down_few<W><<<(unsigned)a.H / 16, 512, 0, stream()>>>(a));
+        APUS_TIMED("k_moe_down_few", k_moe_down_few<W><<<(unsigned)a.H / 16, 64 * kFewWaves, 0, stream()>>>(a));
         return launch_check("k_moe_down_few");
     }
     const bool downs = slots * a.H / 32 >= 1024 && 32 * down_pitch(std::max(a.I, a.Is)) <= kDownH;
