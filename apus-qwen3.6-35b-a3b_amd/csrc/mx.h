@@ -9,12 +9,22 @@ namespace apus {
 int mx_check_dims(size_t M, size_t O, size_t K);   // sizes under 2^31, K in whole blocks
 int mx_ready();                                    // ensure_ready, on the calling thread's device
 
-// products for many rows (mx_wide.hip): tiles of 128 x 128 (shape 2) or 256 x 256
-// (shape 4)
-int mx_gemm_wide(const uint8_t *w, const uint8_t *ws, const uint8_t *x, const uint8_t *xs,
-                 uint16_t *y, size_t ldy, int M, int O, int K, int shape);
-int mx_gemm_wide16(const uint8_t *w, const uint8_t *ws, const uint16_t *x, size_t ldx, uint16_t *y,
-                   size_t ldy, int M, int O, int K, int shape);
+// y = x w^T: M rows, O outputs, K inner elements; x is bf16 rows of pitch ldx, or,
+// with xs, MXFP4
+struct MxProduct {
+    const uint8_t *w, *ws;
+    const void *x;
+    const uint8_t *xs;
+    size_t ldx;
+    uint16_t *y;
+    size_t ldy;
+    int M, O, K;
+};
+// products for many rows (mx_wide.hip): shape 2, tiles of 128 x 128, two a CU; 3, the
+// same, one a CU, with K in two halves side by side; 4, 256 x 256
+int mx_gemm_wide(const MxProduct &a, int shape);
+// of so many 256 x 256 tiles, those that go in quarters, as the last workgroups
+size_t mx_quarters(size_t tiles);
 
 }  // namespace apus
 

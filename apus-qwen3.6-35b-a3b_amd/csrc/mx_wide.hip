@@ -22,23 +22,14 @@ __device__ __forceinline__ uint32_t pk2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, mx_bf16x2));
 }
 
-// 16 (4) bytes a lane from base + off (per lane) to LDS byte lds + 16 (4) *
-// lane. live: all ones, or zero for a copy that is counted (vmcnt) but moves
-// nothing; the wavefront's lanes are all active here. The two moves (the
-// s_nop) are the wait state between the write of M0 and its use.
+// 16 bytes a lane from base + off (per lane) to LDS byte lds + 16 * lane. live:
+// all ones, or zero for a copy past the last stage, into a slot that nobody reads:
+// it counts (vmcnt) like the others, so that what a wait leaves in flight is the
+// same all along. The s_nop is the wait state between the write of M0 and its use.
 __device__ __forceinline__ void copy16(uint32_t off, const void *base, uint32_t lds, int live) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    live = __builtin_amdgcn_readfirstlane(live);
-    asm volatile("s_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\t"
-                 "global_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
-                 ::"v"(off), "s"(base), "{m0}"(lds), "s"(live) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t off, const void *base, uint32_t lds, int live) {
-    lds = __builtin_amdgcn_readfirstlane(lds);
-    live = __builtin_amdgcn_readfirstlane(live);
-    asm volatile("s_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\t"
-                 "global_load_lds_dword %0, %1\n\ts_mov_b64 exec, -1"
-                 ::"v"(off), "s"(base), "{m0}"(lds), "s"(live) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off & (uint32_t)live), "s"(base), "{m0}"(lds)
+                 : "memory");
 }
 
 // p, uniform over the wavefront, in scalar registers
@@ -99,6 +90,24 @@ __device__ __forceinline__ void store_tile(char *sm, const f32x16 (&acc)[TO][TMM
     }
 }
 
+// The c-th 16 scale bytes (512 k) of a row's `ks`, for a thread to bring, zeros past
+// the row's end. So many at a time because a load whose lanes read different rows
+// takes the address unit a clock a lane, however little each lane reads: 8 bytes a
+// row and stage took it as long as the codes.
+struct RowScales {
+    u32x4 v;
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t c, uint32_t ks) {
+        if (ks >= 16) {                                  // (the row's last 16 bytes and a shift)
+            const uint32_t at = min(16 * c, ks - 16), past = 16 * c - at;
+            __builtin_memcpy(&v, row + at, 16);          // (rows may begin at any byte)
+            if (past) v = __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (8 * min(past, 15u)));
+        } else {
+            v = u32x4{};
+            for (uint32_t i = 0; i < ks; i++) v[i / 4] |= (uint32_t)row[i] << (i % 4 * 8);
+        }
+    }
+};
+
 // ---- both operands MXFP4 -----------------------------------------------------
 // A stage is 256 k: 128 bytes of codes and 8 of scales per row, BO weight rows,
 // then BM activation rows, double-buffered in LDS. 16-byte chunk c (block c of
@@ -106,86 +115,68 @@ __device__ __forceinline__ void store_tile(char *sm, const f32x16 (&acc)[TO][TMM
 // read phase hit 8 distinct slots. MFMA step s takes 64 k: lane (row l % 32,
 // half g = l / 32) chunk 2 s + g, and the scale byte of the same number.
 // Blocks past K (in the last stage): zero codes and scale 1 on both sides.
-// AL: rows of scales are 4-byte aligned (K a multiple of 128) and are copied
-// like the codes; else they pass through registers, a byte at a time.
+// Scales come for two stages at a time, through registers.
 constexpr int kMxStage = 256;
 
-template <int TO, int TMM, bool AL>
-__global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide(
-    const uint8_t *__restrict__ w, const uint8_t *__restrict__ ws, const uint8_t *__restrict__ x,
-    const uint8_t *__restrict__ xs, uint16_t *__restrict__ y, size_t ldy, int M, int O, int K) {
+template <int TO, int TMM>
+constexpr int kMxLds = 2 * 64 * (TO + TMM) * (kMxStage / 2 + 16);
+template <int TO, int TMM>
+__device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, int m0, int k0, int nk,
+                                        f32x16 (&acc)[TO][TMM]) {
     constexpr int BO = 64 * TO, BM = 64 * TMM, ROWS = BO + BM;
-    constexpr int PB = BO * 128, SB = ROWS * 128, SCB = ROWS * 8;
+    constexpr int PB = BO * 128, SB = ROWS * 128;
+    constexpr int SCB = ROWS * 16;
     constexpr int PPW = ROWS / 32;                       // code copies a wavefront and stage
-    constexpr int SPW = AL ? ROWS / 128 : 0;             // scale copies
-    constexpr int SPT = AL ? 1 : ROWS / 32;              // else scale bytes a thread
+    constexpr int SPT = ROWS / 256;                      // rows of scales a thread
     constexpr int NF = TO * TMM, NR = TO + TMM;
-    static_assert(ROWS % 128 == 0, "copies must split evenly over the wavefronts");
-    __shared__ __attribute__((aligned(16))) char sm[2 * (SB + SCB)];
+    static_assert(ROWS % 256 == 0, "rows must split evenly over the threads");
+    static_assert(2 * (SB + SCB) == kMxLds<TO, TMM>);
     char *const scales = sm + 2 * SB;
-    const int nbo = (O + BO - 1) / BO, nbm = (M + BM - 1) / BM;
-    int ob, mb;
-    tile_of(blockIdx.x, nbo, nbm, ob, mb);
-    if (ob >= nbo) return;                               // (the grid is a multiple of 8)
-    const int o0 = ob * BO, m0 = mb * BM;
+    const int M = a.M, O = a.O, K = a.K - k0;            // K: from k0 on
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int wo = wave >> 1, wm = wave & 1, g = lane >> 5;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
-    const uint32_t kc = (uint32_t)K / 2, ks = (uint32_t)K / kMxBlock;   // bytes of a row
-    const int nk = (K + kMxStage - 1) / kMxStage;
+    const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
+    const uint32_t kleft = (uint32_t)K / 2, sleft = (uint32_t)K / kMxBlock; // from k0 on
+    const int nsc = (min(nk, (K + kMxStage - 1) / kMxStage) + 1) / 2;
     // tile-relative, so that 32-bit offsets do (rows past O or M read the last
     // row; their products are not stored)
-    const uint8_t *const wt = w + (size_t)o0 * kc, *const xt = x + (size_t)m0 * kc;
-    const uint8_t *const wst = ws + (size_t)o0 * ks, *const xst = xs + (size_t)m0 * ks;
+    const uint8_t *const wt = a.w + (size_t)o0 * kc + k0 / 2, *const xt = (const uint8_t *)a.x + (size_t)m0 * kc + k0 / 2;
+    const uint8_t *const wst = a.ws + (size_t)o0 * ks + k0 / kMxBlock, *const xst = a.xs + (size_t)m0 * ks + k0 / kMxBlock;
     auto row_of = [&](int r) {                           // stage row -> row of its operand's tile
         return r < BO ? min(r, O - 1 - o0) : min(r - BO, M - 1 - m0);
     };
-    uint32_t roff[PPW], soff[AL ? SPW : 1];
-    const void *rbuf[PPW], *sbuf[AL ? SPW : 1];
+    uint32_t roff[PPW];
+    const void *rbuf[PPW];
 #pragma unroll
     for (int i = 0; i < PPW; i++) {
         const int p = wave * PPW + i;
         roff[i] = row_of(p * 8 + (lane >> 3)) * kc;
         rbuf[i] = uniform(p < BO / 8 ? wt : xt);
     }
-#pragma unroll
-    for (int i = 0; i < SPW; i++) {
-        const int p = wave * SPW + i;
-        soff[i] = row_of(p * 32 + (lane >> 1)) * ks;
-        sbuf[i] = uniform(p < BO / 32 ? wst : xst);
-    }
-    const uint32_t cg = ((lane & 7) ^ (lane >> 3)) * 16, sg = (lane & 1) * 4;
+    const uint32_t cg = ((lane & 7) ^ (lane >> 3)) * 16;
     auto copy_codes = [&](int i, int st, int live) {
         uint32_t at = st * 128 + cg;
-        at = at < kc ? at : 0;                           // (past the row's end: masked when read)
+        at = at < kleft ? at : 0;                           // (past the row's end: masked when read)
         const int p = wave * PPW + i;
         copy16(roff[i] + at, rbuf[i], lds0 + (st & 1) * SB + p * 1024, live);
     };
-    auto copy_scales = [&](int i, int st, int live) {
-        uint32_t at = st * 8 + sg;
-        at = at < ks ? at : 0;
-        const int p = wave * SPW + i;
-        copy4(soff[i] + at, sbuf[i], lds0 + 2 * SB + (st & 1) * SCB + p * 256, live);
-    };
-    // the unaligned form: bytes (32 rows of 8 an instruction of the workgroup)
-    uint8_t sbyte[SPT];
-    auto load_bytes = [&](int st) {
-        if (AL) return;
-        const uint32_t at = (uint32_t)st * 8 + (lane & 7);
+    // scales of this thread's rows, through registers
+    const int tid = threadIdx.x & 255;
+    RowScales sreg[SPT];
+    auto load_scales = [&](int c) {
 #pragma unroll
         for (int i = 0; i < SPT; i++) {
-            const int r = i * 32 + wave * 8 + (lane >> 3);
-            sbyte[i] = (r < BO ? wst : xst)[row_of(r) * ks + (at < ks ? at : 0)];
+            const int r = i * 256 + tid;
+            sreg[i].load((r < BO ? wst : xst) + (size_t)row_of(r) * ks, c, sleft);
         }
     };
-    auto put_bytes = [&](int st) {
-        if (AL) return;
+    auto put_scales = [&](int c) {
 #pragma unroll
         for (int i = 0; i < SPT; i++)
-            scales[(st & 1) * SCB + (i * 32 + wave * 8 + (lane >> 3)) * 8 + (lane & 7)] = sbyte[i];
+            *reinterpret_cast<u32x4 *>(scales + (c & 1) * SCB + (i * 256 + tid) * 16) = sreg[i].v;
     };
-    f32x16 acc[TO][TMM];
 #pragma unroll
     for (int t = 0; t < TO; t++)
 #pragma unroll
@@ -209,16 +200,16 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide(
     // a row's 8 scale bytes as two words, shifted so that byte 0 (2) of word
     // s / 2 is this lane half's in an even (odd) step s
     auto rd_scales = [&](int st, Scale &c) {
-        const char *p = scales + (st & 1) * SCB + (lane & 31) * 8;
+        const char *p = scales + (st >> 1 & 1) * SCB + (st & 1) * 8 + (lane & 31) * 16;
 #pragma unroll
         for (int t = 0; t < TO; t++) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p + (wo * TO + t) * 256);
+            const uint2 v = *reinterpret_cast<const uint2 *>(p + (wo * TO + t) * 512);
             c.a[t][0] = v.x >> (8 * g);
             c.a[t][1] = v.y >> (8 * g);
         }
 #pragma unroll
         for (int u = 0; u < TMM; u++) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(p + BO * 8 + (wm * TMM + u) * 256);
+            const uint2 v = *reinterpret_cast<const uint2 *>(p + BO * 16 + (wm * TMM + u) * 512);
             c.b[u][0] = v.x >> (8 * g);
             c.b[u][1] = v.y >> (8 * g);
         }
@@ -255,38 +246,31 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide(
     using s3 = std::integral_constant<int, 3>;
     Frag f0, f1;
     Scale c0, c1;
+    load_scales(0);
 #pragma unroll
     for (int st = 0; st < 2; st++) {
-        const int live = (st - nk) >> 31;
-        load_bytes(min(st, nk - 1));
-        put_bytes(st);
 #pragma unroll
-        for (int i = 0; i < SPW; i++) copy_scales(i, st, live);
-#pragma unroll
-        for (int i = 0; i < PPW; i++) copy_codes(i, st, live);
+        for (int i = 0; i < PPW; i++) copy_codes(i, st, (st - nk) >> 31);
     }
-    if (nk >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW + SPW) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    put_scales(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW) : "memory");
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NR; j++) rd1(0, 0, j, f0);
     rd_scales(0, c0);
     for (int kt = 0; kt < nk - 1; kt++) {
-        load_bytes(min(kt + 2, nk - 1));
+        if ((kt & 1) == 0) load_scales(min(kt / 2 + 1, nsc - 1));
         step(s0{}, f0, c0, f1, yes{}, kt, 1, no{}, 0, 0);
         step(s1{}, f1, c0, f0, yes{}, kt, 2, no{}, 0, 0);
         step(s2{}, f0, c0, f1, yes{}, kt, 3, no{}, 0, 0);
         // every operand of this stage has been read, by this wavefront (it
         // waited for f1) and after the barrier by all, and the next stage's
-        // copies, the only ones in flight, have landed: stage kt + 2 goes into
-        // this stage's slot
+        // copies have landed: stage kt + 2 goes into this stage's slot
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         rd_scales(kt + 1, c1);
-        put_bytes(kt + 2);
+        if ((kt & 1) == 0) put_scales(kt / 2 + 1);
         const int live = (kt + 2 - nk) >> 31;
-#pragma unroll
-        for (int i = 0; i < SPW; i++) copy_scales(i, kt + 2, live);
         step(s3{}, f1, c0, f0, yes{}, kt + 1, 0, yes{}, kt + 2, live);
         c0 = c1;
     }
@@ -323,23 +307,11 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide(
     step(s3{}, f1, c0, f0, no{}, 0, 0, no{}, 0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    store_tile<TO, TMM>(sm, acc, y, ldy, o0 + wo * TO * 32, m0 + wm * TMM * 32, O, M, wave, lane);
-}
-
-template <int TO, int TMM>
-int launch_mx_wide(const uint8_t *w, const uint8_t *ws, const uint8_t *x, const uint8_t *xs,
-                   uint16_t *y, size_t ldy, int M, int O, int K) {
-    const unsigned grid = tile_grid((int)cdiv(O, 64 * TO), (int)cdiv(M, 64 * TMM));
-    const bool al = K % 128 == 0 && ((uintptr_t)ws | (uintptr_t)xs) % 4 == 0;
-    APUS_TIMED("k_mx_gemm_wide",
-               if (al) k_mx_gemm_wide<TO, TMM, true><<<grid, 256, 0, stream()>>>(w, ws, x, xs, y, ldy, M, O, K);
-               else k_mx_gemm_wide<TO, TMM, false><<<grid, 256, 0, stream()>>>(w, ws, x, xs, y, ldy, M, O, K));
-    return launch_check("k_mx_gemm_wide");
 }
 
 // ---- bf16 activations ----------------------------------------------------------
 // A stage is 64 k of the activations, 128 bytes a row; the weights come in
-// chunks of 256 k (128 bytes of codes and 8 of scales a row), both double-
+// chunks of 256 k (128 bytes of codes a row), their scales of 512 k, all double-
 // buffered in LDS. A quarter of a chunk is copied with each stage. In stage t
 // of a chunk, lane (row l % 32, half g) takes the weights' block 2 t + g, one
 // 16-byte read for the whole stage, and MFMA step j its codes 8 j .., widened
@@ -348,33 +320,31 @@ int launch_mx_wide(const uint8_t *w, const uint8_t *ws, const uint8_t *x, const 
 // k as bf16 weights would need.
 constexpr int kMx16Stage = 64;
 
-template <int TO, int TMM, bool AL>
-__global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
-    const uint8_t *__restrict__ w, const uint8_t *__restrict__ ws, const uint16_t *__restrict__ x,
-    size_t ldx, uint16_t *__restrict__ y, size_t ldy, int M, int O, int K) {
+template <int TO, int TMM>
+constexpr int kMx16Lds = 2 * 64 * (TMM * kMx16Stage * 2 + TO * (128 + 16));
+template <int TO, int TMM>
+__device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, int m0, int k0, int nk,
+                                          f32x16 (&acc)[TO][TMM]) {
     constexpr int BO = 64 * TO, BM = 64 * TMM;
-    constexpr int XB = BM * 128, WB = BO * 128, SCB = BO * 8;
+    constexpr int XB = BM * 128, WB = BO * 128, SCB = BO * 16;
     constexpr int XPW = BM / 32, WPW = BO / 128;         // copies a wavefront and stage
-    constexpr int SPW = AL ? BO / 128 : 0;               // and chunk
-    constexpr int SPT = AL ? 1 : BO / 32;
     constexpr int NF = TO * TMM;
-    __shared__ __attribute__((aligned(16))) char sm[2 * (XB + WB + SCB)];
     constexpr int W0 = 2 * XB, S0 = 2 * (XB + WB);
-    const int nbo = (O + BO - 1) / BO, nbm = (M + BM - 1) / BM;
-    int ob, mb;
-    tile_of(blockIdx.x, nbo, nbm, ob, mb);
-    if (ob >= nbo) return;                               // (the grid is a multiple of 8)
-    const int o0 = ob * BO, m0 = mb * BM;
+    static_assert(S0 + 2 * SCB == kMx16Lds<TO, TMM> && BO <= 256);
+    const int M = a.M, O = a.O, K = a.K - k0;            // K: from k0 on
+    const size_t ldx = a.ldx;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int tid = threadIdx.x & 255;
     const int wo = wave >> 1, wm = wave & 1, g = lane >> 5;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
-    const uint32_t kc = (uint32_t)K / 2, ks = (uint32_t)K / kMxBlock, kx = (uint32_t)K * 2;
-    const int nk = (K + kMx16Stage - 1) / kMx16Stage, nch = (nk + 3) / 4;
-    const uint8_t *const wst = ws + (size_t)o0 * ks;
-    const void *const wt = uniform(w + (size_t)o0 * kc), *const wsb = uniform(wst),
-               *const xt = uniform(x + (size_t)m0 * ldx);
-    const uint32_t cg = ((lane & 7) ^ (lane >> 3)) * 16, sg = (lane & 1) * 4;
+    const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
+    const uint32_t kleft = (uint32_t)K / 2, sleft = (uint32_t)K / kMxBlock, kx = (uint32_t)K * 2;    // from k0 on
+    const int nch = (nk + 3) / 4, nsc = (min(nk, (K + kMx16Stage - 1) / kMx16Stage) + 7) / 8;
+    const uint8_t *const wrow = a.ws + (size_t)(o0 + min(tid % BO, O - 1 - o0)) * ks + k0 / kMxBlock;
+    const void *const wt = uniform(a.w + (size_t)o0 * kc + k0 / 2),
+               *const xt = uniform((const uint16_t *)a.x + (size_t)m0 * ldx + k0);
+    const uint32_t cg = ((lane & 7) ^ (lane >> 3)) * 16;
     uint32_t xoff[XPW];
 #pragma unroll
     for (int i = 0; i < XPW; i++)
@@ -387,44 +357,20 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
     // quarter q of chunk c: 64 TO / 4 rows
     auto copy_w = [&](int i, int c, int q, int live) {
         uint32_t at = c * 128 + cg;
-        at = at < kc ? at : 0;
+        at = at < kleft ? at : 0;
         const int p = q * (BO / 32) + wave * WPW + i;
         const uint32_t row = min(p * 8 + (lane >> 3), O - 1 - o0);
         copy16(row * kc + at, wt, lds0 + W0 + (c & 1) * WB + p * 1024, live);
     };
-    auto copy_scales = [&](int i, int c, int live) {
-        uint32_t at = c * 8 + sg;
-        at = at < ks ? at : 0;
-        const int p = wave * SPW + i;
-        const uint32_t row = min(p * 32 + (lane >> 1), O - 1 - o0);
-        copy4(row * ks + at, wsb, lds0 + S0 + (c & 1) * SCB + p * 256, live);
+    // 512 k of a row's scales, through registers
+    RowScales sreg;
+    auto put_scales = [&](int c) {
+        if (BO == 256 || tid < BO) *reinterpret_cast<u32x4 *>(sm + S0 + (c & 1) * SCB + tid * 16) = sreg.v;
     };
-    uint8_t sbyte[SPT];
-    auto load_bytes = [&](int c) {
-        if (AL) return;
-        const uint32_t at = (uint32_t)c * 8 + (lane & 7);
-#pragma unroll
-        for (int i = 0; i < SPT; i++)
-            sbyte[i] = wst[(uint32_t)min(i * 32 + wave * 8 + (lane >> 3), O - 1 - o0) * ks + (at < ks ? at : 0)];
-    };
-    auto put_bytes = [&](int c) {
-        if (AL) return;
-#pragma unroll
-        for (int i = 0; i < SPT; i++)
-            sm[S0 + (c & 1) * SCB + (i * 32 + wave * 8 + (lane >> 3)) * 8 + (lane & 7)] = sbyte[i];
-    };
-    // what is copied at the end of stage kt: the activations of stage kt + 2,
-    // a quarter of chunk (kt + 1) / 4 + 1 (its slot's last reader was the
-    // chunk before (kt + 1) / 4's)
-    auto copy_scales_at = [&](int kt) {
-        const int c = (kt + 1) / 4 + 1;
-        if (((kt + 1) & 3) == 0 && c < nch) {
-#pragma unroll
-            for (int i = 0; i < SPW; i++) copy_scales(i, c, -1);
-            load_bytes(c);
-            put_bytes(c);
-        }
-    };
+    // what is copied at the end of stage kt: the activations of stage kt + 2, a
+    // quarter of chunk (kt + 1) / 4 + 1 (its slot's last reader was the chunk
+    // before (kt + 1) / 4's)
+    constexpr int GROUP = XPW + WPW;
     auto copy_at = [&](int i, int kt) {
         if (i < XPW) {
             copy_x(i, kt + 2, (kt + 2 - nk) >> 31);
@@ -433,7 +379,6 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
             copy_w(i - XPW, c, (kt + 1) & 3, (c - nch) >> 31);
         }
     };
-    f32x16 acc[TO][TMM];
 #pragma unroll
     for (int t = 0; t < TO; t++)
 #pragma unroll
@@ -450,7 +395,7 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
         const int c = st >> 2, b = 2 * (st & 3) + g;
         const char *p = sm + W0 + (c & 1) * WB + (wo * TO + t) * 4096 + rrow + ((b ^ (lane & 7)) << 4);
         f.v[t] = *reinterpret_cast<const u32x4 *>(p);
-        f.s[t] = (uint8_t)sm[S0 + (c & 1) * SCB + ((wo * TO + t) * 32 + (lane & 31)) * 8 + b];
+        f.s[t] = (uint8_t)sm[S0 + (st >> 3 & 1) * SCB + ((wo * TO + t) * 32 + (lane & 31)) * 16 + (2 * (st & 7) + g)];
     };
     auto rd_x = [&](int st, int j, int u, Frag &f) {
         const char *p = sm + (st & 1) * XB + (wm * TMM + u) * 4096 + rrow + (((4 * g + j) ^ (lane & 7)) << 4);
@@ -466,7 +411,6 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
                     Raw &wn, auto cpy, int kt) {
         constexpr int J2 = decltype(j2)::value;
         constexpr bool READ = decltype(read)::value, RAW = decltype(raw)::value, COPY = decltype(cpy)::value;
-        constexpr int NC = XPW + WPW;
         if (RAW) {
 #pragma unroll
             for (int t = 0; t < TO; t++) rd_raw(rst, t, wn);
@@ -486,7 +430,7 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
                 fn.a[a] = mx_widen(c, (RAW ? wn : wr).s[a]);
             }
 #pragma unroll
-            for (; COPY && d < NC && d * NF < (i + 1) * NC; d++) copy_at(d, kt);
+            for (; COPY && d < GROUP && d * NF < (i + 1) * GROUP; d++) copy_at(d, kt);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -499,16 +443,8 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
     using i1 = std::integral_constant<int, 1>;
     using i2 = std::integral_constant<int, 2>;
     using i3 = std::integral_constant<int, 3>;
-    // stages 0 and 1, chunk 0 and the first quarter of chunk 1
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-        if (c < nch) {
-            load_bytes(c);
-            put_bytes(c);
-#pragma unroll
-            for (int i = 0; i < SPW; i++) copy_scales(i, c, -1);
-        }
-    }
+    // chunk 0, and what the loop finds under way: stages 0 and 1, a quarter of chunk 1
+    sreg.load(wrow, 0, sleft);
 #pragma unroll
     for (int q = 0; q < 4; q++)
 #pragma unroll
@@ -516,9 +452,9 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
 #pragma unroll
     for (int i = 0; i < XPW; i++) copy_x(i, 0, -1);
 #pragma unroll
-    for (int i = 0; i < XPW + WPW; i++) copy_at(i, -1);
-    if (nk > 1 && nch > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XPW + WPW) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int i = 0; i < GROUP; i++) copy_at(i, -1);
+    put_scales(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(GROUP) : "memory");
     __syncthreads();
     Raw r0, r1;
     Frag f0, f1;
@@ -532,21 +468,23 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
         f0.a[t] = mx_widen(c, r0.s[t]);
     }
     for (int kt = 0; kt < nk - 1; kt++) {
+        const bool sc = (kt & 7) == 0;     // (the slot's last reader was stage kt - 1)
+        if (sc) sreg.load(wrow, min(kt / 8 + 1, nsc - 1), sleft);
         step(f0, f1, yes{}, kt, i1{}, r0, no{}, r1, no{}, 0);
         step(f1, f0, yes{}, kt, i2{}, r0, no{}, r1, no{}, 0);
         step(f0, f1, yes{}, kt, i3{}, r0, no{}, r1, no{}, 0);
-        // this stage's operands have been read by all after the barrier, and
-        // everything in flight, the next stage's copies, has landed
+        // this stage's operands have been read by all after the barrier, and the
+        // next stage's copies have landed
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        copy_scales_at(kt);
+        if (sc) put_scales(kt / 8 + 1);
         step(f1, f0, yes{}, kt + 1, i0{}, r0, yes{}, r1, yes{}, kt);
         r0 = r1;
     }
-    // the last stage; with an odd number of blocks half of it lies past K
-    const bool odd = K % kMx16Stage != 0;
+    // the last stage; half of it, with a second share of K all, may lie past K
+    const bool past = (nk - 1) * kMx16Stage + 32 * g >= K;
     auto mask = [&](Frag &f) {
-        if (!odd || g == 0) return;
+        if (!past) return;
 #pragma unroll
         for (int t = 0; t < TO; t++) f.a[t] = mx_bf16x8{};
 #pragma unroll
@@ -562,34 +500,98 @@ __global__ __launch_bounds__(256, TO * TMM <= 4 ? 2 : 1) void k_mx_gemm_wide16(
     step(f1, f0, no{}, 0, i0{}, r0, no{}, r1, no{}, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    store_tile<TO, TMM>(sm, acc, y, ldy, o0 + wo * TO * 32, m0 + wm * TMM * 32, O, M, wave, lane);
 }
 
-template <int TO, int TMM>
-int launch_mx_wide16(const uint8_t *w, const uint8_t *ws, const uint16_t *x, size_t ldx,
-                     uint16_t *y, size_t ldy, int M, int O, int K) {
-    const unsigned grid = tile_grid((int)cdiv(O, 64 * TO), (int)cdiv(M, 64 * TMM));
-    const bool al = K % 128 == 0 && (uintptr_t)ws % 4 == 0;
-    APUS_TIMED("k_mx_gemm_wide16",
-               if (al) k_mx_gemm_wide16<TO, TMM, true><<<grid, 256, 0, stream()>>>(w, ws, x, ldx, y, ldy, M, O, K);
-               else k_mx_gemm_wide16<TO, TMM, false><<<grid, 256, 0, stream()>>>(w, ws, x, ldx, y, ldy, M, O, K));
-    return launch_check("k_mx_gemm_wide16");
+// ---- a product's tiles ---------------------------------------------------------
+template <bool XMX, int T>
+constexpr int kWideLds = XMX ? kMxLds<T, T> : kMx16Lds<T, T>;
+
+// y of 64 T outputs from o0 x 64 T rows from m0, by 4 wavefronts, or, with G = 2, by 8,
+// each 4 of them with half of K and LDS of their own
+template <bool XMX, int T, int G>
+__device__ __forceinline__ void wide_tile(char *sm, const MxProduct &a, int o0, int m0) {
+    constexpr int LDS = kWideLds<XMX, T>, STAGE = XMX ? kMxStage : kMx16Stage;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = wave >> 2, w = wave & 3;
+    // (the second half may have a stage less, which it takes as one past K)
+    const int nk = ((a.K + STAGE - 1) / STAGE + G - 1) / G, k0 = grp * nk * STAGE;
+    f32x16 acc[T][T];
+    if constexpr (XMX) mx_tile<T, T>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
+    else mx16_tile<T, T>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
+    if constexpr (G == 2) {                // the sum of the halves, in the first's registers
+        char *p = sm + LDS + w * (T * T * 4096) + lane * 16;
+        static_assert(4 * T * T * 4096 <= LDS, "the second half's sums fit its LDS");
+#pragma unroll
+        for (int i = 0; grp == 1 && i < T * T * 4; i++) {
+            const f32x16 &v = acc[i / 4 / T][i / 4 % T];
+            const int q = i % 4 * 4;
+            *reinterpret_cast<mx_f32x4 *>(p + i * 1024) = mx_f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
+        }
+        __syncthreads();
+        if (grp == 1) return;
+#pragma unroll
+        for (int i = 0; i < T * T * 4; i++) {
+            const mx_f32x4 v = *reinterpret_cast<const mx_f32x4 *>(p + i * 1024);
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[i / 4 / T][i / 4 % T][i % 4 * 4 + j] += v[j];
+        }
+    }
+    store_tile<T, T>(sm, acc, a.y, a.ldy, o0 + (w >> 1) * T * 32, m0 + (w & 1) * T * 32, a.O, a.M, w, lane);
+}
+
+// Workgroups [0, big) take a tile of 64 T x 64 T each; four of the others a quarter
+// each of a tile that would be left for a last round of the chip (T = 4 only).
+template <bool XMX, int T, int G>
+__global__ __launch_bounds__(256 * G, T == 2 ? 2 : 1) void k_mx_gemm_wide(MxProduct a, int big) {
+    __shared__ __attribute__((aligned(16))) char sm[G * kWideLds<XMX, T>];
+    int id = blockIdx.x, part = -1;
+    if (T == 4 && id >= big) {             // (a tile's quarters on its XCD: ids 8 apart)
+        const int q = id - big;
+        part = q / 8 % 4;
+        id = big + q / 32 * 8 + q % 8;
+    }
+    const int nbo = (a.O + 64 * T - 1) / (64 * T), nbm = (a.M + 64 * T - 1) / (64 * T);
+    int ob, mb;
+    tile_of(id, nbo, nbm, ob, mb);
+    if (ob >= nbo) return;                               // (the grid is a multiple of 8)
+    int o0 = ob * 64 * T, m0 = mb * 64 * T;
+    if constexpr (T == 4) {
+        if (part >= 0) {
+            o0 += part % 2 * 128;
+            m0 += part / 2 * 128;
+            if (o0 < a.O && m0 < a.M) wide_tile<XMX, 2, 1>(sm, a, o0, m0);
+            return;
+        }
+    }
+    wide_tile<XMX, T, G>(sm, a, o0, m0);
+}
+
+template <bool XMX, int T, int G>
+int launch_wide(const MxProduct &a) {
+    const int n = tile_grid((int)cdiv(a.O, 64 * T), (int)cdiv(a.M, 64 * T));
+    const int big = T == 4 ? n - (int)mx_quarters(n) : n;
+    const unsigned grid = (unsigned)(big + 4 * (n - big));
+    APUS_TIMED("k_mx_gemm_wide", k_mx_gemm_wide<XMX, T, G><<<grid, 256 * G, 0, stream()>>>(a, big));
+    return launch_check("k_mx_gemm_wide");
 }
 
 }  // namespace
 
 namespace apus {
 
-int mx_gemm_wide(const uint8_t *w, const uint8_t *ws, const uint8_t *x, const uint8_t *xs,
-                 uint16_t *y, size_t ldy, int M, int O, int K, int shape) {
-    return shape == 4 ? launch_mx_wide<4, 4>(w, ws, x, xs, y, ldy, M, O, K)
-                      : launch_mx_wide<2, 2>(w, ws, x, xs, y, ldy, M, O, K);
+size_t mx_quarters(size_t tiles) {
+    const size_t cus = (size_t)cu_count() / 8 * 8, last = (tiles + 7) / 8 * 8 % cus;
+    return tiles > cus && last <= cus / 4 ? last : 0;
 }
 
-int mx_gemm_wide16(const uint8_t *w, const uint8_t *ws, const uint16_t *x, size_t ldx, uint16_t *y,
-                   size_t ldy, int M, int O, int K, int shape) {
-    return shape == 4 ? launch_mx_wide16<4, 4>(w, ws, x, ldx, y, ldy, M, O, K)
-                      : launch_mx_wide16<2, 2>(w, ws, x, ldx, y, ldy, M, O, K);
+int mx_gemm_wide(const MxProduct &a, int shape) {
+    // (halves need a stage each)
+    if (shape == 3 && a.K <= (a.xs ? kMxStage : kMx16Stage)) shape = 2;
+    switch (shape) {
+        case 2: return a.xs ? launch_wide<true, 2, 1>(a) : launch_wide<false, 2, 1>(a);
+        case 3: return a.xs ? launch_wide<true, 2, 2>(a) : launch_wide<false, 2, 2>(a);
+        default: return a.xs ? launch_wide<true, 4, 1>(a) : launch_wide<false, 4, 1>(a);
+    }
 }
 
 }  // namespace apus

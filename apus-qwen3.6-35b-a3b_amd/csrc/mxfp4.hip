@@ -203,6 +203,8 @@ unsigned stream_grid(size_t threads) {
 
 // 32-bit offsets reach 256 rows of activations or codes
 constexpr size_t kMxMaxPitch = (size_t)1 << 21;
+// elements of a matrix with its gaps (no extent overflows, tiles count in 32 bits)
+constexpr size_t kMxMaxElements = (size_t)1 << 40;
 
 // Two sets of M rows (first row, bytes between rows, bytes of a row) share
 // bytes. Rows of one pitch may interleave (column slices of one buffer);
@@ -222,6 +224,7 @@ int gemm_check(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t
     if (M == 0 || O == 0) return kOk;
     if (!y) return set_error(kErrArgument, "NULL output");
     if (ldy < O) return set_error(kErrArgument, "output rows of %zu elements with pitch %zu", O, ldy);
+    if (ldy > kMxMaxElements / M) return set_error(kErrUnsupported, "%zu output rows of pitch %zu", M, ldy);
     if ((uintptr_t)y % 2) return set_error(kErrArgument, "misaligned output");
     if (K == 0) return kOk;
     if (!w || !ws || !x) return set_error(kErrArgument, "NULL operand");
@@ -264,10 +267,11 @@ struct FewCost {
 constexpr FewCost kFewCost[] = {{2.5f, 3.6f, 5.6f}, {2.6f, 1.3f, 2.0f}};         // bf16, MXFP4 activations
 struct WideCost {
     float f1, k1, f2, k2;                   // 128 x 128 tiles: one on the busiest CU, two
+    float k3;                               // the same in two halves of K (fixed part f1)
     float f4, k4, fill;                     // 256 x 256: per round; with every CU busy
 };
-constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 7.0f, 43.0f, 16.0f},
-                                  {3.2f, 4.8f, 4.0f, 10.0f, 6.5f, 10.5f, 12.0f}};
+constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 13.5f, 7.0f, 43.0f, 12.0f},
+                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 10.0f}};
 
 size_t rounds(size_t n) { return (n + cu_count() - 1) / cu_count(); }
 
@@ -279,7 +283,7 @@ bool few_pays_two(size_t n2, size_t n1, size_t M) {
     return c.two * rounds(n2) < c.one * rounds(n1);
 }
 
-// The tile shape of the many-row kernel to take, or 0: the few-row one.
+// The shape of the many-row kernel to take, or 0: the few-row one.
 template <bool XMX>
 int wide_shape(size_t M, size_t O, size_t K) {
     const float kk = (float)K / 2048.0f;
@@ -288,12 +292,13 @@ int wide_shape(size_t M, size_t O, size_t K) {
     const size_t nbm = cdiv(M, 64);
     const float few = c.fixed + kk * std::min(c.one * rounds(cdiv(O, 16) * nbm), c.two * rounds(cdiv(O, 32) * nbm));
     const size_t r2 = rounds((size_t)cdiv(O, 128) * cdiv(M, 128));
-    const float w2 = (r2 / 2) * (v.f2 + v.k2 * kk) + (r2 % 2) * (v.f1 + v.k1 * kk);
-    const size_t n4 = (size_t)cdiv(O, 256) * cdiv(M, 256), r4 = rounds(n4);
-    const float w4 = r4 * (v.f4 + v.k4 * kk) +
-                     v.fill * std::min((float)r4, (float)n4 / cu_count());
+    // (one tile a CU: in halves of K, 1000 rows x 4096 x 2048 of bf16 25 -> 21 us)
+    const float w2 = r2 == 1 ? v.f1 + v.k3 * kk : (r2 / 2) * (v.f2 + v.k2 * kk) + (r2 % 2) * (v.f1 + v.k1 * kk);
+    const size_t n4 = (size_t)cdiv(O, 256) * cdiv(M, 256), part = mx_quarters(n4), r4 = rounds(n4 - std::min(n4, part));
+    const float w4 = r4 * (v.f4 + v.k4 * kk) + v.fill * std::min((float)r4, (float)n4 / cu_count()) +
+                     (part ? v.f1 + v.k1 * kk : 0.0f);
     if (few <= w2 && few <= w4) return 0;
-    return w2 <= w4 ? 2 : 4;
+    return w4 < w2 ? 4 : r2 == 1 ? 3 : 2;
 }
 
 template <bool XMX>
@@ -306,11 +311,8 @@ int gemm_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *
     }
     if (M > 32) {
         const int shape = wide_shape<XMX>(M, O, K);
-        if constexpr (XMX) {
-            if (shape) return mx_gemm_wide(w, ws, (const uint8_t *)x, xs, y, ldy, (int)M, (int)O, (int)K, shape);
-        } else {
-            if (shape) return mx_gemm_wide16(w, ws, (const uint16_t *)x, ldx, y, ldy, (int)M, (int)O, (int)K, shape);
-        }
+        if (shape)
+            return mx_gemm_wide({w, ws, x, XMX ? xs : nullptr, ldx, y, ldy, (int)M, (int)O, (int)K}, shape);
     }
     const size_t tiles = cdiv(M, 16), nt = cdiv(tiles, cdiv(tiles, 4)), nbm = cdiv(tiles, nt);
     const bool two = few_pays_two<XMX>(cdiv(O, 32) * nbm, cdiv(O, 16) * nbm, M);
@@ -359,6 +361,7 @@ int apus_hip_mxfp4_quantize(const uint16_t *x, size_t ldx, uint8_t *codes, uint8
     if (M && K) {
         if (!x || !codes || !scales) return set_error(kErrArgument, "NULL operand");
         if (ldx < K) return set_error(kErrArgument, "rows of %zu elements with pitch %zu", K, ldx);
+        if (ldx > kMxMaxElements / M) return set_error(kErrUnsupported, "%zu rows of pitch %zu", M, ldx);
         if ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)codes % 16)
             return set_error(kErrUnsupported, "MXFP4 quantisation needs 16-byte aligned rows and codes");
         if (rows_overlap(x, ldx * 2, K * 2, codes, K / 2, K / 2, M) ||
@@ -381,6 +384,7 @@ int apus_hip_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, uint1
     if (M && K) {
         if (!x || !codes || !scales) return set_error(kErrArgument, "NULL operand");
         if (ldx < K) return set_error(kErrArgument, "rows of %zu elements with pitch %zu", K, ldx);
+        if (ldx > kMxMaxElements / M) return set_error(kErrUnsupported, "%zu rows of pitch %zu", M, ldx);
         if ((uintptr_t)x % 16 || ldx % 8 || (uintptr_t)codes % 16)
             return set_error(kErrUnsupported, "MXFP4 dequantisation needs 16-byte aligned rows and codes");
         if (rows_overlap(x, ldx * 2, K * 2, codes, K / 2, K / 2, M) ||

@@ -46,6 +46,9 @@ def test_quantize_refusals(f):
     assert quant(f=f, c=off(A, 16)) == ARG                 # codes inside x
     assert quant(f=f, s=off(A, 4 * 128 - 1)) == ARG
     assert quant(f=f, M=1 << 31) == UNS
+    assert quant(f=f, K=(1 << 21) + 32, ldx=1 << 22) == UNS
+    assert quant(f=f, M=1 << 30, ldx=1 << 21) == UNS       # past 2^40 elements
+    assert quant(f=f, ldx=1 << 62) == UNS
 
 
 def test_gemm_refusals():
@@ -59,6 +62,9 @@ def test_gemm_refusals():
     for n in ("w", "ws", "x", "y"):
         assert gemm(**{n: None}) == ARG
     assert gemm(O=1 << 31) == UNS
+    assert gemm(K=(1 << 21) + 32, ldx=1 << 22) == UNS
+    assert gemm(ldx=(1 << 21) + 8) == UNS                  # offsets past 32 bits in a tile
+    assert gemm(ldy=1 << 39) == UNS and gemm(ldy=1 << 62) == UNS
     # y among x's rows: in their columns, or with another pitch
     assert gemm(ldx=128, y=off(D, 2 * 63), ldy=128) == ARG
     assert gemm(ldx=128, y=off(D, 2 * 119), ldy=128) == ARG        # wraps into the next row
@@ -98,6 +104,8 @@ def test_moe_refusals():
         assert work(layer(**{n: 48})) == UNS
         assert work(layer(**{n: 1 << 21})) == UNS
     assert work(layer(hidden=0)) == UNS and work(layer(inter=0)) == UNS
+    assert work(layer(inter=1 << 19), T=1024) == UNS       # 4 GiB of h
+    assert work(layer(hidden=1 << 20), T=1024) == UNS
     assert work(layer(), T=0) == UNS and work(layer(), T=1025) == UNS
     lib = apus_hip.load()
     L = layer()
