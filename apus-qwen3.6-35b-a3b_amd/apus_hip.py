@@ -735,10 +735,20 @@ def free_attn_layer(L):
 
 
 # ---- MXFP4
+_BF16 = set()                              # tensor types that hold bf16 values or their codes
+
+
+def _bf16(t):
+    if not _BF16:
+        import torch
+        _BF16.update((torch.bfloat16, torch.int16, torch.uint16))
+    return t.dtype in _BF16
+
+
 def _rows(t, what, dev, ncols=None):
-    """(pointer, rows, columns, pitch) of a 2-D tensor of 2-byte elements on
+    """(pointer, rows, columns, pitch) of a 2-D tensor of bf16 values or codes on
     device dev whose rows are contiguous (any pitch)."""
-    if t.get_device() != dev or t.dim() != 2 or t.element_size() != 2:
+    if t.get_device() != dev or t.dim() != 2 or not _bf16(t):
         raise ValueError(f"{what}: a 2-D tensor of bf16 values or codes on GPU {dev}, not "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     m, n = t.shape
@@ -828,8 +838,9 @@ def moe_layer(dims, w, norm_topk=True):
 
     def take(name, shape, size):
         t = w[name]
-        if not t.is_cuda or not t.is_contiguous() or t.element_size() != size or tuple(t.shape) != shape:
-            raise ValueError(f"{name}: a contiguous GPU tensor of {size}-byte elements of shape {shape}, "
+        if (not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != shape
+                or not (_bf16(t) if size == 2 else t.element_size() == 1)):
+            raise ValueError(f"{name}: a contiguous GPU tensor of {'bf16' if size == 2 else 'bytes'} of shape {shape}, "
                              f"not {tuple(t.shape)} {t.dtype} on {t.device}")
         ptr[name] = t.data_ptr()
 
@@ -867,7 +878,7 @@ def moe_layer_decode(layer, work, x, y):
     dev, H = _gpu(layer._tensors["w_router"], "w_router"), layer.hidden
     for t, n in ((x, "x"), (y, "y")):
         if (t.get_device() != dev or t.shape != x.shape or t.dim() != 2 or t.shape[1] != H
-                or t.element_size() != 2 or not t.is_contiguous()):
+                or not _bf16(t) or not t.is_contiguous()):
             raise ValueError(f"{n}: contiguous [T, {H}] bf16 on GPU {dev}, not {tuple(t.shape)} {t.dtype} "
                              f"on {t.device}")
     _chk(load().apus_hip_moe_layer_decode(C.byref(layer), work.h, x.shape[0], x.data_ptr(), y.data_ptr()))

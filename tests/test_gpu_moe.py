@@ -205,6 +205,10 @@ def test_moe_refusals(hip):
         hip.moe_layer_decode(L, work, x[:2], torch.empty_like(x))
     with pytest.raises(ValueError):                        # weights of another shape
         hip.moe_layer((64, 64, 8, 2, 32), w)
+    with pytest.raises(ValueError):                        # another 2-byte type
+        hip.moe_layer((64, 32, 8, 2, 32), dict(w, w_router=w["w_router"].half()))
+    with pytest.raises(ValueError):
+        hip.moe_layer_decode(L, work, x[:2].half(), torch.empty_like(x[:2]))
     for T in (0, 1025):
         with pytest.raises(hip.ApusHipError) as e:
             hip.MoeWork(L, T)

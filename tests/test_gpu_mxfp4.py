@@ -225,6 +225,10 @@ def test_python_refusals(hip):
         hip.mxfp4_gemm(u8(5, 32), u8(5, 2), bf(4, 64), bf(3, 5))       # rows of y
     with pytest.raises(ValueError):
         hip.mxfp4_gemm(u8(5, 32), u8(5, 2), bf(4, 96), bf(4, 5))       # another K
+    with pytest.raises(ValueError):                                    # another 2-byte type
+        hip.mxfp4_quantize(bf(4, 64).half(), u8(4, 32), u8(4, 2))
+    with pytest.raises(ValueError):
+        hip.mxfp4_gemm(u8(5, 32), u8(5, 2), bf(4, 64), bf(4, 5).half())
     with pytest.raises(hip.ApusHipError) as e:                         # not whole blocks
         hip.mxfp4_quantize(bf(4, 48), u8(4, 24), u8(4, 1))
     assert e.value.code == 1
