@@ -110,7 +110,7 @@ __device__ __forceinline__ float wave_sum(float f) {
 // The logits were written by other workgroups of this launch, and are read where
 // those meet.
 template <int NJ>
-__device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
+__device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane, int *sids) {
     const float *lg = a.logits + (size_t)t * (a.E + 1);
     auto logit = [&](int e) { return __hip_atomic_load(lg + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     float l[NJ];
@@ -164,6 +164,7 @@ __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane) {
         if (pos[j] >= 0) {
             __hip_atomic_store(a.ids + t * a.k + pos[j], lane + 64 * j, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
+            sids[pos[j]] = lane + 64 * j;
             a.wts[t * (a.k + 1) + pos[j]] = p[j] / sum;
         }
     if (lane == 0)
@@ -175,12 +176,12 @@ constexpr int kRouterWaves = 16;
 // The choices of all tokens by expert, by one workgroup: count, sum, place. (In
 // which order an expert's choices come does not matter: a choice's values do not
 // depend on its place.)
-__device__ __forceinline__ void make_slots(const MoeArgs &a, int lane, int wave) {
+__device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, int lane, int wave) {
     __shared__ int cursor[kMoeMaxExperts], wsum[2][kRouterWaves];
     constexpr int THREADS = 64 * kRouterWaves, KEEP = 4;
     const int tid = threadIdx.x, n = a.T * a.k;
-    auto id = [&](int q) {                 // (chosen by other workgroups of this launch)
-        const int e = __hip_atomic_load(a.ids + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    auto id = [&](int q) {                 // from LDS, or as chosen by other workgroups of this launch
+        const int e = sids ? sids[q] : __hip_atomic_load(a.ids + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return min(max(e, 0), a.E - 1);    // (in range whatever ids holds)
     };
     int mine[KEEP];                        // the first ids, read once
@@ -239,7 +240,7 @@ static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
 template <int NJ>
 __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
     __shared__ mx_f32x4 red[kRouterWaves][64];
-    __shared__ int last;
+    __shared__ int last, sids[16 * kMoeMaxTopk];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int E1 = a.E + 1, t0 = blockIdx.y * 16;
@@ -285,13 +286,17 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
     }
     __syncthreads();
     if (!last) return;
-    if (t0 + wave < a.T) choose<NJ>(a, t0 + wave, lane);
+    if (t0 + wave < a.T) choose<NJ>(a, t0 + wave, lane, sids + wave * a.k);
     if (a.T <= kFewTokens) return;
+    if (gridDim.y == 1) {                  // (one workgroup has chosen for all)
+        __syncthreads();
+        return make_slots(a, sids, lane, wave);
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) count(a.done + gridDim.y, gridDim.y);
     __syncthreads();
-    if (last) make_slots(a, lane, wave);
+    if (last) make_slots(a, nullptr, lane, wave);
 }
 
 // ---- experts ----------------------------------------------------------------
