@@ -239,7 +239,7 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
 static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
 template <int NJ>
 __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
-    __shared__ mx_f32x4 red[kRouterWaves][64];
+    __shared__ __attribute__((aligned(16))) char sm[kRouterWaves * WBf16::kTile];
     __shared__ int last, sids[16 * kMoeMaxTopk];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -248,21 +248,27 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
     const bool gate = a.w_sgate && blockIdx.x == gridDim.x - 1;
     const int e0 = gate ? a.E : blockIdx.x * 16, ne = gate ? 1 : min(16, a.E - e0);
     const auto wt = gate ? WBf16::tile(a.w_sgate, nullptr, 0, 1, a.H) : WBf16::tile(a.w_router, nullptr, e0, ne, a.H);
-    const auto wl = WBf16::lane(lane, a.H);
+    const auto wl = WBf16::raw_lane(lane, a.H);
     using X = XBf16<WBf16>;
     const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
-    const uint32_t xl = X::lane((uint32_t)(t0 + r) * (uint32_t)a.H * 2, g);
+    uint32_t xl[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) xl[i] = (uint32_t)(t0 + 4 * i + g) * (uint32_t)a.H * 2;
+    char *const m = sm + wave * WBf16::kTile;
     mx_f32x4 acc{};
     for (int st = wave; st * 128 < a.H; st += kRouterWaves) {
-        WBf16::Frag wf;
-        X::Frag xf;
-        WBf16::load(wf, wt, wl, st, a.H);
-        X::load(xf, xb, xl, st, a.H);
+        WBf16::Raw wf;
+        RowsBf16::Raw xf;
+        WBf16::load_raw(wf, wt, wl, st, a.H);
+        X::load_raw(xf, xb, xl, st, a.H);
+        WBf16::Frag f;
+        WBf16::put(m, wf, lane);
+        WBf16::get(f, m, wf, lane);
+        RowsBf16::put(m, xf, lane);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            acc = mfma16(WBf16::operand(wf, j), __builtin_bit_cast(mx_bf16x8, xf.v[j]), acc);
+        for (int j = 0; j < 4; j++) acc = mfma16(WBf16::operand(f, j), X::piece(m, j, lane), acc);
     }
-    red[wave][lane] = acc;
+    *reinterpret_cast<mx_f32x4 *>(m + lane * 16) = acc;
     __syncthreads();
     auto count = [&](uint32_t *done, uint32_t of) {      // thread 0: the last of `of`?
         const uint32_t n = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -272,7 +278,8 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
     if (wave == 0) {
         mx_f32x4 s[4] = {};
 #pragma unroll
-        for (int i = 0; i < kRouterWaves; i++) s[i & 3] += red[i][lane];
+        for (int i = 0; i < kRouterWaves; i++)
+            s[i & 3] += *reinterpret_cast<const mx_f32x4 *>(sm + i * WBf16::kTile + lane * 16);
         acc = (s[0] + s[1]) + (s[2] + s[3]);
         if (t0 + r < a.T) {
 #pragma unroll
@@ -354,9 +361,10 @@ constexpr int kMoeWaves = 8;
 // h = silu(gate x) * (up x): 16 outputs a workgroup, 16 rows at a time
 template <class W>
 __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, int nper) {
-    __shared__ mx_f32x4 red[kMoeWaves * 2][64];
-    __shared__ int rows[16];
     constexpr int S = 2;                   // steps in flight at once
+    constexpr int LDS = W::kTile < 2048 ? 2048 : W::kTile;
+    __shared__ __attribute__((aligned(16))) char sm[kMoeWaves * LDS];
+    __shared__ int rows[16];
     using X = XBf16<W>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -369,19 +377,22 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, i
     for (int i = 0; i < 2; i++)
         wt[i] = W::tile(sh ? a.w_sgu : a.w_gu, sh ? a.s_sgu : a.s_gu,
                         (sh ? 0 : (size_t)task.e * 2 * I) + i * I + o0, 16, a.H);
-    const auto wl = W::lane(lane, a.H);
+    const auto wl = W::raw_lane(lane, a.H);
     const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
+    char *const m = sm + wave * LDS;
     for (int c = 0; c < task.n; c += 16) {
         const int q = choice(task, c + r);
+        // (each lane its own row: of few rows most lanes read the same one)
         const uint32_t xl = X::lane((uint32_t)(sh ? q - a.T * a.k : q / a.k) * (uint32_t)a.H * 2, g);
+        if (c) __syncthreads();                          // the sums have been read
         mx_f32x4 acc[2] = {};
         for (int st = wave * S; st * 128 < a.H; st += kMoeWaves * S) {
-            typename W::Frag fw[S][2];
+            typename W::Raw fw[S][2];
             typename X::Frag fx[S];
 #pragma unroll
             for (int s = 0; s < S; s++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) W::load(fw[s][i], wt[i], wl, st + s, a.H);
+                for (int i = 0; i < 2; i++) W::load_raw(fw[s][i], wt[i], wl, st + s, a.H);
 #pragma unroll
             for (int s = 0; s < S; s++) X::load(fx[s], xb, xl, st + s, a.H);
             // (all loads issued before the first use)
@@ -390,14 +401,17 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, i
 #pragma unroll
             for (int s = 0; s < S; s++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int i = 0; i < 2; i++) {
+                    typename W::Frag f;
+                    W::put(m, fw[s][i], lane);
+                    W::get(f, m, fw[s][i], lane);
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        acc[i] = mfma16(W::operand(fw[s][i], j), __builtin_bit_cast(mx_bf16x8, fx[s].v[j]), acc[i]);
+                    for (int j = 0; j < 4; j++)
+                        acc[i] = mfma16(W::operand(f, j), __builtin_bit_cast(mx_bf16x8, fx[s].v[j]), acc[i]);
+                }
         }
-        if (c) __syncthreads();                          // red's readers are done
-        red[wave * 2][lane] = acc[0];
-        red[wave * 2 + 1][lane] = acc[1];
+#pragma unroll
+        for (int i = 0; i < 2; i++) *reinterpret_cast<mx_f32x4 *>(m + i * 1024 + lane * 16) = acc[i];
         if (wave == 0 && g == 0) rows[r] = q;
         __syncthreads();
         // a thread finishes one output of a row, 16 outputs of a row side by side
@@ -408,7 +422,8 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, i
             for (int w = 0; w < kMoeWaves; w++)
 #pragma unroll
                 for (int i = 0; i < 2; i++)
-                    s[i] += reinterpret_cast<const float *>(&red[w * 2 + i][(o >> 2) * 16 + row])[o & 3];
+                    s[i] += *reinterpret_cast<const float *>(sm + w * LDS + i * 1024 + ((o >> 2) * 16 + row) * 16 +
+                                                             (o & 3) * 4);
             uint16_t *h = a.h + h_at(a, rows[row], sh) + o0 + o;
             split_h(silu(s[0]) * s[1], h[0], h[I]);
         }
@@ -423,8 +438,8 @@ __host__ __device__ constexpr int down_rows(int I) { return kMoeWaves / down_spl
 // part[choice] = down h: 32 outputs a group of wavefronts, 16 rows at a time
 template <class W>
 __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh, int nper) {
-    constexpr int RT = 2;
-    __shared__ mx_f32x4 red[kMoeWaves * RT][64];
+    constexpr int RT = 2, LDS = RowsBf16::kTile;
+    __shared__ __attribute__((aligned(16))) char sm[kMoeWaves * LDS];
     __shared__ int rows[16];
     using X = XBf16<W>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -439,33 +454,52 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
     for (int t = 0; t < RT; t++)
         wt[t] = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn,
                         (sh ? 0 : (size_t)task.e * a.H) + min(o0 + (rg * RT + t) * 16, a.H - 16), 16, I);
-    const auto wl = W::lane(lane, I);
+    const auto wl = W::raw_lane(lane, I);
     const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
+    char *const m = sm + wave * LDS;
     for (int c = 0; c < task.n; c += 16) {
         const int q = choice(task, c + r);
-        const uint32_t xl = X::lane(h_at(a, q, sh) * 2, g);
+        uint32_t hl[4], ll[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            hl[i] = h_at(a, choice(task, c + 4 * i + g), sh) * 2;
+            ll[i] = hl[i] + I * 2;
+        }
+        if (c) __syncthreads();                          // the sums have been read
         mx_f32x4 acc[RT] = {};
         for (int st = kw; st * 128 < I; st += ks) {
-            typename W::Frag fw[RT];
-            typename X::Frag fh, fl;
+            typename W::Raw fw[RT];
+            RowsBf16::Raw fh, fl;
 #pragma unroll
-            for (int t = 0; t < RT; t++) W::load(fw[t], wt[t], wl, st, I);
-            X::load(fh, hb, xl, st, I);
-            X::load(fl, hb, xl + I * 2, st, I);
+            for (int t = 0; t < RT; t++) W::load_raw(fw[t], wt[t], wl, st, I);
+            X::load_raw(fh, hb, hl, st, I);
+            X::load_raw(fl, hb, ll, st, I);
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
+            typename W::Frag f[RT];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int t = 0; t < RT; t++) {
+                W::put(m, fw[t], lane);
+                W::get(f[t], m, fw[t], lane);
+            }
+            mx_bf16x8 h[4];
+            RowsBf16::put(m, fh, lane);
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[j] = X::piece(m, j, lane);
+            RowsBf16::put(m, fl, lane);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const mx_bf16x8 lo = X::piece(m, j, lane);
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
-                    const mx_bf16x8 wv = W::operand(fw[t], j);
-                    acc[t] = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fh.v[j]), acc[t]);
-                    acc[t] = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fl.v[j]), acc[t]);
+                    const mx_bf16x8 wv = W::operand(f[t], j);
+                    acc[t] = mfma16(wv, h[j], acc[t]);
+                    acc[t] = mfma16(wv, lo, acc[t]);
                 }
+            }
         }
-        if (c) __syncthreads();                          // red's readers are done
 #pragma unroll
-        for (int t = 0; t < RT; t++) red[wave * RT + t][lane] = acc[t];
+        for (int t = 0; t < RT; t++) *reinterpret_cast<mx_f32x4 *>(m + t * 1024 + lane * 16) = acc[t];
         if (wave == 0 && g == 0) rows[r] = q;
         __syncthreads();
         // a thread finishes 4 outputs of a row
@@ -473,8 +507,9 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
             const int l = e & 63, t = (e >> 6) % RT, x = (e >> 6) / RT;
             const int o = o0 + (x * RT + t) * 16;
             if (c + (l & 15) >= task.n || o >= a.H) continue;
-            mx_f32x4 s = red[x * ks * RT + t][l];
-            for (int y = 1; y < ks; y++) s += red[(x * ks + y) * RT + t][l];
+            const char *p = sm + x * ks * LDS + t * 1024 + l * 16;
+            mx_f32x4 s = *reinterpret_cast<const mx_f32x4 *>(p);
+            for (int y = 1; y < ks; y++) s += *reinterpret_cast<const mx_f32x4 *>(p + y * LDS);
             *reinterpret_cast<mx_f32x4 *>(a.part + (size_t)rows[l & 15] * a.H + o + 4 * (l >> 4)) = s;
         }
     }
@@ -716,7 +751,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a
 constexpr int kFewWaves = 12;
 template <class W>
 __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
-    __shared__ mx_f32x4 red[kFewWaves][64];
+    __shared__ __attribute__((aligned(16))) char sm[kFewWaves * W::kTile];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = blockIdx.x * 16, n = a.T * a.k;
@@ -724,6 +759,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
     const int units = n * si + (a.Is ? a.T * ss : 0);
     constexpr int U = 3;
     using X = XBf16<W>;
+    char *const m = sm + wave * W::kTile;
     const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
     mx_f32x4 acc{};
     for (int b = wave; b < units; b += kFewWaves * U) {
@@ -743,7 +779,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
             p[i] = a.wts[t * (a.k + 1) + (sh[i] ? a.k : q[i] % a.k)];
             on[i] = live && t == r;
         }
-        typename W::Frag fw[U];
+        typename W::Raw fw[U];
         typename X::Frag fh[U], fl[U];
 #pragma unroll
         for (int i = 0; i < U; i++) {
@@ -757,28 +793,31 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
             const int I = sh[i] ? a.Is : a.I, x = __builtin_amdgcn_readfirstlane(e[i]);
             const auto wt = W::tile(sh[i] ? a.w_sdn : a.w_dn, sh[i] ? a.s_sdn : a.s_dn,
                                     (sh[i] ? 0 : (size_t)x * a.H) + o0, 16, I);
-            W::load(fw[i], wt, W::lane(lane, I), st[i], I);
+            W::load_raw(fw[i], wt, W::raw_lane(lane, I), st[i], I);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < U; i++) {
             mx_f32x4 d{};
+            typename W::Frag f;
+            W::put(m, fw[i], lane);
+            W::get(f, m, fw[i], lane);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const mx_bf16x8 wv = W::operand(fw[i], j);
+                const mx_bf16x8 wv = W::operand(f, j);
                 d = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fh[i].v[j]), d);
                 d = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fl[i].v[j]), d);
             }
             if (on[i]) acc += d * p[i];
         }
     }
-    red[wave][lane] = acc;
+    *reinterpret_cast<mx_f32x4 *>(m + lane * 16) = acc;
     __syncthreads();
     if (wave || r >= a.T) return;
     mx_f32x4 s[4] = {};
 #pragma unroll
-    for (int i = 0; i < kFewWaves; i++) s[i & 3] += red[i][lane];
+    for (int i = 0; i < kFewWaves; i++) s[i & 3] += *reinterpret_cast<const mx_f32x4 *>(sm + i * W::kTile + lane * 16);
     acc = (s[0] + s[1]) + (s[2] + s[3]);
     *reinterpret_cast<ushort4 *>(a.y + (size_t)r * a.H + o0 + 4 * g) =
         make_ushort4(f2bf(acc[0]), f2bf(acc[1]), f2bf(acc[2]), f2bf(acc[3]));
