@@ -107,12 +107,8 @@ __device__ __forceinline__ float wave_sum(float f) {
 // l + 64, ... The k-th largest key is found two bits at a time from the top,
 // counting by ballots (k rounds of a maximum over the wavefront took 8 us, this
 // takes about one); of the keys equal to it the lowest indices are taken.
-// The logits were written by other workgroups of this launch, and are read where
-// those meet.
-template <int NJ>
-__device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane, int *sids) {
-    const float *lg = a.logits + (size_t)t * (a.E + 1);
-    auto logit = [&](int e) { return __hip_atomic_load(lg + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+template <int NJ, class Logit>
+__device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane, int *sids, Logit logit) {
     float l[NJ];
     uint32_t key[NJ], best = 0;            // key 0: past E
 #pragma unroll
@@ -229,25 +225,31 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
     for (int q = tid + KEEP * THREADS; q < n; q += THREADS) a.list[atomicAdd(&cursor[id(q)], 1)] = (uint16_t)q;
 }
 
-// 16 experts (the shared gate as one more) x 16 tokens a workgroup, K over its
-// 16 wavefronts. The last workgroup of the 16 tokens to finish chooses for them, a
-// wavefront each, and with more than a few tokens the last of those sorts the
-// choices: what a workgroup hands on it stores where all XCDs see it, waits for the
-// stores, and counts itself; nobody waits for anybody. (One token: 8.2 us, 4.2 of
-// them to the logits. Choosing in every workgroup of the next launch instead costs
-// that launch as much as is saved here, 4 us, most of it fetching the code.)
+// ET tiles of 16 experts (the shared gate's one row is a tile of its own) x 16
+// tokens a workgroup, K over its 16 / ET wavefronts of a tile. The last workgroup
+// of the 16 tokens to finish chooses for them, a wavefront each, and with more than
+// a few tokens the last of those sorts the choices: what a workgroup hands on it
+// stores where all XCDs see it, waits for the stores, and counts itself; nobody
+// waits for anybody. (One token of 2048, 256 experts: 6.6 us. Choosing in every
+// workgroup of the next launch instead costs that launch as much as is saved here.)
+// Of up to kSmallTiles tiles one workgroup takes all, and hands nothing on.
+constexpr int kSmallTiles = 4;
 static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
-template <int NJ>
+int router_tiles(const MoeArgs &a) { return (a.E + 15) / 16 + (a.w_sgate ? 1 : 0); }
+template <int NJ, int ET>
 __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
+    constexpr int KW = kRouterWaves / ET;
     __shared__ __attribute__((aligned(16))) char sm[kRouterWaves * WBf16::kTile];
     __shared__ int last, sids[16 * kMoeMaxTopk];
+    __shared__ float slog[ET == 1 ? 1 : 16 * (16 * ET + 1)];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int E1 = a.E + 1, t0 = blockIdx.y * 16;
-    // the last workgroup of a shared gate takes its one row, as expert E
-    const bool gate = a.w_sgate && blockIdx.x == gridDim.x - 1;
-    const int e0 = gate ? a.E : blockIdx.x * 16, ne = gate ? 1 : min(16, a.E - e0);
-    const auto wt = gate ? WBf16::tile(a.w_sgate, nullptr, 0, 1, a.H) : WBf16::tile(a.w_router, nullptr, e0, ne, a.H);
+    const int ntiles = (a.E + 15) / 16 + (a.w_sgate ? 1 : 0), tile = ET == 1 ? blockIdx.x : wave / KW;
+    const bool gate = a.w_sgate && tile == ntiles - 1;
+    const int e0 = gate ? a.E : tile * 16, ne = tile >= ntiles ? 0 : gate ? 1 : min(16, a.E - e0);
+    const auto wt = gate ? WBf16::tile(a.w_sgate, nullptr, 0, 1, a.H)
+                         : WBf16::tile(a.w_router, nullptr, min(e0, a.E - 1), ne, a.H);
     const auto wl = WBf16::raw_lane(lane, a.H);
     using X = XBf16<WBf16>;
     const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
     for (int i = 0; i < 4; i++) xl[i] = (uint32_t)(t0 + 4 * i + g) * (uint32_t)a.H * 2;
     char *const m = sm + wave * WBf16::kTile;
     mx_f32x4 acc{};
-    for (int st = wave; st * 128 < a.H; st += kRouterWaves) {
+    for (int st = wave % KW; st * 128 < a.H && ne; st += KW) {
         WBf16::Raw wf;
         RowsBf16::Raw xf;
         WBf16::load_raw(wf, wt, wl, st, a.H);
@@ -270,30 +272,45 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
     }
     *reinterpret_cast<mx_f32x4 *>(m + lane * 16) = acc;
     __syncthreads();
+    if (wave % KW == 0) {                  // the logits of a tile: expert 4 g + i of it, token r
+        mx_f32x4 s[4] = {};
+#pragma unroll
+        for (int i = 0; i < KW; i++) s[i & 3] += *reinterpret_cast<const mx_f32x4 *>(m + i * WBf16::kTile + lane * 16);
+        acc = (s[0] + s[1]) + (s[2] + s[3]);
+    }
     auto count = [&](uint32_t *done, uint32_t of) {      // thread 0: the last of `of`?
         const uint32_t n = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         last = n == of - 1;
         if (last) *done = 0;                             // for the next call
     };
-    if (wave == 0) {
-        mx_f32x4 s[4] = {};
+    if constexpr (ET == 1) {
+        if (wave == 0) {
+            if (t0 + r < a.T) {
 #pragma unroll
-        for (int i = 0; i < kRouterWaves; i++)
-            s[i & 3] += *reinterpret_cast<const mx_f32x4 *>(sm + i * WBf16::kTile + lane * 16);
-        acc = (s[0] + s[1]) + (s[2] + s[3]);
-        if (t0 + r < a.T) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (4 * g + i < ne)
-                    __hip_atomic_store(a.logits + (size_t)(t0 + r) * E1 + e0 + 4 * g + i, acc[i],
-                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (int i = 0; i < 4; i++)
+                    if (4 * g + i < ne)
+                        __hip_atomic_store(a.logits + (size_t)(t0 + r) * E1 + e0 + 4 * g + i, acc[i],
+                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (lane == 0) count(a.done + blockIdx.y, gridDim.x);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (lane == 0) count(a.done + blockIdx.y, gridDim.x);
+        __syncthreads();
+        if (!last) return;
+        const float *lg = a.logits + (size_t)(t0 + wave) * E1;
+        if (t0 + wave < a.T)
+            choose<NJ>(a, t0 + wave, lane, sids + wave * a.k, [&](int e) {
+                return __hip_atomic_load(lg + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            });
+    } else {
+        constexpr int P = 16 * ET + 1;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (wave % KW == 0 && 4 * g + i < ne) slog[r * P + e0 + 4 * g + i] = acc[i];
+        __syncthreads();
+        if (t0 + wave < a.T)
+            choose<NJ>(a, t0 + wave, lane, sids + wave * a.k, [&](int e) { return slog[wave * P + e]; });
     }
-    __syncthreads();
-    if (!last) return;
-    if (t0 + wave < a.T) choose<NJ>(a, t0 + wave, lane, sids + wave * a.k);
     if (a.T <= kFewTokens) return;
     if (gridDim.y == 1) {                  // (one workgroup has chosen for all)
         __syncthreads();
@@ -748,7 +765,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a
 // token: 3 each, all on their way at once). A step's product lands in the token's
 // column with the expert's weight; the columns of other tokens (all multiplied
 // with this token's h) are left out.
-constexpr int kFewWaves = 12;
+constexpr int kFewWaves = 12, kFewUnits = 3;
 template <class W>
 __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
     __shared__ __attribute__((aligned(16))) char sm[kFewWaves * W::kTile];
@@ -756,8 +773,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = blockIdx.x * 16, n = a.T * a.k;
     const int si = (a.I + 127) / 128, ss = (a.Is + 127) / 128;
-    const int units = n * si + (a.Is ? a.T * ss : 0);
-    constexpr int U = 3;
+    const int units = n * si + a.T * ss;
+    constexpr int U = kFewUnits;
     using X = XBf16<W>;
     char *const m = sm + wave * W::kTile;
     const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
@@ -893,10 +910,11 @@ template <class W>
 int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
     const bool one = a.T <= 16;            // no slot has more than 16 rows
-    const bool ups = slots * a.I / 16 >= 1024 && (W::mx || a.T * a.k >= 4 * a.E);
+    const bool ups = slots * a.I / 16 >= 1024 && (W::mx || a.T * a.k >= a.E);
     if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, 2>(a, slots))
         return r;
-    if (a.T <= kFewTokens) {
+    const int units = a.T * (a.k * cdiv(a.I, 128) + cdiv(a.Is, 128));
+    if (a.T <= kFewTokens || (a.T <= 16 && units <= kFewWaves * kFewUnits)) {
         APUS_TIMED("k_moe_down_few", k_moe_down_few<W><<<(unsigned)a.H / 16, 64 * kFewWaves, 0, stream()>>>(a));
         return launch_check("k_moe_down_few");
     }
@@ -1044,9 +1062,12 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.Is = (int)L->shared_inter;
     a.norm = L->norm_topk;
     a.nslots = (int)(T <= kFewTokens ? T * L->topk : moe_slots(T, L->topk, L->experts));
-    const dim3 rg(cdiv(L->experts, 16) + (a.w_sgate ? 1 : 0), cdiv(T, 16));
-    APUS_TIMED("k_moe_router", if (a.E <= 256) k_moe_router<4><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
-               else k_moe_router<16><<<rg, 64 * kRouterWaves, 0, stream()>>>(a));
+    const int tiles = router_tiles(a);
+    const dim3 rg(tiles <= kSmallTiles ? 1 : tiles, cdiv(T, 16));
+    APUS_TIMED("k_moe_router",
+               if (tiles <= kSmallTiles) k_moe_router<1, kSmallTiles><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
+               else if (a.E <= 256) k_moe_router<4, 1><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
+               else k_moe_router<16, 1><<<rg, 64 * kRouterWaves, 0, stream()>>>(a));
     APUS_LAUNCHED("k_moe_router");
     return L->mxfp4 ? experts_run<WMx>(a) : experts_run<WBf16>(a);
 }
