@@ -40,15 +40,15 @@ struct ApusHipMoeWork {
     float *part;         // [T topk + T][hidden]
     uint32_t *done;      // workgroups of k_moe_router done, per 16 tokens, then of
                          // those the ones that have chosen (0 between calls)
-    int4 *slots;         // expert, first of its choices in list, how many (up to kGroup)
+    int4 *slots;         // expert, first of its choices in list, how many (up to a.group)
     uint16_t *list;      // [T topk]: choices by expert
 };
 
 namespace {
 
 constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
+constexpr size_t kWideSlots = 8;
 constexpr int kFewTokens = 2;          // up to here a choice is a slot of its own
-constexpr int kGroup = 32;             // most rows of a slot
 
 struct MoeArgs {
     const uint16_t *x, *w_router, *w_sgate;
@@ -62,11 +62,12 @@ struct MoeArgs {
     uint16_t *h;
     uint16_t *y;
     int T, H, I, E, k, Is, norm, nslots;
+    int group;             // most rows of a slot: 16 or 32
 };
 
 // ---- router ---------------------------------------------------------------
 // slots that T tokens can fill
-size_t moe_slots(size_t T, size_t k, size_t E) { return std::min(T * k, E) + T * k / kGroup; }
+size_t moe_slots(size_t T, size_t k, size_t E, size_t group) { return std::min(T * k, E) + T * k / group; }
 
 // Order of logits as unsigned numbers: NaN above all, -0 and +0 alike. No
 // number's key is 0.
@@ -191,7 +192,7 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
     for (int q = tid + KEEP * THREADS; q < n; q += THREADS) atomicAdd(&cursor[id(q)], 1);
     __syncthreads();
     // thread e: running sums over the experts, of the choices and of the slots
-    const int c = cursor[tid], k = (c + kGroup - 1) / kGroup;
+    const int c = cursor[tid], k = (c + a.group - 1) / a.group;
     int at = c, slot = k;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -215,7 +216,7 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
         total += wsum[1][w];
     }
     for (int i = 0; i < k; i++)
-        a.slots[slot - k + i] = make_int4(tid, at - c + i * kGroup, min(kGroup, c - i * kGroup), 0);
+        a.slots[slot - k + i] = make_int4(tid, at - c + i * a.group, min(a.group, c - i * a.group), 0);
     for (int i = total + tid; i < a.nslots; i += THREADS) a.slots[i] = make_int4(0, 0, 0, 0);
     cursor[tid] = at - c;
     __syncthreads();
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
 // ---- experts ----------------------------------------------------------------
 // What a workgroup works on: n rows of the activations, for the expert's row
 // blocks. Blocks of a launch: first the shared expert's, nsh row blocks for
-// every kGroup tokens; then nper row blocks per slot. A slot is up to kGroup of
+// every a.group tokens; then nper row blocks per slot. A slot is up to a.group of
 // an expert's choices (a popular expert has several, side by side on the chip
 // instead of one after the other), or with few tokens a choice.
 struct Task {
@@ -334,10 +335,10 @@ struct Task {
     const uint16_t *list;                  // or null: choices first, first + 1, ..
 };
 __device__ __forceinline__ Task task_of(const MoeArgs &a, int b, int nsh, int nper) {
-    const int groups = nsh ? (a.T + kGroup - 1) / kGroup : 0;
+    const int groups = nsh ? (a.T + a.group - 1) / a.group : 0;
     if (b < nsh * groups) {
-        const int t = b / nsh * kGroup;
-        return {a.E, b % nsh, a.T * a.k + t, min(kGroup, a.T - t), nullptr};
+        const int t = b / nsh * a.group;
+        return {a.E, b % nsh, a.T * a.k + t, min(a.group, a.T - t), nullptr};
     }
     b -= nsh * groups;
     const int slot = b / nper, part = b % nper;
@@ -857,7 +858,7 @@ __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a) {
     *reinterpret_cast<ushort4 *>(a.y + (size_t)t * a.H + c) = o;
 }
 
-// the launch of an expert kernel: nsh row parts of the shared expert per kGroup
+// the launch of an expert kernel: nsh row parts of the shared expert per a.group
 // tokens, nper of every slot
 struct Grid {
     int nsh, nper;
@@ -865,7 +866,7 @@ struct Grid {
 };
 Grid grid_of(const MoeArgs &a, size_t slots, size_t nper, size_t nsh) {
     if (!a.Is) nsh = 0;
-    return {(int)nsh, (int)nper, (unsigned)(nsh * cdiv(a.T, kGroup) + slots * nper)};
+    return {(int)nsh, (int)nper, (unsigned)(nsh * cdiv(a.T, a.group) + slots * nper)};
 }
 
 template <class W>
@@ -909,7 +910,7 @@ int down_stream_run(const MoeArgs &a, size_t slots) {
 template <class W>
 int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
-    const bool one = a.T <= 16;            // no slot has more than 16 rows
+    const bool one = a.group == 16;
     const bool ups = slots * a.I / 16 >= 1024 && (W::mx || a.T * a.k >= a.E);
     if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, 2>(a, slots))
         return r;
@@ -983,7 +984,7 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
                  wts = take(T * (k + 1) * 4), 
                  h = take(hs),
                  part = take(T * (k + 1) * L->hidden * 4), done = take(((T + 15) / 16 + 1) * 4),
-                 slots = take(moe_slots(T, k, L->experts) * 16), list = take(T * k * 2);
+                 slots = take(moe_slots(T, k, L->experts, 16) * 16), list = take(T * k * 2);
     if (hipMalloc((void **)&w->base, n) != hipSuccess) {
         delete w;
         return set_error(kErrHip, "hipMalloc of %zu bytes failed", n);
@@ -1061,7 +1062,8 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.k = (int)L->topk;
     a.Is = (int)L->shared_inter;
     a.norm = L->norm_topk;
-    a.nslots = (int)(T <= kFewTokens ? T * L->topk : moe_slots(T, L->topk, L->experts));
+    a.group = T * L->topk <= kWideSlots * L->experts ? 16 : 32;
+    a.nslots = (int)(T <= kFewTokens ? T * L->topk : moe_slots(T, L->topk, L->experts, a.group));
     const int tiles = router_tiles(a);
     const dim3 rg(tiles <= kSmallTiles ? 1 : tiles, cdiv(T, 16));
     APUS_TIMED("k_moe_router",
