@@ -564,7 +564,8 @@ __device__ __forceinline__ void walk(int n, Load load, Mul mul) {
     walk_on<D>(n, mul);
 }
 
-template <class W, int RT, int NT, int D>
+// XR: loads of four rows that a tile of activations takes (1 for up to 4 rows)
+template <class W, int RT, int NT, int D, int XR>
 __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, int o0, char *m, int lane) {
     using X = XBf16<W>;
     const int r = lane & 15, g = lane >> 4;
@@ -599,7 +600,7 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
 #pragma unroll
             for (int i = 0; i < 2; i++) W::load_raw(fw[d][t][i], wt[t][i], wl, st, a.H);
 #pragma unroll
-        for (int u = 0; u < NT; u++) X::load_raw(fx[d][u], xb, xl[u], st, a.H);
+        for (int u = 0; u < NT; u++) X::template load_raw<XR>(fx[d][u], xb, xl[u], st, a.H);
     };
     mx_f32x4 acc[RT][2][NT] = {};
     walk<D>((a.H + 127) / 128, load, [&](int d, int st) {
@@ -655,8 +656,9 @@ __global__ __launch_bounds__(64 * kStreamWaves, W::mx ? 3 : 2) void k_moe_up_str
     const Task task = task_of(a, blockIdx.x, nsh, nper);
     const int o0 = (task.part * kStreamWaves + wave) * 16 * RT;
     if (task.n == 0 || o0 >= (task.e == a.E ? a.Is : a.I)) return;       // (no barrier in this kernel)
-    if (NT > 1 && task.n > 16) up_stream<W, RT, NT, 2>(a, task, o0, sm + wave * LDS, lane);
-    else up_stream<W, RT, 1, 2>(a, task, o0, sm + wave * LDS, lane);
+    if (NT > 1 && task.n > 16) up_stream<W, RT, NT, 2, 4>(a, task, o0, sm + wave * LDS, lane);
+    else if (task.n > 4) up_stream<W, RT, 1, 2, 4>(a, task, o0, sm + wave * LDS, lane);
+    else up_stream<W, RT, 1, 2, 1>(a, task, o0, sm + wave * LDS, lane);
 }
 
 // part[choice] = down h: 16 RT outputs a block, P blocks a wavefront in one walk.
