@@ -564,8 +564,9 @@ __device__ __forceinline__ void walk(int n, Load load, Mul mul) {
     walk_on<D>(n, mul);
 }
 
-// XR: loads of four rows that a tile of activations takes (1 for up to 4 rows)
-template <class W, int RT, int NT, int D, int XR>
+// XR: loads of four rows that a tile of activations takes (1 for up to 4 rows). SC:
+// MXFP4 weights' scales in strips.
+template <class W, int RT, int NT, int D, int XR, bool SC>
 __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, int o0, char *m, int lane) {
     using X = XBf16<W>;
     const int r = lane & 15, g = lane >> 4;
@@ -593,12 +594,19 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
     }
     typename W::Raw fw[D][RT][2];
     RowsBf16::Raw fx[D][NT];
-    char *const mx = m + RT * 2 * W::kTile;
+    char *const mx = m + RT * 2 * W::kTile, *const ms = mx + NT * RowsBf16::kTile;
+    Strip strip[SC ? RT * 2 : 1];
     auto load = [&](int d, int st) {
+        if constexpr (SC) {
+            if ((st & (Strip::kSteps - 1)) == 0) {
+#pragma unroll
+                for (int t = 0; t < RT * 2; t++) strip[t].load(wt[t / 2][t % 2], st, a.H);
+            }
+        }
 #pragma unroll
         for (int t = 0; t < RT; t++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) W::load_raw(fw[d][t][i], wt[t][i], wl, st, a.H);
+            for (int i = 0; i < 2; i++) W::template load_raw<!SC>(fw[d][t][i], wt[t][i], wl, st, a.H);
 #pragma unroll
         for (int u = 0; u < NT; u++) X::template load_raw<XR>(fx[d][u], xb, xl[u], st, a.H);
     };
@@ -610,7 +618,15 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
         for (int u = 0; u < NT; u++) RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u], lane);
         typename W::Frag f[RT][2];
 #pragma unroll
-        for (int t = 0; t < RT * 2; t++) W::get(f[t / 2][t % 2], m + t * W::kTile, fw[d][t / 2][t % 2], lane);
+        for (int t = 0; t < RT * 2; t++) W::template get<!SC>(f[t / 2][t % 2], m + t * W::kTile, fw[d][t / 2][t % 2], lane);
+        if constexpr (SC) {
+            if ((st & (Strip::kSteps - 1)) == 0) {
+#pragma unroll
+                for (int t = 0; t < RT * 2; t++) strip[t].put(ms + t * Strip::kTile);
+            }
+#pragma unroll
+            for (int t = 0; t < RT * 2; t++) f[t / 2][t % 2].s = Strip::get(ms + t * Strip::kTile, st, lane);
+        }
         fence();
         load(d, st + D);
         fence();
@@ -647,18 +663,18 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
     }
 }
 
-template <class W, int RT, int NT>
+template <class W, int RT, int NT, bool SC>
 __global__ __launch_bounds__(64 * kStreamWaves, W::mx ? 3 : 2) void k_moe_up_stream(MoeArgs a, int nsh, int nper) {
-    constexpr int LDS = RT * 2 * W::kTile + NT * RowsBf16::kTile;
+    constexpr int LDS = RT * 2 * (W::kTile + (SC ? Strip::kTile : 0)) + NT * RowsBf16::kTile;
     __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = task_of(a, blockIdx.x, nsh, nper);
     const int o0 = (task.part * kStreamWaves + wave) * 16 * RT;
     if (task.n == 0 || o0 >= (task.e == a.E ? a.Is : a.I)) return;       // (no barrier in this kernel)
-    if (NT > 1 && task.n > 16) up_stream<W, RT, NT, 2, 4>(a, task, o0, sm + wave * LDS, lane);
-    else if (task.n > 4) up_stream<W, RT, 1, 2, 4>(a, task, o0, sm + wave * LDS, lane);
-    else up_stream<W, RT, 1, 2, 1>(a, task, o0, sm + wave * LDS, lane);
+    if (NT > 1 && task.n > 16) up_stream<W, RT, NT, 2, 4, SC>(a, task, o0, sm + wave * LDS, lane);
+    else if (task.n > 4) up_stream<W, RT, 1, 2, 4, SC>(a, task, o0, sm + wave * LDS, lane);
+    else up_stream<W, RT, 1, 2, 1, SC>(a, task, o0, sm + wave * LDS, lane);
 }
 
 // part[choice] = down h: 16 RT outputs a block, P blocks a wavefront in one walk.
@@ -888,7 +904,8 @@ int up_stream_run(const MoeArgs &a, size_t slots) {
     const int rows = 16 * kStreamWaves;
     const Grid g = grid_of(a, slots, cdiv(a.I, rows), cdiv(a.Is, rows));
     APUS_TIMED("k_moe_up_stream",
-               k_moe_up_stream<W, 1, NT><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper));
+               if (W::mx && a.H % 128 == 0) k_moe_up_stream<W, 1, NT, W::mx><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper);
+               else k_moe_up_stream<W, 1, NT, false><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper));
     return launch_check("k_moe_up_stream");
 }
 template <class W, int NT>

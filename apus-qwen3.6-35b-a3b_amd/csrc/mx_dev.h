@@ -41,6 +41,8 @@ __device__ __forceinline__ mx_bf16x8 mx_widen(uint32_t c, uint32_t s) {
 // under the size: the check subtracts it).
 __device__ f32x4_t llvm_raw_buffer_load_v4f32(i32x4 r, int voff, int soff, int aux)
     __asm("llvm.amdgcn.raw.buffer.load.v4f32");
+__device__ float llvm_raw_buffer_load_f32(i32x4 r, int voff, int soff, int aux)
+    __asm("llvm.amdgcn.raw.buffer.load.f32");
 __device__ uint8_t llvm_raw_buffer_load_u8(i32x4 r, int voff, int soff, int aux)
     __asm("llvm.amdgcn.raw.buffer.load.i8");
 constexpr uint32_t kPast = 0x7fffffff;       // an offset past every tile
@@ -115,6 +117,7 @@ struct WBf16 {
     static __device__ __forceinline__ Lane raw_lane(int l, int K) {
         return {(uint32_t)(l >> 4) * (uint32_t)K * 2 + (l & 15) * 16};
     }
+    template <bool S = true>
     static __device__ __forceinline__ void load_raw(Raw &f, const Tile &t, const Lane &l, int step, int K) {
         const int k = step * 128;
         const bool live = k + 8 * (int)(threadIdx.x & 15) < K;
@@ -123,6 +126,7 @@ struct WBf16 {
             f.v[i] = ld16(t.w, live ? l.off + 8 * i * (uint32_t)K : kPast, k < K ? k * 2 : 0);
     }
     static __device__ __forceinline__ void put(char *m, const Raw &f, int l) { RowsBf16::put(m, f, l); }
+    template <bool S = true>
     static __device__ __forceinline__ void get(Frag &f, const char *m, const Raw &, int l) {
 #pragma unroll
         for (int j = 0; j < 4; j++) f.v[j] = RowsBf16::piece(m, 4 * j + (l >> 4), l);
@@ -151,11 +155,12 @@ struct WMx {
     }
     static __device__ __forceinline__ Lane lane(int l, int K) { return at(l & 15, l >> 4, K); }
     // block: this lane's of the step (past K: zero codes, at the scale 2^-127)
+    template <bool S = true>
     static __device__ __forceinline__ void load_block(Frag &f, const Tile &t, const Lane &l, int step, int block, int K) {
         const int k = step * 128;
         const bool live = k + 32 * block < K;
         f.v = ld16(t.w, live ? l.off : kPast, k < K ? k / 2 : 0);
-        f.s = llvm_raw_buffer_load_u8(t.s, (int)(live ? l.soff : kPast), k < K ? k / kMxBlock : 0, 0);
+        if (S) f.s = llvm_raw_buffer_load_u8(t.s, (int)(live ? l.soff : kPast), k < K ? k / kMxBlock : 0, 0);
     }
     static __device__ __forceinline__ void load(Frag &f, const Tile &t, const Lane &l, int step, int K) {
         load_block(f, t, l, step, (threadIdx.x >> 4) & 3, K);
@@ -163,19 +168,50 @@ struct WMx {
     static __device__ __forceinline__ mx_bf16x8 operand(const Frag &f, int j) {
         return mx_widen(f.v[j], f.s);
     }
-    // 4 lanes a row; the scales go between lanes without LDS memory
+    // 4 lanes a row; the scales go between lanes without LDS memory, or (S false) are
+    // brought in strips (Strip)
     static __device__ __forceinline__ Lane raw_lane(int l, int K) { return at(l >> 2, l & 3, K); }
+    template <bool S = true>
     static __device__ __forceinline__ void load_raw(Raw &f, const Tile &t, const Lane &l, int step, int K) {
-        load_block(f, t, l, step, threadIdx.x & 3, K);
+        load_block<S>(f, t, l, step, threadIdx.x & 3, K);
     }
     static __device__ __forceinline__ void put(char *m, const Raw &f, int l) {
         const int row = l >> 2;
         *reinterpret_cast<u32x4 *>(m + row * 64 + (((l & 3) ^ (row >> 2)) << 4)) = f.v;
     }
+    template <bool S = true>
     static __device__ __forceinline__ void get(Frag &f, const char *m, const Raw &raw, int l) {
         const int r = l & 15, g = l >> 4;
         f.v = *reinterpret_cast<const u32x4 *>(m + r * 64 + ((g ^ (r >> 2)) << 4));
-        f.s = (uint32_t)__builtin_amdgcn_ds_bpermute((r * 4 + g) * 4, (int)raw.s);
+        if (S) f.s = (uint32_t)__builtin_amdgcn_ds_bpermute((r * 4 + g) * 4, (int)raw.s);
+    }
+};
+
+// The scales of 16 steps (64 bytes a row) of a tile's 16 rows, through LDS of the
+// wavefront's own: a byte a lane and step took the streaming kernels a seventh of
+// their time. Rows in whole words (K a multiple of 128); past K zero.
+struct Strip {
+    static constexpr int kTile = 1024, kSteps = 16;
+    uint32_t v[4];
+    __device__ __forceinline__ void load(const WMx::Tile &t, int step, int K) {
+        const uint32_t l = threadIdx.x & 63, w = l & 15, ks = (uint32_t)K / kMxBlock, at = 4 * step;   // step: a multiple of kSteps
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+            v[i] = __builtin_bit_cast(uint32_t, llvm_raw_buffer_load_f32(
+                t.s, (int)(at + 4 * w < ks ? (4 * i + l / 16) * ks + 4 * w : kPast), at < ks ? (int)at : 0, 0));
+    }
+    // word w of row r at w ^ r
+    __device__ __forceinline__ void put(char *m) const {
+        const uint32_t l = threadIdx.x & 63;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t row = 4 * i + l / 16;
+            *reinterpret_cast<uint32_t *>(m + row * 64 + (((l & 15) ^ row) << 2)) = v[i];
+        }
+    }
+    // the scale of lane group g's block in a step, for row l % 16
+    static __device__ __forceinline__ uint32_t get(const char *m, int step, int l) {
+        return (uint8_t)m[(l & 15) * 64 + (((step & (kSteps - 1)) ^ (l & 15)) << 2) + (l >> 4)];
     }
 };
 
