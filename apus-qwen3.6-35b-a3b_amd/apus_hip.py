@@ -193,8 +193,13 @@ def _dp(t):
     return _vp(t.data_ptr())
 
 
+_device = 0                                # the library's GPU
+
+
 def init(device=0):
+    global _device
     err = C.create_string_buffer(512)
+    _device = device
     rc = load().apus_hip_init(C.c_int(device), err, 512)
     if rc != 0:
         raise ApusHipError(rc, err.value.decode(errors="replace"))
@@ -769,10 +774,10 @@ def _bytes(t, rows, cols, what, dev):
 
 
 def _gpu(t, what):
-    """The index of t's GPU."""
+    """The index of t's GPU, which is the library's."""
     dev = t.get_device()
-    if dev < 0:
-        raise ValueError(f"{what}: a GPU tensor, not one on {t.device}")
+    if dev != _device:
+        raise ValueError(f"{what}: a tensor on GPU {_device}, not on {t.device}")
     return dev
 
 

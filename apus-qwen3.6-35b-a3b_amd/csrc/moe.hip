@@ -8,15 +8,24 @@
 //
 // For few tokens the layer is the reading of the chosen experts' weights, so
 // every kernel streams weights through the MFMA with tokens as its 16 columns.
-// Launches: k_moe_router, logits and, by the last workgroup of each 16 tokens
-// to finish, the choice; k_moe_up, gate, up and silu of every (expert, 16
-// outputs); then either k_moe_down, down of every (expert, 64 outputs) into
-// fp32 partial rows, and k_moe_combine, their weighted sum, or for up to
-// kFewTokens tokens k_moe_down_few, both in one.
+// Launches:
+//   k_moe_router     logits; by the last workgroup of each 16 tokens to finish the
+//                    choice, by the last of those the choices in order of experts
+//   k_moe_up[_stream]   h = silu(gate) up of every (expert, 16 outputs)
+//   k_moe_down[_stream] fp32 rows of every (expert, 32 outputs), and
+//   k_moe_combine       their weighted sum; or for little work
+//   k_moe_down_few      both in one.
 // The intermediate h = silu(g) u goes to the down product as two bf16 numbers
 // (its leading 8 bits and the rest rounded to 8), which keeps 16 bits of it: the
 // product reads weights, not h, so the second MFMA costs no time, and a single
 // bf16 h would put an error of a bf16 rounding into y beside y's own.
+//
+// Times below: hidden 2048, 256 experts of 512 inner elements, 8 a token, a shared
+// expert of 512, inputs other than the call before's. The whole layer, us at
+// 1 / 5 / 16 / 64 / 325 tokens: MXFP4 19 / 39 / 60 / 107 / 160 (bytes alone, at a
+// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 26 / 69 / 143 / 287 / 342
+// (11 / 51 / 127 / 272 / 314): with many choices it is bound by the weights' bytes,
+// with few by three launches' latency.
 #include <stdint.h>
 
 #include <algorithm>
@@ -32,6 +41,7 @@ using namespace apus;
 // The device buffers of calls on one layer shape, and the shape they fit.
 struct ApusHipMoeWork {
     size_t max_tokens, hidden, inter, experts, topk, shared;
+    int device;
     char *base = nullptr;
     float *logits;       // [T][E + 1]: the experts', then the shared gate's
     int32_t *ids;        // [T][topk]
@@ -40,15 +50,21 @@ struct ApusHipMoeWork {
     float *part;         // [T topk + T][hidden]
     uint32_t *done;      // workgroups of k_moe_router done, per 16 tokens, then of
                          // those the ones that have chosen (0 between calls)
-    int4 *slots;         // expert, first of its choices in list, how many (up to a.group)
+    int4 *slots;         // expert, first of its choices in list, how many (up to group)
     uint16_t *list;      // [T topk]: choices by expert
 };
 
 namespace {
 
 constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
+// Choices an expert from which slots have up to 32 rows, not 16: the kernel for 16
+// has fewer registers and more wavefronts, but reads the weights of an expert with
+// more rows again (MXFP4, us with 16 | 32: 24 tokens 82 | 86, 96 tokens 127 | 131;
+// bf16, 325 tokens 360 | 351).
 constexpr size_t kWideSlots = 8;
-constexpr int kFewTokens = 2;          // up to here a choice is a slot of its own
+// Up to here a choice is a slot of its own, and nothing is sorted (MXFP4, us with 1 | 2
+// | 4: 2 tokens 29 | 26 | 26, 4 tokens 35 | 35 | 42).
+constexpr int kFewTokens = 2;
 
 struct MoeArgs {
     const uint16_t *x, *w_router, *w_sgate;
@@ -106,8 +122,8 @@ __device__ __forceinline__ float wave_sum(float f) {
 
 // A wavefront's choice for token t, in index order: lane l holds logits l,
 // l + 64, ... The k-th largest key is found two bits at a time from the top,
-// counting by ballots (k rounds of a maximum over the wavefront took 8 us, this
-// takes about one); of the keys equal to it the lowest indices are taken.
+// counting by ballots (of 8 of 256, k rounds of a maximum over the wavefront took
+// 8 us, this takes about one); of the keys equal to it the lowest indices are taken.
 template <int NJ, class Logit>
 __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane, int *sids, Logit logit) {
     float l[NJ];
@@ -170,9 +186,9 @@ __device__ __forceinline__ void choose(const MoeArgs &a, int t, int lane, int *s
 
 constexpr int kRouterWaves = 16;
 
-// The choices of all tokens by expert, by one workgroup: count, sum, place. (In
-// which order an expert's choices come does not matter: a choice's values do not
-// depend on its place.)
+// The choices of all tokens by expert, by one workgroup: count, sum, place (2.5 us).
+// In which order an expert's choices come does not matter: a choice's values do not
+// depend on its place.
 __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, int lane, int wave) {
     __shared__ int cursor[kMoeMaxExperts], wsum[2][kRouterWaves];
     constexpr int THREADS = 64 * kRouterWaves, KEEP = 4;
@@ -231,9 +247,10 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
 // of the 16 tokens to finish chooses for them, a wavefront each, and with more than
 // a few tokens the last of those sorts the choices: what a workgroup hands on it
 // stores where all XCDs see it, waits for the stores, and counts itself; nobody
-// waits for anybody. (One token of 2048, 256 experts: 6.6 us. Choosing in every
-// workgroup of the next launch instead costs that launch as much as is saved here.)
-// Of up to kSmallTiles tiles one workgroup takes all, and hands nothing on.
+// waits for anybody. Bound by latency: 7 us for one token, 12 for 16, 14 for 64, 21
+// for 325. (Choosing in every workgroup of the next launch instead costs that launch
+// as much as is saved here.) Of up to kSmallTiles tiles one workgroup takes all, and
+// hands nothing on: 13 tokens of 1056, 20 experts, 7 us, 9 with the hand-over.
 constexpr int kSmallTiles = 4;
 static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
 int router_tiles(const MoeArgs &a) { return (a.E + 15) / 16 + (a.w_sgate ? 1 : 0); }
@@ -327,7 +344,7 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
 // ---- experts ----------------------------------------------------------------
 // What a workgroup works on: n rows of the activations, for the expert's row
 // blocks. Blocks of a launch: first the shared expert's, nsh row blocks for
-// every a.group tokens; then nper row blocks per slot. A slot is up to a.group of
+// every `group` tokens; then nper row blocks per slot. A slot is up to `group` of
 // an expert's choices (a popular expert has several, side by side on the chip
 // instead of one after the other), or with few tokens a choice.
 struct Task {
@@ -374,9 +391,13 @@ __device__ __forceinline__ void split_h(float v, uint16_t &hi, uint16_t &lo) {
 // bytes on their way at once for a task, for calls with few of them. Where the
 // row blocks are enough wavefronts to fill the chip, in k_moe_up_stream and
 // k_moe_down_stream each walks all of K for its rows by itself.
+// In all of them weights come along their rows (load_raw) and become operands in the
+// wavefront's own LDS; loaded by each lane for itself they took the address unit four
+// times as long (one token: 31 us for the layer, now 26; MXFP4 23, now 19).
 constexpr int kMoeWaves = 8;
 
-// h = silu(gate x) * (up x): 16 outputs a workgroup, 16 rows at a time
+// h = silu(gate x) * (up x): 16 outputs a workgroup, 16 rows at a time. One token: 11
+// us for bf16's 38 MB, 4.5 for MXFP4's 10 MB: latency of one round of loads.
 template <class W>
 __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, int nper) {
     constexpr int S = 2;                   // steps in flight at once
@@ -453,7 +474,8 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, i
 __host__ __device__ constexpr int down_split(int I) { return I > 512 ? 8 : I > 256 ? 4 : I > 128 ? 2 : 1; }
 __host__ __device__ constexpr int down_rows(int I) { return kMoeWaves / down_split(I) * 32; }
 
-// part[choice] = down h: 32 outputs a group of wavefronts, 16 rows at a time
+// part[choice] = down h: 32 outputs a group of wavefronts, 16 rows at a time (13 tokens
+// of 1056, 20 experts of 224: 4.4 us)
 template <class W>
 __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh, int nper) {
     constexpr int RT = 2, LDS = RowsBf16::kTile;
@@ -534,8 +556,10 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
 }
 
 // ---- the same, a wavefront alone: no partial sums, no barrier, and D steps of
-// weights and activations on their way all along its walk. Rows come along their
-// length and become operands in LDS of the wavefront's own.
+// weights and activations on their way all along its walk. Up: bf16, 325 tokens, 200
+// us for 1.07 GB, 5.4 TB/s; MXFP4, 64 tokens, 53 us for 247 MB, 4.7 TB/s. Down: 126
+// us for 0.54 GB, 4.3 TB/s; 32 us for 124 MB, 3.9 TB/s. More steps on their way (3, 4)
+// changed nothing, nor did whole 128-byte lines of MXFP4 codes a load.
 constexpr int kStreamWaves = 4;
 
 constexpr int kDownH = 32 * 1024;      // LDS bytes that k_moe_down_stream has for h of 16 rows
@@ -779,11 +803,11 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a
     else down_stream<W, RT, 1, 2>(a, task, b0, nb, h, sm + wave * LDS, lane);
 }
 
-// y of up to kFewTokens tokens: 16 outputs a workgroup, the steps of 128 k of
-// every (token, expert) dealt to its 12 wavefronts (9 experts of 4 steps, one
-// token: 3 each, all on their way at once). A step's product lands in the token's
-// column with the expert's weight; the columns of other tokens (all multiplied
-// with this token's h) are left out.
+// y of up to 16 tokens: 16 outputs a workgroup, the steps of 128 k of every (token,
+// expert) dealt to its 12 wavefronts (9 experts of 4 steps, one token: 3 each, all on
+// their way at once). A step's product lands in the token's column with the
+// expert's weight; the columns of other tokens (all multiplied with this token's h)
+// are left out. One token: 7.8 us for bf16's 19 MB, 6.4 for MXFP4's 5 MB.
 constexpr int kFewWaves = 12, kFewUnits = 3;
 template <class W>
 __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
@@ -859,7 +883,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
         make_ushort4(f2bf(acc[0]), f2bf(acc[1]), f2bf(acc[2]), f2bf(acc[3]));
 }
 
-// y = rnd(sum over the choices, in order, then the shared expert)
+// y = rnd(sum over the choices, in order, then the shared expert): bytes, 4.6 us for 64
+// tokens, 7 for 325 (27 MB)
 __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a) {
     const int H4 = a.H / 4;
     const int i = blockIdx.x * 256 + threadIdx.x;
@@ -876,7 +901,7 @@ __global__ __launch_bounds__(256) void k_moe_combine(MoeArgs a) {
     *reinterpret_cast<ushort4 *>(a.y + (size_t)t * a.H + c) = o;
 }
 
-// the launch of an expert kernel: nsh row parts of the shared expert per a.group
+// the launch of an expert kernel: nsh row parts of the shared expert per `group`
 // tokens, nper of every slot
 struct Grid {
     int nsh, nper;
@@ -921,11 +946,13 @@ int down_stream_run(const MoeArgs &a, size_t slots) {
     return launch_check("k_moe_down_stream");
 }
 
-// The streaming forms from 1024 wavefronts on (4 a CU; hidden 2048, inter 512,
-// MXFP4, us for the layer split | streamed: 5 tokens 41 | 38, 16 tokens 76 | 57, 64
-// tokens 130 | 97). bf16 weights' up product is 4 times the bytes a step, which
-// the split form keeps on their way as well with few rows a slot (64 tokens 129 |
-// 136 us, 325 tokens 245 | 190).
+// The streaming forms from 1024 wavefronts on, 4 a CU (the layer, us split | streamed;
+// up, MXFP4: 16 tokens 65 | 60, 64 tokens 121 | 107, 325 tokens 182 | 160; down: 5 tokens
+// 44 | 39, 64 tokens 133 | 107). bf16 weights' up product is 4 times the bytes a step,
+// which the split form keeps on their way as well with few rows a slot (16 tokens 143 |
+// 150, 64 tokens 297 | 287, 325 tokens 396 | 359). Streaming down needs h of a slot in
+// LDS. k_moe_down_few for work that one round of loads covers (one token: 25 us with the
+// two kernels, 19 with it; bf16 35 and 29), and for kFewTokens (29 and 26).
 template <class W>
 int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
@@ -987,11 +1014,11 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
     if (!max_tokens || max_tokens > kMoeMaxTokens)
         return set_error(kErrUnsupported, "a mixture-of-experts call takes 1 .. %zu tokens (%zu)",
                          kMoeMaxTokens, max_tokens);
-    const size_t hs = max_tokens * (L->topk * L->inter + L->shared_inter) * 4;
+    const size_t hs = max_tokens * (L->topk * L->inter + L->shared_inter) * 4;   // (offsets are 32 bits)
     if (hs > 0x7fff0000u || max_tokens * L->hidden * 2 > 0x7fff0000u)
         return set_error(kErrUnsupported, "mixture-of-experts intermediates of up to 2 GiB");
     if (int r = mx_ready()) return r;
-    auto *w = new ApusHipMoeWork{max_tokens, L->hidden, L->inter, L->experts, L->topk, L->shared_inter};
+    auto *w = new ApusHipMoeWork{max_tokens, L->hidden, L->inter, L->experts, L->topk, L->shared_inter, current_device()};
     const size_t T = max_tokens, k = L->topk;
     size_t n = 0;
     auto take = [&](size_t bytes) {
@@ -1000,15 +1027,16 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
         return at;
     };
     const size_t logits = take(T * (L->experts + 1) * 4), ids = take(T * k * 4),
-                 wts = take(T * (k + 1) * 4), 
-                 h = take(hs),
+                 wts = take(T * (k + 1) * 4), h = take(hs),
                  part = take(T * (k + 1) * L->hidden * 4), done = take(((T + 15) / 16 + 1) * 4),
                  slots = take(moe_slots(T, k, L->experts, 16) * 16), list = take(T * k * 2);
     if (hipMalloc((void **)&w->base, n) != hipSuccess) {
         delete w;
         return set_error(kErrHip, "hipMalloc of %zu bytes failed", n);
     }
-    if (hipMemset(w->base + done, 0, ((T + 15) / 16 + 1) * 4) != hipSuccess) {
+    // (the counters are clear before any stream's first call)
+    if (hipMemset(w->base + done, 0, ((T + 15) / 16 + 1) * 4) != hipSuccess ||
+        hipStreamSynchronize(nullptr) != hipSuccess) {
         (void)hipFree(w->base);
         delete w;
         return set_error(kErrHip, "clearing the workspace failed");
@@ -1052,6 +1080,8 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
             return set_error(kErrUnsupported, "x and y need 16-byte alignment");
     }
     if (int r = mx_ready()) return r;
+    if (w->device != current_device())
+        return set_error(kErrArgument, "the workspace is on device %d, the library on %d", w->device, current_device());
     if (!T) return kOk;
     MoeArgs a{};
     a.x = x;

@@ -1,6 +1,12 @@
-// mx_wide.hip -- products with MXFP4 weights for many rows: tiles of 64 TO
-// outputs x 64 TMM rows, 4 wavefronts (2 x 2), one per SIMD, on the 32-wide
-// MFMAs.
+// mx_wide.hip -- products y[m][o] = rnd(sum_k w[o][k] x[m][k]) with MXFP4 weights for
+// many rows: tiles of 64 TO outputs x 64 TMM rows, 4 wavefronts (2 x 2), one per SIMD,
+// on the 32-wide MFMAs; w and x are copied to LDS without registers and read there.
+//
+// 4096 rows x 12352 outputs, K 2048, 207 Gflop: bf16 x 180 us, 1.15 Pflop/s (a large
+// bf16 library product reaches 1.32 here); MXFP4 x 82 us, 2.5 Pflop/s. With K 8192, 590
+// and 223 us for 825 Gflop, 1.40 and 3.7 Pflop/s. There the chip's MFMA rate under load
+// is the bound: the same loop without copies and LDS reads takes 195 of the 223 us.
+// With K 2048 a fixed part of a tile, its first copies and its 128 KB of y, is a third.
 #include <stdint.h>
 
 #include <type_traits>
@@ -145,8 +151,10 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
     const int nsc = (min(nk, (K + kMxStage - 1) / kMxStage) + 1) / 2;
     // tile-relative, so that 32-bit offsets do (rows past O or M read the last
     // row; their products are not stored)
-    const uint8_t *const wt = a.w + (size_t)o0 * kc + k0 / 2, *const xt = (const uint8_t *)a.x + (size_t)m0 * kc + k0 / 2;
-    const uint8_t *const wst = a.ws + (size_t)o0 * ks + k0 / kMxBlock, *const xst = a.xs + (size_t)m0 * ks + k0 / kMxBlock;
+    const uint8_t *const wt = a.w + (size_t)o0 * kc + k0 / 2;
+    const uint8_t *const xt = (const uint8_t *)a.x + (size_t)m0 * kc + k0 / 2;
+    const uint8_t *const wst = a.ws + (size_t)o0 * ks + k0 / kMxBlock;
+    const uint8_t *const xst = a.xs + (size_t)m0 * ks + k0 / kMxBlock;
     auto row_of = [&](int r) {                           // stage row -> row of its operand's tile
         return r < BO ? min(r, O - 1 - o0) : min(r - BO, M - 1 - m0);
     };
@@ -543,7 +551,11 @@ __device__ __forceinline__ void wide_tile(char *sm, const MxProduct &a, int o0, 
 }
 
 // Workgroups [0, big) take a tile of 64 T x 64 T each; four of the others a quarter
-// each of a tile that would be left for a last round of the chip (T = 4 only).
+// each of a tile that would be left for a last round of the chip (T = 4 only; 4096 rows x
+// 12352 outputs, K 2048, 784 tiles on 256 CUs: 101 us, 90 with the last 16 in quarters;
+// bf16 x 220 and 206). G = 2 where the tiles are at most one a CU, whose 4 wavefronts
+// alone leave its MFMAs waiting: 512 rows x 4096 x 4096, bf16 x, 44 us, 33 with 8; MXFP4
+// x 15.1 and 13.6.
 template <bool XMX, int T, int G>
 __global__ __launch_bounds__(256 * G, T == 2 ? 2 : 1) void k_mx_gemm_wide(MxProduct a, int big) {
     __shared__ __attribute__((aligned(16))) char sm[G * kWideLds<XMX, T>];

@@ -33,7 +33,8 @@ __device__ __forceinline__ Pos pos_of(size_t i, size_t per_row, bool dense) {
 // is 2^(floor(log2 max|x|) - 2), e2m1's largest exponent being 2, from the
 // exponent field of the largest code (a subnormal maximum: the smallest scale,
 // 2^-127); the hardware conversion rounds to nearest even and saturates at 6.
-// A block with an infinity or NaN gets scale 255 (NaN) and zero codes.
+// A block with an infinity or NaN gets scale 255 (NaN) and zero codes. Bytes: 12352
+// rows of 2048 in 10.2 us, 64 MB, 6.3 TB/s; one row 1.2 us, all launch.
 __global__ __launch_bounds__(256) void k_mx_quantize(const uint16_t *__restrict__ x, size_t ldx,
                                                      uint8_t *__restrict__ codes,
                                                      uint8_t *__restrict__ scales, size_t n8,
@@ -62,6 +63,7 @@ __global__ __launch_bounds__(256) void k_mx_quantize(const uint16_t *__restrict_
     }
 }
 
+// 8 elements a thread, their scale read with them. 12352 rows of 2048: 9.8 us.
 __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict__ codes,
                                                        const uint8_t *__restrict__ scales,
                                                        uint16_t *__restrict__ x, size_t ldx,
@@ -77,8 +79,11 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict
 // A workgroup forms 16 RT outputs x 16 NT rows; its 8 wavefronts take every
 // eighth pair of steps of 128 k, all their loads on the way before the first is
 // used, and their partial sums meet in LDS. Rows come along their length and
-// become operands in LDS of the wavefront's own (mx_dev.h). XR: the loads of four
+// become operands in LDS of the wavefront's own (mx_dev.h): loaded by each lane for
+// itself the product of 37 rows took 10.5 us, now 7.1. XR: the loads of four
 // rows that a tile of bf16 activations has (1 for up to 4 rows).
+// Bound by the latency of a round of loads: 1 row x 12352 outputs, K 2048, 5.7 us for
+// 13.5 MB; 37 rows x 2048 x 4096, 7.1 us; 64 rows of MXFP4 x 2048 x 4096, 5.7 us.
 constexpr int kFewWaves = 8;
 
 template <bool XMX, int RT, int NT, int XR>
@@ -257,10 +262,10 @@ int few_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *x
     return launch_check("k_mx_gemm_few");
 }
 
-// Estimated times in us of the product's forms, from what they take over 512 ..
-// 12352 outputs x 48 .. 1024 rows and K = 2048, 4096 (within 15 % nearly all over
-// that range). What a form takes goes by the workgroups of the busiest CU and, but
-// for a fixed part, by K.
+// Estimated times in us of the product's forms. What a form takes goes by the
+// workgroups of the busiest CU and, but for a fixed part, by K. Over 512 .. 12352
+// outputs x 48 .. 4096 rows and K 1024 .. 4096 (105 sizes, both kinds of activations)
+// the form with the least estimate was within a tenth of the best one measured.
 struct FewCost {
     float fixed, one, two;                  // one, two: tiles of 16 and 32 outputs x 64 rows
 };
@@ -294,7 +299,8 @@ int wide_shape(size_t M, size_t O, size_t K) {
     const size_t r2 = rounds((size_t)cdiv(O, 128) * cdiv(M, 128));
     // (one tile a CU: in halves of K, 1000 rows x 4096 x 2048 of bf16 25 -> 21 us)
     const float w2 = r2 == 1 ? v.f1 + v.k3 * kk : (r2 / 2) * (v.f2 + v.k2 * kk) + (r2 % 2) * (v.f1 + v.k1 * kk);
-    const size_t n4 = (size_t)cdiv(O, 256) * cdiv(M, 256), part = mx_quarters(n4), r4 = rounds(n4 - std::min(n4, part));
+    const size_t n4 = (size_t)cdiv(O, 256) * cdiv(M, 256), part = mx_quarters(n4);
+    const size_t r4 = rounds(n4 - std::min(n4, part));
     const float w4 = r4 * (v.f4 + v.k4 * kk) + v.fill * std::min((float)r4, (float)n4 / cu_count()) +
                      (part ? v.f1 + v.k1 * kk : 0.0f);
     if (few <= w2 && few <= w4) return 0;

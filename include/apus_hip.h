@@ -577,9 +577,11 @@ int apus_hip_attn_layer_decode_paged(const ApusHipAttnLayer *L, const ApusHipAtt
  * scales [rows][K/32], dense. Device pointers; codes and bf16 rows 16-byte
  * aligned. ldx / ldy: elements from one bf16 row to the next (ldx a
  * multiple of 8), so that a column slice of a wider buffer can be given. An
- * output may not overlap an input. No host data, no scratch: a call may be
- * captured into a graph, and calls on different data may run at once. Bad
- * arguments are refused with or without a device. */
+ * output may not overlap an input. K and a product's ldx up to 2^21, rows times
+ * pitch up to 2^40. No host data, no scratch: a call may be captured into a
+ * graph, and calls on different data may run at once. Bad arguments are refused
+ * with or without a device, and a call from a thread whose current device is
+ * not the library's is refused. */
 
 /* x [M][K] bf16 -> codes, scales. The scale is 2^(floor(log2 of the
  * block's largest magnitude) - 2), at least 2^-127; elements round to
@@ -628,7 +630,9 @@ typedef struct {
 } ApusHipMoeLayer;
 
 /* The device buffers of calls of up to max_tokens (<= 1024) tokens on layers
- * of this one's sizes (its weights are not looked at). Calls that share one
+ * of this one's sizes (its weights are not looked at): sizes up to 2^20, and at
+ * most 2 GiB each of x and of the inner rows, max_tokens * (topk * inter +
+ * shared_inter) * 4 bytes. Calls that share one
  * run one after the other: on one stream, or ordered by the caller; calls or
  * graph replays that may overlap need one each. It must outlive the graphs
  * that captured its calls. destroy waits for the library's stream. */
