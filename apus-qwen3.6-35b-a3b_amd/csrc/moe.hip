@@ -928,9 +928,12 @@ template <class W, int NT>
 int up_stream_run(const MoeArgs &a, size_t slots) {
     const int rows = 16 * kStreamWaves;
     const Grid g = grid_of(a, slots, cdiv(a.I, rows), cdiv(a.Is, rows));
+    const unsigned threads = 64 * kStreamWaves;
+    // (strips: rows of scales in whole, aligned words)
+    const bool strips = W::mx && a.H % 128 == 0 && ((uintptr_t)a.s_gu | (uintptr_t)a.s_sgu) % 4 == 0;
     APUS_TIMED("k_moe_up_stream",
-               if (W::mx && a.H % 128 == 0) k_moe_up_stream<W, 1, NT, W::mx><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper);
-               else k_moe_up_stream<W, 1, NT, false><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper));
+               if (strips) k_moe_up_stream<W, 1, NT, W::mx><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper);
+               else k_moe_up_stream<W, 1, NT, false><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper));
     return launch_check("k_moe_up_stream");
 }
 template <class W, int NT>

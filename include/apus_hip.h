@@ -596,11 +596,12 @@ int apus_hip_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, uint1
 /* y[m][o] = rnd(sum_k w[o][k] x[m][k]): w MXFP4 (O rows of K), x bf16, y
  * bf16, fp32 accumulation in the kernel's order (the tolerance class of
  * apus_hip_bf16_gemm_mfma_dev: |c - r| <= 2e-3 (|r| + sum_k |w x|)). K = 0
- * gives zeros. */
+ * gives zeros. A weight past bf16's range (4 or 6 at a scale of 2^126, 2 and
+ * more at 2^127: quantisation makes none) is infinite, as for dequantize. */
 int apus_hip_mxfp4_gemm_dev(const uint8_t *w, const uint8_t *ws, const uint16_t *x, size_t ldx,
                             uint16_t *y, size_t ldy, size_t M, size_t O, size_t K);
 /* The same with x in MXFP4 too (codes x [M][K/2], scales xs [M][K/32]), on
- * the matrix cores' 4-bit form. */
+ * the matrix cores' 4-bit form (no weight is past its range). */
 int apus_hip_mxfp4_gemm_mx_dev(const uint8_t *w, const uint8_t *ws, const uint8_t *x,
                                const uint8_t *xs, uint16_t *y, size_t ldy, size_t M, size_t O,
                                size_t K);
@@ -613,7 +614,7 @@ int apus_hip_mxfp4_gemm_mx_dev(const uint8_t *w, const uint8_t *ws, const uint8_
  *       + sigmoid(w_shared_gate . x) times the same of the shared expert.
  * Logits, softmax and sums are fp32; y is rounded once. Logits that are NaN
  * count as the largest (that token's y is NaN). The experts' weights are
- * bf16, or MXFP4 with their scales; the router's are bf16. */
+ * bf16, or MXFP4 with their scales (as in mxfp4_gemm_dev); the router's are bf16. */
 typedef struct {
     size_t hidden, inter;           /* multiples of 32 */
     size_t experts, topk;           /* up to 1024, up to 32 */

@@ -237,3 +237,21 @@ def test_moe_forms(hip, T, H, I, E, topk, Is, mx):
     r, b, gap = mx_ref.moe(x, w, topk, True, mx)
     assert float(gap.min()) > 0
     mx_ref.check(_run(hip, torch, w, x, topk, True), r, b, "forms")
+
+
+@pytest.mark.parametrize("T", [1, 12, 100])
+def test_moe_scales_of_any_alignment(hip, T):
+    """Scales are bytes: a tensor of them may begin at any address."""
+    import torch
+    g = _gen(torch, T)
+    H, I, E, k = 1024, 512, 24, 4
+    w = mx_ref.moe_weights(g, H, I, E, 512, True, True)
+    x = mx_ref.safe_tokens(g, w, T, k, H)
+    y = _run(hip, torch, w, x, k, True)
+    for off in (1, 2, 3):
+        v = dict(w)
+        for n in [n for n in w if n.startswith("s_")]:
+            b = torch.empty(w[n].numel() + 4, dtype=torch.uint8, device="cuda")
+            v[n] = b[off:off + w[n].numel()].view(w[n].shape).copy_(w[n])
+            assert v[n].data_ptr() % 4 == off
+        assert torch.equal(_run(hip, torch, v, x, k, True), y)

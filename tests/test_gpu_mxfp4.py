@@ -269,3 +269,54 @@ def test_gemm_forms(hip, M, O, K, mx):
         xv = x.double()
     r, b = mx_ref.gemm(mx_ref.values(w, ws), xv)
     mx_ref.check(y, r, b, f"forms mx={mx}")
+
+
+@pytest.mark.parametrize("M,O,K", [(3, 40, 192), (200, 700, 320), (1100, 1300, 192), (4096, 2048, 1024)])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("lo", [0, 247])
+def test_gemm_ends_of_the_scales(hip, M, O, K, mx, lo):
+    """Weight scales 2^-127 .. 2^-120, whose values and bf16 forms are subnormal
+    or next to it, and 2^120 .. 2^127, with activations that bring the products
+    back into range. A weight of 2^128 and more is infinite where it meets bf16
+    activations, as it is for mxfp4_dequantize."""
+    import torch
+    g = _gen(torch, M + O + lo)
+    w, _ = mx_ref.quantize(mx_ref.normal(g, O, K))
+    ws = (torch.randint(lo, lo + 8, (O, K // 32), generator=g, device="cuda")).to(torch.uint8)
+    x = (torch.randn(M, K, generator=g, device="cuda") * 2.0 ** (110 if lo == 0 else -115)).to(torch.bfloat16)
+    y = torch.empty(M, O, dtype=torch.bfloat16, device="cuda")
+    if mx:
+        c, s = _quantize(hip, torch, x)
+        hip.mxfp4_gemm_mx(w, ws, c, s, y)
+        xv = mx_ref.values(c, s)
+    else:
+        hip.mxfp4_gemm(w, ws, x, y)
+        xv = x.double()
+    wv = mx_ref.values(w, ws)
+    if not mx:                                             # (past bf16's range: infinite)
+        wv = wv.to(torch.bfloat16).double()
+    r, b = mx_ref.gemm(wv, xv)
+    fin = r.isfinite()
+    assert torch.equal(y.isnan(), r.isnan()) and torch.equal(y[r.isinf()].double(), r[r.isinf()])
+    assert mx or lo == 0 or not bool(fin.all())
+    mx_ref.check(y[fin], r[fin], b[fin], f"ends of the scales mx={mx}")
+
+
+@pytest.mark.parametrize("M,O,K", [(3, 40, 192), (300, 520, 1056), (4096, 2300, 544)])
+def test_gemm_scales_of_any_alignment(hip, M, O, K):
+    import torch
+    x, w, ws = _operands(torch, M, O, K, 0, M)
+    x = x.contiguous()
+    c, s = _quantize(hip, torch, x)
+    ys = []
+    for off in (0, 1, 3):
+        a, b = (torch.empty(t.numel() + 4, dtype=torch.uint8, device="cuda")[off:off + t.numel()].view(t.shape).copy_(t)
+                for t in (ws, s))
+        y, z = (torch.empty(M, O, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        hip.mxfp4_gemm(w, a, x, y)
+        hip.mxfp4_gemm_mx(w, a, c, b, z)
+        ys.append((y, z))
+    for y, z in ys[1:]:
+        assert torch.equal(y, ys[0][0]) and torch.equal(z, ys[0][1])
+    r, bound = mx_ref.gemm(mx_ref.values(w, ws), x.double())
+    mx_ref.check(ys[0][0], r, bound, "alignment")
