@@ -257,13 +257,24 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
     using s3 = std::integral_constant<int, 3>;
     Frag f0, f1;
     Scale c0, c1;
-    load_scales(0);
+    // the first scales go with the copies where rows of them are whole 16 bytes (a
+    // wait for registers here is one for all the copies)
+    const bool whole = (ks | (uint32_t)(uintptr_t)a.ws | (uint32_t)(uintptr_t)a.xs) % 16 == 0;
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < SPT; i++) {
+            const int p = wave * SPT + i;                // (64 rows)
+            copy16(row_of(p * 64 + lane) * ks, uniform(p * 64 < BO ? wst : xst), lds0 + 2 * SB + p * 1024, -1);
+        }
+    } else {
+        load_scales(0);
+    }
 #pragma unroll
     for (int st = 0; st < 2; st++) {
 #pragma unroll
         for (int i = 0; i < PPW; i++) copy_codes(i, st, (st - nk) >> 31);
     }
-    put_scales(0);
+    if (!whole) put_scales(0);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW) : "memory");
     __syncthreads();
 #pragma unroll
@@ -455,7 +466,14 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     using i2 = std::integral_constant<int, 2>;
     using i3 = std::integral_constant<int, 3>;
     // chunk 0, and what the loop finds under way: stages 0 and 1, a quarter of chunk 1
-    sreg.load(wrow, 0, sleft);
+    const bool whole = (ks | (uint32_t)(uintptr_t)a.ws) % 16 == 0;      // (as above)
+    if (whole) {
+        // (64 rows a wavefront; past the tile's, into the other slot, not in use yet)
+        const int row = min(wave * 64 + lane, min(BO - 1, O - 1 - o0));
+        copy16((uint32_t)row * ks, uniform(a.ws + (size_t)o0 * ks + k0 / kMxBlock), lds0 + S0 + wave * 1024, -1);
+    } else {
+        sreg.load(wrow, 0, sleft);
+    }
 #pragma unroll
     for (int q = 0; q < 4; q++)
 #pragma unroll
@@ -464,7 +482,7 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     for (int i = 0; i < XPW; i++) copy_x(i, 0, -1);
 #pragma unroll
     for (int i = 0; i < GROUP; i++) copy_at(i, -1);
-    put_scales(0);
+    if (!whole) put_scales(0);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(GROUP) : "memory");
     __syncthreads();
     Raw r0, r1;

@@ -276,7 +276,7 @@ struct WideCost {
     float f4, k4, fill;                     // 256 x 256: per round; with every CU busy
 };
 constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 13.5f, 7.0f, 43.0f, 12.0f},
-                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 10.0f}};
+                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 10.9f}};
 
 size_t rounds(size_t n) { return (n + cu_count() - 1) / cu_count(); }
 
