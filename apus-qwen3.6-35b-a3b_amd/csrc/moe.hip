@@ -10,7 +10,7 @@
 // every kernel streams weights through the MFMA with tokens as its 16 columns.
 // Launches:
 //   k_moe_router     logits; by the last workgroup of each 16 tokens to finish the
-//                    choice, by the last of those the choices in order of experts
+//                    choice, by the last of those the choices sorted by expert
 //   k_moe_up[_stream]   h = silu(gate) up of every (expert, 16 outputs)
 //   k_moe_down[_stream] fp32 rows of every (expert, 32 outputs), and
 //   k_moe_combine       their weighted sum; or for little work
@@ -62,8 +62,13 @@ constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
 // more rows again (MXFP4, us with 16 | 32: 24 tokens 82 | 86, 96 tokens 127 | 131;
 // bf16, 325 tokens 360 | 351).
 constexpr size_t kWideSlots = 8;
-// Up to here a choice is a slot of its own, and nothing is sorted (MXFP4, us with 1 | 2
-// | 4: 2 tokens 29 | 26 | 26, 4 tokens 35 | 35 | 42).
+// Choices are slots of their own, and nothing is sorted, while about two of them at
+// most are expected to share an expert, whose weights are then read twice: n choices
+// of E experts, n^2 / (2 E) of them. (Sorted | not, us: 3 tokens, MXFP4 33 | 30, bf16 51 |
+// 48; 6 tokens 41 | 40, 78 | 77; 60 experts of 1408, 4 a token, 3 tokens 39 | 37, 6
+// tokens 46 | 49; 8 experts of 4096, 2 a token, 3 tokens 121 | 128.)
+bool choices_apart(size_t T, size_t n, size_t E) { return T == 1 || n * n <= 4 * E; }
+// k_moe_down_few up to here whatever the work (2 tokens 29 us without, 26 with it)
 constexpr int kFewTokens = 2;
 
 struct MoeArgs {
@@ -79,6 +84,7 @@ struct MoeArgs {
     uint16_t *y;
     int T, H, I, E, k, Is, norm, nslots;
     int group;             // most rows of a slot: 16 or 32
+    int apart;             // choices are slots of their own
 };
 
 // ---- router ---------------------------------------------------------------
@@ -244,8 +250,8 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
 
 // ET tiles of 16 experts (the shared gate's one row is a tile of its own) x 16
 // tokens a workgroup, K over its 16 / ET wavefronts of a tile. The last workgroup
-// of the 16 tokens to finish chooses for them, a wavefront each, and with more than
-// a few tokens the last of those sorts the choices: what a workgroup hands on it
+// of the 16 tokens to finish chooses for them, a wavefront each, and unless choices
+// stay apart the last of those sorts them: what a workgroup hands on it
 // stores where all XCDs see it, waits for the stores, and counts itself; nobody
 // waits for anybody. Bound by latency: 7 us for one token, 12 for 16, 14 for 64, 21
 // for 325. (Choosing in every workgroup of the next launch instead costs that launch
@@ -329,7 +335,7 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
         if (t0 + wave < a.T)
             choose<NJ>(a, t0 + wave, lane, sids + wave * a.k, [&](int e) { return slog[wave * P + e]; });
     }
-    if (a.T <= kFewTokens) return;
+    if (a.apart) return;
     if (gridDim.y == 1) {                  // (one workgroup has chosen for all)
         __syncthreads();
         return make_slots(a, sids, lane, wave);
@@ -346,7 +352,7 @@ __global__ __launch_bounds__(64 * kRouterWaves) void k_moe_router(MoeArgs a) {
 // blocks. Blocks of a launch: first the shared expert's, nsh row blocks for
 // every `group` tokens; then nper row blocks per slot. A slot is up to `group` of
 // an expert's choices (a popular expert has several, side by side on the chip
-// instead of one after the other), or with few tokens a choice.
+// instead of one after the other), or, where they stay apart, a choice.
 struct Task {
     int e, part, first, n;                 // e == E: shared; n = 0: nothing
     const uint16_t *list;                  // or null: choices first, first + 1, ..
@@ -359,7 +365,7 @@ __device__ __forceinline__ Task task_of(const MoeArgs &a, int b, int nsh, int np
     }
     b -= nsh * groups;
     const int slot = b / nper, part = b % nper;
-    if (a.T <= kFewTokens) return {__builtin_amdgcn_readfirstlane(a.ids[slot]), part, slot, 1, nullptr};
+    if (a.apart) return {__builtin_amdgcn_readfirstlane(a.ids[slot]), part, slot, 1, nullptr};
     const int4 s = a.slots[slot];
     return {__builtin_amdgcn_readfirstlane(s.x), part, 0, __builtin_amdgcn_readfirstlane(s.z),
             a.list + __builtin_amdgcn_readfirstlane(s.y)};
@@ -955,7 +961,7 @@ int down_stream_run(const MoeArgs &a, size_t slots) {
 // which the split form keeps on their way as well with few rows a slot (16 tokens 143 |
 // 150, 64 tokens 297 | 287, 325 tokens 396 | 359). Streaming down needs h of a slot in
 // LDS. k_moe_down_few for work that one round of loads covers (one token: 25 us with the
-// two kernels, 19 with it; bf16 35 and 29), and for kFewTokens (29 and 26).
+// two kernels, 19 with it; bf16 35 and 29), and for kFewTokens.
 template <class W>
 int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
@@ -1115,7 +1121,8 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.Is = (int)L->shared_inter;
     a.norm = L->norm_topk;
     a.group = T * L->topk <= kWideSlots * L->experts ? 16 : 32;
-    a.nslots = (int)(T <= kFewTokens ? T * L->topk : moe_slots(T, L->topk, L->experts, a.group));
+    a.apart = choices_apart(T, T * L->topk, L->experts);
+    a.nslots = (int)(a.apart ? T * L->topk : moe_slots(T, L->topk, L->experts, a.group));
     const int tiles = router_tiles(a);
     const dim3 rg(tiles <= kSmallTiles ? 1 : tiles, cdiv(T, 16));
     APUS_TIMED("k_moe_router",

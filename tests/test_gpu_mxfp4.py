@@ -252,7 +252,7 @@ def test_python_refusals(hip):
                                    (47, 20000, 224), (50, 12352, 160), (64, 4100, 2144), (100, 12360, 1056),
                                    (250, 6001, 2208), (513, 4104, 288), (2050, 2049, 4192), (4100, 4090, 8224),
                                    (2048, 8192, 4096), (900, 2050, 320), (1000, 4090, 2080), (2000, 2041, 544),
-                                   (4096, 12345, 2080)])
+                                   (4096, 12345, 2080), (4096, 12345, 4128)])
 @pytest.mark.parametrize("mx", [False, True])
 def test_gemm_forms(hip, M, O, K, mx):
     import torch
