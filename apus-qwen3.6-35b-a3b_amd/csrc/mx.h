@@ -21,7 +21,8 @@ struct MxProduct {
     int M, O, K;
 };
 // products for many rows (mx_wide.hip): shape 2, tiles of 128 x 128, two a CU; 3, the
-// same, one a CU, with K in two halves side by side; 4, 256 x 256
+// same, one a CU, with K in two halves side by side; 4, 256 x 256; 5 (bf16 activations
+// only), 256 outputs x 128 rows, two a CU
 int mx_gemm_wide(const MxProduct &a, int shape);
 // of so many 256 x 256 tiles, those that go in quarters, as the last workgroups
 size_t mx_quarters(size_t tiles);

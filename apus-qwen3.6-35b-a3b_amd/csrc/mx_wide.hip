@@ -2,7 +2,7 @@
 // many rows: tiles of 64 TO outputs x 64 TMM rows, 4 wavefronts (2 x 2), one per SIMD,
 // on the 32-wide MFMAs; w and x are copied to LDS without registers and read there.
 //
-// 4096 rows x 12352 outputs, K 2048, 207 Gflop: bf16 x 180 us, 1.15 Pflop/s (a large
+// 4096 rows x 12352 outputs, K 2048, 207 Gflop: bf16 x 175 us, 1.18 Pflop/s (a large
 // bf16 library product reaches 1.32 here); MXFP4 x 82 us, 2.5 Pflop/s. With K 8192, 590
 // and 223 us for 825 Gflop, 1.40 and 3.7 Pflop/s. There the chip's MFMA rate under load
 // is the bound: the same loop without copies and LDS reads takes 195 of the 223 us.
@@ -333,8 +333,8 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
 
 // ---- bf16 activations ----------------------------------------------------------
 // A stage is 64 k of the activations, 128 bytes a row; the weights come in
-// chunks of 256 k (128 bytes of codes a row), their scales of 512 k, all double-
-// buffered in LDS. A quarter of a chunk is copied with each stage. In stage t
+// chunks of 2 RB k (RB bytes of codes a row), their scales of 512 k, all double-
+// buffered in LDS. A part of a chunk is copied with each of its stages. In stage t
 // of a chunk, lane (row l % 32, half g) takes the weights' block 2 t + g, one
 // 16-byte read for the whole stage, and MFMA step j its codes 8 j .., widened
 // to bf16 in registers, with the activations of the same k: 16-byte chunk
@@ -342,17 +342,23 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
 // k as bf16 weights would need.
 constexpr int kMx16Stage = 64;
 
-template <int TO, int TMM>
-constexpr int kMx16Lds = 2 * 64 * (TMM * kMx16Stage * 2 + TO * (128 + 16));
-template <int TO, int TMM>
+// The place of 16-byte chunk c of row r, rows RB bytes long, so that rows read side by
+// side are in many banks.
+template <int RB>
+__device__ __forceinline__ int slot_of(int c, int r) { return c ^ (RB == 128 ? r & 7 : r >> 2 & 3); }
+
+template <int TO, int TMM, int RB>
+constexpr int kMx16Lds = 2 * 64 * (TMM * kMx16Stage * 2 + TO * (RB + 16));
+template <int TO, int TMM, int RB>
 __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, int m0, int k0, int nk,
                                           f32x16 (&acc)[TO][TMM]) {
     constexpr int BO = 64 * TO, BM = 64 * TMM;
-    constexpr int XB = BM * 128, WB = BO * 128, SCB = BO * 16;
+    constexpr int XB = BM * 128, WB = BO * RB, SCB = BO * 16;
+    constexpr int CH = RB / 16, CPS = RB / 32;           // 16-byte pieces of a row, stages of a chunk
     constexpr int XPW = BM / 32, WPW = BO / 128;         // copies a wavefront and stage
     constexpr int NF = TO * TMM;
     constexpr int W0 = 2 * XB, S0 = 2 * (XB + WB);
-    static_assert(S0 + 2 * SCB == kMx16Lds<TO, TMM> && BO <= 256);
+    static_assert(S0 + 2 * SCB == (kMx16Lds<TO, TMM, RB>) && BO <= 256);
     const int M = a.M, O = a.O, K = a.K - k0;            // K: from k0 on
     const size_t ldx = a.ldx;
     const int lane = threadIdx.x & 63;
@@ -362,11 +368,11 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
     const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
     const uint32_t kleft = (uint32_t)K / 2, sleft = (uint32_t)K / kMxBlock, kx = (uint32_t)K * 2;    // from k0 on
-    const int nch = (nk + 3) / 4, nsc = (min(nk, (K + kMx16Stage - 1) / kMx16Stage) + 7) / 8;
+    const int nch = (nk + CPS - 1) / CPS, nsc = (min(nk, (K + kMx16Stage - 1) / kMx16Stage) + 7) / 8;
     const uint8_t *const wrow = a.ws + (size_t)(o0 + min(tid % BO, O - 1 - o0)) * ks + k0 / kMxBlock;
     const void *const wt = uniform(a.w + (size_t)o0 * kc + k0 / 2),
                *const xt = uniform((const uint16_t *)a.x + (size_t)m0 * ldx + k0);
-    const uint32_t cg = ((lane & 7) ^ (lane >> 3)) * 16;
+    const uint32_t cg = slot_of<128>(lane & 7, lane >> 3) * 16, wg = slot_of<RB>(lane % CH, lane / CH) * 16;
     uint32_t xoff[XPW];
 #pragma unroll
     for (int i = 0; i < XPW; i++)
@@ -376,12 +382,12 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
         at = at < kx ? at : 0;                           // (past the row's end: masked when read)
         copy16(xoff[i] + at, xt, lds0 + (st & 1) * XB + (wave * XPW + i) * 1024, live);
     };
-    // quarter q of chunk c: 64 TO / 4 rows
+    // part q of chunk c: its rows in CPS parts
     auto copy_w = [&](int i, int c, int q, int live) {
-        uint32_t at = c * 128 + cg;
+        uint32_t at = c * RB + wg;
         at = at < kleft ? at : 0;
         const int p = q * (BO / 32) + wave * WPW + i;
-        const uint32_t row = min(p * 8 + (lane >> 3), O - 1 - o0);
+        const uint32_t row = min(p * (64 / CH) + lane / CH, O - 1 - o0);
         copy16(row * kc + at, wt, lds0 + W0 + (c & 1) * WB + p * 1024, live);
     };
     // 512 k of a row's scales, through registers
@@ -390,15 +396,15 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
         if (BO == 256 || tid < BO) *reinterpret_cast<u32x4 *>(sm + S0 + (c & 1) * SCB + tid * 16) = sreg.v;
     };
     // what is copied at the end of stage kt: the activations of stage kt + 2, a
-    // quarter of chunk (kt + 1) / 4 + 1 (its slot's last reader was the chunk
-    // before (kt + 1) / 4's)
+    // part of chunk (kt + 1) / CPS + 1 (its slot's last reader was the chunk
+    // before (kt + 1) / CPS's)
     constexpr int GROUP = XPW + WPW;
     auto copy_at = [&](int i, int kt) {
         if (i < XPW) {
             copy_x(i, kt + 2, (kt + 2 - nk) >> 31);
         } else {
-            const int c = (kt + 1) / 4 + 1;
-            copy_w(i - XPW, c, (kt + 1) & 3, (c - nch) >> 31);
+            const int c = (kt + 1) / CPS + 1;
+            copy_w(i - XPW, c, (kt + 1) & (CPS - 1), (c - nch) >> 31);
         }
     };
 #pragma unroll
@@ -414,8 +420,8 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     };
     const uint32_t rrow = (lane & 31) * 128;
     auto rd_raw = [&](int st, int t, Raw &f) {
-        const int c = st >> 2, b = 2 * (st & 3) + g;
-        const char *p = sm + W0 + (c & 1) * WB + (wo * TO + t) * 4096 + rrow + ((b ^ (lane & 7)) << 4);
+        const int c = st / CPS, b = 2 * (st & (CPS - 1)) + g;
+        const char *p = sm + W0 + (c & 1) * WB + ((wo * TO + t) * 32 + (lane & 31)) * RB + (slot_of<RB>(b, lane & 31) << 4);
         f.v[t] = *reinterpret_cast<const u32x4 *>(p);
         f.s[t] = (uint8_t)sm[S0 + (st >> 3 & 1) * SCB + ((wo * TO + t) * 32 + (lane & 31)) * 16 + (2 * (st & 7) + g)];
     };
@@ -475,7 +481,7 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
         sreg.load(wrow, 0, sleft);
     }
 #pragma unroll
-    for (int q = 0; q < 4; q++)
+    for (int q = 0; q < CPS; q++)
 #pragma unroll
         for (int i = 0; i < WPW; i++) copy_w(i, 0, q, -1);
 #pragma unroll
@@ -532,80 +538,93 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
 }
 
 // ---- a product's tiles ---------------------------------------------------------
-template <bool XMX, int T>
-constexpr int kWideLds = XMX ? kMxLds<T, T> : kMx16Lds<T, T>;
+template <bool XMX, int TO, int TMM, int RB>
+constexpr int kWideLds = XMX ? kMxLds<TO, TMM> : kMx16Lds<TO, TMM, RB>;
+constexpr int max_of(int a, int b) { return a > b ? a : b; }
+// bytes of LDS with G groups: a group's operands, then the tile on its way to y
+template <bool XMX, int TO, int TMM, int RB, int G>
+constexpr int kTileLds = max_of(G * kWideLds<XMX, TO, TMM, RB>, TO * TMM * 64 * 128);
 
-// y of 64 T outputs from o0 x 64 T rows from m0, by 4 wavefronts, or, with G = 2, by 8,
-// each 4 of them with half of K and LDS of their own
-template <bool XMX, int T, int G>
+// y of 64 TO outputs from o0 x 64 TMM rows from m0, by 4 wavefronts, or, with G = 2, by
+// 8, each 4 of them with half of K and LDS of their own. RB: bytes of a row's weights in
+// LDS at once with bf16 activations; with 64 two tiles of 256 x 128 fit a CU, and one's
+// first copies and stores run under the other's products (4096 rows x 12352 outputs, K
+// 1024, 2048, 4096: 92, 175, 341 us; 256 x 256 tiles 102, 179, 339). MXFP4 activations
+// gain nothing by it.
+template <bool XMX, int TO, int TMM, int RB, int G>
 __device__ __forceinline__ void wide_tile(char *sm, const MxProduct &a, int o0, int m0) {
-    constexpr int LDS = kWideLds<XMX, T>, STAGE = XMX ? kMxStage : kMx16Stage;
+    constexpr int LDS = kWideLds<XMX, TO, TMM, RB>, STAGE = XMX ? kMxStage : kMx16Stage;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int grp = wave >> 2, w = wave & 3;
     // (the second half may have a stage less, which it takes as one past K)
     const int nk = ((a.K + STAGE - 1) / STAGE + G - 1) / G, k0 = grp * nk * STAGE;
-    f32x16 acc[T][T];
-    if constexpr (XMX) mx_tile<T, T>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
-    else mx16_tile<T, T>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
+    f32x16 acc[TO][TMM];
+    if constexpr (XMX) mx_tile<TO, TMM>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
+    else mx16_tile<TO, TMM, RB>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
     if constexpr (G == 2) {                // the sum of the halves, in the first's registers
-        char *p = sm + LDS + w * (T * T * 4096) + lane * 16;
-        static_assert(4 * T * T * 4096 <= LDS, "the second half's sums fit its LDS");
+        char *p = sm + LDS + w * (TO * TMM * 4096) + lane * 16;
+        static_assert(4 * TO * TMM * 4096 <= LDS, "the second half's sums fit its LDS");
 #pragma unroll
-        for (int i = 0; grp == 1 && i < T * T * 4; i++) {
-            const f32x16 &v = acc[i / 4 / T][i / 4 % T];
+        for (int i = 0; grp == 1 && i < TO * TMM * 4; i++) {
+            const f32x16 &v = acc[i / 4 / TMM][i / 4 % TMM];
             const int q = i % 4 * 4;
             *reinterpret_cast<mx_f32x4 *>(p + i * 1024) = mx_f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
         }
         __syncthreads();
         if (grp == 1) return;
 #pragma unroll
-        for (int i = 0; i < T * T * 4; i++) {
+        for (int i = 0; i < TO * TMM * 4; i++) {
             const mx_f32x4 v = *reinterpret_cast<const mx_f32x4 *>(p + i * 1024);
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[i / 4 / T][i / 4 % T][i % 4 * 4 + j] += v[j];
+            for (int j = 0; j < 4; j++) acc[i / 4 / TMM][i / 4 % TMM][i % 4 * 4 + j] += v[j];
         }
     }
-    store_tile<T, T>(sm, acc, a.y, a.ldy, o0 + (w >> 1) * T * 32, m0 + (w & 1) * T * 32, a.O, a.M, w, lane);
+    store_tile<TO, TMM>(sm, acc, a.y, a.ldy, o0 + (w >> 1) * TO * 32, m0 + (w & 1) * TMM * 32, a.O, a.M, w, lane);
 }
 
-// Workgroups [0, big) take a tile of 64 T x 64 T each; four of the others a quarter
-// each of a tile that would be left for a last round of the chip (T = 4 only; 4096 rows x
+// Workgroups [0, big) take a tile each; four of the others a quarter each of a
+// tile that would be left for a last round of the chip (256 x 256 only; 4096 rows x
 // 12352 outputs, K 2048, 784 tiles on 256 CUs: 101 us, 90 with the last 16 in quarters;
 // bf16 x 220 and 206). G = 2 where the tiles are at most one a CU, whose 4 wavefronts
 // alone leave its MFMAs waiting: 512 rows x 4096 x 4096, bf16 x, 44 us, 33 with 8; MXFP4
 // x 15.1 and 13.6.
-template <bool XMX, int T, int G>
-__global__ __launch_bounds__(256 * G, T == 2 ? 2 : 1) void k_mx_gemm_wide(MxProduct a, int big) {
-    __shared__ __attribute__((aligned(16))) char sm[G * kWideLds<XMX, T>];
+template <bool XMX, int TO, int TMM, int RB, int G>
+__global__ __launch_bounds__(256 * G, TO * TMM <= 8 ? 2 : 1) void k_mx_gemm_wide(MxProduct a, int big) {
+    constexpr bool QUARTERS = TO * TMM == 16;
+    __shared__ __attribute__((aligned(16))) char sm[kTileLds<XMX, TO, TMM, RB, G>];
     int id = blockIdx.x, part = -1;
-    if (T == 4 && id >= big) {             // (a tile's quarters on its XCD: ids 8 apart)
+    if (QUARTERS && id >= big) {           // (a tile's quarters on its XCD: ids 8 apart)
         const int q = id - big;
         part = q / 8 % 4;
         id = big + q / 32 * 8 + q % 8;
     }
-    const int nbo = (a.O + 64 * T - 1) / (64 * T), nbm = (a.M + 64 * T - 1) / (64 * T);
+    const int nbo = (a.O + 64 * TO - 1) / (64 * TO), nbm = (a.M + 64 * TMM - 1) / (64 * TMM);
     int ob, mb;
     tile_of(id, nbo, nbm, ob, mb);
     if (ob >= nbo) return;                               // (the grid is a multiple of 8)
-    int o0 = ob * 64 * T, m0 = mb * 64 * T;
-    if constexpr (T == 4) {
+    int o0 = ob * 64 * TO, m0 = mb * 64 * TMM;
+    if constexpr (QUARTERS) {
         if (part >= 0) {
             o0 += part % 2 * 128;
             m0 += part / 2 * 128;
-            if (o0 < a.O && m0 < a.M) wide_tile<XMX, 2, 1>(sm, a, o0, m0);
+            if (o0 < a.O && m0 < a.M) wide_tile<XMX, 2, 2, 128, 1>(sm, a, o0, m0);
             return;
         }
     }
-    wide_tile<XMX, T, G>(sm, a, o0, m0);
+    wide_tile<XMX, TO, TMM, RB, G>(sm, a, o0, m0);
 }
 
-template <bool XMX, int T, int G>
+template <bool XMX, int TO, int TMM, int RB, int G>
 int launch_wide(const MxProduct &a) {
-    const int n = tile_grid((int)cdiv(a.O, 64 * T), (int)cdiv(a.M, 64 * T));
-    const int big = T == 4 ? n - (int)mx_quarters(n) : n;
+    const int n = tile_grid((int)cdiv(a.O, 64 * TO), (int)cdiv(a.M, 64 * TMM));
+    const int big = TO * TMM == 16 ? n - (int)mx_quarters(n) : n;
     const unsigned grid = (unsigned)(big + 4 * (n - big));
-    APUS_TIMED("k_mx_gemm_wide", k_mx_gemm_wide<XMX, T, G><<<grid, 256 * G, 0, stream()>>>(a, big));
+    APUS_TIMED("k_mx_gemm_wide", k_mx_gemm_wide<XMX, TO, TMM, RB, G><<<grid, 256 * G, 0, stream()>>>(a, big));
     return launch_check("k_mx_gemm_wide");
+}
+template <int TO, int TMM, int RB, int G>
+int launch_wide_of(const MxProduct &a) {
+    return a.xs ? launch_wide<true, TO, TMM, RB, G>(a) : launch_wide<false, TO, TMM, RB, G>(a);
 }
 
 }  // namespace
@@ -621,9 +640,10 @@ int mx_gemm_wide(const MxProduct &a, int shape) {
     // (halves need a stage each)
     if (shape == 3 && a.K <= (a.xs ? kMxStage : kMx16Stage)) shape = 2;
     switch (shape) {
-        case 2: return a.xs ? launch_wide<true, 2, 1>(a) : launch_wide<false, 2, 1>(a);
-        case 3: return a.xs ? launch_wide<true, 2, 2>(a) : launch_wide<false, 2, 2>(a);
-        default: return a.xs ? launch_wide<true, 4, 1>(a) : launch_wide<false, 4, 1>(a);
+        case 2: return launch_wide_of<2, 2, 128, 1>(a);
+        case 3: return launch_wide_of<2, 2, 128, 2>(a);
+        case 4: return launch_wide_of<4, 4, 128, 1>(a);
+        default: return launch_wide<false, 4, 2, 64, 1>(a);
     }
 }
 

@@ -274,9 +274,10 @@ struct WideCost {
     float f1, k1, f2, k2;                   // 128 x 128 tiles: one on the busiest CU, two
     float k3;                               // the same in two halves of K (fixed part f1)
     float f4, k4, fill;                     // 256 x 256: per round; with every CU busy
+    float k5, f6, k6;                       // 256 x 128: one on the busiest CU (fixed part f1), two
 };
-constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 13.5f, 7.0f, 43.0f, 12.0f},
-                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 10.9f}};
+constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 13.5f, 7.0f, 43.0f, 12.0f, 30.0f, 4.0f, 51.0f},
+                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 10.9f, 0.0f, 0.0f, 0.0f}};
 
 size_t rounds(size_t n) { return (n + cu_count() - 1) / cu_count(); }
 
@@ -303,8 +304,10 @@ int wide_shape(size_t M, size_t O, size_t K) {
     const size_t r4 = rounds(n4 - std::min(n4, part));
     const float w4 = r4 * (v.f4 + v.k4 * kk) + v.fill * std::min((float)r4, (float)n4 / cu_count()) +
                      (part ? v.f1 + v.k1 * kk : 0.0f);
-    if (few <= w2 && few <= w4) return 0;
-    return w4 < w2 ? 4 : r2 == 1 ? 3 : 2;
+    const size_t r5 = rounds((size_t)cdiv(O, 256) * cdiv(M, 128));
+    const float w5 = XMX ? w4 : (r5 / 2) * (v.f6 + v.k6 * kk) + (r5 % 2) * (v.f1 + v.k5 * kk);
+    const float least = std::min(std::min(few, w2), std::min(w4, w5));
+    return least == few ? 0 : least == w2 ? (r2 == 1 ? 3 : 2) : least == w4 ? 4 : 5;
 }
 
 template <bool XMX>
