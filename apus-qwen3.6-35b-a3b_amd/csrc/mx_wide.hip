@@ -3,10 +3,10 @@
 // on the 32-wide MFMAs; w and x are copied to LDS without registers and read there.
 //
 // 4096 rows x 12352 outputs, K 2048, 207 Gflop: bf16 x 175 us, 1.18 Pflop/s (a large
-// bf16 library product reaches 1.32 here); MXFP4 x 82 us, 2.5 Pflop/s. With K 8192, 590
+// bf16 library product reaches 1.32 here); MXFP4 x 78 us, 2.6 Pflop/s. With K 8192, 590
 // and 223 us for 825 Gflop, 1.40 and 3.7 Pflop/s. There the chip's MFMA rate under load
 // is the bound: the same loop without copies and LDS reads takes 195 of the 223 us.
-// With K 2048 a fixed part of a tile, its first copies and its 128 KB of y, is a third.
+// With K 2048 the 101 MB of y count beside it.
 #include <stdint.h>
 
 #include <type_traits>

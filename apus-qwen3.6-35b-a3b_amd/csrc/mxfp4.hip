@@ -277,7 +277,7 @@ struct WideCost {
     float k5, f6, k6;                       // 256 x 128: one on the busiest CU (fixed part f1), two
 };
 constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 13.5f, 7.0f, 43.0f, 12.0f, 30.0f, 4.0f, 51.0f},
-                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 10.9f, 0.0f, 0.0f, 0.0f}};
+                                  {3.2f, 4.8f, 4.0f, 10.0f, 5.0f, 6.5f, 10.5f, 11.2f, 0.0f, 0.0f, 0.0f}};
 
 size_t rounds(size_t n) { return (n + cu_count() - 1) / cu_count(); }
 
