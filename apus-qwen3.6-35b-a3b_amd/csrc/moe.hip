@@ -22,8 +22,8 @@
 //
 // Times below: hidden 2048, 256 experts of 512 inner elements, 8 a token, a shared
 // expert of 512, inputs other than the call before's. The whole layer, us at
-// 1 / 5 / 16 / 64 / 325 tokens: MXFP4 19 / 39 / 60 / 107 / 160 (bytes alone, at a
-// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 26 / 69 / 143 / 287 / 342
+// 1 / 5 / 16 / 64 / 325 tokens: MXFP4 19 / 39 / 60 / 108 / 154 (bytes alone, at a
+// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 26 / 69 / 143 / 287 / 350
 // (11 / 51 / 127 / 272 / 314): with many choices it is bound by the weights' bytes,
 // with few by three launches' latency.
 #include <stdint.h>
@@ -563,9 +563,9 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
 }
 
 // ---- the same, a wavefront alone: no partial sums, no barrier, and D steps of
-// weights and activations on their way all along its walk. Up: bf16, 325 tokens, 200
-// us for 1.07 GB, 5.4 TB/s; MXFP4, 64 tokens, 53 us for 247 MB, 4.7 TB/s. Down: 126
-// us for 0.54 GB, 4.3 TB/s; 32 us for 124 MB, 3.9 TB/s. More steps on their way (3, 4)
+// weights and activations on their way all along its walk. Up: bf16, 325 tokens, 198
+// us for 1.07 GB, 5.4 TB/s; MXFP4, 64 tokens, 53 us for 247 MB, 4.7 TB/s. Down: 119
+// us for 0.54 GB, 4.5 TB/s; 32 us for 124 MB, 3.9 TB/s. More steps on their way (3, 4)
 // changed nothing, nor did whole 128-byte lines of MXFP4 codes a load.
 constexpr int kStreamWaves = 4;
 
