@@ -29,6 +29,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <new>
 
 #include "../../include/apus_hip.h"
 #include "apus_dev.h"
@@ -1029,7 +1030,9 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
     if (hs > 0x7fff0000u || max_tokens * L->hidden * 2 > 0x7fff0000u)
         return set_error(kErrUnsupported, "mixture-of-experts intermediates of up to 2 GiB");
     if (int r = mx_ready()) return r;
-    auto *w = new ApusHipMoeWork{max_tokens, L->hidden, L->inter, L->experts, L->topk, L->shared_inter, current_device()};
+    auto *w = new (std::nothrow) ApusHipMoeWork{max_tokens, L->hidden, L->inter, L->experts, L->topk,
+                                                L->shared_inter, current_device()};
+    if (!w) return set_error(kErrHip, "out of host memory");
     const size_t T = max_tokens, k = L->topk;
     size_t n = 0;
     auto take = [&](size_t bytes) {
@@ -1043,6 +1046,7 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
                  slots = take(moe_slots(T, k, L->experts, 16) * 16), list = take(T * k * 2);
     if (hipMalloc((void **)&w->base, n) != hipSuccess) {
         delete w;
+        (void)hipGetLastError();           // (not for the next launch to report)
         return set_error(kErrHip, "hipMalloc of %zu bytes failed", n);
     }
     // (the counters are clear before any stream's first call)
