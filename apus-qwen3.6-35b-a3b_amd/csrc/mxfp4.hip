@@ -268,8 +268,9 @@ int few_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *x
 // the form with the least estimate was within a tenth of the best one measured.
 struct FewCost {
     float fixed, one, two;                  // one, two: tiles of 16 and 32 outputs x 64 rows
+    float fixed4, four;                     // and of 64 outputs (bf16 activations)
 };
-constexpr FewCost kFewCost[] = {{2.5f, 3.6f, 5.6f}, {2.6f, 1.3f, 2.0f}};         // bf16, MXFP4 activations
+constexpr FewCost kFewCost[] = {{2.5f, 3.6f, 5.6f, 4.5f, 7.0f}, {2.6f, 1.3f, 2.0f}};     // bf16, MXFP4 activations
 struct WideCost {
     float f1, k1, f2, k2;                   // 128 x 128 tiles: one on the busiest CU, two
     float k3;                               // the same in two halves of K (fixed part f1)
@@ -281,22 +282,34 @@ constexpr WideCost kWideCost[] = {{3.0f, 15.2f, 4.0f, 28.0f, 13.5f, 7.0f, 43.0f,
 
 size_t rounds(size_t n) { return (n + cu_count() - 1) / cu_count(); }
 
-// 32 outputs a workgroup instead of 16? (few rows: from two workgroups a CU on.)
+// Tiles of 16 outputs that a workgroup of the few-row kernel takes, and its estimate
+// (more rows than 32). With few rows two from two workgroups a CU on. Four halve the
+// loads of bf16 activations, which are most of a workgroup's (64 rows x 12352 outputs, K
+// 2048: 15.3 us with two, 12.5 with four; 128 x 8192 16.3 and 12.0).
+struct FewForm {
+    int tiles;
+    float cost;
+};
 template <bool XMX>
-bool few_pays_two(size_t n2, size_t n1, size_t M) {
-    if (M <= 32) return n1 >= 2 * (size_t)cu_count();
+FewForm few_form(size_t M, size_t O, size_t K) {
     const FewCost &c = kFewCost[XMX];
-    return c.two * rounds(n2) < c.one * rounds(n1);
+    const float kk = (float)K / 2048.0f;
+    const size_t t16 = cdiv(M, 16), nbm = cdiv(t16, cdiv(t16, cdiv(t16, 4)));
+    auto cost = [&](float fixed, float per, size_t outputs) {
+        return fixed + kk * per * rounds(cdiv(O, outputs) * nbm);
+    };
+    if (M <= 32) return {cdiv(O, 16) * nbm >= 2 * (size_t)cu_count() ? 2 : 1, 0.0f};
+    FewForm f{1, cost(c.fixed, c.one, 16)};
+    if (const float two = cost(c.fixed, c.two, 32); two < f.cost) f = {2, two};
+    if (const float four = cost(c.fixed4, c.four, 64); !XMX && four < f.cost) f = {4, four};
+    return f;
 }
 
 // The shape of the many-row kernel to take, or 0: the few-row one.
 template <bool XMX>
-int wide_shape(size_t M, size_t O, size_t K) {
+int wide_shape(size_t M, size_t O, size_t K, float few) {
     const float kk = (float)K / 2048.0f;
-    const FewCost &c = kFewCost[XMX];
     const WideCost &v = kWideCost[XMX];
-    const size_t nbm = cdiv(M, 64);
-    const float few = c.fixed + kk * std::min(c.one * rounds(cdiv(O, 16) * nbm), c.two * rounds(cdiv(O, 32) * nbm));
     const size_t r2 = rounds((size_t)cdiv(O, 128) * cdiv(M, 128));
     // (one tile a CU: in halves of K, 1000 rows x 4096 x 2048 of bf16 25 -> 21 us)
     const float w2 = r2 == 1 ? v.f1 + v.k3 * kk : (r2 / 2) * (v.f2 + v.k2 * kk) + (r2 % 2) * (v.f1 + v.k1 * kk);
@@ -318,22 +331,25 @@ int gemm_run(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *
         k_mx_zero_rows<<<stream_grid(M * O), 256, 0, stream()>>>(y, ldy, O, M * O);
         return launch_check("k_mx_zero_rows");
     }
+    const FewForm few = few_form<XMX>(M, O, K);
     if (M > 32) {
-        const int shape = wide_shape<XMX>(M, O, K);
+        const int shape = wide_shape<XMX>(M, O, K, few.cost);
         if (shape)
             return mx_gemm_wide({w, ws, x, XMX ? xs : nullptr, ldx, y, ldy, (int)M, (int)O, (int)K}, shape);
     }
-    const size_t tiles = cdiv(M, 16), nt = cdiv(tiles, cdiv(tiles, 4)), nbm = cdiv(tiles, nt);
-    const bool two = few_pays_two<XMX>(cdiv(O, 32) * nbm, cdiv(O, 16) * nbm, M);
-#define FEW(NT, XR)                                                                          \
-    two ? few_run<XMX, 2, NT, XR>(w, ws, x, xs, ldx, y, ldy, M, O, K)                        \
-        : few_run<XMX, 1, NT, XR>(w, ws, x, xs, ldx, y, ldy, M, O, K)
-    switch (nt) {
-        case 1: return M <= 4 ? FEW(1, 1) : FEW(1, 4);
-        case 2: return FEW(2, 4);
-        case 3: return FEW(3, 4);
-        default: return FEW(4, 4);
+    const size_t tiles = cdiv(M, 16), nt = cdiv(tiles, cdiv(tiles, 4));
+#define FEW(RT, NT, XR) few_run<XMX, RT, NT, XR>(w, ws, x, xs, ldx, y, ldy, M, O, K)
+#define FEW2(NT, XR) few.tiles == 2 ? FEW(2, NT, XR) : FEW(1, NT, XR)
+    if constexpr (!XMX) {
+        if (few.tiles == 4) return nt == 3 ? FEW(4, 3, 4) : FEW(4, 4, 4);
     }
+    switch (nt) {
+        case 1: return M <= 4 ? FEW2(1, 1) : FEW2(1, 4);
+        case 2: return FEW2(2, 4);
+        case 3: return FEW2(3, 4);
+        default: return FEW2(4, 4);
+    }
+#undef FEW2
 #undef FEW
 }
 

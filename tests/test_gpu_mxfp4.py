@@ -244,7 +244,7 @@ def test_python_refusals(hip):
 
 
 # the forms of the product: shapes that the estimates give to each (few rows in
-# tiles of 1 to 4 x 16 with 16 and 32 outputs, 128-wide tiles, also with K in two
+# tiles of 1 to 4 x 16 with 16, 32 and 64 outputs, 128-wide tiles, also with K in two
 # halves, 256-wide tiles, also with the last of them in quarters), with row, output
 # and K edges in each; K past one pair of steps a wavefront, K of 4096 and more, odd
 # numbers of blocks
@@ -252,7 +252,8 @@ def test_python_refusals(hip):
                                    (47, 20000, 224), (50, 12352, 160), (64, 4100, 2144), (100, 12360, 1056),
                                    (250, 6001, 2208), (513, 4104, 288), (2050, 2049, 4192), (4100, 4090, 8224),
                                    (2048, 8192, 4096), (900, 2050, 320), (1000, 4090, 2080), (2000, 2041, 544),
-                                   (4096, 12345, 2080), (4096, 12345, 4128)])
+                                   (4096, 12345, 2080), (4096, 12345, 4128),
+                                   (60, 12345, 2080), (120, 8190, 1056), (45, 12401, 2080)])
 @pytest.mark.parametrize("mx", [False, True])
 def test_gemm_forms(hip, M, O, K, mx):
     import torch
