@@ -753,10 +753,11 @@ def _bf16(t):
 def _rows(t, what, dev, ncols=None):
     """(pointer, rows, columns, pitch) of a 2-D tensor of bf16 values or codes on
     device dev whose rows are contiguous (any pitch)."""
-    if t.get_device() != dev or t.dim() != 2 or not _bf16(t):
+    shape = t.shape
+    if len(shape) != 2 or t.get_device() != dev or (t.dtype not in _BF16 and not _bf16(t)):
         raise ValueError(f"{what}: a 2-D tensor of bf16 values or codes on GPU {dev}, not "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    m, n = t.shape
+                         f"{tuple(shape)} {t.dtype} on {t.device}")
+    m, n = shape
     if ncols is not None and n != ncols:
         raise ValueError(f"{what}: rows of {n} elements, expected {ncols}")
     ld, one = t.stride()
@@ -773,18 +774,10 @@ def _bytes(t, rows, cols, what, dev):
     return t.data_ptr()
 
 
-def _gpu(t, what):
-    """The index of t's GPU, which is the library's."""
-    dev = t.get_device()
-    if dev != _device:
-        raise ValueError(f"{what}: a tensor on GPU {_device}, not on {t.device}")
-    return dev
-
-
 def mxfp4_quantize(x, codes, scales):
     """x [M, K] bf16 (rows of any pitch) -> codes [M, K/2], scales [M, K/32]
     (uint8): MXFP4, apus_hip_mxfp4_quantize."""
-    dev = _gpu(x, "x")
+    dev = _device
     xp, M, K, ldx = _rows(x, "x", dev)
     _chk(load().apus_hip_mxfp4_quantize(xp, ldx, _bytes(codes, M, K // 2, "codes", dev),
                                         _bytes(scales, M, K // 32, "scales", dev), M, K))
@@ -792,7 +785,7 @@ def mxfp4_quantize(x, codes, scales):
 
 def mxfp4_dequantize(codes, scales, x):
     """The bf16 values of codes, scales into x [M, K] (rows of any pitch)."""
-    dev = _gpu(x, "x")
+    dev = _device
     xp, M, K, ldx = _rows(x, "x", dev)
     _chk(load().apus_hip_mxfp4_dequantize(_bytes(codes, M, K // 2, "codes", dev),
                                           _bytes(scales, M, K // 32, "scales", dev), xp, ldx, M, K))
@@ -801,7 +794,7 @@ def mxfp4_dequantize(codes, scales, x):
 def mxfp4_gemm(w, ws, x, y):
     """y [M, O] = x [M, K] w^T, w [O, K/2], ws [O, K/32] MXFP4, x and y bf16
     with rows of any pitch."""
-    dev = _gpu(x, "x")
+    dev = _device
     xp, M, K, ldx = _rows(x, "x", dev)
     O = w.shape[0]
     yp, ym, _, ldy = _rows(y, "y", dev, O)
@@ -813,8 +806,7 @@ def mxfp4_gemm(w, ws, x, y):
 
 def mxfp4_gemm_mx(w, ws, x, xs, y):
     """As mxfp4_gemm with the activations in MXFP4: x [M, K/2], xs [M, K/32]."""
-    dev = _gpu(x, "x")
-    M, K, O = x.shape[0], x.shape[1] * 2, w.shape[0]
+    dev, M, K, O = _device, x.shape[0], x.shape[1] * 2, w.shape[0]
     yp, ym, _, ldy = _rows(y, "y", dev, O)
     if ym != M:
         raise ValueError(f"y: {ym} rows, expected {M}")
@@ -833,9 +825,9 @@ def moe_layer(dims, w, norm_topk=True):
     scales. The layer keeps the tensors alive."""
     hidden, inter, experts, topk, shared = dims
     mx = "s_gate_up" in w
-    devs = {t.device for t in w.values() if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"weights on several devices: {sorted(map(str, devs))}")
+    for n, t in w.items():
+        if t is not None and t.get_device() != _device:
+            raise ValueError(f"{n}: a tensor on GPU {_device}, not on {t.device}")
     shapes = {"w_gate_up": (experts, 2 * inter, hidden), "w_down": (experts, hidden, inter)}
     if shared:
         shapes.update(w_shared_gate_up=(2 * shared, hidden), w_shared_down=(hidden, shared))
@@ -880,7 +872,7 @@ class MoeWork:
 def moe_layer_decode(layer, work, x, y):
     """A mixture-of-experts layer on a decode step's tokens: x [T, hidden]
     -> y [T, hidden], contiguous bf16 device tensors; y may be x."""
-    dev, H = _gpu(layer._tensors["w_router"], "w_router"), layer.hidden
+    dev, H = _device, layer.hidden
     for t, n in ((x, "x"), (y, "y")):
         if (t.get_device() != dev or t.shape != x.shape or t.dim() != 2 or t.shape[1] != H
                 or not _bf16(t) or not t.is_contiguous()):
