@@ -257,9 +257,12 @@ __device__ __forceinline__ void make_slots(const MoeArgs &a, const int *sids, in
 // stores where all XCDs see it, waits for the stores, and counts itself; nobody
 // waits for anybody. Bound by latency: 7 us for one token, 12 for 16, 14 for 64, 21
 // for 325. (Choosing in every workgroup of the next launch instead costs that launch
-// as much as is saved here.) Of up to kSmallTiles tiles one workgroup takes all, and
-// hands nothing on: 13 tokens of 1056, 20 experts, 7 us, 9 with the hand-over.
-constexpr int kSmallTiles = 4;
+// as much as is saved here.) Of up to kSmallTiles tiles of few elements one workgroup
+// takes all, and hands nothing on: 13 tokens of 1056, 20 experts, 7 us, 9 with the
+// hand-over (small layers, us with one workgroup | several: one token, 8 experts, hidden
+// 4096 17.0 | 18.1, 8192 27.3 | 26.7; 40 experts, 1024 13.2 | 13.8, 2048 15.4 | 14.8, 4096
+// 20.8 | 18.2).
+constexpr int kSmallTiles = 4, kSmallElements = 4096;    // tiles, tiles times hidden
 static_assert(64 * kRouterWaves >= kMoeMaxExperts, "a thread per expert");
 int router_tiles(const MoeArgs &a) { return (a.E + 15) / 16 + (a.w_sgate ? 1 : 0); }
 template <int NJ, int ET>
@@ -1130,9 +1133,10 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.apart = choices_apart(T, T * L->topk, L->experts);
     a.nslots = (int)(a.apart ? T * L->topk : moe_slots(T, L->topk, L->experts, a.group));
     const int tiles = router_tiles(a);
-    const dim3 rg(tiles <= kSmallTiles ? 1 : tiles, cdiv(T, 16));
+    const bool small = tiles <= kSmallTiles && tiles * a.H <= kSmallElements;
+    const dim3 rg(small ? 1 : tiles, cdiv(T, 16));
     APUS_TIMED("k_moe_router",
-               if (tiles <= kSmallTiles) k_moe_router<1, kSmallTiles><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
+               if (small) k_moe_router<1, kSmallTiles><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
                else if (a.E <= 256) k_moe_router<4, 1><<<rg, 64 * kRouterWaves, 0, stream()>>>(a);
                else k_moe_router<16, 1><<<rg, 64 * kRouterWaves, 0, stream()>>>(a));
     APUS_LAUNCHED("k_moe_router");
