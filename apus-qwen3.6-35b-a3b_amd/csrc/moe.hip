@@ -58,12 +58,15 @@ struct ApusHipMoeWork {
 namespace {
 
 constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
-// Choices an expert up to which slots of bf16 weights have up to 16 rows, then 32: the
-// kernels for 16 have fewer registers and LDS and more wavefronts, but read the weights
-// of an expert with more rows again (us with 16 | 32: 24 tokens 195 | 198, 325 tokens
-// 352 | 359, 512 tokens 396 | 393, 768 tokens 480 | 444). With MXFP4 weights 16 is better
-// all the way (24 tokens 74 | 77, 325 tokens 154 | 158, 1024 tokens 287 | 289).
-constexpr size_t kWideSlots = 14;
+// Most rows of a slot. 32 from 14 choices an expert on, where that leaves 2048 blocks of
+// 16 inner elements; else 16: the kernels for 16 have fewer registers and less LDS and
+// more wavefronts, but read the weights of an expert with more rows again (us with 16 |
+// 32: bf16, 325 tokens 352 | 359, 768 tokens 480 | 444; MXFP4, 96 tokens 116 | 124; 128
+// experts of 768, 8 a token, MXFP4, 256 tokens 186 | 178, 1024 tokens 474 | 420; 20 experts
+// of 224, 3 a token, 512 tokens 36 | 44, bf16 47 | 60).
+int slot_rows(size_t n, size_t E, size_t I) {
+    return n <= 14 * E || (E + n / 32) * (I / 16) < 2048 ? 16 : 32;
+}
 // Choices are slots of their own, and nothing is sorted, while about two of them at
 // most are expected to share an expert, whose weights are then read twice: n choices
 // of E experts, n^2 / (2 E) of them. (Sorted | not, us: 3 tokens, MXFP4 33 | 30, bf16 51 |
@@ -972,8 +975,7 @@ int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
     const bool one = a.group == 16;
     const bool ups = slots * a.I / 16 >= 1024 && (W::mx || a.T * a.k >= a.E);
-    constexpr int NT = W::mx ? 1 : 2;
-    if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, NT>(a, slots))
+    if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, 2>(a, slots))
         return r;
     const int units = a.T * (a.k * cdiv(a.I, 128) + cdiv(a.Is, 128));
     if (a.T <= kFewTokens || (a.T <= 16 && units <= kFewWaves * kFewUnits)) {
@@ -981,7 +983,7 @@ int experts_run(const MoeArgs &a) {
         return launch_check("k_moe_down_few");
     }
     const bool downs = slots * a.H / 32 >= 1024 && 32 * down_pitch(std::max(a.I, a.Is)) <= kDownH;
-    if (int r = !downs ? down_run<W>(a, slots) : one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, NT>(a, slots))
+    if (int r = !downs ? down_run<W>(a, slots) : one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, 2>(a, slots))
         return r;
     APUS_TIMED("k_moe_combine",
                k_moe_combine<<<cdiv((size_t)a.T * (a.H / 4), 256), 256, 0, stream()>>>(a));
@@ -1129,7 +1131,7 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.k = (int)L->topk;
     a.Is = (int)L->shared_inter;
     a.norm = L->norm_topk;
-    a.group = L->mxfp4 || T * L->topk <= kWideSlots * L->experts ? 16 : 32;
+    a.group = slot_rows(T * L->topk, L->experts, L->inter);
     a.apart = choices_apart(T, T * L->topk, L->experts);
     a.nslots = (int)(a.apart ? T * L->topk : moe_slots(T, L->topk, L->experts, a.group));
     const int tiles = router_tiles(a);

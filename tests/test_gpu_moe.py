@@ -227,7 +227,7 @@ def test_moe_refusals(hip):
                                              (20, 4128, 96, 32, 6, 64), (100, 544, 512, 24, 8, 544),
                                              (200, 2080, 160, 12, 4, 32), (300, 256, 1056, 10, 5, 0),
                                              (70, 2048, 480, 100, 8, 1056), (1000, 96, 64, 130, 2, 64),
-                                             (3, 4128, 1184, 9, 5, 2080)])
+                                             (3, 4128, 1184, 9, 5, 2080), (400, 1056, 480, 20, 5, 96)])
 def test_moe_forms(hip, T, H, I, E, topk, Is, mx):
     import torch
     print(f"[moe] forms T={T} H={H} I={I} E={E} topk={topk} Is={Is} mx={mx}", flush=True)
