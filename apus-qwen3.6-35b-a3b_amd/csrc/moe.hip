@@ -12,7 +12,7 @@
 //   k_moe_router     logits; by the last workgroup of each 16 tokens to finish the
 //                    choice, by the last of those the choices sorted by expert
 //   k_moe_up[_stream]   h = silu(gate) up of every (expert, 16 outputs)
-//   k_moe_down[_stream] fp32 rows of every (expert, 32 outputs), and
+//   k_moe_down[_stream, _walk] fp32 rows of every (expert, 32 outputs), and
 //   k_moe_combine       their weighted sum; or for little work
 //   k_moe_down_few      both in one.
 // The intermediate h = silu(g) u goes to the down product as two bf16 numbers
@@ -817,6 +817,116 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a
     else down_stream<W, RT, 1, 2>(a, task, b0, nb, h, sm + wave * LDS, lane);
 }
 
+// The same for inner sizes whose h does not fit: 32 outputs a wavefront, h's two planes
+// walked along with the weights as the activations are in up_stream.
+template <class W, int NT, int D, int XR, bool SC>
+__device__ __forceinline__ void down_walk(const MoeArgs &a, const Task &task, int o0, char *m, int lane) {
+    using X = XBf16<W>;
+    const int r = lane & 15, g = lane >> 4;
+    const bool sh = task.e == a.E;
+    const int I = sh ? a.Is : a.I;
+    typename W::Tile wt[2];                // (a tile past H, not stored, repeats the last)
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+        wt[t] = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn,
+                        (sh ? 0 : (size_t)task.e * a.H) + min(o0 + 16 * t, a.H - 16), 16, I);
+    const auto wl = W::raw_lane(lane, I);
+    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
+    uint32_t hl[NT][2][4];                 // rows 4 i + g of the planes
+#pragma unroll
+    for (int u = 0; u < NT; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            hl[u][0][i] = h_at(a, choice(task, 16 * u + 4 * i + g), sh) * 2;
+            hl[u][1][i] = hl[u][0][i] + I * 2;
+        }
+    typename W::Raw fw[D][2];
+    RowsBf16::Raw fx[D][NT][2];
+    char *const mx = m + 2 * W::kTile, *const ms = mx + NT * RowsBf16::kTile;
+    Strip strip[SC ? 2 : 1];
+    auto load = [&](int d, int st) {
+        if constexpr (SC) {
+            if ((st & (Strip::kSteps - 1)) == 0) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) strip[t].load(wt[t], st, I);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++) W::template load_raw<!SC>(fw[d][t], wt[t], wl, st, I);
+#pragma unroll
+        for (int u = 0; u < NT; u++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) X::template load_raw<XR>(fx[d][u][p], hb, hl[u][p], st, I);
+    };
+    mx_f32x4 acc[2][NT] = {};
+    walk<D>((I + 127) / 128, load, [&](int d, int st) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) W::put(m + t * W::kTile, fw[d][t], lane);
+        typename W::Frag f[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) W::template get<!SC>(f[t], m + t * W::kTile, fw[d][t], lane);
+        if constexpr (SC) {
+            if ((st & (Strip::kSteps - 1)) == 0) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) strip[t].put(ms + t * Strip::kTile);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++) f[t].s = Strip::get(ms + t * Strip::kTile, st, lane);
+        }
+        // (the planes share their LDS: what is written is read before the next)
+        mx_bf16x8 hi[NT][4];
+#pragma unroll
+        for (int u = 0; u < NT; u++) {
+            RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u][0], lane);
+#pragma unroll
+            for (int j = 0; j < 4; j++) hi[u][j] = X::piece(mx + u * RowsBf16::kTile, j, lane);
+            RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u][1], lane);
+        }
+        fence();
+        load(d, st + D);
+        fence();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            mx_bf16x8 lo[NT];
+#pragma unroll
+            for (int u = 0; u < NT; u++) lo[u] = X::piece(mx + u * RowsBf16::kTile, j, lane);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const mx_bf16x8 w = W::operand(f[t], j);
+#pragma unroll
+                for (int u = 0; u < NT; u++) {
+                    acc[t][u] = mfma16(w, hi[u][j], acc[t][u]);
+                    acc[t][u] = mfma16(w, lo[u], acc[t][u]);
+                }
+            }
+        }
+        fence();
+    });
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+        if (16 * u + r >= task.n) continue;
+        float *part = a.part + (size_t)choice(task, 16 * u + r) * a.H + o0 + 4 * g;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+            if (o0 + 16 * t < a.H) *reinterpret_cast<mx_f32x4 *>(part + 16 * t) = acc[t][u];
+    }
+}
+
+template <class W, int NT, bool SC>
+__global__ __launch_bounds__(64 * kStreamWaves, !W::mx ? 1 : NT == 1 ? 3 : 2) void k_moe_down_walk(MoeArgs a, int nsh, int nper) {
+    constexpr int LDS = 2 * (W::kTile + (SC ? Strip::kTile : 0)) + NT * RowsBf16::kTile;
+    __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Task task = task_of(a, blockIdx.x, nsh, nper);
+    const int o0 = (task.part * kStreamWaves + wave) * 32;
+    if (task.n == 0 || o0 >= a.H) return;                // (no barrier in this kernel)
+    char *const m = sm + wave * LDS;
+    if (NT > 1 && task.n > 16) down_walk<W, NT, 2, 4, SC>(a, task, o0, m, lane);
+    else if (task.n > 4) down_walk<W, 1, 2, 4, SC>(a, task, o0, m, lane);
+    else down_walk<W, 1, 2, 1, SC>(a, task, o0, m, lane);
+}
+
 // y of up to 16 tokens: 16 outputs a workgroup, the steps of 128 k of every (token,
 // expert) dealt to its 12 wavefronts (9 experts of 4 steps, one token: 3 each, all on
 // their way at once). A step's product lands in the token's column with the
@@ -963,12 +1073,27 @@ int down_stream_run(const MoeArgs &a, size_t slots) {
     return launch_check("k_moe_down_stream");
 }
 
+template <class W, int NT>
+int down_walk_run(const MoeArgs &a, size_t slots) {
+    const size_t nper = cdiv(a.H, 32 * kStreamWaves);
+    const Grid g = grid_of(a, slots, nper, nper);
+    const unsigned threads = 64 * kStreamWaves;
+    const bool strips = W::mx && a.I % 128 == 0 && a.Is % 128 == 0 && ((uintptr_t)a.s_dn | (uintptr_t)a.s_sdn) % 4 == 0;
+    APUS_TIMED("k_moe_down_walk",
+               if (strips) k_moe_down_walk<W, NT, W::mx><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper);
+               else k_moe_down_walk<W, NT, false><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper));
+    return launch_check("k_moe_down_walk");
+}
+
 // The streaming forms from 1024 wavefronts on, 4 a CU (the layer, us split | streamed;
 // up, MXFP4: 16 tokens 65 | 60, 64 tokens 121 | 107, 325 tokens 182 | 160; down: 5 tokens
 // 44 | 39, 64 tokens 133 | 107). bf16 weights' up product is 4 times the bytes a step,
 // which the split form keeps on their way as well with few rows a slot (16 tokens 143 |
-// 150, 64 tokens 297 | 287, 325 tokens 396 | 359). Streaming down needs h of a slot in
-// LDS. k_moe_down_few for work that one round of loads covers (one token: 25 us with the
+// 150, 64 tokens 297 | 287, 325 tokens 396 | 359). k_moe_down_stream where h of a slot fits
+// its LDS, else k_moe_down_walk (128 experts of 768, 8 a token, MXFP4: 16 tokens 89 | 64, 64
+// tokens 133 | 101; bf16 184 | 167, 262 | 242), but the split form where a wavefront's walk
+// is long and the choices are few (60 experts of 1408, a shared one of 5632, 4 tokens 43 |
+// 52; 8 experts of 14336, bf16, 16 tokens 518 | 533, 256 tokens 1279 | 1140). k_moe_down_few for work that one round of loads covers (one token: 25 us with the
 // two kernels, 19 with it; bf16 35 and 29), and for kFewTokens.
 template <class W>
 int experts_run(const MoeArgs &a) {
@@ -982,8 +1107,12 @@ int experts_run(const MoeArgs &a) {
         APUS_TIMED("k_moe_down_few", k_moe_down_few<W><<<(unsigned)a.H / 16, 64 * kFewWaves, 0, stream()>>>(a));
         return launch_check("k_moe_down_few");
     }
-    const bool downs = slots * a.H / 32 >= 1024 && 32 * down_pitch(std::max(a.I, a.Is)) <= kDownH;
-    if (int r = !downs ? down_run<W>(a, slots) : one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, 2>(a, slots))
+    const int inner = std::max(a.I, a.Is);
+    const bool fits = 32 * down_pitch(inner) <= kDownH;
+    const bool downs = slots * a.H / 32 >= 1024 && (inner <= 2048 || a.T * a.k >= 16 * a.E);
+    if (int r = !downs ? down_run<W>(a, slots)
+                : fits ? (one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, 2>(a, slots))
+                       : (one ? down_walk_run<W, 1>(a, slots) : down_walk_run<W, 2>(a, slots)))
         return r;
     APUS_TIMED("k_moe_combine",
                k_moe_combine<<<cdiv((size_t)a.T * (a.H / 4), 256), 256, 0, stream()>>>(a));

@@ -227,7 +227,9 @@ def test_moe_refusals(hip):
                                              (20, 4128, 96, 32, 6, 64), (100, 544, 512, 24, 8, 544),
                                              (200, 2080, 160, 12, 4, 32), (300, 256, 1056, 10, 5, 0),
                                              (70, 2048, 480, 100, 8, 1056), (1000, 96, 64, 130, 2, 64),
-                                             (3, 4128, 1184, 9, 5, 2080), (400, 1056, 480, 20, 5, 96)])
+                                             (3, 4128, 1184, 9, 5, 2080), (400, 1056, 480, 20, 5, 96),
+                                             (40, 1056, 672, 60, 4, 1056), (9, 4128, 640, 40, 6, 32),
+                                             (500, 1056, 768, 16, 4, 640), (90, 2080, 2112, 5, 2, 64)])
 def test_moe_forms(hip, T, H, I, E, topk, Is, mx):
     import torch
     print(f"[moe] forms T={T} H={H} I={I} E={E} topk={topk} Is={Is} mx={mx}", flush=True)
