@@ -58,12 +58,12 @@ __device__ __forceinline__ u32x4 ld16(i32x4 r, uint32_t off, int at) {
 // 32 k from 32 j, group g 8 of them. What lies past K (a multiple of 32) reads as
 // zero, in both operands.
 //
-// Two ways from memory to these operands. load: each lane loads its own (Frag).
-// Neighbouring lanes then read different rows, and the address unit takes such a
-// load a lane at a time, about 60 clocks instead of 16: for calls that wait for
-// latency, not for it. load_raw, put, get: lanes load along the rows (Raw), write
-// what they got to LDS of the wavefront's own and read the operands from there.
-// The LDS places are permuted so that neither side's lanes share banks.
+// From memory to these operands: lanes load along the rows (load_raw), write what
+// they got to LDS of the wavefront's own (put) and read the operands from there
+// (get). Each lane loading its own has neighbouring lanes read different rows, and
+// the address unit takes such a load a lane at a time, about 60 clocks instead of 16
+// (XBf16::load does, for activations of few rows, most lanes' the same). The LDS
+// places are permuted so that neither side's lanes share banks.
 
 // 16 rows of a step of 128 bf16 values: load i has rows 4 i .., 16 lanes a row
 struct RowsBf16 {
@@ -100,16 +100,6 @@ struct WBf16 {
     // up to 16 rows from r0 (uniform) of w [][K]; rows past them read as zero
     static __device__ __forceinline__ Tile tile(const void *w, const uint8_t *, size_t r0, int rows, int K) {
         return {dma_rsrc((const char *)w + r0 * (size_t)K * 2, (uint32_t)rows * (uint32_t)K * 2)};
-    }
-    static __device__ __forceinline__ Lane lane(int l, int K) {
-        return {(uint32_t)(l & 15) * (uint32_t)K * 2 + (l >> 4) * 16};
-    }
-    static __device__ __forceinline__ void load(Frag &f, const Tile &t, const Lane &l, int step, int K) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int k = step * 128 + 32 * j;
-            f.v[j] = ld16(t.w, k < K ? l.off : kPast, k < K ? k * 2 : 0);
-        }
     }
     static __device__ __forceinline__ mx_bf16x8 operand(const Frag &f, int j) {
         return __builtin_bit_cast(mx_bf16x8, f.v[j]);
@@ -150,30 +140,22 @@ struct WMx {
         return {dma_rsrc((const uint8_t *)w + r0 * (size_t)(K / 2), (uint32_t)rows * (uint32_t)(K / 2)),
                 dma_rsrc(ws + r0 * (size_t)(K / kMxBlock), (uint32_t)rows * (uint32_t)(K / kMxBlock))};
     }
-    static __device__ __forceinline__ Lane at(int row, int block, int K) {
-        return {(uint32_t)row * (uint32_t)(K / 2) + block * 16, (uint32_t)row * (uint32_t)(K / kMxBlock) + block};
-    }
-    static __device__ __forceinline__ Lane lane(int l, int K) { return at(l & 15, l >> 4, K); }
-    // block: this lane's of the step (past K: zero codes, at the scale 2^-127)
-    template <bool S = true>
-    static __device__ __forceinline__ void load_block(Frag &f, const Tile &t, const Lane &l, int step, int block, int K) {
-        const int k = step * 128;
-        const bool live = k + 32 * block < K;
-        f.v = ld16(t.w, live ? l.off : kPast, k < K ? k / 2 : 0);
-        if (S) f.s = llvm_raw_buffer_load_u8(t.s, (int)(live ? l.soff : kPast), k < K ? k / kMxBlock : 0, 0);
-    }
-    static __device__ __forceinline__ void load(Frag &f, const Tile &t, const Lane &l, int step, int K) {
-        load_block(f, t, l, step, (threadIdx.x >> 4) & 3, K);
-    }
     static __device__ __forceinline__ mx_bf16x8 operand(const Frag &f, int j) {
         return mx_widen(f.v[j], f.s);
     }
-    // 4 lanes a row; the scales go between lanes without LDS memory, or (S false) are
+    // 4 lanes a row, each a block of the step (past K: zero codes, at the scale
+    // 2^-127); the scales go between lanes without LDS memory, or (S false) are
     // brought in strips (Strip)
-    static __device__ __forceinline__ Lane raw_lane(int l, int K) { return at(l >> 2, l & 3, K); }
+    static __device__ __forceinline__ Lane raw_lane(int l, int K) {
+        const uint32_t row = l >> 2, block = l & 3;
+        return {row * (uint32_t)(K / 2) + block * 16, row * (uint32_t)(K / kMxBlock) + block};
+    }
     template <bool S = true>
     static __device__ __forceinline__ void load_raw(Raw &f, const Tile &t, const Lane &l, int step, int K) {
-        load_block<S>(f, t, l, step, threadIdx.x & 3, K);
+        const int k = step * 128;
+        const bool live = k + 32 * (int)(threadIdx.x & 3) < K;
+        f.v = ld16(t.w, live ? l.off : kPast, k < K ? k / 2 : 0);
+        if (S) f.s = llvm_raw_buffer_load_u8(t.s, (int)(live ? l.soff : kPast), k < K ? k / kMxBlock : 0, 0);
     }
     static __device__ __forceinline__ void put(char *m, const Raw &f, int l) {
         const int row = l >> 2;
