@@ -1,0 +1,45 @@
+// mx_scales.h -- which k the groups of a many-row MXFP4 product take, and how a thread
+// brings a row's scales. Host code too: the reads are checked against the rows' ends
+// on the CPU.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace apus {
+
+// Group grp of G: nk stages of `stage` k from k0 on. (The second half may have a stage
+// less, which it takes as one past K.)
+struct KShare {
+    int k0, nk;
+};
+__host__ __device__ inline KShare k_share(int K, int stage, int G, int grp) {
+    const int nk = ((K + stage - 1) / stage + G - 1) / G;
+    return {grp * nk * stage, nk};
+}
+
+// The first 16 scales of a group, from scale s0 of rows of ks on, are copied to LDS as
+// they are: rows, start and bases in whole 16 bytes, so that the row has 16 from there.
+__host__ __device__ inline bool scales_whole(uint32_t ks, uint32_t s0, const uint8_t *ws, const uint8_t *xs) {
+    return (ks | s0 | (uint32_t)(uintptr_t)ws | (uint32_t)(uintptr_t)xs) % 16 == 0;
+}
+
+// Scales p .. p + 15 (512 k) of a row's ks, for a thread to bring, zeros past the row's
+// end; p < ks. So many at a time because a load whose lanes read different rows takes
+// the address unit a clock a lane, however little each lane reads: 8 bytes a row and
+// stage took it as long as the codes.
+struct RowScales {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 v;
+    __host__ __device__ __forceinline__ void load(const uint8_t *row, uint32_t p, uint32_t ks) {
+        if (ks >= 16) {                                  // (the row's last 16 bytes and a shift)
+            const uint32_t at = p < ks - 16 ? p : ks - 16, past = p - at;
+            __builtin_memcpy(&v, row + at, 16);          // (rows may begin at any byte)
+            if (past) v = __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (8 * (past & 15)));
+        } else {
+            v = u32x4{};
+            for (uint32_t i = p; i < ks; i++) v[(i - p) / 4] |= (uint32_t)row[i] << ((i - p) % 4 * 8);
+        }
+    }
+};
+
+}  // namespace apus

@@ -15,6 +15,7 @@
 #include "apus_host.h"
 #include "mx.h"
 #include "mx_dev.h"
+#include "mx_scales.h"
 #include "tiles.h"
 
 using namespace apus;
@@ -99,24 +100,6 @@ __device__ __forceinline__ void store_tile(char *sm, const f32x16 (&acc)[TO][TMM
     }
 }
 
-// The c-th 16 scale bytes (512 k) of a row's `ks`, for a thread to bring, zeros past
-// the row's end. So many at a time because a load whose lanes read different rows
-// takes the address unit a clock a lane, however little each lane reads: 8 bytes a
-// row and stage took it as long as the codes.
-struct RowScales {
-    u32x4 v;
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t c, uint32_t ks) {
-        if (ks >= 16) {                                  // (the row's last 16 bytes and a shift)
-            const uint32_t at = min(16 * c, ks - 16), past = 16 * c - at;
-            __builtin_memcpy(&v, row + at, 16);          // (rows may begin at any byte)
-            if (past) v = __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (8 * min(past, 15u)));
-        } else {
-            v = u32x4{};
-            for (uint32_t i = 0; i < ks; i++) v[i / 4] |= (uint32_t)row[i] << (i % 4 * 8);
-        }
-    }
-};
-
 // ---- both operands MXFP4 -----------------------------------------------------
 // A stage is 256 k: 128 bytes of codes and 8 of scales per row, BO weight rows,
 // then BM activation rows, double-buffered in LDS. 16-byte chunk c (block c of
@@ -147,14 +130,14 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
     const int wo = wave >> 1, wm = wave & 1, g = lane >> 5;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
     const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
-    const uint32_t kleft = (uint32_t)K / 2, sleft = (uint32_t)K / kMxBlock; // from k0 on
+    const uint32_t kleft = (uint32_t)K / 2, sc0 = (uint32_t)k0 / kMxBlock;   // from k0 on; its first scale
     const int nsc = (min(nk, (K + kMxStage - 1) / kMxStage) + 1) / 2;
     // tile-relative, so that 32-bit offsets do (rows past O or M read the last
     // row; their products are not stored)
     const uint8_t *const wt = a.w + (size_t)o0 * kc + k0 / 2;
     const uint8_t *const xt = (const uint8_t *)a.x + (size_t)m0 * kc + k0 / 2;
-    const uint8_t *const wst = a.ws + (size_t)o0 * ks + k0 / kMxBlock;
-    const uint8_t *const xst = a.xs + (size_t)m0 * ks + k0 / kMxBlock;
+    const uint8_t *const wst = a.ws + (size_t)o0 * ks;
+    const uint8_t *const xst = a.xs + (size_t)m0 * ks;
     auto row_of = [&](int r) {                           // stage row -> row of its operand's tile
         return r < BO ? min(r, O - 1 - o0) : min(r - BO, M - 1 - m0);
     };
@@ -180,7 +163,7 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
 #pragma unroll
         for (int i = 0; i < SPT; i++) {
             const int r = i * 256 + tid;
-            sreg[i].load((r < BO ? wst : xst) + (size_t)row_of(r) * ks, c, sleft);
+            sreg[i].load((r < BO ? wst : xst) + (size_t)row_of(r) * ks, sc0 + 16 * c, ks);
         }
     };
     auto put_scales = [&](int c) {
@@ -257,14 +240,14 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
     using s3 = std::integral_constant<int, 3>;
     Frag f0, f1;
     Scale c0, c1;
-    // the first scales go with the copies where rows of them are whole 16 bytes (a
-    // wait for registers here is one for all the copies)
-    const bool whole = (ks | (uint32_t)(uintptr_t)a.ws | (uint32_t)(uintptr_t)a.xs) % 16 == 0;
+    // the first scales go with the copies where they are whole 16 bytes (a wait for
+    // registers here is one for all the copies)
+    const bool whole = scales_whole(ks, sc0, a.ws, a.xs);
     if (whole) {
 #pragma unroll
         for (int i = 0; i < SPT; i++) {
             const int p = wave * SPT + i;                // (64 rows)
-            copy16(row_of(p * 64 + lane) * ks, uniform(p * 64 < BO ? wst : xst), lds0 + 2 * SB + p * 1024, -1);
+            copy16(row_of(p * 64 + lane) * ks + sc0, uniform(p * 64 < BO ? wst : xst), lds0 + 2 * SB + p * 1024, -1);
         }
     } else {
         load_scales(0);
@@ -367,9 +350,9 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     const int wo = wave >> 1, wm = wave & 1, g = lane >> 5;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
     const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
-    const uint32_t kleft = (uint32_t)K / 2, sleft = (uint32_t)K / kMxBlock, kx = (uint32_t)K * 2;    // from k0 on
+    const uint32_t kleft = (uint32_t)K / 2, kx = (uint32_t)K * 2, sc0 = (uint32_t)k0 / kMxBlock;      // from k0 on; its first scale
     const int nch = (nk + CPS - 1) / CPS, nsc = (min(nk, (K + kMx16Stage - 1) / kMx16Stage) + 7) / 8;
-    const uint8_t *const wrow = a.ws + (size_t)(o0 + min(tid % BO, O - 1 - o0)) * ks + k0 / kMxBlock;
+    const uint8_t *const wrow = a.ws + (size_t)(o0 + min(tid % BO, O - 1 - o0)) * ks;
     const void *const wt = uniform(a.w + (size_t)o0 * kc + k0 / 2),
                *const xt = uniform((const uint16_t *)a.x + (size_t)m0 * ldx + k0);
     const uint32_t cg = slot_of<128>(lane & 7, lane >> 3) * 16, wg = slot_of<RB>(lane % CH, lane / CH) * 16;
@@ -472,13 +455,13 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     using i2 = std::integral_constant<int, 2>;
     using i3 = std::integral_constant<int, 3>;
     // chunk 0, and what the loop finds under way: stages 0 and 1, a quarter of chunk 1
-    const bool whole = (ks | (uint32_t)(uintptr_t)a.ws) % 16 == 0;      // (as above)
+    const bool whole = scales_whole(ks, sc0, a.ws, nullptr);             // (as above)
     if (whole) {
         // (64 rows a wavefront; past the tile's, into the other slot, not in use yet)
         const int row = min(wave * 64 + lane, min(BO - 1, O - 1 - o0));
-        copy16((uint32_t)row * ks, uniform(a.ws + (size_t)o0 * ks + k0 / kMxBlock), lds0 + S0 + wave * 1024, -1);
+        copy16((uint32_t)row * ks + sc0, uniform(a.ws + (size_t)o0 * ks), lds0 + S0 + wave * 1024, -1);
     } else {
-        sreg.load(wrow, 0, sleft);
+        sreg.load(wrow, sc0, ks);
     }
 #pragma unroll
     for (int q = 0; q < CPS; q++)
@@ -504,7 +487,7 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     }
     for (int kt = 0; kt < nk - 1; kt++) {
         const bool sc = (kt & 7) == 0;     // (the slot's last reader was stage kt - 1)
-        if (sc) sreg.load(wrow, min(kt / 8 + 1, nsc - 1), sleft);
+        if (sc) sreg.load(wrow, sc0 + 16 * min(kt / 8 + 1, nsc - 1), ks);
         step(f0, f1, yes{}, kt, i1{}, r0, no{}, r1, no{}, 0);
         step(f1, f0, yes{}, kt, i2{}, r0, no{}, r1, no{}, 0);
         step(f0, f1, yes{}, kt, i3{}, r0, no{}, r1, no{}, 0);
@@ -556,8 +539,7 @@ __device__ __forceinline__ void wide_tile(char *sm, const MxProduct &a, int o0, 
     constexpr int LDS = kWideLds<XMX, TO, TMM, RB>, STAGE = XMX ? kMxStage : kMx16Stage;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int grp = wave >> 2, w = wave & 3;
-    // (the second half may have a stage less, which it takes as one past K)
-    const int nk = ((a.K + STAGE - 1) / STAGE + G - 1) / G, k0 = grp * nk * STAGE;
+    const auto [k0, nk] = k_share(a.K, STAGE, G, grp);
     f32x16 acc[TO][TMM];
     if constexpr (XMX) mx_tile<TO, TMM>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
     else mx16_tile<TO, TMM, RB>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
