@@ -38,7 +38,7 @@ __device__ __forceinline__ mx_bf16x8 mx_widen(uint32_t c, uint32_t s) {
 // registers, a lane's offset and a uniform one, so that a tile's 16 rows take
 // one address register (as 64-bit pointers the loops' addresses did not fit the
 // registers), and an offset past the size reads zero (the uniform offset stays
-// under the size: the check subtracts it).
+// under the size, which no tile has zero of: the check subtracts it).
 __device__ f32x4_t llvm_raw_buffer_load_v4f32(i32x4 r, int voff, int soff, int aux)
     __asm("llvm.amdgcn.raw.buffer.load.v4f32");
 __device__ float llvm_raw_buffer_load_f32(i32x4 r, int voff, int soff, int aux)

@@ -1,13 +1,23 @@
-// mx_scales.h -- which k the groups of a many-row MXFP4 product take, and how a thread
-// brings a row's scales. Host code too: the reads are checked against the rows' ends
-// on the CPU.
+// mx_reads.h -- which rows, k and scales the MXFP4 products read. Host code too: the
+// reads are checked against the operands' ends on the CPU.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 namespace apus {
 
-// Group grp of G: nk stages of `stage` k from k0 on. (The second half may have a stage
+// The 16 rows from `first` of `total`: those there are. With none left the last row
+// again, for a tile whose products are not stored: a buffer of no bytes would end before
+// the uniform offset that its loads add, which the bounds check is not made for.
+struct Rows16 {
+    int first, n;
+};
+__host__ __device__ inline Rows16 rows16(int first, int total) {
+    const int left = total - first;
+    return left > 0 ? Rows16{first, left < 16 ? left : 16} : Rows16{total - 1, 1};
+}
+
+// Group grp of G of a many-row product: nk stages of `stage` k from k0 on. (The second half may have a stage
 // less, which it takes as one past K.)
 struct KShare {
     int k0, nk;

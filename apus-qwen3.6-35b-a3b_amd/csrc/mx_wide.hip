@@ -15,7 +15,7 @@
 #include "apus_host.h"
 #include "mx.h"
 #include "mx_dev.h"
-#include "mx_scales.h"
+#include "mx_reads.h"
 #include "tiles.h"
 
 using namespace apus;

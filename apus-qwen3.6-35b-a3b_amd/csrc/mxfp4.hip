@@ -13,6 +13,7 @@
 #include "apus_host.h"
 #include "mx.h"
 #include "mx_dev.h"
+#include "mx_reads.h"
 
 using namespace apus;
 
@@ -102,23 +103,25 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_mx_gemm_few(const uint8_t *_
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = (blockIdx.x % nbo) * 16 * RT, m0 = (blockIdx.x / nbo) * 16 * NT;
     char *const mine = sm + wave * PART, *const mx = mine + RT * 1024;
-    // (outputs past O and rows past M read as zero, and are not stored)
+    // (outputs past O and rows past M read as zero or as the last one, and are not stored)
     WMx::Tile wt[RT], xt[NT];
     i32x4 xb[NT];
     uint32_t xl[NT][4];
     const uint32_t pitch = (uint32_t)ldx * 2;
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-        wt[t] = WMx::tile(w, ws, min(o0 + 16 * t, O - 1), max(0, min(16, O - o0 - 16 * t)), K);
+    for (int t = 0; t < RT; t++) {
+        const Rows16 o = rows16(o0 + 16 * t, O);
+        wt[t] = WMx::tile(w, ws, o.first, o.n, K);
+    }
 #pragma unroll
     for (int u = 0; u < NT; u++) {
-        const int m = min(m0 + 16 * u, M - 1), rows = max(0, min(16, M - m0 - 16 * u));
+        const Rows16 m = rows16(m0 + 16 * u, M);
         if constexpr (XMX) {
-            xt[u] = WMx::tile(x, xs, m, rows, K);
+            xt[u] = WMx::tile(x, xs, m.first, m.n, K);
         } else {
-            xb[u] = dma_rsrc((const uint16_t *)x + (size_t)m * ldx, rows ? (rows - 1) * pitch + K * 2 : 0);
+            xb[u] = dma_rsrc((const uint16_t *)x + (size_t)m.first * ldx, (m.n - 1) * pitch + K * 2);
 #pragma unroll
-            for (int i = 0; i < 4; i++) xl[u][i] = 4 * i + g < rows ? (4 * i + g) * pitch : kPast - 256;
+            for (int i = 0; i < 4; i++) xl[u][i] = 4 * i + g < m.n ? (4 * i + g) * pitch : kPast - 256;
         }
     }
     const auto wl = WMx::raw_lane(lane, K);

@@ -1,11 +1,11 @@
-// Host driver: the reads of a many-row MXFP4 product's scales (csrc/mx_scales.h), for
-// every group of every K up to the number given, in buffers that end where the rows do.
-// Built with the address sanitizer, which reports a read past them.
+// Host driver: what the MXFP4 products read (csrc/mx_reads.h), in buffers that end where
+// the operands do: the scales of every group of every K up to the number given, the rows
+// of every tile. Built with the address sanitizer, which reports a read past them.
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
 
-#include "mx_scales.h"
+#include "mx_reads.h"
 
 using namespace apus;
 
@@ -42,6 +42,19 @@ static void group(int K, int stage, int G, int grp) {
     free(buf);
 }
 
+// the tiles of workgroups of `tiles` 16 rows; a load adds a uniform offset of up to the
+// last step's, which has to stay under the tile's bytes
+static void tiles_of(int total, int tiles) {
+    const int K = 416, stage = 128, G = tiles, grp = total, pitch = K / 2;
+    for (int r0 = 0; r0 < total; r0 += 16 * tiles)
+        for (int t = 0; t < tiles; t++) {
+            const Rows16 r = rows16(r0 + 16 * t, total);
+            CHECK(r.n >= 1 && r.n <= 16 && r.first >= 0 && r.first + r.n <= total);
+            CHECK(r0 + 16 * t >= total || (r.first == r0 + 16 * t && r.first + r.n == (total < r.first + 16 ? total : r.first + 16)));
+            for (int k = 0; k < K; k += stage) CHECK(k / 2 < r.n * pitch);
+        }
+}
+
 int main(int argc, char **argv) {
     const int last = argc > 1 ? atoi(argv[1]) : 8192;
     for (int K = 32; K <= last; K += 32)
@@ -50,6 +63,8 @@ int main(int argc, char **argv) {
                 if (G == 2 && K <= stage) continue;      // (halves need a stage each)
                 for (int grp = 0; grp < G; grp++) group(K, stage, G, grp);
             }
+    for (int total = 1; total <= 300; total++)
+        for (int tiles = 1; tiles <= 4; tiles++) tiles_of(total, tiles);
     printf("%s\n", bad ? "FAILED" : "ok");
     return bad != 0;
 }

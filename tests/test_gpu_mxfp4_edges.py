@@ -1,6 +1,6 @@
-"""GPU parity: MXFP4 products whose K is taken in two halves side by side (tiles of
-128 x 128, at most one a CU), within the bound of fp32 accumulation and one bf16
-rounding."""
+"""GPU parity at the edges of the MXFP4 products, within the bound of fp32
+accumulation and one bf16 rounding: K taken in two halves side by side (tiles of
+128 x 128, at most one a CU), and tiles of the few-row form with nothing in them."""
 import pytest
 
 import mx_ref
@@ -51,3 +51,19 @@ def test_scales_of_the_second_half(hip, M, O, K, mx):
     y, xv = _product(hip, torch, w, ws, x, mx)
     r, b = mx_ref.gemm(mx_ref.values(w, ws), xv)
     mx_ref.check(y, r, b, f"halves mx={mx}")
+
+
+# outputs that end before the second (2 x 16 a workgroup) or before one of the last
+# tiles (4 x 16), rows before the last of 3 or 4 tiles; K of many steps
+@pytest.mark.parametrize("M,O,K", [(3, 8200, 4128), (30, 12353, 2080), (65, 130, 4096), (97, 517, 2208),
+                                   (60, 12305, 2080), (113, 8211, 1056), (129, 40, 1568)])
+@pytest.mark.parametrize("mx", [False, True])
+def test_tiles_with_nothing_in_them(hip, M, O, K, mx):
+    import torch
+    print(f"[mx] empty tiles M={M} O={O} K={K} mx={mx}", flush=True)
+    g = _gen(torch, M + O + K)
+    x = mx_ref.normal(g, M, K)
+    w, ws = mx_ref.quantize(mx_ref.normal(g, O, K, scale=K ** -0.5))
+    y, xv = _product(hip, torch, _bytes_at_end(torch, w), _bytes_at_end(torch, ws), x, mx)
+    r, b = mx_ref.gemm(mx_ref.values(w, ws), xv)
+    mx_ref.check(y, r, b, f"empty tiles mx={mx}")
