@@ -17,14 +17,16 @@ __host__ __device__ inline Rows16 rows16(int first, int total) {
     return left > 0 ? Rows16{first, left < 16 ? left : 16} : Rows16{total - 1, 1};
 }
 
-// Group grp of G of a many-row product: nk stages of `stage` k from k0 on. (The second half may have a stage
-// less, which it takes as one past K.)
+// Group grp of G (1 or 2) of a many-row product: n of the K elements, from k0 on, in nk
+// stages of `stage`. All but the last of a group's stages are whole: the kernels mask
+// what lies past its k in the last one only. With K in halves, an odd number of stages
+// leaves the first half one less, which it takes as one past its k.
 struct KShare {
-    int k0, nk;
+    int k0, n, nk;
 };
 __host__ __device__ inline KShare k_share(int K, int stage, int G, int grp) {
-    const int nk = ((K + stage - 1) / stage + G - 1) / G;
-    return {grp * nk * stage, nk};
+    const int all = (K + stage - 1) / stage, nk = (all + G - 1) / G, half = all / 2 * stage;
+    return G == 1 ? KShare{0, K, nk} : grp == 0 ? KShare{0, half, nk} : KShare{half, K - half, nk};
 }
 
 // The first 16 scales of a group, from scale s0 of rows of ks on, are copied to LDS as

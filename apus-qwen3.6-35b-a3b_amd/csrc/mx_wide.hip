@@ -106,14 +106,14 @@ __device__ __forceinline__ void store_tile(char *sm, const f32x16 (&acc)[TO][TMM
 // the stage) of row r lies at slot c ^ (r % 8), so that the 8 rows of one LDS
 // read phase hit 8 distinct slots. MFMA step s takes 64 k: lane (row l % 32,
 // half g = l / 32) chunk 2 s + g, and the scale byte of the same number.
-// Blocks past K (in the last stage): zero codes and scale 1 on both sides.
+// Blocks past the group's k (in its last stage): zero codes and scale 1 on both sides.
 // Scales come for two stages at a time, through registers.
 constexpr int kMxStage = 256;
 
 template <int TO, int TMM>
 constexpr int kMxLds = 2 * 64 * (TO + TMM) * (kMxStage / 2 + 16);
 template <int TO, int TMM>
-__device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, int m0, int k0, int nk,
+__device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, int m0, const KShare &share,
                                         f32x16 (&acc)[TO][TMM]) {
     constexpr int BO = 64 * TO, BM = 64 * TMM, ROWS = BO + BM;
     constexpr int PB = BO * 128, SB = ROWS * 128;
@@ -124,13 +124,13 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
     static_assert(ROWS % 256 == 0, "rows must split evenly over the threads");
     static_assert(2 * (SB + SCB) == kMxLds<TO, TMM>);
     char *const scales = sm + 2 * SB;
-    const int M = a.M, O = a.O, K = a.K - k0;            // K: from k0 on
+    const int M = a.M, O = a.O, k0 = share.k0, K = share.n, nk = share.nk;    // K: of this group
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     const int wo = wave >> 1, wm = wave & 1, g = lane >> 5;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
     const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
-    const uint32_t kleft = (uint32_t)K / 2, sc0 = (uint32_t)k0 / kMxBlock;   // from k0 on; its first scale
+    const uint32_t kleft = (uint32_t)K / 2, sc0 = (uint32_t)k0 / kMxBlock;   // of the group's k; its first scale
     const int nsc = (min(nk, (K + kMxStage - 1) / kMxStage) + 1) / 2;
     // tile-relative, so that 32-bit offsets do (rows past O or M read the last
     // row; their products are not stored)
@@ -279,7 +279,7 @@ __device__ __forceinline__ void mx_tile(char *sm, const MxProduct &a, int o0, in
         step(s3{}, f1, c0, f0, yes{}, kt + 1, 0, yes{}, kt + 2, live);
         c0 = c1;
     }
-    // the last stage, with what lies past K masked
+    // the last stage, with what lies past the group's k masked
     const int left = K - (nk - 1) * kMxStage;
     if (left < kMxStage) {
 #pragma unroll
@@ -333,7 +333,7 @@ __device__ __forceinline__ int slot_of(int c, int r) { return c ^ (RB == 128 ? r
 template <int TO, int TMM, int RB>
 constexpr int kMx16Lds = 2 * 64 * (TMM * kMx16Stage * 2 + TO * (RB + 16));
 template <int TO, int TMM, int RB>
-__device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, int m0, int k0, int nk,
+__device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, int m0, const KShare &share,
                                           f32x16 (&acc)[TO][TMM]) {
     constexpr int BO = 64 * TO, BM = 64 * TMM;
     constexpr int XB = BM * 128, WB = BO * RB, SCB = BO * 16;
@@ -342,7 +342,7 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     constexpr int NF = TO * TMM;
     constexpr int W0 = 2 * XB, S0 = 2 * (XB + WB);
     static_assert(S0 + 2 * SCB == (kMx16Lds<TO, TMM, RB>) && BO <= 256);
-    const int M = a.M, O = a.O, K = a.K - k0;            // K: from k0 on
+    const int M = a.M, O = a.O, k0 = share.k0, K = share.n, nk = share.nk;    // K: of this group
     const size_t ldx = a.ldx;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
@@ -350,7 +350,7 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
     const int wo = wave >> 1, wm = wave & 1, g = lane >> 5;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void *)sm);
     const uint32_t kc = (uint32_t)a.K / 2, ks = (uint32_t)a.K / kMxBlock;   // bytes of a row
-    const uint32_t kleft = (uint32_t)K / 2, kx = (uint32_t)K * 2, sc0 = (uint32_t)k0 / kMxBlock;      // from k0 on; its first scale
+    const uint32_t kleft = (uint32_t)K / 2, kx = (uint32_t)K * 2, sc0 = (uint32_t)k0 / kMxBlock;      // of the group's k; its first scale
     const int nch = (nk + CPS - 1) / CPS, nsc = (min(nk, (K + kMx16Stage - 1) / kMx16Stage) + 7) / 8;
     const uint8_t *const wrow = a.ws + (size_t)(o0 + min(tid % BO, O - 1 - o0)) * ks;
     const void *const wt = uniform(a.w + (size_t)o0 * kc + k0 / 2),
@@ -499,7 +499,7 @@ __device__ __forceinline__ void mx16_tile(char *sm, const MxProduct &a, int o0, 
         step(f1, f0, yes{}, kt + 1, i0{}, r0, yes{}, r1, yes{}, kt);
         r0 = r1;
     }
-    // the last stage; half of it, with a second share of K all, may lie past K
+    // the last stage; half of it, or with K in halves all, may lie past the group's k
     const bool past = (nk - 1) * kMx16Stage + 32 * g >= K;
     auto mask = [&](Frag &f) {
         if (!past) return;
@@ -539,10 +539,10 @@ __device__ __forceinline__ void wide_tile(char *sm, const MxProduct &a, int o0, 
     constexpr int LDS = kWideLds<XMX, TO, TMM, RB>, STAGE = XMX ? kMxStage : kMx16Stage;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int grp = wave >> 2, w = wave & 3;
-    const auto [k0, nk] = k_share(a.K, STAGE, G, grp);
+    const KShare share = k_share(a.K, STAGE, G, grp);
     f32x16 acc[TO][TMM];
-    if constexpr (XMX) mx_tile<TO, TMM>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
-    else mx16_tile<TO, TMM, RB>(sm + grp * LDS, a, o0, m0, k0, nk, acc);
+    if constexpr (XMX) mx_tile<TO, TMM>(sm + grp * LDS, a, o0, m0, share, acc);
+    else mx16_tile<TO, TMM, RB>(sm + grp * LDS, a, o0, m0, share, acc);
     if constexpr (G == 2) {                // the sum of the halves, in the first's registers
         char *p = sm + LDS + w * (TO * TMM * 4096) + lane * 16;
         static_assert(4 * TO * TMM * 4096 <= LDS, "the second half's sums fit its LDS");

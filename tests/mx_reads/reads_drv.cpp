@@ -19,8 +19,11 @@ static int bad = 0;
 static void group(int K, int stage, int G, int grp) {
     const KShare sh = k_share(K, stage, G, grp);
     const uint32_t ks = K / 32, s0 = sh.k0 / 32, rows = 3;
-    const int left = (K - sh.k0 + stage - 1) / stage, own = sh.nk < left ? sh.nk : left, per = 512 / stage;
-    CHECK(sh.k0 < K && sh.k0 % stage == 0);
+    const int own = (sh.n + stage - 1) / stage, per = 512 / stage;
+    CHECK(sh.n > 0 && sh.k0 % stage == 0 && (grp == 0) == (sh.k0 == 0));
+    CHECK(sh.k0 + sh.n == (grp == G - 1 ? K : k_share(K, stage, G, 1).k0));       // all of K, once
+    CHECK(sh.nk == k_share(K, stage, G, 0).nk && own <= sh.nk);                   // (as many barriers)
+    CHECK((sh.nk - 1) * stage <= sh.n);                                           // whole, but for the last
     uint8_t *const buf = (uint8_t *)malloc(rows * ks);   // (16-byte aligned)
     for (uint32_t i = 0; i < rows * ks; i++) buf[i] = (uint8_t)(i * 37 + 11);
     for (uint32_t r = 0; r < rows; r++) {
