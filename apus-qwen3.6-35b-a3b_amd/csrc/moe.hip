@@ -1148,6 +1148,19 @@ int check_weights(const ApusHipMoeLayer *L) {
     return kOk;
 }
 
+// y of T tokens shares bytes with a weight
+bool over_weights(const ApusHipMoeLayer *L, size_t T, const uint16_t *y) {
+    const size_t H = L->hidden, down = L->experts * H * L->inter, sdown = H * L->shared_inter;    // elements
+    auto over = [&](const void *p, size_t bytes) { return bytes && block_overlaps(p, bytes, y, T * H * 2, T * H * 2, 1); };
+    auto weight = [&](const void *p, const uint8_t *s, size_t n) {
+        return over(p, L->mxfp4 ? n / 2 : n * 2) || (L->mxfp4 && over(s, n / kMxBlock));
+    };
+    return over(L->w_router, L->experts * H * 2) || weight(L->w_gate_up, L->s_gate_up, 2 * down) ||
+           weight(L->w_down, L->s_down, down) || weight(L->w_shared_gate_up, L->s_shared_gate_up, 2 * sdown) ||
+           weight(L->w_shared_down, L->s_shared_down, sdown) ||
+           (sdown && L->w_shared_gate && over(L->w_shared_gate, H * 2));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1227,6 +1240,7 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
         if (!x || !y) return set_error(kErrArgument, "NULL operand");
         if ((uintptr_t)x % 16 || (uintptr_t)y % 16)
             return set_error(kErrUnsupported, "x and y need 16-byte alignment");
+        if (over_weights(L, T, y)) return set_error(kErrArgument, "the output overlaps the weights");
     }
     if (int r = mx_ready()) return r;
     if (w->device != current_device())

@@ -9,6 +9,13 @@ namespace apus {
 int mx_check_dims(size_t M, size_t O, size_t K);   // sizes under 2^31, K in whole blocks
 int mx_ready();                                    // ensure_ready, on the calling thread's device
 
+// A block of nb bytes and M rows (first row, bytes between rows, bytes of a row) share bytes.
+inline bool block_overlaps(const void *b, size_t nb, const void *rows, size_t pitch, size_t n, size_t M) {
+    const uintptr_t b0 = (uintptr_t)b, r0 = (uintptr_t)rows;
+    const size_t i = b0 < r0 + n ? 0 : (b0 - r0 - n) / pitch + 1;    // the first row that ends past b0
+    return i < M && r0 + i * pitch < b0 + nb;
+}
+
 // y = x w^T: M rows, O outputs, K inner elements; x is bf16 rows of pitch ldx, or,
 // with xs, MXFP4
 struct MxProduct {

@@ -238,6 +238,8 @@ int gemm_check(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t
     if (!w || !ws || !x) return set_error(kErrArgument, "NULL operand");
     if ((uintptr_t)w % 16) return set_error(kErrUnsupported, "MXFP4 codes need 16-byte alignment");
     const size_t mxk = K / 2, mxs = K / kMxBlock;
+    if (block_overlaps(w, O * mxk, y, ldy * 2, O * 2, M) || block_overlaps(ws, O * mxs, y, ldy * 2, O * 2, M))
+        return set_error(kErrArgument, "the output overlaps the weights");
     if (xs) {
         if ((uintptr_t)x % 16)
             return set_error(kErrUnsupported, "MXFP4 codes need 16-byte alignment");

@@ -641,8 +641,8 @@ typedef struct ApusHipMoeWork ApusHipMoeWork;
 int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHipMoeWork **out);
 int apus_hip_moe_work_destroy(ApusHipMoeWork *w);
 
-/* x [T][hidden] -> y [T][hidden], bf16, 16-byte aligned; y may be x. T up to
- * the workspace's (0: nothing is done). Neither allocates nor waits, and may
+/* x [T][hidden] -> y [T][hidden], bf16, 16-byte aligned; y may be x, and may not
+ * overlap the weights. T up to the workspace's (0: nothing is done). Neither allocates nor waits, and may
  * be captured into a graph. */
 int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_t T,
                               const uint16_t *x, uint16_t *y);

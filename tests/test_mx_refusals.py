@@ -122,3 +122,25 @@ def test_disabled_first():
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
                        env=dict(os.environ, APUS_HIP_DISABLE="1"))
     assert r.returncode == 0 and r.stdout.split() == ["2"] * 5, (r.stdout, r.stderr)
+
+
+def last_error():
+    b = C.create_string_buffer(512)
+    apus_hip.load().apus_hip_last_error(b, SZ(512))
+    return b.value.decode()
+
+
+def test_gemm_output_over_weights():
+    """y among the codes or scales of the weights: from the first byte to the last, by
+    any of its rows. Between y's rows there is room for them."""
+    ld = 1 << 12                                           # rows of y 8 KiB apart, 20 bytes each
+    for f in (gemm, gemm_mx):
+        for k, p, n in (("w", A, 320), ("ws", B, 20)):     # 10 rows of 64
+            for kw in (dict(y=p), dict(y=off(p, n - 2)), dict(y=off(p, -2 * 9)),
+                       dict(y=off(p, n - 2 - 3 * 2 * ld), ldy=ld), {k: off(E, 3 * 2 * ld + 16), "ldy": ld},
+                       {k: off(E, 2 * ld - 16), "ldy": ld}):
+                assert f(**kw) == ARG and last_error() == "the output overlaps the weights", kw
+            # (the next check is reached: x among y's rows)
+            for kw in (dict(y=off(p, n), x=off(p, (n + 15) // 16 * 16)), dict(y=off(p, -80), x=off(p, -64)),
+                       {k: off(E, 2 * ld + 32), "ldy": ld, "x": E}):
+                assert f(**kw) == ARG and last_error() == "the output overlaps the activations", kw
