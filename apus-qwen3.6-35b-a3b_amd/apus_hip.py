@@ -199,10 +199,10 @@ _device = 0                                # the library's GPU
 def init(device=0):
     global _device
     err = C.create_string_buffer(512)
-    _device = device
     rc = load().apus_hip_init(C.c_int(device), err, 512)
     if rc != 0:
         raise ApusHipError(rc, err.value.decode(errors="replace"))
+    _device = device
 
 
 def set_stream(stream_handle):

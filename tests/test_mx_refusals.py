@@ -144,3 +144,17 @@ def test_gemm_output_over_weights():
             for kw in (dict(y=off(p, n), x=off(p, (n + 15) // 16 * 16)), dict(y=off(p, -80), x=off(p, -64)),
                        {k: off(E, 2 * ld + 32), "ldy": ld, "x": E}):
                 assert f(**kw) == ARG and last_error() == "the output overlaps the activations", kw
+
+
+def test_refused_device_is_not_kept():
+    """A device that init refuses is not the one that the binding expects tensors on."""
+    before = apus_hip._device
+    try:
+        with pytest.raises(apus_hip.ApusHipError):
+            apus_hip.init(1000)
+        assert apus_hip._device == before
+    finally:
+        try:
+            apus_hip.init(before)
+        except apus_hip.ApusHipError:                      # (no GPU here)
+            pass
