@@ -806,7 +806,7 @@ def mxfp4_gemm(w, ws, x, y):
 
 def mxfp4_gemm_mx(w, ws, x, xs, y):
     """As mxfp4_gemm with the activations in MXFP4: x [M, K/2], xs [M, K/32]."""
-    dev, M, K, O = _device, x.shape[0], x.shape[1] * 2, w.shape[0]
+    dev, M, K, O = _device, x.shape[0], x.shape[-1] * 2, w.shape[0]
     yp, ym, _, ldy = _rows(y, "y", dev, O)
     if ym != M:
         raise ValueError(f"y: {ym} rows, expected {M}")
@@ -834,7 +834,9 @@ def moe_layer(dims, w, norm_topk=True):
     ptr = {}
 
     def take(name, shape, size):
-        t = w[name]
+        t = w.get(name)
+        if t is None:
+            raise ValueError(f"{name}: no such weight, expected one of shape {shape}")
         if (not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != shape
                 or not (_bf16(t) if size == 2 else t.element_size() == 1)):
             raise ValueError(f"{name}: a contiguous GPU tensor of {'bf16' if size == 2 else 'bytes'} of shape {shape}, "

@@ -47,3 +47,19 @@ def test_output_over_weights_is_refused(hip, mx):
     hip.moe_layer_decode(_layer(hip, dict(w, w_router=r), k), work, x, y)
     assert torch.equal(y, y1)
     work.destroy()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_layer_without_a_weight_is_refused(hip, mx):
+    import torch
+    w = mx_ref.moe_weights(_gen(torch, 6), 64, 32, 8, 32, True, mx)
+    _layer(hip, {n: t for n, t in w.items() if n != "w_shared_gate"}, 2)         # (may be left out)
+    for n in set(w) - {"w_shared_gate", "s_gate_up"}:
+        for v in ({m: t for m, t in w.items() if m != n}, dict(w, **{n: None})):
+            with pytest.raises(ValueError, match=n):
+                hip.moe_layer((64, 32, 8, 2, 32), v)
+    if mx:                                                 # (codes are no bf16 weights)
+        with pytest.raises(ValueError, match="w_gate_up"):
+            hip.moe_layer((64, 32, 8, 2, 32), {m: t for m, t in w.items() if m != "s_gate_up"})
+        with pytest.raises(ValueError, match="s_gate_up"):
+            hip.moe_layer((64, 32, 8, 2, 32), dict(w, s_gate_up=None))

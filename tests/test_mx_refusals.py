@@ -158,3 +158,17 @@ def test_refused_device_is_not_kept():
             apus_hip.init(before)
         except apus_hip.ApusHipError:                      # (no GPU here)
             pass
+
+
+def test_moe_layer_without_a_weight():
+    for w in ({}, {"w_router": None}, {"s_gate_up": None}):
+        with pytest.raises(ValueError, match="w_router"):
+            apus_hip.moe_layer((64, 32, 8, 2, 0), w)
+
+
+def test_gemm_mx_of_a_vector():
+    torch = pytest.importorskip("torch")
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)
+    for x in (u8(32), u8(1, 1, 32)):
+        with pytest.raises(ValueError):
+            apus_hip.mxfp4_gemm_mx(u8(5, 32), u8(5, 2), x, u8(1, 2), torch.zeros(1, 5, dtype=torch.bfloat16))
