@@ -392,12 +392,19 @@ __device__ __forceinline__ uint32_t h_at(const MoeArgs &a, int q, bool sh) {
 }
 __device__ __forceinline__ uint32_t h_all(const MoeArgs &a) { return 2 * a.T * (a.k * a.I + a.Is); }
 
-// h as its leading bits, cut, and the rest, rounded (none of an infinity or NaN)
+// h as its leading bits, cut, and the rest, rounded. Both have h's sign, and (from 2^-132
+// on) neither is zero where h is not, nor finite where h is infinite: times an infinite
+// weight, zero would make NaN of an infinite y. An h of 8 bits is split a bit below them.
 __device__ __forceinline__ void split_h(float v, uint16_t &hi, uint16_t &lo) {
     const uint32_t bits = __float_as_uint(v);
-    const bool fin = (bits & 0x7f800000u) != 0x7f800000u;
-    hi = fin ? (uint16_t)(bits >> 16) : f2bf(v);
-    lo = fin ? f2bf(v - bf2f(hi)) : 0;
+    if ((bits & 0x7f800000u) == 0x7f800000u) {
+        hi = lo = f2bf(v);
+        return;
+    }
+    uint32_t h = bits >> 16;
+    lo = f2bf(v - bf2f((uint16_t)h));
+    if ((lo & 0x7fffu) == 0 && (h & 0x7fffu) > 1) lo = f2bf(v - bf2f((uint16_t)--h));
+    hi = (uint16_t)h;
 }
 
 // Two forms of each expert kernel. k_moe_up and k_moe_down share a row block's K

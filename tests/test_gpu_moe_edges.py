@@ -63,3 +63,45 @@ def test_layer_without_a_weight_is_refused(hip, mx):
             hip.moe_layer((64, 32, 8, 2, 32), {m: t for m, t in w.items() if m != "s_gate_up"})
         with pytest.raises(ValueError, match="s_gate_up"):
             hip.moe_layer((64, 32, 8, 2, 32), dict(w, s_gate_up=None))
+
+
+# k_moe_down_few, _down, _down_stream and _down_walk
+@pytest.mark.parametrize("T,H,I,E,k", [(1, 256, 64, 8, 2), (13, 256, 64, 8, 2), (64, 1024, 64, 64, 8),
+                                       (64, 1024, 544, 64, 8), (300, 1024, 64, 16, 4)])
+@pytest.mark.parametrize("kind", ["bf16", "mx", "overflow"])
+def test_infinite_down_weights(hip, T, H, I, E, k, kind):
+    """Inner values of few bits (64 times a number of e2m1), or past fp32, and one
+    infinite weight an output, or all of them: y is infinite with its sign."""
+    import torch
+    mx = kind == "mx"
+    g = _gen(torch, T + I)
+    w = mx_ref.moe_weights(g, H, I, E, 0, False, False)
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = 1
+    gu = w["w_gate_up"]
+    gu[:] = 0
+    gu[:, :I, 0] = 64 if kind != "overflow" else 2.0 ** 100
+    gu[:, I:, 0] = torch.tensor([1, 2, 3, 4, 6, 1.5, 0.5, 1], device="cuda").repeat(I // 8).to(torch.bfloat16) * (
+        1 if kind != "overflow" else 2.0 ** 60)
+    o = torch.arange(H, device="cuda")
+    sign = (1 - 2 * (o % 2)).to(torch.bfloat16)
+    if kind == "overflow":
+        w["w_down"][:] = sign[None, :, None] * float("inf")
+    elif not mx:
+        w["w_down"][:, o, o % I] = sign * float("inf")
+    else:
+        for n in ("gate_up", "down"):
+            w["w_" + n], w["s_" + n] = mx_ref.quantize(w["w_" + n])
+        at = o % I                                         # the element's block: one code of 6, at 2^127
+        w["s_down"][:, o, at // 32] = 254
+        blocks = w["w_down"].view(E, H, I // 32, 16)
+        blocks[:, o, at // 32] = 0
+        blocks[:, o, at // 32, at % 32 // 2] = torch.where(at % 2 == 0, 7, 7 << 4).to(torch.uint8) | torch.where(
+            sign < 0, torch.where(at % 2 == 0, 8, 8 << 4), torch.zeros_like(at)).to(torch.uint8)
+        assert torch.equal(mx_ref.values(w["w_down"], w["s_down"])[0].to(torch.bfloat16).isinf().sum(1), torch.ones_like(o))
+    L = _layer(hip, w, k)
+    work = hip.MoeWork(L, T)
+    y = torch.empty(T, H, dtype=torch.bfloat16, device="cuda")
+    hip.moe_layer_decode(L, work, x, y)
+    assert torch.equal(y, (sign * float("inf")).expand(T, H))
+    work.destroy()
