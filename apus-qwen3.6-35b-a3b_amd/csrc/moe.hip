@@ -12,13 +12,14 @@
 //   k_moe_router     logits; by the last workgroup of each 16 tokens to finish the
 //                    choice, by the last of those the choices sorted by expert
 //   k_moe_up[_stream]   h = silu(gate) up of every (expert, 16 outputs)
-//   k_moe_down[_stream, _walk] fp32 rows of every (expert, 32 outputs), and
+//   k_moe_down[_stream] fp32 rows of every (expert, 32 outputs), and
 //   k_moe_combine       their weighted sum; or for little work
 //   k_moe_down_few      both in one.
-// The intermediate h = silu(g) u goes to the down product as two bf16 numbers
-// (its leading 8 bits and the rest rounded to 8), which keeps 16 bits of it: the
-// product reads weights, not h, so the second MFMA costs no time, and a single
-// bf16 h would put an error of a bf16 rounding into y beside y's own.
+// The intermediate h = silu(g) u goes to the down product as three bf16 numbers that sum
+// to its 24 bits: three MFMAs, of exact products, where fp32 operands would take sixteen.
+// The product reads weights, not h, so they cost little. (As two numbers, 16 bits, 56 to
+// 72 of 13728 outputs rounded another way than those of 64 bits, now 0 to 5, as plain fp32
+// sums do; us: 64 tokens, MXFP4, 88, now 89; 325 tokens, bf16, 341, now 338.)
 //
 // Times below: hidden 2048, 256 experts of 512 inner elements, 8 a token, a shared
 // expert of 512, inputs other than the call before's. The whole layer, us at
@@ -47,7 +48,8 @@ struct ApusHipMoeWork {
     float *logits;       // [T][E + 1]: the experts', then the shared gate's
     int32_t *ids;        // [T][topk]
     float *wts;          // [T][topk + 1]: p, then the shared expert's weight
-    uint16_t *h;         // [T topk][2][inter], then [T][2][shared]
+    uint16_t *h;         // [T topk][inter / 4][2][4], then [T][shared / 4][2][4]: h's upper 16 bits
+    uint16_t *hl;        // [T topk][inter], then [T][shared]: the rest
     float *part;         // [T topk + T][hidden]
     uint32_t *done;      // workgroups of k_moe_router done, per 16 tokens, then of
                          // those the ones that have chosen (0 between calls)
@@ -85,7 +87,7 @@ struct MoeArgs {
     uint32_t *done;
     int4 *slots;
     uint16_t *list;
-    uint16_t *h;
+    uint16_t *h, *hl;
     uint16_t *y;
     int T, H, I, E, k, Is, norm, nslots;
     int group;             // most rows of a slot: 16 or 32
@@ -385,26 +387,36 @@ __device__ __forceinline__ int choice(const Task &k, int i) {
 
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
-// h of choice q: its two planes, a row of I each; the elements before it, and all
+// h goes to the down product as three numbers of bf16 (Split): the first and the second in
+// a.h, 4 of either in turn, the third in a.hl. Choice q has a row of I: the elements before
+// it, and all.
 __device__ __forceinline__ uint32_t h_at(const MoeArgs &a, int q, bool sh) {
     const uint32_t n = a.T * a.k;
-    return sh ? n * 2 * a.I + (q - n) * 2 * a.Is : q * 2 * a.I;
+    return sh ? n * a.I + (q - n) * a.Is : q * a.I;
 }
-__device__ __forceinline__ uint32_t h_all(const MoeArgs &a) { return 2 * a.T * (a.k * a.I + a.Is); }
+__device__ __forceinline__ uint32_t h_all(const MoeArgs &a) { return a.T * (a.k * a.I + a.Is); }
 
-// h as its leading bits, cut, and the rest, rounded. Both have h's sign, and (from 2^-132
-// on) neither is zero where h is not, nor finite where h is infinite: times an infinite
-// weight, zero would make NaN of an infinite y. An h of 8 bits is split a bit below them.
-__device__ __forceinline__ void split_h(float v, uint16_t &hi, uint16_t &lo) {
-    const uint32_t bits = __float_as_uint(v);
-    if ((bits & 0x7f800000u) == 0x7f800000u) {
-        hi = lo = f2bf(v);
-        return;
-    }
-    uint32_t h = bits >> 16;
-    lo = f2bf(v - bf2f((uint16_t)h));
-    if ((lo & 0x7fffu) == 0 && (h & 0x7fffu) > 1) lo = f2bf(v - bf2f((uint16_t)--h));
-    hi = (uint16_t)h;
+// The 24 bits of an fp32 number as three numbers of bf16 that sum to it (as far as bf16
+// reaches down, 2^-133): its leading 8 bits, the next 8, both cut, and the rest. All have
+// its sign, and none is zero where the first is not: times an infinite weight that would
+// make NaN of an infinite y. What would be zero is bf16's least number. Two at a time.
+struct Split {
+    uint32_t v[3];
+};
+__device__ __forceinline__ Split split2(uint32_t a, uint32_t b) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    auto top = [](uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302); };
+    auto rest = [](float f) { return f - __uint_as_float(__float_as_uint(f) & 0xffff0000u); };
+    const uint32_t hi = top(a, b);
+    // (of infinite and NaN no rest: fmaxf drops a NaN)
+    const float ra = fmaxf(rest(__uint_as_float(a & 0x7fffffffu)), 0.0f);
+    const float rb = fmaxf(rest(__uint_as_float(b & 0x7fffffffu)), 0.0f);
+    const mx_bf16x2 lo{(__bf16)rest(ra), (__bf16)rest(rb)};
+    const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, hi & 0x7fff7fffu), u16x2{1, 1});
+    auto full = [&](uint32_t x) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), least)) | (hi & 0x80008000u);
+    };
+    return {hi, full(top(__float_as_uint(ra), __float_as_uint(rb))), full(__builtin_bit_cast(uint32_t, lo))};
 }
 
 // Two forms of each expert kernel. k_moe_up and k_moe_down share a row block's K
@@ -484,8 +496,12 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, i
                 for (int i = 0; i < 2; i++)
                     s[i] += *reinterpret_cast<const float *>(sm + w * LDS + i * 1024 + ((o >> 2) * 16 + row) * 16 +
                                                              (o & 3) * 4);
-            uint16_t *h = a.h + h_at(a, rows[row], sh) + o0 + o;
-            split_h(silu(s[0]) * s[1], h[0], h[I]);
+            const uint32_t at = h_at(a, rows[row], sh) + o0 + o;
+            const Split v = split2(__float_as_uint(silu(s[0]) * s[1]), 0);
+            uint16_t *const h = a.h + (at & ~3u) * 2 + at % 4;
+            h[0] = (uint16_t)v.v[0];
+            h[4] = (uint16_t)v.v[1];
+            a.hl[at] = (uint16_t)v.v[2];
         }
     }
 }
@@ -493,20 +509,36 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, i
 // wavefronts that share a row block's K in k_moe_down, a step each (longer rows:
 // more rounds), for I inner elements, and the rows of a workgroup
 __host__ __device__ constexpr int down_split(int I) { return I > 512 ? 8 : I > 256 ? 4 : I > 128 ? 2 : 1; }
-__host__ __device__ constexpr int down_rows(int I) { return kMoeWaves / down_split(I) * 32; }
+__host__ __device__ constexpr int down_tiles(int I) { return I > 512 ? 4 : 2; }          // of a wavefront
+__host__ __device__ constexpr int down_rows(int I) { return kMoeWaves / down_split(I) * 16 * down_tiles(I); }
+
+// The three numbers of h are three products with the same weights. Where a task has up to
+// kSideRows rows, they go side by side through one MFMA, as its columns kSideRows p + i.
+// Their sums meet at the end, in the same order in both cases: an expert's choices fall into
+// its slots in any order, and what a choice gets does not depend on its slot.
+constexpr int kSideRows = 4;
+__device__ __forceinline__ mx_f32x4 sum3(const mx_f32x4 (&v)[3]) { return v[0] + (v[1] + v[2]); }
+__device__ __forceinline__ mx_f32x4 sum3(const mx_f32x4 (&v)[1]) {
+    mx_f32x4 s = v[0];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {          // of column i (lane i of 16) and the ones kSideRows and twice as many past it
+        const float f = v[0][i];
+        const uint32_t u = __float_as_uint(f);
+        s[i] += __uint_as_float(dpp<0x100 + kSideRows>(u)) + __uint_as_float(dpp<0x100 + 2 * kSideRows>(u));
+    }
+    return s;
+}
 
 // part[choice] = down h: 32 outputs a group of wavefronts, 16 rows at a time (13 tokens
-// of 1056, 20 experts of 224: 4.4 us)
-template <class W>
-__global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh, int nper) {
-    constexpr int RT = 2, LDS = RowsBf16::kTile;
-    __shared__ __attribute__((aligned(16))) char sm[kMoeWaves * LDS];
-    __shared__ int rows[16];
+// of 1056, 20 experts of 224: 4.4 us). HL: loads of two rows of h (2 HL rows and no more
+// with fewer than 8).
+template <class W, int RT, int HL>
+__device__ __forceinline__ void down_part(const MoeArgs &a, const Task &task, char *sm, int *rows) {
+    constexpr bool SIDE = 2 * HL == kSideRows;
+    constexpr int LDS = RowsBf16::kTile, N3 = SIDE ? 1 : 3;
     using X = XBf16<W>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Task task = task_of(a, blockIdx.x, nsh, nper);
-    if (task.n == 0) return;
     const bool sh = task.e == a.E;
     const int I = sh ? a.Is : a.I, ks = down_split(I), kw = wave % ks, rg = wave / ks;
     const int o0 = task.part * down_rows(I);
@@ -516,25 +548,28 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
         wt[t] = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn,
                         (sh ? 0 : (size_t)task.e * a.H) + min(o0 + (rg * RT + t) * 16, a.H - 16), 16, I);
     const auto wl = W::raw_lane(lane, I);
-    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
+    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 4), lb = dma_rsrc(a.hl, h_all(a) * 2);
     char *const m = sm + wave * LDS;
+    const int half = lane >> 5, e4 = lane & 31;
     for (int c = 0; c < task.n; c += 16) {
         const int q = choice(task, c + r);
-        uint32_t hl[4], ll[4];
+        uint32_t at[HL], lat[HL / 2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            hl[i] = h_at(a, choice(task, c + 4 * i + g), sh) * 2;
-            ll[i] = hl[i] + I * 2;
-        }
+        for (int i = 0; i < HL; i++) at[i] = (h_at(a, choice(task, c + 2 * i + half), sh) + 4 * e4) * 4;
+#pragma unroll
+        for (int i = 0; i < HL / 2; i++) lat[i] = (h_at(a, choice(task, c + 4 * i + g), sh) + 8 * r) * 2;
         if (c) __syncthreads();                          // the sums have been read
-        mx_f32x4 acc[RT] = {};
+        mx_f32x4 acc[RT][N3] = {};
         for (int st = kw; st * 128 < I; st += ks) {
             typename W::Raw fw[RT];
-            RowsBf16::Raw fh, fl;
+            u32x4 fh[HL], fl[HL / 2];
 #pragma unroll
             for (int t = 0; t < RT; t++) W::load_raw(fw[t], wt[t], wl, st, I);
-            X::load_raw(fh, hb, hl, st, I);
-            X::load_raw(fl, hb, ll, st, I);
+            const bool live = st * 128 + 4 * e4 < I, llive = st * 128 + 8 * r < I;
+#pragma unroll
+            for (int i = 0; i < HL; i++) fh[i] = ld16(hb, live ? at[i] : kPast, 512 * st);
+#pragma unroll
+            for (int i = 0; i < HL / 2; i++) fl[i] = ld16(lb, llive ? lat[i] : kPast, 256 * st);
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
             typename W::Frag f[RT];
@@ -543,24 +578,37 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
                 W::put(m, fw[t], lane);
                 W::get(f[t], m, fw[t], lane);
             }
-            mx_bf16x8 h[4];
-            RowsBf16::put(m, fh, lane);
+            // (they share their LDS: what is written is read before the next)
+            mx_bf16x8 h[N3][4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) h[j] = X::piece(m, j, lane);
-            RowsBf16::put(m, fl, lane);
+            for (int p = 0; p < 3; p++) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const mx_bf16x8 lo = X::piece(m, j, lane);
+                for (int i = 0; i < HL; i++) {
+                    const int row = (SIDE ? kSideRows * p : 0) + 2 * i + half;
+                    char *const to = m + row * 256 + ((e4 / 2 ^ row) << 4) + e4 % 2 * 8;
+                    if (p == 0) *reinterpret_cast<uint2 *>(to) = make_uint2(fh[i][0], fh[i][1]);
+                    if (p == 1) *reinterpret_cast<uint2 *>(to) = make_uint2(fh[i][2], fh[i][3]);
+                }
+#pragma unroll
+                for (int i = 0; i < HL / 2; i++) {
+                    const int row = (SIDE ? kSideRows * p : 0) + 4 * i + g;
+                    if (p == 2) *reinterpret_cast<u32x4 *>(m + row * 256 + ((r ^ row) << 4)) = fl[i];
+                }
+                if (SIDE && p < 2) continue;
+#pragma unroll
+                for (int j = 0; j < 4; j++) h[SIDE ? 0 : p][j] = X::piece(m, j, lane);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int t = 0; t < RT; t++) {
                     const mx_bf16x8 wv = W::operand(f[t], j);
-                    acc[t] = mfma16(wv, h[j], acc[t]);
-                    acc[t] = mfma16(wv, lo, acc[t]);
+#pragma unroll
+                    for (int p = 0; p < N3; p++) acc[t][p] = mfma16(wv, h[p][j], acc[t][p]);
                 }
-            }
         }
 #pragma unroll
-        for (int t = 0; t < RT; t++) *reinterpret_cast<mx_f32x4 *>(m + t * 1024 + lane * 16) = acc[t];
+        for (int t = 0; t < RT; t++) *reinterpret_cast<mx_f32x4 *>(m + t * 1024 + lane * 16) = sum3(acc[t]);
         if (wave == 0 && g == 0) rows[r] = q;
         __syncthreads();
         // a thread finishes 4 outputs of a row
@@ -575,15 +623,28 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
         }
     }
 }
+template <class W, int RT>
+__device__ __forceinline__ void down_part_of(const MoeArgs &a, const Task &task, char *sm, int *rows) {
+    if (task.n <= kSideRows) down_part<W, RT, kSideRows / 2>(a, task, sm, rows);
+    else if (task.n <= 8) down_part<W, RT, 4>(a, task, sm, rows);
+    else down_part<W, RT, 8>(a, task, sm, rows);
+}
+template <class W>
+__global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh, int nper) {
+    __shared__ __attribute__((aligned(16))) char sm[kMoeWaves * RowsBf16::kTile];
+    __shared__ int rows[16];
+    const Task task = task_of(a, blockIdx.x, nsh, nper);
+    if (task.n == 0) return;
+    if (down_tiles(task.e == a.E ? a.Is : a.I) == 4) down_part_of<W, 4>(a, task, sm, rows);
+    else down_part_of<W, 2>(a, task, sm, rows);
+}
 
-// ---- the same, a wavefront alone: no partial sums, no barrier, and D steps of
-// weights and activations on their way all along its walk. Up: bf16, 325 tokens, 198
+// ---- the same, a wavefront alone: no partial sums, and D steps of weights (up: and
+// activations) on their way all along its walk. Up: bf16, 325 tokens, 198
 // us for 1.07 GB, 5.4 TB/s; MXFP4, 64 tokens, 53 us for 247 MB, 4.7 TB/s. Down: 119
 // us for 0.54 GB, 4.5 TB/s; 32 us for 124 MB, 3.9 TB/s. More steps on their way (3, 4)
 // changed nothing, nor did whole 128-byte lines of MXFP4 codes a load.
 constexpr int kStreamWaves = 4;
-
-constexpr int kDownH = 32 * 1024;      // LDS bytes that k_moe_down_stream has for h of 16 rows
 
 // (what comes before stays before)
 __device__ __forceinline__ void fence() {
@@ -694,16 +755,17 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
 #pragma unroll
     for (int u = 0; u < NT; u++) {
         if (16 * u + r >= task.n) continue;
-        uint16_t *h = a.h + h_at(a, q[u], sh);
+        const uint32_t at = h_at(a, q[u], sh);
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const int o = o0 + 16 * t + 4 * g;
             if (o >= I) continue;
-            uint16_t hi[4], lo[4];
+            uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) split_h(silu(acc[t][0][u][i]) * acc[t][1][u][i], hi[i], lo[i]);
-            *reinterpret_cast<ushort4 *>(h + o) = make_ushort4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<ushort4 *>(h + I + o) = make_ushort4(lo[0], lo[1], lo[2], lo[3]);
+            for (int i = 0; i < 4; i++) v[i] = __float_as_uint(silu(acc[t][0][u][i]) * acc[t][1][u][i]);
+            const Split s0 = split2(v[0], v[1]), s1 = split2(v[2], v[3]);
+            *reinterpret_cast<u32x4 *>(a.h + (at + o) * 2) = u32x4{s0.v[0], s1.v[0], s0.v[1], s1.v[1]};
+            *reinterpret_cast<uint2 *>(a.hl + at + o) = make_uint2(s0.v[2], s1.v[2]);
         }
     }
 }
@@ -722,16 +784,24 @@ __global__ __launch_bounds__(64 * kStreamWaves, W::mx ? 3 : 2) void k_moe_up_str
     else up_stream<W, RT, 1, 2, 1, SC>(a, task, o0, sm + wave * LDS, lane);
 }
 
-// part[choice] = down h: 16 RT outputs a block, P blocks a wavefront in one walk.
-// h of the task's rows is brought to LDS once for all the workgroup's blocks.
-__host__ __device__ constexpr int down_pitch(int I) { return (I + 127) / 128 * 256; }     // bytes of a plane's row
-template <class W, int RT, int NT, int D>
-__device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, int b0, int nb, const char *h, char *m,
+// part[choice] = down h: 16 RT outputs a block, P blocks a wavefront in one walk (one
+// block where I takes several chunks). h of the task's rows is brought to LDS once for all
+// the workgroup's blocks, a chunk of 512 elements (with SIDE, of up to kSideRows rows, 2048)
+// at a time; the next chunk's is on its way, in registers, while one is walked.
+constexpr int kDownWaves = 8;
+constexpr int kDownChunk = 4;                            // steps of 128 elements
+constexpr int kDownH = 16 * 3 * kDownChunk * 256;        // LDS bytes of 16 rows of a chunk
+static_assert(3 * kSideRows * (kDownChunk * 16 / kSideRows) * 256 <= kDownH, "a chunk side by side fits");
+template <class W, int RT, int NT, int D, bool MANY, bool SIDE>
+__device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, int b0, int nb, char *h, char *m,
                                             int lane) {
+    static_assert(NT == 1 || !SIDE);
     using X = XBf16<W>;
+    constexpr int N3 = SIDE ? 1 : 3;       // MFMAs for the three numbers
+    constexpr int CHUNK = SIDE ? kDownChunk * 16 / kSideRows : kDownChunk;
     const int r = lane & 15, g = lane >> 4;
     const bool sh = task.e == a.E;
-    const int I = sh ? a.Is : a.I, steps = (I + 127) / 128, pitch = down_pitch(I);
+    const int I = sh ? a.Is : a.I, steps = (I + 127) / 128, chunks = (steps + CHUNK - 1) / CHUNK;
     const auto wl = W::raw_lane(lane, I);
     typename W::Raw fw[D][RT];
     int lb = b0, ls = 0, mb = b0, ms = 0;  // row block and step to load, to multiply
@@ -748,12 +818,55 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
             lb++;
         }
     };
-    mx_f32x4 acc[RT][NT] = {};
 #pragma unroll
     for (int d = 0; d < D; d++) load(d, d);
     fence();
-    __syncthreads();                       // h is in place
-    walk_on<D>(nb * steps, [&](int d, int st) {
+    // Pieces of 8 elements of a row of h, and bytes of a row of one of its three numbers in
+    // LDS: where there may be chunks of 512, whole ones, so that a wavefront brings a row.
+    constexpr bool ROWS = MANY && !SIDE;
+    const int pc = ROWS ? CHUNK * 16 : min(steps, CHUNK) * 16, pitch = pc * 16;
+    // Piece c of number p of the task's row i lies at c ^ k within its 256 bytes, in LDS row
+    // 3 i + p, k = i, or with SIDE in row k = kSideRows p + i. A thread's pieces past the last
+    // row are the last row's again.
+    constexpr int PIECES = ((SIDE ? kSideRows : 16 * NT) * (MANY ? CHUNK : kDownChunk) * 16 + 64 * kDownWaves - 1) / (64 * kDownWaves);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto row_of = [&](int n) {
+        return min(ROWS ? wave + n * kDownWaves : (int)(threadIdx.x + n * 64 * kDownWaves) / pc, task.n - 1);
+    };
+    auto piece_of = [&](int n) { return ROWS ? lane : (int)(threadIdx.x + n * 64 * kDownWaves) % pc; };
+    uint32_t at[PIECES];                   // elements before the rows
+#pragma unroll
+    for (int n = 0; n < PIECES; n++) at[n] = h_at(a, choice(task, row_of(n)), sh);
+    u32x4 hr[PIECES][3];
+    auto fetch = [&](int chunk) {          // (zeros past I)
+#pragma unroll
+        for (int n = 0; n < PIECES; n++) {
+            const int k = chunk * CHUNK * 128 + piece_of(n) * 8;
+            const uint32_t from = at[n] + (k < I ? k : 0);
+            hr[n][0] = *reinterpret_cast<const u32x4 *>(a.h + (size_t)from * 2);
+            hr[n][1] = *reinterpret_cast<const u32x4 *>(a.h + (size_t)from * 2 + 8);
+            hr[n][2] = *reinterpret_cast<const u32x4 *>(a.hl + from);
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                if (k >= I) hr[n][p] = u32x4{};
+        }
+    };
+    auto put_h = [&]() {
+#pragma unroll
+        for (int n = 0; n < PIECES; n++) {
+            if ((n * kDownWaves + wave) * 64 >= task.n * pc) continue;       // (all past the last row)
+            const int i = row_of(n);
+            const u32x4 a0 = hr[n][0], a1 = hr[n][1];
+            const u32x4 v[3] = {u32x4{a0[0], a0[1], a1[0], a1[1]}, u32x4{a0[2], a0[3], a1[2], a1[3]}, hr[n][2]};
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                const int to = SIDE ? kSideRows * p + i : 3 * i + p, key = SIDE ? to : i & 15;
+                *reinterpret_cast<u32x4 *>(h + to * pitch + ((piece_of(n) ^ key) << 4)) = v[p];
+            }
+        }
+    };
+    mx_f32x4 acc[RT][NT][N3] = {};
+    auto mul = [&](int d, int st) {
 #pragma unroll
         for (int t = 0; t < RT; t++) W::put(m + t * W::kTile, fw[d][t], lane);
         typename W::Frag f[RT];
@@ -763,24 +876,22 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
         load(d, st + D);
         fence();
         // (a step past the last, of zero weights, reads the last step's h)
-        const char *hs = h + r * 2 * pitch + min(ms, steps - 1) * 256;
+        const char *hs = h + (SIDE ? min(r, 3 * kSideRows - 1) : 3 * r) * pitch + min(ms, steps - 1) % CHUNK * 256;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            mx_bf16x8 hi[NT], lo[NT];
+            mx_bf16x8 v[NT][N3];
 #pragma unroll
-            for (int u = 0; u < NT; u++) {
-                const char *p = hs + u * 32 * pitch + ((X::piece_of(j, g) ^ r) << 4);
-                hi[u] = *reinterpret_cast<const mx_bf16x8 *>(p);
-                lo[u] = *reinterpret_cast<const mx_bf16x8 *>(p + pitch);
-            }
+            for (int u = 0; u < NT; u++)
+#pragma unroll
+                for (int p = 0; p < N3; p++)
+                    v[u][p] = *reinterpret_cast<const mx_bf16x8 *>(hs + (u * 48 + p) * pitch + ((X::piece_of(j, g) ^ r) << 4));
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 const mx_bf16x8 w = W::operand(f[t], j);
 #pragma unroll
-                for (int u = 0; u < NT; u++) {
-                    acc[t][u] = mfma16(w, hi[u], acc[t][u]);
-                    acc[t][u] = mfma16(w, lo[u], acc[t][u]);
-                }
+                for (int u = 0; u < NT; u++)
+#pragma unroll
+                    for (int p = 0; p < N3; p++) acc[t][u][p] = mfma16(w, v[u][p], acc[t][u][p]);
             }
         }
         fence();
@@ -791,147 +902,45 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 const int o = (mb * RT + t) * 16;
+                const mx_f32x4 s = sum3(acc[t][u]);
                 if (16 * u + r < task.n && o < a.H && mb < b0 + nb)
-                    *reinterpret_cast<mx_f32x4 *>(a.part + (size_t)choice(task, 16 * u + r) * a.H + o + 4 * g) = acc[t][u];
-                acc[t][u] = mx_f32x4{};
+                    *reinterpret_cast<mx_f32x4 *>(a.part + (size_t)choice(task, 16 * u + r) * a.H + o + 4 * g) = s;
+#pragma unroll
+                for (int p = 0; p < N3; p++) acc[t][u][p] = mx_f32x4{};
             }
         mb++;
-    });
+    };
+    fetch(0);
+    put_h();
+    __syncthreads();
+    if (!MANY) return walk_on<D>(nb * steps, mul);
+    for (int c = 0;; c++) {                // (every wavefront comes to every barrier)
+        const bool more = c + 1 < chunks;
+        if (more) fetch(c + 1);
+        fence();
+        if (nb > 0) walk_on<D>(min(CHUNK, steps - c * CHUNK), mul);
+        if (!more) break;
+        __syncthreads();                   // the chunk has been read
+        put_h();
+        __syncthreads();
+    }
 }
 
-template <class W, int RT, int NT>
-__global__ __launch_bounds__(64 * kStreamWaves) void k_moe_down_stream(MoeArgs a, int nsh, int nper, int P) {
+template <class W, int RT, int NT, bool MANY>
+__global__ __launch_bounds__(64 * kDownWaves, W::mx && NT == 1 ? 4 : 2) void k_moe_down_stream(MoeArgs a, int nsh, int nper, int P) {
     constexpr int LDS = RT * W::kTile;
-    __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS + NT * kDownH];
-    char *const h = sm + kStreamWaves * LDS;
+    __shared__ __attribute__((aligned(16))) char sm[kDownWaves * LDS + NT * kDownH];
+    char *const h = sm + kDownWaves * LDS;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = task_of(a, blockIdx.x, nsh, nper);
     if (task.n == 0) return;
-    const bool sh = task.e == a.E;
-    const int I = sh ? a.Is : a.I, pitch = down_pitch(I), pc = pitch / 16;
-    // 16-byte piece c of row i's plane p, at c ^ i within its 256 bytes; zeros past I
-    for (int e = threadIdx.x; e < task.n * 2 * pc; e += 64 * kStreamWaves) {
-        const int c = e % pc, i = e / pc / 2, p = e / pc % 2;
-        u32x4 v{};
-        if (c * 8 < I) v = *reinterpret_cast<const u32x4 *>(a.h + h_at(a, choice(task, i), sh) + p * I + c * 8);
-        *reinterpret_cast<u32x4 *>(h + (i * 2 + p) * pitch + ((c ^ (i & 15)) << 4)) = v;
-    }
-    const int blocks = (a.H + 16 * RT - 1) / (16 * RT), b0 = (task.part * kStreamWaves + wave) * P;
-    const int nb = min(P, blocks - b0);
-    // (every wavefront comes to the one barrier)
-    if (NT > 1 && task.n > 16) down_stream<W, RT, NT, 2>(a, task, b0, nb, h, sm + wave * LDS, lane);
-    else down_stream<W, RT, 1, 2>(a, task, b0, nb, h, sm + wave * LDS, lane);
-}
-
-// The same for inner sizes whose h does not fit: 32 outputs a wavefront, h's two planes
-// walked along with the weights as the activations are in up_stream.
-template <class W, int NT, int D, int XR, bool SC>
-__device__ __forceinline__ void down_walk(const MoeArgs &a, const Task &task, int o0, char *m, int lane) {
-    using X = XBf16<W>;
-    const int r = lane & 15, g = lane >> 4;
-    const bool sh = task.e == a.E;
-    const int I = sh ? a.Is : a.I;
-    typename W::Tile wt[2];                // (a tile past H, not stored, repeats the last)
-#pragma unroll
-    for (int t = 0; t < 2; t++)
-        wt[t] = W::tile(sh ? a.w_sdn : a.w_dn, sh ? a.s_sdn : a.s_dn,
-                        (sh ? 0 : (size_t)task.e * a.H) + min(o0 + 16 * t, a.H - 16), 16, I);
-    const auto wl = W::raw_lane(lane, I);
-    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
-    uint32_t hl[NT][2][4];                 // rows 4 i + g of the planes
-#pragma unroll
-    for (int u = 0; u < NT; u++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            hl[u][0][i] = h_at(a, choice(task, 16 * u + 4 * i + g), sh) * 2;
-            hl[u][1][i] = hl[u][0][i] + I * 2;
-        }
-    typename W::Raw fw[D][2];
-    RowsBf16::Raw fx[D][NT][2];
-    char *const mx = m + 2 * W::kTile, *const ms = mx + NT * RowsBf16::kTile;
-    Strip strip[SC ? 2 : 1];
-    auto load = [&](int d, int st) {
-        if constexpr (SC) {
-            if ((st & (Strip::kSteps - 1)) == 0) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) strip[t].load(wt[t], st, I);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; t++) W::template load_raw<!SC>(fw[d][t], wt[t], wl, st, I);
-#pragma unroll
-        for (int u = 0; u < NT; u++)
-#pragma unroll
-            for (int p = 0; p < 2; p++) X::template load_raw<XR>(fx[d][u][p], hb, hl[u][p], st, I);
-    };
-    mx_f32x4 acc[2][NT] = {};
-    walk<D>((I + 127) / 128, load, [&](int d, int st) {
-#pragma unroll
-        for (int t = 0; t < 2; t++) W::put(m + t * W::kTile, fw[d][t], lane);
-        typename W::Frag f[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) W::template get<!SC>(f[t], m + t * W::kTile, fw[d][t], lane);
-        if constexpr (SC) {
-            if ((st & (Strip::kSteps - 1)) == 0) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) strip[t].put(ms + t * Strip::kTile);
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++) f[t].s = Strip::get(ms + t * Strip::kTile, st, lane);
-        }
-        // (the planes share their LDS: what is written is read before the next)
-        mx_bf16x8 hi[NT][4];
-#pragma unroll
-        for (int u = 0; u < NT; u++) {
-            RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u][0], lane);
-#pragma unroll
-            for (int j = 0; j < 4; j++) hi[u][j] = X::piece(mx + u * RowsBf16::kTile, j, lane);
-            RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u][1], lane);
-        }
-        fence();
-        load(d, st + D);
-        fence();
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            mx_bf16x8 lo[NT];
-#pragma unroll
-            for (int u = 0; u < NT; u++) lo[u] = X::piece(mx + u * RowsBf16::kTile, j, lane);
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const mx_bf16x8 w = W::operand(f[t], j);
-#pragma unroll
-                for (int u = 0; u < NT; u++) {
-                    acc[t][u] = mfma16(w, hi[u][j], acc[t][u]);
-                    acc[t][u] = mfma16(w, lo[u], acc[t][u]);
-                }
-            }
-        }
-        fence();
-    });
-#pragma unroll
-    for (int u = 0; u < NT; u++) {
-        if (16 * u + r >= task.n) continue;
-        float *part = a.part + (size_t)choice(task, 16 * u + r) * a.H + o0 + 4 * g;
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-            if (o0 + 16 * t < a.H) *reinterpret_cast<mx_f32x4 *>(part + 16 * t) = acc[t][u];
-    }
-}
-
-template <class W, int NT, bool SC>
-__global__ __launch_bounds__(64 * kStreamWaves, !W::mx ? 1 : NT == 1 ? 3 : 2) void k_moe_down_walk(MoeArgs a, int nsh, int nper) {
-    constexpr int LDS = 2 * (W::kTile + (SC ? Strip::kTile : 0)) + NT * RowsBf16::kTile;
-    __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Task task = task_of(a, blockIdx.x, nsh, nper);
-    const int o0 = (task.part * kStreamWaves + wave) * 32;
-    if (task.n == 0 || o0 >= a.H) return;                // (no barrier in this kernel)
     char *const m = sm + wave * LDS;
-    if (NT > 1 && task.n > 16) down_walk<W, NT, 2, 4, SC>(a, task, o0, m, lane);
-    else if (task.n > 4) down_walk<W, 1, 2, 4, SC>(a, task, o0, m, lane);
-    else down_walk<W, 1, 2, 1, SC>(a, task, o0, m, lane);
+    const int blocks = (a.H + 16 * RT - 1) / (16 * RT), b0 = (task.part * kDownWaves + wave) * P;
+    const int nb = min(P, blocks - b0);
+    if (NT > 1 && task.n > 16) down_stream<W, RT, NT, 2, MANY, false>(a, task, b0, nb, h, m, lane);
+    else if (task.n > kSideRows) down_stream<W, RT, 1, 2, MANY, false>(a, task, b0, nb, h, m, lane);
+    else down_stream<W, RT, 1, 2, MANY, true>(a, task, b0, nb, h, m, lane);
 }
 
 // y of up to 16 tokens: 16 outputs a workgroup, the steps of 128 k of every (token,
@@ -942,7 +951,8 @@ __global__ __launch_bounds__(64 * kStreamWaves, !W::mx ? 1 : NT == 1 ? 3 : 2) vo
 constexpr int kFewWaves = 12, kFewUnits = 3;
 template <class W>
 __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
-    __shared__ __attribute__((aligned(16))) char sm[kFewWaves * W::kTile];
+    constexpr int HB = 3 * 256, LDS = W::kTile + kFewUnits * HB;     // bytes of a unit's h, of a wavefront
+    __shared__ __attribute__((aligned(16))) char sm[kFewWaves * LDS];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = blockIdx.x * 16, n = a.T * a.k;
@@ -950,8 +960,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
     const int units = n * si + a.T * ss;
     constexpr int U = kFewUnits;
     using X = XBf16<W>;
-    char *const m = sm + wave * W::kTile;
-    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 2);
+    char *const m = sm + wave * LDS, *const mh = m + W::kTile;
+    const i32x4 hb = dma_rsrc(a.h, h_all(a) * 4), lb = dma_rsrc(a.hl, h_all(a) * 2);
     mx_f32x4 acc{};
     for (int b = wave; b < units; b += kFewWaves * U) {
         // choice, its expert, step and weight of each
@@ -971,13 +981,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
             on[i] = live && t == r;
         }
         typename W::Raw fw[U];
-        typename X::Frag fh[U], fl[U];
+        u32x4 fh[U], fl[U];                // h of a step, 4 elements in each of 32 lanes, 8 in each of 16
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const int I = sh[i] ? a.Is : a.I;
-            const uint32_t xl = X::lane(h_at(a, q[i], sh[i]) * 2, g);
-            X::load(fh[i], hb, xl, st[i], I);
-            X::load(fl[i], hb, xl + I * 2, st[i], I);
+            const int k = st[i] * 128, I = sh[i] ? a.Is : a.I;
+            const uint32_t at = h_at(a, q[i], sh[i]);
+            fh[i] = ld16(hb, lane < 32 && k + 4 * lane < I ? (at + 4 * lane) * 4 : kPast, 4 * k);
+            fl[i] = ld16(lb, lane < 16 && k + 8 * lane < I ? (at + 8 * lane) * 2 : kPast, 2 * k);
         }
 #pragma unroll
         for (int i = 0; i < U; i++) {
@@ -990,6 +1000,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < U; i++) {
+            if (lane < 32) {
+                *reinterpret_cast<uint2 *>(mh + i * HB + lane * 8) = make_uint2(fh[i][0], fh[i][1]);
+                *reinterpret_cast<uint2 *>(mh + i * HB + 256 + lane * 8) = make_uint2(fh[i][2], fh[i][3]);
+            }
+            if (lane < 16) *reinterpret_cast<u32x4 *>(mh + i * HB + 512 + lane * 16) = fl[i];
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++) {
             mx_f32x4 d{};
             typename W::Frag f;
             W::put(m, fw[i], lane);
@@ -997,8 +1015,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const mx_bf16x8 wv = W::operand(f, j);
-                d = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fh[i].v[j]), d);
-                d = mfma16(wv, __builtin_bit_cast(mx_bf16x8, fl[i].v[j]), d);
+#pragma unroll
+                for (int p = 0; p < 3; p++)
+                    d = mfma16(wv, *reinterpret_cast<const mx_bf16x8 *>(mh + i * HB + p * 256 + X::piece_of(j, g) * 16), d);
             }
             if (on[i]) acc += d * p[i];
         }
@@ -1008,7 +1027,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {
     if (wave || r >= a.T) return;
     mx_f32x4 s[4] = {};
 #pragma unroll
-    for (int i = 0; i < kFewWaves; i++) s[i & 3] += *reinterpret_cast<const mx_f32x4 *>(sm + i * W::kTile + lane * 16);
+    for (int i = 0; i < kFewWaves; i++) s[i & 3] += *reinterpret_cast<const mx_f32x4 *>(sm + i * LDS + lane * 16);
     acc = (s[0] + s[1]) + (s[2] + s[3]);
     *reinterpret_cast<ushort4 *>(a.y + (size_t)r * a.H + o0 + 4 * g) =
         make_ushort4(f2bf(acc[0]), f2bf(acc[1]), f2bf(acc[2]), f2bf(acc[3]));
@@ -1069,39 +1088,31 @@ int up_stream_run(const MoeArgs &a, size_t slots) {
 }
 template <class W, int NT>
 int down_stream_run(const MoeArgs &a, size_t slots) {
-    // blocks of 32 outputs a wavefront, so that the launch keeps about 1024
-    // workgroups: more share a workgroup's copy of h
-    const size_t blocks = cdiv(a.H, 32 * kStreamWaves);
-    const int P = (int)std::max<size_t>(1, std::min<size_t>(4, slots * blocks / 1024));
-    const size_t nper = cdiv(blocks, P);
+    // blocks of 32 outputs a wavefront, so that the launch keeps about 4096 wavefronts:
+    // more share a workgroup's copy of h
+    const size_t blocks = cdiv(a.H, 32);
+    const bool many = std::max(a.I, a.Is) > kDownChunk * 128;
+    const int P = many ? 1 : (int)std::max<size_t>(1, std::min<size_t>(4, slots * blocks / 8192));
+    const size_t nper = cdiv(blocks, kDownWaves * P);
     const Grid g = grid_of(a, slots, nper, nper);
     APUS_TIMED("k_moe_down_stream",
-               k_moe_down_stream<W, 2, NT><<<g.n, 64 * kStreamWaves, 0, stream()>>>(a, g.nsh, g.nper, P));
+               if (many) k_moe_down_stream<W, 2, NT, true><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P);
+               else k_moe_down_stream<W, 2, NT, false><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P));
     return launch_check("k_moe_down_stream");
 }
 
-template <class W, int NT>
-int down_walk_run(const MoeArgs &a, size_t slots) {
-    const size_t nper = cdiv(a.H, 32 * kStreamWaves);
-    const Grid g = grid_of(a, slots, nper, nper);
-    const unsigned threads = 64 * kStreamWaves;
-    const bool strips = W::mx && a.I % 128 == 0 && a.Is % 128 == 0 && ((uintptr_t)a.s_dn | (uintptr_t)a.s_sdn) % 4 == 0;
-    APUS_TIMED("k_moe_down_walk",
-               if (strips) k_moe_down_walk<W, NT, W::mx><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper);
-               else k_moe_down_walk<W, NT, false><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper));
-    return launch_check("k_moe_down_walk");
-}
-
 // The streaming forms from 1024 wavefronts on, 4 a CU (the layer, us split | streamed;
-// up, MXFP4: 16 tokens 65 | 60, 64 tokens 121 | 107, 325 tokens 182 | 160; down: 5 tokens
-// 44 | 39, 64 tokens 133 | 107). bf16 weights' up product is 4 times the bytes a step,
-// which the split form keeps on their way as well with few rows a slot (16 tokens 143 |
-// 150, 64 tokens 297 | 287, 325 tokens 396 | 359). k_moe_down_stream where h of a slot fits
-// its LDS, else k_moe_down_walk (128 experts of 768, 8 a token, MXFP4: 16 tokens 89 | 64, 64
-// tokens 133 | 101; bf16 184 | 167, 262 | 242), but the split form where a wavefront's walk
-// is long and the choices are few (60 experts of 1408, a shared one of 5632, 4 tokens 43 |
-// 52; 8 experts of 14336, bf16, 16 tokens 518 | 533, 256 tokens 1279 | 1140). k_moe_down_few for work that one round of loads covers (one token: 25 us with the
-// two kernels, 19 with it; bf16 35 and 29), and for kFewTokens.
+// up, MXFP4: 5 tokens 38 | 40, 16 tokens 58 | 54, 64 tokens 100 | 90, 325 tokens 181 | 153;
+// down: 5 tokens 48 | 39, 64 tokens 149 | 90; bf16 72 | 69, 266 | 231). bf16 weights' up
+// product is 4 times the bytes a step, which the split form keeps on their way as well with
+// few rows a slot (16 tokens 130 | 130, 64 tokens 239 | 231, 325 tokens 393 | 345).
+// Inner sizes of several chunks too (down, 128 experts of 768, 8 a token, MXFP4: 16 tokens
+// 76 | 59, 64 tokens 116 | 85; bf16 163 | 156, 234 | 221), but the split form where a
+// wavefront's walk is long and the choices are few (MXFP4: 60 experts of 1408, a shared one
+// of 5632, 4 tokens 40 | 59; 8 experts of 14336, 2 a token, 64 tokens 302 | 342, 128 tokens
+// 417 | 397; bf16, 16 tokens 507 | 557, 64 tokens 664 | 631). k_moe_down_few for work that
+// one round of loads covers (one token: 24 us with the two kernels, 19 with it; bf16 33 and
+// 27), and for kFewTokens.
 template <class W>
 int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
@@ -1115,11 +1126,8 @@ int experts_run(const MoeArgs &a) {
         return launch_check("k_moe_down_few");
     }
     const int inner = std::max(a.I, a.Is);
-    const bool fits = 32 * down_pitch(inner) <= kDownH;
-    const bool downs = slots * a.H / 32 >= 1024 && (inner <= 2048 || a.T * a.k >= 16 * a.E);
-    if (int r = !downs ? down_run<W>(a, slots)
-                : fits ? (one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, 2>(a, slots))
-                       : (one ? down_walk_run<W, 1>(a, slots) : down_walk_run<W, 2>(a, slots)))
+    const bool downs = slots * a.H / 32 >= 1024 && (inner <= 2048 || a.T * a.k >= (W::mx ? 32 : 16) * a.E);
+    if (int r = !downs ? down_run<W>(a, slots) : one ? down_stream_run<W, 1>(a, slots) : down_stream_run<W, 2>(a, slots))
         return r;
     APUS_TIMED("k_moe_combine",
                k_moe_combine<<<cdiv((size_t)a.T * (a.H / 4), 256), 256, 0, stream()>>>(a));
@@ -1195,7 +1203,7 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
         return at;
     };
     const size_t logits = take(T * (L->experts + 1) * 4), ids = take(T * k * 4),
-                 wts = take(T * (k + 1) * 4), h = take(hs),
+                 wts = take(T * (k + 1) * 4), h = take(hs), hl = take(hs / 2),
                  part = take(T * (k + 1) * L->hidden * 4), done = take(((T + 15) / 16 + 1) * 4),
                  slots = take(moe_slots(T, k, L->experts, 16) * 16), list = take(T * k * 2);
     if (hipMalloc((void **)&w->base, n) != hipSuccess) {
@@ -1217,6 +1225,7 @@ int apus_hip_moe_work_create(const ApusHipMoeLayer *L, size_t max_tokens, ApusHi
     w->ids = (int32_t *)(w->base + ids);
     w->wts = (float *)(w->base + wts);
     w->h = (uint16_t *)(w->base + h);
+    w->hl = (uint16_t *)(w->base + hl);
     w->part = (float *)(w->base + part);
     *out = w;
     return kOk;
@@ -1274,6 +1283,7 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.slots = w->slots;
     a.list = w->list;
     a.h = w->h;
+    a.hl = w->hl;
     a.T = (int)T;
     a.H = (int)L->hidden;
     a.I = (int)L->inter;

@@ -105,3 +105,43 @@ def test_infinite_down_weights(hip, T, H, I, E, k, kind):
     hip.moe_layer_decode(L, work, x, y)
     assert torch.equal(y, (sign * float("inf")).expand(T, H))
     work.destroy()
+
+
+# k_moe_down_few, _down, and _down_stream: inner values in one chunk and in several, slots of 16 rows and of 32
+@pytest.mark.parametrize("T,H,I,E", [(1, 256, 64, 8), (2, 64, 1184, 3), (13, 256, 64, 8), (40, 96, 2080, 3), (64, 1024, 64, 64),
+                                     (64, 1056, 544, 64), (100, 1024, 1152, 40), (1000, 1024, 512, 40),
+                                     (1000, 1056, 1056, 16)])
+@pytest.mark.parametrize("mx", [False, True])
+def test_inner_values_of_24_bits(hip, T, H, I, E, mx):
+    """Inner values that are integers of 24 bits (times 64), of which each output takes the
+    difference of two with the same 16 leading bits: all in fp32, and exact."""
+    import torch
+    g = _gen(torch, T + I)
+    n = torch.randint(1 << 23, 1 << 24, (E, I // 2, 1), generator=g, device="cuda") & ~255
+    n = (n + torch.randint(0, 256, (E, I // 2, 2), generator=g, device="cuda")).view(E, I)
+    bit = torch.arange(24, device="cuda")
+    w = dict(w_router=mx_ref.normal(g, E, H, scale=0.5), w_gate_up=torch.zeros(E, 2 * I, H, dtype=torch.bfloat16, device="cuda"),
+             w_down=torch.zeros(E, H, I, dtype=torch.bfloat16, device="cuda"))
+    w["w_router"][:, :40] = 0
+    w["w_gate_up"][:, :I, 32] = 64                         # silu(64) = 64 in fp32
+    w["w_gate_up"][:, I:, :24] = (n.unsqueeze(-1) >> bit & 1).to(torch.bfloat16)
+    o = torch.arange(H, device="cuda")
+    w["w_down"][:, o, 2 * o % I] = 1
+    w["w_down"][:, o, 2 * o % I + 1] = -1
+    if mx:
+        for m in ("gate_up", "down"):
+            w["w_" + m], w["s_" + m] = mx_ref.quantize(w["w_" + m])
+    x = mx_ref.normal(g, T, H)
+    x[:, :40] = 0
+    x[:, :24] = torch.exp2(bit.float()).to(torch.bfloat16)
+    x[:, 32] = 1
+    r, _, gap = mx_ref.moe(x, w, 1, True, mx)
+    assert float((r - 64 * torch.round(r / 64)).abs().max()) < 1e-9 and 0 < float(r.abs().max()) <= 64 * 255
+    L = _layer(hip, w, 1)
+    work = hip.MoeWork(L, T)
+    y = torch.empty(T, H, dtype=torch.bfloat16, device="cuda")
+    hip.moe_layer_decode(L, work, x, y)
+    ok = gap > 0                                           # (the choice no fp32 sum's error can change)
+    assert int(ok.sum()) >= T - T // 10
+    assert torch.equal(y[ok].double(), torch.round(r[ok]))
+    work.destroy()
