@@ -60,20 +60,23 @@ struct ApusHipMoeWork {
 namespace {
 
 constexpr size_t kMoeMaxTokens = 1024, kMoeMaxExperts = 1024, kMoeMaxTopk = 32;
-// Most rows of a slot. 32 from 14 choices an expert on, where that leaves 2048 blocks of
-// 16 inner elements; else 16: the kernels for 16 have fewer registers and less LDS and
-// more wavefronts, but read the weights of an expert with more rows again (us with 16 |
-// 32: bf16, 325 tokens 352 | 359, 768 tokens 480 | 444; MXFP4, 96 tokens 116 | 124; 128
-// experts of 768, 8 a token, MXFP4, 256 tokens 186 | 178, 1024 tokens 474 | 420; 20 experts
-// of 224, 3 a token, 512 tokens 36 | 44, bf16 47 | 60).
-int slot_rows(size_t n, size_t E, size_t I) {
-    return n <= 14 * E || (E + n / 32) * (I / 16) < 2048 ? 16 : 32;
+// Most rows of a slot. 32 from 8 choices an expert on, MXFP4 weights from 30, where that
+// leaves 2048 blocks of 16 inner elements; else 16: the kernels for 16 have fewer registers
+// and less LDS and more wavefronts, but read the weights of an expert with more rows again
+// (us with 16 | 32: bf16, 192 tokens 300 | 302, 256 tokens 321 | 320, 768 tokens 471 | 428;
+// 128 experts of 768, 8 a token, 128 tokens 252 | 249, 1024 tokens 602 | 480; 8 experts of
+// 14336, 2 a token, 64 tokens 682 | 631. MXFP4, 96 tokens 104 | 111, 768 tokens 240 | 251,
+// 1024 tokens 294 | 292; 128 experts of 768, 256 tokens 136 | 148, 512 tokens 203 | 205; 60 of
+// 1408, 4 a token, 300 tokens 134 | 137, 900 tokens 264 | 255; 8 of 14336, 100 tokens 370 |
+// 372, 128 tokens 462 | 398. 20 experts of 224, 3 a token, 512 tokens 38 | 44, bf16 49 | 55).
+int slot_rows(size_t n, size_t E, size_t I, bool mx) {
+    return n <= (mx ? 30 : 8) * E || (E + n / 32) * (I / 16) < 2048 ? 16 : 32;
 }
 // Choices are slots of their own, and nothing is sorted, while about two of them at
 // most are expected to share an expert, whose weights are then read twice: n choices
-// of E experts, n^2 / (2 E) of them. (Sorted | not, us: 3 tokens, MXFP4 33 | 30, bf16 51 |
-// 48; 6 tokens 41 | 40, 78 | 77; 60 experts of 1408, 4 a token, 3 tokens 39 | 37, 6
-// tokens 46 | 49; 8 experts of 4096, 2 a token, 3 tokens 121 | 128.)
+// of E experts, n^2 / (2 E) of them. (Sorted | not, us: 3 tokens, MXFP4 32 | 29, bf16 51 |
+// 49; 6 tokens 40 | 39, 74 | 75; 60 experts of 1408, 4 a token, MXFP4, 3 tokens 34 | 33, 6
+// tokens 40 | 41; 8 experts of 4096, 2 a token, 3 tokens 41 | 48.)
 bool choices_apart(size_t T, size_t n, size_t E) { return T == 1 || n * n <= 4 * E; }
 // k_moe_down_few up to here whatever the work (2 tokens 29 us without, 26 with it)
 constexpr int kFewTokens = 2;
@@ -1291,7 +1294,7 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
     a.k = (int)L->topk;
     a.Is = (int)L->shared_inter;
     a.norm = L->norm_topk;
-    a.group = slot_rows(T * L->topk, L->experts, L->inter);
+    a.group = slot_rows(T * L->topk, L->experts, L->inter, L->mxfp4 != 0);
     a.apart = choices_apart(T, T * L->topk, L->experts);
     a.nslots = (int)(a.apart ? T * L->topk : moe_slots(T, L->topk, L->experts, a.group));
     const int tiles = router_tiles(a);
