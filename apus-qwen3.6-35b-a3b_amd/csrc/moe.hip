@@ -78,8 +78,6 @@ int slot_rows(size_t n, size_t E, size_t I, bool mx) {
 // 49; 6 tokens 40 | 39, 74 | 75; 60 experts of 1408, 4 a token, MXFP4, 3 tokens 34 | 33, 6
 // tokens 40 | 41; 8 experts of 4096, 2 a token, 3 tokens 41 | 48.)
 bool choices_apart(size_t T, size_t n, size_t E) { return T == 1 || n * n <= 4 * E; }
-// k_moe_down_few up to here whatever the work (2 tokens 29 us without, 26 with it)
-constexpr int kFewTokens = 2;
 
 struct MoeArgs {
     const uint16_t *x, *w_router, *w_sgate;
@@ -1113,9 +1111,13 @@ int down_stream_run(const MoeArgs &a, size_t slots) {
 // 76 | 59, 64 tokens 116 | 85; bf16 163 | 156, 234 | 221), but the split form where a
 // wavefront's walk is long and the choices are few (MXFP4: 60 experts of 1408, a shared one
 // of 5632, 4 tokens 40 | 59; 8 experts of 14336, 2 a token, 64 tokens 302 | 342, 128 tokens
-// 417 | 397; bf16, 16 tokens 507 | 557, 64 tokens 664 | 631). k_moe_down_few for work that
-// one round of loads covers (one token: 24 us with the two kernels, 19 with it; bf16 33 and
-// 27), and for kFewTokens.
+// 417 | 397; bf16, 16 tokens 507 | 557, 64 tokens 664 | 631).
+// k_moe_down_few for one token (us without | with it: MXFP4 24 | 19, bf16 33 | 27; 128 experts
+// of 768, 8 a token, 23 | 23, 34 | 34; 60 of 1408, 4 a token, and a shared one of 5632, 27 | 27,
+// 47 | 43; 8 of 14336, 69 | 64, 154 | 140), for two whose work a few rounds of its loads cover
+// (MXFP4 26 | 25, the other layers 28 | 29, 31 | 37, 91 | 107; bf16 42 | 38, 50 | 47, 58 | 60,
+// 240 | 248), and for up to 16 whose work one round does (12 tokens, 16 experts of 128, 2 a
+// token 18 | 16).
 template <class W>
 int experts_run(const MoeArgs &a) {
     const size_t slots = a.nslots;
@@ -1124,7 +1126,7 @@ int experts_run(const MoeArgs &a) {
     if (int r = !ups ? up_run<W>(a, slots) : one ? up_stream_run<W, 1>(a, slots) : up_stream_run<W, 2>(a, slots))
         return r;
     const int units = a.T * (a.k * cdiv(a.I, 128) + cdiv(a.Is, 128));
-    if (a.T <= kFewTokens || (a.T <= 16 && units <= kFewWaves * kFewUnits)) {
+    if (a.T == 1 || (a.T <= 16 && units <= kFewWaves * kFewUnits * (a.T > 2 ? 1 : W::mx ? 2 : 3))) {
         APUS_TIMED("k_moe_down_few", k_moe_down_few<W><<<(unsigned)a.H / 16, 64 * kFewWaves, 0, stream()>>>(a));
         return launch_check("k_moe_down_few");
     }

@@ -145,3 +145,21 @@ def test_inner_values_of_24_bits(hip, T, H, I, E, mx):
     assert int(ok.sum()) >= T - T // 10
     assert torch.equal(y[ok].double(), torch.round(r[ok]))
     work.destroy()
+
+
+# one and two tokens: one round of k_moe_down_few's loads, several, and past what it takes of two tokens
+@pytest.mark.parametrize("T,H,I,E,k,Is", [(1, 96, 1184, 9, 5, 544), (1, 2080, 5600, 4, 2, 32), (2, 288, 512, 40, 8, 512),
+                                          (2, 544, 672, 40, 8, 0), (2, 1056, 1184, 12, 4, 2080), (2, 96, 4128, 5, 2, 64)])
+@pytest.mark.parametrize("mx", [False, True])
+def test_one_and_two_tokens(hip, T, H, I, E, k, Is, mx):
+    import torch
+    g = _gen(torch, T + H + I)
+    w = mx_ref.moe_weights(g, H, I, E, Is, True, mx)
+    x = mx_ref.safe_tokens(g, w, T, k, H)
+    r, b, _ = mx_ref.moe(x, w, k, True, mx)
+    L = _layer(hip, w, k)
+    work = hip.MoeWork(L, T)
+    y = torch.empty_like(x)
+    hip.moe_layer_decode(L, work, x, y)
+    mx_ref.check(y, r, b, "one and two tokens")
+    work.destroy()
