@@ -673,19 +673,17 @@ __device__ __forceinline__ void walk(int n, Load load, Mul mul) {
 
 // XR: loads of four rows that a tile of activations takes (1 for up to 4 rows). SC:
 // MXFP4 weights' scales in strips.
-template <class W, int RT, int NT, int D, int XR, bool SC>
+template <class W, int NT, int D, int XR, bool SC>
 __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, int o0, char *m, int lane) {
     using X = XBf16<W>;
     const int r = lane & 15, g = lane >> 4;
     const bool sh = task.e == a.E;
     const int I = sh ? a.Is : a.I;
-    typename W::Tile wt[RT][2];            // (a tile past I, not stored, repeats the last)
+    typename W::Tile wt[2];                // gate, up
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            wt[t][i] = W::tile(sh ? a.w_sgu : a.w_gu, sh ? a.s_sgu : a.s_gu,
-                               (sh ? 0 : (size_t)task.e * 2 * I) + i * I + min(o0 + 16 * t, I - 16), 16, a.H);
+    for (int i = 0; i < 2; i++)
+        wt[i] = W::tile(sh ? a.w_sgu : a.w_gu, sh ? a.s_sgu : a.s_gu,
+                        (sh ? 0 : (size_t)task.e * 2 * I) + i * I + o0, 16, a.H);
     const auto wl = W::raw_lane(lane, a.H);
     const i32x4 xb = dma_rsrc(a.x, (uint32_t)a.T * (uint32_t)a.H * 2);
     int q[NT];
@@ -699,40 +697,38 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
             xl[u][i] = (uint32_t)(sh ? x - a.T * a.k : x / a.k) * (uint32_t)a.H * 2;
         }
     }
-    typename W::Raw fw[D][RT][2];
+    typename W::Raw fw[D][2];
     RowsBf16::Raw fx[D][NT];
-    char *const mx = m + RT * 2 * W::kTile, *const ms = mx + NT * RowsBf16::kTile;
-    Strip strip[SC ? RT * 2 : 1];
+    char *const mx = m + 2 * W::kTile, *const ms = mx + NT * RowsBf16::kTile;
+    Strip strip[SC ? 2 : 1];
     auto load = [&](int d, int st) {
         if constexpr (SC) {
             if ((st & (Strip::kSteps - 1)) == 0) {
 #pragma unroll
-                for (int t = 0; t < RT * 2; t++) strip[t].load(wt[t / 2][t % 2], st, a.H);
+                for (int t = 0; t < 2; t++) strip[t].load(wt[t], st, a.H);
             }
         }
 #pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) W::template load_raw<!SC>(fw[d][t][i], wt[t][i], wl, st, a.H);
+        for (int i = 0; i < 2; i++) W::template load_raw<!SC>(fw[d][i], wt[i], wl, st, a.H);
 #pragma unroll
         for (int u = 0; u < NT; u++) X::template load_raw<XR>(fx[d][u], xb, xl[u], st, a.H);
     };
-    mx_f32x4 acc[RT][2][NT] = {};
+    mx_f32x4 acc[2][NT] = {};
     walk<D>((a.H + 127) / 128, load, [&](int d, int st) {
 #pragma unroll
-        for (int t = 0; t < RT * 2; t++) W::put(m + t * W::kTile, fw[d][t / 2][t % 2], lane);
+        for (int t = 0; t < 2; t++) W::put(m + t * W::kTile, fw[d][t], lane);
 #pragma unroll
         for (int u = 0; u < NT; u++) RowsBf16::put(mx + u * RowsBf16::kTile, fx[d][u], lane);
-        typename W::Frag f[RT][2];
+        typename W::Frag f[2];
 #pragma unroll
-        for (int t = 0; t < RT * 2; t++) W::template get<!SC>(f[t / 2][t % 2], m + t * W::kTile, fw[d][t / 2][t % 2], lane);
+        for (int t = 0; t < 2; t++) W::template get<!SC>(f[t], m + t * W::kTile, fw[d][t], lane);
         if constexpr (SC) {
             if ((st & (Strip::kSteps - 1)) == 0) {
 #pragma unroll
-                for (int t = 0; t < RT * 2; t++) strip[t].put(ms + t * Strip::kTile);
+                for (int t = 0; t < 2; t++) strip[t].put(ms + t * Strip::kTile);
             }
 #pragma unroll
-            for (int t = 0; t < RT * 2; t++) f[t / 2][t % 2].s = Strip::get(ms + t * Strip::kTile, st, lane);
+            for (int t = 0; t < 2; t++) f[t].s = Strip::get(ms + t * Strip::kTile, st, lane);
         }
         fence();
         load(d, st + D);
@@ -743,60 +739,54 @@ __device__ __forceinline__ void up_stream(const MoeArgs &a, const Task &task, in
 #pragma unroll
             for (int u = 0; u < NT; u++) x[u] = X::piece(mx + u * RowsBf16::kTile, j, lane);
 #pragma unroll
-            for (int t = 0; t < RT; t++)
+            for (int i = 0; i < 2; i++) {
+                const mx_bf16x8 w = W::operand(f[i], j);
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const mx_bf16x8 w = W::operand(f[t][i], j);
-#pragma unroll
-                    for (int u = 0; u < NT; u++) acc[t][i][u] = mfma16(w, x[u], acc[t][i][u]);
-                }
+                for (int u = 0; u < NT; u++) acc[i][u] = mfma16(w, x[u], acc[i][u]);
+            }
         }
         fence();
     });
 #pragma unroll
     for (int u = 0; u < NT; u++) {
         if (16 * u + r >= task.n) continue;
-        const uint32_t at = h_at(a, q[u], sh);
+        const uint32_t at = h_at(a, q[u], sh) + o0 + 4 * g;
+        uint32_t v[4];
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int o = o0 + 16 * t + 4 * g;
-            if (o >= I) continue;
-            uint32_t v[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = __float_as_uint(silu(acc[t][0][u][i]) * acc[t][1][u][i]);
-            const Split s0 = split2(v[0], v[1]), s1 = split2(v[2], v[3]);
-            *reinterpret_cast<u32x4 *>(a.h + (at + o) * 2) = u32x4{s0.v[0], s1.v[0], s0.v[1], s1.v[1]};
-            *reinterpret_cast<uint2 *>(a.hl + at + o) = make_uint2(s0.v[2], s1.v[2]);
-        }
+        for (int i = 0; i < 4; i++) v[i] = __float_as_uint(silu(acc[0][u][i]) * acc[1][u][i]);
+        const Split s0 = split2(v[0], v[1]), s1 = split2(v[2], v[3]);
+        *reinterpret_cast<u32x4 *>(a.h + at * 2) = u32x4{s0.v[0], s1.v[0], s0.v[1], s1.v[1]};
+        *reinterpret_cast<uint2 *>(a.hl + at) = make_uint2(s0.v[2], s1.v[2]);
     }
 }
 
-template <class W, int RT, int NT, bool SC>
+template <class W, int NT, bool SC>
 __global__ __launch_bounds__(64 * kStreamWaves, W::mx ? 3 : 2) void k_moe_up_stream(MoeArgs a, int nsh, int nper) {
-    constexpr int LDS = RT * 2 * (W::kTile + (SC ? Strip::kTile : 0)) + NT * RowsBf16::kTile;
+    constexpr int LDS = 2 * (W::kTile + (SC ? Strip::kTile : 0)) + NT * RowsBf16::kTile;
     __shared__ __attribute__((aligned(16))) char sm[kStreamWaves * LDS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = task_of(a, blockIdx.x, nsh, nper);
-    const int o0 = (task.part * kStreamWaves + wave) * 16 * RT;
+    const int o0 = (task.part * kStreamWaves + wave) * 16;
     if (task.n == 0 || o0 >= (task.e == a.E ? a.Is : a.I)) return;       // (no barrier in this kernel)
-    if (NT > 1 && task.n > 16) up_stream<W, RT, NT, 2, 4, SC>(a, task, o0, sm + wave * LDS, lane);
-    else if (task.n > 4) up_stream<W, RT, 1, 2, 4, SC>(a, task, o0, sm + wave * LDS, lane);
-    else up_stream<W, RT, 1, 2, 1, SC>(a, task, o0, sm + wave * LDS, lane);
+    if (NT > 1 && task.n > 16) up_stream<W, NT, 2, 4, SC>(a, task, o0, sm + wave * LDS, lane);
+    else if (task.n > 4) up_stream<W, 1, 2, 4, SC>(a, task, o0, sm + wave * LDS, lane);
+    else up_stream<W, 1, 2, 1, SC>(a, task, o0, sm + wave * LDS, lane);
 }
 
-// part[choice] = down h: 16 RT outputs a block, P blocks a wavefront in one walk (one
+// part[choice] = down h: 32 outputs a block, P blocks a wavefront in one walk (one
 // block where I takes several chunks). h of the task's rows is brought to LDS once for all
 // the workgroup's blocks, a chunk of 512 elements (with SIDE, of up to kSideRows rows, 2048)
 // at a time; the next chunk's is on its way, in registers, while one is walked.
-constexpr int kDownWaves = 8;
+constexpr int kDownWaves = 8, kDownTiles = 2;            // of 16 outputs, in a block
 constexpr int kDownChunk = 4;                            // steps of 128 elements
 constexpr int kDownH = 16 * 3 * kDownChunk * 256;        // LDS bytes of 16 rows of a chunk
 static_assert(3 * kSideRows * (kDownChunk * 16 / kSideRows) * 256 <= kDownH, "a chunk side by side fits");
-template <class W, int RT, int NT, int D, bool MANY, bool SIDE>
+template <class W, int NT, int D, bool MANY, bool SIDE>
 __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, int b0, int nb, char *h, char *m,
                                             int lane) {
     static_assert(NT == 1 || !SIDE);
+    constexpr int RT = kDownTiles;
     using X = XBf16<W>;
     constexpr int N3 = SIDE ? 1 : 3;       // MFMAs for the three numbers
     constexpr int CHUNK = SIDE ? kDownChunk * 16 / kSideRows : kDownChunk;
@@ -927,9 +917,9 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
     }
 }
 
-template <class W, int RT, int NT, bool MANY>
+template <class W, int NT, bool MANY>
 __global__ __launch_bounds__(64 * kDownWaves, W::mx && NT == 1 ? 4 : 2) void k_moe_down_stream(MoeArgs a, int nsh, int nper, int P) {
-    constexpr int LDS = RT * W::kTile;
+    constexpr int LDS = kDownTiles * W::kTile;
     __shared__ __attribute__((aligned(16))) char sm[kDownWaves * LDS + NT * kDownH];
     char *const h = sm + kDownWaves * LDS;
     const int lane = threadIdx.x & 63;
@@ -937,11 +927,11 @@ __global__ __launch_bounds__(64 * kDownWaves, W::mx && NT == 1 ? 4 : 2) void k_m
     const Task task = task_of(a, blockIdx.x, nsh, nper);
     if (task.n == 0) return;
     char *const m = sm + wave * LDS;
-    const int blocks = (a.H + 16 * RT - 1) / (16 * RT), b0 = (task.part * kDownWaves + wave) * P;
+    const int blocks = (a.H + 16 * kDownTiles - 1) / (16 * kDownTiles), b0 = (task.part * kDownWaves + wave) * P;
     const int nb = min(P, blocks - b0);
-    if (NT > 1 && task.n > 16) down_stream<W, RT, NT, 2, MANY, false>(a, task, b0, nb, h, m, lane);
-    else if (task.n > kSideRows) down_stream<W, RT, 1, 2, MANY, false>(a, task, b0, nb, h, m, lane);
-    else down_stream<W, RT, 1, 2, MANY, true>(a, task, b0, nb, h, m, lane);
+    if (NT > 1 && task.n > 16) down_stream<W, NT, 2, MANY, false>(a, task, b0, nb, h, m, lane);
+    else if (task.n > kSideRows) down_stream<W, 1, 2, MANY, false>(a, task, b0, nb, h, m, lane);
+    else down_stream<W, 1, 2, MANY, true>(a, task, b0, nb, h, m, lane);
 }
 
 // y of up to 16 tokens: 16 outputs a workgroup, the steps of 128 k of every (token,
@@ -1083,22 +1073,22 @@ int up_stream_run(const MoeArgs &a, size_t slots) {
     // (strips: rows of scales in whole, aligned words)
     const bool strips = W::mx && a.H % 128 == 0 && ((uintptr_t)a.s_gu | (uintptr_t)a.s_sgu) % 4 == 0;
     APUS_TIMED("k_moe_up_stream",
-               if (strips) k_moe_up_stream<W, 1, NT, W::mx><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper);
-               else k_moe_up_stream<W, 1, NT, false><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper));
+               if (strips) k_moe_up_stream<W, NT, W::mx><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper);
+               else k_moe_up_stream<W, NT, false><<<g.n, threads, 0, stream()>>>(a, g.nsh, g.nper));
     return launch_check("k_moe_up_stream");
 }
 template <class W, int NT>
 int down_stream_run(const MoeArgs &a, size_t slots) {
-    // blocks of 32 outputs a wavefront, so that the launch keeps about 4096 wavefronts:
+    // blocks of a wavefront, so that the launch keeps about 8192 wavefronts:
     // more share a workgroup's copy of h
-    const size_t blocks = cdiv(a.H, 32);
+    const size_t blocks = cdiv(a.H, 16 * kDownTiles);
     const bool many = std::max(a.I, a.Is) > kDownChunk * 128;
     const int P = many ? 1 : (int)std::max<size_t>(1, std::min<size_t>(4, slots * blocks / 8192));
     const size_t nper = cdiv(blocks, kDownWaves * P);
     const Grid g = grid_of(a, slots, nper, nper);
     APUS_TIMED("k_moe_down_stream",
-               if (many) k_moe_down_stream<W, 2, NT, true><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P);
-               else k_moe_down_stream<W, 2, NT, false><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P));
+               if (many) k_moe_down_stream<W, NT, true><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P);
+               else k_moe_down_stream<W, NT, false><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P));
     return launch_check("k_moe_down_stream");
 }
 
