@@ -163,3 +163,51 @@ def test_one_and_two_tokens(hip, T, H, I, E, k, Is, mx):
     hip.moe_layer_decode(L, work, x, y)
     mx_ref.check(y, r, b, "one and two tokens")
     work.destroy()
+
+
+# the last slot of the one popular expert has 2 rows, of 5, and of 1 (of 16 or of 32)
+@pytest.mark.parametrize("T,H,I", [(66, 5472, 2112), (85, 4128, 4192), (994, 1056, 2112), (993, 1056, 544)])
+@pytest.mark.parametrize("mx", [False, True])
+def test_all_to_one_expert_of_long_rows(hip, T, H, I, mx):
+    """One expert gets every token, in slots that are full but for the last; inner sizes of
+    several chunks, each form of a slot."""
+    import torch
+    print(f"[moe] all to one T={T} H={H} I={I} mx={mx}", flush=True)
+    g = _gen(torch, T + I)
+    w = mx_ref.moe_weights(g, H, I, 2, 0, False, mx)
+    x = mx_ref.normal(g, T, H)
+    x[:, 0] = 1
+    w["w_router"][0, 0] = 40
+    r, b, gap = mx_ref.moe(x, w, 1, True, mx)
+    assert float(gap.min()) > 0
+    L = _layer(hip, w, 1)
+    work = hip.MoeWork(L, T)
+    ys = []
+    for _ in range(3):                                     # (the order within the slots is no matter)
+        y = torch.full_like(x, 7.0)
+        hip.moe_layer_decode(L, work, x, y)
+        ys.append(y)
+    mx_ref.check(ys[0], r, b, "all to one")
+    assert torch.equal(ys[0], ys[1]) and torch.equal(ys[0], ys[2])
+    work.destroy()
+
+
+@pytest.mark.parametrize("T,H,I,E,k,Is", [(64, 1024, 512, 24, 4, 96), (150, 288, 160, 6, 2, 64), (400, 1056, 640, 12, 3, 0)])
+@pytest.mark.parametrize("mx", [False, True])
+def test_outputs_repeat(hip, T, H, I, E, k, Is, mx):
+    """The choices come to their experts' slots in any order: a token's output is the
+    same bits, whatever the order of the tokens."""
+    import torch
+    g = _gen(torch, T + H)
+    w = mx_ref.moe_weights(g, H, I, E, Is, True, mx)
+    x = mx_ref.safe_tokens(g, w, T, k, H)
+    L = _layer(hip, w, k)
+    work = hip.MoeWork(L, T)
+    y = torch.empty_like(x)
+    hip.moe_layer_decode(L, work, x, y)
+    for i in range(8):
+        at = torch.randperm(T, generator=g, device="cuda")
+        z = torch.empty_like(x)
+        hip.moe_layer_decode(L, work, x[at].contiguous(), z)
+        assert torch.equal(z, y[at]), i
+    work.destroy()
