@@ -23,10 +23,11 @@
 //
 // Times below: hidden 2048, 256 experts of 512 inner elements, 8 a token, a shared
 // expert of 512, inputs other than the call before's. The whole layer, us at
-// 1 / 5 / 16 / 64 / 325 tokens: MXFP4 19 / 39 / 60 / 108 / 154 (bytes alone, at a
-// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 26 / 69 / 143 / 287 / 350
+// 1 / 5 / 16 / 64 / 325 tokens: MXFP4 19 / 40 / 63 / 110 / 154 (bytes alone, at a
+// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 28 / 72 / 155 / 291 / 359
 // (11 / 51 / 127 / 272 / 314): with many choices it is bound by the weights' bytes,
-// with few by three launches' latency.
+// with few by three launches' latency. Where a rule gives two sides, the tokens share a
+// direction, so that some experts are preferred.
 #include <stdint.h>
 
 #include <algorithm>
@@ -430,8 +431,8 @@ __device__ __forceinline__ Split split2(uint32_t a, uint32_t b) {
 // times as long (one token: 31 us for the layer, now 26; MXFP4 23, now 19).
 constexpr int kMoeWaves = 8;
 
-// h = silu(gate x) * (up x): 16 outputs a workgroup, 16 rows at a time. One token: 11
-// us for bf16's 38 MB, 4.5 for MXFP4's 10 MB: latency of one round of loads.
+// h = silu(gate x) * (up x): 16 outputs a workgroup, 16 rows at a time. One token: 9.2
+// us for bf16's 38 MB, 4.2 for MXFP4's 10 MB: latency of one round of loads.
 template <class W>
 __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_up(MoeArgs a, int nsh, int nper) {
     constexpr int S = 2;                   // steps in flight at once
@@ -531,7 +532,7 @@ __device__ __forceinline__ mx_f32x4 sum3(const mx_f32x4 (&v)[1]) {
 }
 
 // part[choice] = down h: 32 outputs a group of wavefronts, 16 rows at a time (13 tokens
-// of 1056, 20 experts of 224: 4.4 us). HL: loads of two rows of h (2 HL rows and no more
+// of 1056, 20 experts of 224, MXFP4: 4.6 us). HL: loads of two rows of h (2 HL rows and no more
 // with fewer than 8).
 template <class W, int RT, int HL>
 __device__ __forceinline__ void down_part(const MoeArgs &a, const Task &task, char *sm, int *rows) {
@@ -641,9 +642,9 @@ __global__ __launch_bounds__(64 * kMoeWaves) void k_moe_down(MoeArgs a, int nsh,
 }
 
 // ---- the same, a wavefront alone: no partial sums, and D steps of weights (up: and
-// activations) on their way all along its walk. Up: bf16, 325 tokens, 198
-// us for 1.07 GB, 5.4 TB/s; MXFP4, 64 tokens, 53 us for 247 MB, 4.7 TB/s. Down: 119
-// us for 0.54 GB, 4.5 TB/s; 32 us for 124 MB, 3.9 TB/s. More steps on their way (3, 4)
+// activations) on their way all along its walk. Up: bf16, 325 tokens, 191
+// us for 1.09 GB fetched, 5.7 TB/s; MXFP4, 64 tokens, 45 us for 194 MB, 4.3 TB/s. Down:
+// 103 us for 0.57 GB, 5.5 TB/s; 27 us for 103 MB, 3.8 TB/s. More steps on their way (3, 4)
 // changed nothing, nor did whole 128-byte lines of MXFP4 codes a load.
 constexpr int kStreamWaves = 4;
 
@@ -938,7 +939,7 @@ __global__ __launch_bounds__(64 * kDownWaves, W::mx && NT == 1 ? 4 : 2) void k_m
 // expert) dealt to its 12 wavefronts (9 experts of 4 steps, one token: 3 each, all on
 // their way at once). A step's product lands in the token's column with the
 // expert's weight; the columns of other tokens (all multiplied with this token's h)
-// are left out. One token: 7.8 us for bf16's 19 MB, 6.4 for MXFP4's 5 MB.
+// are left out. One token: 6.0 us for bf16's 19 MB, 5.5 for MXFP4's 5 MB.
 constexpr int kFewWaves = 12, kFewUnits = 3;
 template <class W>
 __global__ __launch_bounds__(64 * kFewWaves) void k_moe_down_few(MoeArgs a) {

@@ -35,7 +35,7 @@ __device__ __forceinline__ Pos pos_of(size_t i, size_t per_row, bool dense) {
 // exponent field of the largest code (a subnormal maximum: the smallest scale,
 // 2^-127); the hardware conversion rounds to nearest even and saturates at 6.
 // A block with an infinity or NaN gets scale 255 (NaN) and zero codes. Bytes: 12352
-// rows of 2048 in 10.2 us, 64 MB, 6.3 TB/s; one row 1.2 us, all launch.
+// rows of 2048 in 12.9 us, 64 MB, 5.0 TB/s; one row 1.2 us, all launch.
 __global__ __launch_bounds__(256) void k_mx_quantize(const uint16_t *__restrict__ x, size_t ldx,
                                                      uint8_t *__restrict__ codes,
                                                      uint8_t *__restrict__ scales, size_t n8,
@@ -78,13 +78,15 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict
 
 // ---- products of few rows --------------------------------------------------
 // A workgroup forms 16 RT outputs x 16 NT rows; its 8 wavefronts take every
-// eighth pair of steps of 128 k, all their loads on the way before the first is
-// used, and their partial sums meet in LDS. Rows come along their length and
+// eighth pair of steps of 128 k, and their partial sums meet in LDS. A pair's loads are all
+// on their way before the first is used; with more than 32 rows of bf16 activations, a
+// step's (there are no registers for more). Rows come along their length and
 // become operands in LDS of the wavefront's own (mx_dev.h): loaded by each lane for
 // itself the product of 37 rows took 10.5 us, now 7.1. XR: the loads of four
 // rows that a tile of bf16 activations has (1 for up to 4 rows).
-// Bound by the latency of a round of loads: 1 row x 12352 outputs, K 2048, 5.7 us for
-// 13.5 MB; 37 rows x 2048 x 4096, 7.1 us; 64 rows of MXFP4 x 2048 x 4096, 5.7 us.
+// Bound by the latency of these rounds of loads, one after the other: 1 row x 12352
+// outputs, K 2048, one round, 5.6 us for 13.5 MB; 37 rows x 2048 x 4096, four, on half the
+// CUs, 7.1 us; 64 rows of MXFP4 x 2048 x 4096, two, on half the CUs, 5.6 us.
 constexpr int kFewWaves = 8;
 
 template <bool XMX, int RT, int NT, int XR>

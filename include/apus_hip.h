@@ -612,7 +612,7 @@ int apus_hip_mxfp4_gemm_mx_dev(const uint8_t *w, const uint8_t *ws, const uint8_
  *   p = softmax of l over the chosen ones (norm_topk) or over all experts;
  *   y = sum_e p_e w_down[e] (silu(gate) * up), (gate | up) = w_gate_up[e] x,
  *       + sigmoid(w_shared_gate . x) times the same of the shared expert.
- * Logits, softmax and sums are fp32; y is rounded once. Logits that are NaN
+ * Logits, softmax, inner values and sums are fp32; y is rounded once. Logits that are NaN
  * count as the largest (that token's y is NaN). The experts' weights are
  * bf16, or MXFP4 with their scales (as in mxfp4_gemm_dev); the router's are bf16. */
 typedef struct {
@@ -632,8 +632,8 @@ typedef struct {
 
 /* The device buffers of calls of up to max_tokens (<= 1024) tokens on layers
  * of this one's sizes (its weights are not looked at): sizes up to 2^20, and at
- * most 2 GiB each of x and of the inner rows, max_tokens * (topk * inter +
- * shared_inter) * 4 bytes. Calls that share one
+ * most 2 GiB each of x and of the inner rows in fp32, max_tokens * (topk * inter +
+ * shared_inter) * 4 bytes (it holds half as much again of these). Calls that share one
  * run one after the other: on one stream, or ordered by the caller; calls or
  * graph replays that may overlap need one each. It must outlive the graphs
  * that captured its calls. destroy waits for the library's stream. */
