@@ -24,7 +24,7 @@
 // Times below: hidden 2048, 256 experts of 512 inner elements, 8 a token, a shared
 // expert of 512, inputs other than the call before's. The whole layer, us at
 // 1 / 5 / 16 / 64 / 325 tokens: MXFP4 19 / 40 / 63 / 110 / 154 (bytes alone, at a
-// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 28 / 72 / 155 / 291 / 359
+// large copy's 5.2 TB/s: 3 / 14 / 35 / 74 / 86), bf16 27 / 71 / 152 / 291 / 359
 // (11 / 51 / 127 / 272 / 314): with many choices it is bound by the weights' bytes,
 // with few by three launches' latency. Where a rule gives two sides, the tokens share a
 // direction, so that some experts are preferred.
@@ -779,11 +779,16 @@ __global__ __launch_bounds__(64 * kStreamWaves, W::mx ? 3 : 2) void k_moe_up_str
 // block where I takes several chunks). h of the task's rows is brought to LDS once for all
 // the workgroup's blocks, a chunk of 512 elements (with SIDE, of up to kSideRows rows, 2048)
 // at a time; the next chunk's is on its way, in registers, while one is walked.
-constexpr int kDownWaves = 8, kDownTiles = 2;            // of 16 outputs, in a block
+constexpr int kDownTiles = 2;                            // of 16 outputs, in a block
+// wavefronts of a workgroup: two of 8 a CU, with bf16 weights, whose registers leave room for
+// 8 wavefronts, two of 4, or one of 8 where h takes more LDS (128 experts of 768, 8 a token,
+// bf16, 64 tokens 222 us with one of 8, now 218; 1024 tokens, 32 rows, 661 with 4, 524 with 8)
+template <class W, int NT>
+constexpr int kDownWaves = W::mx || NT > 1 ? 8 : 4;
 constexpr int kDownChunk = 4;                            // steps of 128 elements
 constexpr int kDownH = 16 * 3 * kDownChunk * 256;        // LDS bytes of 16 rows of a chunk
 static_assert(3 * kSideRows * (kDownChunk * 16 / kSideRows) * 256 <= kDownH, "a chunk side by side fits");
-template <class W, int NT, int D, bool MANY, bool SIDE>
+template <class W, int NT, int D, int WAVES, bool MANY, bool SIDE>
 __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, int b0, int nb, char *h, char *m,
                                             int lane) {
     static_assert(NT == 1 || !SIDE);
@@ -820,12 +825,12 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
     // Piece c of number p of the task's row i lies at c ^ k within its 256 bytes, in LDS row
     // 3 i + p, k = i, or with SIDE in row k = kSideRows p + i. A thread's pieces past the last
     // row are the last row's again.
-    constexpr int PIECES = ((SIDE ? kSideRows : 16 * NT) * (MANY ? CHUNK : kDownChunk) * 16 + 64 * kDownWaves - 1) / (64 * kDownWaves);
+    constexpr int PIECES = ((SIDE ? kSideRows : 16 * NT) * (MANY ? CHUNK : kDownChunk) * 16 + 64 * WAVES - 1) / (64 * WAVES);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto row_of = [&](int n) {
-        return min(ROWS ? wave + n * kDownWaves : (int)(threadIdx.x + n * 64 * kDownWaves) / pc, task.n - 1);
+        return min(ROWS ? wave + n * WAVES : (int)(threadIdx.x + n * 64 * WAVES) / pc, task.n - 1);
     };
-    auto piece_of = [&](int n) { return ROWS ? lane : (int)(threadIdx.x + n * 64 * kDownWaves) % pc; };
+    auto piece_of = [&](int n) { return ROWS ? lane : (int)(threadIdx.x + n * 64 * WAVES) % pc; };
     uint32_t at[PIECES];                   // elements before the rows
 #pragma unroll
     for (int n = 0; n < PIECES; n++) at[n] = h_at(a, choice(task, row_of(n)), sh);
@@ -846,7 +851,7 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
     auto put_h = [&]() {
 #pragma unroll
         for (int n = 0; n < PIECES; n++) {
-            if ((n * kDownWaves + wave) * 64 >= task.n * pc) continue;       // (all past the last row)
+            if ((n * WAVES + wave) * 64 >= task.n * pc) continue;       // (all past the last row)
             const int i = row_of(n);
             const u32x4 a0 = hr[n][0], a1 = hr[n][1];
             const u32x4 v[3] = {u32x4{a0[0], a0[1], a1[0], a1[1]}, u32x4{a0[2], a0[3], a1[2], a1[3]}, hr[n][2]};
@@ -919,20 +924,20 @@ __device__ __forceinline__ void down_stream(const MoeArgs &a, const Task &task, 
 }
 
 template <class W, int NT, bool MANY>
-__global__ __launch_bounds__(64 * kDownWaves, W::mx && NT == 1 ? 4 : 2) void k_moe_down_stream(MoeArgs a, int nsh, int nper, int P) {
-    constexpr int LDS = kDownTiles * W::kTile;
-    __shared__ __attribute__((aligned(16))) char sm[kDownWaves * LDS + NT * kDownH];
-    char *const h = sm + kDownWaves * LDS;
+__global__ __launch_bounds__((64 * kDownWaves<W, NT>), W::mx && NT == 1 ? 4 : 2) void k_moe_down_stream(MoeArgs a, int nsh, int nper, int P) {
+    constexpr int LDS = kDownTiles * W::kTile, WAVES = kDownWaves<W, NT>;
+    __shared__ __attribute__((aligned(16))) char sm[WAVES * LDS + NT * kDownH];
+    char *const h = sm + WAVES * LDS;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = task_of(a, blockIdx.x, nsh, nper);
     if (task.n == 0) return;
     char *const m = sm + wave * LDS;
-    const int blocks = (a.H + 16 * kDownTiles - 1) / (16 * kDownTiles), b0 = (task.part * kDownWaves + wave) * P;
+    const int blocks = (a.H + 16 * kDownTiles - 1) / (16 * kDownTiles), b0 = (task.part * WAVES + wave) * P;
     const int nb = min(P, blocks - b0);
-    if (NT > 1 && task.n > 16) down_stream<W, NT, 2, MANY, false>(a, task, b0, nb, h, m, lane);
-    else if (task.n > kSideRows) down_stream<W, 1, 2, MANY, false>(a, task, b0, nb, h, m, lane);
-    else down_stream<W, 1, 2, MANY, true>(a, task, b0, nb, h, m, lane);
+    if (NT > 1 && task.n > 16) down_stream<W, NT, 2, WAVES, MANY, false>(a, task, b0, nb, h, m, lane);
+    else if (task.n > kSideRows) down_stream<W, 1, 2, WAVES, MANY, false>(a, task, b0, nb, h, m, lane);
+    else down_stream<W, 1, 2, WAVES, MANY, true>(a, task, b0, nb, h, m, lane);
 }
 
 // y of up to 16 tokens: 16 outputs a workgroup, the steps of 128 k of every (token,
@@ -1082,24 +1087,25 @@ template <class W, int NT>
 int down_stream_run(const MoeArgs &a, size_t slots) {
     // blocks of a wavefront, so that the launch keeps about 8192 wavefronts:
     // more share a workgroup's copy of h
+    constexpr int WAVES = kDownWaves<W, NT>;
     const size_t blocks = cdiv(a.H, 16 * kDownTiles);
     const bool many = std::max(a.I, a.Is) > kDownChunk * 128;
     const int P = many ? 1 : (int)std::max<size_t>(1, std::min<size_t>(4, slots * blocks / 8192));
-    const size_t nper = cdiv(blocks, kDownWaves * P);
+    const size_t nper = cdiv(blocks, WAVES * P);
     const Grid g = grid_of(a, slots, nper, nper);
     APUS_TIMED("k_moe_down_stream",
-               if (many) k_moe_down_stream<W, NT, true><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P);
-               else k_moe_down_stream<W, NT, false><<<g.n, 64 * kDownWaves, 0, stream()>>>(a, g.nsh, g.nper, P));
+               if (many) k_moe_down_stream<W, NT, true><<<g.n, 64 * WAVES, 0, stream()>>>(a, g.nsh, g.nper, P);
+               else k_moe_down_stream<W, NT, false><<<g.n, 64 * WAVES, 0, stream()>>>(a, g.nsh, g.nper, P));
     return launch_check("k_moe_down_stream");
 }
 
 // The streaming forms from 1024 wavefronts on, 4 a CU (the layer, us split | streamed;
 // up, MXFP4: 5 tokens 38 | 40, 16 tokens 58 | 54, 64 tokens 100 | 90, 325 tokens 181 | 153;
-// down: 5 tokens 48 | 39, 64 tokens 149 | 90; bf16 72 | 69, 266 | 231). bf16 weights' up
+// down: 5 tokens 48 | 39, 64 tokens 149 | 90; bf16 72 | 67, 266 | 231). bf16 weights' up
 // product is 4 times the bytes a step, which the split form keeps on their way as well with
 // few rows a slot (16 tokens 130 | 130, 64 tokens 239 | 231, 325 tokens 393 | 345).
 // Inner sizes of several chunks too (down, 128 experts of 768, 8 a token, MXFP4: 16 tokens
-// 76 | 59, 64 tokens 116 | 85; bf16 163 | 156, 234 | 221), but the split form where a
+// 76 | 59, 64 tokens 116 | 85; bf16 163 | 153, 234 | 218), but the split form where a
 // wavefront's walk is long and the choices are few (MXFP4: 60 experts of 1408, a shared one
 // of 5632, 4 tokens 40 | 59; 8 experts of 14336, 2 a token, 64 tokens 302 | 342, 128 tokens
 // 417 | 397; bf16, 16 tokens 507 | 557, 64 tokens 664 | 631).
