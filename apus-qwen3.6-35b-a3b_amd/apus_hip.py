@@ -56,6 +56,9 @@ EXPORTS = [
     "apus_hip_mxfp4_quantize", "apus_hip_mxfp4_dequantize", "apus_hip_mxfp4_gemm_dev",
     "apus_hip_mxfp4_gemm_mx_dev", "apus_hip_moe_work_create", "apus_hip_moe_work_destroy",
     "apus_hip_moe_layer_decode",
+    "apus_hip_kv8_append", "apus_hip_kv8_read", "apus_hip_kv8_pool_create", "apus_hip_kv8_pool_cache",
+    "apus_hip_attn_kv8_work_create", "apus_hip_attn_kv8_work_destroy", "apus_hip_attn_decode_kv8",
+    "apus_hip_attn_prefill_kv8", "apus_hip_attn_layer_decode_kv8", "apus_hip_block_norm",
 ]
 
 
@@ -76,6 +79,18 @@ class KvCache(C.Structure):
     """ApusHipKvCache (include/apus_hip.h): a paged KV cache."""
     _fields_ = [("k", _vp), ("v", _vp), ("block_table", _vp), ("max_blocks", _sz),
                 ("max_rows", _sz), ("row_blocks", _vp)]
+
+
+class Kv8Cache(C.Structure):
+    """ApusHipKv8Cache (include/apus_hip.h): an 8-bit KV cache, flat or paged."""
+    _fields_ = [("k", _vp), ("v", _vp), ("scale", _vp), ("blocks", _sz), ("block_table", _vp),
+                ("max_blocks", _sz), ("max_rows", _sz), ("row_blocks", _vp)]
+
+
+class BlockNorm(C.Structure):
+    """ApusHipBlockNorm (include/apus_hip.h): the norms around a block."""
+    _fields_ = [("hidden", _sz), ("h_f32", C.c_int), ("scale", C.c_float), ("eps", C.c_float),
+                ("w_post", _vp), ("w_pre", _vp), ("gate", _vp), ("ld_gate", _sz)]
 
 
 class AttnLayer(C.Structure):
@@ -139,7 +154,10 @@ def load(path=None):
         # (argument types declared: plain integers go in as they are)
         for name, types in (("mxfp4_quantize", "pzppzz"), ("mxfp4_dequantize", "pppzzz"),
                             ("mxfp4_gemm_dev", "pppzpzzzz"), ("mxfp4_gemm_mx_dev", "pppppzzzz"),
-                            ("moe_layer_decode", "ppzpp")):
+                            ("moe_layer_decode", "ppzpp"), ("kv8_append", "pzzppppzpz"),
+                            ("kv8_read", "pzzppppzpz"), ("attn_decode_kv8", "ppzpppppppp"),
+                            ("attn_prefill_kv8", "ppzpppppppp"), ("attn_layer_decode_kv8", "pppzpppppp"),
+                            ("block_norm", "pzpzpzpzpz")):
             getattr(_lib, "apus_hip_" + name).argtypes = [_vp if t == "p" else _sz for t in types]
     return _lib
 
@@ -604,14 +622,21 @@ def gdn_prefill_slots(layer, slots, cu, qkv, z, a, b, conv, S, y):
 
 
 class KvPool:
-    """apus_hip_kv_pool_*: a paged KV cache shared by nlayers layers."""
+    """apus_hip_kv_pool_*: a paged KV cache shared by nlayers layers (kv8: of
+    8-bit blocks, apus_hip_kv8_pool_*; cache() then gives a Kv8Cache)."""
 
-    def __init__(self, nlayers, nkv, d, nblocks, max_rows, max_blocks):
+    def __init__(self, nlayers, nkv, d, nblocks, max_rows, max_blocks, kv8=False):
         self.h = C.c_void_p()
-        _chk(load().apus_hip_kv_pool_create(_sz(nlayers), _sz(nkv), _sz(d), _sz(nblocks),
-                                            _sz(max_rows), _sz(max_blocks), C.byref(self.h)))
+        self.kv8, self.nkv = kv8, nkv
+        f = load().apus_hip_kv8_pool_create if kv8 else load().apus_hip_kv_pool_create
+        _chk(f(_sz(nlayers), _sz(nkv), _sz(d), _sz(nblocks), _sz(max_rows), _sz(max_blocks), C.byref(self.h)))
 
     def cache(self, layer):
+        if self.kv8:
+            kv = Kv8Cache()
+            _chk(load().apus_hip_kv8_pool_cache(self.h, _sz(layer), C.byref(kv)))
+            kv.nkv = self.nkv
+            return kv
         kv = KvCache()
         _chk(load().apus_hip_kv_pool_cache(self.h, _sz(layer), C.byref(kv)))
         return kv
@@ -761,7 +786,7 @@ def _rows(t, what, dev, ncols=None):
     if ncols is not None and n != ncols:
         raise ValueError(f"{what}: rows of {n} elements, expected {ncols}")
     ld, one = t.stride()
-    if one != 1 and n > 1:
+    if one != 1 and n > 1 and m:
         raise ValueError(f"{what}: elements of a row must be contiguous")
     return t.data_ptr(), m, n, ld if m > 1 else n
 
@@ -881,6 +906,205 @@ def moe_layer_decode(layer, work, x, y):
             raise ValueError(f"{n}: contiguous [T, {H}] bf16 on GPU {dev}, not {tuple(t.shape)} {t.dtype} "
                              f"on {t.device}")
     _chk(load().apus_hip_moe_layer_decode(C.byref(layer), work.h, x.shape[0], x.data_ptr(), y.data_ptr()))
+
+
+# ---- 8-bit KV cache
+def kv8_cache(nkv, blocks, max_blocks, block_table=None, d=256):
+    """A Kv8Cache of new device arrays for blocks blocks of 32 positions and nkv
+    heads: flat, max_blocks blocks a row, or with block_table (a device tensor
+    [rows, max_blocks] of int32) paged. It keeps its tensors alive."""
+    import torch
+    if d != 256:
+        raise ValueError(f"an 8-bit KV cache has head dim 256, not {d}")
+    if block_table is not None and (
+            block_table.get_device() != _device or block_table.dtype != torch.int32 or block_table.dim() != 2
+            or block_table.shape[1] != max_blocks or not block_table.is_contiguous()):
+        raise ValueError(f"block_table: contiguous int32 [rows, {max_blocks}] on GPU {_device}, not "
+                         f"{tuple(block_table.shape)} {block_table.dtype} on {block_table.device}")
+    dev = torch.device("cuda", _device)
+    k, v = (torch.empty(blocks, nkv, 32 * d, dtype=torch.uint8, device=dev) for _ in range(2))
+    scale = torch.empty(blocks, nkv, 2, dtype=torch.float32, device=dev)
+    kv = Kv8Cache(k.data_ptr(), v.data_ptr(), scale.data_ptr(), blocks,
+                  None if block_table is None else block_table.data_ptr(), max_blocks,
+                  blocks // max_blocks if block_table is None else block_table.shape[0], None)
+    kv.nkv = nkv
+    kv._tensors = (k, v, scale, block_table)
+    return kv
+
+
+def _batch(rows, cu, pos0):
+    """(B, pointers of rows, cu, pos0 as int32 host arrays, the arrays)."""
+    keep = [None if a is None else np.ascontiguousarray(a, dtype=np.int32) for a in (rows, cu, pos0)]
+    r, c, p = keep
+    if c.ndim != 1 or p.shape != (len(c) - 1,) or (r is not None and r.shape != p.shape):
+        raise ValueError(f"cu has one offset more than pos0 (and rows) entries: {c.shape}, {p.shape}, "
+                         f"{None if r is None else r.shape}")
+    return len(p), (None if r is None else r.ctypes.data), c.ctypes.data, p.ctypes.data, keep
+
+
+def _total(cu):
+    return int(cu[-1])
+
+
+def _kv8_rows_call(f, kv, rows, cu, pos0, k, v):
+    B, rp, cp, pp, keep = _batch(rows, cu, pos0)
+    n, T = kv.nkv * 256, _total(keep[1])
+    ld = []
+    for t, what in ((k, "k"), (v, "v")):
+        p, m, _, pitch = _rows(t.flatten(1) if t.dim() == 3 else t, what, _device, n)
+        if m != T:
+            raise ValueError(f"{what}: {m} rows, expected {T}")
+        ld += [p, max(pitch, n)]
+    return BoundCall(f, (C.addressof(kv), kv.nkv, B, rp, cp, pp, *ld), (kv, keep, k, v))
+
+
+def kv8_append_bound(kv, rows, cu, pos0, k, v):
+    """kv8_append as a BoundCall (rows, cu, pos0 as int32 numpy arrays may be
+    changed in place between calls)."""
+    return _kv8_rows_call(load().apus_hip_kv8_append, kv, rows, cu, pos0, k, v)
+
+
+def kv8_append(kv, rows, cu, pos0, k, v):
+    """k, v [T, nkv * 256] bf16 (rows of any pitch) into the 8-bit cache at the
+    positions pos0[s] ... of sequence s's row (rows None: row s)."""
+    kv8_append_bound(kv, rows, cu, pos0, k, v)()
+
+
+def kv8_read_bound(kv, rows, cu, pos0, k, v):
+    """kv8_read as a BoundCall."""
+    return _kv8_rows_call(load().apus_hip_kv8_read, kv, rows, cu, pos0, k, v)
+
+
+def kv8_read(kv, rows, cu, pos0, k, v):
+    """The values of the positions pos0[s] ... into k, v [T, nkv * 256] bf16."""
+    kv8_read_bound(kv, rows, cu, pos0, k, v)()
+
+
+class AttnKv8Work:
+    """apus_hip_attn_kv8_work_*: the device buffers of attention calls on an
+    8-bit cache, for layers of one shape, decode calls of up to max_seqs sequences
+    and positions below max_pos. Calls that may overlap (other streams, graphs
+    replayed at once) need one each."""
+
+    def __init__(self, layer, max_seqs, max_pos):
+        self.h = C.c_void_p()
+        _chk(load().apus_hip_attn_kv8_work_create(C.byref(layer), _sz(max_seqs), _sz(max_pos), C.byref(self.h)))
+
+    def destroy(self):
+        if self.h:
+            _chk(load().apus_hip_attn_kv8_work_destroy(self.h))
+            self.h = C.c_void_p()
+
+
+def _dense(t, shape, what):
+    """Pointer of a contiguous bf16 tensor of so many elements and that last
+    size on the library's device (None: NULL)."""
+    if t is None:
+        return None
+    n = 1
+    for x in shape:
+        n *= x
+    if t.get_device() != _device or not _bf16(t) or not t.is_contiguous() or t.numel() != n or t.shape[0] != shape[0]:
+        raise ValueError(f"{what}: contiguous {shape} bf16 on GPU {_device}, not {tuple(t.shape)} {t.dtype} "
+                         f"on {t.device}")
+    return t.data_ptr()
+
+
+def _attn_kv8_call(f, layer, work, rows, cu, pos0, qg, k, v, kv, y):
+    B, rp, cp, pp, keep = _batch(rows, cu, pos0)
+    T, nh, nkv, d = _total(keep[1]), layer.nh, layer.nkv, layer.d
+    if kv.nkv != nkv:
+        raise ValueError(f"kv: a cache of {kv.nkv} heads, the layer has {nkv}")
+    args = (C.addressof(layer), work.h, B, rp, cp, pp, _dense(qg, (T, nh, 2 * d), "qg"),
+            _dense(k, (T, nkv, d), "k"), _dense(v, (T, nkv, d), "v"), C.addressof(kv), _dense(y, (T, nh * d), "y"))
+    return BoundCall(f, args, (layer, work, keep, qg, k, v, kv, y))
+
+
+def attn_decode_kv8_bound(layer, work, rows, cu, pos0, qg, k, v, kv, y):
+    """attn_decode_kv8 as a BoundCall."""
+    return _attn_kv8_call(load().apus_hip_attn_decode_kv8, layer, work, rows, cu, pos0, qg, k, v, kv, y)
+
+
+def attn_decode_kv8(layer, work, rows, cu, pos0, qg, k, v, kv, y):
+    """Decode / verify of 0..4 new tokens a sequence on an 8-bit cache; k = v =
+    None: their rows are in the cache already."""
+    attn_decode_kv8_bound(layer, work, rows, cu, pos0, qg, k, v, kv, y)()
+
+
+def attn_prefill_kv8_bound(layer, work, rows, cu, pos0, qg, k, v, kv, y):
+    """attn_prefill_kv8 as a BoundCall."""
+    return _attn_kv8_call(load().apus_hip_attn_prefill_kv8, layer, work, rows, cu, pos0, qg, k, v, kv, y)
+
+
+def attn_prefill_kv8(layer, work, rows, cu, pos0, qg, k, v, kv, y):
+    """As attn_decode_kv8 for any number of new tokens a sequence."""
+    attn_prefill_kv8_bound(layer, work, rows, cu, pos0, qg, k, v, kv, y)()
+
+
+def attn_layer_decode_kv8(layer, proj, work, rows, cu, pos0, ln1, kv, ao):
+    """attn_layer_decode on an 8-bit cache: ln1 [T, H] -> ao [T, H]."""
+    B, rp, cp, pp, keep = _batch(rows, cu, pos0)
+    T = _total(keep[1])
+    if kv.nkv != layer.nkv:
+        raise ValueError(f"kv: a cache of {kv.nkv} heads, the layer has {layer.nkv}")
+    _chk(load().apus_hip_attn_layer_decode_kv8(
+        C.addressof(layer), C.addressof(proj), work.h, B, rp, cp, pp, _dense(ln1, (T, proj.hidden), "ln1"),
+        C.addressof(kv), _dense(ao, (T, proj.hidden), "ao")))
+
+
+# ---- the norms around a block
+def block_norm_weights(hidden, w_pre=None, w_post=None, gate=None, scale=1.0, eps=1e-6):
+    """ApusHipBlockNorm from device tensors: w_pre, w_post [hidden] (1+w) norm
+    weights, gate [hidden] (one row for all tokens) or [T, hidden], all bf16 and
+    optional. It keeps them alive."""
+    ptr, ld = {}, 0
+    for what, t in (("w_pre", w_pre), ("w_post", w_post), ("gate", gate)):
+        if t is None:
+            continue
+        if what == "gate" and t.dim() == 2:
+            ptr[what], _, _, ld = _rows(t, what, _device, hidden)
+            ld = max(ld, hidden)
+            continue
+        if t.get_device() != _device or not _bf16(t) or tuple(t.shape) != (hidden,) or not t.is_contiguous():
+            raise ValueError(f"{what}: contiguous ({hidden},) bf16 on GPU {_device}, not {tuple(t.shape)} {t.dtype} "
+                             f"on {t.device}")
+        ptr[what] = t.data_ptr()
+    N = BlockNorm(hidden=hidden, scale=scale, eps=eps, ld_gate=ld, **ptr)
+    N._tensors = (w_pre, w_post, gate)
+    N._gate_rows = gate.shape[0] if gate is not None and gate.dim() == 2 else None
+    return N
+
+
+def _f32_rows(t, what, dev, ncols):
+    import torch
+    if t.dim() != 2 or t.get_device() != dev or t.dtype != torch.float32 or t.shape[1] != ncols or (
+            t.stride(1) != 1 and ncols > 1):
+        raise ValueError(f"{what}: a 2-D tensor of fp32 rows of {ncols} on GPU {dev}, not {tuple(t.shape)} "
+                         f"{t.dtype} on {t.device}")
+    return t.data_ptr(), t.shape[0], ncols, t.stride(0) if t.shape[0] > 1 else ncols
+
+
+def block_norm(norm, y, h, h_out, x):
+    """h_out = h + scale gate post(y), x = pre(h_out): y, x [T, hidden] bf16, h
+    and h_out bf16 or fp32, rows of any pitch. y None: x = pre(h); x None: only
+    h_out. h_out may be h, x may be y."""
+    dev, n = _device, norm.hidden
+    f32 = h.element_size() == 4
+    hp, T, _, ldh = _f32_rows(h, "h", dev, n) if f32 else _rows(h, "h", dev, n)
+    args = []
+    for t, what in ((y, "y"), (h_out, "h_out"), (x, "x")):
+        if t is None:
+            args.append((None, n))
+            continue
+        p, m, _, ld = _f32_rows(t, what, dev, n) if f32 and what == "h_out" else _rows(t, what, dev, n)
+        if m != T:
+            raise ValueError(f"{what}: {m} rows, expected {T}")
+        args.append((p, max(ld, n)))
+    if norm._gate_rows is not None and norm._gate_rows != T:
+        raise ValueError(f"gate: {norm._gate_rows} rows, expected {T}")
+    norm.h_f32 = int(f32)
+    (yp, ldy), (op, ldo), (xp, ldx) = args
+    _chk(load().apus_hip_block_norm(C.addressof(norm), T, yp, ldy, hp, max(ldh, n), op, ldo, xp, ldx))
 
 
 # ---- named-intermediate capture

@@ -1,0 +1,298 @@
+// attn_kv8_fa.hip -- gated-GQA attention of any number of new tokens a sequence
+// over the 8-bit KV cache (kv8.h), the formula of attn_kv8.hip.
+//
+// One workgroup a (tile of 32 tokens, kv head), the longest contexts first: the
+// 8 q heads times 32 tokens are 256 rows, 32 a wavefront, whose q and outputs
+// stay in registers. The keys are walked once, 64 (two blocks) at a time, with a
+// running reference point M and sum of the softmax: a tile's codes go from
+// memory to registers while the tile before is worked on, widen there (exactly: K's
+// codes to fp16, V's times their scale to bf16) and come into LDS in operand order. The
+// products run on the 32x32x16 MFMA with keys (or dims) on the M side:
+// S^T = K Q^T leaves each lane 16 scores of one row, which are the operand of
+// O^T += V^T P^T with no exchange, if V's keys are laid out in the same order:
+// lane half h takes the keys 8 q + 4 h + 0..3, q = 0..3, 8 a step.
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "apus_dev.h"
+#include "apus_host.h"
+#include "attn_mixer.h"
+#include "kv8.h"
+
+using namespace apus;
+
+namespace {
+
+constexpr int D = kKv8D, ROT = 64, GRP = 8, KEYS = kKv8Keys;
+constexpr int kTok = 32;                     // tokens of a tile
+constexpr int kTile = 64;                    // keys of a step
+constexpr int KP = D * 2 + 16;               // LDS pitches (bytes): a key's K row, a dim's V row
+constexpr int VP = kTile * 2 + 16;
+constexpr float kEps = 1e-6f, kL2E = 1.44269504088896341f;
+constexpr float kSlack = 10.0f;              // as in attn_kv8.hip
+
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef kv8_bf16x8 bf16x8;
+typedef kv8_f16x8 f16x8;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// 4 e4m3 codes times a power of two as bf16
+__device__ __forceinline__ u32x2 widen4(uint32_t a, float s) {
+    const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false);
+    const bf16x2 q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true);
+    return u32x2{__builtin_bit_cast(uint32_t, p), __builtin_bit_cast(uint32_t, q)};
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+struct Tile {
+    u32x4 k[2], v[2];                        // a thread's pieces of the two blocks
+    float ks[2], vs[2];
+};
+
+template <int N>
+__global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg,
+                                                const uint16_t *__restrict__ qn_w,
+                                                const uint16_t *__restrict__ rope, int nkv, float c2,
+                                                uint16_t *__restrict__ y) {
+    __shared__ __attribute__((aligned(16))) char kl[2][kTile * KP];
+    __shared__ __attribute__((aligned(16))) char vl[2][D * VP];
+    __shared__ int first_nan[D];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kvh = blockIdx.x % nkv, item = sq.off[sq.n] - 1 - (int)blockIdx.x / nkv;
+    const int s = kv8_seq_of(sq.off, sq.n, item);
+    const int t0 = sq.cu[s], ns = sq.cu[s + 1] - t0, p0 = sq.pos0[s], row = sq.row[s], nh = nkv * GRP;
+    const int f0 = (item - sq.off[s]) * kTok;              // the tile's first token in its sequence
+    const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees
+    const int ctx = p0 + ns, steps = (end + kTile - 1) / kTile;
+    if (tid < D) first_nan[tid] = 0x7fffffff;
+
+    Tile next;
+    auto fetch = [&](int st) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int b = min(st * 2 + u, (ctx - 1) / KEYS);
+            const size_t hb = (size_t)kv8_id_u(kv, row, b) * nkv + kvh;
+            next.k[u] = *reinterpret_cast<const u32x4 *>(kv.k + hb * kKv8Bytes + tid * 16);
+            next.v[u] = *reinterpret_cast<const u32x4 *>(kv.v + hb * kKv8Bytes + tid * 16);
+            const int32_t *sc = (const int32_t *)(kv.scale + hb * 2);
+            next.ks[u] = __int_as_float(sload_i32(sc, 8, 0));
+            next.vs[u] = __int_as_float(sload_i32(sc, 8, 1));
+        }
+    };
+    // a thread's pieces (kv8.h) to their places in LDS
+    auto put = [&](int st, int buf) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int key = u * KEYS + tid / 256 * 16 + tid % 16, c = tid / 16 % 16;
+            char *const kd = kl[buf] + key * KP + c * 32;
+            *reinterpret_cast<f16x8 *>(kd) = kv8_f16(next.k[u][0], next.k[u][1]);
+            *reinterpret_cast<f16x8 *>(kd + 16) = kv8_f16(next.k[u][2], next.k[u][3]);
+            const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16;
+            u32x4 c4 = next.v[u];
+            const int k0_ = (st * 2 + u) * KEYS + g * 4;   // the piece's keys: k0_ .. + 3 and 16 on
+            if (k0_ + 19 >= p0 + f0) {                     // some row does not see some of them
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int left = ctx - (k0_ + w % 2 * 16);      // past the last token: zero
+                    c4[w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+                    const uint32_t bad = kv8_nan_codes(c4[w]);
+                    if (bad) {                             // out of the product, its first key kept
+                        c4[w] &= ~bad;
+                        atomicMin(&first_nan[d + w / 2 * 16], k0_ + w % 2 * 16 + (__ffs((int)bad) - 1) / 8);
+                    }
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                // four keys from 4 G: half G % 2, step G / 4, its first or second four
+                const int G = g + w % 2 * 4, at = u * 64 + (G / 4 * 2 + G % 2) * 16 + G / 2 % 2 * 8;
+                *reinterpret_cast<u32x2 *>(vl[buf] + (d + w / 2 * 16) * VP + at) = widen4(c4[w], next.vs[u]);
+            }
+        }
+    };
+    fetch(0);
+
+    // the wavefront's q rows n = (token 4 wave + n / 8, head n % 8): k-step i, dims 16 i + 8 hf ..
+    const int tok = f0 + wave * 4 + (n >> 3), h = kvh * GRP + (n & 7);
+    const int pos = p0 + min(tok, ns - 1);
+    f16x8 q[16];
+    float qf;                                              // scores' factor, with log2 e / 16
+    {
+        const uint16_t *qr = qg + ((size_t)(t0 + min(tok, ns - 1)) * nh + h) * 2 * D + hf * 8;
+        u16x8 x[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = *reinterpret_cast<const u16x8 *>(qr + i * 16);
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) ss += bf2f(x[i][e]) * bf2f(x[i][e]);
+        ss += __shfl_xor(ss, 32);
+        const float rs = 1.0f / sqrtf(ss / (float)D + kEps);
+        // formed twice: for the largest magnitude, then for the fp16 rows (the
+        // fp32 rows would take another 64 registers)
+        auto form = [&](int i, float (&o)[8]) {            // chunk i, after norm and RoPE
+            const u16x8 w = *reinterpret_cast<const u16x8 *>(qn_w + i * 16 + hf * 8);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = bf2f(x[i][e]) * rs * (1.0f + bf2f(w[e]));
+            if (i >= 4) return;
+            const int j = i ^ 2, p = (i & 1) * 16 + hf * 8;    // the chunk 32 dims away
+            const u16x8 wj = *reinterpret_cast<const u16x8 *>(qn_w + j * 16 + hf * 8);
+            const u16x8 co = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + p);
+            const u16x8 si = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + ROT / 2 + p);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float b = bf2f(x[j][e]) * rs * (1.0f + bf2f(wj[e]));
+                o[e] = o[e] * bf2f(co[e]) + (i < 2 ? -b : b) * bf2f(si[e]);
+            }
+        };
+        float mx = 0.0f, o[8];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            form(i, o);
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(o[e]));
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float sc = kv8_row_scale(mx), inv = 1.0f / sc;
+        qf = sc * c2;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            form(i, o);
+#pragma unroll
+            for (int e = 0; e < 8; e++) q[i][e] = (_Float16)(o[e] * inv);
+        }
+    }
+    __syncthreads();                                       // (first_nan is clear)
+    put(0, 0);
+
+    f32x16 acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
+    float M = -INFINITY, l = 0.0f;
+    const int wfirst = p0 + min(f0 + wave * 4, ns - 1), wlast = p0 + min(f0 + wave * 4 + 3, ns - 1);
+    for (int st = 0; st < steps; st++) {
+        const int buf = st & 1;
+        const float cs[2] = {next.ks[0], next.ks[1]};
+        fetch(min(st + 1, steps - 1));
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int k0 = st * kTile + u * KEYS;
+            if (k0 > wlast) break;                         // (wave-uniform)
+            f32x16 S;
+#pragma unroll
+            for (int e = 0; e < 16; e++) S[e] = 0.0f;
+            const char *kp = kl[buf] + (u * KEYS + n) * KP + hf * 16;
+#pragma unroll
+            for (int i = 0; i < 16; i++) S = mfma32(*reinterpret_cast<const f16x8 *>(kp + i * 32), q[i], S);
+            S *= qf * cs[u];
+            if (k0 + KEYS > wfirst + 1) {
+                const int lim = pos - k0 - 4 * hf;
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (8 * (e / 4) + e % 4 > lim) S[e] = -INFINITY;
+            }
+            float mx = S[0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) mx = fmaxf(mx, S[e]);
+            if (__any(mx > M + kSlack)) {
+                const float m = fmaxf(M, fmaxf(mx, __shfl_xor(mx, 32)));
+                const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - m);
+                M = m;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) acc[i] *= f;
+            }
+            const float ref = M == -INFINITY ? 0.0f : M;
+            uint32_t p[8];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                const float a = __builtin_amdgcn_exp2f(S[e] - ref), b = __builtin_amdgcn_exp2f(S[e + 1] - ref);
+                l += a + b;
+                p[e / 2] = pack2(a, b);
+            }
+            const char *vp = vl[buf] + n * VP + u * 64 + hf * 16;
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                const bf16x8 pb = __builtin_bit_cast(bf16x8, u32x4{p[4 * a], p[4 * a + 1], p[4 * a + 2], p[4 * a + 3]});
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    acc[i] = mfma32(*reinterpret_cast<const bf16x8 *>(vp + i * 32 * VP + a * 32), pb, acc[i]);
+            }
+        }
+        if (st + 1 < steps) put(st + 1, buf ^ 1);
+    }
+    __syncthreads();                                       // (first_nan is whole)
+    l += __shfl_xor(l, 32);
+    if (tok >= ns) return;
+    const float inv = 1.0f / l;
+    const size_t at = (size_t)(t0 + tok) * nh + h;
+    const uint16_t *gate = qg + at * 2 * D + D;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {                      // dims 32 i + 8 c + 4 hf ..
+            const int d = 32 * i + 8 * c + 4 * hf;
+            const uint2 gc = *reinterpret_cast<const uint2 *>(gate + d);
+            const uint32_t gw[2] = {gc.x, gc.y};
+            uint32_t o[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float gv = bf2f((uint16_t)(gw[e / 2] >> (16 * (e % 2))));
+                float v = acc[i][4 * c + e] * inv / (1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
+                if (first_nan[d + e] <= pos) v = NAN;
+                o[e / 2] |= (uint32_t)f2bf(v) << (16 * (e % 2));
+            }
+            *reinterpret_cast<uint2 *>(y + at * D + d) = make_uint2(o[0], o[1]);
+        }
+}
+
+}  // namespace
+
+extern "C" {
+
+int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
+                              const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
+                              const uint16_t *v, const ApusHipKv8Cache *kv, uint16_t *y) {
+    APUS_ENABLED();
+    Kv8Ref r;
+    size_t T = 0;
+    if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, &r, &T)) return e;
+    if (int e = mx_ready()) return e;
+    if (!T) return kOk;
+    const size_t nkv = L->nkv;
+    if (k)
+        if (int e = kv8_append_run(r, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
+    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + kTok - 1) / kTok; },
+                        [&](const auto &q) {
+        constexpr int N = sizeof(q.pos0) / 4;
+        const size_t grid = (size_t)q.off[q.n] * nkv;
+        if (!grid) return (int)kOk;
+        if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
+        const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
+        APUS_TIMED("k_kv8_fa", k_kv8_fa<N><<<(unsigned)grid, 512, 0, stream()>>>(q, r, qg, L->qn_w, w->rope, (int)nkv,
+                                                                                 c2, y));
+        return launch_check("k_kv8_fa");
+    });
+}
+
+}  // extern "C"

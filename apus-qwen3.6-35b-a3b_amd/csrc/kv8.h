@@ -1,0 +1,187 @@
+// kv8.h -- the 8-bit KV cache: its blocks, its scales, and the per-call
+// metadata of the kernels that write, read and attend over it.
+//
+// A block holds 32 positions of one kv head as e4m3 codes, K and V 8 KiB each,
+// with one power-of-two scale for K and one for V: value = code * scale. The
+// bytes lie in the order in which the matrix instructions of the decode kernel
+// take them (16x16x32: lane l holds row l % 16 and the 8 k of group g = l / 16),
+// so that a wavefront's 16-byte loads are whole KiB and go to the matrix cores
+// as they come, without a pass through LDS:
+//   K, key x d: [key / 16][d / 16][key % 16][d % 16]. A 1 KiB load is 16 keys'
+//     d-chunks 4 i .. 4 i + 3, lane group g the chunk 4 i + g: two k-steps of 8.
+//   V, d x key: [d / 32][g][d % 16][(d / 16) % 2][8], the 8 bytes the keys
+//     4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3: those that lane group g has
+//     scores of after K Q^T, so the probabilities go on to P V from the
+//     registers that they are formed in.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../include/apus_hip.h"
+#include "apus_dev.h"
+#include "apus_rt.h"
+#include "mx.h"
+
+namespace apus {
+
+constexpr int kKv8D = 256;                   // head dim
+constexpr int kKv8Keys = 32;                 // positions of a block
+constexpr int kKv8Bytes = kKv8Keys * kKv8D;  // bytes of a head's K or V block
+constexpr int kKv8MinExp = -117;             // smallest exponent of a scale: its codes' steps stay normal in bf16
+
+struct Kv8Ref {
+    uint8_t *k, *v;
+    float *scale;                            // [block][nkv][2]: K's, V's
+    const int32_t *btab;                     // nullptr: flat
+    int32_t bstride;                         // blocks per table row
+    uint32_t blocks;                         // blocks of the arrays
+};
+
+// byte of (key, d) in a K block, of (d, key) in a V block
+__host__ __device__ constexpr int kv8_k_at(int key, int d) {
+    return ((key / 16) * 16 + d / 16) * 256 + (key % 16) * 16 + d % 16;
+}
+__host__ __device__ constexpr int kv8_v_at(int d, int key) {
+    return (d / 32) * 1024 + ((key % 16) / 4 * 16 + d % 16) * 16 + (d / 16 % 2) * 8 +
+           key / 16 * 4 + key % 4;
+}
+
+// The id of block b of the table row h; what the table holds past the arrays'
+// blocks reads as their last block (a stale entry must not reach past them).
+__device__ __forceinline__ uint32_t kv8_id(const Kv8Ref &r, int h, int b) {
+    const size_t at = (size_t)h * r.bstride + b;
+    return min(r.btab ? (uint32_t)r.btab[at] : (uint32_t)at, r.blocks - 1);
+}
+// the same for a wave-uniform (h, b), through the scalar cache
+__device__ __forceinline__ uint32_t kv8_id_u(const Kv8Ref &r, int h, int b) {
+    const size_t at = (size_t)__builtin_amdgcn_readfirstlane(h) * r.bstride;
+    const int bu = __builtin_amdgcn_readfirstlane(b);
+    const uint32_t id = r.btab ? (uint32_t)sload_i32(r.btab + at, (uint32_t)r.bstride * 4, bu)
+                               : (uint32_t)at + (uint32_t)bu;
+    return min(id, r.blocks - 1);
+}
+
+// The sequences of one launch, by value (a captured call keeps them; longer
+// batches take several launches). Few sequences: the short form, whose copy at
+// launch is shorter. off: blocks before each sequence's, in the kernel's count.
+constexpr int kKv8Seqs = 224, kKv8FewSeqs = 8;
+template <int N> struct Kv8SeqsN {
+    int32_t n;
+    int32_t cu[N + 1], pos0[N], off[N + 1], row[N];
+};
+using Kv8Seqs = Kv8SeqsN<kKv8Seqs>;
+
+template <int N> __host__ __device__ inline int kv8_seq_of(const int32_t (&off)[N], int n, int x) {
+    int lo = 0, hi = n - 1;                  // the largest s with off[s] <= x
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (off[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Calls f(seqs, first, blocks) for each launch's share of a batch; count(s) is
+// the number of blocks of sequence s. f returns a status.
+template <class Count, class F>
+int kv8_launches(size_t B, const int32_t *rows, const int32_t *cu, const int32_t *pos0, Count count, F f) {
+    for (size_t s0 = 0; s0 < B; s0 += kKv8Seqs) {
+        const size_t n = B - s0 < (size_t)kKv8Seqs ? B - s0 : (size_t)kKv8Seqs;
+        auto fill = [&](auto &q) {
+            q.n = (int32_t)n;
+            q.off[0] = 0;
+            for (size_t i = 0; i < n; i++) {
+                const size_t s = s0 + i;
+                q.cu[i] = cu[s];
+                q.pos0[i] = pos0[s];
+                q.row[i] = rows ? rows[s] : (int32_t)s;
+                q.off[i + 1] = q.off[i] + count(s);
+            }
+            q.cu[n] = cu[s0 + n];
+            return f(q);
+        };
+        int r;
+        if (n <= (size_t)kKv8FewSeqs) {
+            Kv8SeqsN<kKv8FewSeqs> q;
+            r = fill(q);
+        } else {
+            Kv8Seqs q;
+            r = fill(q);
+        }
+        if (r) return r;
+    }
+    return kOk;
+}
+
+// ---- for the attention kernels -------------------------------------------
+// The scores' product runs in fp16: a code is an fp16 value (up to 448, steps
+// down to 2^-9), and q keeps 11 bits there where bf16 has 8 (its rounding was
+// the largest error of y: 0.004 of y's norm, now 0.002 with y's own rounding).
+// A row of q is divided by a power of two that brings its largest magnitude to
+// [2^6, 2^7), which keeps 256 products with codes in fp32's range with room and
+// the small elements out of fp16's subnormals; the power and the block's scale
+// are factors of the scores. (A row of zeros: 1. One that holds an infinity or
+// NaN: NaN.)
+typedef _Float16 kv8_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 kv8_f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 kv8_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 kv8_bf16x2 __attribute__((ext_vector_type(2)));
+
+// the power of two for a largest magnitude amax (finite)
+__device__ __forceinline__ float kv8_row_scale(float amax) {
+    const int e = min(max((int)(__float_as_uint(amax) >> 23), 1), 247);
+    return amax == 0.0f ? 1.0f : __uint_as_float((uint32_t)max(e - 6, 1) << 23);
+}
+// 8 codes as fp16, and times a power of two as bf16
+__device__ __forceinline__ kv8_f16x8 kv8_f16(uint32_t a, uint32_t b) {
+    const kv8_f16x2 p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+    const kv8_f16x2 q = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+    const kv8_f16x2 r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
+    const kv8_f16x2 u = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+    return kv8_f16x8{p[0], p[1], q[0], q[1], r[0], r[1], u[0], u[1]};
+}
+__device__ __forceinline__ kv8_bf16x8 kv8_bf16(uint32_t a, uint32_t b, float s) {
+    const kv8_bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, false);
+    const kv8_bf16x2 q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, s, true);
+    const kv8_bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false);
+    const kv8_bf16x2 u = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true);
+    return kv8_bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], u[0], u[1]};
+}
+// the codes among c's four that are NaN, 0xff each
+__device__ __forceinline__ uint32_t kv8_nan_codes(uint32_t c) {
+    return ((((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+}
+
+// Host checks, the same with and without a device.
+// The batch against the cache: offsets, positions, rows (distinct where tokens
+// are written). Fills r and the number of tokens.
+int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *rows, const int32_t *cu,
+              const int32_t *pos0, bool writes, Kv8Ref *r, size_t *tokens);
+// k, v: dense rows [token][nkv][256], or of a pitch. kn_w: the K rows are normed
+// and roped first (rope: the table's rows).
+int kv8_append_run(const Kv8Ref &kv, size_t nkv, size_t B, const int32_t *rows, const int32_t *cu,
+                   const int32_t *pos0, const uint16_t *k, size_t ldk, const uint16_t *v, size_t ldv,
+                   const uint16_t *kn_w, const uint16_t *rope);
+bool kv8_overlap(const void *a, size_t na, const void *b, size_t nb);
+
+// Checks of the attention calls (decode's: with its limits), and decode itself.
+int attn_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
+                   const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
+                   const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T);
+int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
+                          const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
+                          const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T);
+int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
+                        const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
+                        const uint16_t *v, const Kv8Ref &kv, uint16_t *y);
+
+}  // namespace apus
+
+struct ApusHipAttnKv8Work {
+    size_t nkv, max_seqs, max_pos;
+    size_t rot;
+    double theta;
+    int device;
+    char *base;
+    float *part;                             // [slot][32 rows][256]
+    float2 *stat;                            // [slot][32 rows]: reference point, sum
+    uint16_t *rope;                          // [max_pos][64] cos, sin
+};

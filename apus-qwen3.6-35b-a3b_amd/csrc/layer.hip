@@ -25,6 +25,7 @@
 #include "apus_host.h"
 #include "attn_mixer.h"
 #include "gdn_mixer.h"
+#include "kv8.h"
 #include "proj.h"
 
 using namespace apus;
@@ -89,12 +90,12 @@ int gdn_layer_run(const ApusHipGdnLayer *L, const ApusHipGdnProj *P, size_t B,
     return gemm_tile(out, y, T, vd, kGemmOut);
 }
 
-// The full-attention layer: wq | wk | wv -> mixer -> wo. rows: the paged
-// cache's block-table rows (HOST), or null for the flat cache (kv built by
-// the caller).
-int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B,
-                   const int32_t *rows, const int32_t *cu, const int32_t *pos0,
-                   const uint16_t *ln1, const KvRef &kv, uint16_t *ao) {
+// The full-attention layer: wq | wk | wv -> mixer -> wo. mixer(qg, k, v, y): the
+// decode mixer on the caller's cache; check(qg, k, v, y), before anything runs:
+// its own checks of its arguments.
+template <class Check, class Mixer>
+int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B, const int32_t *cu,
+                   const uint16_t *ln1, uint16_t *ao, Check check, Mixer mixer) {
     if (int r = attn_check_layer(L)) return r;
     if (!P) return set_error(kErrArgument, "NULL projections");
     if (B == 0) return kOk;
@@ -116,6 +117,7 @@ int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B
     uint16_t *v = (uint16_t *)scratch(kScratchLayerC, T * nk * 2);
     uint16_t *y = (uint16_t *)scratch(kScratchLayerY, T * no * 2);
     if (!qg || !k || !v || !y) return kErrHip;
+    if (int r = check(qg, k, v, y)) return r;
     GemmSegs in{};
     in.n = 3;
     in.row0[1] = (int)nq;
@@ -125,12 +127,22 @@ int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B
     in.w[1] = P->wk; in.y[1] = k;  in.ldy[1] = (int)nk;
     in.w[2] = P->wv; in.y[2] = v;  in.ldy[2] = (int)nk;
     if (int r = gemm_tile(in, ln1, T, H, kGemmIn)) return r;
-    if (int r = attn_decode_kv(L, B, cu, pos0, rows, qg, k, v, kv, y)) return r;
+    if (int r = mixer(qg, k, v, y)) return r;
     GemmSegs out{};
     out.n = 1;
     out.row0[1] = (int)H;
     out.w[0] = P->wo; out.y[0] = ao; out.ldy[0] = (int)H;
     return gemm_tile(out, y, T, no, kGemmOut);
+}
+
+// on a cache given as a KvRef; rows: the paged cache's block-table rows (HOST),
+// or null for the flat cache
+int attn_layer_kv(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B, const int32_t *rows,
+                  const int32_t *cu, const int32_t *pos0, const uint16_t *ln1, const KvRef &kv, uint16_t *ao) {
+    return attn_layer_run(L, P, B, cu, ln1, ao, [](auto...) { return (int)kOk; },
+                          [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, uint16_t *y) {
+        return attn_decode_kv(L, B, cu, pos0, rows, qg, k, v, kv, y);
+    });
 }
 
 }  // namespace
@@ -159,7 +171,7 @@ int apus_hip_attn_layer_decode(const ApusHipAttnLayer *L, const ApusHipAttnProj 
                                uint16_t *ao) {
     APUS_READY();
     if (max_seq % KVB != 0) return set_error(kErrArgument, "max_seq must be a multiple of %d", KVB);
-    return attn_layer_run(L, P, B, nullptr, cu, pos0, ln1, kv_flat(kcache, vcache, max_seq), ao);
+    return attn_layer_kv(L, P, B, nullptr, cu, pos0, ln1, kv_flat(kcache, vcache, max_seq), ao);
 }
 
 int apus_hip_attn_layer_decode_paged(const ApusHipAttnLayer *L, const ApusHipAttnProj *P,
@@ -169,7 +181,23 @@ int apus_hip_attn_layer_decode_paged(const ApusHipAttnLayer *L, const ApusHipAtt
     APUS_READY();
     KvRef r;
     if (int e = kv_paged_ref(kv, B, rows, cu, pos0, &r)) return e;
-    return attn_layer_run(L, P, B, rows, cu, pos0, ln1, r, ao);
+    return attn_layer_kv(L, P, B, rows, cu, pos0, ln1, r, ao);
+}
+
+int apus_hip_attn_layer_decode_kv8(const ApusHipAttnLayer *L, const ApusHipAttnProj *P,
+                                   ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
+                                   const int32_t *cu, const int32_t *pos0, const uint16_t *ln1,
+                                   const ApusHipKv8Cache *kv, uint16_t *ao) {
+    APUS_READY();
+    Kv8Ref r;
+    return attn_layer_run(L, P, B, cu, ln1, ao,
+                          [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, const uint16_t *y) {
+        size_t T = 0;
+        if (int e = attn_decode_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, &r, &T)) return e;
+        return mx_ready();
+    }, [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, uint16_t *y) {
+        return attn_decode_kv8_run(L, w, B, rows, cu, pos0, qg, k, v, r, y);
+    });
 }
 
 }  // extern "C"

@@ -16,6 +16,18 @@ inline bool block_overlaps(const void *b, size_t nb, const void *rows, size_t pi
     return i < M && r0 + i * pitch < b0 + nb;
 }
 
+// Two sets of M rows (first row, bytes between rows, bytes of a row) share
+// bytes. Rows of one pitch may interleave (column slices of one buffer);
+// otherwise the sets' extents decide.
+inline bool rows_overlap(const void *a, size_t pa, size_t na, const void *b, size_t pb, size_t nb, size_t M) {
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    const uintptr_t a1 = a0 + (M - 1) * pa + na, b1 = b0 + (M - 1) * pb + nb;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (pa != pb) return true;
+    const size_t off = (b0 >= a0 ? b0 - a0 : pa - (a0 - b0) % pa) % pa;
+    return off < na || off + nb > pa;
+}
+
 // y = x w^T: M rows, O outputs, K inner elements; x is bf16 rows of pitch ldx, or,
 // with xs, MXFP4
 struct MxProduct {

@@ -216,18 +216,6 @@ constexpr size_t kMxMaxPitch = (size_t)1 << 21;
 // elements of a matrix with its gaps (no extent overflows, tiles count in 32 bits)
 constexpr size_t kMxMaxElements = (size_t)1 << 40;
 
-// Two sets of M rows (first row, bytes between rows, bytes of a row) share
-// bytes. Rows of one pitch may interleave (column slices of one buffer);
-// otherwise the sets' extents decide.
-bool rows_overlap(const void *a, size_t pa, size_t na, const void *b, size_t pb, size_t nb, size_t M) {
-    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-    const uintptr_t a1 = a0 + (M - 1) * pa + na, b1 = b0 + (M - 1) * pb + nb;
-    if (a1 <= b0 || b1 <= a0) return false;
-    if (pa != pb) return true;
-    const size_t off = (b0 >= a0 ? b0 - a0 : pa - (a0 - b0) % pa) % pa;
-    return off < na || off + nb > pa;
-}
-
 int gemm_check(const uint8_t *w, const uint8_t *ws, const void *x, const uint8_t *xs, size_t ldx,
                const uint16_t *y, size_t ldy, size_t M, size_t O, size_t K) {
     if (int r = mx_check_dims(M, O, K)) return r;

@@ -52,7 +52,8 @@ int zero_async(void *p, size_t bytes) {
 
 struct ApusHipKvPool {
     size_t nlayers, nkv, d, nblocks, max_rows, max_blocks;
-    std::vector<uint16_t *> k, v;          // per layer: nblocks blocks of nkv*32*d
+    std::vector<uint16_t *> k, v;          // per layer: nblocks blocks of nkv*32*d (8 bits: half the bytes)
+    std::vector<float *> scale;            // 8-bit blocks: per layer [nblocks][nkv][2]
     int32_t *dtab = nullptr;               // device [max_rows][max_blocks]
     std::vector<int32_t> htab;             // host copy of the table
     std::vector<int32_t> nused;            // blocks held per row; -1: row free
@@ -71,32 +72,42 @@ extern "C" {
 
 // ---- paged KV cache ---------------------------------------------------------
 
-int apus_hip_kv_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblocks,
-                            size_t max_rows, size_t max_blocks, ApusHipKvPool **out) {
+static int kv_pool_make(size_t nlayers, size_t nkv, size_t d, size_t nblocks, size_t max_rows,
+                        size_t max_blocks, bool kv8, ApusHipKvPool **out) {
     APUS_READY();
     if (!out) return set_error(kErrArgument, "NULL output");
     *out = nullptr;
     if (!nlayers || !nkv || d != 256 || !nblocks || !max_rows || !max_blocks ||
         nblocks > 0x7fffffff || max_blocks > 0x7fffffff || max_rows > 0x7fffffff)
         return set_error(kErrArgument, "bad KV pool dimensions (d must be 256)");
-    auto *p = new ApusHipKvPool{nlayers, nkv, d, nblocks, max_rows, max_blocks, {}, {}, nullptr,
-                                {}, {}, {}, {}};
-    const size_t bytes = nblocks * nkv * KVB * d * 2;
+    auto *p = new ApusHipKvPool{};
+    p->nlayers = nlayers;
+    p->nkv = nkv;
+    p->d = d;
+    p->nblocks = nblocks;
+    p->max_rows = max_rows;
+    p->max_blocks = max_blocks;
+    const size_t bytes = nblocks * nkv * KVB * d * (kv8 ? 1 : 2);
     auto fail = [&](int r) {
         for (auto x : p->k) (void)hipFree(x);
         for (auto x : p->v) (void)hipFree(x);
+        for (auto x : p->scale) (void)hipFree(x);
         if (p->dtab) (void)hipFree(p->dtab);
         delete p;
         return r;
     };
     for (size_t l = 0; l < nlayers; l++) {
-        void *a = nullptr, *b = nullptr;
+        void *a = nullptr, *b = nullptr, *c = nullptr;
         if (hipMalloc(&a, bytes) != hipSuccess)
             return fail(set_error(kErrHip, "hipMalloc of %zu bytes of KV blocks failed", bytes));
         p->k.push_back((uint16_t *)a);
         if (hipMalloc(&b, bytes) != hipSuccess)
             return fail(set_error(kErrHip, "hipMalloc of %zu bytes of KV blocks failed", bytes));
         p->v.push_back((uint16_t *)b);
+        if (!kv8) continue;
+        if (hipMalloc(&c, nblocks * nkv * 8) != hipSuccess)
+            return fail(set_error(kErrHip, "hipMalloc of %zu bytes of KV scales failed", nblocks * nkv * 8));
+        p->scale.push_back((float *)c);
     }
     const size_t tbytes = (max_rows * max_blocks * 4 + 15) / 16 * 16;
     if (hipMalloc((void **)&p->dtab, tbytes) != hipSuccess)
@@ -111,12 +122,23 @@ int apus_hip_kv_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblocks
     return kOk;
 }
 
+int apus_hip_kv_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblocks,
+                            size_t max_rows, size_t max_blocks, ApusHipKvPool **out) {
+    return kv_pool_make(nlayers, nkv, d, nblocks, max_rows, max_blocks, false, out);
+}
+
+int apus_hip_kv8_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblocks,
+                             size_t max_rows, size_t max_blocks, ApusHipKvPool **out) {
+    return kv_pool_make(nlayers, nkv, d, nblocks, max_rows, max_blocks, true, out);
+}
+
 int apus_hip_kv_pool_destroy(ApusHipKvPool *p) {
     APUS_READY();
     if (!p) return kOk;
     APUS_HIP_TRY(hipStreamSynchronize(stream()));
     for (auto x : p->k) (void)hipFree(x);
     for (auto x : p->v) (void)hipFree(x);
+    for (auto x : p->scale) (void)hipFree(x);
     (void)hipFree(p->dtab);
     delete p;
     return kOk;
@@ -124,12 +146,21 @@ int apus_hip_kv_pool_destroy(ApusHipKvPool *p) {
 
 int apus_hip_kv_pool_cache(const ApusHipKvPool *p, size_t layer, ApusHipKvCache *out) {
     if (!p || !out || layer >= p->nlayers) return set_error(kErrArgument, "bad pool or layer");
+    if (!p->scale.empty()) return set_error(kErrArgument, "the pool's blocks are 8-bit (kv8_pool_cache)");
     out->k = p->k[layer];
     out->v = p->v[layer];
     out->block_table = p->dtab;
     out->max_blocks = p->max_blocks;
     out->max_rows = p->max_rows;
     out->row_blocks = p->nused.data();
+    return kOk;
+}
+
+int apus_hip_kv8_pool_cache(const ApusHipKvPool *p, size_t layer, ApusHipKv8Cache *out) {
+    if (!p || !out || layer >= p->nlayers) return set_error(kErrArgument, "bad pool or layer");
+    if (p->scale.empty()) return set_error(kErrArgument, "the pool's blocks are bf16 (kv_pool_cache)");
+    *out = ApusHipKv8Cache{(uint8_t *)p->k[layer], (uint8_t *)p->v[layer], p->scale[layer], p->nblocks,
+                           p->dtab, p->max_blocks, p->max_rows, p->nused.data()};
     return kOk;
 }
 

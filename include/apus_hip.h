@@ -647,6 +647,123 @@ int apus_hip_moe_work_destroy(ApusHipMoeWork *w);
 int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_t T,
                               const uint16_t *x, uint16_t *y);
 
+/* ---- 8-bit KV cache ------------------------------------------------------
+ * The KV cache of a full-attention layer in half the bytes: blocks of 32
+ * positions as above, K and V of a kv head as e4m3 codes, with one scale each
+ * for K and V of every block and kv head, a power of two 2^e in fp32: e is the
+ * smallest integer >= -117 with amax <= 448 2^e over the block's positions, a
+ * code is value / 2^e rounded to nearest even. A block that is written in
+ * several calls keeps what it holds of the positions before pos0: where new
+ * tokens need a larger scale, its codes are rounded again at that scale (exact,
+ * but for values that fall below 2^-6 of it). The scale of a block that is
+ * being filled does not fall: positions taken back and written again keep
+ * their mark on it. A block written from its first position on starts anew. An
+ * infinity or NaN is stored as NaN and does not count in the scale.
+ *
+ * k, v: blocks * nkv * 8192 bytes each, 16-byte aligned; scale: blocks * nkv
+ * * 2 floats (K's, V's). block_table: DEVICE [max_rows][max_blocks], or NULL:
+ * a flat cache, where row r owns the blocks r * max_blocks ... An entry that is
+ * no block of the arrays is never written through, and reads as some block.
+ * row_blocks as in ApusHipKvCache. The order of the bytes in a block is the
+ * library's own (kv8_append and kv8_read convert). Head dim 256.
+ *
+ * In all calls below rows (HOST, or NULL: sequence s lives at row s), cu and
+ * pos0 (HOST) say what in apus_hip_attn_decode_paged they say; a sequence may
+ * have no tokens. Host arrays go by value: the calls can be captured into
+ * graphs, allocate nothing and do not wait, and what a captured call was given
+ * stays as it was. Bad arguments are refused with or without a device. Two
+ * sequences of a call that writes may not share a row; calls that write a row
+ * and calls that use it run in the caller's order (one stream, or events).
+ * They are not traced (apus_hip_trace_set). */
+typedef struct {
+    uint8_t *k, *v;
+    float *scale;
+    size_t blocks;
+    const int32_t *block_table;
+    size_t max_blocks, max_rows;
+    const int32_t *row_blocks;
+} ApusHipKv8Cache;
+
+/* k, v [Ttot][nkv * 256] bf16, rows of pitch ldk / ldv (multiples of 8, 16-byte
+ * aligned), as they are, into positions pos0[s] ... of sequence s's row. */
+int apus_hip_kv8_append(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const int32_t *rows,
+                        const int32_t *cu, const int32_t *pos0, const uint16_t *k, size_t ldk,
+                        const uint16_t *v, size_t ldv);
+/* The inverse: the values of the positions pos0[s] ... as bf16 (exact). */
+int apus_hip_kv8_read(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const int32_t *rows,
+                      const int32_t *cu, const int32_t *pos0, uint16_t *k, size_t ldk,
+                      uint16_t *v, size_t ldv);
+
+/* A KV pool (above) of 8-bit blocks: opened, reserved and closed by the same
+ * calls; kv8_pool_cache gives a layer's descriptor (kv_pool_cache refuses it). */
+int apus_hip_kv8_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblocks,
+                             size_t max_rows, size_t max_blocks, ApusHipKvPool **out);
+int apus_hip_kv8_pool_cache(const ApusHipKvPool *pool, size_t layer, ApusHipKv8Cache *out);
+
+/* What attention calls on an 8-bit cache need on the device for layers of this
+ * one's dims (its weights are not looked at): partial results of a decode call
+ * and the RoPE table of positions below max_pos (up to 2^24). max_seqs: the most
+ * sequences of a decode call. Calls that share one run one after the other:
+ * on one stream, or ordered by the caller; calls or graph replays that may
+ * overlap need one each. It must outlive the graphs that captured its calls.
+ * destroy waits for the library's stream. */
+typedef struct ApusHipAttnKv8Work ApusHipAttnKv8Work;
+int apus_hip_attn_kv8_work_create(const ApusHipAttnLayer *L, size_t max_seqs, size_t max_pos,
+                                  ApusHipAttnKv8Work **out);
+int apus_hip_attn_kv8_work_destroy(ApusHipAttnKv8Work *w);
+
+/* apus_hip_attn_decode on an 8-bit cache, 0..4 new tokens a sequence: the k
+ * rows normed and roped as there and v appended as by kv8_append, then causal
+ * GQA over the cache, the output gate. k = v = NULL: the new tokens' positions
+ * hold their rows already (written by kv8_append, normed and roped, or by a
+ * layer that shares its cache); then sequences may share rows. After norm and
+ * RoPE q is rounded to fp16 once, at a power of two of its row, probabilities
+ * to bf16 for their product with V; scores, softmax and sums are fp32 and y is
+ * rounded once: a tolerance class of the result on the cache's values, |c - r| <=
+ * 2^-8 |r| + sum_j P_j |V_j| sigmoid(gate) (2^-8 + 2^-10 + e_j), e_j = 2^-12 (a_j +
+ * sum_i P_i a_i) from q's rounding, a_j = sum_d |q_d K_jd| / 16. A NaN in a position that a token does not attend to
+ * does not reach its row. Supports d=256, rot=64, nh=8*nkv. y may not overlap
+ * the inputs. */
+int apus_hip_attn_decode_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B,
+                             const int32_t *rows, const int32_t *cu, const int32_t *pos0,
+                             const uint16_t *qg, const uint16_t *k, const uint16_t *v,
+                             const ApusHipKv8Cache *kv, uint16_t *y);
+/* The same for any number of new tokens a sequence. */
+int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B,
+                              const int32_t *rows, const int32_t *cu, const int32_t *pos0,
+                              const uint16_t *qg, const uint16_t *k, const uint16_t *v,
+                              const ApusHipKv8Cache *kv, uint16_t *y);
+/* apus_hip_attn_layer_decode on an 8-bit cache (library scratch holds the
+ * projections' outputs: a call that needs more than any before allocates). */
+int apus_hip_attn_layer_decode_kv8(const ApusHipAttnLayer *L, const ApusHipAttnProj *P,
+                                   ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
+                                   const int32_t *cu, const int32_t *pos0, const uint16_t *ln1,
+                                   const ApusHipKv8Cache *kv, uint16_t *ao);
+
+/* ---- the norms around a block ---------------------------------------------
+ * Between one block (mixer or experts) and the next, for T tokens:
+ *   h' = h + scale * gate * post(y)     y the block's output, h the residual
+ *   x  = pre(h')                        the next block's input
+ * post, pre: (1+w) RMSNorm over the hidden size, v / sqrt(mean v^2 + eps) (1 +
+ * w), as apus_hip_attn_rmsnorm's. All of it in fp32; h' and x are each rounded
+ * once (x from the h' before its rounding).
+ * w_post NULL: y as it is. gate: bf16 [T][hidden] of pitch ld_gate, or one row
+ * for all tokens (ld_gate 0), or NULL: 1. h and h' are bf16, or fp32 (h_f32).
+ * y NULL: h' = h (h_out may be NULL: a model's first norm); x NULL: only h'.
+ * h_out may be h, x may be y (with the same pitch); other overlaps of an output
+ * are refused. Rows of any pitch and alignment to an element; hidden up to
+ * 16384, T up to 2^24. Nothing is allocated, and a call may be captured. */
+typedef struct {
+    size_t hidden;
+    int h_f32;
+    float scale, eps;
+    const uint16_t *w_post, *w_pre, *gate;
+    size_t ld_gate;
+} ApusHipBlockNorm;
+int apus_hip_block_norm(const ApusHipBlockNorm *N, size_t T, const uint16_t *y, size_t ldy,
+                        const void *h, size_t ldh, void *h_out, size_t ldo, uint16_t *x,
+                        size_t ldx);
+
 #ifdef __cplusplus
 }
 #endif
