@@ -5,14 +5,16 @@
 // softmax (p = 2^(t - M), t the score times log2 e / 16).
 //
 // The 8 q heads of a kv head times up to 4 new tokens are the rows of the matrix
-// products (one or two blocks of 16), so K and V are read once a (sequence, kv
+// products, one or two blocks of 16, so K and V come from HBM once a (sequence, kv
 // head) pair. The pairs' blocks are laid end to end and cut into equal runs, one
 // a workgroup and as many as CUs, so that every CU reads as much however ragged
 // the contexts are; a run that crosses a pair's border is two segments. The 8
-// wavefronts of a workgroup take every eighth block of a segment, each with its
-// own M, sum and outputs in registers, and meet in LDS at its end. A segment
-// that is a whole pair writes y; others keep 32 rows of (M, sum, outputs) in
-// slot pair + run (no two segments share one), and k_kv8_combine joins them.
+// wavefronts of a workgroup take a segment's blocks in turn (with two row blocks,
+// pairs of wavefronts, a row block each: both blocks' outputs and operands would
+// not fit the registers of two wavefronts a SIMD), each with its own M, sum and
+// outputs in registers, and meet in LDS at its end. A segment that is a whole
+// pair writes y; others keep (M, sum, outputs) of their rows in slot pair + run
+// (no two segments share one), and k_kv8_combine joins them.
 //
 // A wavefront has no LDS traffic in its loop: K's and V's bytes come in operand
 // order (16-byte loads, whole KiB), widen in registers (exactly: K's codes to fp16,
@@ -38,9 +40,7 @@ using namespace apus;
 namespace {
 
 constexpr int D = kKv8D, ROT = 64, GRP = 8, KEYS = kKv8Keys;
-constexpr int kRows = 32;
-// wavefronts of a workgroup: with two row blocks one a SIMD, for their registers
-template <int NRB> constexpr int kv8_waves() { return NRB == 1 ? 8 : 4; }
+constexpr int kRows = 32, kWaves = 4;
 constexpr float kEps = 1e-6f;
 constexpr float kL2E = 1.44269504088896341f;
 constexpr int QP = D + 8, AP = D + 4;        // LDS pitches of q rows and of outputs
@@ -70,9 +70,22 @@ __device__ __forceinline__ float row_max(float x) {
     x = fmaxf(x, __shfl_xor(x, 16));
     return fmaxf(x, __shfl_xor(x, 32));
 }
-__device__ __forceinline__ float row_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+// over 16 lanes
+__device__ __forceinline__ float sum16(float x) {
+    x += dpp<kXor1>(x);
+    x += dpp<kXor2>(x);
+    x += dpp<kHalfMirror>(x);
+    return x + dpp<kMirror>(x);
+}
+__device__ __forceinline__ float max16(float x) {
+    x = fmaxf(x, dpp<kXor1>(x));
+    x = fmaxf(x, dpp<kXor2>(x));
+    x = fmaxf(x, dpp<kHalfMirror>(x));
+    return fmaxf(x, dpp<kMirror>(x));
 }
 __device__ __forceinline__ float sigmoid(float x) {
     return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-x * kL2E));
@@ -80,142 +93,167 @@ __device__ __forceinline__ float sigmoid(float x) {
 
 typedef const __attribute__((address_space(1))) u32x4 *gu32x4p;
 
-template <int NRB, int N>
-__global__ __launch_bounds__(64 * kv8_waves<NRB>()) void k_kv8_attn(
+// a row's 4 outputs o / l times the gate's sigmoid
+__device__ __forceinline__ uint2 finish(f32x4 o, float l, uint2 gate) {
+    const float inv = 1.0f / l;
+    const float g[4] = {bf2f((uint16_t)gate.x), bf2f((uint16_t)(gate.x >> 16)), bf2f((uint16_t)gate.y),
+                        bf2f((uint16_t)(gate.y >> 16))};
+    uint32_t c[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) c[e] = f2bf(o[e] * inv * sigmoid(g[e]));
+    return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+}
+
+// RB: row blocks, 2 where a sequence has more than two new tokens; their q rows
+// then stay in LDS.
+template <int RB, int N>
+__global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
     Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg, const uint16_t *__restrict__ qn_w,
     const uint16_t *__restrict__ rope, int nkv, int total, int run, float c2, uint16_t *__restrict__ y,
     float *__restrict__ part, float2 *__restrict__ stat) {
-    constexpr int kWaves = kv8_waves<NRB>();
-    __shared__ __attribute__((aligned(16))) uint16_t qs[16 * NRB * QP];
-    __shared__ float qsc[16 * NRB];
+    static_assert(64 * kWaves == D, "a thread a dim, a wavefront's threads 4 q rows");
+    // (with two row blocks the q rows lie where the outputs meet later: two
+    // workgroups a CU)
     __shared__ __attribute__((aligned(16))) float os[kWaves * 16 * AP];
-    __shared__ float2 ml[kWaves][16 * NRB];
+    __shared__ __attribute__((aligned(16))) _Float16 qown[RB == 1 ? 16 * QP : 1];
+    _Float16 *const qs = RB == 1 ? qown : reinterpret_cast<_Float16 *>(os);
+    __shared__ float qsc[16 * RB];
+    __shared__ float ms[kWaves][16 * RB];                  // M, and the sum of each of a row's four lanes
+    __shared__ __attribute__((aligned(16))) float ls[kWaves][16 * RB][4];
     __shared__ int first_nan[D];           // the first key whose v is NaN there, in the blocks not all rows see
-    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int x1 = min(((int)blockIdx.x + 1) * run, total);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x1 = min(((int)blockIdx.x + 1) * run, total), nh = nkv * GRP;
     int nx = 0;
     for (int x = (int)blockIdx.x * run; x < x1; x = nx) {
-        const int s = kv8_seq_of(sq.off, sq.n, x / nkv);
+        // (opaque: or every address of a lane is formed ahead of this loop, and spilled)
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+        const int s = kv8_find(sq.off, sq.n, x / nkv);
         const int nb = sq.off[s + 1] - sq.off[s], local = x - nkv * sq.off[s];
         const int kvh = local / nb, b0 = local % nb, b1 = min(b0 + x1 - x, nb), pair = s * nkv + kvh;
         nx = x + b1 - b0;
         const int t0 = sq.cu[s], tq = sq.cu[s + 1] - t0, p0 = sq.pos0[s], row = sq.row[s];
-        const int nh = nkv * GRP;
+        const int rows = tq * GRP, last = b1 - 1;
 
+        // q rows (token, head): 16 threads a row, thread e the dims 8 c .. and 128 + 8 c ..,
+        // c such that the dims +-32 of a rotary pair are the neighbour's
+        const int qr = tid >> 4, e = tid & 15, c8 = ((e & 8) | (e & 6) >> 1 | (e & 1) << 2) * 8;
+        u16x8 qa[RB], qc[RB], wa, wc, co[RB], si[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            const int t = min(rb * 2 + (qr >> 3), tq - 1);
+            const uint16_t *p = qg + ((size_t)(t0 + t) * nh + kvh * GRP + (qr & 7)) * 2 * D + c8;
+            qa[rb] = *reinterpret_cast<const u16x8 *>(p);
+            qc[rb] = *reinterpret_cast<const u16x8 *>(p + 128);
+            const uint16_t *cs = rope + (size_t)(p0 + t) * ROT + (c8 & 31);
+            co[rb] = *reinterpret_cast<const u16x8 *>(cs);
+            si[rb] = *reinterpret_cast<const u16x8 *>(cs + ROT / 2);
+        }
+        wa = *reinterpret_cast<const u16x8 *>(qn_w + c8);
+        wc = *reinterpret_cast<const u16x8 *>(qn_w + 128 + c8);
+        __builtin_amdgcn_sched_barrier(0);
         // the first block's loads, under the q rows' work
-        const int last = b1 - 1;
         u32x4 kr[8], vr[8];
         float ks = 0.0f, vs = 0.0f, kn = 0.0f, vn = 0.0f;
-        auto at = [&](const uint8_t *base, int b) {
-            return base + ((size_t)kv8_id_u(kv, row, b) * nkv + kvh) * kKv8Bytes;
-        };
-        auto load = [&](u32x4 (&r)[8], const uint8_t *p) {
-            const gu32x4p q = (gu32x4p)(p + lane * 16);
+        const uint32_t lane16 = (uint32_t)lane * 16;
+        auto load = [&](u32x4 (&r)[8], const uint8_t *base, uint32_t id) {
+            // (scalar bases 4 KiB apart, so that one register holds the lane's offset)
+            const uint8_t *const p = base + ((size_t)id * nkv + kvh) * kKv8Bytes;
 #pragma unroll
-            for (int i = 0; i < 8; i++) r[i] = __builtin_nontemporal_load(q + i * 64);
+            for (int i = 0; i < 8; i++)
+                r[i] = __builtin_nontemporal_load((gu32x4p)(p + i / 4 * 4096 + (lane16 + i % 4 * 1024)));
         };
-        auto scales = [&](int b, float &k_, float &v_) {
-            const float *p = kv.scale + ((size_t)kv8_id_u(kv, row, b) * nkv + kvh) * 2;
-            k_ = __int_as_float(sload_i32((const int32_t *)p, 8, 0));
-            v_ = __int_as_float(sload_i32((const int32_t *)p, 8, 1));
+        auto scales = [&](uint32_t id, float &k_, float &v_) {
+            const int32_t *p = (const int32_t *)(kv.scale + ((size_t)id * nkv + kvh) * 2);
+            k_ = __int_as_float(sload_i32(p, 8, 0));
+            v_ = __int_as_float(sload_i32(p, 8, 1));
         };
-        int b = min(b0 + wave, last);
-        load(kr, at(kv.k, b));
-        load(vr, at(kv.v, b));
-        scales(b, ks, vs);
-
-        for (int i = tid; i < D; i += 64 * kWaves) first_nan[i] = 0x7fffffff;
-        // q rows n = (token, head) into LDS: 16 threads a row, dims 8 e .. and 128 + 8 e ..
-        for (int r = tid >> 4; r < 16 * NRB; r += 4 * kWaves) {
-            const int e = tid & 15, t = r >> 3, h = kvh * GRP + (r & 7);
-            u16x8 a = {}, c = {};
-            if (t < tq) {
-                const uint16_t *p = qg + ((size_t)(t0 + t) * nh + h) * 2 * D + e * 8;
-                a = *reinterpret_cast<const u16x8 *>(p);
-                c = *reinterpret_cast<const u16x8 *>(p + 128);
-            }
-            const u16x8 wa = *reinterpret_cast<const u16x8 *>(qn_w + e * 8);
-            const u16x8 wc = *reinterpret_cast<const u16x8 *>(qn_w + 128 + e * 8);
-            const uint16_t *cs = rope + (size_t)(p0 + min(t, tq - 1)) * ROT + (e & 3) * 8;
-            const u16x8 co = *reinterpret_cast<const u16x8 *>(cs);
-            const u16x8 si = *reinterpret_cast<const u16x8 *>(cs + ROT / 2);
+        uint32_t id = kv8_id_u(kv, row, min(b0 + wave, last));
+        uint32_t idn = kv8_id_u(kv, row, min(b0 + wave + kWaves, last));
+        load(kr, kv.k, id);
+        load(vr, kv.v, id);
+        scales(id, ks, vs);
+        __builtin_amdgcn_sched_barrier(0);
+        first_nan[tid] = 0x7fffffff;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
             float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss += bf2f(a[i]) * bf2f(a[i]) + bf2f(c[i]) * bf2f(c[i]);
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) ss += __shfl_xor(ss, d);
-            const float rs = 1.0f / sqrtf(ss / (float)D + kEps);
+            for (int i = 0; i < 8; i++) ss += bf2f(qa[rb][i]) * bf2f(qa[rb][i]) + bf2f(qc[rb][i]) * bf2f(qc[rb][i]);
+            const float rs = 1.0f / sqrtf(sum16(ss) / (float)D + kEps);
             float va[8], vc[8], mx = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float v = bf2f(a[i]) * rs * (1.0f + bf2f(wa[i]));
-                const float w = __shfl_xor(v, 4);          // the dims +-32
-                const float r_ = v * bf2f(co[i]) + (e < 4 ? -w : w) * bf2f(si[i]);
-                va[i] = e < 8 ? r_ : v;
-                vc[i] = bf2f(c[i]) * rs * (1.0f + bf2f(wc[i]));
+                const float v = bf2f(qa[rb][i]) * rs * (1.0f + bf2f(wa[i])), w = dpp<kXor1>(v);
+                const float r = v * bf2f(co[rb][i]) + (e & 1 ? w : -w) * bf2f(si[rb][i]);
+                va[i] = e < 8 ? r : v;
+                vc[i] = bf2f(qc[rb][i]) * rs * (1.0f + bf2f(wc[i]));
                 mx = fmaxf(mx, fmaxf(fabsf(va[i]), fabsf(vc[i])));
             }
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-            const float sc = kv8_row_scale(mx), inv = 1.0f / sc;
+            // (rows past the tokens repeat the last one)
+            const float sc = kv8_row_scale(max16(mx)), inv = 1.0f / sc;
             f16x8 oa, oc;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 oa[i] = (_Float16)(va[i] * inv);
                 oc[i] = (_Float16)(vc[i] * inv);
             }
-            *reinterpret_cast<f16x8 *>(qs + r * QP + e * 8) = oa;
-            *reinterpret_cast<f16x8 *>(qs + r * QP + 128 + e * 8) = oc;
-            if (e == 0) qsc[r] = sc * c2;
+            *reinterpret_cast<f16x8 *>(qs + (rb * 16 + qr) * QP + c8) = oa;
+            *reinterpret_cast<f16x8 *>(qs + (rb * 16 + qr) * QP + 128 + c8) = oc;
+            if (e == 0) qsc[rb * 16 + qr] = sc * c2;
         }
         __syncthreads();
         // k-step (i, u): dims (4 i + g) 16 + 8 u ..
-        f16x8 q[NRB][8];
-        float qf[NRB];                                     // scores' factor, with log2 e / 16
+        auto q_of = [&](int rb, int i) {
+            return *reinterpret_cast<const f16x8 *>(qs + (rb * 16 + n) * QP + (i / 2 * 4 + g) * 16 + i % 2 * 8);
+        };
+        f16x8 q[8];
+        float qf[RB];                                      // scores' factor, with log2 e / 16
 #pragma unroll
-        for (int rb = 0; rb < NRB; rb++) qf[rb] = qsc[rb * 16 + n];
+        for (int rb = 0; rb < RB; rb++) qf[rb] = qsc[rb * 16 + n];
+        if (RB == 1) {
 #pragma unroll
-        for (int rb = 0; rb < NRB; rb++)
+            for (int i = 0; i < 8; i++) q[i] = q_of(0, i);
+        }
+        f32x4 acc[RB][16];
+        float M[RB], l[RB];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                q[rb][i] = *reinterpret_cast<const f16x8 *>(qs + (rb * 16 + n) * QP + (i / 2 * 4 + g) * 16 + i % 2 * 8);
-
-        f32x4 acc[NRB][16];
-        float M[NRB], l[NRB];
-#pragma unroll
-        for (int rb = 0; rb < NRB; rb++) {
+        for (int rb = 0; rb < RB; rb++) {
             M[rb] = -INFINITY;
             l[rb] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[rb][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         for (int j = b0 + wave; j < b1; j += kWaves) {
-            const int next = min(j + kWaves, last);
-            f32x4 S[NRB][2];
+            f32x4 S[RB][2];
 #pragma unroll
-            for (int rb = 0; rb < NRB; rb++) S[rb][0] = S[rb][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int rb = 0; rb < RB; rb++) S[rb][0] = S[rb][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 8; i++) {                  // key half i / 4, dims' chunks 4 (i % 4) ..
-                const f16x8 ka = kv8_f16(kr[i][0], kr[i][1]), kb = kv8_f16(kr[i][2], kr[i][3]);
+            for (int i = 0; i < 8; i++) {                  // dims' chunks 4 (i / 2) .., their first or second 8
+                const u32x4 w0 = kr[i / 2], w1 = kr[4 + i / 2];    // both halves of the keys
+                const f16x8 k0 = kv8_f16(w0[i % 2 * 2], w0[i % 2 * 2 + 1]), k1 = kv8_f16(w1[i % 2 * 2], w1[i % 2 * 2 + 1]);
 #pragma unroll
-                for (int rb = 0; rb < NRB; rb++) {
-                    S[rb][i / 4] = mfma16(ka, q[rb][i % 4 * 2], S[rb][i / 4]);
-                    S[rb][i / 4] = mfma16(kb, q[rb][i % 4 * 2 + 1], S[rb][i / 4]);
+                for (int rb = 0; rb < RB; rb++) {
+                    const f16x8 qi = RB == 1 ? q[i] : q_of(rb, i);
+                    S[rb][0] = mfma16(k0, qi, S[rb][0]);
+                    S[rb][1] = mfma16(k1, qi, S[rb][1]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            load(kr, at(kv.k, next));
-            scales(next, kn, vn);
+            id = idn;
+            if (RB == 1) load(kr, kv.k, id);
+            scales(id, kn, vn);
+            idn = kv8_id_u(kv, row, min(j + 2 * kWaves, last));
             __builtin_amdgcn_sched_barrier(0);
             const bool tail = (j + 1) * KEYS > p0 + 1;     // some row does not see some key
-            uint32_t p[NRB][4];                            // the lane's 8 keys, bf16
+            bf16x8 pb[RB];                                 // the lane's 8 keys
 #pragma unroll
-            for (int rb = 0; rb < NRB; rb++) {
+            for (int rb = 0; rb < RB; rb++) {
                 float t[8];
-                const float f_ = qf[rb] * ks;
+                const float f = qf[rb] * ks;
 #pragma unroll
-                for (int i = 0; i < 8; i++) t[i] = S[rb][i / 4][i % 4] * f_;
+                for (int i = 0; i < 8; i++) t[i] = S[rb][i / 4][i % 4] * f;
                 if (tail) {
                     const int lim = p0 + min(rb * 2 + (n >> 3), tq - 1) - j * KEYS - g * 4;
 #pragma unroll
@@ -226,18 +264,18 @@ __global__ __launch_bounds__(64 * kv8_waves<NRB>()) void k_kv8_attn(
                                        fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
                 if (__any(mx > M[rb] + kSlack)) {          // (always at a row's first keys)
                     const float m = fmaxf(M[rb], row_max(mx));
-                    const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M[rb] - m);
+                    const float d = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M[rb] - m);
                     M[rb] = m;
-                    l[rb] *= f;
+                    l[rb] *= d;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) acc[rb][i] *= f;
+                    for (int i = 0; i < 16; i++) acc[rb][i] *= d;
                 }
                 const float ref = M[rb] == -INFINITY ? 0.0f : M[rb];
 #pragma unroll
                 for (int i = 0; i < 8; i++) t[i] = __builtin_amdgcn_exp2f(t[i] - ref);
                 l[rb] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[rb][i] = pack2(t[2 * i], t[2 * i + 1]);
+                pb[rb] = __builtin_bit_cast(bf16x8, u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]),
+                                                          pack2(t[6], t[7])});
             }
             if (tail) {
                 // keys past the last token: whatever lies there counts as zero
@@ -256,153 +294,166 @@ __global__ __launch_bounds__(64 * kv8_waves<NRB>()) void k_kv8_attn(
                     }
                 if (__any(wild != 0)) {
                     // a NaN reaches the rows that see its key and no other: taken
-                    // out of the product, the first key of each dim kept
+                    // out of the product, the first key of each dim kept (in a loop
+                    // over 8 KiB of os of this wavefront's own: unrolled it took 60 registers)
+                    u32x4 *const mine_ = reinterpret_cast<u32x4 *>(os + (RB > 1 ? 16 * RB * QP / 2 : 0)) + wave * 512 + lane;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const uint32_t bad = kv8_nan_codes(vr[i][w]);
-                            vr[i][w] &= ~bad;
-                            if (bad)
-                                atomicMin(&first_nan[(2 * i + w / 2) * 16 + n],
-                                          j * KEYS + w % 2 * 16 + g * 4 + (__ffs((int)bad) - 1) / 8);
+                    for (int i = 0; i < 8; i++) mine_[i * 64] = vr[i];
+#pragma unroll 1
+                    for (int i = 0; i < 32; i++) {
+                        uint32_t *const c = reinterpret_cast<uint32_t *>(mine_ + i / 4 * 64) + i % 4;
+                        const uint32_t bad = kv8_nan_codes(*c);
+                        if (bad) {
+                            *c &= ~bad;
+                            atomicMin(&first_nan[i / 2 * 16 + n],
+                                      j * KEYS + i % 2 * 16 + g * 4 + (__ffs((int)bad) - 1) / 8);
                         }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) vr[i] = mine_[i * 64];
                 }
+            }
+            if (RB > 1) {                                  // (here: the scores' registers are free)
+                __builtin_amdgcn_sched_barrier(0);
+                load(kr, kv.k, id);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const bf16x8 va = kv8_bf16(vr[i][0], vr[i][1], vs), vb = kv8_bf16(vr[i][2], vr[i][3], vs);
 #pragma unroll
-                for (int rb = 0; rb < NRB; rb++) {
-                    const bf16x8 pb = __builtin_bit_cast(bf16x8, u32x4{p[rb][0], p[rb][1], p[rb][2], p[rb][3]});
-                    acc[rb][2 * i] = mfma16(va, pb, acc[rb][2 * i]);
-                    acc[rb][2 * i + 1] = mfma16(vb, pb, acc[rb][2 * i + 1]);
+                for (int rb = 0; rb < RB; rb++) {
+                    acc[rb][2 * i] = mfma16(va, pb[rb], acc[rb][2 * i]);
+                    acc[rb][2 * i + 1] = mfma16(vb, pb[rb], acc[rb][2 * i + 1]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            load(vr, at(kv.v, next));
+            load(vr, kv.v, id);
             __builtin_amdgcn_sched_barrier(0);
             ks = kn;
             vs = vn;
         }
 
-        // the wavefronts' outputs at a common reference point
-#pragma unroll
-        for (int rb = 0; rb < NRB; rb++) {
-            l[rb] = row_sum(l[rb]);
-            if (g == 0) ml[wave][rb * 16 + n] = make_float2(M[rb], l[rb]);
-        }
+        // the wavefronts that had a block meet, a row block at a time
+        const int used = min(kWaves, b1 - b0);
         const bool whole = b0 == 0 && b1 == nb;
         const size_t slot = (size_t)(pair + (int)blockIdx.x) * kRows;
-        const int rows = tq * GRP;
 #pragma unroll
-        for (int rb = 0; rb < NRB; rb++) {
-            __syncthreads();
+        for (int rb = 0; rb < RB; rb++) {
             if (rb * 16 >= rows) break;
-            float m = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) m = fmaxf(m, ml[w][rb * 16 + n].x);
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M[rb] - m);
-            if (rb * 16 + n < rows) {
+            if (RB > 1) __syncthreads();                   // (q rows, or the block before, are done with)
+            if (wave < used && rb * 16 + n < rows) {
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    *reinterpret_cast<f32x4 *>(os + (wave * 16 + n) * AP + i * 16 + g * 4) = acc[rb][i] * f;
+                    *reinterpret_cast<f32x4 *>(os + (wave * 16 + n) * AP + i * 16 + g * 4) = acc[rb][i];
+                ls[wave][rb * 16 + n][g] = l[rb];
+                if (g == 0) ms[wave][rb * 16 + n] = M[rb];
             }
             __syncthreads();
-            // 64 threads a row, four dims each
-#pragma unroll
-            for (int r = tid >> 6; r < 16; r += kWaves) {
-                const int rr = rb * 16 + r, d = lane * 4;
-                if (rr >= rows) break;
-                float mt = -INFINITY, lt = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) mt = fmaxf(mt, ml[w][rr].x);
+            // a row at a time, four dims a lane
+#pragma unroll 1
+            for (int r = rb * 16 + wave; r < min(rows, rb * 16 + 16); r += kWaves) {
+                const int d = lane * 4;
+                float m = -INFINITY, lt = 0.0f;
+                for (int w = 0; w < used; w++) m = fmaxf(m, ms[w][r]);
                 f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) {
-                    const float2 u = ml[w][rr];
-                    lt += u.x == -INFINITY ? 0.0f : u.y * __builtin_amdgcn_exp2f(u.x - mt);
-                    o += *reinterpret_cast<const f32x4 *>(os + (w * 16 + r) * AP + d);
+                for (int w = 0; w < used; w++) {
+                    const float mw = ms[w][r], f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+                    const f32x4 lw = *reinterpret_cast<const f32x4 *>(ls[w][r]);
+                    lt += ((lw[0] + lw[1]) + (lw[2] + lw[3])) * f;
+                    o += *reinterpret_cast<const f32x4 *>(os + (w * 16 + r % 16) * AP + d) * f;
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (first_nan[d + e] <= p0 + (rr >> 3)) o[e] = NAN;
+                for (int i = 0; i < 4; i++)
+                    if (first_nan[d + i] <= p0 + (r >> 3)) o[i] = NAN;
                 if (whole) {
-                    const size_t at_ = ((size_t)(t0 + (rr >> 3)) * nh + kvh * GRP + (rr & 7));
-                    const uint2 gc = *reinterpret_cast<const uint2 *>(qg + at_ * 2 * D + D + d);
-                    const float inv = 1.0f / lt;
-                    const float o0 = o[0] * inv * sigmoid(bf2f((uint16_t)gc.x)), o1 = o[1] * inv * sigmoid(bf2f((uint16_t)(gc.x >> 16)));
-                    const float o2 = o[2] * inv * sigmoid(bf2f((uint16_t)gc.y)), o3 = o[3] * inv * sigmoid(bf2f((uint16_t)(gc.y >> 16)));
-                    *reinterpret_cast<uint2 *>(y + at_ * D + d) =
-                        make_uint2(f2bf(o0) | (uint32_t)f2bf(o1) << 16, f2bf(o2) | (uint32_t)f2bf(o3) << 16);
+                    const size_t at = (size_t)(t0 + (r >> 3)) * nh + kvh * GRP + (r & 7);
+                    const uint2 gate = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
+                    *reinterpret_cast<uint2 *>(y + at * D + d) = finish(o, lt, gate);
                 } else {
-                    *reinterpret_cast<f32x4 *>(part + (slot + rr) * D + d) = o;
-                    if (lane == 0) stat[slot + rr] = make_float2(mt, lt);
+                    *reinterpret_cast<f32x4 *>(part + (slot + r) * D + d) = o;
+                    if (lane == 0) stat[slot + r] = make_float2(m, lt);
                 }
             }
         }
-        __syncthreads();                                   // (qs, ml and os are the next segment's)
+        if (nx < x1) __syncthreads();                      // (qs and os are the next segment's)
     }
 }
 
-// One workgroup a (token, head) of a pair that lies in several runs: its
-// segments' outputs at a common reference point, every fourth by a wavefront.
-template <int N>
+// SP wavefronts a (token, head) of a pair that lies in several runs, each with
+// its share of the segments, 8 loads at a time.
+template <int SP, int N>
 __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float *__restrict__ part,
                                                      const float2 *__restrict__ stat,
-                                                     const uint16_t *__restrict__ qg, int nkv, int run,
+                                                     const uint16_t *__restrict__ qg, int nkv, int run, int items,
                                                      uint16_t *__restrict__ y) {
-    __shared__ f32x4 os[4][64];
-    const int nh = nkv * GRP, h = blockIdx.x % nh, tt = sq.cu[0] + blockIdx.x / nh;
-    const int s = kv8_seq_of(sq.cu, sq.n, tt), kvh = h / GRP, r = (tt - sq.cu[s]) * GRP + h % GRP;
+    const int lane = threadIdx.x & 63, d = lane * 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave % SP;
+    const int item = min((int)blockIdx.x * (4 / SP) + wave / SP, items - 1);   // (the last again: the same y)
+    const int nh = nkv * GRP, h = item % nh, tt = sq.cu[0] + item / nh;
+    const int s = kv8_find(sq.cu, sq.n, tt), kvh = h / GRP, r = (tt - sq.cu[s]) * GRP + h % GRP;
     const int nb = sq.off[s + 1] - sq.off[s], x = nkv * sq.off[s] + kvh * nb;
     const int w0 = x / run, w1 = (x + nb - 1) / run, pair = s * nkv + kvh;
     if (w0 == w1) return;                                  // (the whole pair: written already)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = lane * 4;
     const size_t at = (size_t)tt * nh + h;
-    const uint2 gc = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
+    const uint2 gate = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
     const size_t slot0 = (size_t)(pair + w0) * kRows + r;
-    float m = -INFINITY;
-    for (int w = lane; w <= w1 - w0; w += 64) m = fmaxf(m, stat[slot0 + (size_t)w * kRows].x);
-#pragma unroll
-    for (int e = 32; e; e >>= 1) m = fmaxf(m, __shfl_xor(m, e));
-    float l = 0.0f;
-    for (int w = lane; w <= w1 - w0; w += 64) {
-        const float2 u = stat[slot0 + (size_t)w * kRows];
-        l += u.x == -INFINITY ? 0.0f : u.y * __builtin_amdgcn_exp2f(u.x - m);
-    }
-#pragma unroll
-    for (int e = 32; e; e >>= 1) l += __shfl_xor(l, e);
+    const int segs = w1 - w0 + 1;
+    float m = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int w = wave; w <= w1 - w0; w += 32) {
+    for (int w = share; w < segs; w += 8 * SP) {
         f32x4 v[8];
-        float f[8];
+        float2 u[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const size_t a = slot0 + (size_t)min(w + 4 * i, w1 - w0) * kRows;
+            const size_t a = slot0 + (size_t)min(w + i * SP, segs - 1) * kRows;
             v[i] = *reinterpret_cast<const f32x4 *>(part + a * D + d);
-            f[i] = stat[a].x;
+            u[i] = stat[a];
         }
+        float mn = m;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (w + 4 * i <= w1 - w0 && f[i] != -INFINITY) o += v[i] * __builtin_amdgcn_exp2f(f[i] - m);
+        for (int i = 0; i < 8; i++) mn = fmaxf(mn, u[i].x);
+        const float k = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= k;
+        o *= k;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (w + i * SP >= segs || u[i].x == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f(u[i].x - m);
+            l += u[i].y * f;
+            o += v[i] * f;
+        }
     }
-    os[wave][lane] = o;
-    __syncthreads();
-    if (wave) return;
-    o = (os[0][lane] + os[1][lane]) + (os[2][lane] + os[3][lane]);
-    const float inv = 1.0f / l;
-    const float o0 = o[0] * inv * sigmoid(bf2f((uint16_t)gc.x)), o1 = o[1] * inv * sigmoid(bf2f((uint16_t)(gc.x >> 16)));
-    const float o2 = o[2] * inv * sigmoid(bf2f((uint16_t)gc.y)), o3 = o[3] * inv * sigmoid(bf2f((uint16_t)(gc.y >> 16)));
-    *reinterpret_cast<uint2 *>(y + at * D + d) =
-        make_uint2(f2bf(o0) | (uint32_t)f2bf(o1) << 16, f2bf(o2) | (uint32_t)f2bf(o3) << 16);
+    if (SP > 1) {
+        __shared__ f32x4 os[4][64];
+        __shared__ float2 st[4];
+        os[wave][lane] = o;
+        if (lane == 0) st[wave] = make_float2(m, l);
+        __syncthreads();
+        if (share) return;
+        float mt = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < SP; i++) mt = fmaxf(mt, st[wave + i].x);
+        l = 0.0f;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < SP; i++) {
+            const float2 u = st[wave + i];
+            if (u.x == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f(u.x - mt);
+            l += u.y * f;
+            o += os[wave + i][lane] * f;
+        }
+    }
+    *reinterpret_cast<uint2 *>(y + at * D + d) = finish(o, l, gate);
 }
 
 // Blocks of a sequence's context.
 int32_t ctx_blocks(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n + KEYS - 1) / KEYS : 0; }
 
 // the most runs of a launch
-size_t max_runs() { return (size_t)cu_count(); }
+size_t max_runs() { return 2 * (size_t)cu_count(); }
 
 }  // namespace
 
@@ -449,27 +500,32 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
         int most = 0;
         for (int s = 0; s < q.n; s++) most = std::max(most, q.cu[s + 1] - q.cu[s]);
         // a block for each wavefront at least
-        const size_t waves = most <= 2 ? kv8_waves<1>() : kv8_waves<2>();
-        const size_t run = std::max((total + max_runs() - 1) / max_runs(), waves);
-        bool split = false;
+        const size_t run = std::max((total + max_runs() - 1) / max_runs(), (size_t)kWaves);
+        size_t segs = 1;                                   // the most of a pair
         for (int s = 0; s < q.n; s++) {
             const size_t nb = (size_t)(q.off[s + 1] - q.off[s]), x = nkv * (size_t)q.off[s];
-            for (size_t h = 0; nb && !split && h < nkv; h++) split = (x + h * nb) / run != (x + (h + 1) * nb - 1) / run;
+            for (size_t h = 0; nb && h < nkv; h++)
+                segs = std::max(segs, (x + (h + 1) * nb - 1) / run - (x + h * nb) / run + 1);
         }
         const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
-        auto launch = [&](auto nrb) {
-            constexpr int NRB = decltype(nrb)::value;
+        auto launch = [&](auto rb) {
             APUS_TIMED("k_kv8_attn",
-                       k_kv8_attn<NRB, N><<<(unsigned)((total + run - 1) / run), 64 * kv8_waves<NRB>(), 0, stream()>>>(
+                       k_kv8_attn<decltype(rb)::value, N><<<(unsigned)((total + run - 1) / run), 64 * kWaves, 0, stream()>>>(
                            q, kv, qg, L->qn_w, w->rope, (int)nkv, (int)total, (int)run, c2, y, w->part, w->stat));
         };
         if (most <= 2) launch(std::integral_constant<int, 1>{});
         else launch(std::integral_constant<int, 2>{});
         if (int e = launch_check("k_kv8_attn")) return e;
-        if (!split) return (int)kOk;
-        APUS_TIMED("k_kv8_combine",
-                   k_kv8_combine<N><<<(unsigned)((size_t)(q.cu[q.n] - q.cu[0]) * L->nh), 256, 0, stream()>>>(
-                       q, w->part, w->stat, qg, (int)nkv, (int)run, y));
+        if (segs == 1) return (int)kOk;
+        const size_t items = (size_t)(q.cu[q.n] - q.cu[0]) * L->nh;
+        auto combine = [&](auto sp) {
+            constexpr int SP = decltype(sp)::value;
+            APUS_TIMED("k_kv8_combine",
+                       k_kv8_combine<SP, N><<<cdiv(items, 4 / SP), 256, 0, stream()>>>(
+                           q, w->part, w->stat, qg, (int)nkv, (int)run, (int)items, y));
+        };
+        if (segs <= 8) combine(std::integral_constant<int, 1>{});
+        else combine(std::integral_constant<int, 4>{});
         return launch_check("k_kv8_combine");
     });
 }

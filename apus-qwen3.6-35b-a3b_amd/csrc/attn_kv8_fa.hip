@@ -75,7 +75,7 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % nkv, item = sq.off[sq.n] - 1 - (int)blockIdx.x / nkv;
-    const int s = kv8_seq_of(sq.off, sq.n, item);
+    const int s = kv8_find(sq.off, sq.n, item);
     const int t0 = sq.cu[s], ns = sq.cu[s + 1] - t0, p0 = sq.pos0[s], row = sq.row[s], nh = nkv * GRP;
     const int f0 = (item - sq.off[s]) * kTok;              // the tile's first token in its sequence
     const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees

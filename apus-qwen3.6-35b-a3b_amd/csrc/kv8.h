@@ -70,13 +70,19 @@ template <int N> struct Kv8SeqsN {
 };
 using Kv8Seqs = Kv8SeqsN<kKv8Seqs>;
 
-template <int N> __host__ __device__ inline int kv8_seq_of(const int32_t (&off)[N], int n, int x) {
-    int lo = 0, hi = n - 1;                  // the largest s with off[s] <= x
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (off[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    return lo;
+// The largest i < n with off[i] <= x (off[0] <= x), for a wave-uniform x: the
+// lanes look at all entries at once, one round of loads (a binary search is a
+// chain of them). Called by whole wavefronts.
+template <int N> __device__ __forceinline__ int kv8_find(const int32_t (&off)[N], int n, int x) {
+    const int lane = threadIdx.x & 63;
+    int32_t v[(N + 63) / 64];
+#pragma unroll
+    for (int c = 0; c < (N + 63) / 64; c++) v[c] = off[min(c * 64 + lane, n - 1)];
+    int k = 0;
+#pragma unroll
+    for (int c = 0; c < (N + 63) / 64; c++)
+        k += __builtin_popcountll(__ballot(v[c] <= x && c * 64 + lane < n));
+    return __builtin_amdgcn_readfirstlane(k) - 1;
 }
 
 // Calls f(seqs, first, blocks) for each launch's share of a batch; count(s) is

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, c
     __shared__ uint32_t red[4];
     const int tid = threadIdx.x, which = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % nkv;
     const int item = (blockIdx.x >> 1) / nkv;
-    const int s = kv8_seq_of(sq.off, sq.n, item);
+    const int s = kv8_find(sq.off, sq.n, item);
     const int p0 = sq.pos0[s], ns = sq.cu[s + 1] - sq.cu[s], b = p0 / KEYS + item - sq.off[s];
     const int lo = max(p0 - b * KEYS, 0), hi = min(p0 + ns - b * KEYS, KEYS);
     const int t0 = sq.cu[s] + b * KEYS - p0;       // the token of the block's first position
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8SeqsN<N> sq, Kv8Ref kv, uin
     __shared__ __attribute__((aligned(16))) uint8_t cs[KEYS * CP];
     const int tid = threadIdx.x, which = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % nkv;
     const int item = (blockIdx.x >> 1) / nkv;
-    const int s = kv8_seq_of(sq.off, sq.n, item);
+    const int s = kv8_find(sq.off, sq.n, item);
     const int p0 = sq.pos0[s], ns = sq.cu[s + 1] - sq.cu[s], b = p0 / KEYS + item - sq.off[s];
     const int lo = max(p0 - b * KEYS, 0), hi = min(p0 + ns - b * KEYS, KEYS);
     const int t0 = sq.cu[s] + b * KEYS - p0;
