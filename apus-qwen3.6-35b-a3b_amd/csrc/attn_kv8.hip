@@ -118,8 +118,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
     __shared__ __attribute__((aligned(16))) _Float16 qown[RB == 1 ? 16 * QP : 1];
     _Float16 *const qs = RB == 1 ? qown : reinterpret_cast<_Float16 *>(os);
     __shared__ float qsc[16 * RB];
-    __shared__ float ms[kWaves][16 * RB];                  // M, and the sum of each of a row's four lanes
-    __shared__ __attribute__((aligned(16))) float ls[kWaves][16 * RB][4];
+    // the wavefronts' M, and the sum of each of a row's four lanes
+    __shared__ __attribute__((aligned(16))) float ms[16 * RB][kWaves], ls[16 * RB][kWaves][4];
     __shared__ int first_nan[D];           // the first key whose v is NaN there, in the blocks not all rows see
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x1 = min(((int)blockIdx.x + 1) * run, total), nh = nkv * GRP;
@@ -129,11 +129,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));
         const int lane = tid & 63, n = lane & 15, g = lane >> 4;
-        const int s = kv8_find(sq.off, sq.n, x / nkv);
-        const int nb = sq.off[s + 1] - sq.off[s], local = x - nkv * sq.off[s];
-        const int kvh = local / nb, b0 = local % nb, b1 = min(b0 + x1 - x, nb), pair = s * nkv + kvh;
-        nx = x + b1 - b0;
-        const int t0 = sq.cu[s], tq = sq.cu[s + 1] - t0, p0 = sq.pos0[s], row = sq.row[s];
+        const Kv8At a = kv8_find<false>(sq, x / nkv);
+        const int t0 = a.t0, tq = a.tokens, p0 = a.p0, row = a.row;
+        const int nbp = a.blocks, nb = (p0 + tq + KEYS - 1) / KEYS, local = x - nkv * a.off;
+        const int kvh = local / nbp, b0 = local % nbp, b1 = min(b0 + x1 - x, nb), pair = a.s * nkv + kvh;
+        nx = min(x1, x + nbp - b0);
+        if (b0 >= nb) continue;                            // (nothing but padding)
         const int rows = tq * GRP, last = b1 - 1;
 
         // q rows (token, head): 16 threads a row, thread e the dims 8 c .. and 128 + 8 c ..,
@@ -156,9 +157,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
         // the first block's loads, under the q rows' work
         u32x4 kr[8], vr[8];
         float ks = 0.0f, vs = 0.0f, kn = 0.0f, vn = 0.0f;
-        const uint32_t lane16 = (uint32_t)lane * 16;
+        // (scalar bases 4 KiB apart, so that one register holds the lane's offset; behind
+        // the last block the loads, which the wait counts want, take a line each)
+        uint32_t lane16 = (uint32_t)lane * 16;
         auto load = [&](u32x4 (&r)[8], const uint8_t *base, uint32_t id) {
-            // (scalar bases 4 KiB apart, so that one register holds the lane's offset)
             const uint8_t *const p = base + ((size_t)id * nkv + kvh) * kKv8Bytes;
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -241,6 +243,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
+            if (j + kWaves >= b1) lane16 = 0;
             id = idn;
             if (RB == 1) load(kr, kv.k, id);
             scales(id, kn, vn);
@@ -334,38 +337,41 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
             vs = vn;
         }
 
-        // the wavefronts that had a block meet, a row block at a time
-        const int used = min(kWaves, b1 - b0);
+        // the wavefronts meet, a row block at a time
         const bool whole = b0 == 0 && b1 == nb;
         const size_t slot = (size_t)(pair + (int)blockIdx.x) * kRows;
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
             if (rb * 16 >= rows) break;
             if (RB > 1) __syncthreads();                   // (q rows, or the block before, are done with)
-            if (wave < used && rb * 16 + n < rows) {
+            if (rb * 16 + n < rows) {
 #pragma unroll
                 for (int i = 0; i < 16; i++)
                     *reinterpret_cast<f32x4 *>(os + (wave * 16 + n) * AP + i * 16 + g * 4) = acc[rb][i];
-                ls[wave][rb * 16 + n][g] = l[rb];
-                if (g == 0) ms[wave][rb * 16 + n] = M[rb];
+                ls[rb * 16 + n][wave][g] = l[rb];
+                if (g == 0) ms[rb * 16 + n][wave] = M[rb];
             }
             __syncthreads();
-            // a row at a time, four dims a lane
-#pragma unroll 1
-            for (int r = rb * 16 + wave; r < min(rows, rb * 16 + 16); r += kWaves) {
-                const int d = lane * 4;
-                float m = -INFINITY, lt = 0.0f;
-                for (int w = 0; w < used; w++) m = fmaxf(m, ms[w][r]);
+            // every fourth row, four dims a lane
+            const int d = lane * 4;
+#pragma unroll
+            for (int i = 0; i < 16 / kWaves; i++) {
+                const int r16 = i * kWaves + wave, r = rb * 16 + r16;
+                if (r >= rows) break;
+                const f32x4 mw = *reinterpret_cast<const f32x4 *>(ms[r]);
+                const float m = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
+                float lt = 0.0f;
                 f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int w = 0; w < used; w++) {
-                    const float mw = ms[w][r], f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
-                    const f32x4 lw = *reinterpret_cast<const f32x4 *>(ls[w][r]);
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) {         // (one without a block has zeros)
+                    const float f = mw[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw[w] - m);
+                    const f32x4 lw = *reinterpret_cast<const f32x4 *>(ls[r][w]);
                     lt += ((lw[0] + lw[1]) + (lw[2] + lw[3])) * f;
-                    o += *reinterpret_cast<const f32x4 *>(os + (w * 16 + r % 16) * AP + d) * f;
+                    o += *reinterpret_cast<const f32x4 *>(os + (w * 16 + r16) * AP + d) * f;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (first_nan[d + i] <= p0 + (r >> 3)) o[i] = NAN;
+                for (int e_ = 0; e_ < 4; e_++)
+                    if (first_nan[d + e_] <= p0 + (r >> 3)) o[e_] = NAN;
                 if (whole) {
                     const size_t at = (size_t)(t0 + (r >> 3)) * nh + kvh * GRP + (r & 7);
                     const uint2 gate = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
@@ -390,10 +396,11 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
     const int lane = threadIdx.x & 63, d = lane * 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave % SP;
     const int item = min((int)blockIdx.x * (4 / SP) + wave / SP, items - 1);   // (the last again: the same y)
-    const int nh = nkv * GRP, h = item % nh, tt = sq.cu[0] + item / nh;
-    const int s = kv8_find(sq.cu, sq.n, tt), kvh = h / GRP, r = (tt - sq.cu[s]) * GRP + h % GRP;
-    const int nb = sq.off[s + 1] - sq.off[s], x = nkv * sq.off[s] + kvh * nb;
-    const int w0 = x / run, w1 = (x + nb - 1) / run, pair = s * nkv + kvh;
+    const int nh = nkv * GRP, h = item % nh, tt = sq.e[0].cu + item / nh;
+    const Kv8At a = kv8_find<true>(sq, tt);
+    const int kvh = h / GRP, r = (tt - a.t0) * GRP + h % GRP;
+    const int nb = (a.p0 + a.tokens + KEYS - 1) / KEYS, x = nkv * a.off + kvh * a.blocks;
+    const int w0 = x / run, w1 = (x + nb - 1) / run, pair = a.s * nkv + kvh;
     if (w0 == w1) return;                                  // (the whole pair: written already)
     const size_t at = (size_t)tt * nh + h;
     const uint2 gate = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
@@ -406,9 +413,9 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
         float2 u[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const size_t a = slot0 + (size_t)min(w + i * SP, segs - 1) * kRows;
-            v[i] = *reinterpret_cast<const f32x4 *>(part + a * D + d);
-            u[i] = stat[a];
+            const size_t sl = slot0 + (size_t)min(w + i * SP, segs - 1) * kRows;
+            v[i] = *reinterpret_cast<const f32x4 *>(part + sl * D + d);
+            u[i] = stat[sl];
         }
         float mn = m;
 #pragma unroll
@@ -419,8 +426,8 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
         o *= k;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (w + i * SP >= segs || u[i].x == -INFINITY) continue;
-            const float f = __builtin_amdgcn_exp2f(u[i].x - m);
+            if (w + i * SP >= segs) continue;
+            const float f = u[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(u[i].x - m);   // (0 keeps a NaN)
             l += u[i].y * f;
             o += v[i] * f;
         }
@@ -440,8 +447,7 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
 #pragma unroll
         for (int i = 0; i < SP; i++) {
             const float2 u = st[wave + i];
-            if (u.x == -INFINITY) continue;
-            const float f = __builtin_amdgcn_exp2f(u.x - mt);
+            const float f = u.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(u.x - mt);
             l += u.y * f;
             o += os[wave + i][lane] * f;
         }
@@ -449,8 +455,11 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
     *reinterpret_cast<uint2 *>(y + at * D + d) = finish(o, l, gate);
 }
 
-// Blocks of a sequence's context.
+// Blocks of a sequence's context, and those that it counts for in the runs: a
+// segment's start and end take as long as a few blocks.
+constexpr int32_t kPad = 8;
 int32_t ctx_blocks(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n + KEYS - 1) / KEYS : 0; }
+int32_t counted_blocks(int32_t pos0, int32_t n) { return n > 0 ? ctx_blocks(pos0, n) + kPad : 0; }
 
 // the most runs of a launch
 size_t max_runs() { return 2 * (size_t)cu_count(); }
@@ -492,20 +501,21 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
     const size_t nkv = L->nkv;
     if (k)
         if (int e = kv8_append_run(kv, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
-    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return ctx_blocks(pos0[s], cu[s + 1] - cu[s]); },
+    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return counted_blocks(pos0[s], cu[s + 1] - cu[s]); },
                         [&](const auto &q) {
-        constexpr int N = sizeof(q.pos0) / 4;
-        const size_t total = (size_t)q.off[q.n] * nkv;
+        constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
+        const size_t total = (size_t)q.e[q.n].off * nkv;
         if (!total) return (int)kOk;
         int most = 0;
-        for (int s = 0; s < q.n; s++) most = std::max(most, q.cu[s + 1] - q.cu[s]);
+        for (int s = 0; s < q.n; s++) most = std::max(most, q.e[s + 1].cu - q.e[s].cu);
         // a block for each wavefront at least
         const size_t run = std::max((total + max_runs() - 1) / max_runs(), (size_t)kWaves);
         size_t segs = 1;                                   // the most of a pair
         for (int s = 0; s < q.n; s++) {
-            const size_t nb = (size_t)(q.off[s + 1] - q.off[s]), x = nkv * (size_t)q.off[s];
-            for (size_t h = 0; nb && h < nkv; h++)
-                segs = std::max(segs, (x + (h + 1) * nb - 1) / run - (x + h * nb) / run + 1);
+            const size_t nb = (size_t)ctx_blocks(q.e[s].pos0, q.e[s + 1].cu - q.e[s].cu);
+            size_t x = nkv * (size_t)q.e[s].off;
+            for (size_t h = 0; nb && h < nkv; h++, x += (size_t)(q.e[s + 1].off - q.e[s].off))
+                segs = std::max(segs, (x + nb - 1) / run - x / run + 1);
         }
         const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
         auto launch = [&](auto rb) {
@@ -517,7 +527,7 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
         else launch(std::integral_constant<int, 2>{});
         if (int e = launch_check("k_kv8_attn")) return e;
         if (segs == 1) return (int)kOk;
-        const size_t items = (size_t)(q.cu[q.n] - q.cu[0]) * L->nh;
+        const size_t items = (size_t)(q.e[q.n].cu - q.e[0].cu) * L->nh;
         auto combine = [&](auto sp) {
             constexpr int SP = decltype(sp)::value;
             APUS_TIMED("k_kv8_combine",
@@ -542,7 +552,7 @@ int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w
             return set_error(kErrUnsupported, "decode takes 0..%d new tokens per sequence (got %d)", kRows / GRP,
                              cu[s + 1] - cu[s]);
         if (s % kKv8Seqs == 0) total = 0;
-        total += (size_t)ctx_blocks(pos0[s], cu[s + 1] - cu[s]) * L->nkv;
+        total += (size_t)counted_blocks(pos0[s], cu[s + 1] - cu[s]) * L->nkv;
         if (total > 0x7ff00000) return set_error(kErrUnsupported, "too many cached keys in one call");
     }
     return kOk;

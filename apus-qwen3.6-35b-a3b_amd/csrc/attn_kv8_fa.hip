@@ -74,10 +74,10 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
     __shared__ int first_nan[D];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x % nkv, item = sq.off[sq.n] - 1 - (int)blockIdx.x / nkv;
-    const int s = kv8_find(sq.off, sq.n, item);
-    const int t0 = sq.cu[s], ns = sq.cu[s + 1] - t0, p0 = sq.pos0[s], row = sq.row[s], nh = nkv * GRP;
-    const int f0 = (item - sq.off[s]) * kTok;              // the tile's first token in its sequence
+    const int kvh = blockIdx.x % nkv, item = ((int)gridDim.x - 1 - (int)blockIdx.x) / nkv;
+    const Kv8At a = kv8_find<false>(sq, item);
+    const int t0 = a.t0, ns = a.tokens, p0 = a.p0, row = a.row, nh = nkv * GRP;
+    const int f0 = (item - a.off) * kTok;                  // the tile's first token in its sequence
     const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees
     const int ctx = p0 + ns, steps = (end + kTile - 1) / kTile;
     if (tid < D) first_nan[tid] = 0x7fffffff;
@@ -284,8 +284,8 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
         if (int e = kv8_append_run(r, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
     return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + kTok - 1) / kTok; },
                         [&](const auto &q) {
-        constexpr int N = sizeof(q.pos0) / 4;
-        const size_t grid = (size_t)q.off[q.n] * nkv;
+        constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
+        const size_t grid = (size_t)q.e[q.n].off * nkv;
         if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
         const float c2 = (float)(1.44269504088896341 / sqrt((double)D));

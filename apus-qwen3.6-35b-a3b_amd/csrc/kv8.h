@@ -62,27 +62,55 @@ __device__ __forceinline__ uint32_t kv8_id_u(const Kv8Ref &r, int h, int b) {
 
 // The sequences of one launch, by value (a captured call keeps them; longer
 // batches take several launches). Few sequences: the short form, whose copy at
-// launch is shorter. off: blocks before each sequence's, in the kernel's count.
+// launch is shorter. Entry i: the blocks (in the kernel's count) and tokens
+// before sequence i, its cached positions and its row; entry n has the totals,
+// entries past it none that is ever found.
 constexpr int kKv8Seqs = 224, kKv8FewSeqs = 8;
-template <int N> struct Kv8SeqsN {
-    int32_t n;
-    int32_t cu[N + 1], pos0[N], off[N + 1], row[N];
+struct Kv8Seq {
+    int32_t off, cu, pos0, row;
 };
-using Kv8Seqs = Kv8SeqsN<kKv8Seqs>;
+template <int N> struct alignas(16) Kv8SeqsN {
+    Kv8Seq e[N + 1];
+    int32_t n;
+};
 
-// The largest i < n with off[i] <= x (off[0] <= x), for a wave-uniform x: the
-// lanes look at all entries at once, one round of loads (a binary search is a
-// chain of them). Called by whole wavefronts.
-template <int N> __device__ __forceinline__ int kv8_find(const int32_t (&off)[N], int n, int x) {
+// A sequence of a launch: its number, entry, and what it has of blocks and tokens.
+struct Kv8At {
+    int s, off, blocks, t0, tokens, p0, row;
+};
+// The last sequence whose off (TOKEN: cu) is at most the wave-uniform x. The lanes
+// look at all entries at once, so everything about it is known after one round
+// of loads (with a binary search and scalar loads it was a chain of four, some
+// 2 us at the start of every workgroup). Called by whole wavefronts.
+template <bool TOKEN, int N> __device__ __forceinline__ Kv8At kv8_find(const Kv8SeqsN<N> &sq, int x) {
+    constexpr int C = (N + 64) / 64;
     const int lane = threadIdx.x & 63;
-    int32_t v[(N + 63) / 64];
-#pragma unroll
-    for (int c = 0; c < (N + 63) / 64; c++) v[c] = off[min(c * 64 + lane, n - 1)];
+    Kv8Seq v[C];
     int k = 0;
 #pragma unroll
-    for (int c = 0; c < (N + 63) / 64; c++)
-        k += __builtin_popcountll(__ballot(v[c] <= x && c * 64 + lane < n));
-    return __builtin_amdgcn_readfirstlane(k) - 1;
+    for (int c = 0; c < C; c++) v[c] = sq.e[min(c * 64 + lane, N)];
+#pragma unroll
+    for (int c = 0; c < C; c++)
+        k += __builtin_popcountll(__ballot((TOKEN ? v[c].cu : v[c].off) <= x && c * 64 + lane <= N));
+    const int s = __builtin_amdgcn_readfirstlane(k) - 1;
+    auto get = [&](auto f, int i) {
+        int r = 0;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+            if (i / 64 == c) r = __builtin_amdgcn_readlane(f(v[c]), i % 64);
+        return r;
+    };
+    auto off = [](const Kv8Seq &q) { return q.off; };
+    auto cu = [](const Kv8Seq &q) { return q.cu; };
+    Kv8At a;
+    a.s = s;
+    a.off = get(off, s);
+    a.blocks = get(off, s + 1) - a.off;
+    a.t0 = get(cu, s);
+    a.tokens = get(cu, s + 1) - a.t0;
+    a.p0 = get([](const Kv8Seq &q) { return q.pos0; }, s);
+    a.row = get([](const Kv8Seq &q) { return q.row; }, s);
+    return a;
 }
 
 // Calls f(seqs, first, blocks) for each launch's share of a batch; count(s) is
@@ -92,16 +120,16 @@ int kv8_launches(size_t B, const int32_t *rows, const int32_t *cu, const int32_t
     for (size_t s0 = 0; s0 < B; s0 += kKv8Seqs) {
         const size_t n = B - s0 < (size_t)kKv8Seqs ? B - s0 : (size_t)kKv8Seqs;
         auto fill = [&](auto &q) {
+            constexpr size_t N = sizeof(q.e) / sizeof(q.e[0]) - 1;
             q.n = (int32_t)n;
-            q.off[0] = 0;
+            int32_t off = 0;
             for (size_t i = 0; i < n; i++) {
                 const size_t s = s0 + i;
-                q.cu[i] = cu[s];
-                q.pos0[i] = pos0[s];
-                q.row[i] = rows ? rows[s] : (int32_t)s;
-                q.off[i + 1] = q.off[i] + count(s);
+                q.e[i] = Kv8Seq{off, cu[s], pos0[s], rows ? rows[s] : (int32_t)s};
+                off += count(s);
             }
-            q.cu[n] = cu[s0 + n];
+            q.e[n] = Kv8Seq{off, cu[s0 + n], 0, 0};
+            for (size_t i = n + 1; i <= N; i++) q.e[i] = Kv8Seq{0x7fffffff, 0x7fffffff, 0, 0};
             return f(q);
         };
         int r;
@@ -109,7 +137,7 @@ int kv8_launches(size_t B, const int32_t *rows, const int32_t *cu, const int32_t
             Kv8SeqsN<kKv8FewSeqs> q;
             r = fill(q);
         } else {
-            Kv8Seqs q;
+            Kv8SeqsN<kKv8Seqs> q;
             r = fill(q);
         }
         if (r) return r;

@@ -78,12 +78,12 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, c
     __shared__ uint32_t red[4];
     const int tid = threadIdx.x, which = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % nkv;
     const int item = (blockIdx.x >> 1) / nkv;
-    const int s = kv8_find(sq.off, sq.n, item);
-    const int p0 = sq.pos0[s], ns = sq.cu[s + 1] - sq.cu[s], b = p0 / KEYS + item - sq.off[s];
+    const Kv8At a = kv8_find<false>(sq, item);
+    const int p0 = a.p0, ns = a.tokens, b = p0 / KEYS + item - a.off;
     const int lo = max(p0 - b * KEYS, 0), hi = min(p0 + ns - b * KEYS, KEYS);
-    const int t0 = sq.cu[s] + b * KEYS - p0;       // the token of the block's first position
-    const uint32_t id = kv8_id(kv, sq.row[s], b);
-    if (kv.btab && (uint32_t)kv.btab[(size_t)sq.row[s] * kv.bstride + b] != id) return;   // a stale entry
+    const int t0 = a.t0 + b * KEYS - p0;       // the token of the block's first position
+    const uint32_t id = kv8_id(kv, a.row, b);
+    if (kv.btab && (uint32_t)kv.btab[(size_t)a.row * kv.bstride + b] != id) return;   // a stale entry
     const size_t hb = (size_t)id * nkv + kvh;
     uint8_t *const blk = (which ? kv.v : kv.k) + hb * kKv8Bytes;
     float *const sc = kv.scale + hb * 2 + which;
@@ -158,9 +158,9 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, c
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const uint32_t a = x[i][e] & 0x7fffu;
-            wild |= a >= 0x7f80u;
-            m = max(m, a >= 0x7f80u ? 0u : a);
+            const uint32_t u = x[i][e] & 0x7fffu;
+            wild |= u >= 0x7f80u;
+            m = max(m, u >= 0x7f80u ? 0u : u);
         }
 #pragma unroll
     for (int d = 32; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
@@ -246,11 +246,11 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8SeqsN<N> sq, Kv8Ref kv, uin
     __shared__ __attribute__((aligned(16))) uint8_t cs[KEYS * CP];
     const int tid = threadIdx.x, which = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % nkv;
     const int item = (blockIdx.x >> 1) / nkv;
-    const int s = kv8_find(sq.off, sq.n, item);
-    const int p0 = sq.pos0[s], ns = sq.cu[s + 1] - sq.cu[s], b = p0 / KEYS + item - sq.off[s];
+    const Kv8At a = kv8_find<false>(sq, item);
+    const int p0 = a.p0, ns = a.tokens, b = p0 / KEYS + item - a.off;
     const int lo = max(p0 - b * KEYS, 0), hi = min(p0 + ns - b * KEYS, KEYS);
-    const int t0 = sq.cu[s] + b * KEYS - p0;
-    const size_t hb = (size_t)kv8_id(kv, sq.row[s], b) * nkv + kvh;
+    const int t0 = a.t0 + b * KEYS - p0;
+    const size_t hb = (size_t)kv8_id(kv, a.row, b) * nkv + kvh;
     const uint8_t *const blk = (which ? kv.v : kv.k) + hb * kKv8Bytes;
     const float scale = kv.scale[hb * 2 + which];
     u32x4 piece[2];
@@ -279,9 +279,9 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8SeqsN<N> sq, Kv8Ref kv, uin
         if (r < lo || r >= hi) continue;
         const u32x2 c = *reinterpret_cast<const u32x2 *>(cs + r * CP + pc * 8);
         const uint32_t c0 = c[0], c1 = c[1];
-        const u32x2 a = from_fp8(c0, scale), d = from_fp8(c1, scale);
+        const u32x2 x = from_fp8(c0, scale), z = from_fp8(c1, scale);
         const size_t t = (size_t)(t0 + r);
-        *reinterpret_cast<u32x4 *>((which ? v + t * ldv : k + t * ldk) + kvh * D + pc * 8) = u32x4{a[0], a[1], d[0], d[1]};
+        *reinterpret_cast<u32x4 *>((which ? v + t * ldv : k + t * ldk) + kvh * D + pc * 8) = u32x4{x[0], x[1], z[0], z[1]};
     }
 }
 
@@ -366,8 +366,8 @@ int kv8_append_run(const Kv8Ref &kv, size_t nkv, size_t B, const int32_t *rows, 
                    const uint16_t *kn_w, const uint16_t *rope) {
     return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return touched(pos0[s], cu[s + 1] - cu[s]); },
                         [&](const auto &q) {
-        constexpr int N = sizeof(q.pos0) / 4;
-        const size_t grid = (size_t)q.off[q.n] * nkv * 2;
+        constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
+        const size_t grid = (size_t)q.e[q.n].off * nkv * 2;
         if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many blocks in one call");
         if (kn_w)
@@ -415,8 +415,8 @@ int apus_hip_kv8_read(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const int
     if (!T) return kOk;
     return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return touched(pos0[s], cu[s + 1] - cu[s]); },
                         [&](const auto &q) {
-        constexpr int N = sizeof(q.pos0) / 4;
-        const size_t grid = (size_t)q.off[q.n] * nkv * 2;
+        constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
+        const size_t grid = (size_t)q.e[q.n].off * nkv * 2;
         if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many blocks in one call");
         APUS_TIMED("k_kv8_read", k_kv8_read<N><<<(unsigned)grid, 256, 0, stream()>>>(q, r, k, ldk, v, ldv, (int)nkv));
