@@ -455,14 +455,40 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
     *reinterpret_cast<uint2 *>(y + at * D + d) = finish(o, l, gate);
 }
 
-// Blocks of a sequence's context, and those that it counts for in the runs: a
-// segment's start and end take as long as a few blocks.
-constexpr int32_t kPad = 8;
 int32_t ctx_blocks(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n + KEYS - 1) / KEYS : 0; }
-int32_t counted_blocks(int32_t pos0, int32_t n) { return n > 0 ? ctx_blocks(pos0, n) + kPad : 0; }
 
-// the most runs of a launch
+// How a call is cut. Two workgroups a CU at most (more runs only add segments: 64
+// sequences at 32768, two a CU 328 us, four 340, eight 355).
+//
+// Short contexts: a pair is a run (the same slot for each, as long as the longest
+// context), with no partial results and no second launch: up to 24 blocks (one
+// sequence at 500: 8.9 us, cut 9.3; at 1500, 47 blocks, 20 and 9.5), or to 96
+// where the pairs alone nearly fill the chip (100 sequences at 1500: 28 and 34).
+// Else a segment counts for kPad blocks more than it has, what its start and end
+// take (128 ragged sequences: 250 us with none, 244 with 8, 241 with 16, 244 with
+// 32; 64 equal ones 330, 330, 332, 335), which also keeps two segments out of one
+// short run. Runs have a block for each wavefront at least, and grow with the
+// total as its root, up to 16, since every run costs the second launch a partial
+// result (one sequence at 60000 with 3 tokens: 31 us with runs of 8, 28 with 15).
+constexpr int32_t kPad = 8, kShort = 24, kShortMany = 96;
 size_t max_runs() { return 2 * (size_t)cu_count(); }
+int32_t whole_pairs(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv) {
+    int32_t longest = 0;
+    size_t pairs = 0;
+    for (size_t s = 0; s < B; s++) {
+        longest = std::max(longest, ctx_blocks(pos0[s], cu[s + 1] - cu[s]));
+        pairs += cu[s + 1] > cu[s] ? nkv : 0;
+    }
+    return longest <= kShort || (longest <= kShortMany && 4 * pairs >= 3 * (size_t)cu_count()) ? longest : 0;
+}
+int32_t counted_blocks(int32_t pos0, int32_t n, int32_t whole) {
+    return n <= 0 ? 0 : whole ? whole : ctx_blocks(pos0, n) + kPad;
+}
+size_t run_blocks(size_t total, int32_t whole) {
+    if (whole) return (size_t)whole;
+    const size_t root = std::min<size_t>(16, (size_t)(sqrt((double)total / 16.0) + 0.5));
+    return std::max({(total + max_runs() - 1) / max_runs(), root, (size_t)kWaves});
+}
 
 }  // namespace
 
@@ -501,15 +527,15 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
     const size_t nkv = L->nkv;
     if (k)
         if (int e = kv8_append_run(kv, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
-    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return counted_blocks(pos0[s], cu[s + 1] - cu[s]); },
+    const int32_t whole = whole_pairs(B, cu, pos0, nkv);
+    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return counted_blocks(pos0[s], cu[s + 1] - cu[s], whole); },
                         [&](const auto &q) {
         constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
         const size_t total = (size_t)q.e[q.n].off * nkv;
         if (!total) return (int)kOk;
         int most = 0;
         for (int s = 0; s < q.n; s++) most = std::max(most, q.e[s + 1].cu - q.e[s].cu);
-        // a block for each wavefront at least
-        const size_t run = std::max((total + max_runs() - 1) / max_runs(), (size_t)kWaves);
+        const size_t run = run_blocks(total, whole);
         size_t segs = 1;                                   // the most of a pair
         for (int s = 0; s < q.n; s++) {
             const size_t nb = (size_t)ctx_blocks(q.e[s].pos0, q.e[s + 1].cu - q.e[s].cu);
@@ -552,7 +578,7 @@ int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w
             return set_error(kErrUnsupported, "decode takes 0..%d new tokens per sequence (got %d)", kRows / GRP,
                              cu[s + 1] - cu[s]);
         if (s % kKv8Seqs == 0) total = 0;
-        total += (size_t)counted_blocks(pos0[s], cu[s + 1] - cu[s]) * L->nkv;
+        total += (size_t)counted_blocks(pos0[s], cu[s + 1] - cu[s], 0) * L->nkv;
         if (total > 0x7ff00000) return set_error(kErrUnsupported, "too many cached keys in one call");
     }
     return kOk;
