@@ -28,9 +28,10 @@ namespace {
 
 constexpr int D = kKv8D, ROT = 64, GRP = 8, KEYS = kKv8Keys;
 constexpr int kTok = 32;                     // tokens of a tile
-constexpr int kTile = 64;                    // keys of a step
+constexpr int kWaves = 8;
+constexpr int kAhead = 2;                    // operands read ahead of their products
 constexpr int KP = D * 2 + 16;               // LDS pitches (bytes): a key's K row, a dim's V row
-constexpr int VP = kTile * 2 + 16;
+constexpr int VP = KEYS * 2 + 16;
 constexpr float kEps = 1e-6f, kL2E = 1.44269504088896341f;
 constexpr float kSlack = 10.0f;              // as in attn_kv8.hip
 
@@ -59,17 +60,17 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-struct Tile {
-    u32x4 k[2], v[2];                        // a thread's pieces of the two blocks
-    float ks[2], vs[2];
+struct Step {
+    u32x4 k, v;                              // a thread's pieces of a block
+    float ks, vs;
 };
 
 template <int N>
-__global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg,
-                                                const uint16_t *__restrict__ qn_w,
-                                                const uint16_t *__restrict__ rope, int nkv, float c2,
-                                                uint16_t *__restrict__ y) {
-    __shared__ __attribute__((aligned(16))) char kl[2][kTile * KP];
+__global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg,
+                                                           const uint16_t *__restrict__ qn_w,
+                                                           const uint16_t *__restrict__ rope, int nkv, float c2,
+                                                           uint16_t *__restrict__ y) {
+    __shared__ __attribute__((aligned(16))) char kl[2][KEYS * KP];
     __shared__ __attribute__((aligned(16))) char vl[2][D * VP];
     __shared__ int first_nan[D];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
@@ -79,51 +80,45 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
     const int t0 = a.t0, ns = a.tokens, p0 = a.p0, row = a.row, nh = nkv * GRP;
     const int f0 = (item - a.off) * kTok;                  // the tile's first token in its sequence
     const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees
-    const int ctx = p0 + ns, steps = (end + kTile - 1) / kTile;
+    const int ctx = p0 + ns, steps = (end + KEYS - 1) / KEYS;
     if (tid < D) first_nan[tid] = 0x7fffffff;
 
-    Tile next;
+    Step next;
+    uint32_t id = kv8_id_u(kv, row, 0);
     auto fetch = [&](int st) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int b = min(st * 2 + u, (ctx - 1) / KEYS);
-            const size_t hb = (size_t)kv8_id_u(kv, row, b) * nkv + kvh;
-            next.k[u] = *reinterpret_cast<const u32x4 *>(kv.k + hb * kKv8Bytes + tid * 16);
-            next.v[u] = *reinterpret_cast<const u32x4 *>(kv.v + hb * kKv8Bytes + tid * 16);
-            const int32_t *sc = (const int32_t *)(kv.scale + hb * 2);
-            next.ks[u] = __int_as_float(sload_i32(sc, 8, 0));
-            next.vs[u] = __int_as_float(sload_i32(sc, 8, 1));
-        }
+        const size_t hb = (size_t)id * nkv + kvh;
+        next.k = *reinterpret_cast<const u32x4 *>(kv.k + hb * kKv8Bytes + tid * 16);
+        next.v = *reinterpret_cast<const u32x4 *>(kv.v + hb * kKv8Bytes + tid * 16);
+        const int32_t *sc = (const int32_t *)(kv.scale + hb * 2);
+        next.ks = __int_as_float(sload_i32(sc, 8, 0));
+        next.vs = __int_as_float(sload_i32(sc, 8, 1));
+        id = kv8_id_u(kv, row, min(st + 1, steps - 1));
     };
     // a thread's pieces (kv8.h) to their places in LDS
     auto put = [&](int st, int buf) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int key = u * KEYS + tid / 256 * 16 + tid % 16, c = tid / 16 % 16;
-            char *const kd = kl[buf] + key * KP + c * 32;
-            *reinterpret_cast<f16x8 *>(kd) = kv8_f16(next.k[u][0], next.k[u][1]);
-            *reinterpret_cast<f16x8 *>(kd + 16) = kv8_f16(next.k[u][2], next.k[u][3]);
-            const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16;
-            u32x4 c4 = next.v[u];
-            const int k0_ = (st * 2 + u) * KEYS + g * 4;   // the piece's keys: k0_ .. + 3 and 16 on
-            if (k0_ + 19 >= p0 + f0) {                     // some row does not see some of them
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int left = ctx - (k0_ + w % 2 * 16);      // past the last token: zero
-                    c4[w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
-                    const uint32_t bad = kv8_nan_codes(c4[w]);
-                    if (bad) {                             // out of the product, its first key kept
-                        c4[w] &= ~bad;
-                        atomicMin(&first_nan[d + w / 2 * 16], k0_ + w % 2 * 16 + (__ffs((int)bad) - 1) / 8);
-                    }
-                }
-            }
+        char *const kd = kl[buf] + (tid / 256 * 16 + tid % 16) * KP + tid / 16 % 16 * 32;
+        *reinterpret_cast<f16x8 *>(kd) = kv8_f16(next.k[0], next.k[1]);
+        *reinterpret_cast<f16x8 *>(kd + 16) = kv8_f16(next.k[2], next.k[3]);
+        const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16;
+        u32x4 c4 = next.v;
+        const int k0 = st * KEYS + g * 4;                  // the piece's keys: k0 .. + 3 and 16 on
+        if ((st + 1) * KEYS > p0 + f0) {                   // some row does not see some key
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                // four keys from 4 G: half G % 2, step G / 4, its first or second four
-                const int G = g + w % 2 * 4, at = u * 64 + (G / 4 * 2 + G % 2) * 16 + G / 2 % 2 * 8;
-                *reinterpret_cast<u32x2 *>(vl[buf] + (d + w / 2 * 16) * VP + at) = widen4(c4[w], next.vs[u]);
+                const int left = ctx - (k0 + w % 2 * 16);  // past the last token: zero
+                c4[w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+                const uint32_t bad = kv8_nan_codes(c4[w]);
+                if (bad) {                                 // out of the product, its first key kept
+                    c4[w] &= ~bad;
+                    atomicMin(&first_nan[d + w / 2 * 16], k0 + w % 2 * 16 + (__ffs((int)bad) - 1) / 8);
+                }
             }
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            // four keys from 4 G: half G % 2, step G / 4, its first or second four
+            const int G = g + w % 2 * 4, at = (G / 4 * 2 + G % 2) * 16 + G / 2 % 2 * 8;
+            *reinterpret_cast<u32x2 *>(vl[buf] + (d + w / 2 * 16) * VP + at) = widen4(c4[w], next.vs);
         }
     };
     fetch(0);
@@ -158,8 +153,8 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
             const u16x8 si = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + ROT / 2 + p);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float b = bf2f(x[j][e]) * rs * (1.0f + bf2f(wj[e]));
-                o[e] = o[e] * bf2f(co[e]) + (i < 2 ? -b : b) * bf2f(si[e]);
+                const float z = bf2f(x[j][e]) * rs * (1.0f + bf2f(wj[e]));
+                o[e] = o[e] * bf2f(co[e]) + (i < 2 ? -z : z) * bf2f(si[e]);
             }
         };
         float mx = 0.0f, o[8];
@@ -190,21 +185,30 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
     float M = -INFINITY, l = 0.0f;
     const int wfirst = p0 + min(f0 + wave * 4, ns - 1), wlast = p0 + min(f0 + wave * 4 + 3, ns - 1);
     for (int st = 0; st < steps; st++) {
-        const int buf = st & 1;
-        const float cs[2] = {next.ks[0], next.ks[1]};
+        const int buf = st & 1, k0 = st * KEYS;
+        const float cs = next.ks;
         fetch(min(st + 1, steps - 1));
         __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int k0 = st * kTile + u * KEYS;
-            if (k0 > wlast) break;                         // (wave-uniform)
+        if (k0 <= wlast) {                                 // (wave-uniform)
             f32x16 S;
 #pragma unroll
             for (int e = 0; e < 16; e++) S[e] = 0.0f;
-            const char *kp = kl[buf] + (u * KEYS + n) * KP + hf * 16;
+            const char *kp = kl[buf] + n * KP + hf * 16, *vp = vl[buf] + n * VP + hf * 16;
+            auto k_of = [&](int i) { return *reinterpret_cast<const f16x8 *>(kp + i * 32); };
+            auto v_of = [&](int i) { return *reinterpret_cast<const bf16x8 *>(vp + i % 8 * 32 * VP + i / 8 * 32); };
+            f16x8 kf[kAhead];
 #pragma unroll
-            for (int i = 0; i < 16; i++) S = mfma32(*reinterpret_cast<const f16x8 *>(kp + i * 32), q[i], S);
-            S *= qf * cs[u];
+            for (int i = 0; i < kAhead; i++) kf[i] = k_of(i);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                S = mfma32(kf[i % kAhead], q[i], S);
+                if (i + kAhead < 16) kf[i % kAhead] = k_of(i + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            bf16x8 vf[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) vf[i] = v_of(i);
+            const float sf = qf * cs;
             if (k0 + KEYS > wfirst + 1) {
                 const int lim = pos - k0 - 4 * hf;
 #pragma unroll
@@ -214,6 +218,7 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
             float mx = S[0];
 #pragma unroll
             for (int e = 1; e < 16; e++) mx = fmaxf(mx, S[e]);
+            mx *= sf;
             if (__any(mx > M + kSlack)) {
                 const float m = fmaxf(M, fmaxf(mx, __shfl_xor(mx, 32)));
                 const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - m);
@@ -226,17 +231,20 @@ __global__ __launch_bounds__(512) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const
             uint32_t p[8];
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const float a = __builtin_amdgcn_exp2f(S[e] - ref), b = __builtin_amdgcn_exp2f(S[e + 1] - ref);
-                l += a + b;
-                p[e / 2] = pack2(a, b);
+                const float x0 = __builtin_amdgcn_exp2f(fmaf(S[e], sf, -ref)), x1 = __builtin_amdgcn_exp2f(fmaf(S[e + 1], sf, -ref));
+                l += x0 + x1;
+                p[e / 2] = pack2(x0, x1);
             }
-            const char *vp = vl[buf] + n * VP + u * 64 + hf * 16;
+            bf16x8 pb[2];
 #pragma unroll
-            for (int a = 0; a < 2; a++) {
-                const bf16x8 pb = __builtin_bit_cast(bf16x8, u32x4{p[4 * a], p[4 * a + 1], p[4 * a + 2], p[4 * a + 3]});
+            for (int i = 0; i < 2; i++)
+                pb[i] = __builtin_bit_cast(bf16x8, u32x4{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]});
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    acc[i] = mfma32(*reinterpret_cast<const bf16x8 *>(vp + i * 32 * VP + a * 32), pb, acc[i]);
+            for (int i = 0; i < 16; i++) {
+                acc[i % 8] = mfma32(vf[i % kAhead], pb[i / 8], acc[i % 8]);
+                if (i + kAhead < 16) vf[i % kAhead] = v_of(i + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (st + 1 < steps) put(st + 1, buf ^ 1);
@@ -289,7 +297,7 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
         if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
         const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
-        APUS_TIMED("k_kv8_fa", k_kv8_fa<N><<<(unsigned)grid, 512, 0, stream()>>>(q, r, qg, L->qn_w, w->rope, (int)nkv,
+        APUS_TIMED("k_kv8_fa", k_kv8_fa<N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(q, r, qg, L->qn_w, w->rope, (int)nkv,
                                                                                  c2, y));
         return launch_check("k_kv8_fa");
     });
