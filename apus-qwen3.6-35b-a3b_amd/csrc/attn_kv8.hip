@@ -88,7 +88,7 @@ __device__ __forceinline__ float max16(float x) {
     return fmaxf(x, dpp<kMirror>(x));
 }
 __device__ __forceinline__ float sigmoid(float x) {
-    return 1.0f / (1.0f + __builtin_amdgcn_exp2f(-x * kL2E));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kL2E));
 }
 
 typedef const __attribute__((address_space(1))) u32x4 *gu32x4p;
@@ -98,10 +98,9 @@ __device__ __forceinline__ uint2 finish(f32x4 o, float l, uint2 gate) {
     const float inv = 1.0f / l;
     const float g[4] = {bf2f((uint16_t)gate.x), bf2f((uint16_t)(gate.x >> 16)), bf2f((uint16_t)gate.y),
                         bf2f((uint16_t)(gate.y >> 16))};
-    uint32_t c[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) c[e] = f2bf(o[e] * inv * sigmoid(g[e]));
-    return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    for (int e = 0; e < 4; e++) o[e] *= inv * sigmoid(g[e]);
+    return make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
 }
 
 // RB: row blocks, 2 where a sequence has more than two new tokens; their q rows

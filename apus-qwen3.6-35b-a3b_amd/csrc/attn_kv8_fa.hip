@@ -53,6 +53,17 @@ __device__ __forceinline__ u32x2 widen4(uint32_t a, float s) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
 }
+// over the two lanes of a row, 32 apart
+template <class F> __device__ __forceinline__ float pair32(float x, F f) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max32(float x) {
+    return pair32(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum32(float x) {
+    return pair32(x, [](float a, float b) { return a + b; });
+}
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -60,10 +71,15 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+typedef const __attribute__((address_space(1))) u32x4 *gu32x4p;
+
 struct Step {
     u32x4 k, v;                              // a thread's pieces of a block
-    float ks, vs;
+    f32x2 sc;                                // its scales, K's and V's
 };
+__device__ __forceinline__ float uni(float x) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+}
 
 template <int N>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg,
@@ -72,7 +88,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                                                            uint16_t *__restrict__ y) {
     __shared__ __attribute__((aligned(16))) char kl[2][KEYS * KP];
     __shared__ __attribute__((aligned(16))) char vl[2][D * VP];
-    __shared__ int first_nan[D];
+    __shared__ int first_nan[D], any_nan;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % nkv, item = ((int)gridDim.x - 1 - (int)blockIdx.x) / nkv;
@@ -82,20 +98,30 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees
     const int ctx = p0 + ns, steps = (end + KEYS - 1) / KEYS;
     if (tid < D) first_nan[tid] = 0x7fffffff;
+    if (tid == 0) any_nan = 0;
 
     Step next;
-    uint32_t id = kv8_id_u(kv, row, 0);
+    // Block ids and scales by vector loads (of a zero offset that the compiler does
+    // not know): scalar loads count where LDS reads do, and out of order, so that
+    // every wait for an LDS operand would be one for them too.
+    uint32_t zero = 0;
+    asm volatile("" : "+v"(zero));
+    const uint32_t tid16 = (uint32_t)tid * 16;
+    auto id_of = [&](int b) {
+        const size_t at = (size_t)row * kv.bstride + b;
+        return kv.btab ? *(const __attribute__((address_space(1))) uint32_t *)((const char *)(kv.btab + at) + zero) : (uint32_t)at;
+    };
+    uint32_t id = id_of(0);
     auto fetch = [&](int st) {
-        const size_t hb = (size_t)id * nkv + kvh;
-        next.k = *reinterpret_cast<const u32x4 *>(kv.k + hb * kKv8Bytes + tid * 16);
-        next.v = *reinterpret_cast<const u32x4 *>(kv.v + hb * kKv8Bytes + tid * 16);
-        const int32_t *sc = (const int32_t *)(kv.scale + hb * 2);
-        next.ks = __int_as_float(sload_i32(sc, 8, 0));
-        next.vs = __int_as_float(sload_i32(sc, 8, 1));
-        id = kv8_id_u(kv, row, min(st + 1, steps - 1));
+        const size_t hb = (size_t)min((uint32_t)__builtin_amdgcn_readfirstlane(id), kv.blocks - 1) * nkv + kvh;
+        next.k = *(gu32x4p)(kv.k + hb * kKv8Bytes + tid16);
+        next.v = *(gu32x4p)(kv.v + hb * kKv8Bytes + tid16);
+        next.sc = *(const __attribute__((address_space(1))) f32x2 *)((const char *)(kv.scale + hb * 2) + zero);
+        id = id_of(min(st + 1, steps - 1));
     };
     // a thread's pieces (kv8.h) to their places in LDS
     auto put = [&](int st, int buf) {
+        const float vs = uni(next.sc[1]);
         char *const kd = kl[buf] + (tid / 256 * 16 + tid % 16) * KP + tid / 16 % 16 * 32;
         *reinterpret_cast<f16x8 *>(kd) = kv8_f16(next.k[0], next.k[1]);
         *reinterpret_cast<f16x8 *>(kd + 16) = kv8_f16(next.k[2], next.k[3]);
@@ -110,6 +136,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                 const uint32_t bad = kv8_nan_codes(c4[w]);
                 if (bad) {                                 // out of the product, its first key kept
                     c4[w] &= ~bad;
+                    any_nan = 1;
                     atomicMin(&first_nan[d + w / 2 * 16], k0 + w % 2 * 16 + (__ffs((int)bad) - 1) / 8);
                 }
             }
@@ -118,7 +145,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
         for (int w = 0; w < 4; w++) {
             // four keys from 4 G: half G % 2, step G / 4, its first or second four
             const int G = g + w % 2 * 4, at = (G / 4 * 2 + G % 2) * 16 + G / 2 % 2 * 8;
-            *reinterpret_cast<u32x2 *>(vl[buf] + (d + w / 2 * 16) * VP + at) = widen4(c4[w], next.vs);
+            *reinterpret_cast<u32x2 *>(vl[buf] + (d + w / 2 * 16) * VP + at) = widen4(c4[w], vs);
         }
     };
     fetch(0);
@@ -130,52 +157,62 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     float qf;                                              // scores' factor, with log2 e / 16
     {
         const uint16_t *qr = qg + ((size_t)(t0 + min(tok, ns - 1)) * nh + h) * 2 * D + hf * 8;
-        u16x8 x[16];
+        // (every load at once: the outputs' registers are free yet)
+        u16x8 x[16], w[16], co[2], si[2];
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = *reinterpret_cast<const u16x8 *>(qr + i * 16);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            co[i] = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + i * 16 + hf * 8);
+            si[i] = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + ROT / 2 + i * 16 + hf * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = *reinterpret_cast<const u16x8 *>(qn_w + i * 16 + hf * 8);
+        __builtin_amdgcn_sched_barrier(0);
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) ss += bf2f(x[i][e]) * bf2f(x[i][e]);
-        ss += __shfl_xor(ss, 32);
+        ss = sum32(ss);
         const float rs = 1.0f / sqrtf(ss / (float)D + kEps);
-        // formed twice: for the largest magnitude, then for the fp16 rows (the
-        // fp32 rows would take another 64 registers)
-        auto form = [&](int i, float (&o)[8]) {            // chunk i, after norm and RoPE
-            const u16x8 w = *reinterpret_cast<const u16x8 *>(qn_w + i * 16 + hf * 8);
+        float o[16][8], mq = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = bf2f(x[i][e]) * rs * (1.0f + bf2f(w[e]));
-            if (i >= 4) return;
-            const int j = i ^ 2, p = (i & 1) * 16 + hf * 8;    // the chunk 32 dims away
-            const u16x8 wj = *reinterpret_cast<const u16x8 *>(qn_w + j * 16 + hf * 8);
-            const u16x8 co = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + p);
-            const u16x8 si = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + ROT / 2 + p);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float z = bf2f(x[j][e]) * rs * (1.0f + bf2f(wj[e]));
-                o[e] = o[e] * bf2f(co[e]) + (i < 2 ? -z : z) * bf2f(si[e]);
-            }
-        };
-        float mx = 0.0f, o[8];
+        for (int i = 0; i < 16; i++) {                     // (or their fp32 values are kept from the sum)
+            u32x4 t = __builtin_bit_cast(u32x4, x[i]);
+            asm volatile("" : "+v"(t));
+            x[i] = __builtin_bit_cast(u16x8, t);
+        }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            form(i, o);
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(o[e]));
+            for (int e = 0; e < 8; e++) o[i][e] = bf2f(x[i][e]) * rs * (1.0f + bf2f(w[i][e]));
+            __builtin_amdgcn_sched_barrier(0);
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float sc = kv8_row_scale(mx), inv = 1.0f / sc;
+#pragma unroll
+        for (int i = 0; i < 2; i++)                        // RoPE: with the chunk 32 dims on
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float u = o[i][e], v = o[i + 2][e], c = bf2f(co[i][e]), s_ = bf2f(si[i][e]);
+                o[i][e] = u * c - v * s_;
+                o[i + 2][e] = v * c + u * s_;
+            }
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) mq = fmaxf(mq, fabsf(o[i][e]));
+        mq = max32(mq);
+        const float sc = kv8_row_scale(mq), inv = 1.0f / sc;
         qf = sc * c2;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            form(i, o);
 #pragma unroll
-            for (int e = 0; e < 8; e++) q[i][e] = (_Float16)(o[e] * inv);
+            for (int e = 0; e < 8; e++) q[i][e] = (_Float16)(o[i][e] * inv);
         }
     }
     __syncthreads();                                       // (first_nan is clear)
     put(0, 0);
+    float cs = uni(next.sc[0]);                            // the step's scale of K
 
     f32x16 acc[8];
 #pragma unroll
@@ -186,7 +223,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     const int wfirst = p0 + min(f0 + wave * 4, ns - 1), wlast = p0 + min(f0 + wave * 4 + 3, ns - 1);
     for (int st = 0; st < steps; st++) {
         const int buf = st & 1, k0 = st * KEYS;
-        const float cs = next.ks;
         fetch(min(st + 1, steps - 1));
         __syncthreads();
         if (k0 <= wlast) {                                 // (wave-uniform)
@@ -210,7 +246,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
             for (int i = 0; i < kAhead; i++) vf[i] = v_of(i);
             const float sf = qf * cs;
             if (k0 + KEYS > wfirst + 1) {
-                const int lim = pos - k0 - 4 * hf;
+                int tl = threadIdx.x;
+                asm volatile("" : "+v"(tl));
+                const int lim = p0 + min(f0 + wave * 4 + ((tl & 31) >> 3), ns - 1) - k0 - 4 * ((tl >> 5) & 1);
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (8 * (e / 4) + e % 4 > lim) S[e] = -INFINITY;
@@ -220,7 +258,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
             for (int e = 1; e < 16; e++) mx = fmaxf(mx, S[e]);
             mx *= sf;
             if (__any(mx > M + kSlack)) {
-                const float m = fmaxf(M, fmaxf(mx, __shfl_xor(mx, 32)));
+                const float m = fmaxf(M, max32(mx));
                 const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - m);
                 M = m;
                 l *= f;
@@ -247,31 +285,45 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (st + 1 < steps) put(st + 1, buf ^ 1);
+        if (st + 1 < steps) {
+            put(st + 1, buf ^ 1);
+            cs = uni(next.sc[0]);
+        }
     }
     __syncthreads();                                       // (first_nan is whole)
-    l += __shfl_xor(l, 32);
-    if (tok >= ns) return;
+    l = sum32(l);
+    // (formed again: kept, they took registers from the loop)
+    int tl = threadIdx.x;
+    asm volatile("" : "+v"(tl));
+    const int hf_ = (tl >> 5) & 1, tok_ = f0 + wave * 4 + ((tl & 31) >> 3), pos_ = p0 + tok_;
+    if (tok_ >= ns) return;
     const float inv = 1.0f / l;
-    const size_t at = (size_t)(t0 + tok) * nh + h;
+    const size_t at = (size_t)(t0 + tok_) * nh + kvh * GRP + (tl & 7);
     const uint16_t *gate = qg + at * 2 * D + D;
+    if (any_nan) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (first_nan[32 * i + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) acc[i][e] = NAN;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        uint2 gc[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) gc[c] = *reinterpret_cast<const uint2 *>(gate + 32 * i + 8 * c + 4 * hf_);
 #pragma unroll
         for (int c = 0; c < 4; c++) {                      // dims 32 i + 8 c + 4 hf ..
-            const int d = 32 * i + 8 * c + 4 * hf;
-            const uint2 gc = *reinterpret_cast<const uint2 *>(gate + d);
-            const uint32_t gw[2] = {gc.x, gc.y};
-            uint32_t o[2] = {0, 0};
+            const int d = 32 * i + 8 * c + 4 * hf_;
+            float v[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float gv = bf2f((uint16_t)(gw[e / 2] >> (16 * (e % 2))));
-                float v = acc[i][4 * c + e] * inv / (1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
-                if (first_nan[d + e] <= pos) v = NAN;
-                o[e / 2] |= (uint32_t)f2bf(v) << (16 * (e % 2));
+                const float gv = bf2f((uint16_t)((e < 2 ? gc[c].x : gc[c].y) >> (16 * (e % 2))));
+                v[e] = acc[i][4 * c + e] * inv * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
             }
-            *reinterpret_cast<uint2 *>(y + at * D + d) = make_uint2(o[0], o[1]);
+            *reinterpret_cast<uint2 *>(y + at * D + d) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
         }
+    }
 }
 
 }  // namespace
