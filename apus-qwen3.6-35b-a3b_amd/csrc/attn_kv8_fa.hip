@@ -1,10 +1,10 @@
 // attn_kv8_fa.hip -- gated-GQA attention of any number of new tokens a sequence
 // over the 8-bit KV cache (kv8.h), the formula of attn_kv8.hip.
 //
-// One workgroup a (tile of 32 tokens, kv head), the longest contexts first: the
+// One workgroup a (tile of 32 or 16 tokens, kv head), the last tiles first: the
 // 8 q heads times 32 tokens are 256 rows, 32 a wavefront, whose q and outputs
-// stay in registers. The keys are walked once, 64 (two blocks) at a time, with a
-// running reference point M and sum of the softmax: a tile's codes go from
+// stay in registers. The keys are walked once, a block at a time, with a running
+// reference point M and sum of the softmax: a tile's codes go from
 // memory to registers while the tile before is worked on, widen there (exactly: K's
 // codes to fp16, V's times their scale to bf16) and come into LDS in operand order. The
 // products run on the 32x32x16 MFMA with keys (or dims) on the M side:
@@ -16,6 +16,8 @@
 #include <string.h>
 
 #include <algorithm>
+#include <functional>
+#include <vector>
 
 #include "apus_dev.h"
 #include "apus_host.h"
@@ -27,7 +29,6 @@ using namespace apus;
 namespace {
 
 constexpr int D = kKv8D, ROT = 64, GRP = 8, KEYS = kKv8Keys;
-constexpr int kTok = 32;                     // tokens of a tile
 constexpr int kWaves = 8;
 constexpr int kAhead = 2;                    // operands read ahead of their products
 constexpr int KP = D * 2 + 16;               // LDS pitches (bytes): a key's K row, a dim's V row
@@ -81,26 +82,34 @@ __device__ __forceinline__ float uni(float x) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
 }
 
-template <int N>
+// KS 1: the 8 wavefronts have 32 rows each, of 32 tokens. KS 2: 16 tokens, and
+// wavefronts w and w + 4 have the same rows, the even and the odd blocks of the
+// keys, and join what they have at the end: half the chain of steps, for calls
+// whose longest tile would take longer than their work spread over the chip.
+template <int KS, int N>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg,
                                                            const uint16_t *__restrict__ qn_w,
                                                            const uint16_t *__restrict__ rope, int nkv, float c2,
                                                            uint16_t *__restrict__ y) {
-    __shared__ __attribute__((aligned(16))) char kl[2][KEYS * KP];
-    __shared__ __attribute__((aligned(16))) char vl[2][D * VP];
+    constexpr int kKl = KEYS * KP, kVl = D * VP, kRowBlocks = kWaves / KS, kTok = 4 * kRowBlocks;
+    // two buffers of KS blocks' K and V; then outputs that meet: 64 registers of 8 wavefronts
+    __shared__ __attribute__((aligned(16))) char lds[2 * KS * (kKl + kVl)];
+    static_assert(KS == 1 || 2 * KS * (kKl + kVl) >= kWaves * 64 * (64 * 4 + 8), "");
+    auto kl = [&](int buf, int u) { return lds + (buf * KS + u) * kKl; };
+    auto vl = [&](int buf, int u) { return lds + 2 * KS * kKl + (buf * KS + u) * kVl; };
     __shared__ int first_nan[D], any_nan;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, hf = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rblk = wave % kRowBlocks, kg = wave / kRowBlocks;
     const int kvh = blockIdx.x % nkv, item = ((int)gridDim.x - 1 - (int)blockIdx.x) / nkv;
     const Kv8At a = kv8_find<false>(sq, item);
     const int t0 = a.t0, ns = a.tokens, p0 = a.p0, row = a.row, nh = nkv * GRP;
     const int f0 = (item - a.off) * kTok;                  // the tile's first token in its sequence
     const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees
-    const int ctx = p0 + ns, steps = (end + KEYS - 1) / KEYS;
+    const int ctx = p0 + ns, nb = (end + KEYS - 1) / KEYS, steps = (nb + KS - 1) / KS;
     if (tid < D) first_nan[tid] = 0x7fffffff;
     if (tid == 0) any_nan = 0;
 
-    Step next;
+    Step next;                                             // (one block at a time: KS 2 brings its second after the scores)
     // Block ids and scales by vector loads (of a zero offset that the compiler does
     // not know): scalar loads count where LDS reads do, and out of order, so that
     // every wait for an LDS operand would be one for them too.
@@ -111,47 +120,50 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
         const size_t at = (size_t)row * kv.bstride + b;
         return kv.btab ? *(const __attribute__((address_space(1))) uint32_t *)((const char *)(kv.btab + at) + zero) : (uint32_t)at;
     };
-    uint32_t id = id_of(0);
-    auto fetch = [&](int st) {
-        const size_t hb = (size_t)min((uint32_t)__builtin_amdgcn_readfirstlane(id), kv.blocks - 1) * nkv + kvh;
+    uint32_t id[KS];
+#pragma unroll
+    for (int u = 0; u < KS; u++) id[u] = id_of(min(u, nb - 1));
+    auto fetch = [&](int st, int u) {
+        const size_t hb = (size_t)min((uint32_t)__builtin_amdgcn_readfirstlane(id[u]), kv.blocks - 1) * nkv + kvh;
         next.k = *(gu32x4p)(kv.k + hb * kKv8Bytes + tid16);
         next.v = *(gu32x4p)(kv.v + hb * kKv8Bytes + tid16);
         next.sc = *(const __attribute__((address_space(1))) f32x2 *)((const char *)(kv.scale + hb * 2) + zero);
-        id = id_of(min(st + 1, steps - 1));
+        id[u] = id_of(min((st + 1) * KS + u, nb - 1));
     };
     // a thread's pieces (kv8.h) to their places in LDS
-    auto put = [&](int st, int buf) {
+    float cs = 0.0f;                                       // the scale of this wavefront's K
+    auto put = [&](int st, int u, int buf) {
         const float vs = uni(next.sc[1]);
-        char *const kd = kl[buf] + (tid / 256 * 16 + tid % 16) * KP + tid / 16 % 16 * 32;
+        char *const kd = kl(buf, u) + (tid / 256 * 16 + tid % 16) * KP + tid / 16 % 16 * 32;
         *reinterpret_cast<f16x8 *>(kd) = kv8_f16(next.k[0], next.k[1]);
         *reinterpret_cast<f16x8 *>(kd + 16) = kv8_f16(next.k[2], next.k[3]);
-        const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16;
+        const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16, b = st * KS + u;
         u32x4 c4 = next.v;
-        const int k0 = st * KEYS + g * 4;                  // the piece's keys: k0 .. + 3 and 16 on
-        if ((st + 1) * KEYS > p0 + f0) {                   // some row does not see some key
+        const int k0 = b * KEYS + g * 4;               // the piece's keys: k0 .. + 3 and 16 on
+        if ((b + 1) * KEYS > p0 + f0) {                // some row does not see some key
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                const int left = ctx - (k0 + w % 2 * 16);  // past the last token: zero
+                const int left = ctx - (k0 + w % 2 * 16);      // past the last token: zero
                 c4[w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
                 const uint32_t bad = kv8_nan_codes(c4[w]);
-                if (bad) {                                 // out of the product, its first key kept
+                if (bad) {                             // out of the product, its first key kept
                     c4[w] &= ~bad;
                     any_nan = 1;
                     atomicMin(&first_nan[d + w / 2 * 16], k0 + w % 2 * 16 + (__ffs((int)bad) - 1) / 8);
                 }
             }
         }
+        // four keys from 4 G: half G % 2, step G / 4, its first or second four
+        char *const vd = vl(buf, u) + d * VP + g % 2 * 16 + g / 2 * 8;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            // four keys from 4 G: half G % 2, step G / 4, its first or second four
-            const int G = g + w % 2 * 4, at = (G / 4 * 2 + G % 2) * 16 + G / 2 % 2 * 8;
-            *reinterpret_cast<u32x2 *>(vl[buf] + (d + w / 2 * 16) * VP + at) = widen4(c4[w], vs);
-        }
+        for (int w = 0; w < 4; w++)
+            *reinterpret_cast<u32x2 *>(vd + (w / 2 * 16 * VP + w % 2 * 32)) = widen4(c4[w], vs);
+        if (KS == 1 || u == kg) cs = uni(next.sc[0]);
     };
-    fetch(0);
+    fetch(0, 0);
 
-    // the wavefront's q rows n = (token 4 wave + n / 8, head n % 8): k-step i, dims 16 i + 8 hf ..
-    const int tok = f0 + wave * 4 + (n >> 3), h = kvh * GRP + (n & 7);
+    // the wavefront's q rows n = (token 4 rblk + n / 8, head n % 8): k-step i, dims 16 i + 8 hf ..
+    const int tok = f0 + rblk * 4 + (n >> 3), h = kvh * GRP + (n & 7);
     const int pos = p0 + min(tok, ns - 1);
     f16x8 q[16];
     float qf;                                              // scores' factor, with log2 e / 16
@@ -211,8 +223,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
         }
     }
     __syncthreads();                                       // (first_nan is clear)
-    put(0, 0);
-    float cs = uni(next.sc[0]);                            // the step's scale of K
+    put(0, 0, 0);
+    if (KS == 2) {
+        fetch(0, 1);
+        put(0, 1, 0);
+    }
 
     f32x16 acc[8];
 #pragma unroll
@@ -220,18 +235,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[i][e] = 0.0f;
     float M = -INFINITY, l = 0.0f;
-    const int wfirst = p0 + min(f0 + wave * 4, ns - 1), wlast = p0 + min(f0 + wave * 4 + 3, ns - 1);
+    const int wfirst = p0 + min(f0 + rblk * 4, ns - 1), wlast = p0 + min(f0 + rblk * 4 + 3, ns - 1);
     for (int st = 0; st < steps; st++) {
-        const int buf = st & 1, k0 = st * KEYS;
-        fetch(min(st + 1, steps - 1));
+        const int buf = st & 1, k0 = (st * KS + kg) * KEYS;
+        const float csn = cs;
+        fetch(min(st + 1, steps - 1), 0);
         __syncthreads();
-        if (k0 <= wlast) {                                 // (wave-uniform)
+        bf16x8 pb[2];
+        const char *vp = vl(buf, kg) + n * VP + hf * 16;
+        auto v_of = [&](int i) { return *reinterpret_cast<const bf16x8 *>(vp + i % 8 * 32 * VP + i / 8 * 32); };
+        const bool work = k0 <= wlast;
+        if (work) {                                        // (wave-uniform)
             f32x16 S;
 #pragma unroll
             for (int e = 0; e < 16; e++) S[e] = 0.0f;
-            const char *kp = kl[buf] + n * KP + hf * 16, *vp = vl[buf] + n * VP + hf * 16;
+            const char *kp = kl(buf, kg) + n * KP + hf * 16;
             auto k_of = [&](int i) { return *reinterpret_cast<const f16x8 *>(kp + i * 32); };
-            auto v_of = [&](int i) { return *reinterpret_cast<const bf16x8 *>(vp + i % 8 * 32 * VP + i / 8 * 32); };
             f16x8 kf[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; i++) kf[i] = k_of(i);
@@ -241,14 +260,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                 if (i + kAhead < 16) kf[i % kAhead] = k_of(i + kAhead);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            bf16x8 vf[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) vf[i] = v_of(i);
-            const float sf = qf * cs;
+            const float sf = qf * csn;
             if (k0 + KEYS > wfirst + 1) {
                 int tl = threadIdx.x;
                 asm volatile("" : "+v"(tl));
-                const int lim = p0 + min(f0 + wave * 4 + ((tl & 31) >> 3), ns - 1) - k0 - 4 * ((tl >> 5) & 1);
+                const int lim = p0 + min(f0 + rblk * 4 + ((tl & 31) >> 3), ns - 1) - k0 - 4 * ((tl >> 5) & 1);
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (8 * (e / 4) + e % 4 > lim) S[e] = -INFINITY;
@@ -273,10 +289,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                 l += x0 + x1;
                 p[e / 2] = pack2(x0, x1);
             }
-            bf16x8 pb[2];
 #pragma unroll
             for (int i = 0; i < 2; i++)
                 pb[i] = __builtin_bit_cast(bf16x8, u32x4{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]});
+        }
+        if (KS == 2 && st + 1 < steps) {
+            put(st + 1, 0, buf ^ 1);
+            fetch(st + 1, 1);
+        }
+        if (work) {
+            bf16x8 vf[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) vf[i] = v_of(i);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -285,45 +309,109 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (st + 1 < steps) {
-            put(st + 1, buf ^ 1);
-            cs = uni(next.sc[0]);
-        }
+        if (st + 1 < steps) put(st + 1, KS - 1, buf ^ 1);
     }
     __syncthreads();                                       // (first_nan is whole)
     l = sum32(l);
     // (formed again: kept, they took registers from the loop)
     int tl = threadIdx.x;
     asm volatile("" : "+v"(tl));
-    const int hf_ = (tl >> 5) & 1, tok_ = f0 + wave * 4 + ((tl & 31) >> 3), pos_ = p0 + tok_;
-    if (tok_ >= ns) return;
-    const float inv = 1.0f / l;
-    const size_t at = (size_t)(t0 + tok_) * nh + kvh * GRP + (tl & 7);
-    const uint16_t *gate = qg + at * 2 * D + D;
-    if (any_nan) {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                if (first_nan[32 * i + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) acc[i][e] = NAN;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
+    const int hf_ = (tl >> 5) & 1, tok_ = f0 + rblk * 4 + ((tl & 31) >> 3), pos_ = p0 + tok_;
+    const bool live = tok_ < ns, nans = any_nan != 0;
+    const size_t at = (size_t)(t0 + min(tok_, ns - 1)) * nh + kvh * GRP + (tl & 7);
+    // dims 32 i + 8 c + 4 hf .. + 3 of a row: f times what a holds
+    auto store = [&](f32x16 a, int i, float f) __attribute__((always_inline)) {
+        const uint16_t *gate = qg + at * 2 * D + D + 32 * i + 4 * hf_;
         uint2 gc[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) gc[c] = *reinterpret_cast<const uint2 *>(gate + 32 * i + 8 * c + 4 * hf_);
+        for (int c = 0; c < 4; c++) gc[c] = *reinterpret_cast<const uint2 *>(gate + 8 * c);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {                      // dims 32 i + 8 c + 4 hf ..
-            const int d = 32 * i + 8 * c + 4 * hf_;
+        for (int c = 0; c < 4; c++) {
             float v[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float gv = bf2f((uint16_t)((e < 2 ? gc[c].x : gc[c].y) >> (16 * (e % 2))));
-                v[e] = acc[i][4 * c + e] * inv * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
+                v[e] = a[4 * c + e] * f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
             }
-            *reinterpret_cast<uint2 *>(y + at * D + d) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+            if (live)
+                *reinterpret_cast<uint2 *>(y + at * D + 32 * i + 8 * c + 4 * hf_) =
+                    make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
         }
+    };
+    auto with_nans = [&](f32x16 a, int i) __attribute__((always_inline)) {
+        if (nans) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (first_nan[32 * i + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) a[e] = NAN;
+        }
+        return a;
+    };
+    if (KS == 1) {
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 8; i++) store(with_nans(acc[i], i), i, inv);
+        return;
     }
+    // KS 2: two wavefronts have the same rows; each finishes half of the dims
+    float *const os = reinterpret_cast<float *>(lds) + (tl & 63);
+    float2 *const ml = reinterpret_cast<float2 *>(lds + kWaves * 64 * 64 * 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const f32x16 t = kg ? acc[i] : acc[4 + i];
+#pragma unroll
+        for (int e = 0; e < 16; e++) os[wave * 4096 + (i * 16 + e) * 64] = t[e];
+    }
+    ml[tl] = make_float2(M, l);
+    __syncthreads();
+    const int other = wave ^ kRowBlocks;
+    const float2 o = ml[other * 64 + (tl & 63)];
+    const float m = fmaxf(M, o.x);
+    const float fa = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m);
+    const float fb = o.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(o.x - m);
+    const float inv = 1.0f / (l * fa + o.y * fb);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f32x16 t = kg ? acc[4 + i] : acc[i];
+#pragma unroll
+        for (int e = 0; e < 16; e++) t[e] = t[e] * fa + os[other * 4096 + (i * 16 + e) * 64] * fb;
+        store(with_nans(t, 4 * kg + i), 4 * kg + i, inv);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Tokens of a tile, 32 or 16: the time of the busiest CU with either, from a
+// tile's alone on a CU (us; 20 + 1.37 a block of keys with 32 tokens, 17.5 + 0.86
+// with 16), tiles dealt longest first: the longest, all of them over the CUs, and
+// where a few more tiles than CUs remain, the two that share a CU. Measured (us,
+// 32 / 16 tokens): one prompt of 256 33 / 25, 1024 67 / 46, 4096 206 / 165, 6000
+// 321 / 345; 512 tokens after 8000 377 / 236; 8 times 300 after 300 53 / 65, 500
+// after 4000 273 / 312.
+int fa_tokens(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv) {
+    const size_t cus = (size_t)cu_count();
+    auto busiest = [&](int tok, double base, double per) {
+        size_t tiles = 0;
+        double sum = 0.0, longest = 0.0;
+        for (size_t s = 0; s < B; s++) {
+            const int64_t n = cu[s + 1] - cu[s];
+            if (!n) continue;
+            const size_t t = (size_t)((n + tok - 1) / tok) * nkv;
+            tiles += t;
+            longest = std::max(longest, base + per * (double)(pos0[s] + n) / KEYS);
+            sum += (double)t * (base + per * ((double)pos0[s] + (double)(n + tok) / 2) / KEYS);
+        }
+        double us = std::max(longest, sum / (double)cus);
+        if (tiles > cus && tiles <= 2 * cus) {
+            std::vector<double> t;
+            t.reserve(tiles);
+            for (size_t s = 0; s < B; s++)
+                for (int64_t n = cu[s + 1] - cu[s], x = 0; x < n; x += tok)
+                    t.insert(t.end(), nkv, base + per * (double)(pos0[s] + std::min<int64_t>(x + tok, n)) / KEYS);
+            std::nth_element(t.begin(), t.begin() + (ptrdiff_t)cus, t.end(), std::greater<double>());
+            us = std::max(us, 2.0 * t[cus]);
+        }
+        return us;
+    };
+    return busiest(16, 17.5, 0.86) < busiest(32, 20.0, 1.37) ? 16 : 32;
 }
 
 }  // namespace
@@ -342,15 +430,20 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
     const size_t nkv = L->nkv;
     if (k)
         if (int e = kv8_append_run(r, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
-    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + kTok - 1) / kTok; },
+    const int tok = fa_tokens(B, cu, pos0, nkv);
+    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + tok - 1) / tok; },
                         [&](const auto &q) {
         constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
         const size_t grid = (size_t)q.e[q.n].off * nkv;
         if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
         const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
-        APUS_TIMED("k_kv8_fa", k_kv8_fa<N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(q, r, qg, L->qn_w, w->rope, (int)nkv,
-                                                                                 c2, y));
+        if (tok == 32)
+            APUS_TIMED("k_kv8_fa", k_kv8_fa<1, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
+                                       q, r, qg, L->qn_w, w->rope, (int)nkv, c2, y));
+        else
+            APUS_TIMED("k_kv8_fa", k_kv8_fa<2, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
+                                       q, r, qg, L->qn_w, w->rope, (int)nkv, c2, y));
         return launch_check("k_kv8_fa");
     });
 }
