@@ -4,9 +4,12 @@
 // once, h' stays in registers for the second norm. fp32 throughout; h' and x
 // are each rounded once.
 //
-// A row belongs to a wavefront up to 2048 elements (no barrier between a
-// row's loads and its stores), to a workgroup of four past them. Aligned rows
-// go 8 elements a load, others one.
+// A row belongs to a wavefront up to 1024 elements (no barrier between its
+// loads and its stores), to a workgroup of four past them (2048, 8192 rows: 46.5
+// us with a workgroup a row, 48.8 with a wavefront; 1529, element by element: 11.9
+// and 16.3). Aligned rows go 8 elements a load, others one. Bound by memory: 8192
+// rows of 2048, fp32 residuals and a gate, 235 MB in 46.5 us, 5.05 TB/s, what a
+// copy of 1 GiB reaches; a single row by its launch.
 #include <math.h>
 #include <stdint.h>
 
@@ -36,27 +39,34 @@ struct NormArgs {
     float scale, eps;
 };
 
-// 8 elements of a row from element i on (VEC), or the elements i, i + step, ...
-template <bool VEC> __device__ __forceinline__ void ld8(float (&v)[8], const uint16_t *p, int i, int step, int n) {
-    if (VEC) {
-        const u16x8 u = *reinterpret_cast<const u16x8 *>(p + i);
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = bf2f(u[e]);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = bf2f(p[min(i + e * step, n - 1)]);
+// 8 elements of a row as they lie in memory: from element i on (VEC), or i, i +
+// step, ... one by one. Widened when they are used: as fp32 from the start a
+// row's took twice the registers, and half as many rows were on their way (8192
+// rows of 2048 with fp32 residuals: 64 us).
+template <class T, bool VEC> struct Eight;
+template <> struct Eight<uint16_t, true> {
+    u16x8 u;
+    __device__ void load(const uint16_t *p, int i, int, int) { u = *reinterpret_cast<const u16x8 *>(p + i); }
+    __device__ float operator[](int e) const { return bf2f(u[e]); }
+};
+template <> struct Eight<float, true> {
+    f32x4 a, b;
+    __device__ void load(const float *p, int i, int, int) {
+        a = *reinterpret_cast<const f32x4 *>(p + i);
+        b = *reinterpret_cast<const f32x4 *>(p + i + 4);
     }
-}
-template <bool VEC> __device__ __forceinline__ void ld8(float (&v)[8], const float *p, int i, int step, int n) {
-    if (VEC) {
-        const f32x4 a = *reinterpret_cast<const f32x4 *>(p + i), b = *reinterpret_cast<const f32x4 *>(p + i + 4);
+    __device__ float operator[](int e) const { return e < 4 ? a[e & 3] : b[e & 3]; }
+};
+template <class T> struct Eight<T, false> {
+    T u[8];
+    __device__ void load(const T *p, int i, int step, int n) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = p[min(i + e * step, n - 1)];
+        for (int e = 0; e < 8; e++) u[e] = p[min(i + e * step, n - 1)];
     }
-}
+    __device__ float operator[](int e) const { return widen(u[e]); }
+    static __device__ float widen(uint16_t x) { return bf2f(x); }
+    static __device__ float widen(float x) { return x; }
+};
 template <bool VEC> __device__ __forceinline__ void st8(uint16_t *p, const float (&v)[8], int i, int step, int n) {
     if (VEC) {
         u16x8 u;
@@ -98,39 +108,35 @@ __global__ __launch_bounds__(256) void k_block_norm(NormArgs a) {
         return (red[k][0] + red[k][1]) + (red[k][2] + red[k][3]);
     };
     const int n = a.hidden, step = VEC ? 1 : TPR;
-    int at[NV];
-    bool in[NV][VEC ? 1 : 8];
+    // of the eight j: its first element, and whether its element e is in the row
+    auto at = [&](int j) { return VEC ? min((j * TPR + lane) * 8, n - 8) : j * 8 * TPR + lane; };
+    auto in = [&](int j, int e) { return VEC ? (j * TPR + lane) * 8 < n : j * 8 * TPR + lane + e * step < n; };
+    Eight<H, VEC> hr[NV];
+    Eight<uint16_t, VEC> y[NV], g[NV], w[NV];
+    const H *hp = reinterpret_cast<const H *>(a.h) + (size_t)row * a.ldh;
+    if (a.y) {
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int i = VEC ? (j * TPR + lane) * 8 : j * 8 * TPR + lane;
-        if (VEC) {
-            in[j][0] = i < n;
-            at[j] = min(i, n - 8);
-        } else {
-            at[j] = i;
-#pragma unroll
-            for (int e = 0; e < (VEC ? 1 : 8); e++) in[j][e] = i + e * step < n;
-        }
+        for (int j = 0; j < NV; j++) y[j].load(a.y + (size_t)row * a.ldy, at(j), step, n);
     }
-    float h[NV][8], y[NV][8], g[NV][8], wa[NV][8], wb[NV][8];
-    const H *hr = reinterpret_cast<const H *>(a.h) + (size_t)row * a.ldh;
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        ld8<VEC>(h[j], hr, at[j], step, n);
-        if (a.y) ld8<VEC>(y[j], a.y + (size_t)row * a.ldy, at[j], step, n);
-        if (a.y && a.gate) ld8<VEC>(g[j], a.gate + (size_t)row * a.ldg, at[j], step, n);
-        if (a.y && a.w_post) ld8<VEC>(wa[j], a.w_post, at[j], step, n);
-        if (a.x) ld8<VEC>(wb[j], a.w_pre, at[j], step, n);
+    for (int j = 0; j < NV; j++) hr[j].load(hp, at(j), step, n);
+    if (a.y && a.gate) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) g[j].load(a.gate + (size_t)row * a.ldg, at(j), step, n);
     }
+    if (a.y && a.w_post) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) w[j].load(a.w_post, at(j), step, n);
+    }
+    float h[NV][8], s = 0.0f;
     if (a.y) {
         float rs = 1.0f;
         if (a.w_post) {
-            float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; j++)
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (in[j][VEC ? 0 : e]) s += y[j][e] * y[j][e];
+                    if (in(j, e)) s += y[j][e] * y[j][e];
             rs = 1.0f / sqrtf(total(s, 0) / (float)n + a.eps);
         }
 #pragma unroll
@@ -138,31 +144,40 @@ __global__ __launch_bounds__(256) void k_block_norm(NormArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 float v = y[j][e];
-                if (a.w_post) v = v * rs * (1.0f + wa[j][e]);
+                if (a.w_post) v = v * rs * (1.0f + w[j][e]);
                 if (a.gate) v *= g[j][e];
-                h[j][e] += a.scale * v;
+                h[j][e] = hr[j][e] + a.scale * v;
             }
-        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) h[j][e] = hr[j][e];
+    }
+    if (a.x) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) w[j].load(a.w_pre, at(j), step, n);
+    }
     if (a.h_out && live) {
         H *o = reinterpret_cast<H *>(a.h_out) + (size_t)row * a.ldo;
 #pragma unroll
         for (int j = 0; j < NV; j++)
-            if (in[j][0]) st8<VEC>(o, h[j], at[j], step, n);
+            if (in(j, 0)) st8<VEC>(o, h[j], at(j), step, n);
     }
     if (!a.x) return;
-    float s = 0.0f;
+    s = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            if (in[j][VEC ? 0 : e]) s += h[j][e] * h[j][e];
+            if (in(j, e)) s += h[j][e] * h[j][e];
     const float rs = 1.0f / sqrtf(total(s, 1) / (float)n + a.eps);
     if (!live) return;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) h[j][e] = h[j][e] * rs * (1.0f + wb[j][e]);
-        if (in[j][0]) st8<VEC>(a.x + (size_t)row * a.ldx, h[j], at[j], step, n);
+        for (int e = 0; e < 8; e++) h[j][e] = h[j][e] * rs * (1.0f + w[j][e]);
+        if (in(j, 0)) st8<VEC>(a.x + (size_t)row * a.ldx, h[j], at(j), step, n);
     }
 }
 
@@ -179,7 +194,7 @@ template <class H> int launch(const NormArgs &a, bool vec) {
         const std::integral_constant<int, 256> four;
         if (a.hidden <= 512) return go(v, one, std::integral_constant<int, 1>{});
         if (a.hidden <= 1024) return go(v, one, std::integral_constant<int, 2>{});
-        if (a.hidden <= 2048) return go(v, one, std::integral_constant<int, 4>{});
+        if (a.hidden <= 2048) return go(v, four, std::integral_constant<int, 1>{});
         if (a.hidden <= 4096) return go(v, four, std::integral_constant<int, 2>{});
         if (a.hidden <= 8192) return go(v, four, std::integral_constant<int, 4>{});
         return go(v, four, std::integral_constant<int, 8>{});
