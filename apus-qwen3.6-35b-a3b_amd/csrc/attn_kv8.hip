@@ -20,7 +20,8 @@
 // order (16-byte loads, whole KiB), widen in registers (exactly: K's codes to fp16,
 // V's times their scale to bf16), and the scores' registers are the operand of
 // P V. Probabilities go to bf16 for that product (fp16 would cut those far below
-// the largest).
+// the largest), and their sum is that of the rounded ones: y is a mean of v with
+// weights that add up to 1, and a single large weight brings no error.
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
@@ -275,9 +276,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
                 const float ref = M[rb] == -INFINITY ? 0.0f : M[rb];
 #pragma unroll
                 for (int i = 0; i < 8; i++) t[i] = __builtin_amdgcn_exp2f(t[i] - ref);
+                u32x4 pk;
+#pragma unroll
+                for (int i = 0; i < 4; i++) pk[i] = pack2(t[2 * i], t[2 * i + 1]);
+                pb[rb] = __builtin_bit_cast(bf16x8, pk);
+                // (the rounded ones: what the product with V is made of)
+#pragma unroll
+                for (int i = 0; i < 8; i++) t[i] = __uint_as_float(i % 2 ? pk[i / 2] & 0xffff0000u : pk[i / 2] << 16);
                 l[rb] += ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
-                pb[rb] = __builtin_bit_cast(bf16x8, u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]),
-                                                          pack2(t[6], t[7])});
             }
             if (tail) {
                 // keys past the last token: whatever lies there counts as zero

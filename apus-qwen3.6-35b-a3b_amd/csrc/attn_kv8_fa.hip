@@ -286,8 +286,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
                 const float x0 = __builtin_amdgcn_exp2f(fmaf(S[e], sf, -ref)), x1 = __builtin_amdgcn_exp2f(fmaf(S[e + 1], sf, -ref));
-                l += x0 + x1;
                 p[e / 2] = pack2(x0, x1);
+                l += __uint_as_float(p[e / 2] << 16) + __uint_as_float(p[e / 2] & 0xffff0000u);   // (the rounded ones)
             }
 #pragma unroll
             for (int i = 0; i < 2; i++)
