@@ -112,6 +112,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
     const uint16_t *__restrict__ rope, int nkv, int total, int run, float c2, uint16_t *__restrict__ y,
     float *__restrict__ part, float2 *__restrict__ stat) {
     static_assert(64 * kWaves == D, "a thread a dim, a wavefront's threads 4 q rows");
+    static_assert(16 * AP >= 2048 && 16 * RB * QP / 2 + kWaves * 2048 <= kWaves * 16 * AP, "room for V with a NaN");
     // (with two row blocks the q rows lie where the outputs meet later: two
     // workgroups a CU)
     __shared__ __attribute__((aligned(16))) float os[kWaves * 16 * AP];
@@ -303,8 +304,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
                 if (__any(wild != 0)) {
                     // a NaN reaches the rows that see its key and no other: taken
                     // out of the product, the first key of each dim kept (in a loop
-                    // over 8 KiB of os of this wavefront's own: unrolled it took 60 registers)
-                    u32x4 *const mine_ = reinterpret_cast<u32x4 *>(os + (RB > 1 ? 16 * RB * QP / 2 : 0)) + wave * 512 + lane;
+                    // over 8 KiB of os, unrolled it took 60 registers: with one row block
+                    // where this wavefront's outputs go, since others may have ended and
+                    // written theirs; with two behind the q rows, all wait before they write)
+                    u32x4 *const mine_ = reinterpret_cast<u32x4 *>(
+                        RB == 1 ? os + wave * 16 * AP : os + 16 * RB * QP / 2 + wave * 2048) + lane;
 #pragma unroll
                     for (int i = 0; i < 8; i++) mine_[i * 64] = vr[i];
 #pragma unroll 1
@@ -584,7 +588,7 @@ int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w
                              cu[s + 1] - cu[s]);
         if (s % kKv8Seqs == 0) total = 0;
         total += (size_t)counted_blocks(pos0[s], cu[s + 1] - cu[s], 0) * L->nkv;
-        if (total > 0x7ff00000) return set_error(kErrUnsupported, "too many cached keys in one call");
+        if (total > 0x7f000000) return set_error(kErrUnsupported, "too many cached keys in one call");
     }
     return kOk;
 }

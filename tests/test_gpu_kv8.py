@@ -275,6 +275,35 @@ def test_nan_reaches_only_those_that_see_it(hip, f, what):
     assert (np.abs(got - r)[ok] <= tol[ok]).all()
 
 
+@pytest.mark.parametrize("ctx,new", [([127], [1]), ([255, 100], [2, 1]), ([1000], [2]), ([90, 3, 60], [1, 1, 2])])
+def test_decode_nan_in_the_last_block(hip, ctx, new):
+    """One row block (at most two tokens), a NaN v among the keys of the last block,
+    while the other wavefronts are done with theirs: its dims alone are NaN."""
+    s = Setup(hip, 33, 2, ctx, new, False)
+    n = np.asarray(ctx) + new
+    c = cum(n)
+    bad = np.zeros((int(sum(new)), s.nh, R.D), bool)
+    for i, p in enumerate(ctx):
+        at = c[i] + (n[i] - 1) // 32 * 32                  # the last block's first position
+        s.v[at, 3::7] = 0x7fc0                             # head 0's and 1's dims
+        head = (np.arange(512) % 7 == 3).reshape(2, R.D)
+        for t in range(new[i]):
+            if p + t >= at - c[i]:
+                bad[s.cu[i] + t] = head.repeat(R.GRP, 0)
+    hip.kv8_append(s.kv, None, c, np.zeros(len(ctx), np.int32), dev(s.k), dev(s.v))
+    for i in range(len(ctx)):
+        v = s.v[c[i]:c[i + 1]].copy()
+        v[(v & 0x7fff) > 0x7f80] = 0
+        s.ref.append(i, 0, s.k[c[i]:c[i + 1]], v)
+    y = s.call(hip.attn_decode_kv8)
+    assert np.array_equal(np.isnan(R.f64(y)), bad)
+    for i in range(len(ctx)):
+        k, v = s.ref.values(i, 0, int(n[i]))
+        sl = slice(s.cu[i], s.cu[i + 1])
+        r, tol = R.attention(s.qg[sl], s.w["qn_w"], ctx[i], k, v, THETA)
+        assert (np.abs(R.f64(y[sl]) - r) <= tol)[~bad[sl]].all()
+
+
 def test_shared_rows(hip):
     """Without k and v, sequences may read one row: a shared prompt."""
     s = Setup(hip, 41, 2, [500, 500], [2, 2], True)
