@@ -89,7 +89,7 @@ __device__ __forceinline__ float uni(float x) {
 template <int KS, int N>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg,
                                                            const uint16_t *__restrict__ qn_w,
-                                                           const uint16_t *__restrict__ rope, int nkv, float c2,
+                                                           const uint16_t *__restrict__ rope, int nkv,
                                                            uint16_t *__restrict__ y) {
     constexpr int kKl = KEYS * KP, kVl = D * VP, kRowBlocks = kWaves / KS, kTok = 4 * kRowBlocks;
     // two buffers of KS blocks' K and V; then outputs that meet: 64 registers of 8 wavefronts
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     const int tok = f0 + rblk * 4 + (n >> 3), h = kvh * GRP + (n & 7);
     const int pos = p0 + min(tok, ns - 1);
     f16x8 q[16];
-    float qf;                                              // scores' factor, with log2 e / 16
+    float qf;                                              // scores' factor, a power of two (log2 e is in q)
     {
         const uint16_t *qr = qg + ((size_t)(t0 + min(tok, ns - 1)) * nh + h) * 2 * D + hf * 8;
         // (every load at once: the outputs' registers are free yet)
@@ -214,8 +214,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
 #pragma unroll
             for (int e = 0; e < 8; e++) mq = fmaxf(mq, fabsf(o[i][e]));
         mq = max32(mq);
-        const float sc = kv8_row_scale(mq), inv = 1.0f / sc;
-        qf = sc * c2;
+        // (so the scores' factors are exact, and a score less M, by fma, is what M was
+        // formed from: a rounded product's residual of a score past 2^31 gave infinities)
+        const float sc = kv8_row_scale(mq), inv = kL2E / sc;
+        qf = sc / 16.0f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
 #pragma unroll
@@ -260,7 +262,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
                 if (i + kAhead < 16) kf[i % kAhead] = k_of(i + kAhead);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const float sf = qf * csn;
+            // (at least the smallest normal: 0 would make a NaN of a masked -inf)
+            const float sf = fmaxf(qf * csn, 0x1p-126f);
             if (k0 + KEYS > wfirst + 1) {
                 int tl = threadIdx.x;
                 asm volatile("" : "+v"(tl));
@@ -437,13 +440,12 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
         const size_t grid = (size_t)q.e[q.n].off * nkv;
         if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
-        const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
         if (tok == 32)
             APUS_TIMED("k_kv8_fa", k_kv8_fa<1, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
-                                       q, r, qg, L->qn_w, w->rope, (int)nkv, c2, y));
+                                       q, r, qg, L->qn_w, w->rope, (int)nkv, y));
         else
             APUS_TIMED("k_kv8_fa", k_kv8_fa<2, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
-                                       q, r, qg, L->qn_w, w->rope, (int)nkv, c2, y));
+                                       q, r, qg, L->qn_w, w->rope, (int)nkv, y));
         return launch_check("k_kv8_fa");
     });
 }

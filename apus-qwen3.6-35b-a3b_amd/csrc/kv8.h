@@ -152,7 +152,7 @@ int kv8_launches(size_t B, const int32_t *rows, const int32_t *cu, const int32_t
 // A row of q is divided by a power of two that brings its largest magnitude to
 // [2^6, 2^7), which keeps 256 products with codes in fp32's range with room and
 // the small elements out of fp16's subnormals; the power and the block's scale
-// are factors of the scores. (A row of zeros: 1. One that holds an infinity or
+// are factors of the scores (log2 e too, or it is in q). (A row of zeros: 1. One that holds an infinity or
 // NaN: NaN.)
 typedef _Float16 kv8_f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 kv8_f16x2 __attribute__((ext_vector_type(2)));

@@ -719,11 +719,12 @@ int apus_hip_attn_kv8_work_destroy(ApusHipAttnKv8Work *w);
  * layer that shares its cache); then sequences may share rows. After norm and
  * RoPE q is rounded to fp16 once, at a power of two of its row, probabilities
  * to bf16 for their product with V; scores, softmax and sums are fp32 and y is
- * rounded once: a tolerance class of the result on the cache's values, |c - r| <=
- * 2^-8 |r| + sum_j P_j |V_j| sigmoid(gate) (2^-8 + 2^-10 + e_j), e_j = 2^-12 (a_j +
- * sum_i P_i a_i) from q's rounding, a_j = sum_d |q_d K_jd| / 16. A NaN in a position that a token does not attend to
- * does not reach its row. Supports d=256, rot=64, nh=8*nkv. y may not overlap
- * the inputs. */
+ * rounded once: a tolerance class of the result on the cache's values (o = sum_j
+ * P_j V_j before the gate), |c - r| <= 2^-8 |r| + sigmoid(gate) sum_j P_j (2^-8 |V_j -
+ * o| + (2^-10 + e_j) |V_j|), e_j = 2^-11 (a_j + sum_i P_i a_i) from q's rounding, a_j
+ * = sum_d max(|q_d|, 2^-20 max |q|) |K_jd| / 16. A NaN in a position that a token
+ * does not attend to does not reach its row. Supports d=256, rot=64, nh=8*nkv. y
+ * may not overlap the inputs. */
 int apus_hip_attn_decode_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B,
                              const int32_t *rows, const int32_t *cu, const int32_t *pos0,
                              const uint16_t *qg, const uint16_t *k, const uint16_t *v,

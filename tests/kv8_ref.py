@@ -107,12 +107,17 @@ def q_rows(q, w, pos, theta, eps=1e-6):
 
 def attention(qg, w, pos0, k, v, theta):
     """One sequence: qg [n][nh][2D] codes at positions pos0 ..., k, v [>= pos0 + n]
-    [nkv][D] float64. Returns y [n][nh][D] and its bound: q's rounding to fp16
-    (half a step, 2^-11 / 2 of each element, so 2^-12 a_j of a score, a_j the sum
-    of its terms' magnitudes; a probability moves by that and by the mean of all),
-    the probabilities' rounding for the product with V (U of each term), fp32
-    arithmetic (2^-10 of the terms is far more than it makes: scores of some 20
-    with 256 terms of 2^-24), and the rounding of y."""
+    [nkv][D] float64. Returns y [n][nh][D] and its bound.
+
+    q's rounding to fp16: half a step, 2^-11 of an element, or of 2^-20 of the row's
+    largest m (which lies at 2^6 or above, an element below 2^-14 at steps of
+    2^-24), so a score is off by 2^-11 a_j, a_j = sum_d max(|q_d|, 2^-20 m) |K_jd| /
+    16, and a probability by the factors of its own and of the sum of all.
+    The probabilities' rounding: p_j (1 + d_j), |d_j| <= U, for the product with V
+    and for their sum, y' = sum p_j (1 + d_j) v_j / sum p_j (1 + d_j) = y + sum p_j
+    d_j (v_j - y) / sum p_j (1 + d_j): U / (1 - U) sum_j p_j |v_j - y|.
+    fp32 arithmetic: 2^-10 of the terms is far more than it makes (scores of some
+    20 with 256 terms of 2^-24; exponents of 1 ulp). And the rounding of y."""
     n, nh = qg.shape[:2]
     nkv = k.shape[1]
     q = q_rows(qg[..., :D], w, pos0 + np.arange(n), theta)
@@ -123,12 +128,17 @@ def attention(qg, w, pos0, k, v, theta):
         for h in range(nkv):
             hs = slice(h * GRP, (h + 1) * GRP)
             s = q[t, hs] @ k[:m, h].T / 16.0
-            a = np.abs(q[t, hs]) @ np.abs(k[:m, h]).T / 16.0
+            qa = np.abs(q[t, hs])
+            a = np.maximum(qa, 2.0 ** -20 * qa.max(-1, keepdims=True)) @ np.abs(k[:m, h]).T / 16.0
             p = np.exp(s - s.max(-1, keepdims=True))
             p /= p.sum(-1, keepdims=True)
-            e = 2.0 ** -12 * (a + (p * a).sum(-1, keepdims=True))
+            e = 2.0 ** -11 * (a + (p * a).sum(-1, keepdims=True))
             y[t, hs] = p @ v[:m, h]
-            tol[t, hs] = (p * (U + 2.0 ** -10 + np.expm1(e))) @ np.abs(v[:m, h])
+            with np.errstate(over="ignore", invalid="ignore"):
+                move = np.fmin(p * np.expm1(e), 1.0)       # (between 0 and 1 it cannot move further; 0 inf: 1)
+            tol[t, hs] = (p * 2.0 ** -10 + move) @ np.abs(v[:m, h])
+            for i in range(GRP):
+                tol[t, h * GRP + i] += U / (1 - U) * (p[i] @ np.abs(v[:m, h] - y[t, h * GRP + i]))
     y *= sig
     tol = tol * sig + U * np.abs(y)
     return y, tol * (1 + U) + 2.0 ** -133

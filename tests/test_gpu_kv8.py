@@ -246,6 +246,23 @@ def test_decode_growing_scores(hip):
 
 
 @pytest.mark.parametrize("f", ["attn_decode_kv8", "attn_prefill_kv8"])
+@pytest.mark.parametrize("q,k", [(0.0, 0.0), (2.0 ** -126, 0.0), (2.0 ** -126, 2.0 ** -133), (1.0, 0.0), (2.0 ** -126, 1.0),
+                                 (0.0, 1.0), (1.0, 2.0 ** 100)])
+def test_tiny_and_large_rows(hip, f, q, k):
+    """Rows of zeros and of the smallest values: every key counts the same; and k
+    so large that one key has it all."""
+    s = Setup(hip, 23, 2, [37, 0], [4, 3], False)
+    s.qg.reshape(-1, 2 * R.D)[:, :R.D] = R.bf16(R.f64(s.qg).reshape(-1, 2 * R.D)[:, :R.D] * q)
+    s.k = R.bf16(R.f64(s.k) * k)
+    n = s.ctx + s.new
+    c = cum(n)
+    hip.kv8_append(s.kv, None, c, [0, 0], dev(s.k), dev(s.v))
+    for i in range(2):
+        s.ref.append(i, 0, s.k[c[i]:c[i + 1]], s.v[c[i]:c[i + 1]])
+    s.check(s.call(getattr(hip, f)))
+
+
+@pytest.mark.parametrize("f", ["attn_decode_kv8", "attn_prefill_kv8"])
 @pytest.mark.parametrize("what", ["k", "v"])
 def test_nan_reaches_only_those_that_see_it(hip, f, what):
     """A token whose k or v holds NaN or infinity: rows before it are as without
