@@ -951,16 +951,20 @@ def _kv8_rows_call(f, kv, rows, cu, pos0, k, v):
     n, T = kv.nkv * 256, _total(keep[1])
     ld = []
     for t, what in ((k, "k"), (v, "v")):
-        p, m, _, pitch = _rows(t.flatten(1) if t.dim() == 3 else t, what, _device, n)
+        if t.dim() == 3:
+            if tuple(t.shape[1:]) != (kv.nkv, 256) or (t.shape[0] and kv.nkv > 1 and t.stride(1) != 256):
+                raise ValueError(f"{what}: rows of {kv.nkv} heads of 256, contiguous, not {tuple(t.shape)} of strides {t.stride()}")
+            t = t.flatten(1)
+        p, m, _, pitch = _rows(t, what, _device, n)
         if m != T:
             raise ValueError(f"{what}: {m} rows, expected {T}")
-        ld += [p, max(pitch, n)]
+        ld += [p, pitch]
     return BoundCall(f, (C.addressof(kv), kv.nkv, B, rp, cp, pp, *ld), (kv, keep, k, v))
 
 
 def kv8_append_bound(kv, rows, cu, pos0, k, v):
     """kv8_append as a BoundCall (rows, cu, pos0 as int32 numpy arrays may be
-    changed in place between calls)."""
+    changed in place between calls; the tensors have cu's last entry of rows)."""
     return _kv8_rows_call(load().apus_hip_kv8_append, kv, rows, cu, pos0, k, v)
 
 
@@ -993,7 +997,7 @@ class AttnKv8Work:
     def destroy(self):
         if self.h:
             _chk(load().apus_hip_attn_kv8_work_destroy(self.h))
-            self.h = C.c_void_p()
+            self.h.value = None            # (bound calls hold this object: they are refused from now on)
 
 
 def _dense(t, shape, what):
@@ -1063,7 +1067,8 @@ def block_norm_weights(hidden, w_pre=None, w_post=None, gate=None, scale=1.0, ep
             continue
         if what == "gate" and t.dim() == 2:
             ptr[what], _, _, ld = _rows(t, what, _device, hidden)
-            ld = max(ld, hidden)
+            if ld < hidden:                # (0 would be one row for all)
+                raise ValueError(f"gate: rows of {hidden} elements with pitch {ld}")
             continue
         if t.get_device() != _device or not _bf16(t) or tuple(t.shape) != (hidden,) or not t.is_contiguous():
             raise ValueError(f"{what}: contiguous ({hidden},) bf16 on GPU {_device}, not {tuple(t.shape)} {t.dtype} "
@@ -1078,7 +1083,7 @@ def block_norm_weights(hidden, w_pre=None, w_post=None, gate=None, scale=1.0, ep
 def _f32_rows(t, what, dev, ncols):
     import torch
     if t.dim() != 2 or t.get_device() != dev or t.dtype != torch.float32 or t.shape[1] != ncols or (
-            t.stride(1) != 1 and ncols > 1):
+            t.stride(1) != 1 and ncols > 1 and t.shape[0]):
         raise ValueError(f"{what}: a 2-D tensor of fp32 rows of {ncols} on GPU {dev}, not {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
     return t.data_ptr(), t.shape[0], ncols, t.stride(0) if t.shape[0] > 1 else ncols
@@ -1099,12 +1104,12 @@ def block_norm(norm, y, h, h_out, x):
         p, m, _, ld = _f32_rows(t, what, dev, n) if f32 and what == "h_out" else _rows(t, what, dev, n)
         if m != T:
             raise ValueError(f"{what}: {m} rows, expected {T}")
-        args.append((p, max(ld, n)))
+        args.append((p, ld))
     if norm._gate_rows is not None and norm._gate_rows != T:
         raise ValueError(f"gate: {norm._gate_rows} rows, expected {T}")
     norm.h_f32 = int(f32)
     (yp, ldy), (op, ldo), (xp, ldx) = args
-    _chk(load().apus_hip_block_norm(C.addressof(norm), T, yp, ldy, hp, max(ldh, n), op, ldo, xp, ldx))
+    _chk(load().apus_hip_block_norm(C.addressof(norm), T, yp, ldy, hp, ldh, op, ldo, xp, ldx))
 
 
 # ---- named-intermediate capture

@@ -24,12 +24,11 @@
 // weights that add up to 1, and a single large weight brings no error.
 #include <math.h>
 #include <stdint.h>
-#include <string.h>
 
 #include <algorithm>
 #include <new>
 #include <type_traits>
-#include <vector>
+#include <utility>
 
 #include "apus_dev.h"
 #include "apus_host.h"
@@ -50,7 +49,6 @@ constexpr float kSlack = 10.0f;
 
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef kv8_bf16x8 bf16x8;
 typedef kv8_f16x8 f16x8;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -508,6 +506,8 @@ int attn_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_
                    const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T) {
     if (int e = attn_check_layer(L)) return e;
     if (!w) return set_error(kErrArgument, "NULL workspace");
+    if (w->device != current_device())
+        return set_error(kErrArgument, "the workspace is on device %d, the library on %d", w->device, current_device());
     if (w->nkv != L->nkv || w->rot != L->rot || w->theta != L->theta)
         return set_error(kErrArgument, "the workspace was made for a layer of other dims");
     if (!k != !v) return set_error(kErrArgument, "k and v are both given or both NULL");
@@ -527,6 +527,15 @@ int attn_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_
         kv8_overlap(y, ny, kv->scale, kv->blocks * L->nkv * 8) ||
         kv8_overlap(y, ny, L->qn_w, D * 2) || kv8_overlap(y, ny, L->kn_w, D * 2))
         return set_error(kErrArgument, "y overlaps an input");
+    if (kv->block_table && kv8_overlap(y, ny, kv->block_table, kv->max_rows * kv->max_blocks * 4))
+        return set_error(kErrArgument, "y overlaps the block table");
+    if (k) {                               // (the cache is written)
+        const std::pair<const void *, size_t> in[] = {{qg, 2 * ny}, {k, nk}, {v, nk}, {L->qn_w, D * 2}, {L->kn_w, D * 2}};
+        for (const auto &[p, n] : in)
+            if (kv8_overlap(p, n, kv->k, nb) || kv8_overlap(p, n, kv->v, nb) ||
+                kv8_overlap(p, n, kv->scale, kv->blocks * L->nkv * 8))
+                return set_error(kErrArgument, "an input overlaps the cache");
+    }
     return kOk;
 }
 

@@ -13,11 +13,9 @@
 // lane half h takes the keys 8 q + 4 h + 0..3, q = 0..3, 8 a step.
 #include <math.h>
 #include <stdint.h>
-#include <string.h>
 
 #include <algorithm>
 #include <functional>
-#include <vector>
 
 #include "apus_dev.h"
 #include "apus_host.h"
@@ -403,13 +401,13 @@ int fa_tokens(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv) {
             sum += (double)t * (base + per * ((double)pos0[s] + (double)(n + tok) / 2) / KEYS);
         }
         double us = std::max(longest, sum / (double)cus);
-        if (tiles > cus && tiles <= 2 * cus) {
-            std::vector<double> t;
-            t.reserve(tiles);
+        double t[1024];
+        if (tiles > cus && tiles <= std::min<size_t>(2 * cus, 1024)) {
+            double *e = t;
             for (size_t s = 0; s < B; s++)
-                for (int64_t n = cu[s + 1] - cu[s], x = 0; x < n; x += tok)
-                    t.insert(t.end(), nkv, base + per * (double)(pos0[s] + std::min<int64_t>(x + tok, n)) / KEYS);
-            std::nth_element(t.begin(), t.begin() + (ptrdiff_t)cus, t.end(), std::greater<double>());
+                for (int64_t n = cu[s + 1] - cu[s], x = 0; x < n; x += tok, e += nkv)
+                    std::fill_n(e, nkv, base + per * (double)(pos0[s] + std::min<int64_t>(x + tok, n)) / KEYS);
+            std::nth_element(t, t + cus, e, std::greater<double>());
             us = std::max(us, 2.0 * t[cus]);
         }
         return us;

@@ -13,7 +13,8 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <vector>
+#include <memory>
+#include <new>
 
 #include "apus_dev.h"
 #include "apus_host.h"
@@ -334,7 +335,10 @@ int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *row
     if (!B) return kOk;
     if (B > ((size_t)1 << 24)) return set_error(kErrUnsupported, "%zu sequences", B);
     if (!cu || !pos0 || cu[0] != 0) return set_error(kErrArgument, "bad offsets");
-    std::vector<int32_t> used;
+    // the rows written to (no exception may leave an entry point)
+    std::unique_ptr<int32_t[]> used(writes && rows ? new (std::nothrow) int32_t[B] : nullptr);
+    if (writes && rows && !used) return set_error(kErrHip, "out of host memory");
+    size_t nused = 0;
     for (size_t s = 0; s < B; s++) {
         const int64_t n = (int64_t)cu[s + 1] - cu[s], end = (int64_t)pos0[s] + n;
         if (n < 0) return set_error(kErrArgument, "token offsets must ascend");
@@ -352,10 +356,10 @@ int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *row
                 return set_error(kErrArgument, "sequence %zu reaches position %lld but row %lld has reserved %lld "
                                  "positions", s, (long long)end, (long long)row, (long long)held * KEYS);
         }
-        if (writes && n && rows) used.push_back((int32_t)row);
+        if (writes && n && rows) used[nused++] = (int32_t)row;
     }
-    std::sort(used.begin(), used.end());
-    if (std::adjacent_find(used.begin(), used.end()) != used.end())
+    std::sort(used.get(), used.get() + nused);
+    if (std::adjacent_find(used.get(), used.get() + nused) != used.get() + nused)
         return set_error(kErrArgument, "two sequences of a call write to one row");
     *tokens = (size_t)cu[B];
     return kOk;

@@ -671,10 +671,12 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
  * pos0 (HOST) say what in apus_hip_attn_decode_paged they say; a sequence may
  * have no tokens. Host arrays go by value: the calls can be captured into
  * graphs, allocate nothing and do not wait, and what a captured call was given
- * stays as it was. Bad arguments are refused with or without a device. Two
- * sequences of a call that writes may not share a row; calls that write a row
- * and calls that use it run in the caller's order (one stream, or events).
- * They are not traced (apus_hip_trace_set). */
+ * stays as it was. Bad arguments are refused with or without a device (the layer
+ * call: with one). Two sequences of a call that writes may not share a row, nor
+ * may the blocks that it writes be another row's (blocks that are only read may:
+ * a shared prompt); calls that write a row and calls that use it run in the
+ * caller's order (one stream, or events). They are not traced
+ * (apus_hip_trace_set). */
 typedef struct {
     uint8_t *k, *v;
     float *scale;
@@ -706,7 +708,7 @@ int apus_hip_kv8_pool_cache(const ApusHipKvPool *pool, size_t layer, ApusHipKv8C
  * sequences of a decode call. Calls that share one run one after the other:
  * on one stream, or ordered by the caller; calls or graph replays that may
  * overlap need one each. It must outlive the graphs that captured its calls.
- * destroy waits for the library's stream. */
+ * create and destroy wait for the library's stream: not while it is captured. */
 typedef struct ApusHipAttnKv8Work ApusHipAttnKv8Work;
 int apus_hip_attn_kv8_work_create(const ApusHipAttnLayer *L, size_t max_seqs, size_t max_pos,
                                   ApusHipAttnKv8Work **out);

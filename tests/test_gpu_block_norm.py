@@ -138,3 +138,45 @@ def test_matches_attn_rmsnorm(hip):
     hip.block_norm(norm, None, dev(h)[None], None, x)
     a, b = R.f64(x.cpu().numpy().view(np.uint16)[0]), R.f64(hip.attn_rmsnorm(h, w))
     assert (np.abs(a - b) <= 2.0 ** -7 * np.abs(b)).all() and np.mean(a != b) < 0.01
+
+
+def test_graph_and_strides(hip):
+    """A captured call, replayed between eager work on a stream of its own; rows
+    that lie on top of each other are refused."""
+    rng = np.random.default_rng(3)
+    T, n = 5, 2048
+    y, h, gate = rows(rng, T, n, 0, False), rows(rng, T, n, 0, True), rows(rng, T, n, 0, False)
+    w = [dev(R.bf16(rng.normal(size=n) * 0.1)) for _ in range(2)]
+    norm = hip.block_norm_weights(n, w_pre=w[0], w_post=w[1], gate=gate, scale=0.7)
+    ho, x = torch.empty_like(h), torch.empty_like(y)
+    hip.block_norm(norm, y, h, ho, x)
+    torch.cuda.synchronize()
+    want = ho.clone(), x.clone()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    hip.set_stream(st.cuda_stream)
+    try:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            hip.block_norm(norm, y, h, ho, x)
+        for i in range(3):
+            ho.zero_()
+            x.zero_()
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(ho, want[0]) and torch.equal(x, want[1]), i
+            torch.randn(1000, device="cuda").sum().item()
+    finally:
+        hip.set_stream(0)
+    for a in (dict(h=h[:1].expand(T, n)), dict(y=y[:1].expand(T, n)), dict(h_out=ho[:1].expand(T, n)),
+              dict(x=x[:1].expand(T, n))):
+        with pytest.raises(hip.ApusHipError, match="pitch"):
+            hip.block_norm(norm, **dict(dict(y=y, h=h, h_out=ho, x=x), **a))
+    with pytest.raises(ValueError, match="gate"):
+        hip.block_norm_weights(n, w_pre=w[0], gate=gate[:1].expand(T, n))
+    for a in (dict(h=h[:4]), dict(y=y.float()), dict(h_out=ho.to(torch.bfloat16)), dict(x=x.cpu()), dict(x=x[:, :-8])):
+        with pytest.raises(ValueError):
+            hip.block_norm(norm, **dict(dict(y=y, h=h, h_out=ho, x=x), **a))
+    torch.cuda.synchronize()
+    assert torch.equal(ho, want[0]) and torch.equal(x, want[1])

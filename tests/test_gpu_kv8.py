@@ -366,6 +366,48 @@ def test_prefill(hip, ctx, new, nkv, paged):
     s.check(s.call(hip.attn_prefill_kv8))
 
 
+@pytest.mark.parametrize("nkv,nan", [(2, None), (3, "k"), (2, "v")])
+def test_prefill_many_tokens(hip, nkv, nan):
+    """Work for every CU many times over (tiles of 32 tokens): ragged sequences;
+    with a NaN in a new token of one, which reaches the rows from it on."""
+    rng = np.random.default_rng(13)
+    B = 160
+    ctx, new = rng.integers(0, 200, B), rng.integers(1, 75, B)
+    ctx[:4], new[:4] = [0, 31, 64, 33], [70, 33, 32, 66]
+    s = Setup(hip, 73, nkv, ctx, new, True)
+    picks = [0, 1, 2, 3] + list(range(7, B, 23))
+    if nan is None:
+        s.check(s.call(hip.attn_prefill_kv8), picks)
+        return
+    want = s.call(hip.attn_prefill_kv8)
+    n = ctx + new
+    c, q = cum(n), 3
+    x = {"k": s.k.copy(), "v": s.v.copy()}
+    x[nan][c[q] + 33 + 40, 256 + 17] = 0xffc0              # the 41st new token; head 1, dim 17
+    sl = slice(c[q], c[q + 1])
+    hip.kv8_append(s.kv, [s.row(q)], [0, int(n[q])], [0], dev(x["k"][sl]), dev(x["v"][sl]))
+    y = s.call(hip.attn_prefill_kv8)
+    bad = np.zeros(y.shape, bool)
+    at, end = s.cu[q] + 40, s.cu[q + 1]
+    bad[at:end, 8:16, slice(17, 18) if nan == "v" else slice(None)] = True
+    got = R.f64(y)
+    assert np.array_equal(np.isnan(got), bad)
+    # (the sequence's block has another scale where the NaN stood for its largest value)
+    s.check(want, picks)
+    others = np.ones(len(y), bool)
+    others[s.cu[q]:end] = False
+    assert np.array_equal(y[others], want[others])
+    x[nan][c[q] + 73, 273] = 0
+    s.ref.append(s.row(q), 0, x["k"][sl], x["v"][sl])
+    kk, vv = s.ref.values(s.row(q), 0, int(n[q]))
+    rs = slice(s.cu[q], end)
+    r, tol = R.attention(s.qg[rs], s.w["qn_w"], int(ctx[q]), kk, vv, THETA)
+    ok = ~bad[rs]
+    if nan == "k":
+        ok[40:, 8:16] = False
+    assert (np.abs(got[rs] - r) <= tol)[ok].all()
+
+
 def test_prefill_many_sequences(hip):
     rng = np.random.default_rng(9)
     s = Setup(hip, 71, 1, rng.integers(0, 60, 230), rng.integers(0, 6, 230), True)
@@ -433,3 +475,124 @@ def test_other_stream_and_graph(hip):
             torch.randn(1000, device="cuda").sum().item()
     finally:
         hip.set_stream(0)
+
+
+def test_overlapping_replays(hip):
+    """Two captured calls with a workspace each, replayed at once on two streams;
+    two with one, one after the other."""
+    a, b = (Setup(hip, 95 + i, 2, [3000, 2500 + i], [2, 1], False) for i in range(2))
+    want, graphs = [], []
+    for s in (a, b):
+        want.append(s.call(hip.attn_decode_kv8))
+        st, y = torch.cuda.Stream(), torch.zeros(3, s.nh * R.D, dtype=torch.int16, device="cuda")
+        call = hip.attn_decode_kv8_bound(s.layer, s.work, s.rows, s.cu, s.ctx, dev(s.qg), None, None, s.kv, y)
+        st.wait_stream(torch.cuda.current_stream())
+        hip.set_stream(st.cuda_stream)
+        try:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                for _ in range(20):
+                    call()
+        finally:
+            hip.set_stream(0)
+        graphs.append((g, st, y, call))
+    for i in range(4):
+        for _, _, y, _ in graphs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, st, _, _ in graphs:
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, _, y, _), w in zip(graphs, want):
+            assert np.array_equal(host(y).reshape(w.shape), w), i
+        torch.randn(1000, device="cuda").sum().item()
+    # one workspace: b's call with a's
+    y = torch.zeros(3, b.nh * R.D, dtype=torch.int16, device="cuda")
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    hip.attn_decode_kv8(b.layer, a.work, b.rows, b.cu, b.ctx, dev(b.qg), None, None, b.kv, y)
+    torch.cuda.synchronize()
+    assert np.array_equal(host(y).reshape(want[1].shape), want[1])
+
+
+def test_call_refusals(hip):
+    """What only a workspace's call can refuse, and the binding's own checks;
+    nothing is written."""
+    s = Setup(hip, 97, 2, [100, 64], [1, 4], False)
+    k = torch.zeros(5, 512, dtype=torch.int16, device="cuda")
+    qg, y = dev(s.qg), torch.full((5, s.nh * R.D), 0x77, dtype=torch.int16, device="cuda")
+    base = dict(layer=s.layer, work=s.work, rows=None, cu=s.cu, pos0=s.ctx, qg=qg, k=k, v=k, kv=s.kv, y=y)
+    state = [t.clone().view(torch.uint8) for t in s.kv._tensors[:3]]   # (bytes: untouched scales are NaN)
+
+    def refused(match, f=hip.attn_decode_kv8, exc=hip.ApusHipError, **kw):
+        with pytest.raises(exc, match=match):
+            f(**dict(base, **kw))
+
+    refused("0..4 new", cu=[0, 0, 5])
+    refused("both", k=None)
+    refused("both", v=None, f=hip.attn_prefill_kv8)
+    refused("overlap", y=qg.view(-1)[:5 * s.nh * R.D].view(5, -1))
+    refused("overlap", y=s.kv._tensors[0].view(torch.int16).view(-1)[:5 * s.nh * R.D].view(5, -1))
+    refused("overlap", k=s.kv._tensors[1].view(torch.int16).view(-1)[:5 * 512].view(5, -1))
+    refused("one row", rows=[1, 1])
+    refused("outside", rows=[1, 2])
+    refused("offsets", cu=[1, 1, 5])
+    refused("ascend", cu=[0, 6, 5])
+    refused("overflows", pos0=[-1, 0])
+    refused("overflows", pos0=[0, s.max_blocks * 32 - 3])
+    short, other = hip.AttnKv8Work(s.layer, 1, 100), hip.AttnKv8Work(hip.attn_layer((24, 3, R.D, R.ROT, THETA), s.dw), 2, 200)
+    refused("position", work=short)
+    refused("position", work=short, f=hip.attn_prefill_kv8)
+    refused("holds 1", work=short, pos0=[0, 0])
+    refused("other dims", work=other)
+    for w in (short, other):
+        w.destroy()
+        refused("workspace", work=w)
+    bound = hip.attn_decode_kv8_bound(**dict(base, work=hip.AttnKv8Work(s.layer, 2, 200)))
+    bound._keep[1].destroy()
+    with pytest.raises(hip.ApusHipError, match="workspace"):
+        bound()
+    refused("qg", exc=ValueError, qg=qg[:4])
+    refused("y", exc=ValueError, y=y.float())
+    refused("k", exc=ValueError, k=k.cpu())
+    refused("heads", exc=ValueError, kv=hip.kv8_cache(1, 8, 4))
+    refused("offset", exc=ValueError, cu=[0, 1, 2, 5])
+    rows = lambda **kw: dict(dict(kv=s.kv, rows=None, cu=s.cu, pos0=s.ctx, k=k, v=k), **kw)      # noqa: E731
+    for kw, exc, match in ((dict(k=k[:1].expand(5, 512)), hip.ApusHipError, "pitch"), (dict(k=k[:, ::2]), ValueError, "k"),
+                           (dict(v=k[:, :256]), ValueError, "v"), (dict(k=k.view(5, 2, 256).transpose(1, 2)), ValueError, "k"),
+                           (dict(k=torch.zeros(5, 2, 512, dtype=torch.int16, device="cuda")[:, :, :256]), ValueError, "k"),
+                           (dict(k=k[:4]), ValueError, "k"), (dict(rows=[0, 0]), hip.ApusHipError, "one row")):
+        with pytest.raises(exc, match=match):
+            hip.kv8_append(**rows(**kw))
+    with pytest.raises(ValueError):
+        hip.kv8_cache(2, 8, 4, d=128)
+    with pytest.raises(ValueError, match="block_table"):
+        hip.kv8_cache(2, 8, 4, block_table=torch.zeros(2, 4, dtype=torch.int64, device="cuda"))
+    torch.cuda.synchronize()
+    assert (y == 0x77).all()
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(state, s.kv._tensors))
+    # nothing to do: no tokens at all, no sequences
+    none = torch.empty(0, s.nh * R.D, dtype=torch.int16, device="cuda")
+    for f in (hip.attn_decode_kv8, hip.attn_prefill_kv8):
+        f(s.layer, s.work, None, [0, 0, 0], [5, 0], qg[:0], k[:0], k[:0], s.kv, none)
+        f(s.layer, s.work, None, [0], [], qg[:0], None, None, s.kv, none)
+    hip.kv8_append(s.kv, None, [0, 0, 0], [5, 0], k[:0], k[:0])
+    hip.kv8_read(s.kv, None, [0], [], k[:0], k[:0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(state, s.kv._tensors))
+
+
+def test_nan_stays_through_a_rescale(hip):
+    """A stored NaN and a -0 keep what they are when later tokens of their block
+    bring a larger scale."""
+    rng = np.random.default_rng(99)
+    kv, ref = make(hip, rng, 1, 1, 1, False), R.Cache(1, 1, 1)
+    pos = 0
+    for n, size in ((5, 1.0), (3, 100.0), (1, 3e5), (4, 1e-3), (2, 1e30)):
+        k, v = (R.bf16(rng.normal(size=(n, R.D)) * size) for _ in range(2))
+        k[0, 7], v[0, 9], k[-1, 11], v[-1, 12] = 0x7fc0, 0xff80, 0x8000, 0x8000
+        hip.kv8_append(kv, None, [0, n], [pos], dev(k), dev(v))
+        ref.append(0, pos, k, v)
+        pos += n
+        check_row(hip, kv, ref, 0, 0, pos)
