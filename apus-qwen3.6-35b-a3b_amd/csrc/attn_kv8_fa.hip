@@ -31,6 +31,7 @@ constexpr int kWaves = 8;
 constexpr int kAhead = 2;                    // operands read ahead of their products
 constexpr int KP = D * 2 + 16;               // LDS pitches (bytes): a key's K row, a dim's V row
 constexpr int VP = KEYS * 2 + 16;
+constexpr int kYP = D + 16;                  // of half a row of y
 constexpr float kEps = 1e-6f, kL2E = 1.44269504088896341f;
 constexpr float kSlack = 10.0f;              // as in attn_kv8.hip
 
@@ -92,7 +93,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     constexpr int kKl = KEYS * KP, kVl = D * VP, kRowBlocks = kWaves / KS, kTok = 4 * kRowBlocks;
     // two buffers of KS blocks' K and V; then outputs that meet: 64 registers of 8 wavefronts
     __shared__ __attribute__((aligned(16))) char lds[2 * KS * (kKl + kVl)];
-    static_assert(KS == 1 || 2 * KS * (kKl + kVl) >= kWaves * 64 * (64 * 4 + 8), "");
+    static_assert(2 * KS * (kKl + kVl) >= (KS == 1 ? kWaves * 32 * kYP : kWaves * 64 * (64 * 4 + 8)), "room for outputs");
+    static_assert(32 * kYP <= 16384, "half a wavefront's rows where 64 registers of it were");
     auto kl = [&](int buf, int u) { return lds + (buf * KS + u) * kKl; };
     auto vl = [&](int buf, int u) { return lds + 2 * KS * kKl + (buf * KS + u) * kVl; };
     __shared__ int first_nan[D], any_nan;
@@ -317,44 +319,60 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     // (formed again: kept, they took registers from the loop)
     int tl = threadIdx.x;
     asm volatile("" : "+v"(tl));
-    const int hf_ = (tl >> 5) & 1, tok_ = f0 + rblk * 4 + ((tl & 31) >> 3), pos_ = p0 + tok_;
-    const bool live = tok_ < ns, nans = any_nan != 0;
-    const size_t at = (size_t)(t0 + min(tok_, ns - 1)) * nh + kvh * GRP + (tl & 7);
-    // dims 32 i + 8 c + 4 hf .. + 3 of a row: f times what a holds
-    auto store = [&](f32x16 a, int i, float f) __attribute__((always_inline)) {
-        const uint16_t *gate = qg + at * 2 * D + D + 32 * i + 4 * hf_;
-        uint2 gc[4];
+    const int ln = tl & 63, hf_ = ln >> 5, row_ = ln & 31, pos_ = p0 + f0 + rblk * 4 + (row_ >> 3);
+    const bool nans = any_nan != 0;
+    // Half of the dims of the wavefront's rows, from dim d0: f t sigmoid(gate). A lane
+    // holds four dims here and there of one row, so the gates come and y goes as whole
+    // lines through LDS (8.5 KiB of this wavefront's own; straight from the lanes, 16
+    // bytes of 32 rows an instruction, the end of a tile of 32 tokens took 31000 cycles).
+    auto finish = [&](f32x16 (&t)[4], int d0, float f, char *buf) __attribute__((always_inline)) {
+        // chunk j: the row 4 j + ln / 16, so token j / 2
+        auto at = [&](int j) {
+            return (size_t)(t0 + min(f0 + rblk * 4 + j / 2, ns - 1)) * nh + kvh * GRP + j % 2 * 4 + ln / 16;
+        };
+        char *const mine = buf + row_ * kYP + hf_ * 8, *const line = buf + ln / 16 * kYP + ln % 16 * 16;
+        u32x4 gl[8];
 #pragma unroll
-        for (int c = 0; c < 4; c++) gc[c] = *reinterpret_cast<const uint2 *>(gate + 8 * c);
+        for (int j = 0; j < 8; j++) gl[j] = *reinterpret_cast<const u32x4 *>(qg + at(j) * 2 * D + D + d0 + ln % 16 * 8);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            float v[4];
+        for (int j = 0; j < 8; j++) *reinterpret_cast<u32x4 *>(line + j * 4 * kYP) = gl[j];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float gv = bf2f((uint16_t)((e < 2 ? gc[c].x : gc[c].y) >> (16 * (e % 2))));
-                v[e] = a[4 * c + e] * f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
+        for (int i = 0; i < 4; i++) {
+            if (nans) {
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (first_nan[d0 + 32 * i + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) t[i][e] = NAN;
             }
-            if (live)
-                *reinterpret_cast<uint2 *>(y + at * D + 32 * i + 8 * c + 4 * hf_) =
-                    make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
-        }
-    };
-    auto with_nans = [&](f32x16 a, int i) __attribute__((always_inline)) {
-        if (nans) {
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                if (first_nan[32 * i + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) a[e] = NAN;
+            for (int c = 0; c < 4; c++) {
+                u32x2 *const p = reinterpret_cast<u32x2 *>(mine + i * 64 + c * 16);
+                const u32x2 g = *p;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float gv = __uint_as_float(e % 2 ? g[e / 2] & 0xffff0000u : g[e / 2] << 16);
+                    v[e] = t[i][4 * c + e] * f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
+                }
+                *p = u32x2{pack2(v[0], v[1]), pack2(v[2], v[3])};
+            }
         }
-        return a;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (f0 + rblk * 4 + j / 2 < ns)
+                *reinterpret_cast<u32x4 *>(y + at(j) * D + d0 + ln % 16 * 8) = *reinterpret_cast<u32x4 *>(line + j * 4 * kYP);
     };
     if (KS == 1) {
         const float inv = 1.0f / l;
+        char *const buf = lds + wave * 32 * kYP;
 #pragma unroll
-        for (int i = 0; i < 8; i++) store(with_nans(acc[i], i), i, inv);
+        for (int i = 0; i < 2; i++) {
+            f32x16 t[4] = {acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]};
+            finish(t, 128 * i, inv, buf);
+        }
         return;
     }
     // KS 2: two wavefronts have the same rows; each finishes half of the dims
-    float *const os = reinterpret_cast<float *>(lds) + (tl & 63);
+    float *const os = reinterpret_cast<float *>(lds) + ln;
     float2 *const ml = reinterpret_cast<float2 *>(lds + kWaves * 64 * 64 * 4);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -365,19 +383,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Re
     ml[tl] = make_float2(M, l);
     __syncthreads();
     const int other = wave ^ kRowBlocks;
-    const float2 o = ml[other * 64 + (tl & 63)];
+    const float2 o = ml[other * 64 + ln];
     const float m = fmaxf(M, o.x);
     const float fa = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m);
     const float fb = o.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(o.x - m);
     const float inv = 1.0f / (l * fa + o.y * fb);
+    f32x16 t[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        f32x16 t = kg ? acc[4 + i] : acc[i];
+        t[i] = kg ? acc[4 + i] : acc[i];
 #pragma unroll
-        for (int e = 0; e < 16; e++) t[e] = t[e] * fa + os[other * 4096 + (i * 16 + e) * 64] * fb;
-        store(with_nans(t, 4 * kg + i), 4 * kg + i, inv);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 16; e++) t[i][e] = t[i][e] * fa + os[other * 4096 + (i * 16 + e) * 64] * fb;
     }
+    finish(t, 128 * kg, inv, lds + other * 16384);         // (where only this wavefront reads)
 }
 
 // Tokens of a tile, 32 or 16: the time of the busiest CU with either, from a
