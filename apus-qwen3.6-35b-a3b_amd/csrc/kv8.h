@@ -113,8 +113,8 @@ template <bool TOKEN, int N> __device__ __forceinline__ Kv8At kv8_find(const Kv8
     return a;
 }
 
-// Calls f(seqs, first, blocks) for each launch's share of a batch; count(s) is
-// the number of blocks of sequence s. f returns a status.
+// Calls f(seqs) for each launch's share of a batch; count(s) is the number of
+// blocks of sequence s. f may reorder its copy of the entries, and returns a status.
 template <class Count, class F>
 int kv8_launches(size_t B, const int32_t *rows, const int32_t *cu, const int32_t *pos0, Count count, F f) {
     for (size_t s0 = 0; s0 < B; s0 += kKv8Seqs) {
