@@ -617,11 +617,12 @@ int apus_hip_attn_kv8_work_create(const ApusHipAttnLayer *L, size_t max_seqs, si
                          max_seqs, L->nkv, max_pos);
     if (int r = mx_ready()) return r;
     auto *w = new (std::nothrow) ApusHipAttnKv8Work{L->nkv, max_seqs, max_pos, L->rot, L->theta, current_device(),
-                                                    nullptr, nullptr, nullptr, nullptr};
+                                                    nullptr, 0, nullptr, nullptr, nullptr};
     if (!w) return set_error(kErrHip, "out of host memory");
-    // slots: a segment's is pair + run, both below their counts in one launch
-    const size_t slots = std::min<size_t>(max_seqs, kKv8Seqs) * L->nkv + max_runs();
-    const size_t pb = slots * kRows * D * 4, sb = slots * kRows * 8, rb = max_pos * ROT * 2;
+    // decode: a slot of 32 rows a segment, pair + run, both below their counts in one
+    // launch; prefill: 128 rows a part of a tile, two a CU
+    w->rows = std::max((std::min<size_t>(max_seqs, kKv8Seqs) * L->nkv + max_runs()) * kRows, max_runs() * 128);
+    const size_t pb = w->rows * D * 4, sb = w->rows * 8, rb = max_pos * ROT * 2;
     if (hipMalloc((void **)&w->base, pb + sb + rb) != hipSuccess) {
         delete w;
         (void)hipGetLastError();           // (not for the next launch to report)

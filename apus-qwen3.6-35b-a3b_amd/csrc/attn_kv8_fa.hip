@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <functional>
+#include <type_traits>
 
 #include "apus_dev.h"
 #include "apus_host.h"
@@ -41,6 +42,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef kv8_bf16x8 bf16x8;
 typedef kv8_f16x8 f16x8;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
@@ -73,11 +75,13 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 
 typedef const __attribute__((address_space(1))) u32x4 *gu32x4p;
 
-// What the last tile of each sequence of a launch lacks of being full. (The
-// sequences are not in the batch's order, so the entries' cu do not tell.)
-template <int N> struct Short {
-    uint8_t n[N];
+// Of each sequence of a launch: the tokens that its last tile lacks of being full
+// (the sequences are not in the batch's order, so the entries' cu do not tell),
+// and the parts that each tile's keys are cut into.
+template <int N> struct Cut {
+    uint8_t lack[N], parts[N];
 };
+constexpr int kPartRows = 128;               // rows of a part: of a tile of 16 tokens and a kv head
 
 struct Step {
     u32x4 k, v;                              // a thread's pieces of a block
@@ -90,12 +94,15 @@ __device__ __forceinline__ float uni(float x) {
 // KS 1: the 8 wavefronts have 32 rows each, of 32 tokens. KS 2: 16 tokens, and
 // wavefronts w and w + 4 have the same rows, the even and the odd blocks of the
 // keys, and join what they have at the end: half the chain of steps, for calls
-// whose longest tile would take longer than their work spread over the chip.
+// whose longest tile would take longer than their work spread over the chip. If
+// that is not enough a tile's keys go to several workgroups (KS 2 only), which leave
+// outputs, M and sum in slot item - split0 for k_kv8_fa_combine.
 template <int KS, int N>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short<N> lack, Kv8Ref kv, const uint16_t *__restrict__ qg,
+__global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Cut<N> cut, Kv8Ref kv, const uint16_t *__restrict__ qg,
                                                            const uint16_t *__restrict__ qn_w,
                                                            const uint16_t *__restrict__ rope, int nkv,
-                                                           uint16_t *__restrict__ y) {
+                                                           uint16_t *__restrict__ y, int split0,
+                                                           float *__restrict__ part, float2 *__restrict__ stat) {
     constexpr int kKl = KEYS * KP, kVl = D * VP, kRowBlocks = kWaves / KS, kTok = 4 * kRowBlocks;
     // two buffers of KS blocks' K and V; then outputs that meet: 64 registers of 8 wavefronts
     __shared__ __attribute__((aligned(16))) char lds[2 * KS * (kKl + kVl)];
@@ -108,10 +115,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rblk = wave % kRowBlocks, kg = wave / kRowBlocks;
     const int kvh = blockIdx.x % nkv, item = ((int)gridDim.x - 1 - (int)blockIdx.x) / nkv;
     const Kv8At a = kv8_find<false>(sq, item);
-    const int t0 = a.t0, ns = a.blocks * kTok - lack.n[a.s], p0 = a.p0, row = a.row, nh = nkv * GRP;
-    const int f0 = (item - a.off) * kTok;                  // the tile's first token in its sequence
+    const int parts = KS == 1 ? 1 : cut.parts[a.s], tile = (item - a.off) / parts, pt = (item - a.off) % parts;
+    const int t0 = a.t0, ns = a.blocks / parts * kTok - cut.lack[a.s], p0 = a.p0, row = a.row, nh = nkv * GRP;
+    const int f0 = tile * kTok;                            // the tile's first token in its sequence
     const int end = p0 + min(f0 + kTok, ns);               // keys that some row sees
-    const int ctx = p0 + ns, nb = (end + KEYS - 1) / KEYS, steps = (nb + KS - 1) / KS;
+    const int ctx = p0 + ns, nbt = (end + KEYS - 1) / KEYS;
+    // this workgroup's blocks (none, where a tile has fewer than parts)
+    const int b0 = nbt * pt / parts, nb = nbt * (pt + 1) / parts, steps = (nb - b0 + KS - 1) / KS, last = KS == 1 ? nb - 1 : max(nb - 1, 0);
     if (tid < D) first_nan[tid] = 0x7fffffff;
     if (tid == 0) any_nan = 0;
 
@@ -128,13 +138,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
     };
     uint32_t id[KS];
 #pragma unroll
-    for (int u = 0; u < KS; u++) id[u] = id_of(min(u, nb - 1));
+    for (int u = 0; u < KS; u++) id[u] = id_of(min(b0 + u, last));
     auto fetch = [&](int st, int u) {
         const size_t hb = (size_t)min((uint32_t)__builtin_amdgcn_readfirstlane(id[u]), kv.blocks - 1) * nkv + kvh;
         next.k = *(gu32x4p)(kv.k + hb * kKv8Bytes + tid16);
         next.v = *(gu32x4p)(kv.v + hb * kKv8Bytes + tid16);
         next.sc = *(const __attribute__((address_space(1))) f32x2 *)((const char *)(kv.scale + hb * 2) + zero);
-        id[u] = id_of(min((st + 1) * KS + u, nb - 1));
+        id[u] = id_of(min(b0 + (st + 1) * KS + u, last));
     };
     // a thread's pieces (kv8.h) to their places in LDS
     float cs = 0.0f;                                       // the scale of this wavefront's K
@@ -143,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
         char *const kd = kl(buf, u) + (tid / 256 * 16 + tid % 16) * KP + tid / 16 % 16 * 32;
         *reinterpret_cast<f16x8 *>(kd) = kv8_f16(next.k[0], next.k[1]);
         *reinterpret_cast<f16x8 *>(kd + 16) = kv8_f16(next.k[2], next.k[3]);
-        const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16, b = st * KS + u;
+        const int g = tid / 16 % 4, d = tid / 64 * 32 + tid % 16, b = b0 + st * KS + u;
         u32x4 c4 = next.v;
         const int k0 = b * KEYS + g * 4;               // the piece's keys: k0 .. + 3 and 16 on
         if ((b + 1) * KEYS > p0 + f0) {                // some row does not see some key
@@ -245,14 +255,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
     float M = -INFINITY, l = 0.0f;
     const int wfirst = p0 + min(f0 + rblk * 4, ns - 1), wlast = p0 + min(f0 + rblk * 4 + 3, ns - 1);
     for (int st = 0; st < steps; st++) {
-        const int buf = st & 1, k0 = (st * KS + kg) * KEYS;
+        const int buf = st & 1, k0 = (b0 + st * KS + kg) * KEYS;
         const float csn = cs;
         fetch(min(st + 1, steps - 1), 0);
         __syncthreads();
         bf16x8 pb[2];
         const char *vp = vl(buf, kg) + n * VP + hf * 16;
         auto v_of = [&](int i) { return *reinterpret_cast<const bf16x8 *>(vp + i % 8 * 32 * VP + i / 8 * 32); };
-        const bool work = k0 <= wlast;
+        const bool work = k0 <= wlast && (KS == 1 || k0 < nb * KEYS);
         if (work) {                                        // (wave-uniform)
             f32x16 S;
 #pragma unroll
@@ -327,6 +337,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
     asm volatile("" : "+v"(tl));
     const int ln = tl & 63, hf_ = ln >> 5, row_ = ln & 31, pos_ = p0 + f0 + rblk * 4 + (row_ >> 3);
     const bool nans = any_nan != 0;
+    auto with_nans = [&](f32x16 &t, int d) __attribute__((always_inline)) {
+        if (nans) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (first_nan[d + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) t[e] = NAN;
+        }
+    };
     // Half of the dims of the wavefront's rows, from dim d0: f t sigmoid(gate). A lane
     // holds four dims here and there of one row, so the gates come and y goes as whole
     // lines through LDS (8.5 KiB of this wavefront's own; straight from the lanes, 16
@@ -344,11 +361,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
         for (int j = 0; j < 8; j++) *reinterpret_cast<u32x4 *>(line + j * 4 * kYP) = gl[j];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (nans) {
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (first_nan[d0 + 32 * i + e / 4 * 8 + 4 * hf_ + e % 4] <= pos_) t[i][e] = NAN;
-            }
+            with_nans(t[i], d0 + 32 * i);
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 u32x2 *const p = reinterpret_cast<u32x2 *>(mine + i * 64 + c * 16);
@@ -393,7 +406,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
     const float m = fmaxf(M, o.x);
     const float fa = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - m);
     const float fb = o.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(o.x - m);
-    const float inv = 1.0f / (l * fa + o.y * fb);
     f32x16 t[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -401,64 +413,188 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Short
 #pragma unroll
         for (int e = 0; e < 16; e++) t[i][e] = t[i][e] * fa + os[other * 4096 + (i * 16 + e) * 64] * fb;
     }
-    finish(t, 128 * kg, inv, lds + other * 16384);         // (where only this wavefront reads)
+    if (parts > 1) {                                       // as they lie in the lanes: whole KiB
+        const size_t slot = (size_t)(item - split0) * nkv + kvh;
+        float *const p = part + (slot * kWaves + wave) * 4096 + ln * 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            with_nans(t[i], 128 * kg + 32 * i);
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                *reinterpret_cast<f32x4 *>(p + (i * 4 + c) * 256) =
+                    f32x4{t[i][4 * c], t[i][4 * c + 1], t[i][4 * c + 2], t[i][4 * c + 3]};
+        }
+        if (wave < kRowBlocks && hf_ == 0) stat[slot * kPartRows + rblk * 32 + row_] = make_float2(m, l * fa + o.y * fb);
+        return;
+    }
+    finish(t, 128 * kg, 1.0f / (l * fa + o.y * fb), lds + other * 16384);      // (where only this wavefront reads)
+}
+
+// Joins the parts of the split tiles. A wavefront, or SP of them with parts apart,
+// has 1 KiB of each part: four dims of 32 rows and two lane halves. sq: off counts
+// tiles, pos0 is the number of parts and row the first slot.
+template <int SP, int N>
+__global__ __launch_bounds__(256) void k_kv8_fa_combine(Kv8SeqsN<N> sq, Cut<N> cut, const float *__restrict__ part,
+                                                        const float2 *__restrict__ stat,
+                                                        const uint16_t *__restrict__ qg, int nkv,
+                                                        uint16_t *__restrict__ y) {
+    constexpr int kTok = 16, kTasks = 128 * SP / 4;        // workgroups a tile and kv head
+    const int ln = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wv % SP;
+    const int kvh = blockIdx.x / kTasks % nkv, g = blockIdx.x / kTasks / nkv;
+    const int task = (int)(blockIdx.x % kTasks) * (4 / SP) + wv / SP, w = task / 16, ch = task % 16;
+    const Kv8At a = kv8_find<false>(sq, g);
+    const int parts = a.p0, tile = g - a.off, ns = a.blocks * kTok - cut.lack[a.s];
+    const int r = w % 4 * 32 + (ln & 31), tok = tile * kTok + r / 8;
+    const int d = w / 4 * 128 + ch / 4 * 32 + ch % 4 * 8 + ln / 32 * 4;
+    const size_t at = (size_t)(a.t0 + min(tok, ns - 1)) * nkv * GRP + kvh * GRP + r % 8;
+    const uint2 gate = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
+    const size_t slot0 = (size_t)(a.row + tile * parts) * nkv + kvh;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = share; j < parts; j += 8 * SP) {
+        f32x4 v[8];
+        float2 u[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const size_t s = slot0 + (size_t)min(j + i * SP, parts - 1) * nkv;
+            v[i] = *reinterpret_cast<const f32x4 *>(part + (s * kWaves + w) * 4096 + ch * 256 + ln * 4);
+            u[i] = stat[s * kPartRows + r];
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mn = fmaxf(mn, u[i].x);
+        const float k = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= k;
+        o *= k;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (j + i * SP >= parts) continue;
+            const float f = u[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(u[i].x - m);   // (0 keeps a NaN)
+            l += u[i].y * f;
+            o += v[i] * f;
+        }
+    }
+    if (SP > 1) {
+        __shared__ f32x4 os[4][64];
+        __shared__ float2 st[4][64];
+        os[wv][ln] = o;
+        st[wv][ln] = make_float2(m, l);
+        __syncthreads();
+        if (share) return;
+        float mt = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < SP; i++) mt = fmaxf(mt, st[wv + i][ln].x);
+        l = 0.0f;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < SP; i++) {
+            const float2 u = st[wv + i][ln];
+            const float f = u.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(u.x - mt);
+            l += u.y * f;
+            o += os[wv + i][ln] * f;
+        }
+    }
+    if (tok >= ns) return;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float gv = bf2f((uint16_t)((e < 2 ? gate.x : gate.y) >> (16 * (e % 2))));
+        o[e] *= inv * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-gv * kL2E));
+    }
+    *reinterpret_cast<uint2 *>(y + at * D + d) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
+}
+
+// How a call is cut: tokens of a tile, and blocks of a part (0: tiles are whole).
+struct Plan {
+    int tok;
+    int32_t len;
+};
+constexpr int kMostParts = 64;
+int parts_of(const Plan &p, int32_t end) {
+    const int32_t blocks = (end + KEYS - 1) / KEYS;
+    return p.len ? std::min((blocks + p.len - 1) / p.len, (int32_t)kMostParts) : 1;
 }
 
 // Puts a launch's sequences in the order of their ends: its tiles start with the
 // last, so the longest go first (6 ragged prompts: 105 us in the batch's order,
-// 93 so).
-template <int N> Short<N> by_length(Kv8SeqsN<N> &q, int tok) {
+// 93 so), and those with several parts are the last entries.
+template <int N> Cut<N> by_length(Kv8SeqsN<N> &q, const Plan &p) {
     struct {
         Kv8Seq e;
         int32_t n;
     } s[N];
-    Short<N> lack = {};
+    Cut<N> cut = {};
     for (int i = 0; i < q.n; i++) s[i] = {q.e[i], q.e[i + 1].cu - q.e[i].cu};
     std::sort(s, s + q.n, [](const auto &a, const auto &b) { return a.e.pos0 + a.n < b.e.pos0 + b.n; });
     int32_t off = 0;
     for (int i = 0; i < q.n; i++) {
-        const int32_t tiles = (s[i].n + tok - 1) / tok;
+        const int32_t tiles = (s[i].n + p.tok - 1) / p.tok, parts = parts_of(p, s[i].e.pos0 + s[i].n);
         q.e[i] = s[i].e;
         q.e[i].off = off;
-        lack.n[i] = (uint8_t)(tiles * tok - s[i].n);
-        off += tiles;
+        cut.lack[i] = (uint8_t)(tiles * p.tok - s[i].n);
+        cut.parts[i] = (uint8_t)parts;
+        off += tiles * parts;
     }
-    return lack;
+    q.e[q.n].off = off;
+    return cut;
 }
 
-// Tokens of a tile, 32 or 16: the time of the busiest CU with either, from a
-// tile's alone on a CU (us; 20 + 1.37 a block of keys with 32 tokens, 17.5 + 0.86
-// with 16), tiles dealt longest first: the longest, all of them over the CUs, and
-// where a few more tiles than CUs remain, the two that share a CU. Measured (us,
-// 32 / 16 tokens): one prompt of 256 33 / 25, 1024 67 / 46, 4096 206 / 165, 6000
-// 321 / 345; 512 tokens after 8000 377 / 236; 8 times 300 after 300 53 / 65, 500
-// after 4000 273 / 312.
-int fa_tokens(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv) {
+// The plan of least time by the time of the busiest CU, from a tile's alone on a
+// CU (us; 16 + 1.38 a block of keys with 32 tokens, 15.5 + 0.83 with 16; its
+// products at the clock of a full chip), tiles dealt longest first: the longest, all of them
+// over the CUs, and where a few more than CUs remain, the two that share a CU. Parts
+// cost a start and an end each and the launch that joins them.
+Plan fa_plan(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv, size_t slots) {
     const size_t cus = (size_t)cu_count();
-    auto busiest = [&](int tok, double base, double per) {
-        size_t tiles = 0;
+    int32_t end = 0;
+    auto busiest = [&](const Plan &p, double base, double per, double full) {
+        size_t items = 0, split = 0;
         double sum = 0.0, longest = 0.0;
         for (size_t s = 0; s < B; s++) {
             const int64_t n = cu[s + 1] - cu[s];
             if (!n) continue;
-            const size_t t = (size_t)((n + tok - 1) / tok) * nkv;
-            tiles += t;
-            longest = std::max(longest, base + per * (double)(pos0[s] + n) / KEYS);
-            sum += (double)t * (base + per * ((double)pos0[s] + (double)(n + tok) / 2) / KEYS);
+            const int parts = parts_of(p, pos0[s] + (int32_t)n);
+            const size_t t = (size_t)((n + p.tok - 1) / p.tok) * nkv;
+            items += t * (size_t)parts;
+            if (parts > 1) split += t * (size_t)parts;
+            longest = std::max(longest, base + per * (double)(pos0[s] + n) / KEYS / parts);
+            sum += (double)t * (base * parts + per * ((double)pos0[s] + (double)(n + p.tok) / 2) / KEYS);
         }
-        double us = std::max(longest, sum / (double)cus);
+        if (split > slots) return 1e30;
+        sum /= (double)cus;
+        const double load = 1.0 + 0.15 * std::min(1.0, sum / longest);
+        double us = std::max(longest * load, sum * full);
         double t[1024];
-        if (tiles > cus && tiles <= std::min<size_t>(2 * cus, 1024)) {
+        if (items > cus && items <= std::min<size_t>(2 * cus, 1024)) {
             double *e = t;
-            for (size_t s = 0; s < B; s++)
-                for (int64_t n = cu[s + 1] - cu[s], x = 0; x < n; x += tok, e += nkv)
-                    std::fill_n(e, nkv, base + per * (double)(pos0[s] + std::min<int64_t>(x + tok, n)) / KEYS);
+            for (size_t s = 0; s < B; s++) {
+                const int64_t n = cu[s + 1] - cu[s];
+                const int parts = n ? parts_of(p, pos0[s] + (int32_t)n) : 1;
+                for (int64_t x = 0; x < n; x += p.tok, e += nkv * (size_t)parts)
+                    std::fill_n(e, nkv * (size_t)parts,
+                                base + per * (double)(pos0[s] + std::min<int64_t>(x + p.tok, n)) / KEYS / parts);
+            }
             std::nth_element(t, t + cus, e, std::greater<double>());
-            us = std::max(us, 2.0 * t[cus]);
+            us = std::max(us, 2.0 * t[cus] * load);
         }
-        return us;
+        return us + (split ? 6.0 + 0.05 * (double)split : 0.0);
     };
-    return busiest(16, 17.5, 0.86) < busiest(32, 20.0, 1.37) ? 16 : 32;
+    for (size_t s = 0; s < B; s++)
+        if (cu[s + 1] > cu[s]) end = std::max(end, pos0[s] + cu[s + 1] - cu[s]);
+    Plan best = {32, 0};
+    double us = busiest(best, 16.0, 1.38, 1.26);
+    for (const int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        const int32_t len = k == 1 ? 0 : (end + KEYS - 1) / KEYS / k;
+        if (k > 1 && (len < 2 || B > (size_t)kKv8Seqs)) break;
+        const Plan p = {16, len};
+        const double t = busiest(p, 15.5, 0.83, 1.18);
+        if (t < us) {
+            us = t;
+            best = p;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -477,21 +613,47 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
     const size_t nkv = L->nkv;
     if (k)
         if (int e = kv8_append_run(r, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
-    const int tok = fa_tokens(B, cu, pos0, nkv);
-    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + tok - 1) / tok; },
+    const Plan plan = fa_plan(B, cu, pos0, nkv, w->rows / kPartRows);
+    return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + plan.tok - 1) / plan.tok; },
                         [&](auto &q) {
         constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
-        const Short<N> lack = by_length(q, tok);
+        if (!q.e[q.n].off) return (int)kOk;
+        const Cut<N> cut = by_length(q, plan);
         const size_t grid = (size_t)q.e[q.n].off * nkv;
-        if (!grid) return (int)kOk;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
-        if (tok == 32)
-            APUS_TIMED("k_kv8_fa", k_kv8_fa<1, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
-                                       q, lack, r, qg, L->qn_w, w->rope, (int)nkv, y));
-        else
-            APUS_TIMED("k_kv8_fa", k_kv8_fa<2, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
-                                       q, lack, r, qg, L->qn_w, w->rope, (int)nkv, y));
-        return launch_check("k_kv8_fa");
+        int first = 0;                                     // the first sequence of several parts
+        while (first < q.n && cut.parts[first] == 1) first++;
+        const int split0 = q.e[first].off;
+        auto launch = [&](auto ks) {
+            APUS_TIMED("k_kv8_fa", k_kv8_fa<decltype(ks)::value, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
+                                       q, cut, r, qg, L->qn_w, w->rope, (int)nkv, y, split0, w->part, w->stat));
+            return launch_check("k_kv8_fa");
+        };
+        if (plan.tok == 32) return launch(std::integral_constant<int, 1>{});
+        if (int e = launch(std::integral_constant<int, 2>{})) return e;
+        if (split0 == q.e[q.n].off) return (int)kOk;
+        // the split sequences, in tiles
+        Kv8SeqsN<N> sq;
+        Cut<N> scut = {};
+        sq.n = q.n - first;
+        int32_t off = 0, most = 1;
+        for (int i = 0; i < sq.n; i++) {
+            const Kv8Seq &e = q.e[first + i];
+            const int32_t parts = cut.parts[first + i];
+            sq.e[i] = Kv8Seq{off, e.cu, parts, e.off - split0};
+            scut.lack[i] = cut.lack[first + i];
+            off += (q.e[first + i + 1].off - e.off) / parts;
+            most = std::max(most, parts);
+        }
+        for (int i = sq.n; i <= N; i++) sq.e[i] = Kv8Seq{i == sq.n ? off : 0x7fffffff, 0x7fffffff, 0, 0};
+        auto combine = [&](auto sp) {
+            constexpr int SP = decltype(sp)::value;
+            APUS_TIMED("k_kv8_fa_combine",
+                       k_kv8_fa_combine<SP, N><<<(unsigned)((size_t)off * nkv * 32 * SP), 256, 0, stream()>>>(
+                           sq, scut, w->part, w->stat, qg, (int)nkv, y));
+            return launch_check("k_kv8_fa_combine");
+        };
+        return most <= 8 ? combine(std::integral_constant<int, 1>{}) : combine(std::integral_constant<int, 4>{});
     });
 }
 

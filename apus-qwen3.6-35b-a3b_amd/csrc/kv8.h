@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t kv8_id_u(const Kv8Ref &r, int h, int b) {
 // launch is shorter. Entry i: the blocks (in the kernel's count) and tokens
 // before sequence i, its cached positions and its row; entry n has the totals,
 // entries past it none that is ever found.
-constexpr int kKv8Seqs = 224, kKv8FewSeqs = 8;
+constexpr int kKv8Seqs = 208, kKv8FewSeqs = 8;     // (a kernel's arguments within 4 KiB)
 struct Kv8Seq {
     int32_t off, cu, pos0, row;
 };
@@ -215,7 +215,8 @@ struct ApusHipAttnKv8Work {
     double theta;
     int device;
     char *base;
-    float *part;                             // [slot][32 rows][256]
-    float2 *stat;                            // [slot][32 rows]: reference point, sum
+    size_t rows;                             // of partial results
+    float *part;                             // [row][256]
+    float2 *stat;                            // [row]: reference point, sum
     uint16_t *rope;                          // [max_pos][64] cos, sin
 };

@@ -231,7 +231,7 @@ def test_decode_many_sequences(hip, tq):
     rng = np.random.default_rng(tq)
     ctx = rng.integers(0, 150, 461)
     s = Setup(hip, 7 + tq, 2, ctx, rng.integers(0, tq + 1, 461), True)
-    s.check(s.call(hip.attn_decode_kv8), list(range(0, 461, 9)) + [222, 223, 224, 225, 447, 448, 449, 460])
+    s.check(s.call(hip.attn_decode_kv8), list(range(0, 461, 9)) + [206, 207, 208, 209, 222, 223, 224, 225, 415, 416, 447, 448, 449, 460])
 
 
 def test_decode_growing_scores(hip):
@@ -366,6 +366,36 @@ def test_prefill(hip, ctx, new, nkv, paged):
     s.check(s.call(hip.attn_prefill_kv8))
 
 
+@pytest.mark.parametrize("ctx,new,nkv,paged", [
+    ([5000], [3], 2, True), ([9000], [40], 1, False), ([30000], [1], 2, True), ([5000, 40, 1200, 700], [3, 20, 17, 0], 2, True),
+    ([0, 3000], [700, 5], 1, False), ([0], [1000], 1, True), ([6000] * 9, [1, 2, 15, 16, 17, 1, 0, 33, 8], 3, True)])
+def test_prefill_split(hip, ctx, new, nkv, paged):
+    """Few new tokens after long contexts: a tile's keys in several parts, of which
+    a prompt's first tiles have fewer than the last; rows see NaN by position."""
+    s = Setup(hip, 80 + len(ctx) + new[0], nkv, ctx, new, paged)
+    y = s.call(hip.attn_prefill_kv8)
+    s.check(y)
+    q = int(np.argmax(s.ctx))
+    n = int(s.ctx[q] + s.new[q])
+    c = cum(s.ctx + s.new)
+    v = s.v[c[q]:c[q + 1]].copy()
+    at = [n // 2, n - 1]                                   # dims 5 and 250 of the last head
+    v[at[0], -R.D + 5], v[at[1], -R.D + 250] = 0x7fc0, 0xff80
+    hip.kv8_append(s.kv, [s.row(q)], [0, n], [0], dev(s.k[c[q]:c[q + 1]]), dev(v))
+    bad = np.zeros(y.shape, bool)
+    for t in range(int(s.new[q])):
+        for d, a in ((5, at[0]), (250, at[1])):
+            bad[s.cu[q] + t, -R.GRP:, d] = s.ctx[q] + t >= a
+    z = s.call(hip.attn_prefill_kv8)
+    assert np.array_equal(np.isnan(R.f64(z)), bad)
+    v[at, [-R.D + 5, -R.D + 250]] = 0
+    s.ref.append(s.row(q), 0, s.k[c[q]:c[q + 1]], v)
+    kk, vv = s.ref.values(s.row(q), 0, n)
+    sl = slice(s.cu[q], s.cu[q + 1])
+    r, tol = R.attention(s.qg[sl], s.w["qn_w"], int(s.ctx[q]), kk, vv, THETA)
+    assert (np.abs(R.f64(z[sl]) - r) <= tol)[~bad[sl]].all()
+
+
 @pytest.mark.parametrize("nkv,nan", [(2, None), (3, "k"), (2, "v")])
 def test_prefill_many_tokens(hip, nkv, nan):
     """Work for every CU many times over (tiles of 32 tokens): ragged sequences;
@@ -411,7 +441,7 @@ def test_prefill_many_tokens(hip, nkv, nan):
 def test_prefill_many_sequences(hip):
     rng = np.random.default_rng(9)
     s = Setup(hip, 71, 1, rng.integers(0, 60, 230), rng.integers(0, 6, 230), True)
-    s.check(s.call(hip.attn_prefill_kv8), list(range(0, 230, 11)) + [223, 224, 229])
+    s.check(s.call(hip.attn_prefill_kv8), list(range(0, 230, 11)) + [206, 207, 208, 209, 223, 224, 229])
 
 
 def test_pool(hip):
