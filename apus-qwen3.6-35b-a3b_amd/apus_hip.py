@@ -1080,36 +1080,40 @@ def block_norm_weights(hidden, w_pre=None, w_post=None, gate=None, scale=1.0, ep
     return N
 
 
-def _f32_rows(t, what, dev, ncols):
-    import torch
-    if t.dim() != 2 or t.get_device() != dev or t.dtype != torch.float32 or t.shape[1] != ncols or (
-            t.stride(1) != 1 and ncols > 1 and t.shape[0]):
-        raise ValueError(f"{what}: a 2-D tensor of fp32 rows of {ncols} on GPU {dev}, not {tuple(t.shape)} "
-                         f"{t.dtype} on {t.device}")
-    return t.data_ptr(), t.shape[0], ncols, t.stride(0) if t.shape[0] > 1 else ncols
+def _norm_rows(t, what, shape, f32):
+    """(pointer, pitch) of bf16 or fp32 rows of that shape."""
+    if t.get_device() != _device or t.shape != shape or (
+            t.element_size() != 4 or not t.is_floating_point() if f32 else t.dtype not in _BF16 and not _bf16(t)):
+        raise ValueError(f"{what}: a tensor of {'fp32' if f32 else 'bf16'} rows of shape {tuple(shape)} on GPU {_device}, "
+                         f"not {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.is_contiguous():
+        return t.data_ptr(), shape[1]
+    ld, one = t.stride()
+    if one != 1 and shape[1] > 1:
+        raise ValueError(f"{what}: elements of a row must be contiguous")
+    return t.data_ptr(), ld if shape[0] > 1 else shape[1]
 
 
 def block_norm(norm, y, h, h_out, x):
     """h_out = h + scale gate post(y), x = pre(h_out): y, x [T, hidden] bf16, h
     and h_out bf16 or fp32, rows of any pitch. y None: x = pre(h); x None: only
-    h_out. h_out may be h, x may be y."""
-    dev, n = _device, norm.hidden
-    f32 = h.element_size() == 4
-    hp, T, _, ldh = _f32_rows(h, "h", dev, n) if f32 else _rows(h, "h", dev, n)
-    args = []
-    for t, what in ((y, "y"), (h_out, "h_out"), (x, "x")):
-        if t is None:
-            args.append((None, n))
-            continue
-        p, m, _, ld = _f32_rows(t, what, dev, n) if f32 and what == "h_out" else _rows(t, what, dev, n)
-        if m != T:
-            raise ValueError(f"{what}: {m} rows, expected {T}")
-        args.append((p, ld))
+    h_out. h_out may be h, x may be y. (norm takes up h's type: one norm is not for
+    two threads with h of different types.)"""
+    shape, n = h.shape, norm.hidden
+    if len(shape) != 2 or shape[1] != n:
+        raise ValueError(f"h: rows of {n} elements, not {tuple(shape)}")
+    T = shape[0]
     if norm._gate_rows is not None and norm._gate_rows != T:
         raise ValueError(f"gate: {norm._gate_rows} rows, expected {T}")
-    norm.h_f32 = int(f32)
-    (yp, ldy), (op, ldo), (xp, ldx) = args
-    _chk(load().apus_hip_block_norm(C.addressof(norm), T, yp, ldy, hp, ldh, op, ldo, xp, ldx))
+    f32 = h.element_size() == 4
+    hp, ldh = _norm_rows(h, "h", shape, f32)
+    yp, ldy = (None, n) if y is None else _norm_rows(y, "y", shape, False)
+    op, ldo = (None, n) if h_out is None else _norm_rows(h_out, "h_out", shape, f32)
+    xp, ldx = (None, n) if x is None else _norm_rows(x, "x", shape, False)
+    norm.h_f32 = f32
+    rc = load().apus_hip_block_norm(C.addressof(norm), T, yp, ldy, hp, ldh, op, ldo, xp, ldx)
+    if rc:
+        raise ApusHipError(rc, last_error())
 
 
 # ---- named-intermediate capture

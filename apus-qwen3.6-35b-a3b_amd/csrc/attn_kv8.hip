@@ -396,13 +396,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
 // SP wavefronts a (token, head) of a pair that lies in several runs, each with
 // its share of the segments, 8 loads at a time.
 template <int SP, int N>
-__global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float *__restrict__ part,
+__global__ __launch_bounds__(64 * (SP > 4 ? SP : 4)) void k_kv8_combine(Kv8SeqsN<N> sq, const float *__restrict__ part,
                                                      const float2 *__restrict__ stat,
                                                      const uint16_t *__restrict__ qg, int nkv, int run, int items,
                                                      uint16_t *__restrict__ y) {
     const int lane = threadIdx.x & 63, d = lane * 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave % SP;
-    const int item = min((int)blockIdx.x * (4 / SP) + wave / SP, items - 1);   // (the last again: the same y)
+    constexpr int W = SP > 4 ? SP : 4;
+    const int item = min((int)blockIdx.x * (W / SP) + wave / SP, items - 1);   // (the last again: the same y)
     const int nh = nkv * GRP, h = item % nh, tt = sq.e[0].cu + item / nh;
     const Kv8At a = kv8_find<true>(sq, tt);
     const int kvh = h / GRP, r = (tt - a.t0) * GRP + h % GRP;
@@ -440,8 +441,8 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8SeqsN<N> sq, const float
         }
     }
     if (SP > 1) {
-        __shared__ f32x4 os[4][64];
-        __shared__ float2 st[4];
+        __shared__ f32x4 os[W][64];
+        __shared__ float2 st[W];
         os[wave][lane] = o;
         if (lane == 0) st[wave] = make_float2(m, l);
         __syncthreads();
@@ -574,12 +575,14 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
         const size_t items = (size_t)(q.e[q.n].cu - q.e[0].cu) * L->nh;
         auto combine = [&](auto sp) {
             constexpr int SP = decltype(sp)::value;
+            constexpr int W = SP > 4 ? SP : 4;
             APUS_TIMED("k_kv8_combine",
-                       k_kv8_combine<SP, N><<<cdiv(items, 4 / SP), 256, 0, stream()>>>(
+                       k_kv8_combine<SP, N><<<cdiv(items, W / SP), 64 * W, 0, stream()>>>(
                            q, w->part, w->stat, qg, (int)nkv, (int)run, (int)items, y));
         };
         if (segs <= 8) combine(std::integral_constant<int, 1>{});
-        else combine(std::integral_constant<int, 4>{});
+        else if (segs <= 32) combine(std::integral_constant<int, 4>{});
+        else combine(std::integral_constant<int, 16>{});
         return launch_check("k_kv8_combine");
     });
 }
