@@ -7,21 +7,28 @@
 // The 8 q heads of a kv head times up to 4 new tokens are the rows of the matrix
 // products, one or two blocks of 16, so K and V come from HBM once a (sequence, kv
 // head) pair. The pairs' blocks are laid end to end and cut into equal runs, one
-// a workgroup and as many as CUs, so that every CU reads as much however ragged
-// the contexts are; a run that crosses a pair's border is two segments. The 8
-// wavefronts of a workgroup take a segment's blocks in turn (with two row blocks,
-// pairs of wavefronts, a row block each: both blocks' outputs and operands would
-// not fit the registers of two wavefronts a SIMD), each with its own M, sum and
-// outputs in registers, and meet in LDS at its end. A segment that is a whole
-// pair writes y; others keep (M, sum, outputs) of their rows in slot pair + run
-// (no two segments share one), and k_kv8_combine joins them.
+// a workgroup and at most two a CU, so that every CU reads as much however ragged
+// the contexts are; a run that crosses a pair's border is two segments. The 4
+// wavefronts of a workgroup take a segment's blocks in turn, each with its own M,
+// sum and outputs of all rows in registers, and meet in LDS at its end. A segment
+// that is a whole pair writes y; others keep (M, sum, outputs) of their rows in slot
+// pair + run (no two segments share one), and k_kv8_combine joins them.
 //
-// A wavefront has no LDS traffic in its loop: K's and V's bytes come in operand
-// order (16-byte loads, whole KiB), widen in registers (exactly: K's codes to fp16,
-// V's times their scale to bf16), and the scores' registers are the operand of
-// P V. Probabilities go to bf16 for that product (fp16 would cut those far below
-// the largest), and their sum is that of the rounded ones: y is a mean of v with
+// A wavefront has no LDS traffic for K and V: their bytes come in operand order
+// (16-byte loads, whole KiB), widen in registers (exactly: K's codes to fp16, V's
+// times their scale to bf16), and the scores' registers are the operand of P V.
+// Probabilities go to bf16 for that product (fp16 would cut those far below the
+// largest), and their sum is that of the rounded ones: y is a mean of v with
 // weights that add up to 1, and a single large weight brings no error.
+//
+// Bound by HBM where contexts are long: 64 sequences at 32768 with 2 kv heads, 2.15
+// GB in 328 us, 6.5 TB/s (a pure read stream reaches 7.0; with loads that stay in
+// the caches 361 us); 128 ragged ones verifying 1-4 tokens, 1.36 GB in 237 us,
+// 5.7 TB/s (two row blocks: each block of K and V is worked on for twice as long
+// and K's next loads wait for the scores, else the registers spill; wavefronts in
+// pairs that share the keys, a row block each, 291 us). Few sequences: the chain of
+// a segment, 9 us of launch, block ids, q rows and first loads, the end 4 us, and
+// the second launch (one sequence, 3 tokens at 60001, 61 MB: 27 us).
 #include <math.h>
 #include <stdint.h>
 
@@ -103,7 +110,7 @@ __device__ __forceinline__ uint2 finish(f32x4 o, float l, uint2 gate) {
 }
 
 // RB: row blocks, 2 where a sequence has more than two new tokens; their q rows
-// then stay in LDS.
+// then stay in LDS, and come from there once a block of keys.
 template <int RB, int N>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
     Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg, const uint16_t *__restrict__ qn_w,
@@ -394,7 +401,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
 }
 
 // SP wavefronts a (token, head) of a pair that lies in several runs, each with
-// its share of the segments, 8 loads at a time.
+// its share of the segments, 8 loads at a time: up to 8 segments one wavefront, up
+// to 32 four, else 16, so that a call of few tokens takes one or two rounds of loads
+// (one sequence of 3 tokens at 60001, 126 segments: 28.6 us in all with 4 wavefronts,
+// 26.8 with 16). Bound by the latency of its rounds: 3 to 6 us.
 template <int SP, int N>
 __global__ __launch_bounds__(64 * (SP > 4 ? SP : 4)) void k_kv8_combine(Kv8SeqsN<N> sq, const float *__restrict__ part,
                                                      const float2 *__restrict__ stat,
@@ -477,7 +487,7 @@ int32_t ctx_blocks(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n + KEYS - 
 // 32; 64 equal ones 330, 330, 332, 335), which also keeps two segments out of one
 // short run. Runs have a block for each wavefront at least, and grow with the
 // total as its root, up to 16, since every run costs the second launch a partial
-// result (one sequence at 60000 with 3 tokens: 31 us with runs of 8, 28 with 15).
+// result (one sequence at 60001: 19 us with runs of 15, 22 with 11 and 21 with 8).
 constexpr int32_t kPad = 8, kShort = 24, kShortMany = 96;
 size_t max_runs() { return 2 * (size_t)cu_count(); }
 int32_t whole_pairs(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv) {

@@ -1,16 +1,27 @@
 // attn_kv8_fa.hip -- gated-GQA attention of any number of new tokens a sequence
 // over the 8-bit KV cache (kv8.h), the formula of attn_kv8.hip.
 //
-// One workgroup a (tile of 32 or 16 tokens, kv head), the last tiles first: the
-// 8 q heads times 32 tokens are 256 rows, 32 a wavefront, whose q and outputs
-// stay in registers. The keys are walked once, a block at a time, with a running
-// reference point M and sum of the softmax: a tile's codes go from
-// memory to registers while the tile before is worked on, widen there (exactly: K's
-// codes to fp16, V's times their scale to bf16) and come into LDS in operand order. The
-// products run on the 32x32x16 MFMA with keys (or dims) on the M side:
-// S^T = K Q^T leaves each lane 16 scores of one row, which are the operand of
-// O^T += V^T P^T with no exchange, if V's keys are laid out in the same order:
-// lane half h takes the keys 8 q + 4 h + 0..3, q = 0..3, 8 a step.
+// One workgroup a (tile of 32 or 16 tokens, kv head), the longest first: the 8 q
+// heads times 32 tokens are 256 rows, 32 a wavefront, whose q and outputs stay in
+// registers. The keys are walked once, a block at a time, with a running reference
+// point M and sum of the softmax. A block's codes go from memory to registers while
+// the block before is worked on, widen there (exactly: K's codes to fp16, V's times
+// their scale to bf16) and come into LDS in operand order. The products run on the
+// 32x32x16 MFMA with keys (or dims) on the M side: S^T = K Q^T leaves each lane 16
+// scores of one row, which are the operand of O^T += V^T P^T with no exchange, if
+// V's keys are laid out in the same order: lane half h takes the keys 8 q + 4 h +
+// 0..3, q = 0..3, 8 a step. Roundings (q to fp16, probabilities to bf16, their
+// sum) as in attn_kv8.hip.
+//
+// Bound by the matrix cores under load: a prompt of 8192 tokens, 550 GFLOP in 490
+// us, 1.12 PFLOP/s of the 1.24 to 1.36 that a large bf16 product reaches here, at
+// 1.85 to 2.0 GHz (power). A step of 32 keys is 2048 cycles of MFMA and some 3200 in
+// all: the softmax's exponents and packing stand between the two products of a
+// wavefront, and the other wavefront of its SIMD fills only part of that. Slower:
+// products of one step interleaved with the softmax of the next, q partly in LDS
+// for it (538 us against 497 then), wavefronts half a step apart (540), one operand
+// read ahead instead of two (527; three and four 495 and 499), 64 rows a wavefront
+// (spills). Short calls are bound by a tile's start and end, some 15 us together.
 #include <math.h>
 #include <stdint.h>
 
@@ -540,11 +551,15 @@ template <int N> Cut<N> by_length(Kv8SeqsN<N> &q, const Plan &p) {
     return cut;
 }
 
-// The plan of least time by the time of the busiest CU, from a tile's alone on a
-// CU (us; 16 + 1.38 a block of keys with 32 tokens, 15.5 + 0.83 with 16; its
-// products at the clock of a full chip), tiles dealt longest first: the longest, all of them
-// over the CUs, and where a few more than CUs remain, the two that share a CU. Parts
-// cost a start and an end each and the launch that joins them.
+// The plan of least time, by the time of the busiest CU from a tile's alone on the
+// chip (us; 16 + 1.38 a block of keys with 32 tokens, 15.5 + 0.83 with 16), tiles
+// dealt longest first: the longest, all of them over the CUs (a full chip's clock:
+// 1.26 and 1.18 times), and where some more than CUs remain, two that share a CU.
+// Parts cost a start and an end each, their outputs' way through memory and the
+// launch that joins them. Measured (us; 32 tokens, 16, 16 in parts): one prompt of 256
+// 28, 22; 1024 62, 43, 47; 4096 201, 159; 6000 313, 330; 8192 490; 512 tokens after 8000
+// 389, 235, 90; 16 after 4080 193, 120, 23; 8 times 500 after 4000 256, 294, 263; 16
+// times 128 after 2000 112, 84; 6 ragged prompts of up to 900 143, 92.
 Plan fa_plan(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv, size_t slots) {
     const size_t cus = (size_t)cu_count();
     int32_t end = 0;

@@ -66,8 +66,10 @@ __device__ __forceinline__ int scale_exp(uint32_t m) {
 // layer's weights are given, their largest magnitude, the codes. K's bytes go
 // straight to their places, 8 a time; V's go through LDS, where a thread
 // gathers the 16 of a piece, and a block that is not written as a whole brings
-// its old pieces with the rows (one round of loads in all). Bytes: a prompt of
-// 8192 tokens, 2 heads.
+// its old pieces with the rows (one round of loads in all). Bound by HBM for large
+// fills (2.1 million tokens of 2 heads, 4.3 GB in and 2.15 out: 1.30 ms, 5.0 TB/s);
+// a prompt of 8192 tokens, 25 MB, takes 7.1 us, of which 3.6 are launch, loads and
+// stores of a single block, one after the other.
 template <bool NORM, int N>
 __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ k,
                                                     size_t ldk, const uint16_t *__restrict__ v, size_t ldv,
@@ -239,7 +241,8 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, c
 }
 
 // One workgroup a (block, kv head, K or V): the block's pieces into LDS as
-// [key][d], then rows of it out, 16 bytes a thread.
+// [key][d], then rows of it out, 16 bytes a thread. 8192 tokens of 2 heads, 25 MB,
+// in 4.8 to 6.4 us; one block 2.2.
 template <int N>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8SeqsN<N> sq, Kv8Ref kv, uint16_t *__restrict__ k, size_t ldk,
                                                   uint16_t *__restrict__ v, size_t ldv, int nkv) {
