@@ -597,22 +597,29 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
     });
 }
 
+bool attn_decode_kv8_fits(const ApusHipAttnKv8Work *w, size_t B, const int32_t *cu, const int32_t *pos0) {
+    size_t total = 0;
+    for (size_t s = 0; s < B; s++) {
+        if (cu[s + 1] - cu[s] > kRows / GRP) return false;
+        if (s % kKv8Seqs == 0) total = 0;
+        total += (size_t)counted_blocks(pos0[s], cu[s + 1] - cu[s], 0) * w->nkv;
+        if (total > 0x7f000000) return false;
+    }
+    return B <= w->max_seqs;
+}
+
 int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
                           const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
                           const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T) {
     if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, r, T)) return e;
     if (B > w->max_seqs)
         return set_error(kErrArgument, "%zu sequences, the workspace holds %zu", B, w->max_seqs);
-    size_t total = 0;
-    for (size_t s = 0; s < B; s++) {
+    for (size_t s = 0; s < B; s++)
         if (cu[s + 1] - cu[s] > kRows / GRP)
             return set_error(kErrUnsupported, "decode takes 0..%d new tokens per sequence (got %d)", kRows / GRP,
                              cu[s + 1] - cu[s]);
-        if (s % kKv8Seqs == 0) total = 0;
-        total += (size_t)counted_blocks(pos0[s], cu[s + 1] - cu[s], 0) * L->nkv;
-        if (total > 0x7f000000) return set_error(kErrUnsupported, "too many cached keys in one call");
-    }
-    return kOk;
+    return attn_decode_kv8_fits(w, B, cu, pos0) ? (int)kOk
+                                                : set_error(kErrUnsupported, "too many cached keys in one call");
 }
 
 }  // namespace apus

@@ -625,6 +625,10 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
     if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, &r, &T)) return e;
     if (int e = mx_ready()) return e;
     if (!T) return kOk;
+    // up to 4 new tokens a sequence: decode's kernels, whose tiles are 16 or 32 rows
+    // and not 128 (us, decode's and these: one sequence, 3 tokens after 100 10 and 19;
+    // 2 after 60000 20 and 47; 64, 4 after 8000 106 and 194)
+    if (attn_decode_kv8_fits(w, B, cu, pos0)) return attn_decode_kv8_run(L, w, B, rows, cu, pos0, qg, k, v, r, y);
     const size_t nkv = L->nkv;
     if (k)
         if (int e = kv8_append_run(r, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;

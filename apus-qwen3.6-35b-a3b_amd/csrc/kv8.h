@@ -203,6 +203,7 @@ int attn_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_
 int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
                           const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
                           const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T);
+bool attn_decode_kv8_fits(const ApusHipAttnKv8Work *w, size_t B, const int32_t *cu, const int32_t *pos0);
 int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
                         const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
                         const uint16_t *v, const Kv8Ref &kv, uint16_t *y);
