@@ -6,8 +6,8 @@
 //
 // The 8 q heads of a kv head times up to 4 new tokens are the rows of the matrix
 // products, one or two blocks of 16, so K and V come from HBM once a (sequence, kv
-// head) pair. The pairs' blocks are laid end to end and cut into equal runs, one
-// a workgroup and at most two a CU, so that every CU reads as much however ragged
+// head) pair. The pairs' blocks are laid end to end and cut into runs, one a
+// workgroup and at most two a CU, so that every CU is as long at it however ragged
 // the contexts are; a run that crosses a pair's border is two segments. The 4
 // wavefronts of a workgroup take a segment's blocks in turn, each with its own M,
 // sum and outputs of all rows in registers, and meet in LDS at its end. A segment
@@ -22,9 +22,9 @@
 // weights that add up to 1, and a single large weight brings no error.
 //
 // Bound by HBM where contexts are long: 64 sequences at 32768 with 2 kv heads, 2.15
-// GB in 328 us, 6.5 TB/s (a pure read stream reaches 7.0; with loads that stay in
-// the caches 361 us); 128 ragged ones verifying 1-4 tokens, 1.36 GB in 237 us,
-// 5.7 TB/s (two row blocks: each block of K and V is worked on for twice as long
+// GB in 322 us, 6.7 TB/s (a pure read stream reaches 7.0; with loads that stay in
+// the caches 361 us, against 328 then); 128 ragged ones verifying 1-4 tokens, 1.36 GB
+// in 230 us, 5.9 TB/s (two row blocks: each block of K and V is worked on for twice as long
 // and K's next loads wait for the scores, else the registers spill; wavefronts in
 // pairs that share the keys, a row block each, 291 us). Few sequences: the chain of
 // a segment, 9 us of launch, block ids, q rows and first loads, the end 4 us, and
@@ -109,12 +109,27 @@ __device__ __forceinline__ uint2 finish(f32x4 o, float l, uint2 gate) {
     return make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
 }
 
+// How the pairs' blocks are cut into runs: of len[0] and len[1] in turn, from run
+// half (even) on of len[2] and len[3].
+struct Runs {
+    int32_t len[4], half;
+    __host__ __device__ int start(int i) const {
+        const int h = i < half ? 0 : 2, j = i < half ? i : i - half;
+        return (h ? half / 2 * (len[0] + len[1]) : 0) + j / 2 * (len[h] + len[h + 1]) + (j & 1) * len[h];
+    }
+    __host__ __device__ int of(int x) const {              // the run of block x
+        const int s = half / 2 * (len[0] + len[1]), h = x < s ? 0 : 2, y = x < s ? x : x - s;
+        const int both = len[h] + len[h + 1], q = y / both;
+        return (h ? half : 0) + 2 * q + (y - q * both >= len[h] ? 1 : 0);
+    }
+};
+
 // RB: row blocks, 2 where a sequence has more than two new tokens; their q rows
 // then stay in LDS, and come from there once a block of keys.
 template <int RB, int N>
 __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
     Kv8SeqsN<N> sq, Kv8Ref kv, const uint16_t *__restrict__ qg, const uint16_t *__restrict__ qn_w,
-    const uint16_t *__restrict__ rope, int nkv, int total, int run, float c2, uint16_t *__restrict__ y,
+    const uint16_t *__restrict__ rope, int nkv, int total, Runs runs, float c2, uint16_t *__restrict__ y,
     float *__restrict__ part, float2 *__restrict__ stat) {
     static_assert(64 * kWaves == D, "a thread a dim, a wavefront's threads 4 q rows");
     static_assert(16 * AP >= 2048 && 16 * RB * QP / 2 + kWaves * 2048 <= kWaves * 16 * AP, "room for V with a NaN");
@@ -128,9 +143,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
     __shared__ __attribute__((aligned(16))) float ms[16 * RB][kWaves], ls[16 * RB][kWaves][4];
     __shared__ int first_nan[D];           // the first key whose v is NaN there, in the blocks not all rows see
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int x1 = min(((int)blockIdx.x + 1) * run, total), nh = nkv * GRP;
+    const int x1 = min(runs.start((int)blockIdx.x + 1), total), nh = nkv * GRP;
     int nx = 0;
-    for (int x = (int)blockIdx.x * run; x < x1; x = nx) {
+    for (int x = runs.start((int)blockIdx.x); x < x1; x = nx) {
         // (opaque: or every address of a lane is formed ahead of this loop, and spilled)
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));
@@ -408,7 +423,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
 template <int SP, int N>
 __global__ __launch_bounds__(64 * (SP > 4 ? SP : 4)) void k_kv8_combine(Kv8SeqsN<N> sq, const float *__restrict__ part,
                                                      const float2 *__restrict__ stat,
-                                                     const uint16_t *__restrict__ qg, int nkv, int run, int items,
+                                                     const uint16_t *__restrict__ qg, int nkv, Runs runs, int items,
                                                      uint16_t *__restrict__ y) {
     const int lane = threadIdx.x & 63, d = lane * 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave % SP;
@@ -418,7 +433,7 @@ __global__ __launch_bounds__(64 * (SP > 4 ? SP : 4)) void k_kv8_combine(Kv8SeqsN
     const Kv8At a = kv8_find<true>(sq, tt);
     const int kvh = h / GRP, r = (tt - a.t0) * GRP + h % GRP;
     const int nb = (a.p0 + a.tokens + KEYS - 1) / KEYS, x = nkv * a.off + kvh * a.blocks;
-    const int w0 = x / run, w1 = (x + nb - 1) / run, pair = a.s * nkv + kvh;
+    const int w0 = runs.of(x), w1 = runs.of(x + nb - 1), pair = a.s * nkv + kvh;
     if (w0 == w1) return;                                  // (the whole pair: written already)
     const size_t at = (size_t)tt * nh + h;
     const uint2 gate = *reinterpret_cast<const uint2 *>(qg + at * 2 * D + D + d);
@@ -489,6 +504,16 @@ int32_t ctx_blocks(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n + KEYS - 
 // total as its root, up to 16, since every run costs the second launch a partial
 // result (one sequence at 60001: 19 us with runs of 15, 22 with 11 and 21 with 8).
 constexpr int32_t kPad = 8, kShort = 24, kShortMany = 96;
+// Runs of more than kLong blocks, two a CU, are not equal: of the two workgroups of a
+// CU the first is served first, and of two neighbouring XCDs (workgroups go to the
+// XCDs in turn) the odd one reads less while all of them read (64 equal contexts of
+// 32768 in equal runs: 230 and 277 us on even XCDs, 280 and 313 on odd ones). A
+// run's share of the mean, even and odd ones of the first 256 and of the others:
+// 1.18, 0.97, 0.98 and 0.87 (64 at 32768 328 us equal, 322 so; 128 ragged ones
+// verifying 1-4 tokens 239 and 230; 128 at 8000 171 and 167). Shorter runs differ by
+// few blocks and stay equal.
+constexpr int32_t kLong = 32;
+constexpr double kShare[3] = {1.18, 0.97, 0.98};
 size_t max_runs() { return 2 * (size_t)cu_count(); }
 int32_t whole_pairs(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv) {
     int32_t longest = 0;
@@ -502,10 +527,15 @@ int32_t whole_pairs(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv
 int32_t counted_blocks(int32_t pos0, int32_t n, int32_t whole) {
     return n <= 0 ? 0 : whole ? whole : ctx_blocks(pos0, n) + kPad;
 }
-size_t run_blocks(size_t total, int32_t whole) {
-    if (whole) return (size_t)whole;
-    const size_t root = std::min<size_t>(16, (size_t)(sqrt((double)total / 16.0) + 0.5));
-    return std::max({(total + max_runs() - 1) / max_runs(), root, (size_t)kWaves});
+Runs cut_runs(size_t total, int32_t whole) {
+    const size_t root = std::min<size_t>(16, (size_t)(sqrt((double)total / 16.0) + 0.5)), n = max_runs();
+    const int32_t len = (int32_t)std::max({(total + n - 1) / n, root, (size_t)kWaves});
+    if (whole) return Runs{{whole, whole, whole, whole}, 0};
+    if (len <= kLong || n % 4) return Runs{{len, len, len, len}, 0};
+    const double q = (double)total / (double)n;
+    Runs r = {{(int32_t)(q * kShare[0]), (int32_t)(q * kShare[1]), (int32_t)(q * kShare[2]), 0}, (int32_t)(n / 2)};
+    r.len[3] = (int32_t)((4 * total + n - 1) / n) - r.len[0] - r.len[1] - r.len[2];
+    return r;
 }
 
 }  // namespace
@@ -564,19 +594,19 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
         if (!total) return (int)kOk;
         int most = 0;
         for (int s = 0; s < q.n; s++) most = std::max(most, q.e[s + 1].cu - q.e[s].cu);
-        const size_t run = run_blocks(total, whole);
+        const Runs runs = cut_runs(total, whole);
         size_t segs = 1;                                   // the most of a pair
         for (int s = 0; s < q.n; s++) {
             const size_t nb = (size_t)ctx_blocks(q.e[s].pos0, q.e[s + 1].cu - q.e[s].cu);
             size_t x = nkv * (size_t)q.e[s].off;
             for (size_t h = 0; nb && h < nkv; h++, x += (size_t)(q.e[s + 1].off - q.e[s].off))
-                segs = std::max(segs, (x + nb - 1) / run - x / run + 1);
+                segs = std::max(segs, (size_t)(runs.of((int)(x + nb - 1)) - runs.of((int)x) + 1));
         }
         const float c2 = (float)(1.44269504088896341 / sqrt((double)D));
         auto launch = [&](auto rb) {
             APUS_TIMED("k_kv8_attn",
-                       k_kv8_attn<decltype(rb)::value, N><<<(unsigned)((total + run - 1) / run), 64 * kWaves, 0, stream()>>>(
-                           q, kv, qg, L->qn_w, w->rope, (int)nkv, (int)total, (int)run, c2, y, w->part, w->stat));
+                       k_kv8_attn<decltype(rb)::value, N><<<(unsigned)runs.of((int)total - 1) + 1, 64 * kWaves, 0, stream()>>>(
+                           q, kv, qg, L->qn_w, w->rope, (int)nkv, (int)total, runs, c2, y, w->part, w->stat));
         };
         if (most <= 2) launch(std::integral_constant<int, 1>{});
         else launch(std::integral_constant<int, 2>{});
@@ -588,7 +618,7 @@ int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t
             constexpr int W = SP > 4 ? SP : 4;
             APUS_TIMED("k_kv8_combine",
                        k_kv8_combine<SP, N><<<cdiv(items, W / SP), 64 * W, 0, stream()>>>(
-                           q, w->part, w->stat, qg, (int)nkv, (int)run, (int)items, y));
+                           q, w->part, w->stat, qg, (int)nkv, runs, (int)items, y));
         };
         if (segs <= 8) combine(std::integral_constant<int, 1>{});
         else if (segs <= 32) combine(std::integral_constant<int, 4>{});

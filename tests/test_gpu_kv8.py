@@ -225,6 +225,44 @@ def test_decode_one_sequence(hip, tq, ctx):
     s.check(s.call(hip.attn_decode_kv8))
 
 
+@pytest.mark.parametrize("new", [[1, 1, 0, 1, 1, 1], [4, 1, 0, 2, 3, 4]])
+def test_decode_long_runs(hip, new):
+    """Enough keys for runs of unequal length, two a CU (shared blocks: a row's
+    table repeats a few): every part of each context counts, at its position."""
+    rng = np.random.default_rng(17)
+    nkv, few, max_blocks = 2, 40, 4096
+    ctx = np.array([131000, 64000, 90000, 33, 100, 120001])
+    t = rng.integers(0, few, (len(ctx), max_blocks)).astype(np.int32)
+    kv = hip.kv8_cache(nkv, few, max_blocks, block_table=torch.from_numpy(t).cuda())
+    ident = hip.kv8_cache(nkv, few, few, block_table=torch.arange(few, dtype=torch.int32, device="cuda")[None].contiguous())
+    ident.k, ident.v, ident.scale = kv.k, kv.v, kv.scale
+    x = [kv_rows(rng, few * 32, nkv, 1.0) for _ in range(2)]
+    hip.kv8_append(ident, None, [0, few * 32], [0], dev(x[0]), dev(x[1]))
+    ref = R.Cache(nkv, 1, few)
+    ref.append(0, 0, x[0], x[1])
+    kk, vv = (a.reshape(few, 32, nkv, R.D) for a in ref.values(0, 0, few * 32))
+    w = dict(qn_w=R.bf16(rng.normal(size=R.D) * 0.1), kn_w=R.bf16(rng.normal(size=R.D) * 0.1))
+    layer = hip.attn_layer((nkv * R.GRP, nkv, R.D, R.ROT, THETA), {k: dev(v) for k, v in w.items()})
+    work = hip.AttnKv8Work(layer, len(ctx), max_blocks * 32)
+    cu = cum(new)
+    qg = R.bf16(rng.normal(size=(int(cu[-1]), nkv * R.GRP, 2 * R.D)))
+    y = torch.empty(len(qg), nkv * R.GRP * R.D, dtype=torch.int16, device="cuda")
+    hip.attn_decode_kv8(layer, work, None, cu, ctx, dev(qg), None, None, kv, y)
+    got = R.f64(host(y)).reshape(len(qg), -1, R.D)
+    for s in range(len(ctx)):
+        if not new[s]:
+            continue
+        n = int(ctx[s] + new[s])
+        b = t[s, :-(-n // 32)]
+        k, v = (a[b].reshape(-1, nkv, R.D)[:n] for a in (kk, vv))
+        r, tol = R.attention(qg[cu[s]:cu[s + 1]], w["qn_w"], int(ctx[s]), k, v, THETA)
+        assert (np.abs(got[cu[s]:cu[s + 1]] - r) <= tol).all(), s
+    z = torch.empty_like(y)
+    hip.attn_decode_kv8(layer, work, None, cu, ctx, dev(qg), None, None, kv, z)
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+
+
 @pytest.mark.parametrize("tq", [1, 4])
 def test_decode_many_sequences(hip, tq):
     """More sequences than one launch takes."""
