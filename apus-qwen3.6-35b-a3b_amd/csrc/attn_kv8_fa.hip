@@ -21,7 +21,7 @@
 // products of one step interleaved with the softmax of the next, q partly in LDS
 // for it (538 us against 497 then), wavefronts half a step apart (540), one operand
 // read ahead instead of two (527; three and four 495 and 499), 64 rows a wavefront
-// (spills). Short calls are bound by a tile's start and end, some 15 us together.
+// (spills). Short calls are bound by a tile's start and end, some 13 us together.
 #include <math.h>
 #include <stdint.h>
 
@@ -192,63 +192,88 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Cut<N
     // the wavefront's q rows n = (token 4 rblk + n / 8, head n % 8): k-step i, dims 16 i + 8 hf ..
     const int tok = f0 + rblk * 4 + (n >> 3), h = kvh * GRP + (n & 7);
     const int pos = p0 + min(tok, ns - 1);
+    // (KS 2: wavefronts of the same rows form half of the dims each and exchange them;
+    // both forming all took 22.3 us for 16 tokens after 240, so 19.6)
+    constexpr int QI = 16 / KS;
+    const int c0 = KS == 1 ? 0 : kg * QI;                  // the first of its k-steps
     f16x8 q[16];
     float qf;                                              // scores' factor, a power of two (log2 e is in q)
     {
-        const uint16_t *qr = qg + ((size_t)(t0 + min(tok, ns - 1)) * nh + h) * 2 * D + hf * 8;
+        const uint16_t *qr = qg + ((size_t)(t0 + min(tok, ns - 1)) * nh + h) * 2 * D + c0 * 16 + hf * 8;
         // (every load at once: the outputs' registers are free yet)
-        u16x8 x[16], w[16], co[2], si[2];
+        u16x8 x[QI], w[QI], co[2], si[2];
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = *reinterpret_cast<const u16x8 *>(qr + i * 16);
+        for (int i = 0; i < QI; i++) x[i] = *reinterpret_cast<const u16x8 *>(qr + i * 16);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             co[i] = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + i * 16 + hf * 8);
             si[i] = *reinterpret_cast<const u16x8 *>(rope + (size_t)pos * ROT + ROT / 2 + i * 16 + hf * 8);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++) w[i] = *reinterpret_cast<const u16x8 *>(qn_w + i * 16 + hf * 8);
+        for (int i = 0; i < QI; i++) w[i] = *reinterpret_cast<const u16x8 *>(qn_w + (c0 + i) * 16 + hf * 8);
         __builtin_amdgcn_sched_barrier(0);
         float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < QI; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) ss += bf2f(x[i][e]) * bf2f(x[i][e]);
         ss = sum32(ss);
-        const float rs = 1.0f / sqrtf(ss / (float)D + kEps);
-        float o[16][8], mq = 0.0f;
+        float o[QI][8], mq = 0.0f;                         // (1 + w) x and its RoPE; the norm's factor comes later
 #pragma unroll
-        for (int i = 0; i < 16; i++) {                     // (or their fp32 values are kept from the sum)
+        for (int i = 0; i < QI; i++) {                     // (or their fp32 values are kept from the sum)
             u32x4 t = __builtin_bit_cast(u32x4, x[i]);
             asm volatile("" : "+v"(t));
             x[i] = __builtin_bit_cast(u16x8, t);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < QI; i++) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[i][e] = bf2f(x[i][e]) * rs * (1.0f + bf2f(w[i][e]));
+            for (int e = 0; e < 8; e++) o[i][e] = bf2f(x[i][e]) * (1.0f + bf2f(w[i][e]));
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (KS == 1 || kg == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)                        // RoPE: with the chunk 32 dims on
+            for (int i = 0; i < 2; i++)                    // RoPE: with the chunk 32 dims on
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float u = o[i][e], v = o[i + 2][e], c = bf2f(co[i][e]), s_ = bf2f(si[i][e]);
-                o[i][e] = u * c - v * s_;
-                o[i + 2][e] = v * c + u * s_;
-            }
+                for (int e = 0; e < 8; e++) {
+                    const float u = o[i][e], v = o[i + 2][e], c = bf2f(co[i][e]), s_ = bf2f(si[i][e]);
+                    o[i][e] = u * c - v * s_;
+                    o[i + 2][e] = v * c + u * s_;
+                }
+        }
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < QI; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) mq = fmaxf(mq, fabsf(o[i][e]));
         mq = max32(mq);
+        f16x8 *const ex = reinterpret_cast<f16x8 *>(lds) + lane;       // [wavefront][k-step][lane]
+        if (KS == 2) {
+            float2 *const sm = reinterpret_cast<float2 *>(lds + kWaves * QI * 1024) + n;
+            if (hf == 0) sm[wave * 32] = make_float2(ss, mq);
+            __syncthreads();
+            const float2 u = sm[(wave ^ kRowBlocks) * 32];
+            ss += u.x;
+            mq = fmaxf(mq, u.y);
+        }
+        const float rs = 1.0f / sqrtf(ss / (float)D + kEps);
         // (so the scores' factors are exact, and a score less M, by fma, is what M was
         // formed from: a rounded product's residual of a score past 2^31 gave infinities)
-        const float sc = kv8_row_scale(mq), inv = kL2E / sc;
+        const float sc = kv8_row_scale(mq * rs), inv = kL2E / sc;
         qf = sc / 16.0f;
+        f16x8 mine[QI];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < QI; i++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) q[i][e] = (_Float16)(o[i][e] * inv);
+            for (int e = 0; e < 8; e++) mine[i][e] = (_Float16)(o[i][e] * rs * inv);
+        if (KS == 1) {
+#pragma unroll
+            for (int i = 0; i < QI; i++) q[i] = mine[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < QI; i++) ex[(wave * QI + i) * 64] = mine[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 16; i++) q[i] = ex[((rblk + i / QI * kRowBlocks) * QI + i % QI) * 64];
         }
     }
     __syncthreads();                                       // (first_nan is clear)
@@ -552,13 +577,13 @@ template <int N> Cut<N> by_length(Kv8SeqsN<N> &q, const Plan &p) {
 }
 
 // The plan of least time, by the time of the busiest CU from a tile's alone on the
-// chip (us; 16 + 1.38 a block of keys with 32 tokens, 15.5 + 0.83 with 16), tiles
+// chip (us; 16 + 1.38 a block of keys with 32 tokens, 13.2 + 0.83 with 16), tiles
 // dealt longest first: the longest, all of them over the CUs (a full chip's clock:
 // 1.26 and 1.18 times), and where some more than CUs remain, two that share a CU.
 // Parts cost a start and an end each, their outputs' way through memory and the
 // launch that joins them. Measured (us; 32 tokens, 16, 16 in parts): one prompt of 256
-// 28, 22; 1024 62, 43, 47; 4096 201, 159; 6000 313, 330; 8192 490; 512 tokens after 8000
-// 389, 235, 90; 16 after 4080 193, 120, 23; 8 times 500 after 4000 256, 294, 263; 16
+// 28, 20; 1024 62, 41, 47; 4096 201, 159; 6000 313, 330; 8192 490; 512 tokens after 8000
+// 389, 235, 88; 16 after 4080 193, 120, 20; 8 times 500 after 4000 256, 294, 263; 16
 // times 128 after 2000 112, 84; 6 ragged prompts of up to 900 143, 92.
 Plan fa_plan(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv, size_t slots) {
     const size_t cus = (size_t)cu_count();
@@ -603,7 +628,7 @@ Plan fa_plan(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv, size_
         const int32_t len = k == 1 ? 0 : (end + KEYS - 1) / KEYS / k;
         if (k > 1 && (len < 2 || B > (size_t)kKv8Seqs)) break;
         const Plan p = {16, len};
-        const double t = busiest(p, 15.5, 0.83, 1.18);
+        const double t = busiest(p, 13.2, 0.83, 1.18);
         if (t < us) {
             us = t;
             best = p;

@@ -703,8 +703,8 @@ int apus_hip_kv8_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblock
 int apus_hip_kv8_pool_cache(const ApusHipKvPool *pool, size_t layer, ApusHipKv8Cache *out);
 
 /* What attention calls on an 8-bit cache need on the device for layers of this
- * one's dims (its weights are not looked at): partial results of a decode call
- * and the RoPE table of positions below max_pos (up to 2^24). max_seqs: the most
+ * one's dims (its weights are not looked at): partial results of a call and the
+ * RoPE table of positions below max_pos (up to 2^24). max_seqs: the most
  * sequences of a decode call. Calls that share one run one after the other:
  * on one stream, or ordered by the caller; calls or graph replays that may
  * overlap need one each. It must outlive the graphs that captured its calls.
