@@ -664,3 +664,53 @@ def test_nan_stays_through_a_rescale(hip):
         ref.append(0, pos, k, v)
         pos += n
         check_row(hip, kv, ref, 0, 0, pos)
+
+
+def test_blocks_past_4_gib(hip):
+    """A cache of 4.9 GB each for K and V: blocks on both sides of 4 GiB."""
+    rng = np.random.default_rng(101)
+    nkv, blocks = 2, 300000
+    t = torch.tensor([[299999, 7, 262144, 131072], [262143, 299998, 0, 262145]], dtype=torch.int32).cuda()
+    kv, ref = hip.kv8_cache(nkv, blocks, 4, block_table=t), R.Cache(nkv, 2, 4)
+    ctx, new = np.array([100, 90]), np.array([3, 4])
+    n = ctx + new
+    c = cum(n)
+    k, v = kv_rows(rng, int(c[-1]), nkv, 1.0), kv_rows(rng, int(c[-1]), nkv, 1.0)
+    hip.kv8_append(kv, None, c, [0, 0], dev(k), dev(v))
+    for s in range(2):
+        ref.append(s, 0, k[c[s]:c[s + 1]], v[c[s]:c[s + 1]])
+        check_row(hip, kv, ref, s, 0, int(n[s]))
+    w = dict(qn_w=R.bf16(rng.normal(size=R.D) * 0.1), kn_w=R.bf16(rng.normal(size=R.D) * 0.1))
+    layer = hip.attn_layer((nkv * R.GRP, nkv, R.D, R.ROT, THETA), {a: dev(b) for a, b in w.items()})
+    work = hip.AttnKv8Work(layer, 2, 128)
+    for f, take in ((hip.attn_decode_kv8, new), (hip.attn_prefill_kv8, n)):
+        cu, pos = cum(take), n - take
+        qg = R.bf16(rng.normal(size=(int(cu[-1]), nkv * R.GRP, 2 * R.D)))
+        y = torch.empty(len(qg), nkv * R.GRP * R.D, dtype=torch.int16, device="cuda")
+        f(layer, work, None, cu, pos, dev(qg), None, None, kv, y)
+        got = R.f64(host(y)).reshape(len(qg), -1, R.D)
+        for s in range(2):
+            a, b = ref.values(s, 0, int(n[s]))
+            r, tol = R.attention(qg[cu[s]:cu[s + 1]], w["qn_w"], int(pos[s]), a, b, THETA)
+            assert (np.abs(got[cu[s]:cu[s + 1]] - r) <= tol).all(), s
+
+
+@pytest.mark.parametrize("pad", [0, 8, 24])
+def test_read_leaves_the_rest(hip, pad):
+    """Rows of a pitch, sequences without tokens: nothing beside the rows."""
+    rng = np.random.default_rng(103)
+    kv, ref = make(hip, rng, 2, 3, 3, True), R.Cache(2, 3, 3)
+    x, z = kv_rows(rng, 200, 2), kv_rows(rng, 200, 2)
+    cu, n = [0, 70, 70, 165], [70, 0, 95]
+    hip.kv8_append(kv, None, cu, [0, 0, 0], dev(x[:165]), dev(z[:165]))
+    for s in (0, 2):
+        ref.append(s, 0, x[cu[s]:cu[s + 1]], z[cu[s]:cu[s + 1]])
+    out = [torch.full((60, 512 + pad), 0x55, dtype=torch.int16, device="cuda") for _ in range(2)]
+    hip.kv8_read(kv, [2, 1, 0], [0, 40, 40, 57], [31, 0, 33], out[0][:57, pad:], out[1][:57, pad:])
+    torch.cuda.synchronize()
+    for i, o in enumerate(out):
+        g = host(o)
+        assert (g[57:] == 0x55).all() and (g[:, :pad] == 0x55).all()
+        a = R.bf16(ref.values(2, 31, 71)[i]).reshape(40, 512)
+        b = R.bf16(ref.values(0, 33, 50)[i]).reshape(17, 512)
+        assert same(g[:57, pad:], np.concatenate((a, b)))
