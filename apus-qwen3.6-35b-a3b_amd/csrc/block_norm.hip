@@ -7,9 +7,11 @@
 // A row belongs to a wavefront up to 1024 elements (no barrier between its
 // loads and its stores), to a workgroup of four past them (2048, 8192 rows: 46.5
 // us with a workgroup a row, 48.8 with a wavefront; 1529, element by element: 11.9
-// and 16.3). Aligned rows go 8 elements a load, others one. Bound by memory: 8192
-// rows of 2048, fp32 residuals and a gate, 235 MB in 44.5 us, 5.3 TB/s, what a copy
-// of 1 GiB reaches; a single row (2 us) by its launch.
+// and 16.3), to one of eight past 8192 (16384, 2000 rows: 67 us, with four 74, with
+// sixteen 83; 16001, element by element: 111, 153, 142). Aligned rows go 8
+// elements a load, others one. Bound by memory: 8192 rows of 2048, fp32 residuals
+// and a gate, 235 MB in 44.5 us, 5.3 TB/s, what a copy of 1 GiB reaches; a single
+// row (2 us) by its launch.
 #include <math.h>
 #include <stdint.h>
 
@@ -93,11 +95,12 @@ template <bool VEC> __device__ __forceinline__ void st8(float *p, const float (&
 // TPR threads a row, NV eights a thread; H: the residual's type. VEC: hidden
 // and every row's start in whole vectors.
 template <class H, bool VEC, int TPR, int NV>
-__global__ __launch_bounds__(256) void k_block_norm(NormArgs a) {
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_block_norm(NormArgs a) {
+    constexpr int R = TPR < 256 ? 256 / TPR : 1;           // rows of a workgroup
     const int tid = threadIdx.x, lane = tid % TPR;
-    const int row = min((int)blockIdx.x * (256 / TPR) + tid / TPR, a.rows - 1);   // (the last row again: same values)
-    const bool live = (int)blockIdx.x * (256 / TPR) + tid / TPR < a.rows;
-    __shared__ float red[2][4];
+    const int row = min((int)blockIdx.x * R + tid / TPR, a.rows - 1);     // (the last row again: same values)
+    const bool live = (int)blockIdx.x * R + tid / TPR < a.rows;
+    __shared__ __attribute__((aligned(16))) float red[2][TPR > 64 ? TPR / 64 : 1];
     // the sum over the row's threads
     auto total = [&](float s, int k) {
 #pragma unroll
@@ -105,7 +108,10 @@ __global__ __launch_bounds__(256) void k_block_norm(NormArgs a) {
         if (TPR == 64) return s;
         if ((tid & 63) == 0) red[k][tid >> 6] = s;
         __syncthreads();
-        return (red[k][0] + red[k][1]) + (red[k][2] + red[k][3]);
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; i += 4) s += (red[k][i] + red[k][i + 1]) + (red[k][i + 2] + red[k][i + 3]);
+        return s;
     };
     const int n = a.hidden, step = VEC ? 1 : TPR;
     // of the eight j: its first element, and whether its element e is in the row
@@ -186,7 +192,7 @@ template <class H> int launch(const NormArgs &a, bool vec) {
         constexpr int TPR = decltype(tpr)::value;
         APUS_TIMED("k_block_norm",
                    k_block_norm<H, decltype(v)::value, TPR, decltype(nv)::value>
-                       <<<cdiv((size_t)a.rows, 256 / TPR), 256, 0, stream()>>>(a));
+                       <<<cdiv((size_t)a.rows, TPR < 256 ? 256 / TPR : 1), TPR > 256 ? TPR : 256, 0, stream()>>>(a));
         return launch_check("k_block_norm");
     };
     auto size = [&](auto v) {
@@ -197,7 +203,7 @@ template <class H> int launch(const NormArgs &a, bool vec) {
         if (a.hidden <= 2048) return go(v, four, std::integral_constant<int, 1>{});
         if (a.hidden <= 4096) return go(v, four, std::integral_constant<int, 2>{});
         if (a.hidden <= 8192) return go(v, four, std::integral_constant<int, 4>{});
-        return go(v, four, std::integral_constant<int, 8>{});
+        return go(v, std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
     };
     return vec ? size(std::true_type{}) : size(std::false_type{});
 }
