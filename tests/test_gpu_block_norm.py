@@ -67,7 +67,7 @@ def check(norm, y, h, h_out, x, post, pre, gate, scale, eps):
 @pytest.mark.parametrize("gate", ["none", "one", "rows"])
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("t,n,pad", [(1, 2048, 0), (5, 8, 0), (3, 1, 0), (7, 333, 3), (2, 512, 8), (9, 1000, 72),
-                                     (4, 2056, 0), (3, 4097, 1), (2, 8200, 0), (1, 16384, 8), (130, 64, 1)])
+                                     (4, 2056, 0), (3, 4097, 1), (2, 8200, 0), (1, 16384, 8), (130, 64, 1), (3, 16001, 3), (2, 9001, 0)])
 def test_block_norm(hip, t, n, pad, post, gate, f32):
     rng = np.random.default_rng(n + t)
     y, h = rows(rng, t, n, pad, False, 0.5), rows(rng, t, n, pad, f32, 4.0)
