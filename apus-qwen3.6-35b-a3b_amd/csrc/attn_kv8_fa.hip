@@ -25,8 +25,6 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <algorithm>
-#include <functional>
 #include <type_traits>
 
 #include "apus_dev.h"
@@ -86,12 +84,6 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
 
 typedef const __attribute__((address_space(1))) u32x4 *gu32x4p;
 
-// Of each sequence of a launch: the tokens that its last tile lacks of being full
-// (the sequences are not in the batch's order, so the entries' cu do not tell),
-// and the parts that each tile's keys are cut into.
-template <int N> struct Cut {
-    uint8_t lack[N], parts[N];
-};
 constexpr int kPartRows = 128;               // rows of a part: of a tile of 16 tokens and a kv head
 
 struct Step {
@@ -109,7 +101,7 @@ __device__ __forceinline__ float uni(float x) {
 // that is not enough a tile's keys go to several workgroups (KS 2 only), which leave
 // outputs, M and sum in slot item - split0 for k_kv8_fa_combine.
 template <int KS, int N>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Cut<N> cut, Kv8Ref kv, const uint16_t *__restrict__ qg,
+__global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Cut<N> cut, Kv8Ref kv, const uint16_t *__restrict__ qg,
                                                            const uint16_t *__restrict__ qn_w,
                                                            const uint16_t *__restrict__ rope, int nkv,
                                                            uint16_t *__restrict__ y, int split0,
@@ -470,7 +462,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Cut<N
 // has 1 KiB of each part: four dims of 32 rows and two lane halves. sq: off counts
 // tiles, pos0 is the number of parts and row the first slot.
 template <int SP, int N>
-__global__ __launch_bounds__(256) void k_kv8_fa_combine(Kv8SeqsN<N> sq, Cut<N> cut, const float *__restrict__ part,
+__global__ __launch_bounds__(256) void k_kv8_fa_combine(Kv8SeqsN<N> sq, Kv8Cut<N> cut, const float *__restrict__ part,
                                                         const float2 *__restrict__ stat,
                                                         const uint16_t *__restrict__ qg, int nkv,
                                                         uint16_t *__restrict__ y) {
@@ -541,102 +533,6 @@ __global__ __launch_bounds__(256) void k_kv8_fa_combine(Kv8SeqsN<N> sq, Cut<N> c
     *reinterpret_cast<uint2 *>(y + at * D + d) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
 }
 
-// How a call is cut: tokens of a tile, and blocks of a part (0: tiles are whole).
-struct Plan {
-    int tok;
-    int32_t len;
-};
-constexpr int kMostParts = 64;
-int parts_of(const Plan &p, int32_t end) {
-    const int32_t blocks = (end + KEYS - 1) / KEYS;
-    return p.len ? std::min((blocks + p.len - 1) / p.len, (int32_t)kMostParts) : 1;
-}
-
-// Puts a launch's sequences in the order of their ends: its tiles start with the
-// last, so the longest go first (6 ragged prompts: 105 us in the batch's order,
-// 93 so), and those with several parts are the last entries.
-template <int N> Cut<N> by_length(Kv8SeqsN<N> &q, const Plan &p) {
-    struct {
-        Kv8Seq e;
-        int32_t n;
-    } s[N];
-    Cut<N> cut = {};
-    for (int i = 0; i < q.n; i++) s[i] = {q.e[i], q.e[i + 1].cu - q.e[i].cu};
-    std::sort(s, s + q.n, [](const auto &a, const auto &b) { return a.e.pos0 + a.n < b.e.pos0 + b.n; });
-    int32_t off = 0;
-    for (int i = 0; i < q.n; i++) {
-        const int32_t tiles = (s[i].n + p.tok - 1) / p.tok, parts = parts_of(p, s[i].e.pos0 + s[i].n);
-        q.e[i] = s[i].e;
-        q.e[i].off = off;
-        cut.lack[i] = (uint8_t)(tiles * p.tok - s[i].n);
-        cut.parts[i] = (uint8_t)parts;
-        off += tiles * parts;
-    }
-    q.e[q.n].off = off;
-    return cut;
-}
-
-// The plan of least time, by the time of the busiest CU from a tile's alone on the
-// chip (us; 16 + 1.38 a block of keys with 32 tokens, 13.2 + 0.83 with 16), tiles
-// dealt longest first: the longest, all of them over the CUs (a full chip's clock:
-// 1.26 and 1.18 times), and where some more than CUs remain, two that share a CU.
-// Parts cost a start and an end each, their outputs' way through memory and the
-// launch that joins them. Measured (us; 32 tokens, 16, 16 in parts): one prompt of 256
-// 28, 20; 1024 62, 41, 47; 4096 201, 159; 6000 313, 330; 8192 490; 512 tokens after 8000
-// 389, 235, 88; 16 after 4080 193, 120, 20; 8 times 500 after 4000 256, 294, 263; 16
-// times 128 after 2000 112, 84; 6 ragged prompts of up to 900 143, 92.
-Plan fa_plan(size_t B, const int32_t *cu, const int32_t *pos0, size_t nkv, size_t slots) {
-    const size_t cus = (size_t)cu_count();
-    int32_t end = 0;
-    auto busiest = [&](const Plan &p, double base, double per, double full) {
-        size_t items = 0, split = 0;
-        double sum = 0.0, longest = 0.0;
-        for (size_t s = 0; s < B; s++) {
-            const int64_t n = cu[s + 1] - cu[s];
-            if (!n) continue;
-            const int parts = parts_of(p, pos0[s] + (int32_t)n);
-            const size_t t = (size_t)((n + p.tok - 1) / p.tok) * nkv;
-            items += t * (size_t)parts;
-            if (parts > 1) split += t * (size_t)parts;
-            longest = std::max(longest, base + per * (double)(pos0[s] + n) / KEYS / parts);
-            sum += (double)t * (base * parts + per * ((double)pos0[s] + (double)(n + p.tok) / 2) / KEYS);
-        }
-        if (split > slots) return 1e30;
-        sum /= (double)cus;
-        const double load = 1.0 + 0.15 * std::min(1.0, sum / longest);
-        double us = std::max(longest * load, sum * full);
-        double t[1024];
-        if (items > cus && items <= std::min<size_t>(2 * cus, 1024)) {
-            double *e = t;
-            for (size_t s = 0; s < B; s++) {
-                const int64_t n = cu[s + 1] - cu[s];
-                const int parts = n ? parts_of(p, pos0[s] + (int32_t)n) : 1;
-                for (int64_t x = 0; x < n; x += p.tok, e += nkv * (size_t)parts)
-                    std::fill_n(e, nkv * (size_t)parts,
-                                base + per * (double)(pos0[s] + std::min<int64_t>(x + p.tok, n)) / KEYS / parts);
-            }
-            std::nth_element(t, t + cus, e, std::greater<double>());
-            us = std::max(us, 2.0 * t[cus] * load);
-        }
-        return us + (split ? 6.0 + 0.05 * (double)split : 0.0);
-    };
-    for (size_t s = 0; s < B; s++)
-        if (cu[s + 1] > cu[s]) end = std::max(end, pos0[s] + cu[s + 1] - cu[s]);
-    Plan best = {32, 0};
-    double us = busiest(best, 16.0, 1.38, 1.26);
-    for (const int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-        const int32_t len = k == 1 ? 0 : (end + KEYS - 1) / KEYS / k;
-        if (k > 1 && (len < 2 || B > (size_t)kKv8Seqs)) break;
-        const Plan p = {16, len};
-        const double t = busiest(p, 13.2, 0.83, 1.18);
-        if (t < us) {
-            us = t;
-            best = p;
-        }
-    }
-    return best;
-}
-
 }  // namespace
 
 extern "C" {
@@ -657,17 +553,15 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
     const size_t nkv = L->nkv;
     if (k)
         if (int e = kv8_append_run(r, nkv, B, rows, cu, pos0, k, nkv * D, v, nkv * D, L->kn_w, w->rope)) return e;
-    const Plan plan = fa_plan(B, cu, pos0, nkv, w->rows / kPartRows);
+    const Kv8Plan plan = kv8_fa_plan(B, cu, pos0, nkv, w->rows / kPartRows, (size_t)cu_count());
     return kv8_launches(B, rows, cu, pos0, [&](size_t s) { return (cu[s + 1] - cu[s] + plan.tok - 1) / plan.tok; },
                         [&](auto &q) {
         constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
         if (!q.e[q.n].off) return (int)kOk;
-        const Cut<N> cut = by_length(q, plan);
+        const Kv8Cut<N> cut = kv8_by_length(q, plan);
         const size_t grid = (size_t)q.e[q.n].off * nkv;
         if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
-        int first = 0;                                     // the first sequence of several parts
-        while (first < q.n && cut.parts[first] == 1) first++;
-        const int split0 = q.e[first].off;
+        const int split0 = q.e[kv8_first_split(q, cut)].off;
         auto launch = [&](auto ks) {
             APUS_TIMED("k_kv8_fa", k_kv8_fa<decltype(ks)::value, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(
                                        q, cut, r, qg, L->qn_w, w->rope, (int)nkv, y, split0, w->part, w->stat));
@@ -676,28 +570,15 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
         if (plan.tok == 32) return launch(std::integral_constant<int, 1>{});
         if (int e = launch(std::integral_constant<int, 2>{})) return e;
         if (split0 == q.e[q.n].off) return (int)kOk;
-        // the split sequences, in tiles
-        Kv8SeqsN<N> sq;
-        Cut<N> scut = {};
-        sq.n = q.n - first;
-        int32_t off = 0, most = 1;
-        for (int i = 0; i < sq.n; i++) {
-            const Kv8Seq &e = q.e[first + i];
-            const int32_t parts = cut.parts[first + i];
-            sq.e[i] = Kv8Seq{off, e.cu, parts, e.off - split0};
-            scut.lack[i] = cut.lack[first + i];
-            off += (q.e[first + i + 1].off - e.off) / parts;
-            most = std::max(most, parts);
-        }
-        for (int i = sq.n; i <= N; i++) sq.e[i] = Kv8Seq{i == sq.n ? off : 0x7fffffff, 0x7fffffff, 0, 0};
+        const Kv8Joins<N> j = kv8_joins(q, cut);
         auto combine = [&](auto sp) {
             constexpr int SP = decltype(sp)::value;
             APUS_TIMED("k_kv8_fa_combine",
-                       k_kv8_fa_combine<SP, N><<<(unsigned)((size_t)off * nkv * 32 * SP), 256, 0, stream()>>>(
-                           sq, scut, w->part, w->stat, qg, (int)nkv, y));
+                       k_kv8_fa_combine<SP, N><<<(unsigned)((size_t)j.tiles * nkv * 32 * SP), 256, 0, stream()>>>(
+                           j.sq, j.cut, w->part, w->stat, qg, (int)nkv, y));
             return launch_check("k_kv8_fa_combine");
         };
-        return most <= 8 ? combine(std::integral_constant<int, 1>{}) : combine(std::integral_constant<int, 4>{});
+        return j.most <= 8 ? combine(std::integral_constant<int, 1>{}) : combine(std::integral_constant<int, 4>{});
     });
 }
 

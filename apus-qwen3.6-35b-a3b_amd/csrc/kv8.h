@@ -19,12 +19,12 @@
 #include "../../include/apus_hip.h"
 #include "apus_dev.h"
 #include "apus_rt.h"
+#include "kv8_plan.h"
 #include "mx.h"
 
 namespace apus {
 
 constexpr int kKv8D = 256;                   // head dim
-constexpr int kKv8Keys = 32;                 // positions of a block
 constexpr int kKv8Bytes = kKv8Keys * kKv8D;  // bytes of a head's K or V block
 constexpr int kKv8MinExp = -117;             // smallest exponent of a scale: its codes' steps stay normal in bf16
 
@@ -59,20 +59,6 @@ __device__ __forceinline__ uint32_t kv8_id_u(const Kv8Ref &r, int h, int b) {
                                : (uint32_t)at + (uint32_t)bu;
     return min(id, r.blocks - 1);
 }
-
-// The sequences of one launch, by value (a captured call keeps them; longer
-// batches take several launches). Few sequences: the short form, whose copy at
-// launch is shorter. Entry i: the blocks (in the kernel's count) and tokens
-// before sequence i, its cached positions and its row; entry n has the totals,
-// entries past it none that is ever found.
-constexpr int kKv8Seqs = 208, kKv8FewSeqs = 8;     // (a kernel's arguments within 4 KiB)
-struct Kv8Seq {
-    int32_t off, cu, pos0, row;
-};
-template <int N> struct alignas(16) Kv8SeqsN {
-    Kv8Seq e[N + 1];
-    int32_t n;
-};
 
 // A sequence of a launch: its number, entry, and what it has of blocks and tokens.
 struct Kv8At {
@@ -111,38 +97,6 @@ template <bool TOKEN, int N> __device__ __forceinline__ Kv8At kv8_find(const Kv8
     a.p0 = get([](const Kv8Seq &q) { return q.pos0; }, s);
     a.row = get([](const Kv8Seq &q) { return q.row; }, s);
     return a;
-}
-
-// Calls f(seqs) for each launch's share of a batch; count(s) is the number of
-// blocks of sequence s. f may reorder its copy of the entries, and returns a status.
-template <class Count, class F>
-int kv8_launches(size_t B, const int32_t *rows, const int32_t *cu, const int32_t *pos0, Count count, F f) {
-    for (size_t s0 = 0; s0 < B; s0 += kKv8Seqs) {
-        const size_t n = B - s0 < (size_t)kKv8Seqs ? B - s0 : (size_t)kKv8Seqs;
-        auto fill = [&](auto &q) {
-            constexpr size_t N = sizeof(q.e) / sizeof(q.e[0]) - 1;
-            q.n = (int32_t)n;
-            int32_t off = 0;
-            for (size_t i = 0; i < n; i++) {
-                const size_t s = s0 + i;
-                q.e[i] = Kv8Seq{off, cu[s], pos0[s], rows ? rows[s] : (int32_t)s};
-                off += count(s);
-            }
-            q.e[n] = Kv8Seq{off, cu[s0 + n], 0, 0};
-            for (size_t i = n + 1; i <= N; i++) q.e[i] = Kv8Seq{0x7fffffff, 0x7fffffff, 0, 0};
-            return f(q);
-        };
-        int r;
-        if (n <= (size_t)kKv8FewSeqs) {
-            Kv8SeqsN<kKv8FewSeqs> q;
-            r = fill(q);
-        } else {
-            Kv8SeqsN<kKv8Seqs> q;
-            r = fill(q);
-        }
-        if (r) return r;
-    }
-    return kOk;
 }
 
 // ---- for the attention kernels -------------------------------------------
