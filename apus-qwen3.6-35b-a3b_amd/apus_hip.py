@@ -951,10 +951,11 @@ def _kv8_rows_call(f, kv, rows, cu, pos0, k, v):
     n, T = kv.nkv * 256, _total(keep[1])
     ld = []
     for t, what in ((k, "k"), (v, "v")):
-        if t.dim() == 3:
-            if tuple(t.shape[1:]) != (kv.nkv, 256) or (t.shape[0] and kv.nkv > 1 and t.stride(1) != 256):
+        if t.dim() == 3:                   # (a view of the tensor's own memory, never a copy)
+            if tuple(t.shape[1:]) != (kv.nkv, 256) or (
+                    t.shape[0] and (t.stride(2) != 1 or kv.nkv > 1 and t.stride(1) != 256)):
                 raise ValueError(f"{what}: rows of {kv.nkv} heads of 256, contiguous, not {tuple(t.shape)} of strides {t.stride()}")
-            t = t.flatten(1)
+            t = t.view(t.shape[0], n)
         p, m, _, pitch = _rows(t, what, _device, n)
         if m != T:
             raise ValueError(f"{what}: {m} rows, expected {T}")
