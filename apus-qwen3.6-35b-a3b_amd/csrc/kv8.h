@@ -27,6 +27,7 @@ namespace apus {
 constexpr int kKv8D = 256;                   // head dim
 constexpr int kKv8Bytes = kKv8Keys * kKv8D;  // bytes of a head's K or V block
 constexpr int kKv8MinExp = -117;             // smallest exponent of a scale: its codes' steps stay normal in bf16
+constexpr int kKv8MaxExp = 120;              // the largest, that of bf16's largest values; its codes end at 240
 
 struct Kv8Ref {
     uint8_t *k, *v;

@@ -9,7 +9,10 @@
 // exponents and is exact but for values that become subnormal (below 2^-6 of the
 // scale). The scale of a block that is being filled never falls: tokens taken
 // back (positions written again) keep their mark on it. An infinity or NaN
-// becomes the NaN code and does not count in the scale.
+// becomes the NaN code and does not count in the scale. At the largest scale, 2^120,
+// codes end at 240: 256 2^120 is past bf16 (and fp32), so finite values from 248 2^120
+// on, which would round there, take 240 (at most 15 of their 255 steps off: within
+// half a step, 2^-4).
 #include <stdint.h>
 
 #include <algorithm>
@@ -50,6 +53,12 @@ __device__ __forceinline__ u32x2 from_fp8(uint32_t c, float scale) {
 __device__ __forceinline__ uint32_t rescale(uint32_t c, float up) {
     const u32x2 v = from_fp8(c, 1.0f);
     return to_fp8(v[0], v[1], up);
+}
+
+// codes past 240 as 240 (0x77), NaN too
+__device__ __forceinline__ uint32_t up_to_240(uint32_t c) {
+    const uint32_t over = ((((c & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7) * 0x7fu;
+    return (c & ~over) | (0x77777777u & over);
 }
 
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -172,7 +181,7 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, c
     m = max(max(red[0], red[1]), max(red[2], red[3]));
     int e = scale_exp(m), up = 0;
     if (lo > 0) {
-        const int eo = min(max((int)(__float_as_uint(old_s) >> 23 & 255) - 127, kKv8MinExp), 120);
+        const int eo = min(max((int)(__float_as_uint(old_s) >> 23 & 255) - 127, kKv8MinExp), kKv8MaxExp);
         e = max(e, eo);
         up = min(e - eo, 60);                      // (past 2^18 nothing is left of a code)
     }
@@ -184,6 +193,7 @@ __global__ __launch_bounds__(256) void k_kv8_append(Kv8SeqsN<N> sq, Kv8Ref kv, c
         const u32x4 xi = __builtin_bit_cast(u32x4, x[i]);
         const uint32_t x0 = xi[0], x1 = xi[1], x2 = xi[2], x3 = xi[3];
         uint32_t c0 = to_fp8(x0, x1, scale), c1 = to_fp8(x2, x3, scale);
+        if (e == kKv8MaxExp) c0 = up_to_240(c0), c1 = up_to_240(c1);
         if (__any((int)wild)) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {

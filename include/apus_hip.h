@@ -652,7 +652,8 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
  * positions as above, K and V of a kv head as e4m3 codes, with one scale each
  * for K and V of every block and kv head, a power of two 2^e in fp32: e is the
  * smallest integer >= -117 with amax <= 448 2^e over the block's positions, a
- * code is value / 2^e rounded to nearest even. A block that is written in
+ * code is value / 2^e rounded to nearest even (at e = 120, the largest, to 240 at
+ * most: every finite value stays finite). A block that is written in
  * several calls keeps what it holds of the positions before pos0: where new
  * tokens need a larger scale, its codes are rounded again at that scale (exact,
  * but for values that fall below 2^-6 of it). The scale of a block that is

@@ -1,9 +1,32 @@
 """The 8-bit KV cache on the GPU where its calls are at their limits."""
+import numpy as np
 import pytest
 
-from test_gpu_kv8 import Setup
+import kv8_ref as R
+from test_gpu_kv8 import Setup, check_row, cum, dev, make
 
 pytestmark = pytest.mark.gpu
+TOP = 240.0 * 2.0 ** 120                   # the largest finite value: 256 2^120 is no bf16
+
+
+class Cache(R.Cache):
+    """The reference's cache up to bf16's largest value: codes at 2^120 end at 240."""
+
+    def append(self, row, pos0, k, v):
+        super().append(row, pos0, k, v)
+        c, mag = self.codes[row], self.codes[row] & 0x7f
+        at = (self.exps[row].repeat(R.BLK, 0) == 120)[..., None] & (mag > 0x77) & (mag < 0x7f)
+        self.codes[row] = np.where(at, c & 0x80 | 0x77, c)
+
+
+def refill(s):
+    """The caches of a Setup from its k and v again."""
+    n = s.ctx + s.new
+    c = cum(n)
+    s.hip.kv8_append(s.kv, s.rows, c, np.zeros(len(n), np.int32), dev(s.k), dev(s.v))
+    s.ref = Cache(s.nkv, len(n), s.max_blocks)
+    for i in range(len(n)):
+        s.ref.append(s.row(i), 0, s.k[c[i]:c[i + 1]], s.v[c[i]:c[i + 1]])
 
 
 @pytest.mark.parametrize("ctx,new", [
@@ -13,3 +36,39 @@ def test_prefill_split_beside_idle_rows(hip, ctx, new):
     """Keys in parts, beside sequences without tokens or cached positions."""
     s = Setup(hip, 110 + len(ctx) + new[-1], 2, ctx, new, True)
     s.check(s.call(hip.attn_prefill_kv8))
+
+
+def test_largest_values_stay_finite(hip):
+    """Every bf16 value from 2^127 on, in blocks of their own and with smaller ones
+    before and after them in the block; infinities and NaN beside them are NaN."""
+    kv, ref = make(hip, None, 1, 3, 2, False), Cache(1, 3, 2)
+    big = np.arange(0x7f00, 0x7f80).astype(np.uint16)
+    x = np.concatenate((big, big | 0x8000))[None].repeat(64, 0)                    # [64][256]
+    small = R.bf16(np.random.default_rng(7).normal(size=(64, R.D)) * 2.0 ** np.arange(60, 124).repeat(R.D).reshape(64, R.D))
+    wild = x[:3].copy()
+    wild[:, ::5], wild[:, 1::7] = 0x7f80, 0xffc0
+    for row, pieces in enumerate(([x], [small[:9], x[:1], small[9:30], x[:12], small[:10]], [x[:5], wild, small[:40]])):
+        pos = 0
+        for p in pieces:
+            hip.kv8_append(kv, None, cum([0] * row + [len(p)] + [0] * (2 - row)), [pos if r == row else 0 for r in range(3)],
+                           dev(p), dev(p[::-1].copy()))
+            ref.append(row, pos, p, p[::-1])
+            pos += len(p)
+        check_row(hip, kv, ref, row, 0, pos)
+    assert np.abs(ref.values(0, 0, 64)[0]).max() == TOP
+
+
+@pytest.mark.parametrize("f", ["attn_decode_kv8", "attn_prefill_kv8"])
+@pytest.mark.parametrize("value", [0x7f7f, 0xff78, 0x7f77])
+def test_large_v_of_a_later_token(hip, f, value):
+    """A value at the end of bf16's range in a position that earlier tokens do not
+    attend to: their rows are means of what they see."""
+    s = Setup(hip, 137, 2, [61, 40], [4, 4] if f == "attn_decode_kv8" else [12, 9], False)
+    n = s.ctx + s.new
+    c = cum(n)
+    for i in range(2):
+        s.v[c[i + 1] - 1, 5::9] = value
+    refill(s)
+    y = s.call(getattr(hip, f))
+    s.check(y)
+    assert np.isfinite(R.f64(y)).all()
