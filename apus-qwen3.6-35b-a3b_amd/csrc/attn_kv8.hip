@@ -51,7 +51,7 @@ constexpr int kRows = 32, kWaves = 4;
 constexpr float kEps = 1e-6f;
 constexpr float kL2E = 1.44269504088896341f;
 constexpr int QP = D + 8, AP = D + 4;        // LDS pitches of q rows and of outputs
-// t may pass M by this much before M moves: 2^10 a term, far from overflow
+// t may pass M by this much before M moves: 2^10 a term (kv8_v_up: no sum overflows)
 constexpr float kSlack = 10.0f;
 
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
@@ -271,6 +271,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
             idn = kv8_id_u(kv, row, min(j + 2 * kWaves, last));
             __builtin_amdgcn_sched_barrier(0);
             const bool tail = (j + 1) * KEYS > p0 + 1;     // some row does not see some key
+            const float up = (float)kv8_v_up(vs);
             bf16x8 pb[RB];                                 // the lane's 8 keys
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) {
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_attn(
                         if (i / 4 * 16 + i % 4 > lim) t[i] = -INFINITY;
                 }
                 const float mx = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])),
-                                       fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+                                       fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7]))) + up;
                 if (__any(mx > M[rb] + kSlack)) {          // (always at a row's first keys)
                     const float m = fmaxf(M[rb], row_max(mx));
                     const float d = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M[rb] - m);

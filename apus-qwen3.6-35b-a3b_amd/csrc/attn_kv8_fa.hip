@@ -150,7 +150,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Cu
         id[u] = id_of(min(b0 + (st + 1) * KS + u, last));
     };
     // a thread's pieces (kv8.h) to their places in LDS
-    float cs = 0.0f;                                       // the scale of this wavefront's K
+    float cs = 0.0f;                                       // of this wavefront's block: K's scale,
+    int up = 0;                                            // and kv8_v_up
     auto put = [&](int st, int u, int buf) {
         const float vs = uni(next.sc[1]);
         char *const kd = kl(buf, u) + (tid / 256 * 16 + tid % 16) * KP + tid / 16 % 16 * 32;
@@ -177,7 +178,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Cu
 #pragma unroll
         for (int w = 0; w < 4; w++)
             *reinterpret_cast<u32x2 *>(vd + (w / 2 * 16 * VP + w % 2 * 32)) = widen4(c4[w], vs);
-        if (KS == 1 || u == kg) cs = uni(next.sc[0]);
+        if (KS == 1 || u == kg) {
+            cs = uni(next.sc[0]);
+            up = kv8_v_up(vs);
+        }
     };
     fetch(0, 0);
 
@@ -285,6 +289,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Cu
     for (int st = 0; st < steps; st++) {
         const int buf = st & 1, k0 = (b0 + st * KS + kg) * KEYS;
         const float csn = cs;
+        const int upn = up;
         fetch(min(st + 1, steps - 1), 0);
         __syncthreads();
         bf16x8 pb[2];
@@ -319,7 +324,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void k_kv8_fa(Kv8SeqsN<N> sq, Kv8Cu
             float mx = S[0];
 #pragma unroll
             for (int e = 1; e < 16; e++) mx = fmaxf(mx, S[e]);
-            mx *= sf;
+            mx = mx * sf + (float)upn;
             if (__any(mx > M + kSlack)) {
                 const float m = fmaxf(M, max32(mx));
                 const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - m);

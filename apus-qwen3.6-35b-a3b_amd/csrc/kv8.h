@@ -139,6 +139,16 @@ __device__ __forceinline__ uint32_t kv8_nan_codes(uint32_t c) {
     return ((((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
 }
 
+// Weights p = 2^(t - M) go into the sums of p v as they are, up to 2^10 each (M
+// moves when t passes it by 10), for up to 2^24 keys: fp32 holds the sums while a
+// block's scale of V is at most 2^84 (values below 2^93). For a block past that M is
+// formed as if its scores were higher by so many powers of two, which makes its
+// weights, and all others, as much smaller: no sum passes 2^(24 + 10 + 93) = 2^127.
+// (A weight below 2^-126 is 0, so at the largest scale one below 2^-90 of the largest.)
+__device__ __forceinline__ int kv8_v_up(float vs) {
+    return max((int)(__float_as_uint(vs) >> 23 & 255) - (127 + 84), 0);
+}
+
 // Host checks, the same with and without a device.
 // The batch against the cache: offsets, positions, rows (distinct where tokens
 // are written). Fills r and the number of tokens.

@@ -58,6 +58,50 @@ def test_largest_values_stay_finite(hip):
     assert np.abs(ref.values(0, 0, 64)[0]).max() == TOP
 
 
+def huge(rng, shape, small=0.0):
+    """Values of both signs from 2^120 to bf16's largest; a share of them near 1."""
+    x = rng.choice([-1.0, 1.0], shape) * 2.0 ** rng.uniform(120.0, 127.99, shape)
+    return R.bf16(np.where(rng.random(shape) < small, rng.normal(size=shape), x))
+
+
+BATCHES = {
+    "decode": [([100, 900], [1, 2]), ([0, 1, 40], [4, 3, 1]), ([7000], [3]), ([30000], [1])],
+    "prefill": [([0], [40]), ([64, 3], [33, 70]), ([5000], [20])],
+}
+
+
+@pytest.mark.parametrize("f,ctx,new", [(f, *b) for f in BATCHES for b in BATCHES[f]])
+@pytest.mark.parametrize("kind", ["same sign", "both", "some blocks", "rising scores", "tiny"])
+def test_sums_of_large_and_tiny_v(hip, f, ctx, new, kind):
+    """y is a mean of v whatever v's size: no sum on the way leaves fp32."""
+    s = Setup(hip, 130 + len(ctx) + new[-1], 2, ctx, new, True)
+    rng = np.random.default_rng(3)
+    s.v = huge(rng, s.v.shape)
+    if kind == "same sign":
+        s.v &= 0x7fff
+    elif kind == "some blocks":
+        calm = np.arange(len(s.v)) // 64 % 3 > 0           # (most blocks have values near 1 alone)
+        s.v[calm] = R.bf16(rng.normal(size=(int(calm.sum()), s.v.shape[1])))
+    elif kind == "rising scores":
+        s.v &= 0x7fff
+        up = np.linspace(0.1, 6.0, len(s.k))[:, None]
+        s.k = R.bf16(R.f64(s.k) * up)
+    elif kind == "tiny":
+        s.v = R.bf16(rng.normal(size=s.v.shape) * 2.0 ** -110)
+    refill(s)
+    s.check(s.call(getattr(hip, f"attn_{f}_kv8")))
+
+
+def test_sums_of_large_v_many_tokens(hip):
+    """The same with tiles of 32 tokens."""
+    rng = np.random.default_rng(19)
+    B = 160
+    s = Setup(hip, 131, 2, rng.integers(0, 200, B), rng.integers(5, 75, B), True)
+    s.v = huge(rng, s.v.shape, 0.3)
+    refill(s)
+    s.check(s.call(hip.attn_prefill_kv8), range(3, B, 31))
+
+
 @pytest.mark.parametrize("f", ["attn_decode_kv8", "attn_prefill_kv8"])
 @pytest.mark.parametrize("value", [0x7f7f, 0xff78, 0x7f77])
 def test_large_v_of_a_later_token(hip, f, value):
