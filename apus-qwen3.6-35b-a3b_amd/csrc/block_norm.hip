@@ -187,13 +187,28 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_block_norm(NormArgs a
     }
 }
 
-template <class H> int launch(const NormArgs &a, bool vec) {
+// (rows of a launch: with 512 threads a row 2^31 threads, of the 2^32 - 1 that a
+// launch can have; more rows take several)
+constexpr size_t kLaunchRows = (size_t)1 << 22;
+
+template <class H> int launch(const NormArgs &all, bool vec) {
+    NormArgs a = all;
     auto go = [&](auto v, auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value;
-        APUS_TIMED("k_block_norm",
-                   k_block_norm<H, decltype(v)::value, TPR, decltype(nv)::value>
-                       <<<cdiv((size_t)a.rows, TPR < 256 ? 256 / TPR : 1), TPR > 256 ? TPR : 256, 0, stream()>>>(a));
-        return launch_check("k_block_norm");
+        for (size_t r = 0; r < (size_t)all.rows; r += kLaunchRows) {
+            auto from = [&](auto *p, size_t ld) { return p ? p + r * ld : p; };
+            a.y = from(all.y, a.ldy);
+            a.gate = from(all.gate, a.ldg);
+            a.h = (const H *)all.h + r * a.ldh;
+            a.h_out = from((H *)all.h_out, a.ldo);
+            a.x = from(all.x, a.ldx);
+            a.rows = (int)std::min(kLaunchRows, (size_t)all.rows - r);
+            APUS_TIMED("k_block_norm",
+                       k_block_norm<H, decltype(v)::value, TPR, decltype(nv)::value>
+                           <<<cdiv((size_t)a.rows, TPR < 256 ? 256 / TPR : 1), TPR > 256 ? TPR : 256, 0, stream()>>>(a));
+            if (int e = launch_check("k_block_norm")) return e;
+        }
+        return (int)kOk;
     };
     auto size = [&](auto v) {
         const std::integral_constant<int, 64> one;
