@@ -35,7 +35,6 @@
 #include <algorithm>
 #include <new>
 #include <type_traits>
-#include <utility>
 
 #include "apus_dev.h"
 #include "apus_host.h"
@@ -544,40 +543,43 @@ Runs cut_runs(size_t total, int32_t whole) {
 namespace apus {
 
 int attn_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
-                   const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
-                   const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T) {
+                   const int32_t *cu, const int32_t *pos0, bool writes, const ApusHipKv8Cache *kv, Kv8Ref *r, size_t *T) {
     if (int e = attn_check_layer(L)) return e;
     if (!w) return set_error(kErrArgument, "NULL workspace");
     if (w->device != current_device())
         return set_error(kErrArgument, "the workspace is on device %d, the library on %d", w->device, current_device());
     if (w->nkv != L->nkv || w->rot != L->rot || w->theta != L->theta)
         return set_error(kErrArgument, "the workspace was made for a layer of other dims");
-    if (!k != !v) return set_error(kErrArgument, "k and v are both given or both NULL");
-    if (int e = kv8_check(kv, L->nkv, B, rows, cu, pos0, k != nullptr, r, T)) return e;
+    if (int e = kv8_check(kv, L->nkv, B, rows, cu, pos0, writes, r, T)) return e;
     if (!*T) return kOk;
     for (size_t s = 0; s < B; s++)
         if (cu[s + 1] > cu[s] && (size_t)pos0[s] + (size_t)(cu[s + 1] - cu[s]) > w->max_pos)
             return set_error(kErrArgument, "sequence %zu reaches position %lld, the workspace's tables %zu", s,
                              (long long)pos0[s] + (cu[s + 1] - cu[s]), w->max_pos);
-    if (!L->qn_w || !L->kn_w || !qg || !y) return set_error(kErrArgument, "NULL operand");
-    if ((uintptr_t)qg % 16 || (uintptr_t)y % 16 || (uintptr_t)k % 16 || (uintptr_t)v % 16 ||
-        (uintptr_t)L->qn_w % 16 || (uintptr_t)L->kn_w % 16)
+    if (!L->qn_w || !L->kn_w) return set_error(kErrArgument, "NULL operand");
+    if ((uintptr_t)L->qn_w % 16 || (uintptr_t)L->kn_w % 16)
         return set_error(kErrUnsupported, "the attention operands need 16-byte alignment");
-    const size_t ny = *T * L->nh * D * 2, nk = *T * L->nkv * D * 2, nb = kv->blocks * L->nkv * kKv8Bytes;
+    if (writes && (kv8_overlap_cache(kv, L->nkv, L->qn_w, D * 2) || kv8_overlap_cache(kv, L->nkv, L->kn_w, D * 2)))
+        return set_error(kErrArgument, "an input overlaps the cache");
+    return kOk;
+}
+
+int attn_kv8_check_operands(const ApusHipAttnLayer *L, size_t T, const uint16_t *qg, const uint16_t *k,
+                            const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y) {
+    if (!k != !v) return set_error(kErrArgument, "k and v are both given or both NULL");
+    if (!T) return kOk;
+    if (!qg || !y) return set_error(kErrArgument, "NULL operand");
+    if ((uintptr_t)qg % 16 || (uintptr_t)y % 16 || (uintptr_t)k % 16 || (uintptr_t)v % 16)
+        return set_error(kErrUnsupported, "the attention operands need 16-byte alignment");
+    const size_t ny = T * L->nh * D * 2, nk = T * L->nkv * D * 2;
     if (kv8_overlap(y, ny, qg, 2 * ny) || (k && (kv8_overlap(y, ny, k, nk) || kv8_overlap(y, ny, v, nk))) ||
-        kv8_overlap(y, ny, kv->k, nb) || kv8_overlap(y, ny, kv->v, nb) ||
-        kv8_overlap(y, ny, kv->scale, kv->blocks * L->nkv * 8) ||
-        kv8_overlap(y, ny, L->qn_w, D * 2) || kv8_overlap(y, ny, L->kn_w, D * 2))
+        kv8_overlap_cache(kv, L->nkv, y, ny) || kv8_overlap(y, ny, L->qn_w, D * 2) || kv8_overlap(y, ny, L->kn_w, D * 2))
         return set_error(kErrArgument, "y overlaps an input");
     if (kv->block_table && kv8_overlap(y, ny, kv->block_table, kv->max_rows * kv->max_blocks * 4))
         return set_error(kErrArgument, "y overlaps the block table");
-    if (k) {                               // (the cache is written)
-        const std::pair<const void *, size_t> in[] = {{qg, 2 * ny}, {k, nk}, {v, nk}, {L->qn_w, D * 2}, {L->kn_w, D * 2}};
-        for (const auto &[p, n] : in)
-            if (kv8_overlap(p, n, kv->k, nb) || kv8_overlap(p, n, kv->v, nb) ||
-                kv8_overlap(p, n, kv->scale, kv->blocks * L->nkv * 8))
-                return set_error(kErrArgument, "an input overlaps the cache");
-    }
+    if (k && (kv8_overlap_cache(kv, L->nkv, qg, 2 * ny) || kv8_overlap_cache(kv, L->nkv, k, nk) ||
+              kv8_overlap_cache(kv, L->nkv, v, nk)))       // (the cache is written)
+        return set_error(kErrArgument, "an input overlaps the cache");
     return kOk;
 }
 
@@ -640,9 +642,9 @@ bool attn_decode_kv8_fits(const ApusHipAttnKv8Work *w, size_t B, const int32_t *
 }
 
 int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
-                          const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
-                          const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T) {
-    if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, r, T)) return e;
+                          const int32_t *cu, const int32_t *pos0, bool writes, const ApusHipKv8Cache *kv, Kv8Ref *r,
+                          size_t *T) {
+    if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, writes, kv, r, T)) return e;
     if (B > w->max_seqs)
         return set_error(kErrArgument, "%zu sequences, the workspace holds %zu", B, w->max_seqs);
     for (size_t s = 0; s < B; s++)
@@ -710,7 +712,8 @@ int apus_hip_attn_decode_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, s
     APUS_ENABLED();
     Kv8Ref r;
     size_t T = 0;
-    if (int e = attn_decode_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, &r, &T)) return e;
+    if (int e = attn_decode_kv8_check(L, w, B, rows, cu, pos0, k || v, kv, &r, &T)) return e;
+    if (int e = attn_kv8_check_operands(L, T, qg, k, v, kv, y)) return e;
     if (int e = mx_ready()) return e;
     if (!T) return kOk;
     return attn_decode_kv8_run(L, w, B, rows, cu, pos0, qg, k, v, r, y);

@@ -548,7 +548,8 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
     APUS_ENABLED();
     Kv8Ref r;
     size_t T = 0;
-    if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, &r, &T)) return e;
+    if (int e = attn_kv8_check(L, w, B, rows, cu, pos0, k || v, kv, &r, &T)) return e;
+    if (int e = attn_kv8_check_operands(L, T, qg, k, v, kv, y)) return e;
     if (int e = mx_ready()) return e;
     if (!T) return kOk;
     // up to 4 new tokens a sequence: decode's kernels, whose tiles are 16 or 32 rows

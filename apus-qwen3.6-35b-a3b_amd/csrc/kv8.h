@@ -160,14 +160,18 @@ int kv8_append_run(const Kv8Ref &kv, size_t nkv, size_t B, const int32_t *rows, 
                    const int32_t *pos0, const uint16_t *k, size_t ldk, const uint16_t *v, size_t ldv,
                    const uint16_t *kn_w, const uint16_t *rope);
 bool kv8_overlap(const void *a, size_t na, const void *b, size_t nb);
+bool kv8_overlap_cache(const ApusHipKv8Cache *c, size_t nkv, const void *p, size_t n);    // with its arrays
 
-// Checks of the attention calls (decode's: with its limits), and decode itself.
+// Checks of the attention calls: of everything but their operands (the weights, the
+// batch against workspace and cache; writes: new rows go into it), decode's with its
+// limits; and of the operands, of T tokens.
 int attn_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
-                   const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
-                   const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T);
+                   const int32_t *cu, const int32_t *pos0, bool writes, const ApusHipKv8Cache *kv, Kv8Ref *r, size_t *T);
 int attn_decode_kv8_check(const ApusHipAttnLayer *L, const ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
-                          const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,
-                          const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y, Kv8Ref *r, size_t *T);
+                          const int32_t *cu, const int32_t *pos0, bool writes, const ApusHipKv8Cache *kv, Kv8Ref *r,
+                          size_t *T);
+int attn_kv8_check_operands(const ApusHipAttnLayer *L, size_t T, const uint16_t *qg, const uint16_t *k,
+                            const uint16_t *v, const ApusHipKv8Cache *kv, const uint16_t *y);
 bool attn_decode_kv8_fits(const ApusHipAttnKv8Work *w, size_t B, const int32_t *cu, const int32_t *pos0);
 int attn_decode_kv8_run(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B, const int32_t *rows,
                         const int32_t *cu, const int32_t *pos0, const uint16_t *qg, const uint16_t *k,

@@ -327,6 +327,11 @@ bool kv8_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
 
+bool kv8_overlap_cache(const ApusHipKv8Cache *c, size_t nkv, const void *p, size_t n) {
+    const size_t nb = c->blocks * nkv * kKv8Bytes;
+    return kv8_overlap(p, n, c->k, nb) || kv8_overlap(p, n, c->v, nb) || kv8_overlap(p, n, c->scale, c->blocks * nkv * 8);
+}
+
 int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *rows, const int32_t *cu,
               const int32_t *pos0, bool writes, Kv8Ref *r, size_t *tokens) {
     if (!c || !c->k || !c->v || !c->scale) return set_error(kErrArgument, "bad 8-bit KV cache descriptor");

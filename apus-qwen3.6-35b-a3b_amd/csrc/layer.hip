@@ -91,11 +91,10 @@ int gdn_layer_run(const ApusHipGdnLayer *L, const ApusHipGdnProj *P, size_t B,
 }
 
 // The full-attention layer: wq | wk | wv -> mixer -> wo. mixer(qg, k, v, y): the
-// decode mixer on the caller's cache; check(qg, k, v, y), before anything runs:
-// its own checks of its arguments.
-template <class Check, class Mixer>
+// decode mixer on the caller's cache.
+template <class Mixer>
 int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B, const int32_t *cu,
-                   const uint16_t *ln1, uint16_t *ao, Check check, Mixer mixer) {
+                   const uint16_t *ln1, uint16_t *ao, Mixer mixer) {
     if (int r = attn_check_layer(L)) return r;
     if (!P) return set_error(kErrArgument, "NULL projections");
     if (B == 0) return kOk;
@@ -117,7 +116,6 @@ int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B
     uint16_t *v = (uint16_t *)scratch(kScratchLayerC, T * nk * 2);
     uint16_t *y = (uint16_t *)scratch(kScratchLayerY, T * no * 2);
     if (!qg || !k || !v || !y) return kErrHip;
-    if (int r = check(qg, k, v, y)) return r;
     GemmSegs in{};
     in.n = 3;
     in.row0[1] = (int)nq;
@@ -139,7 +137,7 @@ int attn_layer_run(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B
 // or null for the flat cache
 int attn_layer_kv(const ApusHipAttnLayer *L, const ApusHipAttnProj *P, size_t B, const int32_t *rows,
                   const int32_t *cu, const int32_t *pos0, const uint16_t *ln1, const KvRef &kv, uint16_t *ao) {
-    return attn_layer_run(L, P, B, cu, ln1, ao, [](auto...) { return (int)kOk; },
+    return attn_layer_run(L, P, B, cu, ln1, ao,
                           [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, uint16_t *y) {
         return attn_decode_kv(L, B, cu, pos0, rows, qg, k, v, kv, y);
     });
@@ -190,12 +188,14 @@ int apus_hip_attn_layer_decode_kv8(const ApusHipAttnLayer *L, const ApusHipAttnP
                                    const ApusHipKv8Cache *kv, uint16_t *ao) {
     APUS_READY();
     Kv8Ref r;
+    size_t T = 0;
+    // (before the scratch is sized by a number of tokens that may be refused)
+    if (int e = attn_decode_kv8_check(L, w, B, rows, cu, pos0, true, kv, &r, &T)) return e;
+    if (!P) return set_error(kErrArgument, "NULL projections");
+    if (int e = mx_ready()) return e;
+    if (!T) return kOk;
     return attn_layer_run(L, P, B, cu, ln1, ao,
-                          [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, const uint16_t *y) {
-        size_t T = 0;
-        if (int e = attn_decode_kv8_check(L, w, B, rows, cu, pos0, qg, k, v, kv, y, &r, &T)) return e;
-        return mx_ready();
-    }, [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, uint16_t *y) {
+                          [&](const uint16_t *qg, const uint16_t *k, const uint16_t *v, uint16_t *y) {
         return attn_decode_kv8_run(L, w, B, rows, cu, pos0, qg, k, v, r, y);
     });
 }

@@ -1,9 +1,11 @@
 """The 8-bit KV cache on the GPU where its calls are at their limits."""
 import numpy as np
 import pytest
+import torch
 
 import kv8_ref as R
 from test_gpu_kv8 import Setup, check_row, cum, dev, make
+from test_gpu_kv8_step import H, MAX, Model, empty
 
 pytestmark = pytest.mark.gpu
 TOP = 240.0 * 2.0 ** 120                   # the largest finite value: 256 2^120 is no bf16
@@ -116,3 +118,35 @@ def test_large_v_of_a_later_token(hip, f, value):
     y = s.call(getattr(hip, f))
     s.check(y)
     assert np.isfinite(R.f64(y)).all()
+
+
+def test_layer_refused_before_its_scratch(hip):
+    """The layer call on an 8-bit cache refuses a bad batch before it takes scratch
+    for so many tokens, and a bad workspace or cache where there are no tokens."""
+    m = Model(hip, 7)
+    T = 40000                              # (0.65 GB of q rows, were it to go on)
+    ln, ao = empty(T, H).zero_(), empty(T, H).zero_()
+    call = lambda cu, pos, rows=None, work=m.work, kv=m.kv: hip.attn_layer_decode_kv8(               # noqa: E731
+        m.layer, m.proj, work, rows, cu, pos, ln[:cu[-1]], kv, ao[:cu[-1]])
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for cu, pos, rows, match in (([0, T], [0], [m.rows[0]], "overflows"), ([0, T // 2, T], [0, 0], m.rows[:2], "overflows"),
+                                 ([0] + [MAX * 32 * i for i in range(1, 5)], [0] * 4, m.rows, "0..4 new"),
+                                 ([0, 1], [MAX * 32], [m.rows[0]], "overflows")):
+        with pytest.raises(hip.ApusHipError, match=match):
+            call(cu, pos, rows)
+    assert torch.cuda.mem_get_info()[0] == free
+    gone = hip.AttnKv8Work(m.layer, 4, 64)
+    gone.destroy()
+    bad = m.pool.cache(0)
+    bad.scale = None
+    for cu, pos in (([0], []), ([0, 0], [0])):
+        call(cu, pos, m.rows[:len(pos)])
+        with pytest.raises(hip.ApusHipError, match="workspace"):
+            call(cu, pos, m.rows[:len(pos)], work=gone)
+        with pytest.raises(hip.ApusHipError, match="descriptor"):
+            call(cu, pos, m.rows[:len(pos)], kv=bad)
+    torch.cuda.synchronize()
+    assert not ao.any()
+    for w in (m.work, m.mwork, m.pool):
+        w.destroy()
