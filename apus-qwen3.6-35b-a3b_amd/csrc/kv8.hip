@@ -304,8 +304,9 @@ int32_t touched(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n - 1) / KEYS 
 
 constexpr size_t kMaxPitch = (size_t)1 << 30, kMaxElements = (size_t)1 << 40;
 
-// rows of k or v: T of them, n elements each, apart from the cache
-int check_rows(const ApusHipKv8Cache *c, const void *p, size_t ld, size_t nkv, size_t T, const char *what) {
+// rows of k or v: T of them, n elements each, apart from the cache (and its table,
+// where they are written)
+int check_rows(const ApusHipKv8Cache *c, const void *p, size_t ld, size_t nkv, size_t T, const char *what, bool written) {
     const size_t n = nkv * D;
     if (!p) return set_error(kErrArgument, "NULL %s", what);
     if (ld < n) return set_error(kErrArgument, "%s rows of %zu elements with pitch %zu", what, n, ld);
@@ -316,6 +317,8 @@ int check_rows(const ApusHipKv8Cache *c, const void *p, size_t ld, size_t nkv, s
     if (block_overlaps(c->k, nb, p, ld * 2, n * 2, T) || block_overlaps(c->v, nb, p, ld * 2, n * 2, T) ||
         block_overlaps(c->scale, c->blocks * nkv * 8, p, ld * 2, n * 2, T))
         return set_error(kErrArgument, "the %s rows overlap the cache", what);
+    if (written && c->block_table && block_overlaps(c->block_table, c->max_rows * c->max_blocks * 4, p, ld * 2, n * 2, T))
+        return set_error(kErrArgument, "the %s rows overlap the block table", what);
     return kOk;
 }
 
@@ -348,6 +351,8 @@ int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *row
     const size_t nb = c->blocks * nkv * kKv8Bytes, sb = c->blocks * nkv * 8;
     if (kv8_overlap(c->k, nb, c->v, nb) || kv8_overlap(c->k, nb, c->scale, sb) || kv8_overlap(c->v, nb, c->scale, sb))
         return set_error(kErrArgument, "overlapping 8-bit KV cache arrays");
+    if (c->block_table && kv8_overlap_cache(c, nkv, c->block_table, c->max_rows * c->max_blocks * 4))
+        return set_error(kErrArgument, "the block table overlaps the 8-bit KV cache arrays");
     *r = Kv8Ref{c->k, c->v, c->scale, c->block_table, (int32_t)c->max_blocks, (uint32_t)c->blocks};
     *tokens = 0;
     if (!B) return kOk;
@@ -413,8 +418,8 @@ int apus_hip_kv8_append(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const i
     size_t T = 0;
     if (int e = kv8_check(kv, nkv, B, rows, cu, pos0, true, &r, &T)) return e;
     if (T) {
-        if (int e = check_rows(kv, k, ldk, nkv, T, "k")) return e;
-        if (int e = check_rows(kv, v, ldv, nkv, T, "v")) return e;
+        if (int e = check_rows(kv, k, ldk, nkv, T, "k", false)) return e;
+        if (int e = check_rows(kv, v, ldv, nkv, T, "v", false)) return e;
     }
     if (int e = mx_ready()) return e;
     if (!T) return kOk;
@@ -428,8 +433,8 @@ int apus_hip_kv8_read(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const int
     size_t T = 0;
     if (int e = kv8_check(kv, nkv, B, rows, cu, pos0, false, &r, &T)) return e;
     if (T) {
-        if (int e = check_rows(kv, k, ldk, nkv, T, "k")) return e;
-        if (int e = check_rows(kv, v, ldv, nkv, T, "v")) return e;
+        if (int e = check_rows(kv, k, ldk, nkv, T, "k", true)) return e;
+        if (int e = check_rows(kv, v, ldv, nkv, T, "v", true)) return e;
         if (rows_overlap(k, ldk * 2, nkv * D * 2, v, ldv * 2, nkv * D * 2, T))
             return set_error(kErrArgument, "the k rows overlap the v rows");
     }
