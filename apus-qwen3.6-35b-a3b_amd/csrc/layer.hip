@@ -192,6 +192,10 @@ int apus_hip_attn_layer_decode_kv8(const ApusHipAttnLayer *L, const ApusHipAttnP
     // (before the scratch is sized by a number of tokens that may be refused)
     if (int e = attn_decode_kv8_check(L, w, B, rows, cu, pos0, true, kv, &r, &T)) return e;
     if (!P) return set_error(kErrArgument, "NULL projections");
+    const size_t bytes = T * P->hidden * 2;
+    if (T && (kv8_overlap_cache(kv, L->nkv, ln1, bytes) || kv8_overlap_cache(kv, L->nkv, ao, bytes) ||
+              (kv->block_table && kv8_overlap(ao, bytes, kv->block_table, kv->max_rows * kv->max_blocks * 4))))
+        return set_error(kErrArgument, "ln1 or ao overlaps the cache or its block table");
     if (int e = mx_ready()) return e;
     if (!T) return kOk;
     return attn_layer_run(L, P, B, cu, ln1, ao,

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import kv8_ref as R
-from test_gpu_kv8 import Setup, check_row, cum, dev, make
+from test_gpu_kv8 import Setup, check_row, cum, dev, make, table
 from test_gpu_kv8_step import H, MAX, Model, empty
 
 pytestmark = pytest.mark.gpu
@@ -148,5 +148,25 @@ def test_layer_refused_before_its_scratch(hip):
             call(cu, pos, m.rows[:len(pos)], kv=bad)
     torch.cuda.synchronize()
     assert not ao.any()
+    for w in (m.work, m.mwork, m.pool):
+        w.destroy()
+
+
+def test_layer_operands_apart_from_the_cache(hip):
+    """ln1 and ao may not lie in the cache's arrays, nor ao in its block table."""
+    m = Model(hip, 8)
+    t, blocks = table(np.random.default_rng(1), 4, 512)    # (8 KiB: two rows of ao)
+    kv = hip.kv8_cache(m.kv.nkv, blocks, 512, block_table=t)
+    cu, pos = [0, 1, 2], [0, 0]
+    ln, ao = empty(2, H).zero_(), empty(2, H).zero_()
+    k, v, scale = (x.view(torch.int16).flatten()[:2 * H].view(2, H) for x in kv._tensors[:3])
+    over = t.view(torch.int16).flatten()[-2 * H:].view(2, H)
+    before = [x.clone().view(torch.uint8) for x in kv._tensors]
+    for args in ((k, ao), (v, ao), (scale, ao), (ln, k), (ln, v), (ln, scale), (ln, over)):
+        with pytest.raises(hip.ApusHipError, match="overlap"):
+            hip.attn_layer_decode_kv8(m.layer, m.proj, m.work, [0, 1], cu, pos, args[0], kv, args[1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, kv._tensors))
+    hip.attn_layer_decode_kv8(m.layer, m.proj, m.work, [0, 1], cu, pos, ln, kv, ao)
     for w in (m.work, m.mwork, m.pool):
         w.destroy()
