@@ -1098,8 +1098,8 @@ def _norm_rows(t, what, shape, f32):
 def block_norm(norm, y, h, h_out, x):
     """h_out = h + scale gate post(y), x = pre(h_out): y, x [T, hidden] bf16, h
     and h_out bf16 or fp32, rows of any pitch. y None: x = pre(h); x None: only
-    h_out. h_out may be h, x may be y. (norm takes up h's type: one norm is not for
-    two threads with h of different types.)"""
+    h_out. h_out may be h, x may be y. The residual's type is h's, whatever
+    norm.h_f32 says; norm itself is only read."""
     shape, n = h.shape, norm.hidden
     if len(shape) != 2 or shape[1] != n:
         raise ValueError(f"h: rows of {n} elements, not {tuple(shape)}")
@@ -1111,8 +1111,11 @@ def block_norm(norm, y, h, h_out, x):
     yp, ldy = (None, n) if y is None else _norm_rows(y, "y", shape, False)
     op, ldo = (None, n) if h_out is None else _norm_rows(h_out, "h_out", shape, f32)
     xp, ldx = (None, n) if x is None else _norm_rows(x, "x", shape, False)
-    norm.h_f32 = f32
-    rc = load().apus_hip_block_norm(C.addressof(norm), T, yp, ldy, hp, ldh, op, ldo, xp, ldx)
+    N = norm
+    if norm.h_f32 != f32:                  # (a copy of the call's own: another thread may be using norm)
+        N = BlockNorm.from_buffer_copy(norm)
+        N.h_f32 = f32
+    rc = load().apus_hip_block_norm(C.addressof(N), T, yp, ldy, hp, ldh, op, ldo, xp, ldx)
     if rc:
         raise ApusHipError(rc, last_error())
 

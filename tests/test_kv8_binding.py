@@ -1,6 +1,9 @@
-"""CPU checks of the Python binding of the 8-bit cache's calls: what it hands to
-the library of the tensors that it is given, which here lie in host memory (no
-call is made)."""
+"""CPU checks of the Python binding of the 8-bit cache's calls and the norms around
+a block: what it hands to the library of the tensors that it is given, which here
+lie in host memory (no call is made)."""
+import ctypes as C
+import threading
+
 import pytest
 import torch
 
@@ -47,3 +50,66 @@ def test_rows_of_heads_are_the_tensors_own(kv, f):
         bind(f, kv, x, x)
     none = torch.zeros(0, 1, 256, dtype=torch.bfloat16)
     bind(f, kv, none, none)
+
+
+@pytest.fixture
+def norm_calls(monkeypatch):
+    """What block_norm hands over: (the norm as the library would see it, its address)."""
+    got = []
+
+    class Lib:
+        @staticmethod
+        def apus_hip_block_norm(norm, *args):
+            got.append((H.BlockNorm.from_buffer_copy(C.string_at(norm, C.sizeof(H.BlockNorm))), norm))
+            return 0
+    monkeypatch.setattr(H, "_device", -1)
+    monkeypatch.setattr(H, "load", lambda: Lib)
+    return got
+
+
+def test_a_norm_is_only_read(norm_calls):
+    """One norm for bf16 and fp32 residuals, by turns: each call has its own type,
+    and the caller's descriptor stays as it was."""
+    w = torch.zeros(64, dtype=torch.bfloat16)
+    norm = H.block_norm_weights(64, w_pre=w, w_post=w, scale=0.5, eps=1e-5)
+    was = bytes(norm)
+    y = torch.zeros(3, 64, dtype=torch.bfloat16)
+    for dtype in (torch.bfloat16, torch.float32, torch.float32, torch.bfloat16, torch.float32):
+        h = torch.zeros(3, 64, dtype=dtype)
+        H.block_norm(norm, y, h, h, torch.empty_like(y))
+        seen = norm_calls[-1][0]
+        assert seen.h_f32 == (dtype == torch.float32) and bytes(norm) == was
+        assert (seen.hidden, seen.scale, seen.w_pre, seen.w_post) == (64, 0.5, w.data_ptr(), w.data_ptr())
+    norm.scale, norm.h_f32 = 2.0, 1                        # (what the caller changes counts from the next call on)
+    for dtype in (torch.float32, torch.bfloat16):
+        h = torch.zeros(3, 64, dtype=dtype)
+        H.block_norm(norm, y, h, h, torch.empty_like(y))
+        assert norm_calls[-1][0].scale == 2.0 and norm_calls[-1][0].h_f32 == (dtype == torch.float32)
+
+
+def test_two_threads_with_one_norm(norm_calls, monkeypatch):
+    """A call that waits inside the library keeps its type while another thread
+    calls with the other."""
+    w = torch.zeros(64, dtype=torch.bfloat16)
+    norm = H.block_norm_weights(64, w_pre=w)
+    inside, go, types = threading.Event(), threading.Event(), {}
+
+    class Lib:
+        @staticmethod
+        def apus_hip_block_norm(at, *args):
+            first = threading.current_thread().name == "first"
+            if first:
+                inside.set()
+                assert go.wait(30)
+            types[first] = H.BlockNorm.from_buffer_copy(C.string_at(at, C.sizeof(H.BlockNorm))).h_f32
+            return 0
+    monkeypatch.setattr(H, "load", lambda: Lib)
+    call = lambda dtype: H.block_norm(norm, None, torch.zeros(2, 64, dtype=dtype), None,             # noqa: E731
+                                      torch.zeros(2, 64, dtype=torch.bfloat16))
+    t = threading.Thread(target=call, args=(torch.float32,), name="first")
+    t.start()
+    assert inside.wait(30)
+    call(torch.bfloat16)
+    go.set()
+    t.join(30)
+    assert types == {True: 1, False: 0}
