@@ -946,6 +946,21 @@ def _total(cu):
     return int(cu[-1])
 
 
+class _BatchCall(BoundCall):
+    """A BoundCall whose offsets may be changed in place: never past the rows of
+    the tensors that it was made with."""
+    __slots__ = ("_cu", "_rows")
+
+    def __init__(self, f, args, keep, cu):
+        super().__init__(f, args, keep)
+        self._cu, self._rows = cu, _total(cu)
+
+    def __call__(self):
+        if self._cu[-1] > self._rows:
+            raise ValueError(f"cu: {self._cu[-1]} tokens, the call's tensors have {self._rows}")
+        super().__call__()
+
+
 def _kv8_rows_call(f, kv, rows, cu, pos0, k, v):
     B, rp, cp, pp, keep = _batch(rows, cu, pos0)
     n, T = kv.nkv * 256, _total(keep[1])
@@ -960,12 +975,13 @@ def _kv8_rows_call(f, kv, rows, cu, pos0, k, v):
         if m != T:
             raise ValueError(f"{what}: {m} rows, expected {T}")
         ld += [p, pitch]
-    return BoundCall(f, (C.addressof(kv), kv.nkv, B, rp, cp, pp, *ld), (kv, keep, k, v))
+    return _BatchCall(f, (C.addressof(kv), kv.nkv, B, rp, cp, pp, *ld), (kv, keep, k, v), keep[1])
 
 
 def kv8_append_bound(kv, rows, cu, pos0, k, v):
     """kv8_append as a BoundCall (rows, cu, pos0 as int32 numpy arrays may be
-    changed in place between calls; the tensors have cu's last entry of rows)."""
+    changed in place between calls; the tensors have cu's last entry of rows, and
+    offsets past them are refused)."""
     return _kv8_rows_call(load().apus_hip_kv8_append, kv, rows, cu, pos0, k, v)
 
 
@@ -1022,7 +1038,7 @@ def _attn_kv8_call(f, layer, work, rows, cu, pos0, qg, k, v, kv, y):
         raise ValueError(f"kv: a cache of {kv.nkv} heads, the layer has {nkv}")
     args = (C.addressof(layer), work.h, B, rp, cp, pp, _dense(qg, (T, nh, 2 * d), "qg"),
             _dense(k, (T, nkv, d), "k"), _dense(v, (T, nkv, d), "v"), C.addressof(kv), _dense(y, (T, nh * d), "y"))
-    return BoundCall(f, args, (layer, work, keep, qg, k, v, kv, y))
+    return _BatchCall(f, args, (layer, work, keep, qg, k, v, kv, y), keep[1])
 
 
 def attn_decode_kv8_bound(layer, work, rows, cu, pos0, qg, k, v, kv, y):

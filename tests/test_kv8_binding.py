@@ -4,6 +4,7 @@ lie in host memory (no call is made)."""
 import ctypes as C
 import threading
 
+import numpy as np
 import pytest
 import torch
 
@@ -113,3 +114,30 @@ def test_two_threads_with_one_norm(norm_calls, monkeypatch):
     go.set()
     t.join(30)
     assert types == {True: 1, False: 0}
+
+
+def test_bound_offsets_stay_in_the_tensors(kv, monkeypatch):
+    """Offsets changed in place after a call was bound: up to the tensors' rows."""
+    calls = []
+    x = torch.zeros(7, 512, dtype=torch.bfloat16)
+    layer = H.AttnLayer(16, 2, 256, 64, 1e7)
+    work = type("Work", (), {"h": None})
+    cu = np.array([0, 3, 7], np.int32)
+    pos = np.zeros(2, np.int32)
+    y = torch.zeros(7, 16 * 256, dtype=torch.bfloat16)
+    qg = torch.zeros(7, 16, 512, dtype=torch.bfloat16)
+    bound = [H.kv8_append_bound(kv, None, cu, pos, x, x), H.kv8_read_bound(kv, None, cu, pos, x, x.clone()),
+             H.attn_decode_kv8_bound(layer, work, None, cu, pos, qg, x, x, kv, y),
+             H.attn_prefill_kv8_bound(layer, work, None, cu, pos, qg, None, None, kv, y)]
+    for b in bound:
+        monkeypatch.setattr(b, "_f", lambda *a: calls.append(a) or 0)
+    for last, fits in ((7, True), (8, False), (5, True), (1 << 30, False), (7, True)):
+        cu[-1] = last
+        for b in bound:
+            calls.clear()
+            if fits:
+                b()
+            else:
+                with pytest.raises(ValueError, match="cu: "):
+                    b()
+            assert len(calls) == fits
