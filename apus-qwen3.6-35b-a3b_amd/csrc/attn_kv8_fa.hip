@@ -566,7 +566,6 @@ int apus_hip_attn_prefill_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, 
         if (!q.e[q.n].off) return (int)kOk;
         const Kv8Cut<N> cut = kv8_by_length(q, plan);
         const size_t grid = (size_t)q.e[q.n].off * nkv;
-        if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many tokens in one call");
         const int split0 = q.e[kv8_first_split(q, cut)].off;
         auto launch = [&](auto ks) {
             APUS_TIMED("k_kv8_fa", k_kv8_fa<decltype(ks)::value, N><<<(unsigned)grid, 64 * kWaves, 0, stream()>>>(

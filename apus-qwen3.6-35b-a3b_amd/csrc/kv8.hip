@@ -303,6 +303,10 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8SeqsN<N> sq, Kv8Ref kv, uin
 int32_t touched(int32_t pos0, int32_t n) { return n > 0 ? (pos0 + n - 1) / KEYS - pos0 / KEYS + 1 : 0; }
 
 constexpr size_t kMaxPitch = (size_t)1 << 30, kMaxElements = (size_t)1 << 40;
+// (block, kv head) pairs of a launch's new tokens: with two workgroups of 256 threads
+// each (cache), or two of 512 (prefill: a tile of 16 tokens and a head) it stays under
+// HIP's 2^32 threads. k and v of so many take 137 GB.
+constexpr size_t kMaxHeadBlocks = (size_t)1 << 22;
 
 // rows of k or v: T of them, n elements each, apart from the cache (and its table,
 // where they are written)
@@ -361,7 +365,7 @@ int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *row
     // the rows written to (no exception may leave an entry point)
     std::unique_ptr<int32_t[]> used(writes && rows ? new (std::nothrow) int32_t[B] : nullptr);
     if (writes && rows && !used) return set_error(kErrHip, "out of host memory");
-    size_t nused = 0;
+    size_t nused = 0, heads = 0;
     for (size_t s = 0; s < B; s++) {
         const int64_t n = (int64_t)cu[s + 1] - cu[s], end = (int64_t)pos0[s] + n;
         if (n < 0) return set_error(kErrArgument, "token offsets must ascend");
@@ -380,6 +384,11 @@ int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *row
                                  "positions", s, (long long)end, (long long)row, (long long)held * KEYS);
         }
         if (writes && n && rows) used[nused++] = (int32_t)row;
+        if (s % kKv8Seqs == 0) heads = 0;
+        heads += (size_t)touched(pos0[s], (int32_t)n) * nkv;
+        if (heads >= kMaxHeadBlocks)
+            return set_error(kErrUnsupported, "the new tokens of %d sequences touch %zu blocks and kv heads, of up to %zu",
+                             kKv8Seqs, heads, kMaxHeadBlocks - 1);
     }
     std::sort(used.get(), used.get() + nused);
     if (std::adjacent_find(used.get(), used.get() + nused) != used.get() + nused)
@@ -396,7 +405,6 @@ int kv8_append_run(const Kv8Ref &kv, size_t nkv, size_t B, const int32_t *rows, 
         constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
         const size_t grid = (size_t)q.e[q.n].off * nkv * 2;
         if (!grid) return (int)kOk;
-        if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many blocks in one call");
         if (kn_w)
             APUS_TIMED("k_kv8_append", k_kv8_append<true, N><<<(unsigned)grid, 256, 0, stream()>>>(
                                            q, kv, k, ldk, v, ldv, (int)nkv, kn_w, rope));
@@ -445,7 +453,6 @@ int apus_hip_kv8_read(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const int
         constexpr int N = sizeof(q.e) / sizeof(q.e[0]) - 1;
         const size_t grid = (size_t)q.e[q.n].off * nkv * 2;
         if (!grid) return (int)kOk;
-        if (grid > 0x7fffffff) return set_error(kErrUnsupported, "too many blocks in one call");
         APUS_TIMED("k_kv8_read", k_kv8_read<N><<<(unsigned)grid, 256, 0, stream()>>>(q, r, k, ldk, v, ldv, (int)nkv));
         return launch_check("k_kv8_read");
     });

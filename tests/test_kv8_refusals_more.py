@@ -2,7 +2,7 @@
 for a device (device addresses here are never read)."""
 import pytest
 
-from test_kv8_refusals import ARG, K, S, T, V, X, Y, cache, rows
+from test_kv8_refusals import ARG, K, S, T, UNS, V, X, Y, cache, rows
 
 PAGED = dict(block_table=T, max_blocks=8, max_rows=8)      # 256 bytes of table
 
@@ -17,3 +17,14 @@ def test_rows_are_not_read_over_the_block_table():
 def test_table_lies_apart_from_the_cache(f):
     for at in (K, V + 1024, S, S + 64 * 2 * 8 - 4, K - 252):
         assert rows(f, cache(**dict(PAGED, block_table=at)), rows=(0, 1), k=X, v=Y) == ARG
+
+
+@pytest.mark.parametrize("f", ["append", "read"])
+@pytest.mark.parametrize("nkv,lens", [(2, (1 << 26,)), (1, (1 << 27,)), (1024, (32 * 2048, 32 * 2048)), (1, (1 << 26, 1 << 26))])
+def test_no_more_blocks_than_a_launch_has(f, nkv, lens):
+    """2^22 (block, head) pairs and more: refused, not left to fail at the launch."""
+    cu = (0,) + tuple(sum(lens[:i + 1]) for i in range(len(lens)))
+    far = 1 << 46                          # (arrays of terabytes, apart)
+    c = cache(k=far, v=2 * far, scale=3 * far, blocks=1 << 23, max_blocks=1 << 22, max_rows=2)
+    assert rows(f, c, nkv=nkv, B=len(lens), cu=cu, pos=(0,) * len(lens), k=4 * far, ldk=nkv * 256, v=6 * far,
+                ldv=nkv * 256) == UNS
