@@ -170,3 +170,86 @@ def test_layer_operands_apart_from_the_cache(hip):
     hip.attn_layer_decode_kv8(m.layer, m.proj, m.work, [0, 1], cu, pos, ln, kv, ao)
     for w in (m.work, m.mwork, m.pool):
         w.destroy()
+
+
+# Prefill's own kernels (calls of up to 4 tokens a sequence are decode's): tiles of 16
+# tokens, the same with the keys in parts, tiles of 32 (work for every CU many times
+# over; a few sequences are checked)
+def prefill_batch(hip, kind, seed, **kw):
+    if kind == "tiles of 32":
+        rng = np.random.default_rng(29)
+        ctx, new = rng.integers(0, 200, 160), rng.integers(5, 75, 160)
+        ctx[:3], new[:3] = [0, 31, 200], [70, 33, 5]
+        return Setup(hip, seed, 2, ctx, new, True, **kw), [0, 1, 2, 80, 159]
+    ctx, new = ([37, 0], [5, 40]) if kind == "tiles of 16" else ([9000, 0], [6, 5])
+    return Setup(hip, seed, 2, ctx, new, True, **kw), None
+
+
+def prefill_call(s, kind):
+    """The call, having run the kernels that the batch is for."""
+    s.hip.timing_enable(True)
+    try:
+        y = s.call(s.hip.attn_prefill_kv8)
+        ran = [s.hip.timing_get(n)[1] for n in ("k_kv8_fa", "k_kv8_fa_combine", "k_kv8_attn")]
+    finally:
+        s.hip.timing_enable(False)
+    assert ran == [1, int(kind == "parts"), 0]
+    return y
+
+
+KERNELS = ["tiles of 16", "parts", "tiles of 32"]
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("q,k", [(0.0, 0.0), (2.0 ** -126, 0.0), (2.0 ** -126, 2.0 ** -133), (1.0, 0.0), (2.0 ** -126, 1.0),
+                                 (0.0, 1.0), (1.0, 2.0 ** 100)])
+def test_prefill_tiny_and_large_rows(hip, kind, q, k):
+    """Rows of zeros and of the smallest values: every key counts the same, masked
+    ones not at all; and k so large that one key has it all."""
+    s, picks = prefill_batch(hip, kind, 151)
+    rows = s.qg.reshape(-1, 2 * R.D)
+    rows[:, :R.D] = R.bf16(R.f64(rows[:, :R.D]) * q)
+    s.k = R.bf16(R.f64(s.k) * k)
+    refill(s)
+    s.check(prefill_call(s, kind), picks)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+def test_prefill_growing_scores(hip, kind):
+    """Scores that rise along the context, far past the first keys': the reference
+    point moves, and what was summed with it."""
+    s, picks = prefill_batch(hip, kind, 157, spread=0.1)
+    c = cum(s.ctx + s.new)
+    up = np.concatenate([np.linspace(0.1, 40.0, int(n)) for n in np.diff(c)])[:, None]
+    s.k = R.bf16(R.f64(s.k) * up)
+    refill(s)
+    s.check(prefill_call(s, kind), picks)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_prefill_nan_reaches_only_those_that_see_it(hip, kind, what):
+    """A NaN and an infinity in a new token's k or v: rows before it are as without
+    it; rows that see a NaN k are NaN, those that see NaN v are NaN in that dim."""
+    s, picks = prefill_batch(hip, kind, 163)
+    q = 0                                  # of the sequence: its third new token; head 1, dims 44 and 45
+    c = cum(s.ctx + s.new)
+    at, first, end = c[q] + s.ctx[q] + 2, s.cu[q] + 2, s.cu[q + 1]
+    x = s.k if what == "k" else s.v
+    x[at, 300], x[at, 301] = 0x7fc0, 0xff80
+    refill(s)
+    y = prefill_call(s, kind)
+    bad = np.zeros(y.shape, bool)
+    bad[first:end, 8:16, slice(44, 46) if what == "v" else slice(None)] = True
+    got = R.f64(y)
+    assert np.array_equal(np.isnan(got), bad)
+    x[at, 300:302] = 0                     # (does not count in the block's scale, as these do not)
+    refilled = Cache(2, len(s.ctx), s.max_blocks)
+    for i in picks or range(len(s.ctx)):
+        refilled.append(s.row(i), 0, s.k[c[i]:c[i + 1]], s.v[c[i]:c[i + 1]])
+    s.ref = refilled
+    s.check(y, [i for i in picks or range(len(s.ctx)) if i != q])
+    k, v = refilled.values(s.row(q), 0, int(s.ctx[q] + s.new[q]))
+    r, tol = R.attention(s.qg[s.cu[q]:end], s.w["qn_w"], int(s.ctx[q]), k, v, 1e7)
+    ok = ~bad[s.cu[q]:end]
+    assert (np.abs(got[s.cu[q]:end] - r) <= tol)[ok].all()
