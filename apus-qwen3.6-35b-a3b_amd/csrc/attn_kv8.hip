@@ -665,7 +665,7 @@ int apus_hip_attn_kv8_work_create(const ApusHipAttnLayer *L, size_t max_seqs, si
     if (!out) return set_error(kErrArgument, "NULL output");
     *out = nullptr;
     if (int r = attn_check_layer(L)) return r;
-    if (!max_seqs || max_seqs > ((size_t)1 << 24) || L->nkv > 1024 || !max_pos || max_pos > ((size_t)1 << 24))
+    if (!max_seqs || max_seqs > ((size_t)1 << 24) || L->nkv > kKv8MaxHeads || !max_pos || max_pos > ((size_t)1 << 24))
         return set_error(kErrUnsupported, "an attention workspace for %zu sequences, %zu kv heads, %zu positions",
                          max_seqs, L->nkv, max_pos);
     if (int r = mx_ready()) return r;

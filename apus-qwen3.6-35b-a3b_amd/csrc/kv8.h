@@ -29,6 +29,9 @@ constexpr int kKv8Bytes = kKv8Keys * kKv8D;  // bytes of a head's K or V block
 constexpr int kKv8MinExp = -117;             // smallest exponent of a scale: its codes' steps stay normal in bf16
 constexpr int kKv8MaxExp = 120;              // the largest, that of bf16's largest values; its codes end at 240
 
+constexpr size_t kKv8MaxHeads = 1024;        // kv heads, and blocks of a row (positions count in 32 bits)
+constexpr size_t kKv8MaxBlocks = (size_t)1 << 25;
+
 struct Kv8Ref {
     uint8_t *k, *v;
     float *scale;                            // [block][nkv][2]: K's, V's

@@ -342,8 +342,8 @@ bool kv8_overlap_cache(const ApusHipKv8Cache *c, size_t nkv, const void *p, size
 int kv8_check(const ApusHipKv8Cache *c, size_t nkv, size_t B, const int32_t *rows, const int32_t *cu,
               const int32_t *pos0, bool writes, Kv8Ref *r, size_t *tokens) {
     if (!c || !c->k || !c->v || !c->scale) return set_error(kErrArgument, "bad 8-bit KV cache descriptor");
-    if (!nkv || nkv > 1024) return set_error(kErrUnsupported, "%zu kv heads", nkv);
-    if (!c->blocks || c->blocks > 0x7fffffff || !c->max_blocks || c->max_blocks > ((size_t)1 << 25) ||
+    if (!nkv || nkv > kKv8MaxHeads) return set_error(kErrUnsupported, "%zu kv heads", nkv);
+    if (!c->blocks || c->blocks > 0x7fffffff || !c->max_blocks || c->max_blocks > kKv8MaxBlocks ||
         !c->max_rows || c->max_rows > 0x7fffffff)
         return set_error(kErrArgument, "8-bit KV cache: %zu blocks, %zu rows of %zu", c->blocks, c->max_rows,
                          c->max_blocks);

@@ -20,11 +20,13 @@
 #include <string.h>
 
 #include <algorithm>
+#include <exception>
 #include <vector>
 
 #include "../../include/apus_hip.h"
 #include "apus_host.h"
 #include "apus_rt.h"
+#include "kv8.h"
 
 using namespace apus;
 
@@ -74,13 +76,31 @@ extern "C" {
 
 static int kv_pool_make(size_t nlayers, size_t nkv, size_t d, size_t nblocks, size_t max_rows,
                         size_t max_blocks, bool kv8, ApusHipKvPool **out) {
-    APUS_READY();
+    if (int r = check_enabled()) return r;
     if (!out) return set_error(kErrArgument, "NULL output");
     *out = nullptr;
     if (!nlayers || !nkv || d != 256 || !nblocks || !max_rows || !max_blocks ||
         nblocks > 0x7fffffff || max_blocks > 0x7fffffff || max_rows > 0x7fffffff)
         return set_error(kErrArgument, "bad KV pool dimensions (d must be 256)");
-    auto *p = new ApusHipKvPool{};
+    // (what the calls on an 8-bit cache refuse; and no product of sizes below overflows)
+    if (kv8 && (nkv > kKv8MaxHeads || max_blocks > kKv8MaxBlocks))
+        return set_error(kErrUnsupported, "an 8-bit KV pool of %zu kv heads and rows of %zu blocks", nkv, max_blocks);
+    if (nkv > 0xffff) return set_error(kErrUnsupported, "%zu kv heads", nkv);
+    ApusHipKvPool *p = nullptr;
+    try {                                  // (no exception may leave an entry point)
+        p = new ApusHipKvPool{};
+        p->k.reserve(nlayers);
+        p->v.reserve(nlayers);
+        if (kv8) p->scale.reserve(nlayers);
+        p->htab.assign(max_rows * max_blocks, 0);
+        p->nused.assign(max_rows, -1);
+        p->free_blocks.reserve(nblocks);
+        p->free_rows.reserve(max_rows);
+    } catch (const std::exception &) {
+        delete p;
+        return set_error(kErrHip, "out of host memory for a KV pool of %zu layers, %zu blocks, %zu rows of %zu",
+                         nlayers, nblocks, max_rows, max_blocks);
+    }
     p->nlayers = nlayers;
     p->nkv = nkv;
     p->d = d;
@@ -96,6 +116,7 @@ static int kv_pool_make(size_t nlayers, size_t nkv, size_t d, size_t nblocks, si
         delete p;
         return r;
     };
+    if (int r = ensure_ready()) return fail(r);
     for (size_t l = 0; l < nlayers; l++) {
         void *a = nullptr, *b = nullptr, *c = nullptr;
         if (hipMalloc(&a, bytes) != hipSuccess)
@@ -112,8 +133,6 @@ static int kv_pool_make(size_t nlayers, size_t nkv, size_t d, size_t nblocks, si
     const size_t tbytes = (max_rows * max_blocks * 4 + 15) / 16 * 16;
     if (hipMalloc((void **)&p->dtab, tbytes) != hipSuccess)
         return fail(set_error(kErrHip, "hipMalloc of the block table failed"));
-    p->htab.assign(max_rows * max_blocks, 0);
-    p->nused.assign(max_rows, -1);
     for (size_t i = nblocks; i-- > 0;) p->free_blocks.push_back((int32_t)i);
     for (size_t i = max_rows; i-- > 0;) p->free_rows.push_back((int32_t)i);
     // entries past a row's blocks hold block 0: a valid address, never read

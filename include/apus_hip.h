@@ -698,7 +698,8 @@ int apus_hip_kv8_read(const ApusHipKv8Cache *kv, size_t nkv, size_t B, const int
                       uint16_t *v, size_t ldv);
 
 /* A KV pool (above) of 8-bit blocks: opened, reserved and closed by the same
- * calls; kv8_pool_cache gives a layer's descriptor (kv_pool_cache refuses it). */
+ * calls; kv8_pool_cache gives a layer's descriptor (kv_pool_cache refuses it). nkv up
+ * to 1024, max_blocks to 2^25, as in the calls on such a cache. */
 int apus_hip_kv8_pool_create(size_t nlayers, size_t nkv, size_t d, size_t nblocks,
                              size_t max_rows, size_t max_blocks, ApusHipKvPool **out);
 int apus_hip_kv8_pool_cache(const ApusHipKvPool *pool, size_t layer, ApusHipKv8Cache *out);
