@@ -953,12 +953,14 @@ class _BatchCall(BoundCall):
 
     def __init__(self, f, args, keep, cu):
         super().__init__(f, args, keep)
-        self._cu, self._rows = cu, _total(cu)
+        self._cu, self._rows = memoryview(cu), _total(cu)      # (the array itself, read as plain integers)
 
     def __call__(self):
         if self._cu[-1] > self._rows:
             raise ValueError(f"cu: {self._cu[-1]} tokens, the call's tensors have {self._rows}")
-        super().__call__()
+        rc = self._f(*self._args)
+        if rc != 0:
+            raise ApusHipError(rc, last_error())
 
 
 def _kv8_rows_call(f, kv, rows, cu, pos0, k, v):
