@@ -511,7 +511,8 @@ constexpr int32_t kPad = 8, kShort = 24, kShortMany = 96;
 // run's share of the mean, even and odd ones of the first 256 and of the others:
 // 1.18, 0.97, 0.98 and 0.87 (64 at 32768 328 us equal, 322 so; 128 ragged ones
 // verifying 1-4 tokens 239 and 230; 128 at 8000 171 and 167). Shorter runs differ by
-// few blocks and stay equal.
+// few blocks and stay equal. The shares are those of a card with nothing else on it:
+// where other work shifts them the runs end less evenly, with the same results.
 constexpr int32_t kLong = 32;
 constexpr double kShare[3] = {1.18, 0.97, 0.98};
 size_t max_runs() { return 2 * (size_t)cu_count(); }

@@ -13,9 +13,9 @@
 // 0..3, q = 0..3, 8 a step. Roundings (q to fp16, probabilities to bf16, their
 // sum) as in attn_kv8.hip.
 //
-// Bound by the matrix cores under load: a prompt of 8192 tokens, 550 GFLOP in 490
-// us, 1.12 PFLOP/s of the 1.24 to 1.36 that a large bf16 product reaches here, at
-// 1.85 to 2.0 GHz (power). A step of 32 keys is 2048 cycles of MFMA and some 3200 in
+// Bound by the matrix cores under load: a prompt of 8192 tokens, 550 GFLOP in 483 to
+// 505 us from card to card, 1.09 to 1.14 PFLOP/s of the 1.24 to 1.36 that a large bf16
+// product reaches here, at 1.85 to 2.0 GHz (power). A step of 32 keys is 2048 cycles of MFMA and some 3200 in
 // all: the softmax's exponents and packing stand between the two products of a
 // wavefront, and the other wavefront of its SIMD fills only part of that. Slower:
 // products of one step interleaved with the softmax of the next, q partly in LDS

@@ -8,10 +8,14 @@
 // loads and its stores), to a workgroup of four past them (2048, 8192 rows: 46.5
 // us with a workgroup a row, 48.8 with a wavefront; 1529, element by element: 11.9
 // and 16.3), to one of eight past 8192 (16384, 2000 rows: 67 us, with four 74, with
-// sixteen 83; 16001, element by element: 111, 153, 142). Aligned rows go 8
-// elements a load, others one. Bound by memory: 8192 rows of 2048, fp32 residuals
-// and a gate, 235 MB in 44.5 us, 5.3 TB/s, what a copy of 1 GiB reaches; a single
-// row (2 us) by its launch.
+// sixteen 83; 16001, element by element: 111, 153, 142). Aligned rows go 8 elements a
+// load, others one, at about twice what memory would take: 2000 rows of 16001 97 us, of
+// 16384 56 (bf16, no gate; 49 and 50 at a copy's rate), of 5001 36, of 5008 22. An
+// element is a load and a register of its own: with two eights a thread or more that is
+// 128 to 256 registers, which leave two to four wavefronts a SIMD to hide the loads (the
+// bf16 kernel of eight wavefronts a row spills 4). Bound by memory: 8192 rows of 2048,
+// fp32 residuals and a gate, 235 MB in 44.5 us, 5.3 TB/s, what a copy of 1 GiB reaches; a
+// single row (2 us) by its launch.
 #include <math.h>
 #include <stdint.h>
 

@@ -674,9 +674,10 @@ int apus_hip_moe_layer_decode(const ApusHipMoeLayer *L, ApusHipMoeWork *w, size_
  * graphs, allocate nothing and do not wait, and what a captured call was given
  * stays as it was. Bad arguments are refused with or without a device (the layer
  * call: with one). Two sequences of a call that writes may not share a row, nor
- * may the blocks that it writes be another row's (blocks that are only read may:
- * a shared prompt); calls that write a row and calls that use it run in the
- * caller's order (one stream, or events). They are not traced
+ * may the blocks that it writes be another row's or stand twice in one (blocks that
+ * are only read may: a shared prompt); calls that write a row and calls that use it
+ * run in the caller's order (one stream, or events). The new tokens of a call touch
+ * fewer than 2^22 (block, kv head) pairs in each 208 sequences. They are not traced
  * (apus_hip_trace_set). */
 typedef struct {
     uint8_t *k, *v;
