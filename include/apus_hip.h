@@ -730,7 +730,8 @@ int apus_hip_attn_kv8_work_destroy(ApusHipAttnKv8Work *w);
  * = sum_d max(|q_d|, 2^-20 max |q|) |K_jd| / 16. That holds for scores within fp32's
  * range and any finite V (beside values past 2^93 a P_j below 2^-90 of the row's
  * largest may count as 0, and so may what V below 2^-80 brings). A NaN in a position
- * that a token does not attend to does not reach its row. Supports d=256, rot=64, nh=8*nkv. y may not overlap the inputs. */
+ * that a token does not attend to does not reach its row. Supports d=256, rot=64,
+ * nh=8*nkv. y may not overlap the inputs. */
 int apus_hip_attn_decode_kv8(const ApusHipAttnLayer *L, ApusHipAttnKv8Work *w, size_t B,
                              const int32_t *rows, const int32_t *cu, const int32_t *pos0,
                              const uint16_t *qg, const uint16_t *k, const uint16_t *v,
